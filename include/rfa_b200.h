@@ -51,8 +51,9 @@ enum {
   RFA_EDEVICE = -5       /* not an sm_100 device / driver entry point missing  */
 };
 
-/* element types accepted where a signature has a *_dtype argument */
-enum { RFA_F16 = 0, RFA_F32 = 1 };
+/* element types accepted where a signature has a *_dtype argument (RFA_BF16 by the
+ * state-space entry points at the end only) */
+enum { RFA_F16 = 0, RFA_F32 = 1, RFA_BF16 = 2 };
 
 typedef void* rfa_stream_t;
 
@@ -411,6 +412,99 @@ int rfa_causal_fwd_fused_layer(const void* x_q, const void* x_k, const void* v,
  * pattern; bench.py reports it beside the copy bandwidth. */
 int rfa_stream_probe(const void* in, void* out, int64_t T, int BH, int nb, int with_store,
                      rfa_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * State-space operators: the short causal convolution, the selective scan and
+ * the gated group norm of a layer whose running state, like S and z above, has
+ * one size whatever the sequence's length.  No upstream counterpart.
+ *
+ * Activations are time-major, [T, B, D] with D channels adjacent; an input may
+ * have any other strides (in elements, *_t from token to token, *_b from batch
+ * row to batch row), outputs and gradients are contiguous.  dtype (RFA_F16,
+ * RFA_F32 or RFA_BF16) is the type of all activations; sums, states and their
+ * gradients are fp32.  mask [B, T] bytes or NULL, non-zero = a padded token:
+ * every result of the others is what it would be if padded tokens were not
+ * there, whatever stands in them, and a padded token's outputs and gradients
+ * are zero.  No alignment is asked for beyond the elements' own, except that
+ * states, checkpoints and workspaces are 16-byte aligned.  T < 2^31 - 64,
+ * B <= 65535; a size of zero is refused (there is nothing to launch).
+ * ---------------------------------------------------------------------- */
+
+/* Causal depthwise convolution over the last W tokens (1 <= W <= 8):
+ *   pre_t = bias + sum_j weight[.][j] x_(t - W + 1 + j),  y_t = silu(pre_t) or pre_t.
+ * weight [D, W] and bias [D] (or NULL) of dtype.  state_in [B, W-1, D] of dtype, or
+ * NULL for zeros: the inputs in front of the first token, oldest first; state_out, or
+ * NULL: the last W - 1 inputs including those of state_in.  state_out may be state_in
+ * where T is 1 (and not otherwise). */
+typedef struct {
+  const void* x;
+  int64_t x_t, x_b;
+  const void *weight, *bias, *state_in;
+  const uint8_t* mask;
+  int64_t T;
+  int B, D, W, dtype, silu;
+} rfa_causal_conv_t;
+int rfa_causal_conv_fwd(const rfa_causal_conv_t* conv, void* y, void* state_out,
+                        rfa_stream_t stream);
+/* Gradients: g [T, B, D] with strides g_t, g_b, g_state [B, W-1, D] of the outgoing
+ * state or NULL -> gx [T, B, D]; g_weight [D, W] and g_bias [D], g_state_in [B, W-1, D],
+ * each or NULL. */
+size_t rfa_causal_conv_workspace_bytes(int64_t T, int B, int D, int W);
+int rfa_causal_conv_bwd(const rfa_causal_conv_t* conv, const void* g, int64_t g_t, int64_t g_b,
+                        const void* g_state, void* gx, void* g_weight, void* g_bias, void* g_state_in,
+                        void* workspace, size_t workspace_bytes, rfa_stream_t stream);
+
+/* Selective scan, per batch row and channel i of group i / (D / G):
+ *   delta_t = softplus(dt_t + dt_bias)     (dt_t + dt_bias where softplus is 0)
+ *   s_t = exp(delta_t a) s_(t-1) + delta_t b_t x_t        (N states, 1 <= N <= 64)
+ *   y_t = c_t . s_t + d x_t
+ * x, dt [T, B, D]; b, c [T, B, G, N], the N adjacent, *_g from group to group; a [D, N]
+ * (finite, delta a <= 88), d [D] or NULL, dt_bias [D] or NULL, states [B, D, N], all fp32. */
+typedef struct {
+  const void *x, *dt, *b, *c;
+  int64_t x_t, x_b, dt_t, dt_b, b_t, b_b, b_g, c_t, c_b, c_g;
+  const float *a, *d, *dt_bias, *s_in;      /* s_in NULL: zeros */
+  const uint8_t* mask;
+  int64_t T;
+  int B, D, N, G, dtype, softplus;
+} rfa_scan_t;
+/* Scratch of a forward (backward = 0) or backward (1) call with `scan`'s sizes, and what
+ * a forward leaves for the backward (the state in front of every 16th token). */
+size_t rfa_selective_scan_workspace_bytes(int64_t T, int B, int D, int N, int G, int backward);
+size_t rfa_selective_scan_checkpoint_bytes(int64_t T, int B, int D, int N);
+/* y [T, B, D]; s_out [B, D, N] or NULL (not s_in); checkpoints or NULL. */
+int rfa_selective_scan_fwd(const rfa_scan_t* scan, void* y, float* s_out, float* checkpoints,
+                           void* workspace, size_t workspace_bytes, rfa_stream_t stream);
+/* g [T, B, D] contiguous, g_s [B, D, N] of the last state or NULL, the forward's
+ * checkpoints -> gx, gdt [T, B, D], gb, gc [T, B, G, N] of dtype; ga [D, N]; gd, g_dt_bias
+ * [D], gs_in [B, D, N], each or NULL. */
+int rfa_selective_scan_bwd(const rfa_scan_t* scan, const void* g, const float* g_s,
+                           const float* checkpoints, void* gx, void* gdt, float* ga, void* gb,
+                           void* gc, float* gd, float* g_dt_bias, float* gs_in,
+                           void* workspace, size_t workspace_bytes, rfa_stream_t stream);
+/* One token (T = 1): the state s [B, D, N] is updated in place (s_in is not read). */
+int rfa_selective_scan_step(const rfa_scan_t* scan, void* y, float* s, rfa_stream_t stream);
+
+/* Group norm of rows: each of `groups` runs of C / groups (<= 16384) adjacent channels of
+ * x's row is brought to mean 0 and variance 1 (eps added to the variance), times weight
+ * plus bias ([C] of dtype, each or NULL): n.  y = n silu(gate) with a gate, else silu(n);
+ * n gate and n where silu is 0.  x, gate rows x_r, gate_r elements apart; y [rows, C]. */
+typedef struct {
+  const void* x;
+  const void* gate;
+  int64_t x_r, gate_r;
+  const void *weight, *bias;
+  int64_t rows;
+  int C, groups, dtype, silu;
+  float eps;
+} rfa_group_norm_t;
+int rfa_group_norm_fwd(const rfa_group_norm_t* norm, void* y, rfa_stream_t stream);
+/* g rows g_r elements apart -> gx [rows, C]; g_gate [rows, C], g_weight, g_bias [C], each
+ * or NULL. */
+size_t rfa_group_norm_workspace_bytes(int64_t rows, int C, int groups);
+int rfa_group_norm_bwd(const rfa_group_norm_t* norm, const void* g, int64_t g_r, void* gx,
+                       void* g_gate, void* g_weight, void* g_bias,
+                       void* workspace, size_t workspace_bytes, rfa_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -13,9 +13,10 @@ import sys
 from .utils import CrossAttentionState
 from .causal_attention import CausalAttention
 from .cross_attention import CrossAttention, CrossAttentionProject
+from .state_space import SelectiveStateSpace
 
 __all__ = ["CausalAttention", "CrossAttention", "CrossAttentionState", "CrossAttentionProject",
-           "install_aliases"]
+           "SelectiveStateSpace",            "install_aliases"]
 
 
 def install_aliases() -> None:

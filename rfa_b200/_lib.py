@@ -62,6 +62,17 @@ SIGNATURES = {
     "rfa_column_sums": (_int, [_vp, _vp, _int, _i64, _int, _vp]),
     "rfa_layer_matrices": (_int, [_vp, _vp, _f32, _vp, _int, _int, _int, _vp, _vp, _i64, _int, _vp]),
     "rfa_layer_matrices_bwd": (_int, [_vp, _vp, _vp, _f32, _vp, _vp, _int, _int, _int, _vp]),
+    "rfa_causal_conv_fwd": (_int, [_vp] * 4),
+    "rfa_causal_conv_workspace_bytes": (_sz, [_i64, _int, _int, _int]),
+    "rfa_causal_conv_bwd": (_int, [_vp, _vp, _i64, _i64] + [_vp] * 6 + [_sz, _vp]),
+    "rfa_selective_scan_workspace_bytes": (_sz, [_i64] + [_int] * 5),
+    "rfa_selective_scan_checkpoint_bytes": (_sz, [_i64] + [_int] * 3),
+    "rfa_selective_scan_fwd": (_int, [_vp] * 5 + [_sz, _vp]),
+    "rfa_selective_scan_bwd": (_int, [_vp] * 13 + [_sz, _vp]),
+    "rfa_selective_scan_step": (_int, [_vp] * 4),
+    "rfa_group_norm_fwd": (_int, [_vp] * 3),
+    "rfa_group_norm_workspace_bytes": (_sz, [_i64, _int, _int]),
+    "rfa_group_norm_bwd": (_int, [_vp, _vp, _i64] + [_vp] * 5 + [_sz, _vp]),
     "rfa_decode_step_fused": (_int, [_vp, _vp, _vp, _int, _vp, _f32, _vp, _vp, _int, _vp, _int, _int, _int, _int, _vp]),
 }
 

@@ -1,5 +1,5 @@
 """Build the C-ABI shared library ``rfa_b200/csrc/librfa_b200.so`` with nvcc for sm_100a, and ``rfa_b200/_native.so``, the
-tensor-level calls over it (``csrc/torch_ops.cpp``, against this interpreter's torch).
+tensor-level calls over it (``csrc/torch_ops.cpp`` and ``torch_state_space.cpp``, against this interpreter's torch).
 
     python -m rfa_b200.build [--force] [--verbose]
 
@@ -18,7 +18,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "librfa_b200.so")
-NATIVE_SRC, NATIVE = os.path.join(CSRC, "torch_ops.cpp"), os.path.join(HERE, "_native.so")
+NATIVE_SRCS = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_state_space.cpp")]
+NATIVE = os.path.join(HERE, "_native.so")
 NATIVE_KEY = os.path.join(HERE, "_native.key")      # what the module was built for (see native_key)
 
 NVCC_FLAGS = [
@@ -76,7 +77,7 @@ def native_key() -> str:
 
 
 def native_stale() -> bool:
-    if stale(NATIVE, [NATIVE_SRC, os.path.join(os.path.dirname(HERE), "include", "rfa_b200.h")]) or not os.path.exists(NATIVE_KEY):
+    if stale(NATIVE, [*NATIVE_SRCS, os.path.join(CSRC, "torch_call.h"), os.path.join(os.path.dirname(HERE), "include", "rfa_b200.h")]) or not os.path.exists(NATIVE_KEY):
         return True
     with open(NATIVE_KEY) as f:
         return f.read() != native_key()
@@ -92,12 +93,21 @@ def build_native() -> str:
         root = os.path.dirname(torch.__file__)
         cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
         incs = [*include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
-        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-               *[f"-I{i}" for i in incs], NATIVE_SRC, "-o", NATIVE, "-L" + CSRC, "-l:librfa_b200.so", "-L" + os.path.join(root, "lib"),
-               "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN/csrc"]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("building _native.so failed:\n" + r.stdout + r.stderr)
+        def run(cmd):
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            if r.returncode != 0:
+                raise RuntimeError("building _native.so failed:\n" + r.stdout + r.stderr)
+
+        def one(src):
+            obj = src[:-4] + ".native.o"
+            run(["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_native",
+                 *[f"-I{i}" for i in incs], "-c", src, "-o", obj])
+            return obj
+
+        with cf.ThreadPoolExecutor(max_workers=len(NATIVE_SRCS)) as ex:
+            objs = list(ex.map(one, NATIVE_SRCS))
+        run(["g++", "-shared", *objs, "-o", NATIVE, "-L" + CSRC, "-l:librfa_b200.so", "-L" + os.path.join(root, "lib"),
+             "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN/csrc"])
         with open(NATIVE_KEY, "w") as f:
             f.write(native_key())
     return NATIVE

@@ -1,0 +1,119 @@
+// Shared by the state-space operators (causal_conv.cu, selective_scan.cu, selective_scan_bwd.cu, group_norm.cu): element types, runs of
+// eight adjacent channels, and the sums of partial results.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace rfa {
+
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// NV adjacent elements as they stand in memory: asked for early, converted when they are needed.
+template <typename T, int NV>
+struct Raw {
+  static constexpr int kWords = NV * (int)sizeof(T) / 4;
+  static_assert(kWords > 0, "whole words");
+  uint32_t w[kWords];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  // `wide`: the address is a multiple of the run's size (at most 16 bytes); n elements are there
+  __device__ __forceinline__ void load(const T* p, int n, bool wide) {
+    if (wide && n >= NV) {
+      if constexpr (kWords % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < kWords; i += 4) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+          w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+        }
+      } else if constexpr (kWords == 2) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        w[0] = v.x; w[1] = v.y;
+      } else {
+        w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) set(i, i < n ? p[i] : from_f<T>(0.f));
+    }
+  }
+  __device__ __forceinline__ void set(int i, T v) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(to_f(v));
+    } else {
+      const uint32_t h = *reinterpret_cast<const uint16_t*>(&v);
+      w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | h << 16 : (w[i / 2] & 0xffff0000u) | h;
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else {
+      const uint16_t h = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffff;
+      return to_f(*reinterpret_cast<const T*>(&h));
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int n, bool wide) const {
+    if (wide && n >= NV) {
+      if constexpr (kWords % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < kWords; i += 4) reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+      } else if constexpr (kWords == 2) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+      } else {
+        *reinterpret_cast<uint32_t*>(p) = w[0];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i < n) p[i] = from_f<T>(get(i));
+    }
+  }
+};
+
+// Whether runs of NV elements at p, p + stride ... may be taken as wide words.
+inline bool wide_ok(const void* p, int64_t stride, int64_t stride2, int size, int nv) {
+  const int64_t bytes = nv * size < 16 ? nv * size : 16;
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0 && stride2 * size % bytes == 0;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+
+// 1 / (1 + exp(-x)), at most 5e-7 off in itself; exp's overflow gives 0
+__device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
+
+// log(1 + exp(v)) = max(v, 0) + log1p(z), z = exp(-|v|) in (0, 1]; log1p(z) = 2 atanh(w), w = z / (2 + z) in (0, 1/3]: an odd polynomial in w,
+// interpolated at Chebyshev nodes of w^2 in [0, 1/9] (4.1e-9 relative).  No difference of near numbers, so that steps of 1e-3 and less keep
+// fp32's precision; 16 instructions, where log1pf(expf(v)) takes about 45.  `sig`: its derivative.
+__device__ __forceinline__ float softplus(float v, float& sig) {
+  const float z = ex2(-kLog2e * fabsf(v)), w = z * rcp(2.f + z), s = w * w, r = rcp(1.f + z);
+  sig = v >= 0.f ? r : z * r;
+  const float q = fmaf(fmaf(fmaf(fmaf(0.281577788f, s, 0.279651582f), s, 0.400245965f), s, 0.666663229f), s, 2.f);
+  return fmaxf(v, 0.f) + w * q;
+}
+
+// ---- sums of partial results: dst[i] = sum over p of src[p * n + i], in a fixed order ----------------------------------------
+struct SumJob {
+  const float* src;
+  void* dst;
+  int64_t n;
+  int parts, dtype;
+};
+constexpr int kSumJobs = 5;
+int sum_parts(const SumJob* jobs, int count, cudaStream_t stream);      // state_space.cu
+
+}  // namespace rfa

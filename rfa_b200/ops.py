@@ -361,3 +361,43 @@ def cross_decode_step(phi_q: Tensor, states: CrossDecodeStates, out: Optional[Te
         check(_lib.load().rfa_cross_decode_step(ptr(phi_q), dtype_code(phi_q), ptr(states.s_ptrs), ptr(states.z_ptrs), ptr(out),
                                                 L, B * H, K, states.d, stream_of(phi_q)), "rfa_cross_decode_step")
     return out
+
+
+# --------------------------------------------------------------------------- state space
+def causal_conv_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, state: Optional[Tensor] = None, mask: Optional[Tensor] = None,
+                    silu: bool = True, return_state: bool = False, in_place: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
+    """x [T,B,C], weight [C,W], bias [C], state [B,W-1,C] (the inputs in front), mask [B,T] -> (y [T,B,C], the last W-1 inputs
+    if asked: in place of ``state`` with ``in_place``)."""
+    return native().causal_conv_fwd(x, weight, bias, state, mask, silu, return_state, in_place)
+
+
+def causal_conv_bwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: Optional[Tensor], mask: Optional[Tensor], silu: bool, g: Tensor,
+                    g_state: Optional[Tensor], need_weight: bool, need_bias: bool, need_state: bool):
+    """(g_x, g_weight, g_bias, g_state_in), None for those not needed; g [T,B,C], g_state [B,W-1,C] of the outgoing state."""
+    return native().causal_conv_bwd(x, weight, bias, state, mask, silu, g, g_state, need_weight, need_bias, need_state)
+
+
+def selective_scan_fwd(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, d: Optional[Tensor] = None, dt_bias: Optional[Tensor] = None,
+                       s: Optional[Tensor] = None, mask: Optional[Tensor] = None, softplus: bool = True, return_state: bool = False,
+                       in_place: bool = False, save: bool = False):
+    """x, dt [T,B,C], a [C,N], b, c [T,B,G,N], d, dt_bias [C], s [B,C,N], mask [B,T] -> (y [T,B,C], the last state if asked: in
+    place of ``s`` with ``in_place``, with ``save`` the checkpoints that ``selective_scan_bwd`` wants)."""
+    return native().selective_scan_fwd(x, dt, a, b, c, d, dt_bias, s, mask, softplus, return_state, in_place, save)
+
+
+def selective_scan_bwd(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, d: Optional[Tensor], dt_bias: Optional[Tensor], s: Optional[Tensor],
+                       mask: Optional[Tensor], softplus: bool, g: Tensor, g_s: Optional[Tensor], kept: Optional[Tensor], need_state: bool):
+    """(g_x, g_dt, g_a, g_b, g_c, g_d, g_dt_bias, g_s_in); g [T,B,C], g_s [B,C,N] of the last state."""
+    return native().selective_scan_bwd(x, dt, a, b, c, d, dt_bias, s, mask, softplus, g, g_s, kept, need_state)
+
+
+def group_norm_fwd(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, gate: Optional[Tensor] = None,
+                   silu: bool = True, eps: float = 1e-5) -> Tensor:
+    """x, gate [..., C], weight, bias [C] -> n * silu(gate), or silu(n) without a gate, n = the normalised groups * weight + bias."""
+    return native().group_norm_fwd(x, groups, weight, bias, gate, silu, eps)
+
+
+def group_norm_bwd(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], gate: Optional[Tensor], silu: bool, eps: float, g: Tensor,
+                   need_weight: bool, need_bias: bool, need_gate: bool):
+    """(g_x, g_weight, g_bias, g_gate), None for those not needed."""
+    return native().group_norm_bwd(x, groups, weight, bias, gate, silu, eps, g, need_weight, need_bias, need_gate)

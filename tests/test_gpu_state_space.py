@@ -1,0 +1,578 @@
+"""The state-space operators on the GPU against their oracle in 64 bits.
+
+Tolerances.  A result in a 16-bit type is off by its own rounding, half a step of that type relative to the value, and by what
+fp32 sums lose: a bound that scales with ``size``, the same sum over the magnitudes of its terms (the oracle's ``absolute``).
+  convolution  W + 1 terms, the sigmoid 5e-7 relative (ex2 2^-22, two roundings, a reciprocal): 2^-19 size; its weight gradients, chains
+               of 32 tokens, four warps and the parts: 2^-17 size
+  scan         a state is a product of at most T decays, each off by 2^-22 (ex2) + 2^-24 (the product) and by its argument's roundings (three, and
+               softplus 2^-22: times |delta a| exp(delta a) <= 0.37 each), times a term of three roundings, summed T times:
+               (8 T + 16) 2^-24 size; outputs sum N states; gradients are products of two such, summed over T tokens, B rows and
+               the channels: (20 T + 64 + B + D + 2 N) 2^-24 size
+  norm         mean and variance of C / groups terms in chains of at most 32 and a tree, rsqrt 2 ulp, the sigmoid: 2^-18 size with the
+               condition of the subtraction of the mean; weight gradients are sums of `rows` terms: (2^-18 + rows 2^-24) size
+The smallest normal number is added where a type has subnormal results."""
+import itertools
+
+import pytest
+import torch
+
+from oracle import state_space_oracle as O
+from rfa_b200 import SelectiveStateSpace, ops
+from rfa_b200 import state_space as ss
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def near(got, want, size, unit, what):
+    """|got - want| <= half a step of got's type + unit * size, element by element; the same places finite."""
+    info = torch.finfo(got.dtype)
+    got, want, size = got.detach().double().cpu(), want.double().cpu(), size.double().cpu()
+    assert got.shape == want.shape, what
+    rounding = info.eps / 2 if info.bits < 32 else 0.0
+    bad = (got - want).abs() > rounding * want.abs() + unit * size + info.tiny
+    bad |= ~got.isfinite()
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(((got - want).abs() / (size + 1e-30)).max()):.2e} of size"
+
+
+def padding(B, T, kind, gen):
+    if kind is None:
+        return None
+    m = torch.zeros(B, T, dtype=torch.bool)
+    for b in range(B):
+        n = int(torch.randint(0, T + 1, (1,), generator=gen))
+        if kind == "right":
+            m[b, n:] = True
+        elif kind == "left":
+            m[b, :T - n] = True
+        else:
+            m[b] = torch.rand(T, generator=gen) < 0.5
+    m[0] = kind == "right"                                        # a row that is all padding, or none of it
+    return m
+
+
+def poison(t, mask):
+    """Values that must not be read in padded places."""
+    if mask is not None:
+        t[mask.t()] = torch.tensor([float("nan"), float("inf"), -float("inf"), torch.finfo(t.dtype).min])[
+            torch.randint(0, 4, t[mask.t()].shape, generator=torch.Generator().manual_seed(7))].to(t.dtype)
+    return t
+
+
+def clean(t, mask):
+    return t if mask is None else torch.where(mask.t().view(*mask.t().shape, *[1] * (t.dim() - 2)), 0.0, t)
+
+
+def strided(t, kind, dev):
+    """The same values on the device: contiguous, batch first, a slice of wider rows, at an odd address."""
+    if kind == "batch first":
+        return t.transpose(0, 1).contiguous().to(dev).transpose(0, 1)
+    if kind == "slice":
+        wide = torch.full((*t.shape[:-1], 2 * t.shape[-1] + 8), float("nan"), dtype=t.dtype, device=dev)
+        wide[..., 8:8 + t.shape[-1]] = t.to(dev)
+        return wide[..., 8:8 + t.shape[-1]]
+    if kind == "odd":
+        flat = torch.full((t.numel() + 1,), float("nan"), dtype=t.dtype, device=dev)
+        flat[1:] = t.flatten().to(dev)
+        return flat[1:].view(t.shape)
+    return t.to(dev)
+
+
+def leaves(*ts):
+    return [None if t is None else t.detach().requires_grad_() for t in ts]
+
+
+# --------------------------------------------------------------------------- convolution
+CONV = list(itertools.product([(1, 1, 1), (1, 3, 8), (2, 2, 5), (3, 3, 40), (17, 2, 264), (33, 3, 64), (129, 3, 136), (300, 2, 1000)], [4, 2, 3]))
+CONV += [((67, 3, 24), w) for w in (1, 5, 6, 7, 8)]
+
+
+@pytest.mark.parametrize("shape,width", CONV)
+@pytest.mark.parametrize("dtype,pad,state,layout,silu", [(F16, None, False, None, True), (BF16, "right", True, "slice", True),
+                                                         (F32, "left", True, "odd", True), (F16, "mixed", True, "batch first", False)])
+def test_convolution(dev, shape, width, dtype, pad, state, layout, silu):
+    T, B, D = shape
+    gen = torch.Generator().manual_seed(T * 100 + D + width)
+    draw = lambda *s: torch.randn(*s, generator=gen).to(dtype)
+    mask = padding(B, T, pad, gen)
+    x, g, w, bias = poison(draw(T, B, D), mask), poison(draw(T, B, D), mask), draw(D, width), draw(D) if state else None
+    s, gs = (draw(B, width - 1, D), draw(B, width - 1, D)) if state else (None, None)
+    args = [None if t is None else t.double() for t in (clean(x, mask), w, bias, s)]
+    more = [None if t is None else t.double() for t in (clean(g, mask), gs)]
+    want, size = (O.conv(*args, mask, silu, *more, absolute=a) for a in (False, True))
+
+    xd, wd, bd, sd = leaves(strided(x, layout, dev), *(None if t is None else t.to(dev) for t in (w, bias, s)))
+    md = None if mask is None else mask.to(dev)
+    act = "silu" if silu else None
+    if state:
+        y, out = ss.incremental_causal_conv(x=xd, weight=wd, bias=bd, state=sd, activation=act, key_padding_mask=md)
+        assert torch.equal(out.cpu().double(), want["state"]) and out.dtype == dtype
+        ins = [t for t in (xd, wd, bd, sd) if t.numel()]
+        grads = torch.autograd.grad([y, out], ins, [strided(g, layout, dev), gs.to(dev)], allow_unused=True)
+        names = [n for n, t in zip(("gx", "gweight", "gbias", "gstate"), (xd, wd, bd, sd)) if t.numel()]
+        with torch.no_grad():                                     # the state updated in place gives the same bits
+            kept = s.to(dev)
+            y2, out2 = ss.incremental_causal_conv(x=xd, weight=wd, bias=bd, state=kept, activation=act, key_padding_mask=md)
+            assert out2 is kept and torch.equal(out2, out) and torch.equal(y2, y)
+    else:
+        y = ss.causal_conv(x=xd, weight=wd, bias=bd, activation=act, key_padding_mask=md)
+        grads, names = torch.autograd.grad(y, [xd, wd], strided(g, layout, dev)), ("gx", "gweight")
+    near(y, want["y"], size["y"], 2.0 ** -19, "y")
+    for n, t in zip(names, grads):
+        assert t.dtype == dtype
+        near(t, want[n], size[n], 2.0 ** (-17 if n in ("gweight", "gbias") else -19), n)
+
+
+def test_convolution_of_one_long_row_of_padding(dev):
+    """The window in front of a run lies thousands of padded tokens back."""
+    T, D = 9000, 8
+    x, w = torch.randn(T, 1, D, device=dev), torch.randn(D, 4, device=dev)
+    mask = torch.ones(1, T, dtype=torch.bool, device=dev)
+    there = [0, 1, 2, 5, 8000, 8990, 8999]
+    mask[0, there] = False
+    y, state = ss.incremental_causal_conv(x=x, weight=w, key_padding_mask=mask)
+    assert torch.equal(y[there], ss.causal_conv(x=x[there], weight=w))
+    assert torch.equal(state[0], x[there[-3:], 0]) and int(y.ne(0).any(-1).sum()) == len(there)
+
+
+# --------------------------------------------------------------------------- selective scan
+SCAN = [(1, 1, 1, 1, 1), (1, 3, 8, 16, 1), (2, 2, 6, 3, 2), (15, 2, 64, 16, 1), (16, 3, 40, 4, 1), (17, 1, 72, 8, 1), (33, 2, 130, 12, 1), (48, 1, 136, 17, 2),
+        (65, 2, 36, 32, 4), (80, 2, 24, 33, 1), (70, 1, 16, 64, 1), (150, 3, 264, 16, 1), (531, 1, 48, 16, 2), (700, 1, 20, 64, 1)]
+
+
+def scan_inputs(shape, dtype, gen, layout=None, dev="cpu"):
+    T, B, D, N, G = shape
+    draw = lambda *s: torch.randn(*s, generator=gen)
+    step = torch.exp(torch.rand(D, generator=gen) * 4.6 - 6.9)
+    ins = dict(x=draw(T, B, D).to(dtype), dt=(0.5 * draw(T, B, D)).to(dtype),
+               a=-(torch.arange(1, N + 1).float() * torch.exp(0.1 * draw(D, N))), b=draw(T, B, G, N).to(dtype), c=draw(T, B, G, N).to(dtype), d=draw(D),
+               dt_bias=step + torch.log(-torch.expm1(-step)), s=draw(B, D, N))
+    return ins, draw(T, B, D).to(dtype), draw(B, D, N)
+
+
+def scan_check(dev, shape, dtype, pad, layout, softplus=True, optional=True, state=True):
+    T, B, D, N, G = shape
+    gen = torch.Generator().manual_seed(T * 1000 + D + N)
+    ins, g, gs = scan_inputs(shape, dtype, gen)
+    if not softplus:
+        ins["dt"] = ins["dt"].abs() / 8
+        ins["dt_bias"] = ins["dt_bias"].abs() / 64
+    if not optional:
+        ins["d"] = ins["dt_bias"] = None
+    if not state:
+        ins["s"] = gs = None
+    mask = padding(B, T, pad, gen)
+    for n in ("x", "dt", "b", "c"):
+        poison(ins[n], mask)
+    poison(g, mask)
+    seq = ("x", "dt", "b", "c")
+    args = [None if t is None else (clean(t, mask) if n in seq else t).double() for n, t in ins.items()]
+    more = [clean(g, mask).double(), None if gs is None else gs.double()]
+    want, size = (O.scan(*args, mask, softplus, *more, absolute=a) for a in (False, True))
+
+    on = {n: None if t is None else strided(t, layout, dev) if n in seq else t.to(dev) for n, t in ins.items()}
+    on = dict(zip(on, leaves(*on.values())))
+    md = None if mask is None else mask.to(dev)
+    names = dict(x="gx", dt="gdt", a="ga", b="gb", c="gc", d="gd", dt_bias="gbias", s="gs")
+    diff = [n for n in names if on[n] is not None]
+    if state:
+        y, out = ss.incremental_selective_scan(**on, dt_softplus=softplus, key_padding_mask=md)
+        grads = torch.autograd.grad([y, out], [on[n] for n in diff], [strided(g, layout, dev), gs.to(dev)])
+        with torch.no_grad():
+            kept = ins["s"].to(dev)
+            y2, out2 = ss.incremental_selective_scan(**{**on, "s": kept}, dt_softplus=softplus, key_padding_mask=md)
+            assert out2 is kept
+        for got in (out, out2):
+            near(got, want["s"], size["s"], (8 * T + 16) * 2.0 ** -24, "s")
+        near(y2, want["y"], size["y"], (8 * T + 16 + 2 * N) * 2.0 ** -24, "y in place")
+    else:
+        rest = {n: t for n, t in on.items() if n != "s"}
+        y = ss.selective_scan(**rest, dt_softplus=softplus, key_padding_mask=md)
+        grads = torch.autograd.grad(y, [on[n] for n in diff], strided(g, layout, dev))
+    near(y, want["y"], size["y"], (8 * T + 16 + 2 * N) * 2.0 ** -24, "y")
+    for n, t in zip(diff, grads):
+        assert t.dtype == on[n].dtype
+        near(t, want[names[n]], size[names[n]], (20 * T + 64 + B + D + 2 * N) * 2.0 ** -24, names[n])
+
+
+@pytest.mark.parametrize("shape", SCAN)
+@pytest.mark.parametrize("dtype,pad,layout", [(F16, None, None), (BF16, "right", "slice"), (F32, "left", "odd"), (F32, "mixed", "batch first")])
+def test_scan(dev, shape, dtype, pad, layout):
+    scan_check(dev, shape, dtype, pad, layout)
+
+
+@pytest.mark.parametrize("softplus,optional,state", [(False, True, True), (True, False, True), (True, True, False), (False, False, False)])
+@pytest.mark.parametrize("shape", [(1, 2, 24, 16, 1), (40, 2, 24, 16, 1)])
+def test_scan_without_its_optional_parts(dev, shape, softplus, optional, state):
+    scan_check(dev, shape, F32, None, None, softplus, optional, state)
+    scan_check(dev, shape, BF16, "mixed", "slice", softplus, optional, state)
+
+
+@pytest.mark.parametrize("cut", [1, 16, 100, 299])
+def test_scan_in_two_calls(dev, cut):
+    """A prompt in two calls is the prompt in one, whichever way either is cut into segments."""
+    gen = torch.Generator().manual_seed(cut)
+    ins, _, _ = scan_inputs((300, 2, 72, 16, 1), F32, gen)
+    on = {n: t.to(dev) for n, t in ins.items() if n != "s"}
+    y, s = ss.incremental_selective_scan(**on)
+    part = lambda lo, hi: {n: t[lo:hi] if n in ("x", "dt", "b", "c") else t for n, t in on.items()}
+    y1, held = ss.incremental_selective_scan(**part(0, cut))
+    y2, same = ss.incremental_selective_scan(**part(cut, 300), s=held)
+    assert same is held
+    for a, b in ((torch.cat([y1, y2]), y), (held, s)):
+        assert (a - b).norm() <= 1e-6 * b.norm()
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_scan_keeps_non_finite_values_where_they_belong(dev, value):
+    """One token of one channel's x: its channel from that token on, its group's b and c gradients; nothing else."""
+    ins, _, _ = scan_inputs((40, 2, 72, 16, 1), F32, torch.Generator().manual_seed(0))
+    on = {n: t.to(dev) for n, t in ins.items() if n != "s"}
+    clean_y = ss.selective_scan(**on)
+    on["x"][20, 1, 5] = value
+    y = ss.selective_scan(**on)
+    hit = torch.zeros_like(y, dtype=torch.bool)
+    hit[20:, 1, 5] = True
+    assert not y[20:, 1, 5].isfinite().any() and torch.equal(y[~hit], clean_y[~hit])
+
+
+# --------------------------------------------------------------------------- group norm
+NORM = [((1,), 1, 1), ((3, 2), 4, 2), ((5,), 7, 1), ((2, 3), 24, 3), ((1, 9), 64, 1), ((33,), 200, 5), ((130, 3), 1024, 16), ((7,), 300, 100), ((40,), 1000, 1),
+        ((5, 2), 2048, 1), ((3,), 5000, 1), ((2,), 12000, 1), ((3,), 16384, 1), ((2,), 16383, 1), ((1500,), 40, 1), ((2,), 4096, 1), ((257,), 513, 3)]
+
+
+@pytest.mark.parametrize("lead,C,groups", NORM)
+@pytest.mark.parametrize("dtype,gated,weights,layout,silu", [(F16, True, True, None, True), (BF16, True, True, "slice", True), (F32, False, True, "odd", True),
+                                                             (F32, True, False, "slice", False), (F16, False, False, None, False)])
+def test_norm(dev, lead, C, groups, dtype, gated, weights, layout, silu):
+    gen = torch.Generator().manual_seed(C + groups)
+    draw = lambda *s: torch.randn(*s, generator=gen).to(dtype)
+    x, g, w, bias, gate = 2 * draw(*lead, C) + 1, draw(*lead, C), draw(C) if weights else None, draw(C) if weights else None, draw(*lead, C) if gated else None
+    x.view(-1, C)[0] = 3.0                                        # a row without variance
+    args = [None if t is None else t.double() for t in (w, bias, gate)]
+    want, size = (O.norm(x.double(), groups, *args, silu, 1e-5, g.double(), absolute=a) for a in (False, True))
+    put = lambda t: None if t is None else strided(t, layout, dev)
+    xd, wd, bd, zd = leaves(put(x), *(None if t is None else t.to(dev) for t in (w, bias)), put(gate))
+    y = ss.group_norm(x=xd, num_groups=groups, weight=wd, bias=bd, gate=zd, activation="silu" if silu else None)
+    near(y, want["y"], size["y"], 2.0 ** -18, "y")
+    pairs = [(n, t) for n, t in zip(("gx", "gweight", "gbias", "ggate"), (xd, wd, bd, zd)) if t is not None]
+    rows = x.numel() // C
+    for (n, t), got in zip(pairs, torch.autograd.grad(y, [t for _, t in pairs], put(g))):
+        assert got.dtype == dtype and got.shape == t.shape
+        near(got, want[n], size[n], 2.0 ** -18 + (rows * 2.0 ** -24 if n in ("gweight", "gbias") else 0), n)
+
+
+# --------------------------------------------------------------------------- what goes for all of them
+def calls(dev, dtype=F16, T=20, B=3, D=64, N=16):
+    """Each operator's call on fresh inputs: (function of the tensors, tensors)."""
+    gen = torch.Generator().manual_seed(1)
+    draw = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(dev)
+    ins, _, _ = scan_inputs((T, B, D, N, 1), dtype, gen)
+    names = [n for n in ins if n != "s"]
+    return {"conv": (lambda x, w, b: ss.causal_conv(x=x, weight=w, bias=b), [draw(T, B, D), draw(D, 4), draw(D)]),
+            "scan": (lambda *t: ss.selective_scan(**dict(zip(names, t))), [ins[n].to(dev) for n in names]),
+            "norm": (lambda x, w, b, z: ss.group_norm(x=x, num_groups=4, weight=w, bias=b, gate=z), [draw(T, B, D), draw(D), draw(D), draw(T, B, D)])}
+
+
+KINDS = ["conv", "scan", "norm"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_empty_calls(dev, kind):
+    call, ts = calls(dev)[kind]
+    for sizes in ((0, 3), (20, 0)):
+        cut = [t[:sizes[0], :sizes[1]].detach().requires_grad_() if t.dim() >= 3 else t.detach().requires_grad_() for t in ts]
+        y = call(*cut)
+        assert y.shape == (*sizes, 64)
+        for t, g in zip(cut, torch.autograd.grad(y, cut, torch.zeros_like(y))):
+            assert g.shape == t.shape and not g.any()
+    if kind == "norm":
+        return
+    s = torch.ones(3, 3, 64, device=dev).half() if kind == "conv" else torch.ones(3, 64, 16, device=dev)
+    empty = [t[:0] if t.dim() >= 3 else t for t in ts]
+    if kind == "conv":
+        y, out = ss.incremental_causal_conv(x=empty[0], weight=empty[1], state=s)
+    else:
+        y, out = ss.incremental_selective_scan(**dict(zip(("x", "dt", "a", "b", "c"), empty)), s=s)
+    assert out is s and bool((s == 1).all()) and y.shape == (0, 3, 64)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_backward_pass_is_the_same_twice_and_against_differences(dev, kind):
+    call, ts = calls(dev, F32, T=37)[kind]
+    ts = [t.requires_grad_() for t in ts]
+    g = torch.randn(ts[0].shape, generator=torch.Generator().manual_seed(3)).to(dev)
+    first, second = (torch.autograd.grad(call(*ts), ts, g) for _ in range(2))
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    # along a direction v: (f(t + h v) - f(t - h v)) / 2h, h = 2^-6: fp32 results off by 2^-24 sqrt(n) |terms| / h, third derivatives h^2
+    for i, t in enumerate(ts):
+        v = torch.randn(t.shape, generator=torch.Generator().manual_seed(i)).to(dev)
+        v /= v.norm()
+        h = 2.0 ** -6
+        with torch.no_grad():
+            up, down = (call(*[t + s * h * v if k == i else u for k, u in enumerate(ts)]).double() for s in (1, -1))
+        slope, mine = float(((up - down) * g.double()).sum() / (2 * h)), float((first[i].double() * v.double()).sum())
+        assert abs(slope - mine) <= 2e-3 * float(first[i].norm()) + 1e-3
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_other_streams_and_repeated_graphs(dev, kind):
+    """A call on a side stream, forward and backward; a captured forward replayed on new inputs beside another graph of the same sizes."""
+    call, ts = calls(dev)[kind]
+    ts = [t.requires_grad_() for t in ts]
+    g = torch.ones_like(ts[0])
+    want = [call(*ts)]
+    want += torch.autograd.grad(want[0], ts, g)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = [call(*ts)]
+        got += torch.autograd.grad(got[0], ts, g)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():
+        held = [[t.detach().clone() for t in ts] for _ in range(2)]
+        graphs, outs = [torch.cuda.CUDAGraph() for _ in held], []
+        torch.cuda.synchronize()
+        for graph, tensors in zip(graphs, held):
+            with torch.cuda.graph(graph):
+                outs.append(call(*tensors))
+        held[1][0].copy_(held[1][0].flip(0))
+        for _ in range(2):
+            for graph in graphs:
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, tensors in zip(outs, held):
+            assert torch.equal(out, call(*tensors))
+
+
+def test_a_long_scan_captured_twice_has_workspaces_of_its_own(dev):
+    """Segments' states go through a workspace: two graphs that run at once on two streams do not share it."""
+    runs = []
+    for seed in range(2):
+        ins, _, _ = scan_inputs((2000, 1, 64, 16, 1), F16, torch.Generator().manual_seed(seed))
+        runs.append({n: t.to(dev) for n, t in ins.items() if n != "s"})
+    want = [ss.selective_scan(**r) for r in runs]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in runs]
+    torch.cuda.synchronize()
+    for r in runs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(ss.selective_scan(**r))
+    for _ in range(5):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_expanded_inputs_and_gradients(dev, kind):
+    """Inputs broadcast over the batch: read with stride 0, their gradients summed by autograd."""
+    call, ts = calls(dev, F32)[kind]
+    base = [t[:, :1].detach().clone().requires_grad_() if t.dim() >= 3 else t.detach().requires_grad_() for t in ts]
+    wide = [t.expand(t.shape[0], 3, *t.shape[2:]) if t.dim() >= 3 else t for t in base]
+    y = call(*wide)
+    assert torch.equal(y[:, 0], y[:, 2])
+    got = torch.autograd.grad(y.sum(), base)
+    whole = [t.detach().contiguous().requires_grad_() for t in wide]
+    want = torch.autograd.grad(call(*whole).sum(), whole)
+    for a, b, t in zip(got, want, base):
+        b = b.sum(1, keepdim=True) if t.dim() >= 3 else b
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-5 * float(b.abs().max()))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_what_is_refused(dev, kind):
+    call, ts = calls(dev)[kind]
+    with pytest.raises(TypeError, match="one dtype"):
+        call(ts[0].float(), *ts[1:])
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        call(*[t.double() for t in ts])
+    with pytest.raises(RuntimeError, match="expected all tensors on|no CPU path"):
+        call(ts[0], *[t.cpu() for t in ts[1:]])
+    with pytest.raises(AssertionError, match="expected"):
+        call(ts[0], ts[1][1:], *ts[2:])
+    t = [u.detach().requires_grad_() for u in ts]
+    y = call(*t)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(y.sum(), t, create_graph=True)
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call(fw.make_dual(ts[0], torch.ones_like(ts[0])), *ts[1:])
+    y = call(*t)
+    with torch.no_grad():
+        t[0].add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_states_that_cannot_be_updated_in_place_are_refused(dev):
+    _, (x, w, _) = calls(dev)["conv"]
+    with pytest.raises(ValueError, match="contiguous"):
+        ss.incremental_causal_conv(x=x, weight=w, state=torch.zeros(3, 64, 3, device=dev).half().transpose(1, 2))
+    with pytest.raises(AssertionError, match="state"):
+        ss.incremental_causal_conv(x=x, weight=w, state=torch.zeros(3, 4, 64, device=dev).half())
+    with pytest.raises(ValueError, match="window"):
+        ss.causal_conv(x=x, weight=torch.zeros(64, 9, device=dev).half())
+    _, ts = calls(dev)["scan"]
+    args = dict(zip(("x", "dt", "a", "b", "c"), ts))
+    with pytest.raises(ValueError, match="contiguous"):
+        ss.incremental_selective_scan(**args, s=torch.zeros(3, 16, 64, device=dev).transpose(1, 2))
+    with pytest.raises(TypeError, match="fp32"):
+        ss.incremental_selective_scan(**args, s=torch.zeros(3, 64, 16, device=dev).half())
+    with pytest.raises(TypeError, match="fp32"):
+        ss.selective_scan(**{**args, "a": ts[2].half()})
+    with pytest.raises(ValueError, match="states per channel"):
+        big = torch.zeros(20, 3, 1, 65, device=dev).half()
+        ss.selective_scan(**{**args, "a": torch.zeros(64, 65, device=dev), "b": big, "c": big})
+    with pytest.raises(ValueError, match="groups"):
+        ss.selective_scan(**{**args, "b": ts[3].repeat(1, 1, 3, 1), "c": ts[4].repeat(1, 1, 3, 1)})
+    with pytest.raises(AssertionError, match="key_padding_mask"):
+        ss.selective_scan(**args, key_padding_mask=torch.zeros(20, 3, device=dev))
+    with pytest.raises(ValueError, match="groups"):
+        ss.group_norm(x=x, num_groups=3)
+
+
+def test_a_state_at_an_odd_address_is_updated_in_place(dev):
+    _, ts = calls(dev, T=1)["scan"]
+    args = dict(zip(("x", "dt", "a", "b", "c", "d", "dt_bias"), ts))
+    s = torch.randn(3 * 64 * 16 + 1, device=dev)
+    odd, plain = s[1:].view(3, 64, 16), s[1:].view(3, 64, 16).clone()
+    y, same = ss.incremental_selective_scan(**args, s=odd)
+    y2, _ = ss.incremental_selective_scan(**args, s=plain)
+    assert same is odd and torch.equal(odd, plain) and torch.equal(y, y2)
+
+
+# --------------------------------------------------------------------------- the layer, a run of them together
+def layer(dev, dtype, **more):
+    torch.manual_seed(0)
+    return SelectiveStateSpace(embed_dim=96, state_dim=12, **more).to(dev).to(dtype)
+
+
+def layer_oracle(m, x, mask):
+    """The layer's forward from the oracle's functions, fp64 on the CPU."""
+    p = {n: t.detach().double().cpu() for n, t in m.named_parameters()}
+    u, gate = (x @ p["in_proj.weight"].t()).chunk(2, -1)
+    u = O.conv(clean(u, mask), p["conv_weight"], p["conv_bias"], None, mask, True)["y"]
+    n, g = m.state_dim, m.num_groups
+    low, b, c = (u @ p["x_proj.weight"].t()).split([m.dt_rank, g * n, g * n], -1)
+    y = O.scan(u, low @ p["dt_proj.weight"].t(), -torch.exp(p["a_log"]), b.unflatten(-1, (g, n)), c.unflatten(-1, (g, n)), p["d"], p["dt_bias"], None, mask,
+               True)["y"]
+    y = O.norm(y, m.norm_groups, p["norm_weight"], p["norm_bias"], gate, True, 1e-5)["y"]
+    return y @ p["out_proj.weight"].t() + p["out_proj.bias"]
+
+
+@pytest.mark.parametrize("pad", [None, "right", "left"])
+@pytest.mark.parametrize("more", [{}, dict(num_groups=2, norm_groups=4, conv_width=3)])
+def test_layer(dev, pad, more):
+    """fp32: a dozen operators of fp32 precision and TF32-free products one after another, 1e-5 of the norm."""
+    m = layer(dev, F32, **more)
+    gen = torch.Generator().manual_seed(5)
+    x, mask = torch.randn(45, 3, 96, generator=gen), padding(3, 45, pad, gen)
+    y = m(x.to(dev), key_padding_mask=None if mask is None else mask.to(dev))
+    want = layer_oracle(m, x.double(), mask)
+    there = torch.ones(45, 3, dtype=torch.bool) if mask is None else ~mask.t()
+    assert (y.cpu().double() - want)[there].norm() <= 1e-5 * want[there].norm()
+    g = torch.randn(45, 3, 96, generator=gen).to(dev) * there[..., None].to(dev)
+    xs = x.to(dev).requires_grad_()
+    m(xs, key_padding_mask=None if mask is None else mask.to(dev)).backward(g)
+    v = torch.randn(45, 3, 96, generator=gen).double()
+    h = 2.0 ** -12                                                # differences of the oracle: its third derivative times h^2
+    slope = ((layer_oracle(m, x.double() + h * v, mask) - layer_oracle(m, x.double() - h * v, mask)) * g.cpu().double()).sum() / (2 * h)
+    mine = (xs.grad.cpu().double() * v).sum()
+    assert abs(slope - mine) <= 1e-4 * float(xs.grad.norm()) * float(v.norm()) / 45 + 1e-4 * abs(float(slope))
+    assert all(p.grad is not None and p.grad.isfinite().all() for p in m.parameters())
+
+
+@pytest.mark.parametrize("dtype,tol", [(F32, 1e-5), (F16, 1e-2), (BF16, 8e-2)])
+def test_layer_prompt_then_tokens(dev, dtype, tol):
+    """A padded prompt and then single tokens with the kept state, a reordered batch on the way, is the whole sequence at once.  Products
+    of other shapes round differently: a few steps of the type through seven roundings (2^-9, 2^-6), relative to the norm."""
+    m = layer(dev, dtype).requires_grad_(False)
+    gen = torch.Generator().manual_seed(2)
+    T, P, B = 30, 19, 3
+    x = torch.randn(T, B, 96, generator=gen).to(dtype).to(dev)
+    mask = torch.zeros(B, P, dtype=torch.bool, device=dev)
+    mask[0, 11:], mask[2, 1:] = True, True
+    state = {}
+    m(x[:P], key_padding_mask=mask, saved_state=state)
+    order = torch.tensor([2, 0, 1])
+    m.reorder_incremental_state(state, order)
+    steps = torch.cat([m(x[t:t + 1], saved_state=state) for t in range(P, T)])
+    for slot, row in enumerate(order.tolist()):
+        alone = torch.cat([x[:P, row][~mask[row]], x[P:, slot]]).unsqueeze(1)
+        want = m(alone)[-(T - P):, 0]
+        assert (steps[:, slot] - want).float().norm() <= tol * want.float().norm()
+
+
+def test_layer_under_autocast_and_with_gradients_through_its_state(dev):
+    m = layer(dev, F32)
+    x = torch.randn(6, 2, 96, device=dev)
+    with torch.autocast("cuda", dtype=BF16):
+        y = m(x)
+    assert y.dtype == BF16 and (y.float() - m(x)).norm() <= 0.08 * m(x).norm()
+    xs = x.clone().requires_grad_()
+    state = {}
+    a = m(xs[:4], saved_state=state)
+    first = dict(state)
+    b = m(xs[4:], saved_state=state)
+    assert state["prev_s"] is not first["prev_s"] and state["prev_s"].requires_grad
+    got = torch.autograd.grad(torch.cat([a, b]).sum(), xs)[0]
+    want = torch.autograd.grad(m(xs).sum(), xs)[0]
+    assert (got - want).norm() <= 1e-5 * want.norm()
+
+
+def test_layer_trains_inside_a_graph(dev):
+    """A whole step with its backward captured after warm-up on a side stream, replayed twice, gives the eager gradients."""
+    m, x = layer(dev, F16), torch.randn(33, 2, 96, device=dev).half()
+    params = list(m.parameters())
+    want = torch.autograd.grad(m(x).float().sum(), params)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        torch.autograd.grad(m(x).float().sum(), params)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = torch.autograd.grad(m(x).float().sum(), params)
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert (a - b).float().norm() <= 1e-2 * b.float().norm() + 1e-6
+
+
+def test_the_python_node_gives_the_native_ones_results(dev):
+    """Inside a dispatch mode the calls go through Python autograd functions."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    for call, ts in calls(dev).values():
+        ts = [t.requires_grad_() for t in ts]
+        want = call(*ts)
+        with Seen():
+            got = call(*ts)
+        assert torch.equal(got, want) and "Backward" in type(got.grad_fn).__name__
+        for a, b in zip(torch.autograd.grad(got.sum(), ts), torch.autograd.grad(want.sum(), ts)):
+            assert torch.equal(a, b)
+
+
+def test_tensor_level_calls(dev):
+    """``ops``: what is not asked for is None, and a state that is not updated in place is left alone."""
+    _, (x, w, b) = calls(dev)["conv"]
+    s = torch.ones(3, 3, 64, device=dev).half()
+    y, out = ops.causal_conv_fwd(x, w, b, s, None, True, True)
+    assert out is not s and bool((s == 1).all()) and torch.equal(out, x[-3:].transpose(0, 1))
+    gx, gw, gb, gs = ops.causal_conv_bwd(x, w, b, s, None, True, y, None, False, False, False)
+    assert gw is None and gb is None and gs is None and gx.shape == x.shape
+    _, ts = calls(dev, T=1)["scan"]
+    s = torch.ones(3, 64, 16, device=dev)
+    y, out, kept = ops.selective_scan_fwd(*ts, s, return_state=True)
+    assert kept is None and bool((s == 1).all()) and not torch.equal(out, s)
+    with pytest.raises(ValueError, match="checkpoints"):
+        ops.selective_scan_bwd(*ts, s, None, True, y, None, None, False)
