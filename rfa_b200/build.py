@@ -18,8 +18,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "librfa_b200.so")
-NATIVE_SRCS = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_state_space.cpp")]
-NATIVE = os.path.join(HERE, "_native.so")
+NATIVE_SRC, NATIVE = os.path.join(CSRC, "torch_ops.cpp"), os.path.join(HERE, "_native.so")
+NATIVE_SRCS = [NATIVE_SRC, os.path.join(CSRC, "torch_state_space.cpp")]
 NATIVE_KEY = os.path.join(HERE, "_native.key")      # what the module was built for (see native_key)
 
 NVCC_FLAGS = [
