@@ -1,38 +1,132 @@
 // Shared by the selective scan's forward and backward: the work of a CTA, its tiles in shared memory, how inputs are staged.
 //
-// A state element (channel i, state n) evolves alone, so a thread holds 2 adjacent channels x 4 adjacent states in registers and walks the
-// tokens; LN = 2, 4, 8 or 16 neighbouring lanes hold a channel's up to 4 LN states.  A CTA of four warps has 256 / LN channels
-// of one group and one batch row, and a segment of the tokens; tiles of 16 tokens go through shared memory: inputs are asked for a
-// tile ahead as wide loads along the channels, turned into fp32 (delta = softplus(dt + bias) once per channel) by the thread that
-// loaded them, and read by the scan as one 16-byte word per token (both channels' delta and x, broadcast to the LN lanes) and one each of b, c.
+// A state element (channel i, state n) evolves alone, so a thread holds 2 adjacent channels x 4 states in registers and walks the
+// tokens; LN = 2, 4, 8 or 16 neighbouring lanes hold a channel's up to 4 LN states, lane l the states l, LN + l, 2 LN + l, 3 LN + l.  A CTA
+// has 256 / LN channels of one group and one batch row, and a segment of the tokens.  Four of its warps scan; four others bring tiles of
+// inputs and take results away meanwhile, so that a scheduler with few CTAs still has work while one warp waits.
+//
+// Exponentials are what bounds it: 16 a clock and SM come from the special function unit.  The first of a thread's four states -- the first
+// quarter of a channel's -- takes a polynomial on the FMA units instead (`decays`), at which both are busy equally long.  Issue slots come
+// next: arithmetic whose operands stand side by side is packed, both channels in one instruction (`fma.rn.f32x2`); products with
+// b and c, one value for both, are not, as copying those into pairs costs what it saves.
+//
+// Tiles of 16 tokens go through shared memory, two of them by turns: a thread asks for a pair of channels' inputs a tile ahead (a warp's loads are whole 128-byte
+// rows), turns them into delta and delta x and leaves them as one 16-byte word, which the scan's lanes read.  Shared memory hands a
+// warp 128 bytes a clock whether lanes read the same words or not: 48 bytes a lane and token (b and c as pairs of equal
+// values were 80, and bound the forward at 245 us for 8 x 2048 x 2048).
 #pragma once
 
 #include "state_space.cuh"
 
 namespace rfa {
 
-constexpr int kScanThreads = 128, kScanTile = 16;      // tokens of a tile, and of a checkpoint
+constexpr int kScanThreads = 128, kScanTile = 16;      // threads of either half of a CTA; tokens of a tile, and of a checkpoint
 
 struct ScanShape {
   int64_t T;
   int B, D, N, G, heads;          // heads = D / G channels share b and c
-  int per_group, tiles, seg_tiles, segs, n4;      // CTAs per group, tiles of the sequence, tiles per segment, segments; states rounded up to 4
+  int per_group, tiles, seg_tiles, segs, kn;      // CTAs per group, tiles of the sequence, tiles per segment, segments; states of a kept row (4 LN)
 };
+
+// The two halves of a CTA meet at named barriers: a tile is there (kFull + buffer), a tile has been scanned (kDone + buffer).  Every tile
+// passes both once, on each side, in one order: no wait is left over.
+enum { kFull = 1, kDone = 3 };
+__device__ __forceinline__ void meet_wait(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(2 * kScanThreads) : "memory"); }
+__device__ __forceinline__ void meet_go(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(2 * kScanThreads) : "memory"); }
 
 template <int LN> struct ScanTile {
   static constexpr int kChannels = 256 / LN, kN = 4 * LN, kPairs = kChannels / 2;
-  static constexpr int kVecs = kChannels / 8;                       // runs of eight channels
-  static constexpr int kRows = kScanThreads / kVecs;                // tokens that the CTA loads side by side
-  static constexpr int kPasses = kRows >= kScanTile ? 1 : kScanTile / kRows;
+  static constexpr int kRows = kScanThreads / kPairs;               // tokens that the CTA loads side by side
+  static constexpr int kPasses = kScanTile / kRows;
   static constexpr int kBc = kScanTile * kN / kScanThreads;         // elements of b (and of c) per thread and tile
-  static_assert(kBc >= 1, "a tile of b");
+  static_assert(kPasses >= 1 && kBc >= 1, "a tile is work for every thread");
 };
 
-// What a thread of the CTA is.
+// ---- two floats in one instruction -------------------------------------------------------------------------------------------
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
+
+__device__ __forceinline__ f32x2 exp2_unit(f32x2 u) {
+  const float2 v = split2(u);
+  return pack2(ex2(v.x), ex2(v.y));
+}
+// The first state's on the FMA units, -126 <= u < 128 (below: 2^-126): u = k + r with k whole (the addition of 1.5 * 2^23 rounds) and
+// |r| <= 1/2, 2^r by a polynomial of degree 5 with 1 + r log 2 in front (least maximum of the relative error, by Lawson's iteration:
+// 1.1e-7, and 2.3e-7 |r| near 0, so that a decay near 1 is as near as its argument is), k added to the exponent.
+//
+// For R tokens, one step at a time: few warps share an SM's scheduler, and a chain alone would wait for itself.
+template <int R> struct Poly {
+  f32x2 t[R], r[R], p[R];
+  __device__ __forceinline__ void begin(const f32x2* delta, f32x2 a2) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float2 v = split2(mul2(delta[i], a2));
+      r[i] = pack2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+    }
+  }
+  __device__ __forceinline__ void step(int k) {        // 0 ... 7, all in order
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (k == 0) t[i] = add2(r[i], both(12582912.f));
+      if (k == 1) p[i] = add2(t[i], both(-12582912.f));
+      if (k == 2) r[i] = fma2(p[i], both(-1.f), r[i]);
+      if (k == 3) p[i] = fma2(both(1.33006054e-3f), r[i], both(9.66969132e-3f));
+      if (k == 4) p[i] = fma2(p[i], r[i], both(5.55055849e-2f));
+      if (k == 5) p[i] = fma2(p[i], r[i], both(2.40222827e-1f));
+      if (k == 6) p[i] = fma2(p[i], r[i], both(kLn2));
+      if (k == 7) p[i] = fma2(p[i], r[i], both(1.f));
+    }
+  }
+  __device__ __forceinline__ f32x2 end(int i) const {
+    const float2 q = split2(p[i]), k = split2(t[i]);
+    return pack2(__int_as_float(__float_as_int(q.x) + (__float_as_int(k.x) << 23)), __int_as_float(__float_as_int(q.y) + (__float_as_int(k.y) << 23)));
+  }
+};
+// exp(delta a) of both channels for R tokens and the thread's four states, a in units of log 2
+template <int R> __device__ __forceinline__ void decays(const f32x2* delta, const f32x2* a2, f32x2 (*e)[4]) {
+  Poly<R> poly;
+  poly.begin(delta, a2[0]);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 1; j < 4; ++j) e[i][j] = exp2_unit(mul2(delta[i], a2[j]));
+#pragma unroll
+  for (int k = 0; k < 8; ++k) poly.step(k);
+#pragma unroll
+  for (int i = 0; i < R; ++i) e[i][0] = poly.end(i);
+}
+
+// ---- the work of a thread ----------------------------------------------------------------------------------------------------
 template <int LN> struct ScanThread {
   int group, c0, nch, b;          // the CTA's group, first channel, channels (<= kChannels), batch row
-  int lane, warp, ln, pair;       // this thread's place in the scan: lane of the channel, pair of channels in the CTA
-  int vec, row;                   // and when it loads: run of eight channels, first token
+  bool scans;                     // or brings and takes
+  int tid, ln, pair;              // in the scan: lane of the channel, pair of channels in the CTA
+  int vpair, row, vn;             // when it brings: pair of channels, first token, how many of the two channels there are
   __device__ ScanThread(const ScanShape& s) {
     using Tile = ScanTile<LN>;
     group = blockIdx.x / s.per_group;
@@ -40,69 +134,137 @@ template <int LN> struct ScanThread {
     c0 = group * s.heads + in_group;
     nch = min(Tile::kChannels, s.heads - in_group);
     b = blockIdx.y;
-    lane = threadIdx.x & 31; warp = threadIdx.x >> 5;
-    ln = lane % LN;
-    pair = warp * (32 / LN) + lane / LN;
-    vec = threadIdx.x % Tile::kVecs;
-    row = threadIdx.x / Tile::kVecs;
+    scans = threadIdx.x < kScanThreads;
+    tid = threadIdx.x % kScanThreads;
+    ln = tid % LN;
+    pair = tid / LN;
+    vpair = tid % Tile::kPairs;
+    row = tid / Tile::kPairs;
+    vn = max(0, min(2, nch - 2 * vpair));
   }
-  __device__ int first_channel() const { return 2 * pair; }      // in the CTA
+  // n of the thread's state j, and whether channel k of its pair has it
+  __device__ __forceinline__ int state(int j) const { return j * LN + ln; }
+  __device__ __forceinline__ bool has(int k, int j, int N) const { return 2 * pair + k < nch && state(j) < N; }
+  __device__ __forceinline__ int channel(int k) const { return c0 + 2 * pair + k; }
+  // rows [D][N] of fp32 at p, both channels' state j; 0 where there is none
+  __device__ __forceinline__ f32x2 get(const float* p, int j, int N) const {
+    float v[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) v[k] = has(k, j, N) ? p[(size_t)channel(k) * N + state(j)] : 0.f;
+    return pack2(v[0], v[1]);
+  }
+  __device__ __forceinline__ void put(float* p, int j, int N, f32x2 v) const {
+    const float2 f = split2(v);
+    if (has(0, j, N)) p[(size_t)channel(0) * N + state(j)] = f.x;
+    if (has(1, j, N)) p[(size_t)channel(1) * N + state(j)] = f.y;
+  }
+  // kept rows [D][kN], a lane's four states adjacent
+  __device__ __forceinline__ void load_kept(const float* p, f32x2* v) const {
+    float4 f[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      f[k] = 2 * pair + k < nch ? *reinterpret_cast<const float4*>(p + (size_t)channel(k) * (4 * LN) + 4 * ln) : make_float4(0.f, 0.f, 0.f, 0.f);
+    v[0] = pack2(f[0].x, f[1].x); v[1] = pack2(f[0].y, f[1].y); v[2] = pack2(f[0].z, f[1].z); v[3] = pack2(f[0].w, f[1].w);
+  }
+  __device__ __forceinline__ void store_kept(float* p, const f32x2* v) const {
+    const float2 a = split2(v[0]), b = split2(v[1]), c = split2(v[2]), d = split2(v[3]);
+    if (2 * pair < nch) *reinterpret_cast<float4*>(p + (size_t)channel(0) * (4 * LN) + 4 * ln) = make_float4(a.x, b.x, c.x, d.x);
+    if (2 * pair + 1 < nch) *reinterpret_cast<float4*>(p + (size_t)channel(1) * (4 * LN) + 4 * ln) = make_float4(a.y, b.y, c.y, d.y);
+  }
 };
 
-// One tile's raw b or c: element e = thread + i * 128 of [token][state].
-template <typename T, int LN> struct RawStates {
-  T v[ScanTile<LN>::kBc];
-  __device__ __forceinline__ void load(const T* p, int64_t stride, int tokens, int N, const uint8_t* gone) {
+// Which of a thread's tokens of a tile are there: bit i of pass i.  A plain tile is full, of a full CTA, without a mask and in wide words:
+// nothing is asked about its elements (the questions were a quarter of the forward's instructions).
+template <int LN> __device__ __forceinline__ uint32_t tokens_here(const ScanThread<LN>& th, const uint8_t* mask, int64_t t0, int64_t T) {
+  uint32_t here = 0;
 #pragma unroll
-    for (int i = 0; i < ScanTile<LN>::kBc; ++i) {
-      const int e = threadIdx.x + i * kScanThreads, t = e / ScanTile<LN>::kN, n = e % ScanTile<LN>::kN;
-      v[i] = t < tokens && n < N && !(gone && gone[t]) ? p[(int64_t)t * stride + n] : from_f<T>(0.f);
+  for (int i = 0; i < ScanTile<LN>::kPasses; ++i) {
+    const int64_t t = t0 + th.row + i * ScanTile<LN>::kRows;
+    if (t < T && !(mask && mask[t])) here |= 1u << i;
+  }
+  return here;
+}
+// Both channels of a thread's tokens, as they stand in memory; p: at the thread's first token of the tile.
+template <typename T, int LN> struct RawPairs {
+  Raw<T, 2> v[ScanTile<LN>::kPasses];
+  template <bool kPlain> __device__ __forceinline__ void load(const T* p, int64_t stride, uint32_t here, int vn, bool wide) {
+#pragma unroll
+    for (int i = 0; i < ScanTile<LN>::kPasses; ++i) {
+      const T* at = p + i * ScanTile<LN>::kRows * stride;
+      if (kPlain) {
+        v[i].load(at, 2, true);
+      } else {
+        v[i].zero();
+        if (here >> i & 1) v[i].load(at, vn, wide);
+      }
     }
   }
-  __device__ __forceinline__ void store(float* smem) const {
+};
+// One tile's b or c, as they stand in memory, n = thread % kN of tokens thread / kN + i * 128 / kN; in shared memory a lane's four states are
+// adjacent.
+template <typename T, int LN> struct RawStates {
+  static constexpr int kN = ScanTile<LN>::kN, kStep = kScanThreads / kN;
+  T v[ScanTile<LN>::kBc];
+  template <bool kPlain> __device__ __forceinline__ void load(const T* p, int64_t stride, int64_t t0, int64_t T_, int N, const uint8_t* mask) {
+    const int tid = threadIdx.x % kScanThreads, n = tid % kN;
+    const T* at = p + (t0 + tid / kN) * stride + n;
 #pragma unroll
-    for (int i = 0; i < ScanTile<LN>::kBc; ++i) smem[threadIdx.x + i * kScanThreads] = to_f(v[i]);
+    for (int i = 0; i < ScanTile<LN>::kBc; ++i) {
+      const int64_t t = t0 + tid / kN + i * kStep;
+      v[i] = kPlain || (t < T_ && n < N && !(mask && mask[t])) ? at[i * kStep * stride] : from_f<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void store(float (*smem)[kN]) const {
+    const int tid = threadIdx.x % kScanThreads, n = tid % kN, t = tid / kN;
+#pragma unroll
+    for (int i = 0; i < ScanTile<LN>::kBc; ++i) smem[t + i * kStep][(n % LN) * 4 + n / LN] = to_f(v[i]);
   }
 };
+struct Plain { static constexpr bool value = true; };
+struct Ragged { static constexpr bool value = false; };
 
-__device__ __forceinline__ void load4f(const float* p, int n, float* v) {      // n of 4, the rest 0; 16 | p's address
-  if (n >= 4) {
-    const float4 f = *reinterpret_cast<const float4*>(p);
-    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
+// softplus of both channels, and with `kSlope` its derivatives (state_space.cuh has one alone)
+template <bool kSlope> __device__ __forceinline__ f32x2 softplus2(float2 v, float2& sig) {
+  const float2 z = make_float2(ex2(-kLog2e * fabsf(v.x)), ex2(-kLog2e * fabsf(v.y)));
+  const f32x2 z2 = pack2(z.x, z.y);
+  const float2 d = split2(add2(z2, both(2.f)));
+  const f32x2 w = mul2(z2, pack2(rcp(d.x), rcp(d.y))), s = mul2(w, w);
+  f32x2 q = fma2(both(0.281577788f), s, both(0.279651582f));
+  q = fma2(q, s, both(0.400245965f));
+  q = fma2(q, s, both(0.666663229f));
+  q = fma2(q, s, both(2.f));
+  if (kSlope) {
+    const float r0 = rcp(1.f + z.x), r1 = rcp(1.f + z.y);
+    sig = make_float2(v.x >= 0.f ? r0 : z.x * r0, v.y >= 0.f ? r1 : z.y * r1);
   }
+  return fma2(w, q, pack2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
 }
-__device__ __forceinline__ void load4u(const float* p, int n, float* v) {      // any address
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
+__device__ __forceinline__ void lane_states(const float* row, int ln, float* v) {
+  const float4 f = *reinterpret_cast<const float4*>(row + 4 * ln);
+  v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
 }
-__device__ __forceinline__ void store4u(float* p, int n, const float* v, bool wide) {
-  if (wide && n >= 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) p[i] = v[i];
-  }
+// both channels' products with one factor, and sums of such
+__device__ __forceinline__ f32x2 scale(float2 v, float f) { return pack2(v.x * f, v.y * f); }
+__device__ __forceinline__ f32x2 scale_add(float2 v, float f, f32x2 c) {
+  const float2 d = split2(c);
+  return pack2(fmaf(v.x, f, d.x), fmaf(v.y, f, d.y));
 }
 
 // Sums `K` values over LN lanes, dealing the results out: afterwards v[0 .. max(1, K / LN)) of lane l are the totals of values
 // l * K / LN ... (K >= LN), or of value l * K / LN in every lane (K < LN).  K / 2 + K / 4 + ... exchanges instead of K log LN.
-template <int K, int LN, int W = LN> __device__ __forceinline__ void lanes_sum(float* v, int ln, int stride = 1) {
+template <int K, int LN, int W = LN> __device__ __forceinline__ void lanes_sum(float* v, int ln) {
   if constexpr (W > 1) {
-    const bool upper = ln & (W / 2);
     if constexpr (K > 1) {
+      const bool upper = ln & (W / 2);
 #pragma unroll
       for (int i = 0; i < K / 2; ++i) {
         const float give = upper ? v[i] : v[i + K / 2], keep = upper ? v[i + K / 2] : v[i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, give, (W / 2) * stride);
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, give, W / 2);
       }
-      lanes_sum<K / 2, LN, W / 2>(v, ln, stride);
+      lanes_sum<K / 2, LN, W / 2>(v, ln);
     } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], (W / 2) * stride);
-      lanes_sum<1, LN, W / 2>(v, ln, stride);
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], W / 2);
+      lanes_sum<1, LN, W / 2>(v, ln);
     }
   }
 }

@@ -7,6 +7,7 @@
 // Few rows (a prompt of one sequence) leave SMs idle: the tokens are then cut into segments.  A first kernel leaves each segment's own state
 // from zero and the sum of its deltas -- over which a whole segment's decay is exp(a sum delta), one exponential -- and the main kernel's
 // CTAs begin with the states of the segments before theirs joined up, which costs the first kernel's pass over dt, x and b once more.
+#include <stdlib.h>
 #include "scan.cuh"
 
 namespace rfa {
@@ -20,8 +21,8 @@ ScanShape scan_shape(int64_t T, int B, int D, int N, int G, bool backward) {
   s.heads = D / G;
   s.per_group = (s.heads + channels - 1) / channels;
   s.tiles = (int)((T + kScanTile - 1) / kScanTile);
-  s.n4 = (N + 3) / 4 * 4;
-  const int64_t ctas = (int64_t)s.per_group * G * B, want = 148 * (backward ? 2 : 4);
+  s.kn = 4 * scan_lanes(N);
+  const int64_t ctas = (int64_t)s.per_group * G * B, want = getenv("SW") ? atoi(getenv("SW")) : 148 * (backward ? 2 : 4);
   int64_t segs = ctas >= want ? 1 : (want + ctas - 1) / ctas;
   segs = segs < s.tiles / 4 ? segs : s.tiles / 4;
   if (segs < 1) segs = 1;
@@ -45,21 +46,117 @@ int scan_check(const rfa_scan_t* s, const char* what) {
 namespace {
 
 template <int LN> struct __align__(16) FwdSmem {
-  float4 in[2][kScanTile][ScanTile<LN>::kPairs];      // delta, delta', x, x' of two adjacent channels; then y, y' in place of the deltas
-  float b[2][kScanTile][ScanTile<LN>::kN], c[2][kScanTile][ScanTile<LN>::kN];
+  using Tile = ScanTile<LN>;
+  static constexpr int kRow = Tile::kPairs * 2 + 8;    // the 8: neighbouring rows in other banks
+  float4 in[2][kScanTile][Tile::kPairs];               // delta, delta', delta x, delta' x' of two adjacent channels
+  float b[2][kScanTile][Tile::kN], c[2][kScanTile][Tile::kN];
+  f32x2 y[2][kScanTile][LN / 2][kRow];                 // c . s, each lane's share; two lanes' side by side
 };
 
 struct FwdArgs {
   ScanShape sh;
   rfa_scan_t p;
   void* y;
-  float *s_out, *ckpt, *seg_state, *seg_sum;      // seg_state [segs - 1][B][D][n4], seg_sum [segs - 1][B][D]
-  bool wide, states16;                            // x and dt in 16-byte words; states in 16-byte words
+  float *s_out, *ckpt, *seg_state, *seg_sum;      // seg_state [segs - 1][B][D][kn], seg_sum [segs - 1][B][D]
+  bool wide;                                      // pairs of x, dt and y as one word
 };
 
-// kSummary: the state a segment reaches from zero, and its sum of deltas; no c, no y.
+// Brings the tiles of a segment and takes their outputs away.  kSummary: no c, no y.
 template <typename T, int LN, bool kSummary>
-__global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(const __grid_constant__ FwdArgs A) {
+__device__ __forceinline__ void fwd_bring(const FwdArgs& A, FwdSmem<LN>& sm, const ScanThread<LN>& th, int tile0, int tile1) {
+  using Tile = ScanTile<LN>;
+  const ScanShape& sh = A.sh;
+  const rfa_scan_t& p = A.p;
+  const int ch = th.c0 + 2 * th.vpair;
+  const T* x = static_cast<const T*>(p.x) + (int64_t)th.b * p.x_b + ch;
+  const T* dt = static_cast<const T*>(p.dt) + (int64_t)th.b * p.dt_b + ch;
+  const T* bp = static_cast<const T*>(p.b) + (int64_t)th.b * p.b_b + (int64_t)th.group * p.b_g;
+  const T* cp = static_cast<const T*>(p.c) + (int64_t)th.b * p.c_b + (int64_t)th.group * p.c_g;
+  T* y = static_cast<T*>(A.y) + (int64_t)th.b * sh.D + ch;
+  const int64_t y_t = (int64_t)sh.B * sh.D;
+  const uint8_t* mask = p.mask ? p.mask + (int64_t)th.b * sh.T : nullptr;
+  float bias[2], skip[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    bias[k] = p.dt_bias && k < th.vn ? p.dt_bias[ch + k] : 0.f;
+    skip[k] = !kSummary && p.d && k < th.vn ? p.d[ch + k] : 0.f;
+  }
+  RawPairs<T, LN> rx, rd, kept;
+  RawStates<T, LN> rb, rc;
+  uint32_t here = 0, next = 0;                         // which of this thread's tokens are there: in the tile that is scanned, in the next one
+  const int plain = A.wide && !mask && th.nch == Tile::kChannels && sh.N == Tile::kN ? (int)(sh.T / kScanTile) : 0;      // tiles in front of it are
+  const auto ask = [&](int tile, auto kind) {
+    constexpr bool kPlain = decltype(kind)::value;
+    const int64_t t0 = (int64_t)tile * kScanTile, t = t0 + th.row;
+    next = kPlain ? ~0u : tokens_here<LN>(th, mask, t0, sh.T);
+    rx.template load<kPlain>(x + t * p.x_t, p.x_t, next, th.vn, A.wide);
+    rd.template load<kPlain>(dt + t * p.dt_t, p.dt_t, next, th.vn, A.wide);
+    rb.template load<kPlain>(bp, p.b_t, t0, sh.T, sh.N, mask);
+    if (!kSummary) rc.template load<kPlain>(cp, p.c_t, t0, sh.T, sh.N, mask);
+  };
+  const auto ask_tile = [&](int tile) { tile < plain ? ask(tile, Plain()) : ask(tile, Ragged()); };
+  const auto put = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < Tile::kPasses; ++i) {
+      float2 sig;
+      const float2 v = make_float2(rd.v[i].get(0) + bias[0], rd.v[i].get(1) + bias[1]);
+      const f32x2 delta = p.softplus ? softplus2<false>(v, sig) : pack2(v.x, v.y);
+      const f32x2 dx = mul2(delta, pack2(rx.v[i].get(0), rx.v[i].get(1)));
+      const bool on = next >> i & 1;
+      *reinterpret_cast<ulonglong2*>(&sm.in[buf][th.row + i * Tile::kRows][th.vpair]) = make_ulonglong2(on ? delta : 0, on ? dx : 0);
+    }
+    rb.store(sm.b[buf]);
+    if (!kSummary) rc.store(sm.c[buf]);
+  };
+  const auto take = [&](int tile, int buf) {
+    const int64_t t0 = (int64_t)tile * kScanTile;
+#pragma unroll
+    for (int i = 0; i < Tile::kPasses; ++i) {
+      const int t = th.row + i * Tile::kRows;
+      if (t0 + t >= sh.T) continue;
+      f32x2 v[LN];
+#pragma unroll
+      for (int l = 0; l < LN; l += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&sm.y[buf][t][l / 2][2 * th.vpair]);
+        v[l] = two.x; v[l + 1] = two.y;
+      }
+#pragma unroll
+      for (int w = LN / 2; w > 0; w /= 2)
+#pragma unroll
+        for (int l = 0; l < w; ++l) v[l] = add2(v[l], v[l + w]);
+      const float2 f = split2(v[0]);
+      const bool on = here >> i & 1;
+      Raw<T, 2> out;
+      out.zero();
+      out.set(0, from_f<T>(on ? fmaf(skip[0], kept.v[i].get(0), f.x) : 0.f));
+      out.set(1, from_f<T>(on ? fmaf(skip[1], kept.v[i].get(1), f.y) : 0.f));
+      out.store(y + (t0 + t) * y_t, th.vn, A.wide);
+    }
+  };
+
+  ask_tile(tile0);
+  for (int tile = tile0; tile < tile1; ++tile) {
+    const int buf = (tile - tile0) & 1;
+    put(buf);
+    meet_go(kFull + buf);
+    RawPairs<T, LN> x_now = rx;
+    const uint32_t here_now = next;
+    if (tile + 1 < tile1) ask_tile(tile + 1);
+    if (tile > tile0) {                                // the other buffer's tile
+      meet_wait(kDone + (buf ^ 1));
+      if (!kSummary) take(tile - 1, buf ^ 1);
+    }
+    kept = x_now;
+    here = here_now;
+  }
+  const int last = (tile1 - 1 - tile0) & 1;
+  meet_wait(kDone + last);
+  if (!kSummary) take(tile1 - 1, last);
+}
+
+// kSummary: the state a segment reaches from zero, and its sum of deltas.
+template <typename T, int LN, bool kSummary>
+__global__ void __launch_bounds__(2 * kScanThreads, 2) scan_fwd_kernel(const __grid_constant__ FwdArgs A) {
   using Tile = ScanTile<LN>;
   extern __shared__ char smem_raw[];
   FwdSmem<LN>& sm = *reinterpret_cast<FwdSmem<LN>*>(smem_raw);
@@ -67,190 +164,112 @@ __global__ void __launch_bounds__(kScanThreads) scan_fwd_kernel(const __grid_con
   const rfa_scan_t& p = A.p;
   const ScanThread<LN> th(sh);
   const int seg = blockIdx.z, tile0 = seg * sh.seg_tiles, tile1 = min(tile0 + sh.seg_tiles, sh.tiles);
-  const int n0 = 4 * th.ln, ns = max(0, min(4, sh.N - n0));
-
-  // this thread's states: a in units of log 2, and s
-  float a2[2][4], s[2][4], sum[2] = {};
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int ch = th.first_channel() + k;
-    const int nk = ch < th.nch ? ns : 0;
-    load4u(p.a + (size_t)(th.c0 + ch) * sh.N + n0, nk, a2[k]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) a2[k][j] *= kLog2e;
-    if (kSummary || !p.s_in) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[k][j] = 0.f;
-    } else {
-      load4u(p.s_in + ((size_t)th.b * sh.D + th.c0 + ch) * sh.N + n0, nk, s[k]);
-    }
-    if (!kSummary)
-      for (int i = 0; i < seg; ++i) {                  // the segments before this one
-        if (ch >= th.nch) continue;
-        const size_t at = ((size_t)i * sh.B + th.b) * sh.D + th.c0 + ch;
-        float v[4];
-        load4f(A.seg_state + at * sh.n4 + n0, n0 < sh.n4 ? 4 : 0, v);
-        const float total = A.seg_sum[at];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[k][j] = fmaf(ex2(total * a2[k][j]), s[k][j], v[j]);
-      }
+  if (!th.scans) {
+    fwd_bring<T, LN, kSummary>(A, sm, th, tile0, tile1);
+    return;
   }
 
-  // what this thread loads and writes: eight channels, kPasses tokens of a tile
-  const T *x = static_cast<const T*>(p.x), *dt = static_cast<const T*>(p.dt);
-  const T* bp = static_cast<const T*>(p.b) + (int64_t)th.b * p.b_b + (int64_t)th.group * p.b_g;
-  const T* cp = static_cast<const T*>(p.c) + (int64_t)th.b * p.c_b + (int64_t)th.group * p.c_g;
-  const int vch = 8 * th.vec, vn = min(8, th.nch - vch);
-  const bool loads = th.row < kScanTile && vn > 0;
-  x += (int64_t)th.b * p.x_b + th.c0 + vch;
-  dt += (int64_t)th.b * p.dt_b + th.c0 + vch;
-  T* y = static_cast<T*>(A.y) + (int64_t)th.b * sh.D + th.c0 + vch;
-  const uint8_t* mask = p.mask ? p.mask + (int64_t)th.b * sh.T : nullptr;
-  float bias[8], skip[8];
+  f32x2 a2[4], s[4], sum = both(0.f);                  // a in units of log 2
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    bias[i] = p.dt_bias && i < vn ? p.dt_bias[th.c0 + vch + i] : 0.f;
-    skip[i] = !kSummary && p.d && i < vn ? p.d[th.c0 + vch + i] : 0.f;
+  for (int j = 0; j < 4; ++j) {
+    a2[j] = mul2(th.get(p.a, j, sh.N), both(kLog2e));
+    s[j] = !kSummary && p.s_in ? th.get(p.s_in + (size_t)th.b * sh.D * sh.N, j, sh.N) : both(0.f);
   }
-
-  Raw<T, 8> rx[Tile::kPasses], rd[Tile::kPasses];
-  RawStates<T, LN> rb, rc;
-  uint32_t here = 0, next = 0;                         // which of this thread's tokens are there: bit i of pass i
-  const auto ask = [&](int tile) {
-    const int64_t t0 = (int64_t)tile * kScanTile;
-    const int tokens = (int)min((int64_t)kScanTile, sh.T - t0);
-    next = 0;
+  if (!kSummary)
+    for (int i = 0; i < seg; ++i) {                    // the segments before this one
+      const size_t at = ((size_t)i * sh.B + th.b) * sh.D;
+      f32x2 v[4];
+      th.load_kept(A.seg_state + at * sh.kn, v);
+      const float* total = A.seg_sum + at + th.channel(0);
+      const f32x2 over = pack2(2 * th.pair < th.nch ? total[0] : 0.f, 2 * th.pair + 1 < th.nch ? total[1] : 0.f);
 #pragma unroll
-    for (int i = 0; i < Tile::kPasses; ++i) {
-      const int t = th.row + i * Tile::kRows;
-      rx[i].zero(); rd[i].zero();
-      if (loads && t < tokens && !(mask && mask[t0 + t])) {
-        next |= 1u << i;
-        rx[i].load(x + (t0 + t) * p.x_t, vn, A.wide);
-        rd[i].load(dt + (t0 + t) * p.dt_t, vn, A.wide);
-      }
+      for (int j = 0; j < 4; ++j) s[j] = fma2(exp2_unit(mul2(over, a2[j])), s[j], v[j]);
     }
-    rb.load(bp + t0 * p.b_t, p.b_t, tokens, sh.N, mask ? mask + t0 : nullptr);
-    if (!kSummary) rc.load(cp + t0 * p.c_t, p.c_t, tokens, sh.N, mask ? mask + t0 : nullptr);
-  };
-  const auto put = [&](int buf) {
-    here = next;
-    if (th.row < kScanTile) {
-#pragma unroll
-      for (int i = 0; i < Tile::kPasses; ++i) {
-        const bool on = here >> i & 1;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (on) {
-            float sig;
-            const float u0 = rd[i].get(j) + bias[j], u1 = rd[i].get(j + 1) + bias[j + 1];
-            v = make_float4(p.softplus ? softplus(u0, sig) : u0, p.softplus ? softplus(u1, sig) : u1, rx[i].get(j), rx[i].get(j + 1));
-          }
-          sm.in[buf][th.row + i * Tile::kRows][th.vec * 4 + j / 2] = v;
-        }
-      }
-    }
-    rb.store(&sm.b[buf][0][0]);
-    if (!kSummary) rc.store(&sm.c[buf][0][0]);
-  };
-
-  ask(tile0);
-  put(0);
   for (int tile = tile0; tile < tile1; ++tile) {
     const int buf = (tile - tile0) & 1;
-    __syncthreads();
-    const uint32_t mine = here;
-    if (tile + 1 < tile1) ask(tile + 1);
-    if (!kSummary && A.ckpt && n0 < sh.n4) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (th.first_channel() + k < th.nch)
-          store4u(A.ckpt + (((size_t)th.b * sh.tiles + tile) * sh.D + th.c0 + th.first_channel() + k) * sh.n4 + n0, 4, s[k], true);
-    }
-    constexpr int kRun = kSummary ? 4 : (LN / 2 < 1 ? 1 : LN / 2);      // tokens whose outputs are summed over the lanes together
+    if (!kSummary && A.ckpt) th.store_kept(A.ckpt + ((size_t)th.b * sh.tiles + tile) * sh.D * sh.kn, s);
+    meet_wait(kFull + buf);
+    constexpr int kRun = 4;                            // tokens whose decays are formed side by side
 #pragma unroll
     for (int t0 = 0; t0 < kScanTile; t0 += kRun) {
-      float out[2 * kRun];
+      f32x2 delta[kRun], dx[kRun], e[kRun][4];
 #pragma unroll
       for (int r = 0; r < kRun; ++r) {
-        const float4 in = sm.in[buf][t0 + r][th.pair];
-        const float4 bv = *reinterpret_cast<const float4*>(&sm.b[buf][t0 + r][n0]);
-        const float bt[4] = {bv.x, bv.y, bv.z, bv.w};
-        const float delta[2] = {in.x, in.y}, dx[2] = {in.x * in.z, in.y * in.w};
-        float ct[4];
-        if (!kSummary) {
-          const float4 cv = *reinterpret_cast<const float4*>(&sm.c[buf][t0 + r][n0]);
-          ct[0] = cv.x; ct[1] = cv.y; ct[2] = cv.z; ct[3] = cv.w;
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float acc = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[k][j] = fmaf(ex2(delta[k] * a2[k][j]), s[k][j], dx[k] * bt[j]);
-            if (!kSummary) acc = fmaf(s[k][j], ct[j], acc);
-          }
-          if (kSummary) sum[k] += delta[k];
-          else out[2 * r + k] = acc;
-        }
+        const ulonglong2 in = *reinterpret_cast<const ulonglong2*>(&sm.in[buf][t0 + r][th.pair]);
+        delta[r] = in.x;
+        dx[r] = in.y;
       }
-      if constexpr (!kSummary) {
-        lanes_sum<2 * kRun, LN>(out, th.ln);           // lane l has value l: token l / 2, channel l % 2
-        __syncwarp();                                  // every lane of the pair has read the deltas
-        float* at = reinterpret_cast<float*>(&sm.in[buf][t0 + th.ln / 2][th.pair]);
-        at[th.ln % 2] = out[0];
+      decays<kRun>(delta, a2, e);
+#pragma unroll
+      for (int r = 0; r < kRun; ++r) {
+        float bt[4];
+        lane_states(sm.b[buf][t0 + r], th.ln, bt);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[r][j] = s[j] = fma2(e[r][j], s[j], scale(split2(dx[r]), bt[j]));
       }
-    }
-    if constexpr (!kSummary) {
-      __syncthreads();
-      const int64_t t0 = (int64_t)tile * kScanTile;
+      if constexpr (kSummary) {
+        sum = add2(sum, add2(add2(delta[0], delta[1]), add2(delta[2], delta[3])));
+      } else {
+        f32x2 out[kRun];
 #pragma unroll
-      for (int i = 0; i < Tile::kPasses; ++i) {
-        const int t = th.row + i * Tile::kRows;
-        if (loads && t0 + t < sh.T) {
-          Raw<T, 8> out;
-          out.zero();
-          if (mine >> i & 1) {
+        for (int r = 0; r < kRun; ++r) {
+          float ct[4];
+          lane_states(sm.c[buf][t0 + r], th.ln, ct);
+          out[r] = scale(split2(e[r][0]), ct[0]);
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-              const float4 v = sm.in[buf][t][th.vec * 4 + j / 2];
-              out.set(j, from_f<T>(fmaf(skip[j], v.z, v.x)));
-              out.set(j + 1, from_f<T>(fmaf(skip[j + 1], v.w, v.y)));
-            }
-          }
-          out.store(y + (t0 + t) * (int64_t)sh.B * sh.D, vn, A.wide);
+          for (int j = 1; j < 4; ++j) out[r] = scale_add(split2(e[r][j]), ct[j], out[r]);
         }
+#pragma unroll
+        for (int r = 0; r < kRun; ++r) sm.y[buf][t0 + r][th.ln / 2][2 * th.pair + th.ln % 2] = out[r];
       }
     }
-    if (tile + 1 < tile1) put(buf ^ 1);
+    meet_go(kDone + buf);
   }
 
+  if (kSummary) {
+    const size_t at = ((size_t)seg * sh.B + th.b) * sh.D;
+    th.store_kept(A.seg_state + at * sh.kn, s);
+    const float2 f = split2(sum);
+    if (th.ln == 0 && 2 * th.pair < th.nch) A.seg_sum[at + th.channel(0)] = f.x;
+    if (th.ln == 0 && 2 * th.pair + 1 < th.nch) A.seg_sum[at + th.channel(1)] = f.y;
+  } else if (A.s_out && seg == sh.segs - 1) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int ch = th.first_channel() + k;
-    if (ch >= th.nch) continue;
-    const size_t row = (size_t)th.b * sh.D + th.c0 + ch;
-    if (kSummary) {
-      const size_t at = (size_t)seg * sh.B * sh.D + row;
-      if (n0 < sh.n4) store4u(A.seg_state + at * sh.n4 + n0, 4, s[k], true);
-      if (th.ln == 0) A.seg_sum[at] = sum[k];
-    } else if (A.s_out && seg == sh.segs - 1) {
-      store4u(A.s_out + row * sh.N + n0, ns, s[k], A.states16);
-    }
+    for (int j = 0; j < 4; ++j) th.put(A.s_out + (size_t)th.b * sh.D * sh.N, j, sh.N, s[j]);
   }
 }
 
 template <typename T, int LN> int launch_fwd(const FwdArgs& a, cudaStream_t stream) {
-  constexpr size_t bytes = sizeof(FwdSmem<LN>);
-  static_assert(bytes <= 48 * 1024, "no opt-in is made for more");
+  constexpr int bytes = (int)sizeof(FwdSmem<LN>);
+  cudaError_t err = cudaFuncSetAttribute(scan_fwd_kernel<T, LN, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) err = cudaFuncSetAttribute(scan_fwd_kernel<T, LN, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  RFA_REQUIRE(err == cudaSuccess, (int)err, "selective_scan_fwd: %s", cudaGetErrorString(err));
   const dim3 grid(a.sh.per_group * a.sh.G, a.sh.B, a.sh.segs);
   if (a.sh.segs > 1) {
-    scan_fwd_kernel<T, LN, true><<<dim3(grid.x, grid.y, a.sh.segs - 1), kScanThreads, bytes, stream>>>(a);
+    scan_fwd_kernel<T, LN, true><<<dim3(grid.x, grid.y, a.sh.segs - 1), 2 * kScanThreads, bytes, stream>>>(a);
     if (int r = check_launch("selective_scan_fwd (segments)")) return r;
   }
-  scan_fwd_kernel<T, LN, false><<<grid, kScanThreads, bytes, stream>>>(a);
+  scan_fwd_kernel<T, LN, false><<<grid, 2 * kScanThreads, bytes, stream>>>(a);
   return check_launch("selective_scan_fwd");
+}
+
+// n of 4 floats, the rest 0; `wide`: as one 16-byte word
+__device__ __forceinline__ void load4(const float* p, int n, bool wide, float* v) {
+  if (wide && n >= 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
+  }
+}
+__device__ __forceinline__ void store4(float* p, int n, bool wide, const float* v) {
+  if (wide && n >= 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = v[i];
+  }
 }
 
 // ---- one token ---------------------------------------------------------------------------------------------------------------
@@ -264,13 +283,8 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ 
   const bool gone = p.mask && p.mask[b];
   float s[4], a[4];
   float* at = state + item * p.N + n0;
-  if (kWide) {
-    load4f(at, n, s);
-    load4f(p.a + (size_t)ch * p.N + n0, n, a);
-  } else {
-    load4u(at, n, s);
-    load4u(p.a + (size_t)ch * p.N + n0, n, a);
-  }
+  load4(at, n, kWide, s);
+  load4(p.a + (size_t)ch * p.N + n0, n, kWide, a);
   const int g = ch / (p.D / p.G);
   const T* bp = static_cast<const T*>(p.b) + (int64_t)b * p.b_b + (int64_t)g * p.b_g + n0;
   const T* cp = static_cast<const T*>(p.c) + (int64_t)b * p.c_b + (int64_t)g * p.c_g + n0;
@@ -293,7 +307,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ 
 #pragma unroll
   for (int o = LN / 2; o > 0; o >>= 1) out += __shfl_xor_sync(0xffffffffu, out, o);
   if (!there) return;
-  if (!gone) store4u(at, n, s, kWide);
+  if (!gone) store4(at, n, kWide, s);
   if (n0 == 0) y[item] = from_f<T>(gone ? 0.f : p.d ? fmaf(p.d[ch], x, out) : out);
 }
 
@@ -302,7 +316,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ 
 
 extern "C" size_t rfa_selective_scan_checkpoint_bytes(int64_t T, int B, int D, int N) {
   if (T <= 0 || B <= 0 || D <= 0 || N <= 0) return 0;
-  return (size_t)((T + rfa::kScanTile - 1) / rfa::kScanTile) * B * D * ((N + 3) / 4 * 4) * 4;
+  return (size_t)((T + rfa::kScanTile - 1) / rfa::kScanTile) * B * D * (4 * rfa::scan_lanes(N)) * 4;
 }
 
 extern "C" int rfa_selective_scan_fwd(const rfa_scan_t* scan, void* y, float* s_out, float* checkpoints, void* workspace, size_t workspace_bytes,
@@ -318,10 +332,9 @@ extern "C" int rfa_selective_scan_fwd(const rfa_scan_t* scan, void* y, float* s_
   a.p = *scan;
   a.y = y; a.s_out = s_out; a.ckpt = checkpoints;
   a.seg_state = static_cast<float*>(workspace);
-  a.seg_sum = a.seg_state + (size_t)(a.sh.segs - 1) * scan->B * scan->D * a.sh.n4;
+  a.seg_sum = a.seg_state + (size_t)(a.sh.segs - 1) * scan->B * scan->D * a.sh.kn;
   const int size = scan->dtype == RFA_F32 ? 4 : 2;
-  a.wide = wide_ok(scan->x, scan->x_t, scan->x_b, size, 8) && wide_ok(scan->dt, scan->dt_t, scan->dt_b, size, 8) && wide_ok(y, scan->D, a.sh.heads, size, 8);
-  a.states16 = scan->N % 4 == 0;
+  a.wide = wide_ok(scan->x, scan->x_t, scan->x_b, size, 2) && wide_ok(scan->dt, scan->dt_t, scan->dt_b, size, 2) && wide_ok(y, scan->D, a.sh.heads, size, 2);
 #define CALL(T, LN) return launch_fwd<T, LN>(a, as_stream(stream))
   RFA_SCAN_DISPATCH(scan->dtype, scan_lanes(scan->N), CALL);
 #undef CALL
