@@ -1,14 +1,13 @@
 // Shared by the selective scan's forward and backward: the work of a CTA, its tiles in shared memory, how inputs are staged.
 //
-// A state element (channel i, state n) evolves alone, so a thread holds 2 adjacent channels x 4 states in registers and walks the
+// A state element (channel i, state n) evolves alone, so a thread holds 2 (backward: 4) adjacent channels x 4 states in registers and walks the
 // tokens; LN = 2, 4, 8 or 16 neighbouring lanes hold a channel's up to 4 LN states, lane l the states l, LN + l, 2 LN + l, 3 LN + l.  A CTA
-// has 256 / LN channels of one group and one batch row, and a segment of the tokens.  Four of its warps scan; four others bring tiles of
+// has 256 / LN channels of one group and one batch row, and a segment of the tokens.  Some of its warps scan; others bring tiles of
 // inputs and take results away meanwhile, so that a scheduler with few CTAs still has work while one warp waits.
 //
 // Exponentials are what bounds it: 16 a clock and SM come from the special function unit.  The first of a thread's four states -- the first
 // quarter of a channel's -- takes a polynomial on the FMA units instead (`decays`), at which both are busy equally long.  Issue slots come
-// next: arithmetic whose operands stand side by side is packed, both channels in one instruction (`fma.rn.f32x2`); products with
-// b and c, one value for both, are not, as copying those into pairs costs what it saves.
+// next: all arithmetic is packed, both channels in one instruction (`fma.rn.f32x2`; 68 instructions a token and warp, 96 without).
 //
 // Tiles of 16 tokens go through shared memory, two of them by turns: a thread asks for a pair of channels' inputs a tile ahead (a warp's loads are whole 128-byte
 // rows), turns them into delta and delta x and leaves them as one 16-byte word, which the scan's lanes read.  Shared memory hands a
@@ -20,7 +19,7 @@
 
 namespace rfa {
 
-constexpr int kScanThreads = 128, kScanTile = 16;      // threads of either half of a CTA; tokens of a tile, and of a checkpoint
+constexpr int kScanTile = 16;      // tokens of a tile, and of a checkpoint
 
 struct ScanShape {
   int64_t T;
@@ -31,15 +30,11 @@ struct ScanShape {
 // The two halves of a CTA meet at named barriers: a tile is there (kFull + buffer), a tile has been scanned (kDone + buffer).  Every tile
 // passes both once, on each side, in one order: no wait is left over.
 enum { kFull = 1, kDone = 3 };
-__device__ __forceinline__ void meet_wait(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(2 * kScanThreads) : "memory"); }
-__device__ __forceinline__ void meet_go(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(2 * kScanThreads) : "memory"); }
+template <int kThreads> __device__ __forceinline__ void meet_wait(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kThreads) : "memory"); }
+template <int kThreads> __device__ __forceinline__ void meet_go(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kThreads) : "memory"); }
 
 template <int LN> struct ScanTile {
   static constexpr int kChannels = 256 / LN, kN = 4 * LN, kPairs = kChannels / 2;
-  static constexpr int kRows = kScanThreads / kPairs;               // tokens that the CTA loads side by side
-  static constexpr int kPasses = kScanTile / kRows;
-  static constexpr int kBc = kScanTile * kN / kScanThreads;         // elements of b (and of c) per thread and tile
-  static_assert(kPasses >= 1 && kBc >= 1, "a tile is work for every thread");
 };
 
 // ---- two floats in one instruction -------------------------------------------------------------------------------------------
@@ -79,118 +74,135 @@ __device__ __forceinline__ f32x2 exp2_unit(f32x2 u) {
 // |r| <= 1/2, 2^r by a polynomial of degree 5 with 1 + r log 2 in front (least maximum of the relative error, by Lawson's iteration:
 // 1.1e-7, and 2.3e-7 |r| near 0, so that a decay near 1 is as near as its argument is), k added to the exponent.
 //
-// For R tokens, one step at a time: few warps share an SM's scheduler, and a chain alone would wait for itself.
+// R of them side by side: few warps share an SM's scheduler, and a chain alone would wait for itself.
 template <int R> struct Poly {
   f32x2 t[R], r[R], p[R];
-  __device__ __forceinline__ void begin(const f32x2* delta, f32x2 a2) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const float2 v = split2(mul2(delta[i], a2));
-      r[i] = pack2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
-    }
+  __device__ __forceinline__ void begin(int i, f32x2 u) {
+    const float2 v = split2(u);
+    r[i] = pack2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
   }
-  __device__ __forceinline__ void step(int k) {        // 0 ... 7, all in order
+  __device__ __forceinline__ void run() {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (k == 0) t[i] = add2(r[i], both(12582912.f));
-      if (k == 1) p[i] = add2(t[i], both(-12582912.f));
-      if (k == 2) r[i] = fma2(p[i], both(-1.f), r[i]);
-      if (k == 3) p[i] = fma2(both(1.33006054e-3f), r[i], both(9.66969132e-3f));
-      if (k == 4) p[i] = fma2(p[i], r[i], both(5.55055849e-2f));
-      if (k == 5) p[i] = fma2(p[i], r[i], both(2.40222827e-1f));
-      if (k == 6) p[i] = fma2(p[i], r[i], both(kLn2));
-      if (k == 7) p[i] = fma2(p[i], r[i], both(1.f));
-    }
+    for (int i = 0; i < R; ++i) t[i] = add2(r[i], both(12582912.f));
+#pragma unroll
+    for (int i = 0; i < R; ++i) r[i] = fma2(add2(t[i], both(-12582912.f)), both(-1.f), r[i]);
+#pragma unroll
+    for (int i = 0; i < R; ++i) p[i] = fma2(both(1.33006054e-3f), r[i], both(9.66969132e-3f));
+#pragma unroll
+    for (int i = 0; i < R; ++i) p[i] = fma2(p[i], r[i], both(5.55055849e-2f));
+#pragma unroll
+    for (int i = 0; i < R; ++i) p[i] = fma2(p[i], r[i], both(2.40222827e-1f));
+#pragma unroll
+    for (int i = 0; i < R; ++i) p[i] = fma2(p[i], r[i], both(kLn2));
+#pragma unroll
+    for (int i = 0; i < R; ++i) p[i] = fma2(p[i], r[i], both(1.f));
   }
   __device__ __forceinline__ f32x2 end(int i) const {
     const float2 q = split2(p[i]), k = split2(t[i]);
     return pack2(__int_as_float(__float_as_int(q.x) + (__float_as_int(k.x) << 23)), __int_as_float(__float_as_int(q.y) + (__float_as_int(k.y) << 23)));
   }
 };
-// exp(delta a) of both channels for R tokens and the thread's four states, a in units of log 2
-template <int R> __device__ __forceinline__ void decays(const f32x2* delta, const f32x2* a2, f32x2 (*e)[4]) {
-  Poly<R> poly;
-  poly.begin(delta, a2[0]);
+// exp(delta a) for R tokens, P pairs of channels and the thread's four states, a in units of log 2; kPoly: the first one's as above
+template <int R, int P, bool kPoly> __device__ __forceinline__ void decays(const f32x2 (*delta)[P], const f32x2 (*a2)[4], f32x2 (*e)[P][4]) {
+  Poly<R * P> poly;
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 1; j < 4; ++j) e[i][j] = exp2_unit(mul2(delta[i], a2[j]));
+    for (int k = 0; k < P; ++k) {
+      if (kPoly) poly.begin(i * P + k, mul2(delta[i][k], a2[k][0]));
 #pragma unroll
-  for (int k = 0; k < 8; ++k) poly.step(k);
+      for (int j = kPoly; j < 4; ++j) e[i][k][j] = exp2_unit(mul2(delta[i][k], a2[k][j]));
+    }
+  if (!kPoly) return;
+  poly.run();
 #pragma unroll
-  for (int i = 0; i < R; ++i) e[i][0] = poly.end(i);
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int k = 0; k < P; ++k) e[i][k][0] = poly.end(i * P + k);
 }
 
 // ---- the work of a thread ----------------------------------------------------------------------------------------------------
-template <int LN> struct ScanThread {
+// Of kScan threads that scan, P pairs of adjacent channels each, and kBring that bring and take, one pair each.
+template <int LN, int kScan, int kBring, int P = 1> struct ScanThread {
+  using Tile = ScanTile<LN>;
+  static constexpr int kRows = kBring / Tile::kPairs;            // tokens that are brought side by side
+  static constexpr int kPasses = kScanTile / kRows;
+  static constexpr int kStep = kBring / Tile::kN;                // tokens whose b (and c) are
+  static constexpr int kBc = kScanTile / kStep;
+  static_assert(kScan * P == LN * Tile::kPairs && kPasses >= 1 && kStep >= 1, "work for every thread");
   int group, c0, nch, b;          // the CTA's group, first channel, channels (<= kChannels), batch row
   bool scans;                     // or brings and takes
-  int tid, ln, pair;              // in the scan: lane of the channel, pair of channels in the CTA
+  int tid, ln, pair;              // of its kind; in the scan: lane of the channels, first pair in the CTA
   int vpair, row, vn;             // when it brings: pair of channels, first token, how many of the two channels there are
   __device__ ScanThread(const ScanShape& s) {
-    using Tile = ScanTile<LN>;
     group = blockIdx.x / s.per_group;
     const int in_group = (blockIdx.x % s.per_group) * Tile::kChannels;
     c0 = group * s.heads + in_group;
     nch = min(Tile::kChannels, s.heads - in_group);
     b = blockIdx.y;
-    scans = threadIdx.x < kScanThreads;
-    tid = threadIdx.x % kScanThreads;
+    scans = threadIdx.x < kScan;
+    tid = scans ? threadIdx.x : threadIdx.x - kScan;
     ln = tid % LN;
-    pair = tid / LN;
+    pair = tid / LN * P;
     vpair = tid % Tile::kPairs;
     row = tid / Tile::kPairs;
     vn = max(0, min(2, nch - 2 * vpair));
   }
-  // n of the thread's state j, and whether channel k of its pair has it
+  // n of the thread's state j; channel h of its pair k, and whether it is there
   __device__ __forceinline__ int state(int j) const { return j * LN + ln; }
-  __device__ __forceinline__ bool has(int k, int j, int N) const { return 2 * pair + k < nch && state(j) < N; }
-  __device__ __forceinline__ int channel(int k) const { return c0 + 2 * pair + k; }
+  __device__ __forceinline__ int channel(int k, int h) const { return c0 + 2 * (pair + k) + h; }
+  __device__ __forceinline__ bool has(int k, int h) const { return 2 * (pair + k) + h < nch; }
   // rows [D][N] of fp32 at p, both channels' state j; 0 where there is none
-  __device__ __forceinline__ f32x2 get(const float* p, int j, int N) const {
-    float v[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) v[k] = has(k, j, N) ? p[(size_t)channel(k) * N + state(j)] : 0.f;
-    return pack2(v[0], v[1]);
+  __device__ __forceinline__ f32x2 get(const float* p, int k, int j, int N) const {
+    const bool n = state(j) < N;
+    return pack2(n && has(k, 0) ? p[(size_t)channel(k, 0) * N + state(j)] : 0.f, n && has(k, 1) ? p[(size_t)channel(k, 1) * N + state(j)] : 0.f);
   }
-  __device__ __forceinline__ void put(float* p, int j, int N, f32x2 v) const {
+  __device__ __forceinline__ void put(float* p, int k, int j, int N, f32x2 v) const {
     const float2 f = split2(v);
-    if (has(0, j, N)) p[(size_t)channel(0) * N + state(j)] = f.x;
-    if (has(1, j, N)) p[(size_t)channel(1) * N + state(j)] = f.y;
+    if (state(j) < N && has(k, 0)) p[(size_t)channel(k, 0) * N + state(j)] = f.x;
+    if (state(j) < N && has(k, 1)) p[(size_t)channel(k, 1) * N + state(j)] = f.y;
+  }
+  __device__ __forceinline__ f32x2 get1(const float* p, int k) const {      // [D]
+    return pack2(has(k, 0) ? p[channel(k, 0)] : 0.f, has(k, 1) ? p[channel(k, 1)] : 0.f);
+  }
+  __device__ __forceinline__ void put1(float* p, int k, f32x2 v) const {
+    const float2 f = split2(v);
+    if (ln == 0 && has(k, 0)) p[channel(k, 0)] = f.x;
+    if (ln == 0 && has(k, 1)) p[channel(k, 1)] = f.y;
   }
   // kept rows [D][kN], a lane's four states adjacent
-  __device__ __forceinline__ void load_kept(const float* p, f32x2* v) const {
+  __device__ __forceinline__ void load_kept(const float* p, int k, f32x2* v) const {
     float4 f[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      f[k] = 2 * pair + k < nch ? *reinterpret_cast<const float4*>(p + (size_t)channel(k) * (4 * LN) + 4 * ln) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int h = 0; h < 2; ++h)
+      f[h] = has(k, h) ? *reinterpret_cast<const float4*>(p + (size_t)channel(k, h) * Tile::kN + 4 * ln) : make_float4(0.f, 0.f, 0.f, 0.f);
     v[0] = pack2(f[0].x, f[1].x); v[1] = pack2(f[0].y, f[1].y); v[2] = pack2(f[0].z, f[1].z); v[3] = pack2(f[0].w, f[1].w);
   }
-  __device__ __forceinline__ void store_kept(float* p, const f32x2* v) const {
+  __device__ __forceinline__ void store_kept(float* p, int k, const f32x2* v) const {
     const float2 a = split2(v[0]), b = split2(v[1]), c = split2(v[2]), d = split2(v[3]);
-    if (2 * pair < nch) *reinterpret_cast<float4*>(p + (size_t)channel(0) * (4 * LN) + 4 * ln) = make_float4(a.x, b.x, c.x, d.x);
-    if (2 * pair + 1 < nch) *reinterpret_cast<float4*>(p + (size_t)channel(1) * (4 * LN) + 4 * ln) = make_float4(a.y, b.y, c.y, d.y);
+    if (has(k, 0)) *reinterpret_cast<float4*>(p + (size_t)channel(k, 0) * Tile::kN + 4 * ln) = make_float4(a.x, b.x, c.x, d.x);
+    if (has(k, 1)) *reinterpret_cast<float4*>(p + (size_t)channel(k, 1) * Tile::kN + 4 * ln) = make_float4(a.y, b.y, c.y, d.y);
+  }
+  // Which of a bringing thread's tokens of a tile are there: bit i of pass i.  A plain tile is full, of a full CTA, without a mask and in wide
+  // words: nothing is asked about its elements (the questions were a quarter of the forward's instructions).
+  __device__ __forceinline__ uint32_t tokens_here(const uint8_t* mask, int64_t t0, int64_t T) const {
+    uint32_t here = 0;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int64_t t = t0 + row + i * kRows;
+      if (t < T && !(mask && mask[t])) here |= 1u << i;
+    }
+    return here;
   }
 };
 
-// Which of a thread's tokens of a tile are there: bit i of pass i.  A plain tile is full, of a full CTA, without a mask and in wide words:
-// nothing is asked about its elements (the questions were a quarter of the forward's instructions).
-template <int LN> __device__ __forceinline__ uint32_t tokens_here(const ScanThread<LN>& th, const uint8_t* mask, int64_t t0, int64_t T) {
-  uint32_t here = 0;
-#pragma unroll
-  for (int i = 0; i < ScanTile<LN>::kPasses; ++i) {
-    const int64_t t = t0 + th.row + i * ScanTile<LN>::kRows;
-    if (t < T && !(mask && mask[t])) here |= 1u << i;
-  }
-  return here;
-}
-// Both channels of a thread's tokens, as they stand in memory; p: at the thread's first token of the tile.
-template <typename T, int LN> struct RawPairs {
-  Raw<T, 2> v[ScanTile<LN>::kPasses];
+// Both channels of a bringing thread's tokens, as they stand in memory; p: at the thread's first token of the tile.
+template <typename T, class Thread> struct RawPairs {
+  Raw<T, 2> v[Thread::kPasses];
   template <bool kPlain> __device__ __forceinline__ void load(const T* p, int64_t stride, uint32_t here, int vn, bool wide) {
 #pragma unroll
-    for (int i = 0; i < ScanTile<LN>::kPasses; ++i) {
-      const T* at = p + i * ScanTile<LN>::kRows * stride;
+    for (int i = 0; i < Thread::kPasses; ++i) {
+      const T* at = p + i * Thread::kRows * stride;
       if (kPlain) {
         v[i].load(at, 2, true);
       } else {
@@ -200,24 +212,23 @@ template <typename T, int LN> struct RawPairs {
     }
   }
 };
-// One tile's b or c, as they stand in memory, n = thread % kN of tokens thread / kN + i * 128 / kN; in shared memory a lane's four states are
-// adjacent.
-template <typename T, int LN> struct RawStates {
-  static constexpr int kN = ScanTile<LN>::kN, kStep = kScanThreads / kN;
-  T v[ScanTile<LN>::kBc];
-  template <bool kPlain> __device__ __forceinline__ void load(const T* p, int64_t stride, int64_t t0, int64_t T_, int N, const uint8_t* mask) {
-    const int tid = threadIdx.x % kScanThreads, n = tid % kN;
-    const T* at = p + (t0 + tid / kN) * stride + n;
+// One tile's b or c, as they stand in memory, n = tid % kN of tokens tid / kN + i * kStep; in shared memory a lane's four states are adjacent.
+template <typename T, int LN, class Thread> struct RawStates {
+  static constexpr int kN = ScanTile<LN>::kN, kStep = Thread::kStep;
+  T v[Thread::kBc];
+  template <bool kPlain> __device__ __forceinline__ void load(const Thread& th, const T* p, int64_t stride, int64_t t0, int64_t T_, int N, const uint8_t* mask) {
+    const int n = th.tid % kN;
+    const T* at = p + (t0 + th.tid / kN) * stride + n;
 #pragma unroll
-    for (int i = 0; i < ScanTile<LN>::kBc; ++i) {
-      const int64_t t = t0 + tid / kN + i * kStep;
+    for (int i = 0; i < Thread::kBc; ++i) {
+      const int64_t t = t0 + th.tid / kN + i * kStep;
       v[i] = kPlain || (t < T_ && n < N && !(mask && mask[t])) ? at[i * kStep * stride] : from_f<T>(0.f);
     }
   }
-  __device__ __forceinline__ void store(float (*smem)[kN]) const {
-    const int tid = threadIdx.x % kScanThreads, n = tid % kN, t = tid / kN;
+  __device__ __forceinline__ void store(const Thread& th, float (*smem)[kN]) const {
+    const int n = th.tid % kN, t = th.tid / kN;
 #pragma unroll
-    for (int i = 0; i < ScanTile<LN>::kBc; ++i) smem[t + i * kStep][(n % LN) * 4 + n / LN] = to_f(v[i]);
+    for (int i = 0; i < Thread::kBc; ++i) smem[t + i * kStep][(n % LN) * 4 + n / LN] = to_f(v[i]);
   }
 };
 struct Plain { static constexpr bool value = true; };
@@ -243,13 +254,6 @@ __device__ __forceinline__ void lane_states(const float* row, int ln, float* v) 
   const float4 f = *reinterpret_cast<const float4*>(row + 4 * ln);
   v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
 }
-// both channels' products with one factor, and sums of such
-__device__ __forceinline__ f32x2 scale(float2 v, float f) { return pack2(v.x * f, v.y * f); }
-__device__ __forceinline__ f32x2 scale_add(float2 v, float f, f32x2 c) {
-  const float2 d = split2(c);
-  return pack2(fmaf(v.x, f, d.x), fmaf(v.y, f, d.y));
-}
-
 // Sums `K` values over LN lanes, dealing the results out: afterwards v[0 .. max(1, K / LN)) of lane l are the totals of values
 // l * K / LN ... (K >= LN), or of value l * K / LN in every lane (K < LN).  K / 2 + K / 4 + ... exchanges instead of K log LN.
 template <int K, int LN, int W = LN> __device__ __forceinline__ void lanes_sum(float* v, int ln) {

@@ -7,13 +7,18 @@
 // Few rows (a prompt of one sequence) leave SMs idle: the tokens are then cut into segments.  A first kernel leaves each segment's own state
 // from zero and the sum of its deltas -- over which a whole segment's decay is exp(a sum delta), one exponential -- and the main kernel's
 // CTAs begin with the states of the segments before theirs joined up, which costs the first kernel's pass over dt, x and b once more.
-#include <stdlib.h>
 #include "scan.cuh"
 
 namespace rfa {
 
 int scan_lanes(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
+// Two CTAs run side by side on an SM, 296 in all; one alone takes 0.63 of the time of two (forward, 0.66 backward).  A segment more costs the
+// forward about half of its pass again, the backward an eighth.  us at T = 2048 (N = 16, bf16), one segment / several:
+//   forward   16 CTAs 137 / 37, 64 CTAs 138 / 101 with about 592 in all; 128 CTAs 147 / 183, 160 CTAs 233 / 233, 256 CTAs 233 / 321
+//   backward  the same below 120; above, whatever fills the last round: 160 CTAs 855 / 603 in six, 320 CTAs (T = 1024) 686 / 588 in three,
+//             256 CTAs 877 / 906 in four, so one
+// Segments of less than six tiles lose to their own ends (16 CTAs, T = 2048: 19 segments 37 us, 32 segments 42).
 ScanShape scan_shape(int64_t T, int B, int D, int N, int G, bool backward) {
   ScanShape s{};
   const int channels = 256 / scan_lanes(N);
@@ -22,9 +27,19 @@ ScanShape scan_shape(int64_t T, int B, int D, int N, int G, bool backward) {
   s.per_group = (s.heads + channels - 1) / channels;
   s.tiles = (int)((T + kScanTile - 1) / kScanTile);
   s.kn = 4 * scan_lanes(N);
-  const int64_t ctas = (int64_t)s.per_group * G * B, want = getenv("SW") ? atoi(getenv("SW")) : 148 * (backward ? 2 : 4);
-  int64_t segs = ctas >= want ? 1 : (want + ctas - 1) / ctas;
-  segs = segs < s.tiles / 4 ? segs : s.tiles / 4;
+  const int64_t ctas = (int64_t)s.per_group * G * B;
+  int64_t segs = 1;
+  if (ctas < 120) {
+    segs = (592 + ctas - 1) / ctas;
+  } else if (backward) {
+    double best = 1e30;
+    for (int n = 1; n <= 6; ++n) {
+      const int64_t last = ctas * n % 296;
+      const double cost = (ctas * n / 296 + (last == 0 ? 0. : last <= 148 ? 0.66 : 1.) + 0.12 * (n - 1)) / n;
+      if (cost < 0.97 * best) { best = cost; segs = n; }
+    }
+  }
+  segs = segs < s.tiles / 6 ? segs : s.tiles / 6;
   if (segs < 1) segs = 1;
   s.seg_tiles = (int)((s.tiles + segs - 1) / segs);
   s.segs = (s.tiles + s.seg_tiles - 1) / s.seg_tiles;
@@ -53,6 +68,9 @@ template <int LN> struct __align__(16) FwdSmem {
   f32x2 y[2][kScanTile][LN / 2][kRow];                 // c . s, each lane's share; two lanes' side by side
 };
 
+constexpr int kFwdScan = 128, kFwdBring = 128, kFwdThreads = kFwdScan + kFwdBring;
+template <int LN> using FwdThread = ScanThread<LN, kFwdScan, kFwdBring>;
+
 struct FwdArgs {
   ScanShape sh;
   rfa_scan_t p;
@@ -63,7 +81,7 @@ struct FwdArgs {
 
 // Brings the tiles of a segment and takes their outputs away.  kSummary: no c, no y.
 template <typename T, int LN, bool kSummary>
-__device__ __forceinline__ void fwd_bring(const FwdArgs& A, FwdSmem<LN>& sm, const ScanThread<LN>& th, int tile0, int tile1) {
+__device__ __forceinline__ void fwd_bring(const FwdArgs& A, FwdSmem<LN>& sm, const FwdThread<LN>& th, int tile0, int tile1) {
   using Tile = ScanTile<LN>;
   const ScanShape& sh = A.sh;
   const rfa_scan_t& p = A.p;
@@ -81,38 +99,39 @@ __device__ __forceinline__ void fwd_bring(const FwdArgs& A, FwdSmem<LN>& sm, con
     bias[k] = p.dt_bias && k < th.vn ? p.dt_bias[ch + k] : 0.f;
     skip[k] = !kSummary && p.d && k < th.vn ? p.d[ch + k] : 0.f;
   }
-  RawPairs<T, LN> rx, rd, kept;
-  RawStates<T, LN> rb, rc;
+  using Thread = FwdThread<LN>;
+  RawPairs<T, Thread> rx, rd, kept;
+  RawStates<T, LN, Thread> rb, rc;
   uint32_t here = 0, next = 0;                         // which of this thread's tokens are there: in the tile that is scanned, in the next one
   const int plain = A.wide && !mask && th.nch == Tile::kChannels && sh.N == Tile::kN ? (int)(sh.T / kScanTile) : 0;      // tiles in front of it are
   const auto ask = [&](int tile, auto kind) {
     constexpr bool kPlain = decltype(kind)::value;
     const int64_t t0 = (int64_t)tile * kScanTile, t = t0 + th.row;
-    next = kPlain ? ~0u : tokens_here<LN>(th, mask, t0, sh.T);
+    next = kPlain ? ~0u : th.tokens_here(mask, t0, sh.T);
     rx.template load<kPlain>(x + t * p.x_t, p.x_t, next, th.vn, A.wide);
     rd.template load<kPlain>(dt + t * p.dt_t, p.dt_t, next, th.vn, A.wide);
-    rb.template load<kPlain>(bp, p.b_t, t0, sh.T, sh.N, mask);
-    if (!kSummary) rc.template load<kPlain>(cp, p.c_t, t0, sh.T, sh.N, mask);
+    rb.template load<kPlain>(th, bp, p.b_t, t0, sh.T, sh.N, mask);
+    if (!kSummary) rc.template load<kPlain>(th, cp, p.c_t, t0, sh.T, sh.N, mask);
   };
   const auto ask_tile = [&](int tile) { tile < plain ? ask(tile, Plain()) : ask(tile, Ragged()); };
   const auto put = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < Tile::kPasses; ++i) {
+    for (int i = 0; i < Thread::kPasses; ++i) {
       float2 sig;
       const float2 v = make_float2(rd.v[i].get(0) + bias[0], rd.v[i].get(1) + bias[1]);
       const f32x2 delta = p.softplus ? softplus2<false>(v, sig) : pack2(v.x, v.y);
       const f32x2 dx = mul2(delta, pack2(rx.v[i].get(0), rx.v[i].get(1)));
       const bool on = next >> i & 1;
-      *reinterpret_cast<ulonglong2*>(&sm.in[buf][th.row + i * Tile::kRows][th.vpair]) = make_ulonglong2(on ? delta : 0, on ? dx : 0);
+      *reinterpret_cast<ulonglong2*>(&sm.in[buf][th.row + i * Thread::kRows][th.vpair]) = make_ulonglong2(on ? delta : 0, on ? dx : 0);
     }
-    rb.store(sm.b[buf]);
-    if (!kSummary) rc.store(sm.c[buf]);
+    rb.store(th, sm.b[buf]);
+    if (!kSummary) rc.store(th, sm.c[buf]);
   };
   const auto take = [&](int tile, int buf) {
     const int64_t t0 = (int64_t)tile * kScanTile;
 #pragma unroll
-    for (int i = 0; i < Tile::kPasses; ++i) {
-      const int t = th.row + i * Tile::kRows;
+    for (int i = 0; i < Thread::kPasses; ++i) {
+      const int t = th.row + i * Thread::kRows;
       if (t0 + t >= sh.T) continue;
       f32x2 v[LN];
 #pragma unroll
@@ -138,103 +157,100 @@ __device__ __forceinline__ void fwd_bring(const FwdArgs& A, FwdSmem<LN>& sm, con
   for (int tile = tile0; tile < tile1; ++tile) {
     const int buf = (tile - tile0) & 1;
     put(buf);
-    meet_go(kFull + buf);
-    RawPairs<T, LN> x_now = rx;
+    meet_go<kFwdThreads>(kFull + buf);
+    RawPairs<T, Thread> x_now = rx;
     const uint32_t here_now = next;
     if (tile + 1 < tile1) ask_tile(tile + 1);
     if (tile > tile0) {                                // the other buffer's tile
-      meet_wait(kDone + (buf ^ 1));
+      meet_wait<kFwdThreads>(kDone + (buf ^ 1));
       if (!kSummary) take(tile - 1, buf ^ 1);
     }
     kept = x_now;
     here = here_now;
   }
   const int last = (tile1 - 1 - tile0) & 1;
-  meet_wait(kDone + last);
+  meet_wait<kFwdThreads>(kDone + last);
   if (!kSummary) take(tile1 - 1, last);
 }
 
 // kSummary: the state a segment reaches from zero, and its sum of deltas.
 template <typename T, int LN, bool kSummary>
-__global__ void __launch_bounds__(2 * kScanThreads, 2) scan_fwd_kernel(const __grid_constant__ FwdArgs A) {
+__global__ void __launch_bounds__(kFwdThreads, 2) scan_fwd_kernel(const __grid_constant__ FwdArgs A) {
   using Tile = ScanTile<LN>;
   extern __shared__ char smem_raw[];
   FwdSmem<LN>& sm = *reinterpret_cast<FwdSmem<LN>*>(smem_raw);
   const ScanShape& sh = A.sh;
   const rfa_scan_t& p = A.p;
-  const ScanThread<LN> th(sh);
+  const FwdThread<LN> th(sh);
   const int seg = blockIdx.z, tile0 = seg * sh.seg_tiles, tile1 = min(tile0 + sh.seg_tiles, sh.tiles);
   if (!th.scans) {
     fwd_bring<T, LN, kSummary>(A, sm, th, tile0, tile1);
     return;
   }
 
-  f32x2 a2[4], s[4], sum = both(0.f);                  // a in units of log 2
+  f32x2 a2[1][4], s[4], sum = both(0.f);                  // a in units of log 2
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    a2[j] = mul2(th.get(p.a, j, sh.N), both(kLog2e));
-    s[j] = !kSummary && p.s_in ? th.get(p.s_in + (size_t)th.b * sh.D * sh.N, j, sh.N) : both(0.f);
+    a2[0][j] = mul2(th.get(p.a, 0, j, sh.N), both(kLog2e));
+    s[j] = !kSummary && p.s_in ? th.get(p.s_in + (size_t)th.b * sh.D * sh.N, 0, j, sh.N) : both(0.f);
   }
   if (!kSummary)
     for (int i = 0; i < seg; ++i) {                    // the segments before this one
       const size_t at = ((size_t)i * sh.B + th.b) * sh.D;
       f32x2 v[4];
-      th.load_kept(A.seg_state + at * sh.kn, v);
-      const float* total = A.seg_sum + at + th.channel(0);
-      const f32x2 over = pack2(2 * th.pair < th.nch ? total[0] : 0.f, 2 * th.pair + 1 < th.nch ? total[1] : 0.f);
+      th.load_kept(A.seg_state + at * sh.kn, 0, v);
+      const f32x2 over = th.get1(A.seg_sum + at, 0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] = fma2(exp2_unit(mul2(over, a2[j])), s[j], v[j]);
+      for (int j = 0; j < 4; ++j) s[j] = fma2(exp2_unit(mul2(over, a2[0][j])), s[j], v[j]);
     }
   for (int tile = tile0; tile < tile1; ++tile) {
     const int buf = (tile - tile0) & 1;
-    if (!kSummary && A.ckpt) th.store_kept(A.ckpt + ((size_t)th.b * sh.tiles + tile) * sh.D * sh.kn, s);
-    meet_wait(kFull + buf);
+    if (!kSummary && A.ckpt) th.store_kept(A.ckpt + ((size_t)th.b * sh.tiles + tile) * sh.D * sh.kn, 0, s);
+    meet_wait<kFwdThreads>(kFull + buf);
     constexpr int kRun = 4;                            // tokens whose decays are formed side by side
 #pragma unroll
     for (int t0 = 0; t0 < kScanTile; t0 += kRun) {
-      f32x2 delta[kRun], dx[kRun], e[kRun][4];
+      f32x2 delta[kRun][1], dx[kRun], e[kRun][1][4];
 #pragma unroll
       for (int r = 0; r < kRun; ++r) {
         const ulonglong2 in = *reinterpret_cast<const ulonglong2*>(&sm.in[buf][t0 + r][th.pair]);
-        delta[r] = in.x;
+        delta[r][0] = in.x;
         dx[r] = in.y;
       }
-      decays<kRun>(delta, a2, e);
+      decays<kRun, 1, true>(delta, a2, e);
 #pragma unroll
       for (int r = 0; r < kRun; ++r) {
         float bt[4];
         lane_states(sm.b[buf][t0 + r], th.ln, bt);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[r][j] = s[j] = fma2(e[r][j], s[j], scale(split2(dx[r]), bt[j]));
+        for (int j = 0; j < 4; ++j) e[r][0][j] = s[j] = fma2(e[r][0][j], s[j], mul2(dx[r], both(bt[j])));
       }
       if constexpr (kSummary) {
-        sum = add2(sum, add2(add2(delta[0], delta[1]), add2(delta[2], delta[3])));
+        sum = add2(sum, add2(add2(delta[0][0], delta[1][0]), add2(delta[2][0], delta[3][0])));
       } else {
         f32x2 out[kRun];
 #pragma unroll
         for (int r = 0; r < kRun; ++r) {
           float ct[4];
           lane_states(sm.c[buf][t0 + r], th.ln, ct);
-          out[r] = scale(split2(e[r][0]), ct[0]);
+          out[r] = mul2(e[r][0][0], both(ct[0]));
 #pragma unroll
-          for (int j = 1; j < 4; ++j) out[r] = scale_add(split2(e[r][j]), ct[j], out[r]);
+          for (int j = 1; j < 4; ++j) out[r] = fma2(e[r][0][j], both(ct[j]), out[r]);
         }
 #pragma unroll
         for (int r = 0; r < kRun; ++r) sm.y[buf][t0 + r][th.ln / 2][2 * th.pair + th.ln % 2] = out[r];
       }
     }
-    meet_go(kDone + buf);
+    meet_go<kFwdThreads>(kDone + buf);
   }
 
   if (kSummary) {
     const size_t at = ((size_t)seg * sh.B + th.b) * sh.D;
-    th.store_kept(A.seg_state + at * sh.kn, s);
-    const float2 f = split2(sum);
-    if (th.ln == 0 && 2 * th.pair < th.nch) A.seg_sum[at + th.channel(0)] = f.x;
-    if (th.ln == 0 && 2 * th.pair + 1 < th.nch) A.seg_sum[at + th.channel(1)] = f.y;
+    th.store_kept(A.seg_state + at * sh.kn, 0, s);
+    th.put1(A.seg_sum + at, 0, sum);
   } else if (A.s_out && seg == sh.segs - 1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) th.put(A.s_out + (size_t)th.b * sh.D * sh.N, j, sh.N, s[j]);
+    for (int j = 0; j < 4; ++j) th.put(A.s_out + (size_t)th.b * sh.D * sh.N, 0, j, sh.N, s[j]);
   }
 }
 
@@ -245,10 +261,10 @@ template <typename T, int LN> int launch_fwd(const FwdArgs& a, cudaStream_t stre
   RFA_REQUIRE(err == cudaSuccess, (int)err, "selective_scan_fwd: %s", cudaGetErrorString(err));
   const dim3 grid(a.sh.per_group * a.sh.G, a.sh.B, a.sh.segs);
   if (a.sh.segs > 1) {
-    scan_fwd_kernel<T, LN, true><<<dim3(grid.x, grid.y, a.sh.segs - 1), 2 * kScanThreads, bytes, stream>>>(a);
+    scan_fwd_kernel<T, LN, true><<<dim3(grid.x, grid.y, a.sh.segs - 1), kFwdThreads, bytes, stream>>>(a);
     if (int r = check_launch("selective_scan_fwd (segments)")) return r;
   }
-  scan_fwd_kernel<T, LN, false><<<grid, 2 * kScanThreads, bytes, stream>>>(a);
+  scan_fwd_kernel<T, LN, false><<<grid, kFwdThreads, bytes, stream>>>(a);
   return check_launch("selective_scan_fwd");
 }
 

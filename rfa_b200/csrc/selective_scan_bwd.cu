@@ -16,18 +16,26 @@
 namespace rfa {
 namespace {
 
-constexpr int kRun = 4;      // tokens whose decays and decayed states are in registers at a time
+constexpr int kRun = 2;       // tokens whose decays and states are in registers at a time
+constexpr int kPart = 4;      // tokens after which the scanning warps hand their partial sums over
+
+constexpr int kP = 1;         // pairs of channels of a scanning thread
+constexpr int kBwdScan = 128 / kP, kBwdBring = 128, kBwdThreads = kBwdScan + kBwdBring;
+template <int LN> using BwdThread = ScanThread<LN, kBwdScan, kBwdBring, kP>;
 
 template <int LN> struct __align__(16) BwdSmem {
   using Tile = ScanTile<LN>;
-  static constexpr int kParts = 4 * (32 / LN);         // pairs of channels in a CTA: partial sums over channels
-  float4 in[kScanTile][Tile::kPairs];                  // delta, delta', delta x, delta' x' of two adjacent channels
-  float4 up[kScanTile][Tile::kPairs];                  // g, g', and softplus' of both
+  static constexpr int kThreads = Tile::kPairs / kP;     // that share a lane's states
+  float4 in[2][kScanTile][Tile::kPairs];               // delta, delta', delta x, delta' x' of two adjacent channels
+  float2 g[2][kScanTile][Tile::kPairs], slope[2][kScanTile][Tile::kPairs];      // g and softplus' of both
+  float b[2][kScanTile][Tile::kN], c[2][kScanTile][Tile::kN];
   float4 res[kScanTile][Tile::kPairs];                 // sum_n G b of both channels, sum_n a log2(e) p of both
-  float b[kScanTile][Tile::kN], c[kScanTile][Tile::kN];
-  ulonglong2 start[kScanTile / kRun][2][kScanThreads]; // each thread's states in front of a part of the tile
-  float4 part[kScanTile][2][kParts][LN];               // gb and gc of each pair's channels, a lane's four states adjacent
+  ulonglong2 start[kScanTile / kRun][2 * kP][kBwdScan];     // each thread's states in front of a run
+  float4 over_ch[2][kPart][2][kThreads][LN];           // gb and gc of each thread's channels, a lane's four states adjacent; two parts by turns
 };
+// Further places where the halves of a CTA meet: a part's sums are there, have been taken.
+enum { kSums = 5, kTaken = 7 };
+
 template <int LN> struct __align__(16) SummarySmem {
   using Tile = ScanTile<LN>;
   float4 in[kScanTile][Tile::kPairs];                  // delta, delta', g, g'
@@ -46,19 +54,21 @@ struct BwdArgs {
   bool wide;
 };
 
+constexpr int kSummaryThreads = 128;
 // The gradient that the tokens of a segment alone hand to the state in front of it, and the segment's sum of deltas.
 template <typename T, int LN>
-__global__ void __launch_bounds__(kScanThreads) scan_bwd_summary_kernel(const __grid_constant__ BwdArgs A) {
+__global__ void __launch_bounds__(kSummaryThreads) scan_bwd_summary_kernel(const __grid_constant__ BwdArgs A) {
   using Tile = ScanTile<LN>;
+  using Thread = ScanThread<LN, kSummaryThreads, kSummaryThreads>;      // each does both
   __shared__ SummarySmem<LN> sm;
   const ScanShape& sh = A.sh;
   const rfa_scan_t& p = A.p;
-  const ScanThread<LN> th(sh);
+  const Thread th(sh);
   const int seg = blockIdx.z + 1, tile0 = seg * sh.seg_tiles, tile1 = min(tile0 + sh.seg_tiles, sh.tiles);
-  f32x2 a2[4], G[4], sum = both(0.f);
+  f32x2 a2[1][4], G[4], sum = both(0.f);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    a2[j] = mul2(th.get(p.a, j, sh.N), both(kLog2e));
+    a2[0][j] = mul2(th.get(p.a, 0, j, sh.N), both(kLog2e));
     G[j] = both(0.f);
   }
   const int ch = th.c0 + 2 * th.vpair;
@@ -71,91 +81,69 @@ __global__ void __launch_bounds__(kScanThreads) scan_bwd_summary_kernel(const __
 #pragma unroll
   for (int k = 0; k < 2; ++k) bias[k] = p.dt_bias && k < th.vn ? p.dt_bias[ch + k] : 0.f;
 
-  RawPairs<T, LN> rd, rg;
-  RawStates<T, LN> rc;
+  RawPairs<T, Thread> rd, rg;
+  RawStates<T, LN, Thread> rc;
   uint32_t next = 0;
   const int plain = A.wide && !mask && th.nch == Tile::kChannels && sh.N == Tile::kN ? (int)(sh.T / kScanTile) : 0;      // tiles in front of it are
   const auto ask = [&](int tile, auto kind) {
     constexpr bool kPlain = decltype(kind)::value;
     const int64_t t0 = (int64_t)tile * kScanTile, t = t0 + th.row;
-    next = kPlain ? ~0u : tokens_here<LN>(th, mask, t0, sh.T);
+    next = kPlain ? ~0u : th.tokens_here(mask, t0, sh.T);
     rd.template load<kPlain>(dt + t * p.dt_t, p.dt_t, next, th.vn, A.wide);
     rg.template load<kPlain>(g + t * row_stride, row_stride, next, th.vn, A.wide);
-    rc.template load<kPlain>(cp, p.c_t, t0, sh.T, sh.N, mask);
+    rc.template load<kPlain>(th, cp, p.c_t, t0, sh.T, sh.N, mask);
   };
   const auto ask_tile = [&](int tile) { tile < plain ? ask(tile, Plain()) : ask(tile, Ragged()); };
   const auto put = [&]() {
 #pragma unroll
-    for (int i = 0; i < Tile::kPasses; ++i) {
+    for (int i = 0; i < Thread::kPasses; ++i) {
       float2 sig;
       const float2 v = make_float2(rd.v[i].get(0) + bias[0], rd.v[i].get(1) + bias[1]);
       const f32x2 delta = p.softplus ? softplus2<false>(v, sig) : pack2(v.x, v.y);
       const bool on = next >> i & 1;
-      *reinterpret_cast<ulonglong2*>(&sm.in[th.row + i * Tile::kRows][th.vpair]) = make_ulonglong2(on ? delta : 0, pack2(rg.v[i].get(0), rg.v[i].get(1)));
+      *reinterpret_cast<ulonglong2*>(&sm.in[th.row + i * Thread::kRows][th.vpair]) = make_ulonglong2(on ? delta : 0, pack2(rg.v[i].get(0), rg.v[i].get(1)));
     }
-    rc.store(sm.c);
+    rc.store(th, sm.c);
   };
   ask_tile(tile1 - 1);
   for (int tile = tile1 - 1; tile >= tile0; --tile) {
     put();
     __syncthreads();
     if (tile > tile0) ask_tile(tile - 1);
+    constexpr int kLook = 4;                           // tokens whose decays are formed side by side
 #pragma unroll
-    for (int t0 = kScanTile - kRun; t0 >= 0; t0 -= kRun) {
-      f32x2 delta[kRun], gt[kRun], e[kRun][4];
+    for (int t0 = kScanTile - kLook; t0 >= 0; t0 -= kLook) {
+      f32x2 delta[kLook][1], gt[kLook], e[kLook][1][4];
 #pragma unroll
-      for (int r = 0; r < kRun; ++r) {
+      for (int r = 0; r < kLook; ++r) {
         const ulonglong2 in = *reinterpret_cast<const ulonglong2*>(&sm.in[t0 + r][th.pair]);
-        delta[r] = in.x;
+        delta[r][0] = in.x;
         gt[r] = in.y;
       }
-      decays<kRun>(delta, a2, e);
+      decays<kLook, 1, true>(delta, a2, e);
 #pragma unroll
-      for (int r = kRun - 1; r >= 0; --r) {
+      for (int r = kLook - 1; r >= 0; --r) {
         float ct[4];
         lane_states(sm.c[t0 + r], th.ln, ct);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) G[j] = mul2(scale_add(split2(gt[r]), ct[j], G[j]), e[r][j]);
-        sum = add2(sum, delta[r]);
+        for (int j = 0; j < 4; ++j) G[j] = mul2(fma2(gt[r], both(ct[j]), G[j]), e[r][0][j]);
+        sum = add2(sum, delta[r][0]);
       }
     }
     __syncthreads();
   }
   const size_t at = ((size_t)(seg - 1) * sh.B + th.b) * sh.D;
-  th.store_kept(A.seg_grad + at * sh.kn, G);
-  const float2 f = split2(sum);
-  if (th.ln == 0 && 2 * th.pair < th.nch) A.seg_sum[at + th.channel(0)] = f.x;
-  if (th.ln == 0 && 2 * th.pair + 1 < th.nch) A.seg_sum[at + th.channel(1)] = f.y;
+  th.store_kept(A.seg_grad + at * sh.kn, 0, G);
+  th.put1(A.seg_sum + at, 0, sum);
 }
 
+// Brings the tiles of a segment, from the last to the first, and takes their gradients away.
 template <typename T, int LN>
-__global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const __grid_constant__ BwdArgs A) {
+__device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, const BwdThread<LN>& th, int seg, int tile0, int tile1) {
   using Tile = ScanTile<LN>;
-  using Smem = BwdSmem<LN>;
-  extern __shared__ char smem_raw[];
-  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  using Thread = BwdThread<LN>;
   const ScanShape& sh = A.sh;
   const rfa_scan_t& p = A.p;
-  const ScanThread<LN> th(sh);
-  const int seg = blockIdx.z, tile0 = seg * sh.seg_tiles, tile1 = min(tile0 + sh.seg_tiles, sh.tiles);
-
-  f32x2 a2[4], G[4], da[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    a2[j] = mul2(th.get(p.a, j, sh.N), both(kLog2e));
-    G[j] = A.g_s ? th.get(A.g_s + (size_t)th.b * sh.D * sh.N, j, sh.N) : both(0.f);
-    da[j] = both(0.f);
-  }
-  for (int i = sh.segs - 2; i >= seg; --i) {           // the segments behind this one
-    const size_t at = ((size_t)i * sh.B + th.b) * sh.D;
-    f32x2 v[4];
-    th.load_kept(A.seg_grad + at * sh.kn, v);
-    const float* total = A.seg_sum + at + th.channel(0);
-    const f32x2 over = pack2(2 * th.pair < th.nch ? total[0] : 0.f, 2 * th.pair + 1 < th.nch ? total[1] : 0.f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) G[j] = fma2(exp2_unit(mul2(over, a2[j])), G[j], v[j]);
-  }
-
   const int ch = th.c0 + 2 * th.vpair;
   const T* x = static_cast<const T*>(p.x) + (int64_t)th.b * p.x_b + ch;
   const T* dt = static_cast<const T*>(p.dt) + (int64_t)th.b * p.dt_b + ch;
@@ -170,165 +158,48 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const __grid_
     bias[k] = p.dt_bias && k < th.vn ? p.dt_bias[ch + k] : 0.f;
     skip[k] = p.d && k < th.vn ? p.d[ch + k] : 0.f;
   }
-
-  RawPairs<T, LN> rx, rd, rg, kept;
-  RawStates<T, LN> rb, rc;
-  f32x2 first[4];                                      // the state in front of the tile
-  uint32_t here = 0, next = 0;
+  RawPairs<T, Thread> rx, rd, rg, kept;
+  RawStates<T, LN, Thread> rb, rc;
+  uint32_t here = 0, next = 0;                         // which of this thread's tokens are there: in the tile that is scanned, in the next one
   const int plain = A.wide && !mask && th.nch == Tile::kChannels && sh.N == Tile::kN ? (int)(sh.T / kScanTile) : 0;      // tiles in front of it are
   const auto ask = [&](int tile, auto kind) {
     constexpr bool kPlain = decltype(kind)::value;
     const int64_t t0 = (int64_t)tile * kScanTile, t = t0 + th.row;
-    next = kPlain ? ~0u : tokens_here<LN>(th, mask, t0, sh.T);
+    next = kPlain ? ~0u : th.tokens_here(mask, t0, sh.T);
     rx.template load<kPlain>(x + t * p.x_t, p.x_t, next, th.vn, A.wide);
     rd.template load<kPlain>(dt + t * p.dt_t, p.dt_t, next, th.vn, A.wide);
     rg.template load<kPlain>(g + t * row_stride, row_stride, next, th.vn, A.wide);
-    rb.template load<kPlain>(bp, p.b_t, t0, sh.T, sh.N, mask);
-    rc.template load<kPlain>(cp, p.c_t, t0, sh.T, sh.N, mask);
-    th.load_kept(A.ckpt + ((size_t)th.b * sh.tiles + tile) * sh.D * sh.kn, first);
+    rb.template load<kPlain>(th, bp, p.b_t, t0, sh.T, sh.N, mask);
+    rc.template load<kPlain>(th, cp, p.c_t, t0, sh.T, sh.N, mask);
   };
   const auto ask_tile = [&](int tile) { tile < plain ? ask(tile, Plain()) : ask(tile, Ragged()); };
-  const auto put = [&]() {
-    here = next;
+  const auto put = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < Tile::kPasses; ++i) {
+    for (int i = 0; i < Thread::kPasses; ++i) {
       float2 sig = make_float2(1.f, 1.f);
       const float2 v = make_float2(rd.v[i].get(0) + bias[0], rd.v[i].get(1) + bias[1]);
       const f32x2 delta = p.softplus ? softplus2<true>(v, sig) : pack2(v.x, v.y);
       const f32x2 dx = mul2(delta, pack2(rx.v[i].get(0), rx.v[i].get(1)));
-      const bool on = here >> i & 1;
-      *reinterpret_cast<ulonglong2*>(&sm.in[th.row + i * Tile::kRows][th.vpair]) = make_ulonglong2(on ? delta : 0, on ? dx : 0);
-      sm.up[th.row + i * Tile::kRows][th.vpair] = make_float4(rg.v[i].get(0), rg.v[i].get(1), sig.x, sig.y);
-      kept.v[i] = rx.v[i];
+      const bool on = next >> i & 1;
+      *reinterpret_cast<ulonglong2*>(&sm.in[buf][th.row + i * Thread::kRows][th.vpair]) = make_ulonglong2(on ? delta : 0, on ? dx : 0);
+      sm.g[buf][th.row + i * Thread::kRows][th.vpair] = make_float2(rg.v[i].get(0), rg.v[i].get(1));
+      sm.slope[buf][th.row + i * Thread::kRows][th.vpair] = sig;
     }
-    rb.store(sm.b);
-    rc.store(sm.c);
+    rb.store(th, sm.b[buf]);
+    rc.store(th, sm.c[buf]);
   };
-
-  ask_tile(tile1 - 1);
-  for (int tile = tile1 - 1; tile >= tile0; --tile) {
-    f32x2 s[4];
+  // gx and gdt of a part's tokens
+  const auto take = [&](int64_t t0, int buf, int part) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = first[j];
-    put();
-    __syncthreads();
-    if (tile > tile0) ask_tile(tile - 1);
-    const int64_t t0 = (int64_t)tile * kScanTile;
-
-    // The states in front of each part of the tile, then part by part from the last: forward with what the way back needs, and back.
-#pragma unroll 1
-    for (int part = 0; part < kScanTile / kRun; ++part) {
-      f32x2 delta[kRun], dx[kRun], e[kRun][4];
-      sm.start[part][0][threadIdx.x] = make_ulonglong2(s[0], s[1]);
-      sm.start[part][1][threadIdx.x] = make_ulonglong2(s[2], s[3]);
-      if (part == kScanTile / kRun - 1) break;
-#pragma unroll
-      for (int r = 0; r < kRun; ++r) {
-        const ulonglong2 in = *reinterpret_cast<const ulonglong2*>(&sm.in[part * kRun + r][th.pair]);
-        delta[r] = in.x;
-        dx[r] = in.y;
-      }
-      decays<kRun>(delta, a2, e);
-#pragma unroll
-      for (int r = 0; r < kRun; ++r) {
-        float bt[4];
-        lane_states(sm.b[part * kRun + r], th.ln, bt);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = fma2(e[r][j], s[j], scale(split2(dx[r]), bt[j]));
-      }
-    }
-#pragma unroll 1
-    for (int part = kScanTile / kRun - 1; part >= 0; --part) {
-      const int base = part * kRun;
-      f32x2 delta[kRun], dx[kRun], e[kRun][4], st[kRun + 1][4];      // decays; the states in front of each token
-      const ulonglong2 lo = sm.start[part][0][threadIdx.x], hi = sm.start[part][1][threadIdx.x];
-      st[0][0] = lo.x; st[0][1] = lo.y; st[0][2] = hi.x; st[0][3] = hi.y;
-#pragma unroll
-      for (int r = 0; r < kRun; ++r) {
-        const ulonglong2 in = *reinterpret_cast<const ulonglong2*>(&sm.in[base + r][th.pair]);
-        delta[r] = in.x;
-        dx[r] = in.y;
-      }
-      decays<kRun>(delta, a2, e);
-#pragma unroll
-      for (int r = 0; r < kRun; ++r) {
-        float bt[4];
-        lane_states(sm.b[base + r], th.ln, bt);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) st[r + 1][j] = fma2(e[r][j], st[r][j], scale(split2(dx[r]), bt[j]));
-      }
-#pragma unroll
-      for (int t = kRun - 1; t >= 0; --t) {
-        const float2 gt = *reinterpret_cast<const float2*>(&sm.up[base + t][th.pair]), dxt = split2(dx[t]);
-        float bt[4], ct[4], gb[4], gc[4];              // gb, gc: of the four states, over both channels
-        f32x2 over_b = both(0.f), over_p = both(0.f);  // sum_n G b, sum_n a2 p of both channels
-        lane_states(sm.b[base + t], th.ln, bt);
-        lane_states(sm.c[base + t], th.ln, ct);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x2 Gt = scale_add(gt, ct[j], G[j]), pt = mul2(Gt, mul2(e[t][j], st[t][j]));
-          const float2 Gs = split2(Gt), ss = split2(st[t + 1][j]);
-          gb[j] = fmaf(Gs.x, dxt.x, Gs.y * dxt.y);
-          gc[j] = fmaf(ss.x, gt.x, ss.y * gt.y);
-          over_b = scale_add(Gs, bt[j], over_b);
-          over_p = fma2(pt, a2[j], over_p);
-          da[j] = fma2(pt, delta[t], da[j]);
-          G[j] = mul2(Gt, e[t][j]);
-        }
-        sm.part[base + t][0][th.pair][th.ln] = make_float4(gb[0], gb[1], gb[2], gb[3]);
-        sm.part[base + t][1][th.pair][th.ln] = make_float4(gc[0], gc[1], gc[2], gc[3]);
-        const float2 ob = split2(over_b), op = split2(over_p);
-        float over_n[4] = {ob.x, ob.y, op.x, op.y};
-        lanes_sum<4, LN>(over_n, th.ln);
-        float* res = reinterpret_cast<float*>(&sm.res[base + t][th.pair]);
-        if constexpr (LN <= 4) {
-#pragma unroll
-          for (int i = 0; i < 4 / LN; ++i) res[th.ln * (4 / LN) + i] = over_n[i];
-        } else {
-          if (th.ln % (LN / 4) == 0) res[th.ln / (LN / 4)] = over_n[0];
-        }
-      }
-    }
-    __syncthreads();
-    // gb and gc of the CTA's channels: kEach neighbouring threads share the sum of one token's four states
-    constexpr int kOut = kScanTile * 2 * LN, kEach = kOut < kScanThreads ? kScanThreads / kOut : 1;
-#pragma unroll
-    for (int o = threadIdx.x / kEach; o < kOut; o += kScanThreads / kEach) {
-      const int l = o % LN, which = o / LN % 2, t = o / (2 * LN);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int r = 0; r < Smem::kParts / kEach; ++r) {
-        const float4 w = sm.part[t][which][r * kEach + threadIdx.x % kEach][l];
-        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-      }
-      float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int w = kEach / 2; w > 0; w >>= 1)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] += __shfl_xor_sync(0xffffffffu, f[j], w);
-      const int64_t token = t0 + t;
-      if (token >= sh.T || threadIdx.x % kEach) continue;
-      const bool gone = mask && mask[token];
-      const int64_t to = ((token * sh.B + th.b) * sh.G + th.group) * sh.N;
-      const int64_t part = (int64_t)(blockIdx.x % sh.per_group) * sh.T * sh.B * sh.G * sh.N + to;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = j * LN + l;
-        if (n >= sh.N) continue;
-        const float out = gone ? 0.f : f[j];
-        if (sh.per_group == 1) static_cast<T*>(which ? A.gc : A.gb)[to + n] = from_f<T>(out);
-        else (which ? A.part_c : A.part_b)[part + n] = out;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < Tile::kPasses; ++i) {
-      const int t = th.row + i * Tile::kRows;
-      if (t0 + t >= sh.T) continue;
+    for (int i = 0; i < Thread::kPasses; ++i) {
+      const int t = th.row + i * Thread::kRows;
+      if (t / kPart != part || t0 + t >= sh.T) continue;
       Raw<T, 2> ox, od;
       ox.zero(); od.zero();
       if (here >> i & 1) {
-        const float4 in = sm.in[t][th.vpair], up = sm.up[t][th.vpair], res = sm.res[t][th.vpair];
-        const float delta[2] = {in.x, in.y}, gt[2] = {up.x, up.y}, sig[2] = {up.z, up.w}, gu[2] = {res.x, res.y}, gp[2] = {res.z, res.w};
+        const float4 in = sm.in[buf][t][th.vpair], res = sm.res[t][th.vpair];
+        const float2 gv = sm.g[buf][t][th.vpair], sv = sm.slope[buf][t][th.vpair];
+        const float delta[2] = {in.x, in.y}, gt[2] = {gv.x, gv.y}, sig[2] = {sv.x, sv.y}, gu[2] = {res.x, res.y}, gp[2] = {res.z, res.w};
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float xv = kept.v[i].get(k), v = fmaf(xv, gu[k], kLn2 * gp[k]) * sig[k];
@@ -341,22 +212,79 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const __grid_
       ox.store(static_cast<T*>(A.gx) + (t0 + t) * row_stride + out0, th.vn, A.wide);
       od.store(static_cast<T*>(A.gdt) + (t0 + t) * row_stride + out0, th.vn, A.wide);
     }
-    __syncthreads();
+  };
+  // gb and gc of a part's tokens over the CTA's channels: kEach threads share the sum of one token's and lane's four states
+  const auto sum = [&](int64_t t0, int part, int w) {
+    constexpr int kOut = kPart * 2 * LN, kEach = kOut < kBwdBring ? kBwdBring / kOut : 1;
+#pragma unroll
+    for (int o = 0; o < kOut * kEach; o += kBwdBring) {
+      const int at = o + th.tid, l = at % LN, share = at / LN % kEach, which = at / (LN * kEach) % 2, t = at / (LN * kEach * 2);
+      ulonglong2 f = make_ulonglong2(0, 0);
+#pragma unroll
+      for (int r = 0; r < BwdSmem<LN>::kThreads / kEach; ++r) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.over_ch[w][t][which][r * kEach + share][l]);
+        f.x = add2(f.x, v.x);
+        f.y = add2(f.y, v.y);
+      }
+      const float2 lo = split2(f.x), hi = split2(f.y);
+      float v[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+      for (int s = kEach / 2; s > 0; s >>= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], s * LN);
+      const int64_t token = t0 + part * kPart + t;
+      if (token >= sh.T || share) continue;
+      const bool gone = mask && mask[token];
+      const int64_t to = ((token * sh.B + th.b) * sh.G + th.group) * sh.N;
+      const int64_t to_part = (int64_t)(blockIdx.x % sh.per_group) * sh.T * sh.B * sh.G * sh.N + to;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = j * LN + l;
+        if (n >= sh.N) continue;
+        const float out = gone ? 0.f : v[j];
+        if (sh.per_group == 1) static_cast<T*>(which ? A.gc : A.gb)[to + n] = from_f<T>(out);
+        else (which ? A.part_c : A.part_b)[to_part + n] = out;
+      }
+    }
+  };
+
+  ask_tile(tile1 - 1);
+  put(0);
+  meet_go<kBwdThreads>(kFull);
+  kept = rx;
+  here = next;
+  if (tile1 - 1 > tile0) ask_tile(tile1 - 2);
+  for (int tile = tile1 - 1; tile >= tile0; --tile) {
+    const int buf = (tile1 - 1 - tile) & 1;
+    RawPairs<T, Thread> x_next = rx;
+    const uint32_t here_next = next;
+    if (tile > tile0) {                                // its last tile has been scanned and taken
+      put(buf ^ 1);
+      meet_go<kBwdThreads>(kFull + (buf ^ 1));
+      if (tile - 1 > tile0) ask_tile(tile - 2);
+    }
+    const int64_t t0 = (int64_t)tile * kScanTile;
+#pragma unroll 1
+    for (int part = kScanTile / kPart - 1; part >= 0; --part) {
+      const int w = part & 1;
+      meet_wait<kBwdThreads>(kSums + w);
+      sum(t0, part, w);
+      take(t0, buf, part);
+      if (tile > tile0 || part > 1) meet_go<kBwdThreads>(kTaken + w);      // somebody waits for it
+    }
+    kept = x_next;
+    here = here_next;
   }
 
   const size_t row = (size_t)th.b * sh.segs + seg;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    th.put(A.part_a + row * sh.D * sh.N, j, sh.N, da[j]);
-    if (seg == 0 && A.gs_in) th.put(A.gs_in + (size_t)th.b * sh.D * sh.N, j, sh.N, G[j]);
-  }
-  float4* over_rows = &sm.in[0][0];                    // gd and gbias over the rows of loading threads
-  over_rows[threadIdx.x] = make_float4(gd[0], gd[1], gbias[0], gbias[1]);
-  __syncthreads();
+  // gd and gbias over the rows of loading threads, where the scanning warps have nothing left to read: they handed over their last part
+  float4* over_rows = &sm.in[0][0][0];
+  over_rows[th.tid] = make_float4(gd[0], gd[1], gbias[0], gbias[1]);
+  asm volatile("bar.sync 9, %0;" ::"n"(kBwdBring) : "memory");
   if (th.row == 0) {
-    float4 v = over_rows[threadIdx.x];
-    for (int r = 1; r < Tile::kRows; ++r) {
-      const float4 w = over_rows[r * Tile::kPairs + threadIdx.x];
+    float4 v = over_rows[th.tid];
+    for (int r = 1; r < Thread::kRows; ++r) {
+      const float4 w = over_rows[r * Tile::kPairs + th.tid];
       v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
     }
 #pragma unroll
@@ -368,16 +296,172 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_bwd_kernel(const __grid_
   }
 }
 
+template <typename T, int LN>
+__global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_constant__ BwdArgs A) {
+  using Smem = BwdSmem<LN>;
+  extern __shared__ char smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  const ScanShape& sh = A.sh;
+  const rfa_scan_t& p = A.p;
+  const BwdThread<LN> th(sh);
+  const int seg = blockIdx.z, tile0 = seg * sh.seg_tiles, tile1 = min(tile0 + sh.seg_tiles, sh.tiles);
+  if (!th.scans) {
+    bwd_bring<T, LN>(A, sm, th, seg, tile0, tile1);
+    return;
+  }
+
+  f32x2 a2[kP][4], G[kP][4], da[kP][4];
+#pragma unroll
+  for (int k = 0; k < kP; ++k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a2[k][j] = mul2(th.get(p.a, k, j, sh.N), both(kLog2e));
+      G[k][j] = A.g_s ? th.get(A.g_s + (size_t)th.b * sh.D * sh.N, k, j, sh.N) : both(0.f);
+      da[k][j] = both(0.f);
+    }
+    for (int i = sh.segs - 2; i >= seg; --i) {         // the segments behind this one
+      const size_t at = ((size_t)i * sh.B + th.b) * sh.D;
+      f32x2 v[4];
+      th.load_kept(A.seg_grad + at * sh.kn, k, v);
+      const f32x2 over = th.get1(A.seg_sum + at, k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) G[k][j] = fma2(exp2_unit(mul2(over, a2[k][j])), G[k][j], v[j]);
+    }
+  }
+
+  f32x2 s[kP][4];                                      // the state in front of the tile
+  const float* ckpt = A.ckpt + (size_t)th.b * sh.tiles * sh.D * sh.kn;
+  const auto load_state = [&](int tile) {
+#pragma unroll
+    for (int k = 0; k < kP; ++k) th.load_kept(ckpt + (size_t)tile * sh.D * sh.kn, k, s[k]);
+  };
+  load_state(tile1 - 1);
+  for (int tile = tile1 - 1; tile >= tile0; --tile) {
+    const int buf = (tile1 - 1 - tile) & 1;
+    const auto inputs = [&](int base, f32x2 (*delta)[kP], f32x2 (*dx)[kP]) {
+#pragma unroll
+      for (int r = 0; r < kRun; ++r)
+#pragma unroll
+        for (int k = 0; k < kP; ++k) {
+          const ulonglong2 in = *reinterpret_cast<const ulonglong2*>(&sm.in[buf][base + r][th.pair + k]);
+          delta[r][k] = in.x;
+          dx[r][k] = in.y;
+        }
+    };
+    meet_wait<kBwdThreads>(kFull + buf);
+    // The states in front of each run of the tile, then run by run from the last: forward with what the way back needs, and back.
+#pragma unroll 1
+    for (int run = 0;; ++run) {
+#pragma unroll
+      for (int k = 0; k < kP; ++k) {
+        sm.start[run][2 * k][th.tid] = make_ulonglong2(s[k][0], s[k][1]);
+        sm.start[run][2 * k + 1][th.tid] = make_ulonglong2(s[k][2], s[k][3]);
+      }
+      if (run == kScanTile / kRun - 1) break;
+      f32x2 delta[kRun][kP], dx[kRun][kP], e[kRun][kP][4];
+      inputs(run * kRun, delta, dx);
+      decays<kRun, kP, false>(delta, a2, e);
+#pragma unroll
+      for (int r = 0; r < kRun; ++r) {
+        float bt[4];
+        lane_states(sm.b[buf][run * kRun + r], th.ln, bt);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int k = 0; k < kP; ++k) s[k][j] = fma2(e[r][k][j], s[k][j], mul2(dx[r][k], both(bt[j])));
+      }
+    }
+    if (tile > tile0) load_state(tile - 1);            // asked for early
+#pragma unroll 2
+    for (int run = kScanTile / kRun - 1; run >= 0; --run) {
+      const int base = run * kRun, w = base / kPart & 1;
+      f32x2 delta[kRun][kP], dx[kRun][kP], e[kRun][kP][4], q[kRun][kP][4], st[kRun][kP][4];      // decays, decayed states, states
+      float bt[kRun][4];
+      inputs(base, delta, dx);
+#pragma unroll
+      for (int k = 0; k < kP; ++k) {
+        const ulonglong2 lo = sm.start[run][2 * k][th.tid], hi = sm.start[run][2 * k + 1][th.tid];
+        q[0][k][0] = lo.x; q[0][k][1] = lo.y; q[0][k][2] = hi.x; q[0][k][3] = hi.y;
+      }
+      decays<kRun, kP, true>(delta, a2, e);
+#pragma unroll
+      for (int r = 0; r < kRun; ++r) {
+        lane_states(sm.b[buf][base + r], th.ln, bt[r]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int k = 0; k < kP; ++k) {
+            q[r][k][j] = mul2(e[r][k][j], r ? st[r - 1][k][j] : q[0][k][j]);
+            st[r][k][j] = fma2(dx[r][k], both(bt[r][j]), q[r][k][j]);
+          }
+      }
+      // the part's place is free
+      if (base % kPart == kPart - kRun && (tile < tile1 - 1 || base < kScanTile - 2 * kPart)) meet_wait<kBwdThreads>(kTaken + w);
+#pragma unroll
+      for (int r = kRun - 1; r >= 0; --r) {
+        f32x2 gt[kP], over_b[kP], over_p[kP];          // g; sum_n G b, sum_n a2 p
+#pragma unroll
+        for (int k = 0; k < kP; ++k) gt[k] = *reinterpret_cast<const f32x2*>(&sm.g[buf][base + r][th.pair + k]);
+        float ct[4], gb[4], gc[4];                     // gb, gc: of the four states, over the thread's channels
+        lane_states(sm.c[buf][base + r], th.ln, ct);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x2 vb, vc;
+#pragma unroll
+          for (int k = 0; k < kP; ++k) {
+            const f32x2 Gt = fma2(gt[k], both(ct[j]), G[k][j]), pt = mul2(Gt, q[r][k][j]);
+            vb = k ? fma2(Gt, dx[r][k], vb) : mul2(Gt, dx[r][k]);
+            vc = k ? fma2(st[r][k][j], gt[k], vc) : mul2(st[r][k][j], gt[k]);
+            over_b[k] = j ? fma2(Gt, both(bt[r][j]), over_b[k]) : mul2(Gt, both(bt[r][j]));
+            over_p[k] = j ? fma2(pt, a2[k][j], over_p[k]) : mul2(pt, a2[k][j]);
+            da[k][j] = fma2(pt, delta[r][k], da[k][j]);
+            G[k][j] = mul2(Gt, e[r][k][j]);
+          }
+          const float2 fb = split2(vb), fc = split2(vc);
+          gb[j] = fb.x + fb.y;
+          gc[j] = fc.x + fc.y;
+        }
+        const int t = base % kPart + r;
+        sm.over_ch[w][t][0][th.pair / kP][th.ln] = make_float4(gb[0], gb[1], gb[2], gb[3]);
+        sm.over_ch[w][t][1][th.pair / kP][th.ln] = make_float4(gc[0], gc[1], gc[2], gc[3]);
+        float over_n[4 * kP];                          // as kP rows of res
+#pragma unroll
+        for (int k = 0; k < kP; ++k) {
+          const float2 ob = split2(over_b[k]), op = split2(over_p[k]);
+          over_n[4 * k] = ob.x; over_n[4 * k + 1] = ob.y; over_n[4 * k + 2] = op.x; over_n[4 * k + 3] = op.y;
+        }
+        lanes_sum<4 * kP, LN>(over_n, th.ln);
+        float* res = reinterpret_cast<float*>(&sm.res[base + r][th.pair]);
+        constexpr int kEach = 4 * kP / LN, kLanes = LN / (4 * kP);      // totals of a lane, or lanes with one total
+        if constexpr (kEach == 4) *reinterpret_cast<float4*>(res + 4 * th.ln) = make_float4(over_n[0], over_n[1], over_n[2], over_n[3]);
+        else if constexpr (kEach == 2) *reinterpret_cast<float2*>(res + 2 * th.ln) = make_float2(over_n[0], over_n[1]);
+        else if constexpr (kEach == 1) res[th.ln] = over_n[0];
+        else if (th.ln % kLanes == 0) res[th.ln / kLanes] = over_n[0];
+      }
+      if (base % kPart == 0) meet_go<kBwdThreads>(kSums + w);
+    }
+  }
+
+  const size_t row = (size_t)th.b * sh.segs + seg;
+#pragma unroll
+  for (int k = 0; k < kP; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      th.put(A.part_a + row * sh.D * sh.N, k, j, sh.N, da[k][j]);
+      if (seg == 0 && A.gs_in) th.put(A.gs_in + (size_t)th.b * sh.D * sh.N, k, j, sh.N, G[k][j]);
+    }
+}
+
 template <typename T, int LN> int launch_bwd(const BwdArgs& a, cudaStream_t stream) {
   constexpr int bytes = (int)sizeof(BwdSmem<LN>);
   const dim3 grid(a.sh.per_group * a.sh.G, a.sh.B, a.sh.segs);
   const cudaError_t err = cudaFuncSetAttribute(scan_bwd_kernel<T, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   RFA_REQUIRE(err == cudaSuccess, (int)err, "selective_scan_bwd: %s", cudaGetErrorString(err));
   if (a.sh.segs > 1) {
-    scan_bwd_summary_kernel<T, LN><<<dim3(grid.x, grid.y, a.sh.segs - 1), kScanThreads, 0, stream>>>(a);
+    scan_bwd_summary_kernel<T, LN><<<dim3(grid.x, grid.y, a.sh.segs - 1), kSummaryThreads, 0, stream>>>(a);
     if (int r = check_launch("selective_scan_bwd (segments)")) return r;
   }
-  scan_bwd_kernel<T, LN><<<grid, kScanThreads, bytes, stream>>>(a);
+  scan_bwd_kernel<T, LN><<<grid, kBwdThreads, bytes, stream>>>(a);
   return check_launch("selective_scan_bwd");
 }
 
