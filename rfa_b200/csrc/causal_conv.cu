@@ -11,7 +11,8 @@
 namespace rfa {
 namespace {
 
-constexpr int kConvWarps = 4, kConvRun = 16, kConvBwdRun = 32, kConvFlight = 4, kConvMax = 8;
+constexpr int kConvWarps = 4, kConvRun = 32, kConvFlight = 4, kConvMax = 8;
+constexpr int kConvVec = 4;      // adjacent channels of a thread
 
 struct ConvArgs {
   rfa_causal_conv_t p;
@@ -19,7 +20,8 @@ struct ConvArgs {
   const void *g, *g_state;
   int64_t g_t, g_b;
   void *gx, *g_state_in;
-  float *part_w, *part_b;      // [gridDim.x * B][D][W], [gridDim.x * B][D]; null: not wanted
+  float *part_w, *part_b;      // [row_blocks * B][D][W], [row_blocks * B][D]; null: not wanted
+  int row_blocks, ch_blocks;   // a CTA's place: channels fastest, so that what runs side by side reads whole rows
   bool wide;
 };
 
@@ -34,13 +36,27 @@ __device__ __forceinline__ int64_t token_before(const uint8_t* mask, int64_t t) 
   return -1;
 }
 
-__device__ __forceinline__ float silu_or(float v, bool silu) { return silu ? v * sigmoid(v) : v; }
+// The first token from t on that is not masked, T for none.
+__device__ __forceinline__ int64_t token_after(const uint8_t* mask, int64_t t, int64_t T) {
+  const int lane = threadIdx.x & 31;
+  for (; t < T; t += 32) {
+    const uint32_t there = __ballot_sync(0xffffffffu, t + lane < T && !mask[t + lane]);
+    if (there) return t + __ffs(there) - 1;
+  }
+  return T;
+}
 
 template <typename T, int NV> __device__ __forceinline__ void load_row(const T* p, int n, bool wide, float* v) {
   Raw<T, NV> r;
   r.load(p, n, wide);
 #pragma unroll
   for (int c = 0; c < NV; ++c) v[c] = r.get(c);
+}
+
+// Whether the four tokens from the run's i-th on are there.
+__device__ __forceinline__ bool four_there(uint32_t there, int i) {
+  static_assert(kConvFlight == 4 && kConvRun == 32, "bits of a run, four at a time");
+  return i < kConvRun && (there >> i & 15u) == 15u;
 }
 
 // What a thread of either kernel is; the window in front of its run.
@@ -52,24 +68,36 @@ template <typename T, int NV, int W, bool kMask> struct ConvThread {
   const T* x;
   const uint8_t* mask;
   float w[W][NV], bias[NV];
-  __device__ ConvThread(const ConvArgs& a, int run) : p(a.p), wide(a.wide) {
-    c0 = (blockIdx.y * 32 + (threadIdx.x & 31)) * NV;
+  int ch_block, row_block;
+  __device__ ConvThread(const ConvArgs& a) : p(a.p), wide(a.wide) {
+    ch_block = blockIdx.x % a.ch_blocks;
+    row_block = blockIdx.x / a.ch_blocks;
+    c0 = (ch_block * 32 + (threadIdx.x & 31)) * NV;
     n = min(NV, p.D - c0);                             // may be negative: such a thread only takes part in its warp's ballots
-    b = blockIdx.z;
-    t0 = ((int64_t)blockIdx.x * kConvWarps + (threadIdx.x >> 5)) * run;
-    t1 = min(t0 + run, p.T);
+    b = blockIdx.y;
+    t0 = ((int64_t)row_block * kConvWarps + (threadIdx.x >> 5)) * kConvRun;
+    t1 = min(t0 + kConvRun, p.T);
     x = static_cast<const T*>(p.x) + (int64_t)b * p.x_b + c0;
     mask = kMask ? p.mask + (int64_t)b * p.T : nullptr;
+    Raw<T, NV * W> rw;
+    rw.load(static_cast<const T*>(p.weight) + (size_t)c0 * W, n * W, wide);
+    Raw<T, NV> rb;
+    rb.zero();
+    if (p.bias) rb.load(static_cast<const T*>(p.bias) + c0, n, wide);
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) w[j][c] = c < n ? to_f(static_cast<const T*>(p.weight)[(size_t)(c0 + c) * W + j]) : 0.f;
-      bias[c] = p.bias && c < n ? to_f(static_cast<const T*>(p.bias)[c0 + c]) : 0.f;
+      for (int j = 0; j < W; ++j) w[j][c] = rw.get(c * W + j);
+      bias[c] = rb.get(c);
     }
   }
-  __device__ __forceinline__ bool gone(int64_t t) const { return kMask && mask[t]; }
+  // The run's tokens that are there: bit t - t0.
+  __device__ __forceinline__ uint32_t tokens() const {
+    const int64_t t = t0 + (threadIdx.x & 31);
+    return __ballot_sync(0xffffffffu, t < t1 && !(kMask && mask[t]));
+  }
   // win[0 .. W - 2]: the tokens in front of t0, oldest first; at[]: where they stand (-1 ... -(W - 1): in the incoming state)
-  __device__ __forceinline__ void before(float (*win)[NV], int64_t* at) const {
+  __device__ __forceinline__ void before(float (*win)[NV], int* at) const {
     int64_t t = t0;
     int slot = W - 2;                                  // of the incoming state
 #pragma unroll
@@ -78,7 +106,7 @@ template <typename T, int NV, int W, bool kMask> struct ConvThread {
       else t = -1;
       if (t >= 0) {
         load_row<T, NV>(x + t * p.x_t, n, wide, win[j]);
-        at[j] = t;
+        at[j] = (int)t;
       } else {
         if (p.state_in) load_row<T, NV>(static_cast<const T*>(p.state_in) + ((size_t)b * (W - 1) + slot) * p.D + c0, n, wide, win[j]);
         else
@@ -94,69 +122,75 @@ template <typename T, int NV, int W, bool kMask> struct ConvThread {
 
 template <typename T, int NV, int W, bool kMask>
 __global__ void __launch_bounds__(32 * kConvWarps) conv_fwd_kernel(const __grid_constant__ ConvArgs a) {
-  const ConvThread<T, NV, W, kMask> th(a, kConvRun);
+  const ConvThread<T, NV, W, kMask> th(a);
   const rfa_causal_conv_t& p = a.p;
   if (th.t0 >= p.T) return;
   const bool last = th.t1 == p.T && a.state_out;
   const int64_t out_t = (int64_t)p.B * p.D;
-  T* y = static_cast<T*>(a.y) + (int64_t)th.b * p.D + th.c0;
-  Raw<T, NV> none;
-  none.zero();
-  if (kMask && !last) {                                // a run of padding has no window to look for
-    const int64_t t = th.t0 + (threadIdx.x & 31);
-    if (!__ballot_sync(0xffffffffu, t < th.t1 && !th.mask[t])) {
-      for (int64_t u = th.t0; u < th.t1; ++u) none.store(y + u * out_t, th.n, th.wide);
-      return;
-    }
-  }
+  const int count = (int)(th.t1 - th.t0);
+  const uint32_t there = th.tokens();
+  const T* from = th.x + th.t0 * p.x_t;
+  T* to = static_cast<T*>(a.y) + (int64_t)th.b * p.D + th.c0 + th.t0 * out_t;
   float win[W - 1 + kConvFlight][NV];
-  int64_t at[W];
-  th.before(win, at);
-  for (int64_t t = th.t0; t < th.t1; t += kConvFlight) {
-    Raw<T, NV> raw[kConvFlight];
+  if (there || last) {                                 // (a run of padding has no window to look for)
+    int at[W];
+    th.before(win, at);
+  }
+  const auto put = [&](int first, T* out_at) {         // one output, from the window that begins at `first`
+    float v[NV];
 #pragma unroll
-    for (int i = 0; i < kConvFlight; ++i) {
-      raw[i].zero();
-      if (t + i < th.t1 && !th.gone(t + i)) raw[i].load(th.x + (t + i) * p.x_t, th.n, th.wide);
+    for (int c = 0; c < NV; ++c) {
+      v[c] = th.bias[c];
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[c] = fmaf(th.w[j][c], win[first + j][c], v[c]);
     }
-    int len = 0;                                       // tokens of these that are there
+    if (p.silu) {
 #pragma unroll
-    for (int i = 0; i < kConvFlight; ++i) {
-      if (t + i >= th.t1) break;
-      if (th.gone(t + i)) {
-        none.store(y + (t + i) * out_t, th.n, th.wide);
-        continue;
-      }
-      const int at_i = kMask ? 0 : i;                  // with a mask the window is moved on token by token, else after four
-#pragma unroll
-      for (int c = 0; c < NV; ++c) win[W - 1 + at_i][c] = raw[i].get(c);
-      Raw<T, NV> out;
-      out.zero();
-#pragma unroll
-      for (int c = 0; c < NV; ++c) {
-        float pre = th.bias[c];
-#pragma unroll
-        for (int j = 0; j < W; ++j) pre = fmaf(th.w[j][c], win[at_i + j][c], pre);
-        out.set(c, from_f<T>(silu_or(pre, p.silu)));
-      }
-      out.store(y + (t + i) * out_t, th.n, th.wide);
-      if (kMask) {
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-          for (int c = 0; c < NV; ++c) win[j][c] = win[j + 1][c];
-      }
-      ++len;
+      for (int c = 0; c < NV; ++c) v[c] *= sigmoid(v[c]);
     }
-    if (!kMask) {
+    Raw<T, NV> out;
 #pragma unroll
-      for (int k = 1; k <= kConvFlight; ++k)           // len is at most four, and less only at the end
-        if (len == k) {
+    for (int c = 0; c < NV; c += 2) out.set2(c / 2, v[c], v[c + 1]);
+    out.store(out_at, th.n, th.wide);
+  };
+  const auto move = [&](int by) {
 #pragma unroll
-          for (int j = 0; j < W - 1; ++j)
+    for (int j = 0; j < W - 1; ++j)
 #pragma unroll
-            for (int c = 0; c < NV; ++c) win[j][c] = win[j + k][c];
-        }
+      for (int c = 0; c < NV; ++c) win[j][c] = win[j + by][c];
+  };
+  Raw<T, NV> raw[kConvFlight];
+  const auto ask = [&](int i) {
+    const T* at = from + i * p.x_t;
+#pragma unroll
+    for (int k = 0; k < kConvFlight; ++k, at += p.x_t) raw[k].load(at, th.n, th.wide);
+  };
+  bool on_way = false;
+  for (int i = 0; i < count;) {
+    if (four_there(there, i)) {                        // four tokens together, the next four on the way
+      if (!on_way) ask(i);
+#pragma unroll
+      for (int k = 0; k < kConvFlight; ++k)
+#pragma unroll
+        for (int c = 0; c < NV; ++c) win[W - 1 + k][c] = raw[k].get(c);
+      on_way = four_there(there, i + kConvFlight);
+      if (on_way) ask(i + kConvFlight);
+      T* out_at = to + i * out_t;
+#pragma unroll
+      for (int k = 0; k < kConvFlight; ++k, out_at += out_t) put(k, out_at);
+      move(kConvFlight);
+      i += kConvFlight;
+    } else {
+      if (there >> i & 1) {
+        load_row<T, NV>(from + i * p.x_t, th.n, th.wide, win[W - 1]);
+        put(0, to + i * out_t);
+        move(1);
+      } else {
+        Raw<T, NV> none;
+        none.zero();
+        none.store(to + i * out_t, th.n, th.wide);
+      }
+      ++i;
     }
   }
   if (last) {
@@ -165,7 +199,7 @@ __global__ void __launch_bounds__(32 * kConvWarps) conv_fwd_kernel(const __grid_
       Raw<T, NV> out;
       out.zero();
 #pragma unroll
-      for (int c = 0; c < NV; ++c) out.set(c, from_f<T>(win[j][c]));
+      for (int c = 0; c < NV; c += 2) out.set2(c / 2, win[j][c], win[j][c + 1]);
       out.store(static_cast<T*>(a.state_out) + ((size_t)th.b * (W - 1) + j) * p.D + th.c0, th.n, th.wide);
     }
   }
@@ -174,86 +208,143 @@ __global__ void __launch_bounds__(32 * kConvWarps) conv_fwd_kernel(const __grid_
 template <typename T, int NV, int W, bool kMask>
 __global__ void __launch_bounds__(32 * kConvWarps) conv_bwd_kernel(const __grid_constant__ ConvArgs a) {
   __shared__ float red[kConvWarps][32 * NV + 1];
-  const ConvThread<T, NV, W, kMask> th(a, kConvBwdRun);
+  const ConvThread<T, NV, W, kMask> th(a);
   const rfa_causal_conv_t& p = a.p;
   const int64_t out_t = (int64_t)p.B * p.D;
   const T* g = static_cast<const T*>(a.g) + (int64_t)th.b * a.g_b + th.c0;
   T* gx = static_cast<T*>(a.gx) + (int64_t)th.b * p.D + th.c0;
   float dw[W][NV] = {}, db[NV] = {};
-  bool walk = th.t0 < p.T;
-  if (kMask && walk) {                                 // padded tokens' gradients; a run without others has nothing to do but the state's
-    Raw<T, NV> none;
-    none.zero();
-    for (int64_t u = th.t0; u < th.t1; ++u)
-      if (th.mask[u]) none.store(gx + u * out_t, th.n, th.wide);
-    const int64_t t = th.t0 + (threadIdx.x & 31);
-    const bool any = __ballot_sync(0xffffffffu, t < th.t1 && !th.mask[t]);
-    walk = any || (th.t0 == 0 && a.g_state_in);
-  }
-  if (walk) {
-    float win[W][NV], pend[W][NV];                     // the last W tokens, oldest first, and their gradients as far as they have come
-    int64_t at[W];
+  const int count = th.t0 < p.T ? (int)(th.t1 - th.t0) : 0;
+  const uint32_t there = th.tokens();
+  if (kMask)                                           // padded tokens' gradients
+    for (int i = 0; i < count; ++i)
+      if (!(there >> i & 1)) {
+        Raw<T, NV> none;
+        none.zero();
+        none.store(gx + (th.t0 + i) * out_t, th.n, th.wide);
+      }
+  if (there || (count && th.t0 == 0 && a.g_state_in)) {      // a run of padding has nothing to do but the state's
+    // The last W - 1 tokens and their gradients as far as they have come, oldest first; then those that are worked on.
+    float win[W - 1 + kConvFlight][NV], pend[W - 1 + kConvFlight][NV];
+    int at[W - 1 + kConvFlight];
     th.before(win, at);
 #pragma unroll
-    for (int j = 0; j < W; ++j)
+    for (int j = 0; j < W - 1 + kConvFlight; ++j)
 #pragma unroll
       for (int c = 0; c < NV; ++c) pend[j][c] = 0.f;
-    const auto give = [&](int64_t where, const float* v) {
+    const auto give = [&](int where, const float* v) {
       const bool mine = where >= th.t0 && where < th.t1, state = where < 0 && th.t0 == 0 && a.g_state_in;
       if (!mine && !state) return;
       Raw<T, NV> out;
-      out.zero();
 #pragma unroll
-      for (int c = 0; c < NV; ++c) out.set(c, from_f<T>(v[c]));
-      T* to = mine ? gx + where * out_t : static_cast<T*>(a.g_state_in) + ((size_t)th.b * (W - 1) + (W - 1 + where)) * p.D + th.c0;
+      for (int c = 0; c < NV; c += 2) out.set2(c / 2, v[c], v[c + 1]);
+      T* to = mine ? gx + (int64_t)where * out_t : static_cast<T*>(a.g_state_in) + ((size_t)th.b * (W - 1) + (W - 1 + where)) * p.D + th.c0;
       out.store(to, th.n, th.wide);
     };
-    int more = W - 1;                                  // tokens behind the run that its own still take part in
-    for (int64_t t = th.t0; t < p.T && (t < th.t1 || more > 0); t += kConvFlight) {
-      Raw<T, NV> rx[kConvFlight], rg[kConvFlight];
+    // the token whose window begins at `first`
+    const auto work = [&](int first, const Raw<T, NV>& rx, const Raw<T, NV>& rg, bool own) {
+      float gp[NV];
 #pragma unroll
-      for (int i = 0; i < kConvFlight; ++i) {
-        rx[i].zero(); rg[i].zero();
-        if (t + i < p.T && !th.gone(t + i)) {
-          rx[i].load(th.x + (t + i) * p.x_t, th.n, th.wide);
-          rg[i].load(g + (t + i) * a.g_t, th.n, th.wide);
-        }
+      for (int c = 0; c < NV; ++c) {
+        win[first + W - 1][c] = rx.get(c);
+        gp[c] = rg.get(c);
       }
-#pragma unroll
-      for (int i = 0; i < kConvFlight; ++i) {
-        const bool own = t + i < th.t1;
-        if (t + i >= p.T || (!own && more == 0)) break;
-        if (th.gone(t + i)) continue;
-        if (!own) --more;
-        at[W - 1] = t + i;
+      if (p.silu) {
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
-          win[W - 1][c] = rx[i].get(c);
-          float gp = rg[i].get(c);
-          if (p.silu) {
-            float pre = th.bias[c];
+          float pre = th.bias[c];
 #pragma unroll
-            for (int j = 0; j < W; ++j) pre = fmaf(th.w[j][c], win[j][c], pre);
-            const float sig = sigmoid(pre);
-            gp *= fmaf(pre * sig, 1.f - sig, sig);
-          }
-#pragma unroll
-          for (int j = 0; j < W; ++j) {
-            pend[j][c] = fmaf(th.w[j][c], gp, pend[j][c]);
-            if (own) dw[j][c] = fmaf(gp, win[j][c], dw[j][c]);
-          }
-          if (own) db[c] += gp;
+          for (int j = 0; j < W; ++j) pre = fmaf(th.w[j][c], win[first + j][c], pre);
+          const float sig = sigmoid(pre);
+          gp[c] *= fmaf(pre * sig, 1.f - sig, sig);
         }
-        give(at[0], pend[0]);
-#pragma unroll
-        for (int j = 0; j + 1 < W; ++j) {
-          at[j] = at[j + 1];
-#pragma unroll
-          for (int c = 0; c < NV; ++c) { win[j][c] = win[j + 1][c]; pend[j][c] = pend[j + 1][c]; }
-        }
-#pragma unroll
-        for (int c = 0; c < NV; ++c) pend[W - 1][c] = 0.f;
       }
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) pend[first + j][c] = fmaf(th.w[j][c], gp[c], pend[first + j][c]);
+        if (own) {
+#pragma unroll
+          for (int j = 0; j < W; ++j) dw[j][c] = fmaf(gp[c], win[first + j][c], dw[j][c]);
+          db[c] += gp[c];
+        }
+      }
+    };
+    const auto move = [&](int by) {
+#pragma unroll
+      for (int j = 0; j < W - 1 + kConvFlight; ++j)
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+          if (j < W - 1) win[j][c] = win[j + by][c];
+          pend[j][c] = j < W - 1 ? pend[j + by][c] : 0.f;
+        }
+    };
+    // the oldest `by` tokens have passed
+    const auto pass = [&](int by) {
+#pragma unroll
+      for (int k = 0; k < kConvFlight; ++k)
+        if (k < by) give(at[k], pend[k]);
+      move(by);
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) at[j] = at[j + by];
+    };
+    const T *from_x = th.x + th.t0 * p.x_t, *from_g = g + th.t0 * a.g_t;
+    Raw<T, NV> rx[kConvFlight], rg[kConvFlight];
+    const auto ask = [&](int i) {
+      const T *at_x = from_x + i * p.x_t, *at_g = from_g + i * a.g_t;
+#pragma unroll
+      for (int k = 0; k < kConvFlight; ++k, at_x += p.x_t, at_g += a.g_t) {
+        rx[k].load(at_x, th.n, th.wide);
+        rg[k].load(at_g, th.n, th.wide);
+      }
+    };
+    bool on_way = false;
+    for (int i = 0; i < count;) {
+      if (four_there(there, i)) {                      // four tokens together, the next four on the way
+        if (!on_way) ask(i);
+        Raw<T, NV> ux[kConvFlight], ug[kConvFlight];
+#pragma unroll
+        for (int k = 0; k < kConvFlight; ++k) { ux[k] = rx[k]; ug[k] = rg[k]; }
+        on_way = four_there(there, i + kConvFlight);
+        if (on_way) ask(i + kConvFlight);
+#pragma unroll
+        for (int k = 0; k < kConvFlight; ++k) {
+          at[W - 1 + k] = (int)th.t0 + i + k;
+          work(k, ux[k], ug[k], true);
+        }
+        pass(kConvFlight);
+        i += kConvFlight;
+      } else {
+        if (there >> i & 1) {
+          rx[0].load(from_x + i * p.x_t, th.n, th.wide);
+          rg[0].load(from_g + i * a.g_t, th.n, th.wide);
+          at[W - 1] = (int)th.t0 + i;
+          work(0, rx[0], rg[0], true);
+          pass(1);
+        }
+        ++i;
+      }
+    }
+    // the tokens behind the run that its own still take part in
+    int64_t behind[W];
+    Raw<T, NV> bx[W], bg[W];
+    int more = W - 1;
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+      const int64_t t = j ? behind[j - 1] + 1 : th.t1;
+      behind[j] = kMask ? token_after(th.mask, t, p.T) : t;
+      if (behind[j] < p.T) {
+        bx[j].load(th.x + behind[j] * p.x_t, th.n, th.wide);
+        bg[j].load(g + behind[j] * a.g_t, th.n, th.wide);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+      if (behind[j] >= p.T) continue;
+      --more;
+      at[W - 1] = (int)behind[j];
+      work(0, bx[j], bg[j], false);
+      pass(1);
     }
     if (more > 0) {                                    // the sequence ended: the last W - 1 tokens are the outgoing state
 #pragma unroll
@@ -270,7 +361,7 @@ __global__ void __launch_bounds__(32 * kConvWarps) conv_bwd_kernel(const __grid_
   }
   if (!a.part_w) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const size_t part = (size_t)blockIdx.z * gridDim.x + blockIdx.x;
+  const size_t part = (size_t)th.b * a.row_blocks + th.row_block;
   for (int j = 0; j <= W; ++j) {
     __syncthreads();
 #pragma unroll
@@ -283,7 +374,7 @@ __global__ void __launch_bounds__(32 * kConvWarps) conv_bwd_kernel(const __grid_
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 32 * NV; i += 32 * kConvWarps) {
-      const int ch = blockIdx.y * 32 * NV + i;
+      const int ch = th.ch_block * 32 * NV + i;
       if (ch >= p.D) continue;
       float v = 0.f;
 #pragma unroll
@@ -294,9 +385,7 @@ __global__ void __launch_bounds__(32 * kConvWarps) conv_bwd_kernel(const __grid_
   }
 }
 
-constexpr int conv_vec(int size) { return size == 2 ? 8 : 4; }
-constexpr int conv_bwd_vec(int) { return 4; }
-int conv_row_blocks(int64_t T, int run) { return (int)((T + kConvWarps * run - 1) / (kConvWarps * run)); }
+int conv_row_blocks(int64_t T) { return (int)((T + kConvWarps * kConvRun - 1) / (kConvWarps * kConvRun)); }
 
 int conv_check(const rfa_causal_conv_t* p, const char* what) {
   RFA_REQUIRE(p, RFA_EINVAL, "%s: null argument", what);
@@ -304,22 +393,16 @@ int conv_check(const rfa_causal_conv_t* p, const char* what) {
   RFA_REQUIRE(p->T > 0 && p->B > 0 && p->D > 0, RFA_EINVAL, "%s: empty or negative size", what);
   RFA_REQUIRE(p->dtype == RFA_F16 || p->dtype == RFA_F32 || p->dtype == RFA_BF16, RFA_EUNSUPPORTED, "%s: dtype %d", what, p->dtype);
   RFA_REQUIRE(p->W >= 1 && p->W <= kConvMax, RFA_EUNSUPPORTED, "%s: a window of %d tokens (1 to %d)", what, p->W, kConvMax);
-  RFA_REQUIRE(p->T < ((int64_t)1 << 31) - 64 && p->B <= 65535 && p->D <= 65535 * 128, RFA_EUNSUPPORTED, "%s: T %lld, B %d, D %d", what,
+  RFA_REQUIRE(p->T < ((int64_t)1 << 31) - 64 && p->B <= 65535 && p->T / 128 * p->D < (int64_t)1 << 37, RFA_EUNSUPPORTED, "%s: T %lld, B %d, D %d", what,
               (long long)p->T, p->B, p->D);
   return 0;
 }
 
 template <typename T, int W, bool kMask> int conv_launch(const ConvArgs& a, bool backward, cudaStream_t stream) {
-  if (backward) {
-    constexpr int NV = conv_bwd_vec(sizeof(T));
-    const dim3 grid(conv_row_blocks(a.p.T, kConvBwdRun), (a.p.D + 32 * NV - 1) / (32 * NV), a.p.B);
-    conv_bwd_kernel<T, NV, W, kMask><<<grid, 32 * kConvWarps, 0, stream>>>(a);
-    return check_launch("causal_conv_bwd");
-  }
-  constexpr int NV = conv_vec(sizeof(T));
-  const dim3 grid(conv_row_blocks(a.p.T, kConvRun), (a.p.D + 32 * NV - 1) / (32 * NV), a.p.B);
-  conv_fwd_kernel<T, NV, W, kMask><<<grid, 32 * kConvWarps, 0, stream>>>(a);
-  return check_launch("causal_conv_fwd");
+  const dim3 grid((unsigned)((int64_t)a.row_blocks * a.ch_blocks), a.p.B);
+  if (backward) conv_bwd_kernel<T, kConvVec, W, kMask><<<grid, 32 * kConvWarps, 0, stream>>>(a);
+  else conv_fwd_kernel<T, kConvVec, W, kMask><<<grid, 32 * kConvWarps, 0, stream>>>(a);
+  return check_launch(backward ? "causal_conv_bwd" : "causal_conv_fwd");
 }
 template <typename T> int conv_width(const ConvArgs& a, bool backward, cudaStream_t stream) {
   switch (a.p.W * 2 + (a.p.mask != nullptr)) {
@@ -348,16 +431,18 @@ extern "C" int rfa_causal_conv_fwd(const rfa_causal_conv_t* conv, void* y, void*
   ConvArgs a{};
   a.p = *conv;
   a.y = y; a.state_out = conv->W > 1 ? state_out : nullptr;
-  const int size = conv->dtype == RFA_F32 ? 4 : 2, nv = conv_vec(size);
+  const int size = conv->dtype == RFA_F32 ? 4 : 2, nv = kConvVec;
+  a.row_blocks = conv_row_blocks(conv->T);
+  a.ch_blocks = (conv->D + 32 * nv - 1) / (32 * nv);
   a.wide = wide_ok(conv->x, conv->x_t, conv->x_b, size, nv) && wide_ok(y, conv->D, 0, size, nv) && wide_ok(state_out, 0, 0, size, nv) &&
-           wide_ok(conv->state_in, 0, 0, size, nv);
+           wide_ok(conv->state_in, 0, 0, size, nv) && wide_ok(conv->weight, 0, 0, size, nv) && wide_ok(conv->bias, 0, 0, size, nv);
   return conv_dtype(a, false, as_stream(stream));
 }
 
 extern "C" size_t rfa_causal_conv_workspace_bytes(int64_t T, int B, int D, int W) {
   using namespace rfa;
   if (T <= 0 || B <= 0 || D <= 0 || W < 1 || W > kConvMax) return 0;
-  return (size_t)conv_row_blocks(T, kConvBwdRun) * B * D * (W + 1) * 4;
+  return (size_t)conv_row_blocks(T) * B * D * (W + 1) * 4;
 }
 
 extern "C" int rfa_causal_conv_bwd(const rfa_causal_conv_t* conv, const void* g, int64_t g_t, int64_t g_b, const void* g_state, void* gx, void* g_weight,
@@ -374,14 +459,17 @@ extern "C" int rfa_causal_conv_bwd(const rfa_causal_conv_t* conv, const void* g,
   a.g = g; a.g_t = g_t; a.g_b = g_b;
   a.gx = gx;
   if (conv->W > 1) { a.g_state = g_state; a.g_state_in = g_state_in; }
-  const int parts = conv_row_blocks(conv->T, kConvBwdRun) * conv->B;
+  const int parts = conv_row_blocks(conv->T) * conv->B;
   if (weights) {
     a.part_w = static_cast<float*>(workspace);
     a.part_b = a.part_w + (size_t)parts * conv->D * conv->W;
   }
-  const int size = conv->dtype == RFA_F32 ? 4 : 2, nv = conv_bwd_vec(size);
+  const int size = conv->dtype == RFA_F32 ? 4 : 2, nv = kConvVec;
+  a.row_blocks = conv_row_blocks(conv->T);
+  a.ch_blocks = (conv->D + 32 * nv - 1) / (32 * nv);
   a.wide = wide_ok(conv->x, conv->x_t, conv->x_b, size, nv) && wide_ok(g, g_t, g_b, size, nv) && wide_ok(gx, conv->D, 0, size, nv) &&
-           wide_ok(conv->state_in, 0, 0, size, nv) && wide_ok(a.g_state, 0, 0, size, nv) && wide_ok(a.g_state_in, 0, 0, size, nv);
+           wide_ok(conv->state_in, 0, 0, size, nv) && wide_ok(a.g_state, 0, 0, size, nv) && wide_ok(a.g_state_in, 0, 0, size, nv) &&
+           wide_ok(conv->weight, 0, 0, size, nv) && wide_ok(conv->bias, 0, 0, size, nv);
   if (int r = conv_dtype(a, true, as_stream(stream))) return r;
   const SumJob jobs[2] = {{a.part_w, g_weight, (int64_t)conv->D * conv->W, parts, conv->dtype}, {a.part_b, g_bias, conv->D, parts, conv->dtype}};
   return weights ? sum_parts(jobs, 2, as_stream(stream)) : 0;

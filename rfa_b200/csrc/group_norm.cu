@@ -3,9 +3,9 @@
 //   gx = rstd (h - mean(h) - xhat mean(h xhat)), h = gn w,  gw = sum over rows of gn xhat,  gbias = sum of gn,  ggate = g n silu'(gate).
 //
 // Bound by memory: x and gate once, y once (backward: x, gate, g; gx, ggate).  A group stays in the registers of 1 to 512 threads, with 16-byte
-// words where the sizes allow; mean and variance are two passes over registers (no difference of squares), joined by
-// shuffles, beyond a warp through shared memory.  The backward forms the statistics again rather than reading them; its threads keep
-// their channels over many rows, so that the weights' gradients stay in registers until a CTA's end, and sum_parts adds the CTAs' up.
+// words where the sizes allow; threads keep their channels, and weight and bias, over many rows, the next of which is on the way; mean and variance are two passes over registers (no difference of squares), joined by
+// shuffles, beyond a warp through shared memory.  The backward forms the statistics again rather than reading them; the
+// weights' gradients stay in registers until a CTA's end, and sum_parts adds the CTAs' up.
 #include "state_space.cuh"
 
 namespace rfa {
@@ -18,8 +18,8 @@ struct NormArgs {
   int64_t g_r;
   void *gx, *g_gate;
   float *part_w, *part_b;      // [gridDim.y][C] each
-  int size, groups_here, rows_here;      // channels of a group; groups and rows side by side in a CTA of the backward
-  bool wide;
+  int size, groups_here, rows_here;      // channels of a group; groups and rows side by side in a CTA
+  float over_size;                       // 1 / size
 };
 
 // Sum over the `TPG` threads of a group; K values at once.
@@ -46,89 +46,124 @@ template <int TPG, int K> __device__ __forceinline__ void group_sum(float* v, fl
 
 constexpr int norm_threads(int tpg) { return tpg > 256 ? tpg : tpg > 32 ? tpg : 256; }
 
-// A thread's elements of a group: vectors first + i * TPG of NV elements.
+// A thread's elements of a group: vectors first + i * TPG of NV elements; NV > 2: in wide accesses, and whole (NV divides the group).
 template <typename T, int NV, int V, int TPG> struct NormPart {
+  static constexpr bool kWide = NV > 2;
   int first;
   __device__ NormPart() : first(threadIdx.x % TPG) {}
   __device__ __forceinline__ int at(int i) const { return (first + i * TPG) * NV; }
-  __device__ __forceinline__ void load(const T* p, int size, bool wide, Raw<T, NV>* r) const {
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[i].load(p + at(i), size - at(i), wide);
-  }
-  __device__ __forceinline__ void floats(const T* p, int size, bool wide, float none, float* v) const {
+  __device__ __forceinline__ void load(const T* p, int size, Raw<T, NV>* r) const {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (p) {
-        Raw<T, NV> r;
-        r.load(p + at(i), size - at(i), wide);
-#pragma unroll
-        for (int c = 0; c < NV; ++c) v[i * NV + c] = r.get(c);
+      if (kWide) {
+        r[i].zero();
+        if (at(i) < size) r[i].load(p + at(i), NV, true);
       } else {
-#pragma unroll
-        for (int c = 0; c < NV; ++c) v[i * NV + c] = none;
+        r[i].load(p + at(i), size - at(i), false);
       }
     }
+  }
+  __device__ __forceinline__ void store(T* p, int i, int size, const Raw<T, NV>& r) const {
+    if (!kWide) r.store(p + at(i), size - at(i), false);
+    else if (at(i) < size) r.store(p + at(i), NV, true);
+  }
+  __device__ __forceinline__ void floats(const T* p, int size, float none, float* v) const {
+    Raw<T, NV> r[V];
+    if (p) load(p, size, r);
+#pragma unroll
+    for (int k = 0; k < V * NV; ++k) v[k] = p ? r[k / NV].get(k % NV) : none;
   }
 };
 
 // x -> x - mean (0 beyond the group's end); returns 1 / sqrt(variance + eps)
-template <int NV, int V, int TPG> __device__ __forceinline__ float centre(float* x, int first, int size, float eps, float (*red)[1]) {
+template <int NV, int V, int TPG> __device__ __forceinline__ float centre(float* x, int first, int size, float over_size, float eps, float (*red)[1]) {
   float sum[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < V * NV; ++i) sum[0] += x[i];     // zeros beyond the end
   group_sum<TPG, 1>(sum, red);
-  const float mean = sum[0] / (float)size;
+  const float mean = sum[0] * over_size;
   float var[1] = {0.f};
 #pragma unroll
-  for (int i = 0; i < V; ++i)
+  for (int i = 0; i < V; ++i) {
+    const bool whole = (first + i * TPG) * NV < size;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       float& v = x[i * NV + c];
-      v = (first + i * TPG) * NV + c < size ? v - mean : 0.f;
+      v = (NV > 2 ? whole : (first + i * TPG) * NV + c < size) ? v - mean : 0.f;
       var[0] = fmaf(v, v, var[0]);
     }
+  }
   group_sum<TPG, 1>(var, red);
-  return rsqrtf(var[0] / (float)size + eps);
+  return rsqrtf(fmaf(var[0], over_size, eps));
 }
+
+// Rows r0 + row0, r0 + row0 + step ... of one group: what a thread of either kernel walks, the next row on the way while one is worked on.
+struct NormPlace {
+  int group, row0, c0;
+  bool mine;
+  __device__ NormPlace(const NormArgs& a, int tpg) {
+    const int sub = threadIdx.x / tpg;
+    group = blockIdx.x * a.groups_here + sub % a.groups_here;
+    row0 = sub / a.groups_here;
+    mine = group < a.p.groups && row0 < a.rows_here;
+    c0 = mine ? group * a.size : 0;
+  }
+};
 
 template <typename T, int NV, int V, int TPG>
 __global__ void __launch_bounds__(norm_threads(TPG)) norm_fwd_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float red[32][1];
   const rfa_group_norm_t& p = a.p;
   const NormPart<T, NV, V, TPG> part;
-  const int64_t items = p.rows * p.groups, item = (int64_t)blockIdx.x * (blockDim.x / TPG) + threadIdx.x / TPG;
-  const bool there = item < items;
-  int64_t row = 0;
-  int group = 0;
-  if (there) {
-    if (items < (int64_t)1 << 31) { row = (uint32_t)item / (uint32_t)p.groups; group = (uint32_t)item % (uint32_t)p.groups; }
-    else { row = item / p.groups; group = (int)(item % p.groups); }
-  }
-  const int c0 = group * a.size, size = there ? a.size : 0;
-  Raw<T, NV> rx[V], rg[V];
-  part.load(static_cast<const T*>(p.x) + row * p.x_r + c0, size, a.wide, rx);
-  if (p.gate) part.load(static_cast<const T*>(p.gate) + row * p.gate_r + c0, size, a.wide, rg);
-  float x[V * NV], w[V * NV], bias[V * NV];
-  part.floats(p.weight ? static_cast<const T*>(p.weight) + c0 : nullptr, size, a.wide, 1.f, w);
-  part.floats(p.bias ? static_cast<const T*>(p.bias) + c0 : nullptr, size, a.wide, 0.f, bias);
+  const NormPlace at(a, TPG);
+  float w[V * NV], bias[V * NV];
+  part.floats(p.weight ? static_cast<const T*>(p.weight) + at.c0 : nullptr, at.mine ? a.size : 0, 1.f, w);
+  part.floats(p.bias ? static_cast<const T*>(p.bias) + at.c0 : nullptr, at.mine ? a.size : 0, 0.f, bias);
+  const int64_t step = (int64_t)gridDim.y * a.rows_here;
+  int64_t row = (int64_t)blockIdx.y * a.rows_here + at.row0;
+  const T* px = static_cast<const T*>(p.x) + row * p.x_r + at.c0;
+  const T* pg = p.gate ? static_cast<const T*>(p.gate) + row * p.gate_r + at.c0 : nullptr;
+  T* py = static_cast<T*>(a.y) + row * p.C + at.c0;
+  Raw<T, NV> next_x[V], next_g[V];
+  int next_size = 0;
+  const auto ask = [&]() {
+    next_size = at.mine && row < p.rows ? a.size : 0;
+    part.load(px, next_size, next_x);
+    if (p.gate) part.load(pg, next_size, next_g);
+    px += step * p.x_r;
+    if (p.gate) pg += step * p.gate_r;
+    row += step;
+  };
+  ask();
+  for (int64_t r0 = (int64_t)blockIdx.y * a.rows_here; r0 < p.rows; r0 += step, py += step * p.C) {
+    const int size = next_size;
+    float x[V * NV];
+    Raw<T, NV> rg[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i)
+    for (int i = 0; i < V; ++i) {
+      rg[i] = next_g[i];
 #pragma unroll
-    for (int c = 0; c < NV; ++c) x[i * NV + c] = rx[i].get(c);
-  const float rstd = centre<NV, V, TPG>(x, part.first, a.size, p.eps, red);
-  T* y = static_cast<T*>(a.y) + row * p.C + c0;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    Raw<T, NV> out;
-    out.zero();
-#pragma unroll
-    for (int c = 0; c < NV; ++c) {
-      const int k = i * NV + c;
-      const float n = fmaf(x[k] * rstd, w[k], bias[k]), by = p.gate ? rg[i].get(c) : n;
-      const float act = p.silu ? by * sigmoid(by) : by;
-      out.set(c, from_f<T>(p.gate ? n * act : act));
+      for (int c = 0; c < NV; ++c) x[i * NV + c] = next_x[i].get(c);
     }
-    out.store(y + part.at(i), size - part.at(i), a.wide);
+    ask();
+    const float rstd = centre<NV, V, TPG>(x, part.first, a.size, a.over_size, p.eps, red);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      Raw<T, NV> out;
+#pragma unroll
+      for (int c = 0; c < NV; c += 2) {
+        float v[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k = i * NV + c + h;
+          const float n = fmaf(x[k] * rstd, w[k], bias[k]), by = p.gate ? rg[i].get(c + h) : n;
+          const float act = p.silu ? by * sigmoid(by) : by;
+          v[h] = p.gate ? n * act : act;
+        }
+        out.set2(c / 2, v[0], v[1]);
+      }
+      part.store(py, i, size, out);
+    }
   }
 }
 
@@ -138,42 +173,59 @@ __global__ void __launch_bounds__(norm_threads(TPG)) norm_bwd_kernel(const __gri
   __shared__ float red[32][1], red2[32][2], over_rows[norm_threads(TPG)];
   const rfa_group_norm_t& p = a.p;
   const NormPart<T, NV, V, TPG> part;
-  const int sub = threadIdx.x / TPG, group = blockIdx.x * a.groups_here + sub % a.groups_here, row0 = sub / a.groups_here;
-  const bool mine = group < p.groups && row0 < a.rows_here;
-  const int c0 = mine ? group * a.size : 0;
+  const NormPlace at(a, TPG);
   float w[E], dw[E], db[E];
-  part.floats(p.weight ? static_cast<const T*>(p.weight) + c0 : nullptr, mine ? a.size : 0, a.wide, 1.f, w);
+  part.floats(p.weight ? static_cast<const T*>(p.weight) + at.c0 : nullptr, at.mine ? a.size : 0, 1.f, w);
+  Raw<T, NV> bias[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) bias[i].zero();
+  if (p.bias) part.load(static_cast<const T*>(p.bias) + at.c0, at.mine ? a.size : 0, bias);
 #pragma unroll
   for (int k = 0; k < E; ++k) dw[k] = db[k] = 0.f;
   const int64_t step = (int64_t)gridDim.y * a.rows_here;
-  for (int64_t r0 = (int64_t)blockIdx.y * a.rows_here; r0 < p.rows; r0 += step) {
-    const int64_t row = r0 + row0;
-    const int size = mine && row < p.rows ? a.size : 0;
-    Raw<T, NV> rx[V], rg[V], rz[V];
-    part.load(static_cast<const T*>(p.x) + row * p.x_r + c0, size, a.wide, rx);
-    part.load(static_cast<const T*>(a.g) + row * a.g_r + c0, size, a.wide, rg);
-    if (p.gate) part.load(static_cast<const T*>(p.gate) + row * p.gate_r + c0, size, a.wide, rz);
+  int64_t row = (int64_t)blockIdx.y * a.rows_here + at.row0;
+  const T* px = static_cast<const T*>(p.x) + row * p.x_r + at.c0;
+  const T* pu = static_cast<const T*>(a.g) + row * a.g_r + at.c0;
+  const T* pg = p.gate ? static_cast<const T*>(p.gate) + row * p.gate_r + at.c0 : nullptr;
+  int64_t out = row * p.C + at.c0;
+  Raw<T, NV> next_x[V], next_u[V], next_g[V];
+  int next_size = 0;
+  const auto ask = [&]() {
+    next_size = at.mine && row < p.rows ? a.size : 0;
+    part.load(px, next_size, next_x);
+    part.load(pu, next_size, next_u);
+    if (p.gate) part.load(pg, next_size, next_g);
+    px += step * p.x_r;
+    pu += step * a.g_r;
+    if (p.gate) pg += step * p.gate_r;
+    row += step;
+  };
+  ask();
+  for (int64_t r0 = (int64_t)blockIdx.y * a.rows_here; r0 < p.rows; r0 += step, out += step * p.C) {
+    const int size = next_size;
     float x[E], h[E];
+    Raw<T, NV> ru[V], rz[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i)
+    for (int i = 0; i < V; ++i) {
+      ru[i] = next_u[i];
+      rz[i] = next_g[i];
 #pragma unroll
-      for (int c = 0; c < NV; ++c) x[i * NV + c] = rx[i].get(c);
-    const float rstd = centre<NV, V, TPG>(x, part.first, a.size, p.eps, red);
+      for (int c = 0; c < NV; ++c) x[i * NV + c] = next_x[i].get(c);
+    }
+    ask();
+    const float rstd = centre<NV, V, TPG>(x, part.first, a.size, a.over_size, p.eps, red);
     float sums[2] = {};
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      Raw<T, NV> bias, out;
-      bias.zero();
-      out.zero();
-      if (p.bias) bias.load(static_cast<const T*>(p.bias) + c0 + part.at(i), size - part.at(i), a.wide);
+      float gg[NV];
 #pragma unroll
       for (int c = 0; c < NV; ++c) {
         const int k = i * NV + c;
-        const float xn = x[k] * rstd, n = fmaf(xn, w[k], bias.get(c)), g = rg[i].get(c);
+        const float xn = x[k] * rstd, n = fmaf(xn, w[k], bias[i].get(c)), g = ru[i].get(c);
         const float by = p.gate ? rz[i].get(c) : n, sig = p.silu ? sigmoid(by) : 1.f;
         const float slope = p.silu ? fmaf(by * sig, 1.f - sig, sig) : 1.f;      // of the activation
         const float gn = p.gate ? g * (by * sig) : g * slope;
-        if (p.gate) out.set(c, from_f<T>(g * n * slope));
+        gg[c] = g * n * slope;
         db[k] += gn;
         dw[k] = fmaf(gn, xn, dw[k]);
         x[k] = xn;
@@ -181,20 +233,24 @@ __global__ void __launch_bounds__(norm_threads(TPG)) norm_bwd_kernel(const __gri
         sums[0] += h[k];
         sums[1] = fmaf(h[k], xn, sums[1]);
       }
-      if (p.gate && a.g_gate) out.store(static_cast<T*>(a.g_gate) + row * p.C + c0 + part.at(i), size - part.at(i), a.wide);
+      if (p.gate && a.g_gate) {
+        Raw<T, NV> o;
+#pragma unroll
+        for (int c = 0; c < NV; c += 2) o.set2(c / 2, gg[c], gg[c + 1]);
+        part.store(static_cast<T*>(a.g_gate) + out, i, size, o);
+      }
     }
     group_sum<TPG, 2>(sums, red2);
-    const float mh = sums[0] / (float)a.size, mhx = sums[1] / (float)a.size;
+    const float mh = sums[0] * a.over_size, mhx = sums[1] * a.over_size;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      Raw<T, NV> out;
-      out.zero();
+      Raw<T, NV> o;
 #pragma unroll
-      for (int c = 0; c < NV; ++c) {
+      for (int c = 0; c < NV; c += 2) {
         const int k = i * NV + c;
-        out.set(c, from_f<T>(rstd * (h[k] - fmaf(x[k], mhx, mh))));
+        o.set2(c / 2, rstd * (h[k] - fmaf(x[k], mhx, mh)), rstd * (h[k + 1] - fmaf(x[k + 1], mhx, mh)));
       }
-      out.store(static_cast<T*>(a.gx) + row * p.C + c0 + part.at(i), size - part.at(i), a.wide);
+      part.store(static_cast<T*>(a.gx) + out, i, size, o);
     }
   }
   if (!a.part_w) return;
@@ -206,20 +262,20 @@ __global__ void __launch_bounds__(norm_threads(TPG)) norm_bwd_kernel(const __gri
         __syncthreads();
         over_rows[threadIdx.x] = v;
         __syncthreads();
-        if (row0 == 0)
+        if (at.row0 == 0)
           for (int r = 1; r < a.rows_here; ++r) v += over_rows[threadIdx.x + r * a.groups_here * TPG];
       }
-      const int at = part.at(k / NV) + k % NV;
-      if (mine && row0 == 0 && at < a.size) (pass ? a.part_b : a.part_w)[(size_t)blockIdx.y * p.C + c0 + at] = v;
+      const int c = part.at(k / NV) + k % NV;
+      if (at.mine && at.row0 == 0 && c < a.size) (pass ? a.part_b : a.part_w)[(size_t)blockIdx.y * p.C + at.c0 + c] = v;
     }
   }
 }
 
-// The rows that one CTA of the backward takes side by side, and how many CTAs share the rows.
+// The groups and rows that a CTA takes side by side, and how many CTAs share the rows.
 struct NormGrid {
   int nv, tpg, v, groups_here, rows_here, x, y;
 };
-NormGrid norm_grid(int64_t rows, int C, int groups, int nv) {
+NormGrid norm_grid(int64_t rows, int C, int groups, int nv, bool backward) {
   NormGrid s{};
   s.nv = nv;
   const int n = (C / groups + nv - 1) / nv;            // vectors of a group
@@ -231,21 +287,16 @@ NormGrid norm_grid(int64_t rows, int C, int groups, int nv) {
   s.groups_here = groups < subs ? groups : subs;
   s.rows_here = subs / s.groups_here;
   s.x = (groups + s.groups_here - 1) / s.groups_here;
-  const int64_t most = (rows + s.rows_here - 1) / s.rows_here, want = 148 * 4 / s.x > 1 ? 148 * 4 / s.x : 1;
+  const int64_t most = (rows + s.rows_here - 1) / s.rows_here, ctas = 148 * (backward ? 4 : 8), want = ctas / s.x > 1 ? ctas / s.x : 1;
   s.y = (int)(most < want ? most : want);
   return s;
 }
 
 template <typename T, int NV, int V, int TPG> int norm_launch(const NormArgs& a, const NormGrid& s, cudaStream_t stream) {
   constexpr int threads = norm_threads(TPG);
-  if (a.g) {
-    norm_bwd_kernel<T, NV, V, TPG><<<dim3(s.x, s.y), threads, 0, stream>>>(a);
-    return check_launch("group_norm_bwd");
-  }
-  const int64_t blocks = (a.p.rows * a.p.groups + threads / TPG - 1) / (threads / TPG);
-  RFA_REQUIRE(blocks < (int64_t)1 << 31, RFA_EUNSUPPORTED, "group_norm_fwd: too many rows");
-  norm_fwd_kernel<T, NV, V, TPG><<<(unsigned)blocks, threads, 0, stream>>>(a);
-  return check_launch("group_norm_fwd");
+  if (a.g) norm_bwd_kernel<T, NV, V, TPG><<<dim3(s.x, s.y), threads, 0, stream>>>(a);
+  else norm_fwd_kernel<T, NV, V, TPG><<<dim3(s.x, s.y), threads, 0, stream>>>(a);
+  return check_launch(a.g ? "group_norm_bwd" : "group_norm_fwd");
 }
 template <typename T, int NV> int norm_shape(const NormArgs& a, const NormGrid& s, cudaStream_t stream) {
   switch (s.tpg * 32 + s.v) {
@@ -270,10 +321,11 @@ int norm_run(NormArgs a, const char* what, void* workspace, size_t workspace_byt
   RFA_REQUIRE(p.C % p.groups == 0 && p.C / p.groups <= 16384, RFA_EUNSUPPORTED, "%s: %d channels in %d groups (of at most 16384)", what, p.C, p.groups);
   a.size = p.C / p.groups;
   const int bytes = p.dtype == RFA_F32 ? 4 : 2, nv = bytes == 2 ? 8 : 4;
-  a.wide = a.size % nv == 0 && wide_ok(p.x, p.x_r, 0, bytes, nv) && wide_ok(p.gate, p.gate ? p.gate_r : 0, 0, bytes, nv) && wide_ok(a.y, 0, 0, bytes, nv) &&
+  a.over_size = 1.f / (float)a.size;
+  const bool wide = a.size % nv == 0 && wide_ok(p.x, p.x_r, p.C, bytes, nv) && wide_ok(p.gate, p.gate ? p.gate_r : 0, 0, bytes, nv) && wide_ok(a.y, 0, 0, bytes, nv) &&
            wide_ok(p.weight, 0, 0, bytes, nv) && wide_ok(p.bias, 0, 0, bytes, nv) && wide_ok(a.g, a.g_r, 0, bytes, nv) && wide_ok(a.gx, 0, 0, bytes, nv) &&
            wide_ok(a.g_gate, 0, 0, bytes, nv);
-  const NormGrid s = norm_grid(p.rows, p.C, p.groups, a.wide ? nv : 2);
+  const NormGrid s = norm_grid(p.rows, p.C, p.groups, wide ? nv : 2, a.g);
   a.groups_here = s.groups_here; a.rows_here = s.rows_here;
   if (g_weight || g_bias) {
     const size_t need = rfa_group_norm_workspace_bytes(p.rows, p.C, p.groups);
@@ -282,9 +334,9 @@ int norm_run(NormArgs a, const char* what, void* workspace, size_t workspace_byt
     a.part_b = a.part_w + (size_t)s.y * p.C;
   }
   int r;
-  if (p.dtype == RFA_F32) r = a.wide ? norm_shape<float, 4>(a, s, stream) : norm_shape<float, 2>(a, s, stream);
-  else if (p.dtype == RFA_F16) r = a.wide ? norm_shape<__half, 8>(a, s, stream) : norm_shape<__half, 2>(a, s, stream);
-  else r = a.wide ? norm_shape<__nv_bfloat16, 8>(a, s, stream) : norm_shape<__nv_bfloat16, 2>(a, s, stream);
+  if (p.dtype == RFA_F32) r = wide ? norm_shape<float, 4>(a, s, stream) : norm_shape<float, 2>(a, s, stream);
+  else if (p.dtype == RFA_F16) r = wide ? norm_shape<__half, 8>(a, s, stream) : norm_shape<__half, 2>(a, s, stream);
+  else r = wide ? norm_shape<__nv_bfloat16, 8>(a, s, stream) : norm_shape<__nv_bfloat16, 2>(a, s, stream);
   if (r || !a.part_w) return r;
   const SumJob jobs[2] = {{a.part_w, g_weight, p.C, s.y, p.dtype}, {a.part_b, g_bias, p.C, s.y, p.dtype}};
   return sum_parts(jobs, 2, stream);
@@ -307,7 +359,7 @@ extern "C" size_t rfa_group_norm_workspace_bytes(int64_t rows, int C, int groups
   if (rows <= 0 || C <= 0 || groups <= 0 || C % groups) return 0;
   int y = 1;
   for (int nv : {2, 4, 8}) {
-    const NormGrid s = norm_grid(rows, C, groups, nv);
+    const NormGrid s = norm_grid(rows, C, groups, nv, true);
     y = s.y > y ? s.y : y;
   }
   return (size_t)2 * y * C * 4;

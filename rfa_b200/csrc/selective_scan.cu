@@ -147,8 +147,7 @@ __device__ __forceinline__ void fwd_bring(const FwdArgs& A, FwdSmem<LN>& sm, con
       const bool on = here >> i & 1;
       Raw<T, 2> out;
       out.zero();
-      out.set(0, from_f<T>(on ? fmaf(skip[0], kept.v[i].get(0), f.x) : 0.f));
-      out.set(1, from_f<T>(on ? fmaf(skip[1], kept.v[i].get(1), f.y) : 0.f));
+      out.set2(0, on ? fmaf(skip[0], kept.v[i].get(0), f.x) : 0.f, on ? fmaf(skip[1], kept.v[i].get(1), f.y) : 0.f);
       out.store(y + (t0 + t) * y_t, th.vn, A.wide);
     }
   };
@@ -289,42 +288,53 @@ __device__ __forceinline__ void store4(float* p, int n, bool wide, const float* 
 }
 
 // ---- one token ---------------------------------------------------------------------------------------------------------------
-// Bound by the state's way from memory and back, 8 bytes per element.  LN lanes a channel, four states (one 16-byte word) each.
-template <typename T, int LN, bool kWide>
-__global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ rfa_scan_t p, T* y, float* state) {
-  const int at_ch = (blockIdx.x * 256 + threadIdx.x) / LN, n0 = 4 * (threadIdx.x % LN), b = blockIdx.y;
+// Bound by the state's way from memory and back, 8 bytes per element.  LN lanes a channel, four adjacent states (one 16-byte word) each; a
+// thread has one channel of kRows batch rows, all of whose loads are on the way at once, so that a, the group and the addresses are
+// found once for them.
+template <typename T, int LN, int kRows>
+__global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ rfa_scan_t p, T* y, float* state, bool wide, bool wide_bc) {
+  const int at_ch = (blockIdx.x * 256 + threadIdx.x) / LN, n0 = 4 * (threadIdx.x % LN), b0 = blockIdx.y * kRows;
   const bool there = at_ch < p.D;
-  const int ch = there ? at_ch : 0, n = there ? max(0, min(4, p.N - n0)) : 0;
-  const int64_t item = (int64_t)b * p.D + ch;
-  const bool gone = p.mask && p.mask[b];
-  float s[4], a[4];
-  float* at = state + item * p.N + n0;
-  load4(at, n, kWide, s);
-  load4(p.a + (size_t)ch * p.N + n0, n, kWide, a);
-  const int g = ch / (p.D / p.G);
-  const T* bp = static_cast<const T*>(p.b) + (int64_t)b * p.b_b + (int64_t)g * p.b_g + n0;
-  const T* cp = static_cast<const T*>(p.c) + (int64_t)b * p.c_b + (int64_t)g * p.c_g + n0;
-  float bt[4], ct[4];
+  const int ch = there ? at_ch : 0, n = there ? max(0, min(4, p.N - n0)) : 0, rows = min(kRows, p.B - b0);
+  const int g = p.G == 1 ? 0 : ch / (p.D / p.G);
+  const T* bp = static_cast<const T*>(p.b) + (int64_t)g * p.b_g + n0;
+  const T* cp = static_cast<const T*>(p.c) + (int64_t)g * p.c_g + n0;
+  float* at = state + ((int64_t)b0 * p.D + ch) * p.N + n0;
+  const int64_t row = (int64_t)p.D * p.N;
+  float s[kRows][4], a[4];
+  Raw<T, 4> rb[kRows], rc[kRows];
+  T x[kRows], dt[kRows];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    bt[j] = j < n ? to_f(bp[j]) : 0.f;
-    ct[j] = j < n ? to_f(cp[j]) : 0.f;
+  for (int r = 0; r < kRows; ++r) {
+    const int b = b0 + (r < rows ? r : 0);             // a row that is not there: another's loads, nothing stored
+    load4(at + (b - b0) * row, n, wide, s[r]);
+    x[r] = static_cast<const T*>(p.x)[(int64_t)b * p.x_b + ch];
+    dt[r] = static_cast<const T*>(p.dt)[(int64_t)b * p.dt_b + ch];
+    rb[r].load(bp + (int64_t)b * p.b_b, n, wide_bc);
+    rc[r].load(cp + (int64_t)b * p.c_b, n, wide_bc);
   }
-  const float x = to_f(static_cast<const T*>(p.x)[(int64_t)b * p.x_b + ch]);
-  float delta = to_f(static_cast<const T*>(p.dt)[(int64_t)b * p.dt_b + ch]) + (p.dt_bias ? p.dt_bias[ch] : 0.f), sig;
-  if (p.softplus) delta = softplus(delta, sig);
-  const float dx = delta * x;
-  float out = 0.f;
+  load4(p.a + (size_t)ch * p.N + n0, n, wide, a);
+  const float bias = p.dt_bias ? p.dt_bias[ch] : 0.f, skip = p.d ? p.d[ch] : 0.f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    s[j] = fmaf(ex2(delta * (a[j] * kLog2e)), s[j], dx * bt[j]);
-    out = fmaf(s[j], ct[j], out);
+  for (int j = 0; j < 4; ++j) a[j] *= kLog2e;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const float xv = to_f(x[r]);
+    float delta = to_f(dt[r]) + bias, sig, out = 0.f;
+    if (p.softplus) delta = softplus(delta, sig);
+    const float dx = delta * xv;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[r][j] = fmaf(ex2(delta * a[j]), s[r][j], dx * rb[r].get(j));
+      out = fmaf(s[r][j], rc[r].get(j), out);
+    }
+#pragma unroll
+    for (int o = LN / 2; o > 0; o >>= 1) out += __shfl_xor_sync(0xffffffffu, out, o);
+    if (r >= rows || !there) continue;
+    const bool gone = p.mask && p.mask[b0 + r];
+    if (!gone) store4(at + r * row, n, wide, s[r]);
+    if (n0 == 0) y[(int64_t)(b0 + r) * p.D + ch] = from_f<T>(gone ? 0.f : p.d ? fmaf(skip, xv, out) : out);
   }
-#pragma unroll
-  for (int o = LN / 2; o > 0; o >>= 1) out += __shfl_xor_sync(0xffffffffu, out, o);
-  if (!there) return;
-  if (!gone) store4(at, n, kWide, s);
-  if (n0 == 0) y[item] = from_f<T>(gone ? 0.f : p.d ? fmaf(p.d[ch], x, out) : out);
 }
 
 }  // namespace
@@ -363,12 +373,17 @@ extern "C" int rfa_selective_scan_step(const rfa_scan_t* scan, void* y, float* s
   RFA_REQUIRE(y && s, RFA_EINVAL, "selective_scan_step: null pointer");
   RFA_REQUIRE(scan->T == 1, RFA_EINVAL, "selective_scan_step: %lld tokens", (long long)scan->T);
   RFA_REQUIRE(aligned16(s), RFA_EALIGN, "selective_scan_step: s is not 16-byte aligned");
+  const int size = scan->dtype == RFA_F32 ? 4 : 2;
   const bool wide = scan->N % 4 == 0 && aligned16(scan->a);
-#define CALL(T, LN)                                                                                                       \
-  do {                                                                                                                    \
-    const dim3 grid((unsigned)(((int64_t)scan->D * LN + 255) / 256), scan->B);                                            \
-    if (wide) scan_step_kernel<T, LN, true><<<grid, 256, 0, as_stream(stream)>>>(*scan, static_cast<T*>(y), s);           \
-    else scan_step_kernel<T, LN, false><<<grid, 256, 0, as_stream(stream)>>>(*scan, static_cast<T*>(y), s);               \
+  const bool wide_bc = wide_ok(scan->b, scan->b_b, scan->b_g, size, 4) && wide_ok(scan->c, scan->c_b, scan->c_g, size, 4);
+  // Four rows a thread from eight CTAs of one row per SM on; below, all SMs are wanted.
+#define CALL(T, LN)                                                                                                          \
+  do {                                                                                                                       \
+    const unsigned x = (unsigned)(((int64_t)scan->D * LN + 255) / 256);                                                      \
+    if ((int64_t)x * scan->B >= 8 * 148)                                                                                     \
+      scan_step_kernel<T, LN, 4><<<dim3(x, (scan->B + 3) / 4), 256, 0, as_stream(stream)>>>(*scan, static_cast<T*>(y), s, wide, wide_bc); \
+    else                                                                                                                     \
+      scan_step_kernel<T, LN, 1><<<dim3(x, scan->B), 256, 0, as_stream(stream)>>>(*scan, static_cast<T*>(y), s, wide, wide_bc);           \
   } while (0)
   RFA_SCAN_DISPATCH(scan->dtype, scan_lanes(scan->N), CALL);
 #undef CALL

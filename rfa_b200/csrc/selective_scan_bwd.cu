@@ -200,14 +200,17 @@ __device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, con
         const float4 in = sm.in[buf][t][th.vpair], res = sm.res[t][th.vpair];
         const float2 gv = sm.g[buf][t][th.vpair], sv = sm.slope[buf][t][th.vpair];
         const float delta[2] = {in.x, in.y}, gt[2] = {gv.x, gv.y}, sig[2] = {sv.x, sv.y}, gu[2] = {res.x, res.y}, gp[2] = {res.z, res.w};
+        float v[2], vx[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float xv = kept.v[i].get(k), v = fmaf(xv, gu[k], kLn2 * gp[k]) * sig[k];
-          ox.set(k, from_f<T>(fmaf(delta[k], gu[k], skip[k] * gt[k])));
-          od.set(k, from_f<T>(v));
+          const float xv = kept.v[i].get(k);
+          v[k] = fmaf(xv, gu[k], kLn2 * gp[k]) * sig[k];
+          vx[k] = fmaf(delta[k], gu[k], skip[k] * gt[k]);
           gd[k] = fmaf(xv, gt[k], gd[k]);
-          gbias[k] += v;
+          gbias[k] += v[k];
         }
+        ox.set2(0, vx[0], vx[1]);
+        od.set2(0, v[0], v[1]);
       }
       ox.store(static_cast<T*>(A.gx) + (t0 + t) * row_stride + out0, th.vn, A.wide);
       od.store(static_cast<T*>(A.gdt) + (t0 + t) * row_stride + out0, th.vn, A.wide);

@@ -4,6 +4,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace rfa {
@@ -21,61 +23,86 @@ struct Raw {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = 0;
   }
-  // `wide`: the address is a multiple of the run's size (at most 16 bytes); n elements are there
+  static constexpr int kStep = kWords % 4 == 0 ? 4 : kWords % 2 == 0 ? 2 : 1;      // words of a wide access
+  // `wide`: the address is a multiple of a wide access; n elements are there
   __device__ __forceinline__ void load(const T* p, int n, bool wide) {
     if (wide && n >= NV) {
-      if constexpr (kWords % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < kWords; i += 4) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+      for (int i = 0; i < kWords; i += kStep) {
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(p) + i;
+        if constexpr (kStep == 4) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
           w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+        } else if constexpr (kStep == 2) {
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+          w[i] = v.x; w[i + 1] = v.y;
+        } else {
+          w[i] = __ldg(at);
         }
-      } else if constexpr (kWords == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        w[0] = v.x; w[1] = v.y;
-      } else {
-        w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) set(i, i < n ? p[i] : from_f<T>(0.f));
+      for (int i = 0; i < NV; ++i) put_bits(i, i < n ? p[i] : from_f<T>(0.f));
     }
   }
-  __device__ __forceinline__ void set(int i, T v) {
+  // Elements in pairs: a conversion of one alone goes to the special function unit, which has enough to do.
+  __device__ __forceinline__ float2 get2(int k) const {
     if constexpr (sizeof(T) == 4) {
-      w[i] = __float_as_uint(to_f(v));
+      return make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+    } else if constexpr (std::is_same_v<T, __half>) {
+      return __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+    } else {
+      return make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+    }
+  }
+  __device__ __forceinline__ void set2(int k, float a, float b) {
+    if constexpr (sizeof(T) == 4) {
+      w[2 * k] = __float_as_uint(a);
+      w[2 * k + 1] = __float_as_uint(b);
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const __half2 h = __floats2half2_rn(a, b);
+      w[k] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+      w[k] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  __device__ __forceinline__ float get(int i) const { return i & 1 ? get2(i / 2).y : get2(i / 2).x; }
+  // element i as it stands in memory
+  __device__ __forceinline__ T bits(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else {
+      const uint16_t h = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffff;
+      return *reinterpret_cast<const T*>(&h);
+    }
+  }
+  __device__ __forceinline__ void put_bits(int i, T v) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(v);
     } else {
       const uint32_t h = *reinterpret_cast<const uint16_t*>(&v);
       w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | h << 16 : (w[i / 2] & 0xffff0000u) | h;
     }
   }
-  __device__ __forceinline__ float get(int i) const {
-    if constexpr (sizeof(T) == 4) {
-      return __uint_as_float(w[i]);
-    } else {
-      const uint16_t h = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffff;
-      return to_f(*reinterpret_cast<const T*>(&h));
-    }
-  }
   __device__ __forceinline__ void store(T* p, int n, bool wide) const {
     if (wide && n >= NV) {
-      if constexpr (kWords % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < kWords; i += 4) reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-      } else if constexpr (kWords == 2) {
-        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-      } else {
-        *reinterpret_cast<uint32_t*>(p) = w[0];
+      for (int i = 0; i < kWords; i += kStep) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(p) + i;
+        if constexpr (kStep == 4) *reinterpret_cast<uint4*>(at) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        else if constexpr (kStep == 2) *reinterpret_cast<uint2*>(at) = make_uint2(w[i], w[i + 1]);
+        else *at = w[i];
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (i < n) p[i] = from_f<T>(get(i));
+        if (i < n) p[i] = bits(i);
     }
   }
 };
 
-// Whether runs of NV elements at p, p + stride ... may be taken as wide words.
+// Whether runs of NV elements at p, p + stride ... may be taken in wide accesses (of at most 16 bytes).
 inline bool wide_ok(const void* p, int64_t stride, int64_t stride2, int size, int nv) {
   const int64_t bytes = nv * size < 16 ? nv * size : 16;
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0 && stride2 * size % bytes == 0;
