@@ -160,37 +160,39 @@ __global__ void __launch_bounds__(32 * kConvWarps) conv_fwd_kernel(const __grid_
       for (int c = 0; c < NV; ++c) win[j][c] = win[j + by][c];
   };
   Raw<T, NV> raw[kConvFlight];
-  const auto ask = [&](int i) {
-    const T* at = from + i * p.x_t;
+  const auto ask = [&](const T* at) {
 #pragma unroll
     for (int k = 0; k < kConvFlight; ++k, at += p.x_t) raw[k].load(at, th.n, th.wide);
   };
+  const auto four = [&](int i) { return kMask ? four_there(there, i) : i + kConvFlight <= count; };
   bool on_way = false;
   for (int i = 0; i < count;) {
-    if (four_there(there, i)) {                        // four tokens together, the next four on the way
-      if (!on_way) ask(i);
+    if (four(i)) {                                     // four tokens together, the next four on the way
+      if (!on_way) ask(from);
+      from += kConvFlight * p.x_t;
 #pragma unroll
       for (int k = 0; k < kConvFlight; ++k)
 #pragma unroll
         for (int c = 0; c < NV; ++c) win[W - 1 + k][c] = raw[k].get(c);
-      on_way = four_there(there, i + kConvFlight);
-      if (on_way) ask(i + kConvFlight);
-      T* out_at = to + i * out_t;
-#pragma unroll
-      for (int k = 0; k < kConvFlight; ++k, out_at += out_t) put(k, out_at);
-      move(kConvFlight);
       i += kConvFlight;
+      on_way = four(i);
+      if (on_way) ask(from);
+#pragma unroll
+      for (int k = 0; k < kConvFlight; ++k, to += out_t) put(k, to);
+      move(kConvFlight);
     } else {
-      if (there >> i & 1) {
-        load_row<T, NV>(from + i * p.x_t, th.n, th.wide, win[W - 1]);
-        put(0, to + i * out_t);
+      if (!kMask || (there >> i & 1)) {
+        load_row<T, NV>(from, th.n, th.wide, win[W - 1]);
+        put(0, to);
         move(1);
       } else {
         Raw<T, NV> none;
         none.zero();
-        none.store(to + i * out_t, th.n, th.wide);
+        none.store(to, th.n, th.wide);
       }
       ++i;
+      from += p.x_t;
+      to += out_t;
     }
   }
   if (last) {
@@ -290,39 +292,57 @@ __global__ void __launch_bounds__(32 * kConvWarps) conv_bwd_kernel(const __grid_
     };
     const T *from_x = th.x + th.t0 * p.x_t, *from_g = g + th.t0 * a.g_t;
     Raw<T, NV> rx[kConvFlight], rg[kConvFlight];
-    const auto ask = [&](int i) {
-      const T *at_x = from_x + i * p.x_t, *at_g = from_g + i * a.g_t;
+    const auto ask = [&](const T* at_x, const T* at_g) {
 #pragma unroll
       for (int k = 0; k < kConvFlight; ++k, at_x += p.x_t, at_g += a.g_t) {
         rx[k].load(at_x, th.n, th.wide);
         rg[k].load(at_g, th.n, th.wide);
       }
     };
+    const auto four = [&](int i) { return kMask ? four_there(there, i) : i + kConvFlight <= count; };
     bool on_way = false;
     for (int i = 0; i < count;) {
-      if (four_there(there, i)) {                      // four tokens together, the next four on the way
-        if (!on_way) ask(i);
+      if (four(i)) {                                   // four tokens together, the next four on the way
+        if (!on_way) ask(from_x, from_g);
         Raw<T, NV> ux[kConvFlight], ug[kConvFlight];
 #pragma unroll
         for (int k = 0; k < kConvFlight; ++k) { ux[k] = rx[k]; ug[k] = rg[k]; }
-        on_way = four_there(there, i + kConvFlight);
-        if (on_way) ask(i + kConvFlight);
+        from_x += kConvFlight * p.x_t;
+        from_g += kConvFlight * a.g_t;
+        on_way = four(i + kConvFlight);
+        if (on_way) ask(from_x, from_g);
 #pragma unroll
         for (int k = 0; k < kConvFlight; ++k) {
           at[W - 1 + k] = (int)th.t0 + i + k;
           work(k, ux[k], ug[k], true);
         }
-        pass(kConvFlight);
+        if (!kMask && i >= W - 1) {                    // four of the run's own, side by side
+          T* to = gx + (th.t0 + i - (W - 1)) * out_t;
+#pragma unroll
+          for (int k = 0; k < kConvFlight; ++k, to += out_t) {
+            Raw<T, NV> out;
+#pragma unroll
+            for (int c = 0; c < NV; c += 2) out.set2(c / 2, pend[k][c], pend[k][c + 1]);
+            out.store(to, th.n, th.wide);
+          }
+          move(kConvFlight);
+#pragma unroll
+          for (int j = 0; j < W - 1; ++j) at[j] = at[j + kConvFlight];
+        } else {
+          pass(kConvFlight);
+        }
         i += kConvFlight;
       } else {
-        if (there >> i & 1) {
-          rx[0].load(from_x + i * p.x_t, th.n, th.wide);
-          rg[0].load(from_g + i * a.g_t, th.n, th.wide);
+        if (!kMask || (there >> i & 1)) {
+          rx[0].load(from_x, th.n, th.wide);
+          rg[0].load(from_g, th.n, th.wide);
           at[W - 1] = (int)th.t0 + i;
           work(0, rx[0], rg[0], true);
           pass(1);
         }
         ++i;
+        from_x += p.x_t;
+        from_g += a.g_t;
       }
     }
     // the tokens behind the run that its own still take part in

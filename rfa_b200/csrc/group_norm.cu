@@ -77,6 +77,7 @@ template <typename T, int NV, int V, int TPG> struct NormPart {
 
 // x -> x - mean (0 beyond the group's end); returns 1 / sqrt(variance + eps)
 template <int NV, int V, int TPG> __device__ __forceinline__ float centre(float* x, int first, int size, float over_size, float eps, float (*red)[1]) {
+  const bool full = size == TPG * V * NV;              // for all threads: nothing lies beyond the end
   float sum[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < V * NV; ++i) sum[0] += x[i];     // zeros beyond the end
@@ -84,15 +85,14 @@ template <int NV, int V, int TPG> __device__ __forceinline__ float centre(float*
   const float mean = sum[0] * over_size;
   float var[1] = {0.f};
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const bool whole = (first + i * TPG) * NV < size;
+  for (int k = 0; k < V * NV; ++k) x[k] -= mean;
+  if (!full) {
 #pragma unroll
-    for (int c = 0; c < NV; ++c) {
-      float& v = x[i * NV + c];
-      v = (NV > 2 ? whole : (first + i * TPG) * NV + c < size) ? v - mean : 0.f;
-      var[0] = fmaf(v, v, var[0]);
-    }
+    for (int k = 0; k < V * NV; ++k)
+      if ((first + k / NV * TPG) * NV + k % NV >= size) x[k] = 0.f;
   }
+#pragma unroll
+  for (int k = 0; k < V * NV; ++k) var[0] = fmaf(x[k], x[k], var[0]);
   group_sum<TPG, 1>(var, red);
   return rsqrtf(fmaf(var[0], over_size, eps));
 }
@@ -149,19 +149,27 @@ __global__ void __launch_bounds__(norm_threads(TPG)) norm_fwd_kernel(const __gri
     const float rstd = centre<NV, V, TPG>(x, part.first, a.size, a.over_size, p.eps, red);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
+      float n[NV], v[NV];                              // v: what the activation is of, then the result (branches that a call takes one way)
+#pragma unroll
+      for (int c = 0; c < NV; ++c) n[c] = fmaf(x[i * NV + c] * rstd, w[i * NV + c], bias[i * NV + c]);
+      if (p.gate) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) v[c] = rg[i].get(c);
+      } else {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) v[c] = n[c];
+      }
+      if (p.silu) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) v[c] *= sigmoid(v[c]);
+      }
+      if (p.gate) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) v[c] *= n[c];
+      }
       Raw<T, NV> out;
 #pragma unroll
-      for (int c = 0; c < NV; c += 2) {
-        float v[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int k = i * NV + c + h;
-          const float n = fmaf(x[k] * rstd, w[k], bias[k]), by = p.gate ? rg[i].get(c + h) : n;
-          const float act = p.silu ? by * sigmoid(by) : by;
-          v[h] = p.gate ? n * act : act;
-        }
-        out.set2(c / 2, v[0], v[1]);
-      }
+      for (int c = 0; c < NV; c += 2) out.set2(c / 2, v[c], v[c + 1]);
       part.store(py, i, size, out);
     }
   }
@@ -217,27 +225,52 @@ __global__ void __launch_bounds__(norm_threads(TPG)) norm_bwd_kernel(const __gri
     float sums[2] = {};
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      float gg[NV];
+      float n[NV], act[NV], slope[NV], gn[NV];         // act, slope: the activation and its derivative (branches that a call takes one way)
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        x[i * NV + c] *= rstd;
+        n[c] = fmaf(x[i * NV + c], w[i * NV + c], bias[i].get(c));
+        gn[c] = ru[i].get(c);
+      }
+      if (p.gate) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) act[c] = rz[i].get(c);
+      } else {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) act[c] = n[c];
+      }
+      if (p.silu) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+          const float sig = sigmoid(act[c]);
+          act[c] *= sig;
+          slope[c] = fmaf(act[c], 1.f - sig, sig);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) slope[c] = 1.f;
+      }
+      if (p.gate) {
+        if (a.g_gate) {
+          Raw<T, NV> o;
+#pragma unroll
+          for (int c = 0; c < NV; c += 2) o.set2(c / 2, gn[c] * n[c] * slope[c], gn[c + 1] * n[c + 1] * slope[c + 1]);
+          part.store(static_cast<T*>(a.g_gate) + out, i, size, o);
+        }
+#pragma unroll
+        for (int c = 0; c < NV; ++c) gn[c] *= act[c];
+      } else {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) gn[c] *= slope[c];
+      }
 #pragma unroll
       for (int c = 0; c < NV; ++c) {
         const int k = i * NV + c;
-        const float xn = x[k] * rstd, n = fmaf(xn, w[k], bias[i].get(c)), g = ru[i].get(c);
-        const float by = p.gate ? rz[i].get(c) : n, sig = p.silu ? sigmoid(by) : 1.f;
-        const float slope = p.silu ? fmaf(by * sig, 1.f - sig, sig) : 1.f;      // of the activation
-        const float gn = p.gate ? g * (by * sig) : g * slope;
-        gg[c] = g * n * slope;
-        db[k] += gn;
-        dw[k] = fmaf(gn, xn, dw[k]);
-        x[k] = xn;
-        h[k] = gn * w[k];
+        db[k] += gn[c];
+        dw[k] = fmaf(gn[c], x[k], dw[k]);
+        h[k] = gn[c] * w[k];
         sums[0] += h[k];
-        sums[1] = fmaf(h[k], xn, sums[1]);
-      }
-      if (p.gate && a.g_gate) {
-        Raw<T, NV> o;
-#pragma unroll
-        for (int c = 0; c < NV; c += 2) o.set2(c / 2, gg[c], gg[c + 1]);
-        part.store(static_cast<T*>(a.g_gate) + out, i, size, o);
+        sums[1] = fmaf(h[k], x[k], sums[1]);
       }
     }
     group_sum<TPG, 2>(sums, red2);
