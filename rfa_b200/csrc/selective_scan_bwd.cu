@@ -272,16 +272,16 @@ __device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, con
       const int w = part & 1;
       meet_wait<kBwdThreads>(kSums + w);
       sum(t0, part, w);
+      if (tile > tile0 || part > 1) meet_go<kBwdThreads>(kTaken + w);      // somebody waits for it (and reaches this part's rows of res four parts on)
       take(t0, buf, part);
-      if (tile > tile0 || part > 1) meet_go<kBwdThreads>(kTaken + w);      // somebody waits for it
     }
     kept = x_next;
     here = here_next;
   }
 
   const size_t row = (size_t)th.b * sh.segs + seg;
-  // gd and gbias over the rows of loading threads, where the scanning warps have nothing left to read: they handed over their last part
-  float4* over_rows = &sm.in[0][0][0];
+  // gd and gbias over the rows of bringing threads, where the scanning warps, done with their last part, kept their states
+  float4* over_rows = reinterpret_cast<float4*>(&sm.start[0][0][0]);
   over_rows[th.tid] = make_float4(gd[0], gd[1], gbias[0], gbias[1]);
   asm volatile("bar.sync 9, %0;" ::"n"(kBwdBring) : "memory");
   if (th.row == 0) {
