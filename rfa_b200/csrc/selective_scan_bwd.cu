@@ -31,6 +31,7 @@ template <int LN> struct __align__(16) BwdSmem {
   float b[2][kScanTile][Tile::kN], c[2][kScanTile][Tile::kN];
   float4 res[kScanTile][Tile::kPairs];                 // sum_n G b of both channels, sum_n a log2(e) p of both
   ulonglong2 start[kScanTile / kRun][2 * kP][kBwdScan];     // each thread's states in front of a run
+  ulonglong2 da[2 * kP][kBwdScan];                     // each thread's ga: tiles are summed apart (one chain of 2048 tokens is 1e-6 off)
   float4 over_ch[2][kPart][2][kThreads][LN];           // gb and gc of each thread's channels, a lane's four states adjacent; two parts by turns
 };
 // Further places where the halves of a CTA meet: a part's sums are there, have been taken.
@@ -152,7 +153,7 @@ __device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, con
   const T* cp = static_cast<const T*>(p.c) + (int64_t)th.b * p.c_b + (int64_t)th.group * p.c_g;
   const uint8_t* mask = p.mask ? p.mask + (int64_t)th.b * sh.T : nullptr;
   const int64_t row_stride = (int64_t)sh.B * sh.D, out0 = (int64_t)th.b * sh.D + ch;
-  float bias[2], skip[2], gd[2] = {}, gbias[2] = {};
+  float bias[2], skip[2], gd[2] = {}, gbias[2] = {}, tile_gd[2] = {}, tile_gbias[2] = {};
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     bias[k] = p.dt_bias && k < th.vn ? p.dt_bias[ch + k] : 0.f;
@@ -206,8 +207,8 @@ __device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, con
           const float xv = kept.v[i].get(k);
           v[k] = fmaf(xv, gu[k], kLn2 * gp[k]) * sig[k];
           vx[k] = fmaf(delta[k], gu[k], skip[k] * gt[k]);
-          gd[k] = fmaf(xv, gt[k], gd[k]);
-          gbias[k] += v[k];
+          tile_gd[k] = fmaf(xv, gt[k], tile_gd[k]);
+          tile_gbias[k] += v[k];
         }
         ox.set2(0, vx[0], vx[1]);
         od.set2(0, v[0], v[1]);
@@ -275,6 +276,12 @@ __device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, con
       if (tile > tile0 || part > 1) meet_go<kBwdThreads>(kTaken + w);      // somebody waits for it (and reaches this part's rows of res four parts on)
       take(t0, buf, part);
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      gd[k] += tile_gd[k];
+      gbias[k] += tile_gbias[k];
+      tile_gd[k] = tile_gbias[k] = 0.f;
+    }
     kept = x_next;
     here = here_next;
   }
@@ -322,6 +329,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_c
       G[k][j] = A.g_s ? th.get(A.g_s + (size_t)th.b * sh.D * sh.N, k, j, sh.N) : both(0.f);
       da[k][j] = both(0.f);
     }
+    sm.da[2 * k][th.tid] = sm.da[2 * k + 1][th.tid] = make_ulonglong2(0, 0);
     for (int i = sh.segs - 2; i >= seg; --i) {         // the segments behind this one
       const size_t at = ((size_t)i * sh.B + th.b) * sh.D;
       f32x2 v[4];
@@ -443,6 +451,14 @@ __global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_c
       }
       if (base % kPart == 0) meet_go<kBwdThreads>(kSums + w);
     }
+#pragma unroll
+    for (int k = 0; k < kP; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ulonglong2& total = sm.da[2 * k + h][th.tid];
+        total = make_ulonglong2(add2(total.x, da[k][2 * h]), add2(total.y, da[k][2 * h + 1]));
+        da[k][2 * h] = da[k][2 * h + 1] = both(0.f);
+      }
   }
 
   const size_t row = (size_t)th.b * sh.segs + seg;
@@ -450,7 +466,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_c
   for (int k = 0; k < kP; ++k)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      th.put(A.part_a + row * sh.D * sh.N, k, j, sh.N, da[k][j]);
+      const ulonglong2 total = sm.da[2 * k + j / 2][th.tid];
+      th.put(A.part_a + row * sh.D * sh.N, k, j, sh.N, j % 2 ? total.y : total.x);
       if (seg == 0 && A.gs_in) th.put(A.gs_in + (size_t)th.b * sh.D * sh.N, k, j, sh.N, G[k][j]);
     }
 }
