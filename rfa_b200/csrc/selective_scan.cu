@@ -288,35 +288,41 @@ __device__ __forceinline__ void store4(float* p, int n, bool wide, const float* 
 }
 
 // ---- one token ---------------------------------------------------------------------------------------------------------------
-// Bound by the state's way from memory and back, 8 bytes per element.  LN lanes a channel, four adjacent states (one 16-byte word) each; a
-// thread has one channel of kRows batch rows, all of whose loads are on the way at once, so that a, the group and the addresses are
-// found once for them.
+// Bound by the state's way from memory and back, 8 bytes per element, where it is large enough.  A thread has eight adjacent states (two
+// 16-byte words) of one channel, LN / 2 lanes a channel, in kRows batch rows, all of whose loads are on the way at once: the step size, a, the
+// group and the addresses, which are most of the instructions, are found once for them.
 template <typename T, int LN, int kRows>
 __global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ rfa_scan_t p, T* y, float* state, bool wide, bool wide_bc) {
-  const int at_ch = (blockIdx.x * 256 + threadIdx.x) / LN, n0 = 4 * (threadIdx.x % LN), b0 = blockIdx.y * kRows;
+  constexpr int kLanes = LN / 2;
+  const int at_ch = (blockIdx.x * 256 + threadIdx.x) / kLanes, n0 = 8 * (threadIdx.x % kLanes), b0 = blockIdx.y * kRows;
   const bool there = at_ch < p.D;
-  const int ch = there ? at_ch : 0, n = there ? max(0, min(4, p.N - n0)) : 0, rows = min(kRows, p.B - b0);
+  const int ch = there ? at_ch : 0, rows = min(kRows, p.B - b0);
+  const int n[2] = {there ? p.N - n0 : 0, there ? p.N - n0 - 4 : 0};
   const int g = p.G == 1 ? 0 : ch / (p.D / p.G);
   const T* bp = static_cast<const T*>(p.b) + (int64_t)g * p.b_g + n0;
   const T* cp = static_cast<const T*>(p.c) + (int64_t)g * p.c_g + n0;
   float* at = state + ((int64_t)b0 * p.D + ch) * p.N + n0;
   const int64_t row = (int64_t)p.D * p.N;
-  float s[kRows][4], a[4];
-  Raw<T, 4> rb[kRows], rc[kRows];
+  float s[kRows][8], a[8];
+  Raw<T, 4> rb[kRows][2], rc[kRows][2];
   T x[kRows], dt[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int b = b0 + (r < rows ? r : 0);             // a row that is not there: another's loads, nothing stored
-    load4(at + (b - b0) * row, n, wide, s[r]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      load4(at + (b - b0) * row + 4 * h, n[h], wide, s[r] + 4 * h);
+      rb[r][h].load(bp + (int64_t)b * p.b_b + 4 * h, n[h], wide_bc);
+      rc[r][h].load(cp + (int64_t)b * p.c_b + 4 * h, n[h], wide_bc);
+    }
     x[r] = static_cast<const T*>(p.x)[(int64_t)b * p.x_b + ch];
     dt[r] = static_cast<const T*>(p.dt)[(int64_t)b * p.dt_b + ch];
-    rb[r].load(bp + (int64_t)b * p.b_b, n, wide_bc);
-    rc[r].load(cp + (int64_t)b * p.c_b, n, wide_bc);
   }
-  load4(p.a + (size_t)ch * p.N + n0, n, wide, a);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) load4(p.a + (size_t)ch * p.N + n0 + 4 * h, n[h], wide, a + 4 * h);
   const float bias = p.dt_bias ? p.dt_bias[ch] : 0.f, skip = p.d ? p.d[ch] : 0.f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) a[j] *= kLog2e;
+  for (int j = 0; j < 8; ++j) a[j] *= kLog2e;
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const float xv = to_f(x[r]);
@@ -324,15 +330,18 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ 
     if (p.softplus) delta = softplus(delta, sig);
     const float dx = delta * xv;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[r][j] = fmaf(ex2(delta * a[j]), s[r][j], dx * rb[r].get(j));
-      out = fmaf(s[r][j], rc[r].get(j), out);
+    for (int j = 0; j < 8; ++j) {
+      s[r][j] = fmaf(ex2(delta * a[j]), s[r][j], dx * rb[r][j / 4].get(j % 4));
+      out = fmaf(s[r][j], rc[r][j / 4].get(j % 4), out);
     }
 #pragma unroll
-    for (int o = LN / 2; o > 0; o >>= 1) out += __shfl_xor_sync(0xffffffffu, out, o);
+    for (int o = kLanes / 2; o > 0; o >>= 1) out += __shfl_xor_sync(0xffffffffu, out, o);
     if (r >= rows || !there) continue;
     const bool gone = p.mask && p.mask[b0 + r];
-    if (!gone) store4(at + r * row, n, wide, s[r]);
+    if (!gone) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) store4(at + r * row + 4 * h, n[h], wide, s[r] + 4 * h);
+    }
     if (n0 == 0) y[(int64_t)(b0 + r) * p.D + ch] = from_f<T>(gone ? 0.f : p.d ? fmaf(skip, xv, out) : out);
   }
 }
@@ -376,12 +385,12 @@ extern "C" int rfa_selective_scan_step(const rfa_scan_t* scan, void* y, float* s
   const int size = scan->dtype == RFA_F32 ? 4 : 2;
   const bool wide = scan->N % 4 == 0 && aligned16(scan->a);
   const bool wide_bc = wide_ok(scan->b, scan->b_b, scan->b_g, size, 4) && wide_ok(scan->c, scan->c_b, scan->c_g, size, 4);
-  // Four rows a thread from eight CTAs of one row per SM on; below, all SMs are wanted.
+  // Two rows a thread from eight CTAs of one row per SM on; below, all SMs are wanted.
 #define CALL(T, LN)                                                                                                          \
   do {                                                                                                                       \
-    const unsigned x = (unsigned)(((int64_t)scan->D * LN + 255) / 256);                                                      \
+    const unsigned x = (unsigned)(((int64_t)scan->D * (LN / 2) + 255) / 256);                                                \
     if ((int64_t)x * scan->B >= 8 * 148)                                                                                     \
-      scan_step_kernel<T, LN, 4><<<dim3(x, (scan->B + 3) / 4), 256, 0, as_stream(stream)>>>(*scan, static_cast<T*>(y), s, wide, wide_bc); \
+      scan_step_kernel<T, LN, 2><<<dim3(x, (scan->B + 1) / 2), 256, 0, as_stream(stream)>>>(*scan, static_cast<T*>(y), s, wide, wide_bc); \
     else                                                                                                                     \
       scan_step_kernel<T, LN, 1><<<dim3(x, scan->B), 256, 0, as_stream(stream)>>>(*scan, static_cast<T*>(y), s, wide, wide_bc);           \
   } while (0)
