@@ -1,6 +1,6 @@
 // Shared by the selective scan's forward and backward: the work of a CTA, its tiles in shared memory, how inputs are staged.
 //
-// A state element (channel i, state n) evolves alone, so a thread holds 2 (backward: 4) adjacent channels x 4 states in registers and walks the
+// A state element (channel i, state n) evolves alone, so a thread holds 2 adjacent channels x 4 states in registers and walks the
 // tokens; LN = 2, 4, 8 or 16 neighbouring lanes hold a channel's up to 4 LN states, lane l the states l, LN + l, 2 LN + l, 3 LN + l.  A CTA
 // has 256 / LN channels of one group and one batch row, and a segment of the tokens.  Some of its warps scan; others bring tiles of
 // inputs and take results away meanwhile, so that a scheduler with few CTAs still has work while one warp waits.
@@ -9,8 +9,8 @@
 // quarter of a channel's -- takes a polynomial on the FMA units instead (`decays`), at which both are busy equally long.  Issue slots come
 // next: all arithmetic is packed, both channels in one instruction (`fma.rn.f32x2`; 68 instructions a token and warp, 96 without).
 //
-// Tiles of 16 tokens go through shared memory, two of them by turns: a thread asks for a pair of channels' inputs a tile ahead (a warp's loads are whole 128-byte
-// rows), turns them into delta and delta x and leaves them as one 16-byte word, which the scan's lanes read.  Shared memory hands a
+// Tiles of 16 tokens go through shared memory, two of them by turns: a thread asks for a pair of channels' inputs a tile ahead (a
+// warp's loads are whole 128-byte rows), turns them into delta and delta x and leaves them as one 16-byte word, which the scan's lanes read.  Shared memory hands a
 // warp 128 bytes a clock whether lanes read the same words or not: 48 bytes a lane and token (b and c as pairs of equal
 // values were 80, and bound the forward at 245 us for 8 x 2048 x 2048).
 #pragma once
@@ -102,37 +102,33 @@ template <int R> struct Poly {
     return pack2(__int_as_float(__float_as_int(q.x) + (__float_as_int(k.x) << 23)), __int_as_float(__float_as_int(q.y) + (__float_as_int(k.y) << 23)));
   }
 };
-// exp(delta a) for R tokens, P pairs of channels and the thread's four states, a in units of log 2; kPoly: the first one's as above
-template <int R, int P, bool kPoly> __device__ __forceinline__ void decays(const f32x2 (*delta)[P], const f32x2 (*a2)[4], f32x2 (*e)[P][4]) {
-  Poly<R * P> poly;
+// exp(delta a) of both channels for R tokens and the thread's four states, a in units of log 2; kPoly: the first one's as above
+template <int R, bool kPoly> __device__ __forceinline__ void decays(const f32x2* delta, const f32x2* a2, f32x2 (*e)[4]) {
+  Poly<R> poly;
 #pragma unroll
-  for (int i = 0; i < R; ++i)
+  for (int i = 0; i < R; ++i) {
+    if (kPoly) poly.begin(i, mul2(delta[i], a2[0]));
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-      if (kPoly) poly.begin(i * P + k, mul2(delta[i][k], a2[k][0]));
-#pragma unroll
-      for (int j = kPoly; j < 4; ++j) e[i][k][j] = exp2_unit(mul2(delta[i][k], a2[k][j]));
-    }
+    for (int j = kPoly; j < 4; ++j) e[i][j] = exp2_unit(mul2(delta[i], a2[j]));
+  }
   if (!kPoly) return;
   poly.run();
 #pragma unroll
-  for (int i = 0; i < R; ++i)
-#pragma unroll
-    for (int k = 0; k < P; ++k) e[i][k][0] = poly.end(i * P + k);
+  for (int i = 0; i < R; ++i) e[i][0] = poly.end(i);
 }
 
 // ---- the work of a thread ----------------------------------------------------------------------------------------------------
-// Of kScan threads that scan, P pairs of adjacent channels each, and kBring that bring and take, one pair each.
-template <int LN, int kScan, int kBring, int P = 1> struct ScanThread {
+// Of kScan threads that scan and kBring that bring and take, a pair of adjacent channels each.
+template <int LN, int kScan, int kBring> struct ScanThread {
   using Tile = ScanTile<LN>;
   static constexpr int kRows = kBring / Tile::kPairs;            // tokens that are brought side by side
   static constexpr int kPasses = kScanTile / kRows;
   static constexpr int kStep = kBring / Tile::kN;                // tokens whose b (and c) are
   static constexpr int kBc = kScanTile / kStep;
-  static_assert(kScan * P == LN * Tile::kPairs && kPasses >= 1 && kStep >= 1, "work for every thread");
+  static_assert(kScan == LN * Tile::kPairs && kPasses >= 1 && kStep >= 1, "work for every thread");
   int group, c0, nch, b;          // the CTA's group, first channel, channels (<= kChannels), batch row
   bool scans;                     // or brings and takes
-  int tid, ln, pair;              // of its kind; in the scan: lane of the channels, first pair in the CTA
+  int tid, ln, pair;              // of its kind; in the scan: lane of the channels, pair in the CTA
   int vpair, row, vn;             // when it brings: pair of channels, first token, how many of the two channels there are
   __device__ ScanThread(const ScanShape& s) {
     group = blockIdx.x / s.per_group;
@@ -143,45 +139,45 @@ template <int LN, int kScan, int kBring, int P = 1> struct ScanThread {
     scans = threadIdx.x < kScan;
     tid = scans ? threadIdx.x : threadIdx.x - kScan;
     ln = tid % LN;
-    pair = tid / LN * P;
+    pair = tid / LN;
     vpair = tid % Tile::kPairs;
     row = tid / Tile::kPairs;
     vn = max(0, min(2, nch - 2 * vpair));
   }
-  // n of the thread's state j; channel h of its pair k, and whether it is there
+  // n of the thread's state j; channel h of its pair, and whether it is there
   __device__ __forceinline__ int state(int j) const { return j * LN + ln; }
-  __device__ __forceinline__ int channel(int k, int h) const { return c0 + 2 * (pair + k) + h; }
-  __device__ __forceinline__ bool has(int k, int h) const { return 2 * (pair + k) + h < nch; }
+  __device__ __forceinline__ int channel(int h) const { return c0 + 2 * pair + h; }
+  __device__ __forceinline__ bool has(int h) const { return 2 * pair + h < nch; }
   // rows [D][N] of fp32 at p, both channels' state j; 0 where there is none
-  __device__ __forceinline__ f32x2 get(const float* p, int k, int j, int N) const {
+  __device__ __forceinline__ f32x2 get(const float* p, int j, int N) const {
     const bool n = state(j) < N;
-    return pack2(n && has(k, 0) ? p[(size_t)channel(k, 0) * N + state(j)] : 0.f, n && has(k, 1) ? p[(size_t)channel(k, 1) * N + state(j)] : 0.f);
+    return pack2(n && has(0) ? p[(size_t)channel(0) * N + state(j)] : 0.f, n && has(1) ? p[(size_t)channel(1) * N + state(j)] : 0.f);
   }
-  __device__ __forceinline__ void put(float* p, int k, int j, int N, f32x2 v) const {
+  __device__ __forceinline__ void put(float* p, int j, int N, f32x2 v) const {
     const float2 f = split2(v);
-    if (state(j) < N && has(k, 0)) p[(size_t)channel(k, 0) * N + state(j)] = f.x;
-    if (state(j) < N && has(k, 1)) p[(size_t)channel(k, 1) * N + state(j)] = f.y;
+    if (state(j) < N && has(0)) p[(size_t)channel(0) * N + state(j)] = f.x;
+    if (state(j) < N && has(1)) p[(size_t)channel(1) * N + state(j)] = f.y;
   }
-  __device__ __forceinline__ f32x2 get1(const float* p, int k) const {      // [D]
-    return pack2(has(k, 0) ? p[channel(k, 0)] : 0.f, has(k, 1) ? p[channel(k, 1)] : 0.f);
+  __device__ __forceinline__ f32x2 get1(const float* p) const {      // [D]
+    return pack2(has(0) ? p[channel(0)] : 0.f, has(1) ? p[channel(1)] : 0.f);
   }
-  __device__ __forceinline__ void put1(float* p, int k, f32x2 v) const {
+  __device__ __forceinline__ void put1(float* p, f32x2 v) const {
     const float2 f = split2(v);
-    if (ln == 0 && has(k, 0)) p[channel(k, 0)] = f.x;
-    if (ln == 0 && has(k, 1)) p[channel(k, 1)] = f.y;
+    if (ln == 0 && has(0)) p[channel(0)] = f.x;
+    if (ln == 0 && has(1)) p[channel(1)] = f.y;
   }
   // kept rows [D][kN], a lane's four states adjacent
-  __device__ __forceinline__ void load_kept(const float* p, int k, f32x2* v) const {
+  __device__ __forceinline__ void load_kept(const float* p, f32x2* v) const {
     float4 f[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      f[h] = has(k, h) ? *reinterpret_cast<const float4*>(p + (size_t)channel(k, h) * Tile::kN + 4 * ln) : make_float4(0.f, 0.f, 0.f, 0.f);
+      f[h] = has(h) ? *reinterpret_cast<const float4*>(p + (size_t)channel(h) * Tile::kN + 4 * ln) : make_float4(0.f, 0.f, 0.f, 0.f);
     v[0] = pack2(f[0].x, f[1].x); v[1] = pack2(f[0].y, f[1].y); v[2] = pack2(f[0].z, f[1].z); v[3] = pack2(f[0].w, f[1].w);
   }
-  __device__ __forceinline__ void store_kept(float* p, int k, const f32x2* v) const {
+  __device__ __forceinline__ void store_kept(float* p, const f32x2* v) const {
     const float2 a = split2(v[0]), b = split2(v[1]), c = split2(v[2]), d = split2(v[3]);
-    if (has(k, 0)) *reinterpret_cast<float4*>(p + (size_t)channel(k, 0) * Tile::kN + 4 * ln) = make_float4(a.x, b.x, c.x, d.x);
-    if (has(k, 1)) *reinterpret_cast<float4*>(p + (size_t)channel(k, 1) * Tile::kN + 4 * ln) = make_float4(a.y, b.y, c.y, d.y);
+    if (has(0)) *reinterpret_cast<float4*>(p + (size_t)channel(0) * Tile::kN + 4 * ln) = make_float4(a.x, b.x, c.x, d.x);
+    if (has(1)) *reinterpret_cast<float4*>(p + (size_t)channel(1) * Tile::kN + 4 * ln) = make_float4(a.y, b.y, c.y, d.y);
   }
   // Which of a bringing thread's tokens of a tile are there: bit i of pass i.  A plain tile is full, of a full CTA, without a mask and in wide
   // words: nothing is asked about its elements (the questions were a quarter of the forward's instructions).

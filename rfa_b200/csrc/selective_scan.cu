@@ -1,8 +1,11 @@
 // Selective scan, forward and one token:
 //   delta = softplus(dt + bias),  s_t = exp(delta_t a) s_(t-1) + delta_t b_t x_t,  y_t = c_t . s_t + d x_t.
 //
-// Bound by the exponentials: one per token, channel and state, 16 a clock and SM, where a token and channel of 16 states moves 6 bytes in
-// 16 bits (8 x 2048 tokens x 2048 channels: 537 M exponentials are 119 us of that unit, 201 MB are 31 us of memory).  Layout in scan.cuh.
+// Bound by arithmetic: one exponential per token, channel and state, where a token and channel of 16 states moves 6 bytes in 16 bits
+// (8 x 2048 tokens x 2048 channels: 537 M exponentials are 119 us of the special function units, 201 MB are 31 us of memory).  That size
+// takes 226 us in bf16: of the 105 cycles of a token on an SM's scheduler the special function unit is busy for 60 (with softplus),
+// the FMA units for 63, shared memory for 61 of the SM's, and 68 are issue slots; 256 CTAs on 148 SMs leave a seventh of the card idle.
+// Tiles of 32 tokens: 220 us, for twice the shared memory and code.  Layout in scan.cuh.
 //
 // Few rows (a prompt of one sequence) leave SMs idle: the tokens are then cut into segments.  A first kernel leaves each segment's own state
 // from zero and the sum of its deltas -- over which a whole segment's decay is exp(a sum delta), one exponential -- and the main kernel's
@@ -187,54 +190,54 @@ __global__ void __launch_bounds__(kFwdThreads, 2) scan_fwd_kernel(const __grid_c
     return;
   }
 
-  f32x2 a2[1][4], s[4], sum = both(0.f);                  // a in units of log 2
+  f32x2 a2[4], s[4], sum = both(0.f);                  // a in units of log 2
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    a2[0][j] = mul2(th.get(p.a, 0, j, sh.N), both(kLog2e));
-    s[j] = !kSummary && p.s_in ? th.get(p.s_in + (size_t)th.b * sh.D * sh.N, 0, j, sh.N) : both(0.f);
+    a2[j] = mul2(th.get(p.a, j, sh.N), both(kLog2e));
+    s[j] = !kSummary && p.s_in ? th.get(p.s_in + (size_t)th.b * sh.D * sh.N, j, sh.N) : both(0.f);
   }
   if (!kSummary)
     for (int i = 0; i < seg; ++i) {                    // the segments before this one
       const size_t at = ((size_t)i * sh.B + th.b) * sh.D;
       f32x2 v[4];
-      th.load_kept(A.seg_state + at * sh.kn, 0, v);
-      const f32x2 over = th.get1(A.seg_sum + at, 0);
+      th.load_kept(A.seg_state + at * sh.kn, v);
+      const f32x2 over = th.get1(A.seg_sum + at);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] = fma2(exp2_unit(mul2(over, a2[0][j])), s[j], v[j]);
+      for (int j = 0; j < 4; ++j) s[j] = fma2(exp2_unit(mul2(over, a2[j])), s[j], v[j]);
     }
   for (int tile = tile0; tile < tile1; ++tile) {
     const int buf = (tile - tile0) & 1;
-    if (!kSummary && A.ckpt) th.store_kept(A.ckpt + ((size_t)th.b * sh.tiles + tile) * sh.D * sh.kn, 0, s);
+    if (!kSummary && A.ckpt) th.store_kept(A.ckpt + ((size_t)th.b * sh.tiles + tile) * sh.D * sh.kn, s);
     meet_wait<kFwdThreads>(kFull + buf);
     constexpr int kRun = 4;                            // tokens whose decays are formed side by side
 #pragma unroll
     for (int t0 = 0; t0 < kScanTile; t0 += kRun) {
-      f32x2 delta[kRun][1], dx[kRun], e[kRun][1][4];
+      f32x2 delta[kRun], dx[kRun], e[kRun][4];
 #pragma unroll
       for (int r = 0; r < kRun; ++r) {
         const ulonglong2 in = *reinterpret_cast<const ulonglong2*>(&sm.in[buf][t0 + r][th.pair]);
-        delta[r][0] = in.x;
+        delta[r] = in.x;
         dx[r] = in.y;
       }
-      decays<kRun, 1, true>(delta, a2, e);
+      decays<kRun, true>(delta, a2, e);
 #pragma unroll
       for (int r = 0; r < kRun; ++r) {
         float bt[4];
         lane_states(sm.b[buf][t0 + r], th.ln, bt);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[r][0][j] = s[j] = fma2(e[r][0][j], s[j], mul2(dx[r], both(bt[j])));
+        for (int j = 0; j < 4; ++j) e[r][j] = s[j] = fma2(e[r][j], s[j], mul2(dx[r], both(bt[j])));
       }
       if constexpr (kSummary) {
-        sum = add2(sum, add2(add2(delta[0][0], delta[1][0]), add2(delta[2][0], delta[3][0])));
+        sum = add2(sum, add2(add2(delta[0], delta[1]), add2(delta[2], delta[3])));
       } else {
         f32x2 out[kRun];
 #pragma unroll
         for (int r = 0; r < kRun; ++r) {
           float ct[4];
           lane_states(sm.c[buf][t0 + r], th.ln, ct);
-          out[r] = mul2(e[r][0][0], both(ct[0]));
+          out[r] = mul2(e[r][0], both(ct[0]));
 #pragma unroll
-          for (int j = 1; j < 4; ++j) out[r] = fma2(e[r][0][j], both(ct[j]), out[r]);
+          for (int j = 1; j < 4; ++j) out[r] = fma2(e[r][j], both(ct[j]), out[r]);
         }
 #pragma unroll
         for (int r = 0; r < kRun; ++r) sm.y[buf][t0 + r][th.ln / 2][2 * th.pair + th.ln % 2] = out[r];
@@ -245,11 +248,11 @@ __global__ void __launch_bounds__(kFwdThreads, 2) scan_fwd_kernel(const __grid_c
 
   if (kSummary) {
     const size_t at = ((size_t)seg * sh.B + th.b) * sh.D;
-    th.store_kept(A.seg_state + at * sh.kn, 0, s);
-    th.put1(A.seg_sum + at, 0, sum);
+    th.store_kept(A.seg_state + at * sh.kn, s);
+    th.put1(A.seg_sum + at, sum);
   } else if (A.s_out && seg == sh.segs - 1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) th.put(A.s_out + (size_t)th.b * sh.D * sh.N, 0, j, sh.N, s[j]);
+    for (int j = 0; j < 4; ++j) th.put(A.s_out + (size_t)th.b * sh.D * sh.N, j, sh.N, s[j]);
   }
 }
 

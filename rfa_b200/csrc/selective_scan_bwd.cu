@@ -4,11 +4,18 @@
 //   gdt_t = softplus'(dt_t + bias) (x_t sum_n G_t b_t + sum_n a p_t),  gbias = sum_t gdt_t.
 //
 // Layout in scan.cuh; tiles from the last to the first.  The states come back from the forward's checkpoints, one in front of every
-// 16 tokens (as many bytes as two 16-bit activations at 16 states, instead of all states): a half of 8 tokens is walked forward with
-// its decays and decayed states left in registers (128 of them), then backward; the first half's walk is made twice.
-// Sums over states go over the LN lanes of a channel; sums over channels over a thread's two, then through shared memory over the CTA's
-// pairs (12 instructions a token and thread, where exchanging them within the warp takes 28), then over CTAs in sum_parts: a fixed
-// order, no atomics.
+// 16 tokens (as many bytes as two 16-bit activations at 16 states, instead of all states): a tile is walked forward once for the state
+// in front of every second token, then two tokens at a time, from the last, forward with decays, decayed states and states left in
+// registers and backward.  Sums over states go over the LN lanes of a channel; sums over channels over a thread's two, then every four tokens
+// through shared memory to the warps that bring and take, over the CTA's pairs (12 instructions a token and thread, where exchanging
+// them within the warp takes 28), then over CTAs in sum_parts: a fixed order, no atomics.
+//
+// 8 x 2048 tokens x 2048 channels x 16 states, bf16: about 860 of the 1100 us of a training step.  Bound by issue slots (215 instructions a
+// token and warp), shared memory (57 passes of 128 bytes) and the FMA units (190 cycles) together, each 50 to 60 % busy of the 385 cycles that
+// a token takes; memory traffic is 5 % of what could be.  Taking away one of its parts (the sums over channels, over states, the walk for
+// the states) saves 7 to 9 % each.  Also measured: four channels a thread (one scanning warp per scheduler, 1430 us a step), parts of two
+// tokens (1310), mbarriers instead of named barriers (1180), exponentials of the special function unit alone (1120), four tokens in
+// registers (1150).
 //
 // Few rows: segments as in the forward, whose summaries run backward here (the gradient a segment hands to the one before it).
 #include "scan.cuh"
@@ -19,20 +26,18 @@ namespace {
 constexpr int kRun = 2;       // tokens whose decays and states are in registers at a time
 constexpr int kPart = 4;      // tokens after which the scanning warps hand their partial sums over
 
-constexpr int kP = 1;         // pairs of channels of a scanning thread
-constexpr int kBwdScan = 128 / kP, kBwdBring = 128, kBwdThreads = kBwdScan + kBwdBring;
-template <int LN> using BwdThread = ScanThread<LN, kBwdScan, kBwdBring, kP>;
+constexpr int kBwdScan = 128, kBwdBring = 128, kBwdThreads = kBwdScan + kBwdBring;
+template <int LN> using BwdThread = ScanThread<LN, kBwdScan, kBwdBring>;
 
 template <int LN> struct __align__(16) BwdSmem {
   using Tile = ScanTile<LN>;
-  static constexpr int kThreads = Tile::kPairs / kP;     // that share a lane's states
   float4 in[2][kScanTile][Tile::kPairs];               // delta, delta', delta x, delta' x' of two adjacent channels
   float2 g[2][kScanTile][Tile::kPairs], slope[2][kScanTile][Tile::kPairs];      // g and softplus' of both
   float b[2][kScanTile][Tile::kN], c[2][kScanTile][Tile::kN];
   float4 res[kScanTile][Tile::kPairs];                 // sum_n G b of both channels, sum_n a log2(e) p of both
-  ulonglong2 start[kScanTile / kRun][2 * kP][kBwdScan];     // each thread's states in front of a run
-  ulonglong2 da[2 * kP][kBwdScan];                     // each thread's ga: tiles are summed apart (one chain of 2048 tokens is 1e-6 off)
-  float4 over_ch[2][kPart][2][kThreads][LN];           // gb and gc of each thread's channels, a lane's four states adjacent; two parts by turns
+  ulonglong2 start[kScanTile / kRun][2][kBwdScan]; // each thread's states in front of a run
+  ulonglong2 da[2][kBwdScan];                          // each thread's ga: tiles are summed apart (one chain of 2048 tokens is 1e-6 off)
+  float4 over_ch[2][kPart][2][Tile::kPairs][LN];       // gb and gc of each pair's channels, a lane's four states adjacent; two parts by turns
 };
 // Further places where the halves of a CTA meet: a part's sums are there, have been taken.
 enum { kSums = 5, kTaken = 7 };
@@ -66,10 +71,10 @@ __global__ void __launch_bounds__(kSummaryThreads) scan_bwd_summary_kernel(const
   const rfa_scan_t& p = A.p;
   const Thread th(sh);
   const int seg = blockIdx.z + 1, tile0 = seg * sh.seg_tiles, tile1 = min(tile0 + sh.seg_tiles, sh.tiles);
-  f32x2 a2[1][4], G[4], sum = both(0.f);
+  f32x2 a2[4], G[4], sum = both(0.f);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    a2[0][j] = mul2(th.get(p.a, 0, j, sh.N), both(kLog2e));
+    a2[j] = mul2(th.get(p.a, j, sh.N), both(kLog2e));
     G[j] = both(0.f);
   }
   const int ch = th.c0 + 2 * th.vpair;
@@ -114,28 +119,28 @@ __global__ void __launch_bounds__(kSummaryThreads) scan_bwd_summary_kernel(const
     constexpr int kLook = 4;                           // tokens whose decays are formed side by side
 #pragma unroll
     for (int t0 = kScanTile - kLook; t0 >= 0; t0 -= kLook) {
-      f32x2 delta[kLook][1], gt[kLook], e[kLook][1][4];
+      f32x2 delta[kLook], gt[kLook], e[kLook][4];
 #pragma unroll
       for (int r = 0; r < kLook; ++r) {
         const ulonglong2 in = *reinterpret_cast<const ulonglong2*>(&sm.in[t0 + r][th.pair]);
-        delta[r][0] = in.x;
+        delta[r] = in.x;
         gt[r] = in.y;
       }
-      decays<kLook, 1, true>(delta, a2, e);
+      decays<kLook, true>(delta, a2, e);
 #pragma unroll
       for (int r = kLook - 1; r >= 0; --r) {
         float ct[4];
         lane_states(sm.c[t0 + r], th.ln, ct);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) G[j] = mul2(fma2(gt[r], both(ct[j]), G[j]), e[r][0][j]);
-        sum = add2(sum, delta[r][0]);
+        for (int j = 0; j < 4; ++j) G[j] = mul2(fma2(gt[r], both(ct[j]), G[j]), e[r][j]);
+        sum = add2(sum, delta[r]);
       }
     }
     __syncthreads();
   }
   const size_t at = ((size_t)(seg - 1) * sh.B + th.b) * sh.D;
-  th.store_kept(A.seg_grad + at * sh.kn, 0, G);
-  th.put1(A.seg_sum + at, 0, sum);
+  th.store_kept(A.seg_grad + at * sh.kn, G);
+  th.put1(A.seg_sum + at, sum);
 }
 
 // Brings the tiles of a segment, from the last to the first, and takes their gradients away.
@@ -225,7 +230,7 @@ __device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, con
       const int at = o + th.tid, l = at % LN, share = at / LN % kEach, which = at / (LN * kEach) % 2, t = at / (LN * kEach * 2);
       ulonglong2 f = make_ulonglong2(0, 0);
 #pragma unroll
-      for (int r = 0; r < BwdSmem<LN>::kThreads / kEach; ++r) {
+      for (int r = 0; r < Tile::kPairs / kEach; ++r) {
         const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.over_ch[w][t][which][r * kEach + share][l]);
         f.x = add2(f.x, v.x);
         f.y = add2(f.y, v.y);
@@ -320,156 +325,119 @@ __global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_c
     return;
   }
 
-  f32x2 a2[kP][4], G[kP][4], da[kP][4];
+  f32x2 a2[4], G[4], da[4];
 #pragma unroll
-  for (int k = 0; k < kP; ++k) {
+  for (int j = 0; j < 4; ++j) {
+    a2[j] = mul2(th.get(p.a, j, sh.N), both(kLog2e));
+    G[j] = A.g_s ? th.get(A.g_s + (size_t)th.b * sh.D * sh.N, j, sh.N) : both(0.f);
+    da[j] = both(0.f);
+  }
+  sm.da[0][th.tid] = sm.da[1][th.tid] = make_ulonglong2(0, 0);
+  for (int i = sh.segs - 2; i >= seg; --i) {           // the segments behind this one
+    const size_t at = ((size_t)i * sh.B + th.b) * sh.D;
+    f32x2 v[4];
+    th.load_kept(A.seg_grad + at * sh.kn, v);
+    const f32x2 over = th.get1(A.seg_sum + at);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      a2[k][j] = mul2(th.get(p.a, k, j, sh.N), both(kLog2e));
-      G[k][j] = A.g_s ? th.get(A.g_s + (size_t)th.b * sh.D * sh.N, k, j, sh.N) : both(0.f);
-      da[k][j] = both(0.f);
-    }
-    sm.da[2 * k][th.tid] = sm.da[2 * k + 1][th.tid] = make_ulonglong2(0, 0);
-    for (int i = sh.segs - 2; i >= seg; --i) {         // the segments behind this one
-      const size_t at = ((size_t)i * sh.B + th.b) * sh.D;
-      f32x2 v[4];
-      th.load_kept(A.seg_grad + at * sh.kn, k, v);
-      const f32x2 over = th.get1(A.seg_sum + at, k);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) G[k][j] = fma2(exp2_unit(mul2(over, a2[k][j])), G[k][j], v[j]);
-    }
+    for (int j = 0; j < 4; ++j) G[j] = fma2(exp2_unit(mul2(over, a2[j])), G[j], v[j]);
   }
 
-  f32x2 s[kP][4];                                      // the state in front of the tile
+  f32x2 s[4];                                          // the state in front of the tile
   const float* ckpt = A.ckpt + (size_t)th.b * sh.tiles * sh.D * sh.kn;
-  const auto load_state = [&](int tile) {
-#pragma unroll
-    for (int k = 0; k < kP; ++k) th.load_kept(ckpt + (size_t)tile * sh.D * sh.kn, k, s[k]);
-  };
-  load_state(tile1 - 1);
+  th.load_kept(ckpt + (size_t)(tile1 - 1) * sh.D * sh.kn, s);
   for (int tile = tile1 - 1; tile >= tile0; --tile) {
     const int buf = (tile1 - 1 - tile) & 1;
-    const auto inputs = [&](int base, f32x2 (*delta)[kP], f32x2 (*dx)[kP]) {
+    const auto inputs = [&](int base, f32x2* delta, f32x2* dx) {
 #pragma unroll
-      for (int r = 0; r < kRun; ++r)
-#pragma unroll
-        for (int k = 0; k < kP; ++k) {
-          const ulonglong2 in = *reinterpret_cast<const ulonglong2*>(&sm.in[buf][base + r][th.pair + k]);
-          delta[r][k] = in.x;
-          dx[r][k] = in.y;
-        }
+      for (int r = 0; r < kRun; ++r) {
+        const ulonglong2 in = *reinterpret_cast<const ulonglong2*>(&sm.in[buf][base + r][th.pair]);
+        delta[r] = in.x;
+        dx[r] = in.y;
+      }
     };
     meet_wait<kBwdThreads>(kFull + buf);
     // The states in front of each run of the tile, then run by run from the last: forward with what the way back needs, and back.
 #pragma unroll 1
     for (int run = 0;; ++run) {
-#pragma unroll
-      for (int k = 0; k < kP; ++k) {
-        sm.start[run][2 * k][th.tid] = make_ulonglong2(s[k][0], s[k][1]);
-        sm.start[run][2 * k + 1][th.tid] = make_ulonglong2(s[k][2], s[k][3]);
-      }
+      sm.start[run][0][th.tid] = make_ulonglong2(s[0], s[1]);
+      sm.start[run][1][th.tid] = make_ulonglong2(s[2], s[3]);
       if (run == kScanTile / kRun - 1) break;
-      f32x2 delta[kRun][kP], dx[kRun][kP], e[kRun][kP][4];
+      f32x2 delta[kRun], dx[kRun], e[kRun][4];
       inputs(run * kRun, delta, dx);
-      decays<kRun, kP, false>(delta, a2, e);
+      decays<kRun, false>(delta, a2, e);               // over at most 15 tokens: the special function unit's own error does not add up
 #pragma unroll
       for (int r = 0; r < kRun; ++r) {
         float bt[4];
         lane_states(sm.b[buf][run * kRun + r], th.ln, bt);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int k = 0; k < kP; ++k) s[k][j] = fma2(e[r][k][j], s[k][j], mul2(dx[r][k], both(bt[j])));
+        for (int j = 0; j < 4; ++j) s[j] = fma2(e[r][j], s[j], mul2(dx[r], both(bt[j])));
       }
     }
-    if (tile > tile0) load_state(tile - 1);            // asked for early
+    if (tile > tile0) th.load_kept(ckpt + (size_t)(tile - 1) * sh.D * sh.kn, s);      // asked for early
 #pragma unroll 2
     for (int run = kScanTile / kRun - 1; run >= 0; --run) {
       const int base = run * kRun, w = base / kPart & 1;
-      f32x2 delta[kRun][kP], dx[kRun][kP], e[kRun][kP][4], q[kRun][kP][4], st[kRun][kP][4];      // decays, decayed states, states
+      f32x2 delta[kRun], dx[kRun], e[kRun][4], q[kRun][4], st[kRun][4];      // decays, decayed states, states
       float bt[kRun][4];
       inputs(base, delta, dx);
-#pragma unroll
-      for (int k = 0; k < kP; ++k) {
-        const ulonglong2 lo = sm.start[run][2 * k][th.tid], hi = sm.start[run][2 * k + 1][th.tid];
-        q[0][k][0] = lo.x; q[0][k][1] = lo.y; q[0][k][2] = hi.x; q[0][k][3] = hi.y;
-      }
-      decays<kRun, kP, true>(delta, a2, e);
+      const ulonglong2 lo = sm.start[run][0][th.tid], hi = sm.start[run][1][th.tid];
+      const f32x2 first[4] = {lo.x, lo.y, hi.x, hi.y};
+      decays<kRun, true>(delta, a2, e);
 #pragma unroll
       for (int r = 0; r < kRun; ++r) {
         lane_states(sm.b[buf][base + r], th.ln, bt[r]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int k = 0; k < kP; ++k) {
-            q[r][k][j] = mul2(e[r][k][j], r ? st[r - 1][k][j] : q[0][k][j]);
-            st[r][k][j] = fma2(dx[r][k], both(bt[r][j]), q[r][k][j]);
-          }
+        for (int j = 0; j < 4; ++j) {
+          q[r][j] = mul2(e[r][j], r ? st[r - 1][j] : first[j]);
+          st[r][j] = fma2(dx[r], both(bt[r][j]), q[r][j]);
+        }
       }
       // the part's place is free
       if (base % kPart == kPart - kRun && (tile < tile1 - 1 || base < kScanTile - 2 * kPart)) meet_wait<kBwdThreads>(kTaken + w);
 #pragma unroll
       for (int r = kRun - 1; r >= 0; --r) {
-        f32x2 gt[kP], over_b[kP], over_p[kP];          // g; sum_n G b, sum_n a2 p
-#pragma unroll
-        for (int k = 0; k < kP; ++k) gt[k] = *reinterpret_cast<const f32x2*>(&sm.g[buf][base + r][th.pair + k]);
-        float ct[4], gb[4], gc[4];                     // gb, gc: of the four states, over the thread's channels
+        const f32x2 gt = *reinterpret_cast<const f32x2*>(&sm.g[buf][base + r][th.pair]);
+        f32x2 over_b, over_p;                          // sum_n G b, sum_n a2 p
+        float ct[4], gb[4], gc[4];                     // gb, gc: of the four states, over both channels
         lane_states(sm.c[buf][base + r], th.ln, ct);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          f32x2 vb, vc;
-#pragma unroll
-          for (int k = 0; k < kP; ++k) {
-            const f32x2 Gt = fma2(gt[k], both(ct[j]), G[k][j]), pt = mul2(Gt, q[r][k][j]);
-            vb = k ? fma2(Gt, dx[r][k], vb) : mul2(Gt, dx[r][k]);
-            vc = k ? fma2(st[r][k][j], gt[k], vc) : mul2(st[r][k][j], gt[k]);
-            over_b[k] = j ? fma2(Gt, both(bt[r][j]), over_b[k]) : mul2(Gt, both(bt[r][j]));
-            over_p[k] = j ? fma2(pt, a2[k][j], over_p[k]) : mul2(pt, a2[k][j]);
-            da[k][j] = fma2(pt, delta[r][k], da[k][j]);
-            G[k][j] = mul2(Gt, e[r][k][j]);
-          }
-          const float2 fb = split2(vb), fc = split2(vc);
-          gb[j] = fb.x + fb.y;
-          gc[j] = fc.x + fc.y;
+          const f32x2 Gt = fma2(gt, both(ct[j]), G[j]), pt = mul2(Gt, q[r][j]);
+          const float2 vb = split2(mul2(Gt, dx[r])), vc = split2(mul2(st[r][j], gt));
+          gb[j] = vb.x + vb.y;
+          gc[j] = vc.x + vc.y;
+          over_b = j ? fma2(Gt, both(bt[r][j]), over_b) : mul2(Gt, both(bt[r][j]));
+          over_p = j ? fma2(pt, a2[j], over_p) : mul2(pt, a2[j]);
+          da[j] = fma2(pt, delta[r], da[j]);
+          G[j] = mul2(Gt, e[r][j]);
         }
         const int t = base % kPart + r;
-        sm.over_ch[w][t][0][th.pair / kP][th.ln] = make_float4(gb[0], gb[1], gb[2], gb[3]);
-        sm.over_ch[w][t][1][th.pair / kP][th.ln] = make_float4(gc[0], gc[1], gc[2], gc[3]);
-        float over_n[4 * kP];                          // as kP rows of res
-#pragma unroll
-        for (int k = 0; k < kP; ++k) {
-          const float2 ob = split2(over_b[k]), op = split2(over_p[k]);
-          over_n[4 * k] = ob.x; over_n[4 * k + 1] = ob.y; over_n[4 * k + 2] = op.x; over_n[4 * k + 3] = op.y;
-        }
-        lanes_sum<4 * kP, LN>(over_n, th.ln);
+        sm.over_ch[w][t][0][th.pair][th.ln] = make_float4(gb[0], gb[1], gb[2], gb[3]);
+        sm.over_ch[w][t][1][th.pair][th.ln] = make_float4(gc[0], gc[1], gc[2], gc[3]);
+        const float2 ob = split2(over_b), op = split2(over_p);
+        float over_n[4] = {ob.x, ob.y, op.x, op.y};    // as a row of res
+        lanes_sum<4, LN>(over_n, th.ln);
         float* res = reinterpret_cast<float*>(&sm.res[base + r][th.pair]);
-        constexpr int kEach = 4 * kP / LN, kLanes = LN / (4 * kP);      // totals of a lane, or lanes with one total
-        if constexpr (kEach == 4) *reinterpret_cast<float4*>(res + 4 * th.ln) = make_float4(over_n[0], over_n[1], over_n[2], over_n[3]);
-        else if constexpr (kEach == 2) *reinterpret_cast<float2*>(res + 2 * th.ln) = make_float2(over_n[0], over_n[1]);
-        else if constexpr (kEach == 1) res[th.ln] = over_n[0];
-        else if (th.ln % kLanes == 0) res[th.ln / kLanes] = over_n[0];
+        if constexpr (LN == 2) *reinterpret_cast<float2*>(res + 2 * th.ln) = make_float2(over_n[0], over_n[1]);
+        else if (th.ln % (LN / 4) == 0) res[th.ln / (LN / 4)] = over_n[0];
       }
       if (base % kPart == 0) meet_go<kBwdThreads>(kSums + w);
     }
 #pragma unroll
-    for (int k = 0; k < kP; ++k)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        ulonglong2& total = sm.da[2 * k + h][th.tid];
-        total = make_ulonglong2(add2(total.x, da[k][2 * h]), add2(total.y, da[k][2 * h + 1]));
-        da[k][2 * h] = da[k][2 * h + 1] = both(0.f);
-      }
+    for (int h = 0; h < 2; ++h) {
+      ulonglong2& total = sm.da[h][th.tid];
+      total = make_ulonglong2(add2(total.x, da[2 * h]), add2(total.y, da[2 * h + 1]));
+      da[2 * h] = da[2 * h + 1] = both(0.f);
+    }
   }
 
   const size_t row = (size_t)th.b * sh.segs + seg;
 #pragma unroll
-  for (int k = 0; k < kP; ++k)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const ulonglong2 total = sm.da[2 * k + j / 2][th.tid];
-      th.put(A.part_a + row * sh.D * sh.N, k, j, sh.N, j % 2 ? total.y : total.x);
-      if (seg == 0 && A.gs_in) th.put(A.gs_in + (size_t)th.b * sh.D * sh.N, k, j, sh.N, G[k][j]);
-    }
+  for (int j = 0; j < 4; ++j) {
+    const ulonglong2 total = sm.da[j / 2][th.tid];
+    th.put(A.part_a + row * sh.D * sh.N, j, sh.N, j % 2 ? total.y : total.x);
+    if (seg == 0 && A.gs_in) th.put(A.gs_in + (size_t)th.b * sh.D * sh.N, j, sh.N, G[j]);
+  }
 }
 
 template <typename T, int LN> int launch_bwd(const BwdArgs& a, cudaStream_t stream) {
