@@ -52,6 +52,10 @@ OptTensor mask_of(const char* what, const OptTensor& mask, int64_t B, int64_t T,
   need_shape(what, "key_padding_mask", *mask, {B, T});
   return mask_bytes(mask, B * T, like);
 }
+// A kernel wrote to it: autograd is to notice where an earlier graph keeps it.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 bool wants(const OptTensor& t) { return t && t->requires_grad(); }
 template <class... Ts> bool records(const Ts&... ts) {      // decided in front of a node, whose own forward records nothing
   return at::GradMode::is_enabled() && (wants(OptTensor(ts)) || ...);
@@ -110,6 +114,7 @@ std::tuple<Tensor, OptTensor> causal_conv_fwd(const Tensor& x, const Tensor& wei
   if (v.empty()) return {y, in_place && state ? state : out};
   Call c(x);
   check(rfa_causal_conv_fwd(&v.c, y.data_ptr(), out && W > 1 ? out->data_ptr() : nullptr, c.stream), "rfa_causal_conv_fwd");
+  if (out && state && out->is_same(*state)) written(*state);
   if (out && in_place && state && !out->is_same(*state)) {
     state->copy_(*out);
     out = state;
@@ -248,6 +253,7 @@ std::tuple<Tensor, OptTensor, OptTensor> selective_scan_fwd(const Tensor& x, con
       Call call(x);
       check(rfa_selective_scan_step(&v.c, y.data_ptr(), out->data_ptr<float>(), call.stream), "rfa_selective_scan_step");
     }
+    if (here) written(*s);
   } else {
     if (return_state) out = fresh({x.size(1), x.size(2), a.size(1)}, x, at::kFloat);
     if (save) kept = scratch(rfa_selective_scan_checkpoint_bytes(v.c.T, v.c.B, v.c.D, v.c.N), x);

@@ -6,7 +6,8 @@ sequence's length.  Functional forms and the ``SelectiveStateSpace`` layer, in t
 * ``group_norm``                                    -> groups of a token's channels normalised, gated by silu(gate)
 
 Activations are time-major, ``[tgt_len, bsz, channels]``, fp16, bf16 or fp32, with any strides as long as channels are
-adjacent (views of a projection's output are taken as they are); sums and the scan's states are fp32.  No upstream counterpart.
+adjacent (views of a projection's output are taken as they are); sums and the scan's states are fp32.  At most 65535 sequences
+a call.  The backward passes are not differentiable themselves.  No upstream counterpart.
 
 ``key_padding_mask`` ``[bsz, tgt_len]`` (1 = padding): padded tokens are skipped, wherever they stand -- every result is
 what it would be without them, whatever values they hold, and their own outputs and gradients are zero.
@@ -161,7 +162,8 @@ def group_norm(*, x: Tensor, num_groups: int, weight: Optional[Tensor] = None, b
     """Each token's channels in ``num_groups`` runs of adjacent ones, every run brought to mean 0 and variance 1 (eps added
     to the variance), times weight plus bias: n.  Returns ``n * act(gate)``, without a gate ``act(n)``.
 
-    x and gate ``[..., channels]``, weight and bias ``[channels]``, all of one dtype; activation "silu" or None.  The
+    x and gate ``[..., channels]``, weight and bias ``[channels]``, all of one dtype, runs of at most 16384 channels;
+    activation "silu" or None.  The
     statistics are a token's own (``torch.nn.GroupNorm`` on ``[tokens, channels]``), so that a causal layer stays causal
     and a token's result does not depend on the ones it is called with."""
     silu = _silu(activation)

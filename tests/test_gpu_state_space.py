@@ -223,6 +223,26 @@ def test_scan_in_two_calls(dev, cut):
         assert (a - b).norm() <= 1e-6 * b.norm()
 
 
+def test_scan_with_more_rows_than_the_gpu_takes_side_by_side(dev):
+    """128 CTAs: the forward in one segment, the backward in two, whose summaries join."""
+    scan_check(dev, (230, 2, 4096, 16, 1), F32, "right", None)
+
+
+def test_scan_keeps_fp32_over_long_sequences(dev):
+    """Random errors of a chain of n steps grow as sqrt(n) half steps of 2^-24: a state's memory is at most 1000 tokens here (steps of 0.001), sums
+    over tokens are chains of T / 16 tiles.  With the special function unit's 2^-22, whose sign does not change, 2^-19 of the norm in
+    all; sums that keep fp32's precision are well below it, a chain of 4096 roundings to 16 bits is 2^-6."""
+    T, B, D, N = 4096, 1, 40, 16
+    gen = torch.Generator().manual_seed(9)
+    ins, g, gs = scan_inputs((T, B, D, N, 1), F32, gen)
+    want = O.scan(*[t.double() for t in ins.values()], None, True, g.double(), gs.double())
+    on = dict(zip(ins, leaves(*[t.to(dev) for t in ins.values()])))
+    y, s = ss.incremental_selective_scan(**on)
+    got = dict(zip(("gx", "gdt", "ga", "gb", "gc", "gd", "gbias", "gs"), torch.autograd.grad([y, s], list(on.values()), [g.to(dev), gs.to(dev)])), y=y, s=s)
+    for n, t in got.items():
+        assert (t.detach().cpu().double() - want[n]).norm() <= 2.0 ** -19 * want[n].norm(), n
+
+
 @pytest.mark.parametrize("value", [float("inf"), float("nan")])
 def test_scan_keeps_non_finite_values_where_they_belong(dev, value):
     """One token of one channel's x: its channel from that token on, its group's b and c gradients; nothing else."""
@@ -436,6 +456,39 @@ def test_states_that_cannot_be_updated_in_place_are_refused(dev):
         ss.group_norm(x=x, num_groups=3)
 
 
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("kind", ["conv", "scan"])
+def test_a_state_that_a_graph_keeps_is_not_overwritten_unnoticed(dev, kind, T):
+    _, ts = calls(dev, F32, T=T)[kind]
+    if kind == "conv":
+        s = torch.randn(3, 3, 64, device=dev)
+        call = lambda: ss.incremental_causal_conv(x=ts[0], weight=ts[1], state=s)
+    else:
+        s = torch.randn(3, 64, 16, device=dev)
+        call = lambda: ss.incremental_selective_scan(**dict(zip(("x", "dt", "a", "b", "c"), ts)), s=s)
+    ts[0].requires_grad_()
+    y, new = call()
+    assert new is not s
+    with torch.no_grad():
+        assert call()[1] is s
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("kind", ["conv", "scan"])
+def test_gradients_of_one_result_alone(dev, kind):
+    """Of y alone and of the state alone; together they are the sum."""
+    _, ts = calls(dev, F32)[kind]
+    ts = [t.requires_grad_() for t in ts]
+    if kind == "conv":
+        y, s = ss.incremental_causal_conv(x=ts[0], weight=ts[1], bias=ts[2])
+    else:
+        y, s = ss.incremental_selective_scan(**dict(zip(("x", "dt", "a", "b", "c", "d", "dt_bias"), ts)))
+    one, two, both = (torch.autograd.grad(sum(t.sum() for t in of), ts, retain_graph=True, allow_unused=True) for of in ((y,), (s,), (y, s)))
+    for a, b, c in zip(one, two, both):
+        assert (a + (0 if b is None else b) - c).norm() <= 1e-5 * c.norm()
+
+
 def test_a_state_at_an_odd_address_is_updated_in_place(dev):
     _, ts = calls(dev, T=1)["scan"]
     args = dict(zip(("x", "dt", "a", "b", "c", "d", "dt_bias"), ts))
@@ -560,6 +613,24 @@ def test_the_python_node_gives_the_native_ones_results(dev):
         assert torch.equal(got, want) and "Backward" in type(got.grad_fn).__name__
         for a, b in zip(torch.autograd.grad(got.sum(), ts), torch.autograd.grad(want.sum(), ts)):
             assert torch.equal(a, b)
+
+
+def test_a_compiled_caller_runs(dev):
+    for call, ts in calls(dev).values():
+        want = call(*ts)
+        assert torch.equal(torch.compile(lambda *a: call(*a) * 2, backend="eager")(*ts), want * 2)
+
+
+def test_one_tensor_as_several_inputs(dev):
+    """x as dt, b as c, x as its own gate: gradients add up as for separate tensors of the same values."""
+    _, (x, dt, a, b, c, d, bias) = calls(dev, F32)["scan"]
+    x, b = x.requires_grad_(), b.requires_grad_()
+    f = lambda x1, x2, b1, b2: ss.selective_scan(x=x1, dt=x2, a=a, b=b1, c=b2, d=d, dt_bias=bias).square().sum() + \
+        ss.group_norm(x=x1, num_groups=4, gate=x2).square().sum()
+    got = torch.autograd.grad(f(x, x, b, b), [x, b])
+    apart = [t.detach().clone().requires_grad_() for t in (x, x, b, b)]
+    want = torch.autograd.grad(f(*apart), apart)
+    assert torch.allclose(got[0], want[0] + want[1], rtol=1e-5, atol=1e-5) and torch.allclose(got[1], want[2] + want[3], rtol=1e-5, atol=1e-5)
 
 
 def test_tensor_level_calls(dev):
