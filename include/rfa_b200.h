@@ -471,7 +471,8 @@ typedef struct {
   int B, D, N, G, dtype, softplus;
 } rfa_scan_t;
 /* Scratch of a forward (backward = 0) or backward (1) call with `scan`'s sizes, and what
- * a forward leaves for the backward (the state in front of every 16th token). */
+ * a forward leaves for the backward (the state in front of every 16th token, every 8th
+ * with up to 8 states). */
 size_t rfa_selective_scan_workspace_bytes(int64_t T, int B, int D, int N, int G, int backward);
 size_t rfa_selective_scan_checkpoint_bytes(int64_t T, int B, int D, int N);
 /* y [T, B, D]; s_out [B, D, N] or NULL (not s_in); checkpoints or NULL. */

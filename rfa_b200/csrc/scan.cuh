@@ -19,7 +19,10 @@
 
 namespace rfa {
 
-constexpr int kScanTile = 16;      // tokens of a tile, and of a checkpoint
+constexpr int kScanTile = 16;      // tokens of a forward's tile
+// Tokens of a backward's tile, in front of each of which the forward leaves the states: fewer where a CTA has 128 channels, so that two CTAs' tiles
+// fit an SM (8 states, 8 x 2048 tokens x 2048 channels: 1215 us a training step with tiles of 16, one CTA per SM)
+__host__ __device__ constexpr int kept_tokens(int lanes) { return lanes == 2 ? 8 : 16; }
 
 struct ScanShape {
   int64_t T;
@@ -119,12 +122,14 @@ template <int R, bool kPoly> __device__ __forceinline__ void decays(const f32x2*
 
 // ---- the work of a thread ----------------------------------------------------------------------------------------------------
 // Of kScan threads that scan and kBring that bring and take, a pair of adjacent channels each.
-template <int LN, int kScan, int kBring> struct ScanThread {
+template <int LN, int kScan, int kBring, int kTokens> struct ScanThread {
   using Tile = ScanTile<LN>;
   static constexpr int kRows = kBring / Tile::kPairs;            // tokens that are brought side by side
-  static constexpr int kPasses = kScanTile / kRows;
+  static constexpr int kPasses = kTokens / kRows;
   static constexpr int kStep = kBring / Tile::kN;                // tokens whose b (and c) are
-  static constexpr int kBc = kScanTile / kStep;
+  static constexpr int kBc = kTokens > kStep ? kTokens / kStep : 1;
+  // whether the thread's elements of b and c are of the tile's tokens
+  __device__ __forceinline__ bool has_states() const { return kBc * kStep == kTokens || tid / Tile::kN < kTokens; }
   static_assert(kScan == LN * Tile::kPairs && kPasses >= 1 && kStep >= 1, "work for every thread");
   int group, c0, nch, b;          // the CTA's group, first channel, channels (<= kChannels), batch row
   bool scans;                     // or brings and takes
@@ -218,11 +223,13 @@ template <typename T, int LN, class Thread> struct RawStates {
 #pragma unroll
     for (int i = 0; i < Thread::kBc; ++i) {
       const int64_t t = t0 + th.tid / kN + i * kStep;
-      v[i] = kPlain || (t < T_ && n < N && !(mask && mask[t])) ? at[i * kStep * stride] : from_f<T>(0.f);
+      const bool there = n < N && th.has_states() && (kPlain || (t < T_ && !(mask && mask[t])));
+      v[i] = there ? at[i * kStep * stride] : from_f<T>(0.f);
     }
   }
   __device__ __forceinline__ void store(const Thread& th, float (*smem)[kN]) const {
     const int n = th.tid % kN, t = th.tid / kN;
+    if (!th.has_states()) return;
 #pragma unroll
     for (int i = 0; i < Thread::kBc; ++i) smem[t + i * kStep][(n % LN) * 4 + n / LN] = to_f(v[i]);
   }

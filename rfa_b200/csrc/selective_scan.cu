@@ -21,14 +21,15 @@ int scan_lanes(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 //   forward   16 CTAs 137 / 37, 64 CTAs 138 / 101 with about 592 in all; 128 CTAs 147 / 183, 160 CTAs 233 / 233, 256 CTAs 233 / 321
 //   backward  the same below 120; above, whatever fills the last round: 160 CTAs 855 / 603 in six, 320 CTAs (T = 1024) 686 / 588 in three,
 //             256 CTAs 877 / 906 in four, so one
-// Segments of less than six tiles lose to their own ends (16 CTAs, T = 2048: 19 segments 37 us, 32 segments 42).
+// Segments of less than 96 tokens lose to their own ends (16 CTAs, T = 2048: 19 segments 37 us, 32 segments 42).
 ScanShape scan_shape(int64_t T, int B, int D, int N, int G, bool backward) {
   ScanShape s{};
   const int channels = 256 / scan_lanes(N);
   s.T = T; s.B = B; s.D = D; s.N = N; s.G = G;
   s.heads = D / G;
   s.per_group = (s.heads + channels - 1) / channels;
-  s.tiles = (int)((T + kScanTile - 1) / kScanTile);
+  const int tokens = backward ? kept_tokens(scan_lanes(N)) : kScanTile;
+  s.tiles = (int)((T + tokens - 1) / tokens);
   s.kn = 4 * scan_lanes(N);
   const int64_t ctas = (int64_t)s.per_group * G * B;
   int64_t segs = 1;
@@ -42,7 +43,8 @@ ScanShape scan_shape(int64_t T, int B, int D, int N, int G, bool backward) {
       if (cost < 0.97 * best) { best = cost; segs = n; }
     }
   }
-  segs = segs < s.tiles / 6 ? segs : s.tiles / 6;
+  const int64_t most = T / 96;
+  segs = segs < most ? segs : most;
   if (segs < 1) segs = 1;
   s.seg_tiles = (int)((s.tiles + segs - 1) / segs);
   s.segs = (s.tiles + s.seg_tiles - 1) / s.seg_tiles;
@@ -72,13 +74,14 @@ template <int LN> struct __align__(16) FwdSmem {
 };
 
 constexpr int kFwdScan = 128, kFwdBring = 128, kFwdThreads = kFwdScan + kFwdBring;
-template <int LN> using FwdThread = ScanThread<LN, kFwdScan, kFwdBring>;
+template <int LN> using FwdThread = ScanThread<LN, kFwdScan, kFwdBring, kScanTile>;
 
 struct FwdArgs {
   ScanShape sh;
   rfa_scan_t p;
   void* y;
   float *s_out, *ckpt, *seg_state, *seg_sum;      // seg_state [segs - 1][B][D][kn], seg_sum [segs - 1][B][D]
+  int ckpts;                                      // of a batch row
   bool wide;                                      // pairs of x, dt and y as one word
 };
 
@@ -106,7 +109,7 @@ __device__ __forceinline__ void fwd_bring(const FwdArgs& A, FwdSmem<LN>& sm, con
   RawPairs<T, Thread> rx, rd, kept;
   RawStates<T, LN, Thread> rb, rc;
   uint32_t here = 0, next = 0;                         // which of this thread's tokens are there: in the tile that is scanned, in the next one
-  const int plain = A.wide && !mask && th.nch == Tile::kChannels && sh.N == Tile::kN ? (int)(sh.T / kScanTile) : 0;      // tiles in front of it are
+  const int plain = A.wide && !mask && th.nch == Tile::kChannels ? (int)(sh.T / kScanTile) : 0;      // tiles in front of it are
   const auto ask = [&](int tile, auto kind) {
     constexpr bool kPlain = decltype(kind)::value;
     const int64_t t0 = (int64_t)tile * kScanTile, t = t0 + th.row;
@@ -207,11 +210,14 @@ __global__ void __launch_bounds__(kFwdThreads, 2) scan_fwd_kernel(const __grid_c
     }
   for (int tile = tile0; tile < tile1; ++tile) {
     const int buf = (tile - tile0) & 1;
-    if (!kSummary && A.ckpt) th.store_kept(A.ckpt + ((size_t)th.b * sh.tiles + tile) * sh.D * sh.kn, s);
     meet_wait<kFwdThreads>(kFull + buf);
     constexpr int kRun = 4;                            // tokens whose decays are formed side by side
 #pragma unroll
     for (int t0 = 0; t0 < kScanTile; t0 += kRun) {
+      if (!kSummary && A.ckpt && t0 % kept_tokens(LN) == 0) {
+        const int at = tile * (kScanTile / kept_tokens(LN)) + t0 / kept_tokens(LN);
+        if (at < A.ckpts) th.store_kept(A.ckpt + ((size_t)th.b * A.ckpts + at) * sh.D * sh.kn, s);
+      }
       f32x2 delta[kRun], dx[kRun], e[kRun][4];
 #pragma unroll
       for (int r = 0; r < kRun; ++r) {
@@ -354,7 +360,8 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ 
 
 extern "C" size_t rfa_selective_scan_checkpoint_bytes(int64_t T, int B, int D, int N) {
   if (T <= 0 || B <= 0 || D <= 0 || N <= 0) return 0;
-  return (size_t)((T + rfa::kScanTile - 1) / rfa::kScanTile) * B * D * (4 * rfa::scan_lanes(N)) * 4;
+  const int lanes = rfa::scan_lanes(N), tokens = rfa::kept_tokens(lanes);
+  return (size_t)((T + tokens - 1) / tokens) * B * D * (4 * lanes) * 4;
 }
 
 extern "C" int rfa_selective_scan_fwd(const rfa_scan_t* scan, void* y, float* s_out, float* checkpoints, void* workspace, size_t workspace_bytes,
@@ -369,6 +376,7 @@ extern "C" int rfa_selective_scan_fwd(const rfa_scan_t* scan, void* y, float* s_
   a.sh = scan_shape(scan->T, scan->B, scan->D, scan->N, scan->G, false);
   a.p = *scan;
   a.y = y; a.s_out = s_out; a.ckpt = checkpoints;
+  a.ckpts = (int)((scan->T + kept_tokens(scan_lanes(scan->N)) - 1) / kept_tokens(scan_lanes(scan->N)));
   a.seg_state = static_cast<float*>(workspace);
   a.seg_sum = a.seg_state + (size_t)(a.sh.segs - 1) * scan->B * scan->D * a.sh.kn;
   const int size = scan->dtype == RFA_F32 ? 4 : 2;

@@ -4,7 +4,7 @@
 //   gdt_t = softplus'(dt_t + bias) (x_t sum_n G_t b_t + sum_n a p_t),  gbias = sum_t gdt_t.
 //
 // Layout in scan.cuh; tiles from the last to the first.  The states come back from the forward's checkpoints, one in front of every
-// 16 tokens (as many bytes as two 16-bit activations at 16 states, instead of all states): a tile is walked forward once for the state
+// tile (16 tokens: as many bytes as two 16-bit activations at 16 states, instead of all states): a tile is walked forward once for the state
 // in front of every second token, then two tokens at a time, from the last, forward with decays, decayed states and states left in
 // registers and backward.  Sums over states go over the LN lanes of a channel; sums over channels over a thread's two, then every four tokens
 // through shared memory to the warps that bring and take, over the CTA's pairs (12 instructions a token and thread, where exchanging
@@ -27,15 +27,16 @@ constexpr int kRun = 2;       // tokens whose decays and states are in registers
 constexpr int kPart = 4;      // tokens after which the scanning warps hand their partial sums over
 
 constexpr int kBwdScan = 128, kBwdBring = 128, kBwdThreads = kBwdScan + kBwdBring;
-template <int LN> using BwdThread = ScanThread<LN, kBwdScan, kBwdBring>;
+template <int LN> using BwdThread = ScanThread<LN, kBwdScan, kBwdBring, kept_tokens(LN)>;
 
 template <int LN> struct __align__(16) BwdSmem {
   using Tile = ScanTile<LN>;
-  float4 in[2][kScanTile][Tile::kPairs];               // delta, delta', delta x, delta' x' of two adjacent channels
-  float2 g[2][kScanTile][Tile::kPairs], slope[2][kScanTile][Tile::kPairs];      // g and softplus' of both
-  float b[2][kScanTile][Tile::kN], c[2][kScanTile][Tile::kN];
-  float4 res[kScanTile][Tile::kPairs];                 // sum_n G b of both channels, sum_n a log2(e) p of both
-  ulonglong2 start[kScanTile / kRun][2][kBwdScan]; // each thread's states in front of a run
+  static constexpr int kTokens = kept_tokens(LN);
+  float4 in[2][kTokens][Tile::kPairs];               // delta, delta', delta x, delta' x' of two adjacent channels
+  float2 g[2][kTokens][Tile::kPairs], slope[2][kTokens][Tile::kPairs];      // g and softplus' of both
+  float b[2][kTokens][Tile::kN], c[2][kTokens][Tile::kN];
+  float4 res[kTokens][Tile::kPairs];                 // sum_n G b of both channels, sum_n a log2(e) p of both
+  ulonglong2 start[kTokens / kRun][2][kBwdScan]; // each thread's states in front of a run
   ulonglong2 da[2][kBwdScan];                          // each thread's ga: tiles are summed apart (one chain of 2048 tokens is 1e-6 off)
   float4 over_ch[2][kPart][2][Tile::kPairs][LN];       // gb and gc of each pair's channels, a lane's four states adjacent; two parts by turns
 };
@@ -44,8 +45,9 @@ enum { kSums = 5, kTaken = 7 };
 
 template <int LN> struct __align__(16) SummarySmem {
   using Tile = ScanTile<LN>;
-  float4 in[kScanTile][Tile::kPairs];                  // delta, delta', g, g'
-  float c[kScanTile][Tile::kN];
+  static constexpr int kTokens = kept_tokens(LN);
+  float4 in[kTokens][Tile::kPairs];                  // delta, delta', g, g'
+  float c[kTokens][Tile::kN];
 };
 
 struct BwdArgs {
@@ -65,7 +67,8 @@ constexpr int kSummaryThreads = 128;
 template <typename T, int LN>
 __global__ void __launch_bounds__(kSummaryThreads) scan_bwd_summary_kernel(const __grid_constant__ BwdArgs A) {
   using Tile = ScanTile<LN>;
-  using Thread = ScanThread<LN, kSummaryThreads, kSummaryThreads>;      // each does both
+  constexpr int kTokens = kept_tokens(LN);
+  using Thread = ScanThread<LN, kSummaryThreads, kSummaryThreads, kTokens>;      // each does both
   __shared__ SummarySmem<LN> sm;
   const ScanShape& sh = A.sh;
   const rfa_scan_t& p = A.p;
@@ -90,10 +93,10 @@ __global__ void __launch_bounds__(kSummaryThreads) scan_bwd_summary_kernel(const
   RawPairs<T, Thread> rd, rg;
   RawStates<T, LN, Thread> rc;
   uint32_t next = 0;
-  const int plain = A.wide && !mask && th.nch == Tile::kChannels && sh.N == Tile::kN ? (int)(sh.T / kScanTile) : 0;      // tiles in front of it are
+  const int plain = A.wide && !mask && th.nch == Tile::kChannels ? (int)(sh.T / kTokens) : 0;      // tiles in front of it are
   const auto ask = [&](int tile, auto kind) {
     constexpr bool kPlain = decltype(kind)::value;
-    const int64_t t0 = (int64_t)tile * kScanTile, t = t0 + th.row;
+    const int64_t t0 = (int64_t)tile * kTokens, t = t0 + th.row;
     next = kPlain ? ~0u : th.tokens_here(mask, t0, sh.T);
     rd.template load<kPlain>(dt + t * p.dt_t, p.dt_t, next, th.vn, A.wide);
     rg.template load<kPlain>(g + t * row_stride, row_stride, next, th.vn, A.wide);
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(kSummaryThreads) scan_bwd_summary_kernel(const
     if (tile > tile0) ask_tile(tile - 1);
     constexpr int kLook = 4;                           // tokens whose decays are formed side by side
 #pragma unroll
-    for (int t0 = kScanTile - kLook; t0 >= 0; t0 -= kLook) {
+    for (int t0 = kTokens - kLook; t0 >= 0; t0 -= kLook) {
       f32x2 delta[kLook], gt[kLook], e[kLook][4];
 #pragma unroll
       for (int r = 0; r < kLook; ++r) {
@@ -148,6 +151,7 @@ template <typename T, int LN>
 __device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, const BwdThread<LN>& th, int seg, int tile0, int tile1) {
   using Tile = ScanTile<LN>;
   using Thread = BwdThread<LN>;
+  constexpr int kTokens = kept_tokens(LN);
   const ScanShape& sh = A.sh;
   const rfa_scan_t& p = A.p;
   const int ch = th.c0 + 2 * th.vpair;
@@ -167,10 +171,10 @@ __device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, con
   RawPairs<T, Thread> rx, rd, rg, kept;
   RawStates<T, LN, Thread> rb, rc;
   uint32_t here = 0, next = 0;                         // which of this thread's tokens are there: in the tile that is scanned, in the next one
-  const int plain = A.wide && !mask && th.nch == Tile::kChannels && sh.N == Tile::kN ? (int)(sh.T / kScanTile) : 0;      // tiles in front of it are
+  const int plain = A.wide && !mask && th.nch == Tile::kChannels ? (int)(sh.T / kTokens) : 0;      // tiles in front of it are
   const auto ask = [&](int tile, auto kind) {
     constexpr bool kPlain = decltype(kind)::value;
-    const int64_t t0 = (int64_t)tile * kScanTile, t = t0 + th.row;
+    const int64_t t0 = (int64_t)tile * kTokens, t = t0 + th.row;
     next = kPlain ? ~0u : th.tokens_here(mask, t0, sh.T);
     rx.template load<kPlain>(x + t * p.x_t, p.x_t, next, th.vn, A.wide);
     rd.template load<kPlain>(dt + t * p.dt_t, p.dt_t, next, th.vn, A.wide);
@@ -272,14 +276,19 @@ __device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, con
       meet_go<kBwdThreads>(kFull + (buf ^ 1));
       if (tile - 1 > tile0) ask_tile(tile - 2);
     }
-    const int64_t t0 = (int64_t)tile * kScanTile;
+    const int64_t t0 = (int64_t)tile * kTokens;
 #pragma unroll 1
-    for (int part = kScanTile / kPart - 1; part >= 0; --part) {
+    for (int part = kTokens / kPart - 1; part >= 0; --part) {
       const int w = part & 1;
       meet_wait<kBwdThreads>(kSums + w);
+      // The part's place is given back, where somebody waits for it, before its gradients are stored: the scanning warps come to its rows of
+      // res a tile on, and wait for another part's place in between -- unless a tile is two parts.
+      constexpr bool kEarly = kTokens > 2 * kPart;
+      const bool wanted = tile > tile0 || part > 1;
       sum(t0, part, w);
-      if (tile > tile0 || part > 1) meet_go<kBwdThreads>(kTaken + w);      // somebody waits for it (and reaches this part's rows of res four parts on)
+      if (kEarly && wanted) meet_go<kBwdThreads>(kTaken + w);
       take(t0, buf, part);
+      if (!kEarly && wanted) meet_go<kBwdThreads>(kTaken + w);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -314,6 +323,7 @@ __device__ __forceinline__ void bwd_bring(const BwdArgs& A, BwdSmem<LN>& sm, con
 template <typename T, int LN>
 __global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_constant__ BwdArgs A) {
   using Smem = BwdSmem<LN>;
+  constexpr int kTokens = kept_tokens(LN);
   extern __shared__ char smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const ScanShape& sh = A.sh;
@@ -361,7 +371,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_c
     for (int run = 0;; ++run) {
       sm.start[run][0][th.tid] = make_ulonglong2(s[0], s[1]);
       sm.start[run][1][th.tid] = make_ulonglong2(s[2], s[3]);
-      if (run == kScanTile / kRun - 1) break;
+      if (run == kTokens / kRun - 1) break;
       f32x2 delta[kRun], dx[kRun], e[kRun][4];
       inputs(run * kRun, delta, dx);
       decays<kRun, false>(delta, a2, e);               // over at most 15 tokens: the special function unit's own error does not add up
@@ -375,7 +385,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_c
     }
     if (tile > tile0) th.load_kept(ckpt + (size_t)(tile - 1) * sh.D * sh.kn, s);      // asked for early
 #pragma unroll 2
-    for (int run = kScanTile / kRun - 1; run >= 0; --run) {
+    for (int run = kTokens / kRun - 1; run >= 0; --run) {
       const int base = run * kRun, w = base / kPart & 1;
       f32x2 delta[kRun], dx[kRun], e[kRun][4], q[kRun][4], st[kRun][4];      // decays, decayed states, states
       float bt[kRun][4];
@@ -393,7 +403,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_c
         }
       }
       // the part's place is free
-      if (base % kPart == kPart - kRun && (tile < tile1 - 1 || base < kScanTile - 2 * kPart)) meet_wait<kBwdThreads>(kTaken + w);
+      if (base % kPart == kPart - kRun && (tile < tile1 - 1 || base < kTokens - 2 * kPart)) meet_wait<kBwdThreads>(kTaken + w);
 #pragma unroll
       for (int r = kRun - 1; r >= 0; --r) {
         const f32x2 gt = *reinterpret_cast<const f32x2*>(&sm.g[buf][base + r][th.pair]);

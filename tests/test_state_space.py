@@ -130,7 +130,8 @@ def test_c_abi_refuses_before_a_device_is_touched():
     long = Scan(**{**scan, "T": 1 << 16})
     assert lib.rfa_selective_scan_workspace_bytes(1 << 16, 2, 8, 16, 1, 0) > 0           # few rows: cut into segments
     assert lib.rfa_selective_scan_fwd(C.addressof(long), 16, None, None, None, 0, None) == EWORKSPACE
-    assert lib.rfa_selective_scan_checkpoint_bytes(17, 2, 8, 3) == 2 * 2 * 8 * 8 * 4
+    assert lib.rfa_selective_scan_checkpoint_bytes(17, 2, 8, 3) == 3 * 2 * 8 * 8 * 4
+    assert lib.rfa_selective_scan_checkpoint_bytes(17, 2, 8, 16) == 2 * 2 * 8 * 16 * 4
     norm = dict(x=16, x_r=8, rows=3, C=8, groups=2)
     for status, change in ((EINVAL, dict(x=None)), (EINVAL, dict(rows=0)), (EINVAL, dict(groups=0)), (EUNSUPPORTED, dict(groups=3)),
                            (EUNSUPPORTED, dict(dtype=-1)), (EUNSUPPORTED, dict(C=32768, groups=1))):
