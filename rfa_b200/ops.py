@@ -1,7 +1,7 @@
 """Tensor-level wrappers over the C ABI: allocate outputs, pass raw pointers and
 the current stream, turn status codes into exceptions.  No arithmetic happens
 here; every function launches kernels from ``librfa_b200.so``.  The calls of the
-forward, backward and decoding paths are in ``csrc/torch_ops.cpp``; the rest go
+forward, backward and decoding paths are in ``csrc/torch_ops.cpp``, those of the state-space operators in ``csrc/torch_state_space.cpp``; the rest go
 through ctypes.
 """
 from __future__ import annotations
