@@ -427,8 +427,8 @@ int rfa_stream_probe(const void* in, void* out, int64_t T, int BH, int nb, int w
  * there, whatever stands in them, and a padded token's outputs and gradients
  * are zero.  No alignment is asked for beyond the elements' own, except that
  * states, checkpoints and workspaces are 16-byte aligned.  T < 2^31 - 64,
- * B <= 65535 (convolution: T D < 2^44); a size of zero is refused (there is
- * nothing to launch).  What a batch row holds reaches no other row's results; the
+ * B <= 65535, D and C <= 2^24 (convolution: T D < 2^44); a size of zero is
+ * refused (there is nothing to launch).  What a batch row holds reaches no other row's results; the
  * same call gives the same bits.
  * ---------------------------------------------------------------------- */
 

@@ -416,7 +416,7 @@ int conv_check(const rfa_causal_conv_t* p, const char* what) {
   RFA_REQUIRE(p->T > 0 && p->B > 0 && p->D > 0, RFA_EINVAL, "%s: empty or negative size", what);
   RFA_REQUIRE(p->dtype == RFA_F16 || p->dtype == RFA_F32 || p->dtype == RFA_BF16, RFA_EUNSUPPORTED, "%s: dtype %d", what, p->dtype);
   RFA_REQUIRE(p->W >= 1 && p->W <= kConvMax, RFA_EUNSUPPORTED, "%s: a window of %d tokens (1 to %d)", what, p->W, kConvMax);
-  RFA_REQUIRE(p->T < ((int64_t)1 << 31) - 64 && p->B <= 65535 && p->T / 128 * p->D < (int64_t)1 << 37, RFA_EUNSUPPORTED, "%s: T %lld, B %d, D %d", what,
+  RFA_REQUIRE(p->T < ((int64_t)1 << 31) - 64 && p->B <= 65535 && p->D <= kMaxChannels && p->T / 128 * p->D < (int64_t)1 << 37, RFA_EUNSUPPORTED, "%s: T %lld, B %d, D %d", what,
               (long long)p->T, p->B, p->D);
   return 0;
 }

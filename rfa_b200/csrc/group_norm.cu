@@ -354,6 +354,7 @@ int norm_run(NormArgs a, const char* what, void* workspace, size_t workspace_byt
   RFA_REQUIRE(p.rows > 0 && p.C > 0 && p.groups > 0, RFA_EINVAL, "%s: empty or negative size", what);
   RFA_REQUIRE(p.dtype == RFA_F16 || p.dtype == RFA_F32 || p.dtype == RFA_BF16, RFA_EUNSUPPORTED, "%s: dtype %d", what, p.dtype);
   RFA_REQUIRE(p.C % p.groups == 0 && p.C / p.groups <= 16384, RFA_EUNSUPPORTED, "%s: %d channels in %d groups (of at most 16384)", what, p.C, p.groups);
+  RFA_REQUIRE(p.C <= kMaxChannels, RFA_EUNSUPPORTED, "%s: %d channels", what, p.C);
   a.size = p.C / p.groups;
   const int bytes = p.dtype == RFA_F32 ? 4 : 2, nv = bytes == 2 ? 8 : 4;
   a.over_size = 1.f / (float)a.size;

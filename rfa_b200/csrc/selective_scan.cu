@@ -58,7 +58,8 @@ int scan_check(const rfa_scan_t* s, const char* what) {
   RFA_REQUIRE(s->dtype == RFA_F16 || s->dtype == RFA_F32 || s->dtype == RFA_BF16, RFA_EUNSUPPORTED, "%s: dtype %d", what, s->dtype);
   RFA_REQUIRE(s->D % s->G == 0, RFA_EUNSUPPORTED, "%s: %d channels in %d groups", what, s->D, s->G);
   RFA_REQUIRE(s->N <= 64, RFA_EUNSUPPORTED, "%s: %d states (at most 64)", what, s->N);
-  RFA_REQUIRE(s->T < ((int64_t)1 << 31) - 64 && s->B <= 65535, RFA_EUNSUPPORTED, "%s: T %lld, B %d", what, (long long)s->T, s->B);
+  RFA_REQUIRE(s->T < ((int64_t)1 << 31) - 64 && s->B <= 65535 && s->D <= kMaxChannels, RFA_EUNSUPPORTED, "%s: T %lld, B %d, D %d", what, (long long)s->T,
+              s->B, s->D);
   RFA_REQUIRE(aligned16(s->s_in), RFA_EALIGN, "%s: s_in is not 16-byte aligned", what);
   return 0;
 }

@@ -133,6 +133,8 @@ __device__ __forceinline__ float softplus(float v, float& sig) {
   return fmaxf(v, 0.f) + w * q;
 }
 
+constexpr int kMaxChannels = 1 << 24;     // a call: with 64 states or 8 taps a channel, their indexes and thread numbers stay below 2^31
+
 // ---- sums of partial results: dst[i] = sum over p of src[p * n + i], in a fixed order ----------------------------------------
 struct SumJob {
   const float* src;

@@ -7,7 +7,7 @@ sequence's length.  Functional forms and the ``SelectiveStateSpace`` layer, in t
 
 Activations are time-major, ``[tgt_len, bsz, channels]``, fp16, bf16 or fp32, with any strides as long as channels are
 adjacent (views of a projection's output are taken as they are); sums and the scan's states are fp32.  At most 65535 sequences
-a call.  The backward passes are not differentiable themselves.  No upstream counterpart.
+and 2^24 channels a call.  The backward passes are not differentiable themselves.  No upstream counterpart.
 
 ``key_padding_mask`` ``[bsz, tgt_len]`` (1 = padding): padded tokens are skipped, wherever they stand -- every result is
 what it would be without them, whatever values they hold, and their own outputs and gradients are zero.

@@ -142,6 +142,21 @@ def test_c_abi_refuses_before_a_device_is_touched():
     assert lib.rfa_group_norm_bwd(C.addressof(s), 16, 8, 16, None, 16, None, None, 0, None) == EWORKSPACE
 
 
+def test_c_abi_refuses_more_channels_than_its_indexes_hold():
+    lib, most = _lib.load(), 1 << 24
+    for d in (most + 1, 1 << 28, (1 << 31) - 1):
+        conv = Conv(x=16, x_t=d, x_b=d, weight=16, T=1, B=1, D=d, W=4)
+        assert lib.rfa_causal_conv_fwd(C.addressof(conv), 16, None, None) == EUNSUPPORTED
+        assert lib.rfa_causal_conv_bwd(C.addressof(conv), 16, d, d, None, 16, None, None, None, None, 0, None) == EUNSUPPORTED
+        scan = Scan(x=16, dt=16, a=16, b=16, c=16, T=1, B=1, D=d, N=64, G=1)
+        assert lib.rfa_selective_scan_fwd(C.addressof(scan), 16, None, None, None, 0, None) == EUNSUPPORTED
+        assert lib.rfa_selective_scan_step(C.addressof(scan), 16, 16, None) == EUNSUPPORTED
+        assert lib.rfa_selective_scan_bwd(C.addressof(scan), *[16] * 11, 16, 1 << 40, None) == EUNSUPPORTED
+        norm = Norm(x=16, x_r=d, rows=1, C=d, groups=d)
+        assert lib.rfa_group_norm_fwd(C.addressof(norm), 16, None) == EUNSUPPORTED
+        assert lib.rfa_group_norm_bwd(C.addressof(norm), 16, d, 16, None, None, None, None, 0, None) == EUNSUPPORTED
+
+
 def test_older_entry_points_refuse_bf16():
     """The code of bf16 names a type of the state-space entry points only."""
     lib = _lib.load()
