@@ -3,7 +3,7 @@
 //   gx = rstd (h - mean(h) - xhat mean(h xhat)), h = gn w,  gw = sum over rows of gn xhat,  gbias = sum of gn,  ggate = g n silu'(gate).
 //
 // Bound by memory: x and gate once, y once (backward: x, gate, g; gx, ggate); 8 x 2048 tokens x 2048 channels in groups of 64, bf16, forward:
-// 41 us, 4.9 TB/s of 6.5 (issue slots are 75 % busy; a launch of one row per thread, with weight and bias read for each, took 60 us).
+// 41 us, 4.9 TB/s of 6.5 (issue slots are 73 % busy; a launch of one row per thread, with weight and bias read for each, took 60 us).
 // A group stays in the registers of 1 to 512 threads, with 16-byte
 // words where the sizes allow; threads keep their channels, and weight and bias, over many rows, the next of which is on the way; mean and variance are two passes over registers (no difference of squares), joined by
 // shuffles, beyond a warp through shared memory.  The backward forms the statistics again rather than reading them; the

@@ -3,7 +3,7 @@
 //
 // Bound by arithmetic: one exponential per token, channel and state, where a token and channel of 16 states moves 6 bytes in 16 bits
 // (8 x 2048 tokens x 2048 channels: 537 M exponentials are 119 us of the special function units, 201 MB are 31 us of memory).  That size
-// takes 226 to 230 us in bf16: of the 105 cycles of a token on an SM's scheduler the special function unit is busy for 60 (with softplus),
+// takes 226 to 230 us in bf16: of the 105 cycles of a token on an SM's scheduler the special function unit is busy for 56 (with softplus),
 // the FMA units for 63, shared memory for 61 of the SM's, and 68 are issue slots; 256 CTAs on 148 SMs leave a seventh of the card idle.
 // Tiles of 32 tokens: 220 us, for twice the shared memory and code.  Layout in scan.cuh.
 //

@@ -11,7 +11,7 @@
 // them within the warp takes 28), then over CTAs in sum_parts: a fixed order, no atomics.
 //
 // 8 x 2048 tokens x 2048 channels x 16 states, bf16: about 860 of the 1100 us of a training step.  Bound by issue slots (224 instructions a
-// token and warp), shared memory (55 passes of 128 bytes) and the FMA units (180 cycles) together, each 50 to 60 % busy of the 385 cycles that
+// token and warp), shared memory (55 passes of 128 bytes) and the FMA units (190 cycles) together, each 50 to 60 % busy of the 385 cycles that
 // a token takes; memory traffic is 5 % of what could be.  Taking away one of its parts (the sums over channels, over states, the walk for
 // the states) saves 7 to 9 % each.  Also measured: four channels a thread (one scanning warp per scheduler, 1430 us a step), parts of two
 // tokens (1310), mbarriers instead of named barriers (1180), exponentials of the special function unit alone (1120), four tokens in
