@@ -25,7 +25,7 @@ struct ConvArgs {
   void *gx, *g_state_in;
   float *part_w, *part_b;      // [row_blocks * B][D][W], [row_blocks * B][D]; null: not wanted
   int row_blocks, ch_blocks;   // a CTA's place: channels fastest, so that what runs side by side reads whole rows
-  bool wide;
+  bool wide, wide_w;           // vectors of activations and states, a vector's weights in wide accesses
 };
 
 // The last token before t that is not masked, -1 for none; all lanes of a warp together.
@@ -83,7 +83,7 @@ template <typename T, int NV, int W, bool kMask> struct ConvThread {
     x = static_cast<const T*>(p.x) + (int64_t)b * p.x_b + c0;
     mask = kMask ? p.mask + (int64_t)b * p.T : nullptr;
     Raw<T, NV * W> rw;
-    rw.load(static_cast<const T*>(p.weight) + (size_t)c0 * W, n * W, wide);
+    rw.load(static_cast<const T*>(p.weight) + (size_t)c0 * W, n * W, a.wide_w);
     Raw<T, NV> rb;
     rb.zero();
     if (p.bias) rb.load(static_cast<const T*>(p.bias) + c0, n, wide);
@@ -458,7 +458,8 @@ extern "C" int rfa_causal_conv_fwd(const rfa_causal_conv_t* conv, void* y, void*
   a.row_blocks = conv_row_blocks(conv->T);
   a.ch_blocks = (conv->D + 32 * nv - 1) / (32 * nv);
   a.wide = wide_ok(conv->x, conv->x_t, conv->x_b, size, nv) && wide_ok(y, conv->D, 0, size, nv) && wide_ok(state_out, 0, 0, size, nv) &&
-           wide_ok(conv->state_in, 0, 0, size, nv) && wide_ok(conv->weight, 0, 0, size, nv) && wide_ok(conv->bias, 0, 0, size, nv);
+           wide_ok(conv->state_in, 0, 0, size, nv) && wide_ok(conv->bias, 0, 0, size, nv);
+  a.wide_w = wide_ok(conv->weight, 0, 0, size, nv * conv->W);
   return conv_dtype(a, false, as_stream(stream));
 }
 
@@ -492,7 +493,8 @@ extern "C" int rfa_causal_conv_bwd(const rfa_causal_conv_t* conv, const void* g,
   a.ch_blocks = (conv->D + 32 * nv - 1) / (32 * nv);
   a.wide = wide_ok(conv->x, conv->x_t, conv->x_b, size, nv) && wide_ok(g, g_t, g_b, size, nv) && wide_ok(gx, conv->D, 0, size, nv) &&
            wide_ok(conv->state_in, 0, 0, size, nv) && wide_ok(a.g_state, 0, 0, size, nv) && wide_ok(a.g_state_in, 0, 0, size, nv) &&
-           wide_ok(conv->weight, 0, 0, size, nv) && wide_ok(conv->bias, 0, 0, size, nv);
+           wide_ok(conv->bias, 0, 0, size, nv);
+  a.wide_w = wide_ok(conv->weight, 0, 0, size, nv * conv->W);
   if (int r = conv_dtype(a, true, as_stream(stream))) return r;
   const SumJob jobs[2] = {{a.part_w, g_weight, (int64_t)conv->D * conv->W, parts, conv->dtype}, {a.part_b, g_bias, conv->D, parts, conv->dtype}};
   return weights ? sum_parts(jobs, 2, as_stream(stream)) : 0;

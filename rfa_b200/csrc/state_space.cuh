@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "wide.h"
 
 namespace rfa {
 
@@ -24,6 +25,7 @@ struct Raw {
     for (int i = 0; i < kWords; ++i) w[i] = 0;
   }
   static constexpr int kStep = kWords % 4 == 0 ? 4 : kWords % 2 == 0 ? 2 : 1;      // words of a wide access
+  static_assert(kStep * 4 == access_bytes(NV * (int)sizeof(T)), "what wide_ok asks for");
   // `wide`: the address is a multiple of a wide access; n elements are there
   __device__ __forceinline__ void load(const T* p, int n, bool wide) {
     if (wide && n >= NV) {
@@ -101,12 +103,6 @@ struct Raw {
     }
   }
 };
-
-// Whether runs of NV elements at p, p + stride ... may be taken in wide accesses (of at most 16 bytes).
-inline bool wide_ok(const void* p, int64_t stride, int64_t stride2, int size, int nv) {
-  const int64_t bytes = nv * size < 16 ? nv * size : 16;
-  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0 && stride2 * size % bytes == 0;
-}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

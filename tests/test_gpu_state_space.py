@@ -135,6 +135,28 @@ def test_convolution_of_one_long_row_of_padding(dev):
     assert torch.equal(state[0], x[there[-3:], 0]) and int(y.ne(0).any(-1).sum()) == len(there)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("width", range(1, 9))
+def test_convolution_parameters_anywhere_in_a_flat_buffer(dev, width, dtype):
+    """Weights and biases are taken at any element's address, forward, backward and one token, with the bits of aligned ones."""
+    T, B, D = 37, 2, 136
+    gen = torch.Generator().manual_seed(width)
+    draw = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(dev)
+    x, g, w, b, s = draw(T, B, D).requires_grad_(), draw(T, B, D), draw(D, width), draw(D), draw(B, width - 1, D)
+    flat = lambda t, at: torch.cat([t.new_zeros(at), t.flatten()])[at:].view(t.shape).detach().requires_grad_()
+    want = None
+    for at in (0, 1, 2, 3, 4, 6, 8):
+        wd, bd = flat(w, at), flat(b, at)
+        assert wd.is_contiguous() and wd.data_ptr() % 16 == at * wd.element_size() % 16
+        y = ss.causal_conv(x=x, weight=wd, bias=bd)
+        got = [y, *torch.autograd.grad(y, [x, wd, bd], g)]
+        with torch.no_grad():
+            one, held = ss.incremental_causal_conv(x=x[:1], weight=wd, bias=bd, state=s.clone())
+        got += [one, held]
+        want = want or got
+        assert all(torch.equal(a, c) for a, c in zip(got, want)), at
+
+
 # --------------------------------------------------------------------------- selective scan
 SCAN = [(1, 1, 1, 1, 1), (1, 3, 8, 16, 1), (2, 2, 6, 3, 2), (15, 2, 64, 16, 1), (16, 3, 40, 4, 1), (17, 1, 72, 8, 1), (33, 2, 130, 12, 1), (48, 1, 136, 17, 2),
         (65, 2, 36, 32, 4), (80, 2, 24, 33, 1), (70, 1, 16, 64, 1), (150, 3, 264, 16, 1), (531, 1, 48, 16, 2), (700, 1, 20, 64, 1)]

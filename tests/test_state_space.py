@@ -178,3 +178,26 @@ def test_reordering_keeps_the_state_of_the_old_slot():
 def test_tensor_calls_are_exported():
     for name in ("causal_conv_fwd", "causal_conv_bwd", "selective_scan_fwd", "selective_scan_bwd", "group_norm_fwd", "group_norm_bwd"):
         assert callable(getattr(ops, name)) and callable(getattr(_lib.native(), name))
+
+
+def test_wide_accesses_are_taken_of_addresses_that_hold_them(tmp_path):
+    """The host's rule, by itself: a run of `nv` elements is taken in words of 16, 8 or 4 bytes, whichever divides it; an address that is
+    not a multiple of them is refused, and none that is."""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    src, exe = tmp_path / "wide.cpp", tmp_path / "wide"
+    src.write_text('#include "wide.h"\n#include <cstdio>\n#include <initializer_list>\n'
+                   "int main() {\n"
+                   "  for (int size : {2, 4}) for (int nv = 2; nv <= 32; nv += 2) for (int at = 0; at < 32; at += size)\n"
+                   '    std::printf("%d %d %d %d\\n", size, nv, at, (int)rfa::wide_ok(reinterpret_cast<const void*>((uintptr_t)4096 + at), 0, 0, size, nv));\n'
+                   "}\n")
+    subprocess.run(["g++", "-std=c++17", "-I" + csrc, str(src), "-o", str(exe)], check=True)
+    rows = [tuple(map(int, line.split())) for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()]
+    assert len(rows) == 16 * (16 + 8)
+    for size, nv, at, taken in rows:
+        words = nv * size // 4                                    # a run in 32-bit words: four, two or one of them at a time
+        access = 16 if words % 4 == 0 else 8 if words % 2 == 0 else 4
+        assert bool(taken) == (at % access == 0), (size, nv, at)
+    # the convolution's weights: 4 channels of `width` taps; 8 modulo 16 holds them in 16 bits only where the width is odd
+    assert {w: dict(((s, n, a), t) for s, n, a, t in rows)[2, 4 * w, 8] for w in range(1, 9)} == {1: 1, 2: 0, 3: 1, 4: 0, 5: 1, 6: 0, 7: 1, 8: 0}
