@@ -49,9 +49,9 @@ __device__ __forceinline__ int64_t token_after(const uint8_t* mask, int64_t t, i
   return T;
 }
 
-template <typename T, int NV> __device__ __forceinline__ void load_row(const T* p, int n, bool wide, float* v) {
+template <typename T, int NV, bool kConst = true> __device__ __forceinline__ void load_row(const T* p, int n, bool wide, float* v) {
   Raw<T, NV> r;
-  r.load(p, n, wide);
+  r.template load<kConst>(p, n, wide);
 #pragma unroll
   for (int c = 0; c < NV; ++c) v[c] = r.get(c);
 }
@@ -99,7 +99,8 @@ template <typename T, int NV, int W, bool kMask> struct ConvThread {
     const int64_t t = t0 + (threadIdx.x & 31);
     return __ballot_sync(0xffffffffu, t < t1 && !(kMask && mask[t]));
   }
-  // win[0 .. W - 2]: the tokens in front of t0, oldest first; at[]: where they stand (-1 ... -(W - 1): in the incoming state)
+  // win[0 .. W - 2]: the tokens in front of t0, oldest first; at[]: where they stand (-1 ... -(W - 1): in the incoming state,
+  // which may be the outgoing one of a single token: not a constant of the launch)
   __device__ __forceinline__ void before(float (*win)[NV], int* at) const {
     int64_t t = t0;
     int slot = W - 2;                                  // of the incoming state
@@ -111,7 +112,7 @@ template <typename T, int NV, int W, bool kMask> struct ConvThread {
         load_row<T, NV>(x + t * p.x_t, n, wide, win[j]);
         at[j] = (int)t;
       } else {
-        if (p.state_in) load_row<T, NV>(static_cast<const T*>(p.state_in) + ((size_t)b * (W - 1) + slot) * p.D + c0, n, wide, win[j]);
+        if (p.state_in) load_row<T, NV, false>(static_cast<const T*>(p.state_in) + ((size_t)b * (W - 1) + slot) * p.D + c0, n, wide, win[j]);
         else
 #pragma unroll
           for (int c = 0; c < NV; ++c) win[j][c] = 0.f;

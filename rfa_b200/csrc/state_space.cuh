@@ -26,20 +26,25 @@ struct Raw {
   }
   static constexpr int kStep = kWords % 4 == 0 ? 4 : kWords % 2 == 0 ? 2 : 1;      // words of a wide access
   static_assert(kStep * 4 == access_bytes(NV * (int)sizeof(T)), "what wide_ok asks for");
-  // `wide`: the address is a multiple of a wide access; n elements are there
-  __device__ __forceinline__ void load(const T* p, int n, bool wide) {
+  // `wide`: the address is a multiple of a wide access; n elements are there.  kConst: nobody writes to them during the launch, so that the
+  // read-only path may be taken; a state that is updated in place is not constant.
+  template <bool kConst = true> __device__ __forceinline__ void load(const T* p, int n, bool wide) {
+    const auto get = [](const auto* at) {
+      if constexpr (kConst) return __ldg(at);
+      else return *at;
+    };
     if (wide && n >= NV) {
 #pragma unroll
       for (int i = 0; i < kWords; i += kStep) {
         const uint32_t* at = reinterpret_cast<const uint32_t*>(p) + i;
         if constexpr (kStep == 4) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
+          const uint4 v = get(reinterpret_cast<const uint4*>(at));
           w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
         } else if constexpr (kStep == 2) {
-          const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+          const uint2 v = get(reinterpret_cast<const uint2*>(at));
           w[i] = v.x; w[i + 1] = v.y;
         } else {
-          w[i] = __ldg(at);
+          w[i] = get(at);
         }
       }
     } else {

@@ -157,6 +157,22 @@ def test_convolution_parameters_anywhere_in_a_flat_buffer(dev, width, dtype):
         assert all(torch.equal(a, c) for a, c in zip(got, want)), at
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("width", [2, 3, 4, 8])
+def test_a_kept_window_is_updated_in_place_token_by_token(dev, width, dtype):
+    """Every CTA reads the window that it writes: the same bits as from one buffer into another, some tokens padded."""
+    B, D = 37, 1028
+    gen = torch.Generator().manual_seed(width)
+    draw = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(dev)
+    x, w, b, s = draw(9, B, D), draw(D, width), draw(D), draw(B, width - 1, D)
+    mask = (torch.rand(9, B, 1, generator=gen) < 0.3).to(dev)
+    held, apart = s.clone(), s
+    for t in range(9):
+        y, same = ss.incremental_causal_conv(x=x[t:t + 1], weight=w, bias=b, state=held, key_padding_mask=mask[t])
+        want, apart = ops.causal_conv_fwd(x[t:t + 1], w, b, apart, mask[t], True, True)
+        assert same is held and torch.equal(y, want) and torch.equal(held, apart)
+
+
 # --------------------------------------------------------------------------- selective scan
 SCAN = [(1, 1, 1, 1, 1), (1, 3, 8, 16, 1), (2, 2, 6, 3, 2), (15, 2, 64, 16, 1), (16, 3, 40, 4, 1), (17, 1, 72, 8, 1), (33, 2, 130, 12, 1), (48, 1, 136, 17, 2),
         (65, 2, 36, 32, 4), (80, 2, 24, 33, 1), (70, 1, 16, 64, 1), (150, 3, 264, 16, 1), (531, 1, 48, 16, 2), (700, 1, 20, 64, 1)]
