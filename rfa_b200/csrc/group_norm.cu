@@ -223,7 +223,8 @@ __global__ void __launch_bounds__(norm_threads(TPG)) norm_bwd_kernel(const __gri
       for (int c = 0; c < NV; ++c) x[i * NV + c] = next_x[i].get(c);
     }
     ask();
-    const float rstd = centre<NV, V, TPG>(x, part.first, a.size, a.over_size, p.eps, red);
+    float rstd = centre<NV, V, TPG>(x, part.first, a.size, a.over_size, p.eps, red);
+    if (!size) rstd = 0.f;                             // no such row: without a variance, and eps may be 0
     float sums[2] = {};
 #pragma unroll
     for (int i = 0; i < V; ++i) {

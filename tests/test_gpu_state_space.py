@@ -320,6 +320,24 @@ def test_norm(dev, lead, C, groups, dtype, gated, weights, layout, silu):
         near(got, want[n], size[n], 2.0 ** -18 + (rows * 2.0 ** -24 if n in ("gweight", "gbias") else 0), n)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("gated,silu", [(True, True), (False, True), (False, False)])
+@pytest.mark.parametrize("rows,C,groups", [(1, 8, 1), (5, 24, 3), (131, 64, 1), (77, 1024, 16), (3, 300, 1)])
+def test_norm_without_an_eps(dev, rows, C, groups, gated, silu, dtype):
+    """A CTA's rows are more than there are: what it walks beyond them has no variance, and leaves the weights' gradients alone."""
+    gen = torch.Generator().manual_seed(rows)
+    draw = lambda *s: torch.randn(*s, generator=gen).to(dtype)
+    x, g, w, bias, gate = draw(rows, C), draw(rows, C), draw(C), draw(C), draw(rows, C) if gated else None
+    args = [None if t is None else t.double() for t in (w, bias, gate)]
+    want, size = (O.norm(x.double(), groups, *args, silu, 0.0, g.double(), absolute=a) for a in (False, True))
+    xd, wd, bd, zd = leaves(*(None if t is None else t.to(dev) for t in (x, w, bias, gate)))
+    y = ss.group_norm(x=xd, num_groups=groups, weight=wd, bias=bd, gate=zd, activation="silu" if silu else None, eps=0.0)
+    near(y, want["y"], size["y"], 2.0 ** -18, "y")
+    pairs = [(n, t) for n, t in zip(("gx", "gweight", "gbias", "ggate"), (xd, wd, bd, zd)) if t is not None]
+    for (n, t), got in zip(pairs, torch.autograd.grad(y, [t for _, t in pairs], g.to(dev))):
+        near(got, want[n], size[n], 2.0 ** -18 + (rows * 2.0 ** -24 if n in ("gweight", "gbias") else 0), n)
+
+
 # --------------------------------------------------------------------------- what goes for all of them
 def calls(dev, dtype=F16, T=20, B=3, D=64, N=16):
     """Each operator's call on fresh inputs: (function of the tensors, tensors)."""
