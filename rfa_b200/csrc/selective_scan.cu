@@ -370,6 +370,8 @@ extern "C" int rfa_selective_scan_fwd(const rfa_scan_t* scan, void* y, float* s_
   using namespace rfa;
   if (int r = scan_check(scan, "selective_scan_fwd")) return r;
   RFA_REQUIRE(y, RFA_EINVAL, "selective_scan_fwd: null pointer");
+  // a segment's CTA may read s_in after the last segment's has written s_out
+  RFA_REQUIRE(!s_out || s_out != scan->s_in, RFA_EINVAL, "selective_scan_fwd: s_out is s_in");
   RFA_REQUIRE(aligned16(s_out) && aligned16(checkpoints) && aligned16(workspace), RFA_EALIGN, "selective_scan_fwd: s_out, checkpoints or workspace is not 16-byte aligned");
   const size_t need = rfa_selective_scan_workspace_bytes(scan->T, scan->B, scan->D, scan->N, scan->G, 0);
   RFA_REQUIRE(!need || (workspace && workspace_bytes >= need), RFA_EWORKSPACE, "selective_scan_fwd: workspace %zu bytes, %zu needed", workspace_bytes, need);

@@ -201,3 +201,11 @@ def test_wide_accesses_are_taken_of_addresses_that_hold_them(tmp_path):
         assert bool(taken) == (at % access == 0), (size, nv, at)
     # the convolution's weights: 4 channels of `width` taps; 8 modulo 16 holds them in 16 bits only where the width is odd
     assert {w: dict(((s, n, a), t) for s, n, a, t in rows)[2, 4 * w, 8] for w in range(1, 9)} == {1: 1, 2: 0, 3: 1, 4: 0, 5: 1, 6: 0, 7: 1, 8: 0}
+
+
+def test_c_abi_refuses_a_scan_whose_last_state_is_its_first():
+    lib = _lib.load()
+    for T in (1, 4, 1 << 16):                                     # in one segment and in several
+        s = Scan(x=16, dt=16, a=16, b=16, c=16, T=T, B=2, D=8, N=16, G=1, b_t=16, s_in=32)
+        assert lib.rfa_selective_scan_fwd(C.addressof(s), 16, 32, None, 16, 1 << 40, None) == EINVAL
+        assert b"s_out is s_in" in lib.rfa_last_error()
