@@ -428,8 +428,9 @@ int rfa_stream_probe(const void* in, void* out, int64_t T, int BH, int nb, int w
  * are zero.  No alignment is asked for beyond the elements' own, except that
  * states, checkpoints and workspaces are 16-byte aligned.  T < 2^31 - 64,
  * B <= 65535, D and C <= 2^24 (convolution: T D < 2^44); a size of zero is
- * refused (there is nothing to launch).  What a batch row holds reaches no other row's results; the
- * same call gives the same bits.
+ * refused (there is nothing to launch).  Outputs overlap neither inputs nor each other,
+ * but for states where that is said.  What a batch row holds reaches no other row's
+ * results; the same call gives the same bits.
  * ---------------------------------------------------------------------- */
 
 /* Causal depthwise convolution over the last W tokens (1 <= W <= 8):

@@ -452,6 +452,7 @@ extern "C" int rfa_causal_conv_fwd(const rfa_causal_conv_t* conv, void* y, void*
   if (int r = conv_check(conv, "causal_conv_fwd")) return r;
   RFA_REQUIRE(y, RFA_EINVAL, "causal_conv_fwd: null pointer");
   RFA_REQUIRE(!state_out || state_out != conv->state_in || conv->T == 1, RFA_EINVAL, "causal_conv_fwd: the state in place of %lld tokens", (long long)conv->T);
+  RFA_REQUIRE(y != conv->x, RFA_EINVAL, "causal_conv_fwd: y is x");      // other runs' warps read it
   ConvArgs a{};
   a.p = *conv;
   a.y = y; a.state_out = conv->W > 1 ? state_out : nullptr;
@@ -479,6 +480,9 @@ extern "C" int rfa_causal_conv_bwd(const rfa_causal_conv_t* conv, const void* g,
   const size_t need = weights ? rfa_causal_conv_workspace_bytes(conv->T, conv->B, conv->D, conv->W) : 0;
   RFA_REQUIRE(!need || (workspace && workspace_bytes >= need), RFA_EWORKSPACE, "causal_conv_bwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
   RFA_REQUIRE(aligned16(workspace), RFA_EALIGN, "causal_conv_bwd: the workspace is not 16-byte aligned");
+  // other runs' warps read what these would overwrite
+  RFA_REQUIRE(gx != g && gx != conv->x, RFA_EINVAL, "causal_conv_bwd: gx is g or x");
+  RFA_REQUIRE(!g_state_in || (g_state_in != g_state && g_state_in != conv->state_in), RFA_EINVAL, "causal_conv_bwd: g_state_in is g_state or state_in");
   ConvArgs a{};
   a.p = *conv;
   a.g = g; a.g_t = g_t; a.g_b = g_b;

@@ -497,6 +497,8 @@ extern "C" int rfa_selective_scan_bwd(const rfa_scan_t* scan, const void* g, con
   RFA_REQUIRE(aligned16(checkpoints) && aligned16(workspace), RFA_EALIGN, "selective_scan_bwd: checkpoints or workspace is not 16-byte aligned");
   const size_t need = rfa_selective_scan_workspace_bytes(scan->T, scan->B, scan->D, scan->N, scan->G, 1);
   RFA_REQUIRE(workspace && workspace_bytes >= need, RFA_EWORKSPACE, "selective_scan_bwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
+  // every segment's CTAs read g_s, the first one's write gs_in
+  RFA_REQUIRE(!gs_in || gs_in != g_s, RFA_EINVAL, "selective_scan_bwd: gs_in is g_s");
   BwdArgs a{};
   a.sh = scan_shape(scan->T, scan->B, scan->D, scan->N, scan->G, true);
   const BwdSpace space(a.sh);

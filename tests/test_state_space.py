@@ -209,3 +209,17 @@ def test_c_abi_refuses_a_scan_whose_last_state_is_its_first():
         s = Scan(x=16, dt=16, a=16, b=16, c=16, T=T, B=2, D=8, N=16, G=1, b_t=16, s_in=32)
         assert lib.rfa_selective_scan_fwd(C.addressof(s), 16, 32, None, 16, 1 << 40, None) == EINVAL
         assert b"s_out is s_in" in lib.rfa_last_error()
+
+
+def test_c_abi_refuses_outputs_in_place_of_what_other_ctas_read():
+    lib = _lib.load()
+    conv = Conv(x=16, x_t=16, x_b=8, weight=32, T=400, B=2, D=8, W=4, state_in=48)
+    assert lib.rfa_causal_conv_fwd(C.addressof(conv), 16, None, None) == EINVAL and b"y is x" in lib.rfa_last_error()
+    back = lambda g, g_state, gx, gs: lib.rfa_causal_conv_bwd(C.addressof(conv), g, 16, 8, g_state, gx, None, None, gs, None, 0, None)
+    for gx in (16, 64):
+        assert back(64, None, gx, None) == EINVAL and b"gx is g or x" in lib.rfa_last_error()
+    for gs in (48, 80):
+        assert back(64, 80, 96, gs) == EINVAL and b"g_state_in is g_state or state_in" in lib.rfa_last_error()
+    scan = Scan(x=16, dt=16, a=16, b=16, c=16, T=4, B=2, D=8, N=16, G=1, b_t=16)
+    assert lib.rfa_selective_scan_bwd(C.addressof(scan), 16, 32, *[16] * 8, 32, 16, 1 << 40, None) == EINVAL
+    assert b"gs_in is g_s" in lib.rfa_last_error()
