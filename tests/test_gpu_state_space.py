@@ -239,6 +239,14 @@ def test_scan(dev, shape, dtype, pad, layout):
     scan_check(dev, shape, dtype, pad, layout)
 
 
+@pytest.mark.parametrize("shape", [(531, 1, 48, 8, 1), (400, 2, 130, 4, 2), (197, 1, 16, 1, 1), (641, 1, 24, 6, 3), (531, 1, 48, 32, 1), (400, 2, 30, 24, 2),
+                                   (325, 1, 20, 17, 1)])
+@pytest.mark.parametrize("dtype,pad,layout", [(F16, None, None), (BF16, "right", "slice"), (F32, "mixed", "odd"), (F32, "left", "batch first")])
+def test_scan_in_segments(dev, shape, dtype, pad, layout):
+    """Few rows: several segments with a ragged last tile, for up to 8 states (backward tiles of 8 tokens) and for 17 to 32."""
+    scan_check(dev, shape, dtype, pad, layout)
+
+
 @pytest.mark.parametrize("softplus,optional,state", [(False, True, True), (True, False, True), (True, True, False), (False, False, False)])
 @pytest.mark.parametrize("shape", [(1, 2, 24, 16, 1), (40, 2, 24, 16, 1)])
 def test_scan_without_its_optional_parts(dev, shape, softplus, optional, state):
