@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) scan_fwd_kernel(const __grid_c
       th.load_kept(A.seg_state + at * sh.kn, v);
       const f32x2 over = th.get1(A.seg_sum + at);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] = fma2(exp2_unit(mul2(over, a2[j])), s[j], v[j]);
+      for (int j = 0; j < 4; ++j) s[j] = over_segment(mul2(over, a2[j]), s[j], v[j]);
     }
   for (int tile = tile0; tile < tile1; ++tile) {
     const int buf = (tile - tile0) & 1;

@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_c
     th.load_kept(A.seg_grad + at * sh.kn, v);
     const f32x2 over = th.get1(A.seg_sum + at);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) G[j] = fma2(exp2_unit(mul2(over, a2[j])), G[j], v[j]);
+    for (int j = 0; j < 4; ++j) G[j] = over_segment(mul2(over, a2[j]), G[j], v[j]);
   }
 
   f32x2 s[4];                                          // the state in front of the tile

@@ -254,6 +254,35 @@ def test_scan_without_its_optional_parts(dev, shape, softplus, optional, state):
     scan_check(dev, shape, BF16, "mixed", "slice", softplus, optional, state)
 
 
+@pytest.mark.parametrize("N", [4, 16, 24])
+def test_scan_of_states_that_grow(dev, N):
+    """exp(delta a) is e at every token, 1000 of them: a state that is zero until the last 20, and a gradient until the first 20, stays
+    finite, although growth over a whole segment does not; so does one that begins at 1e-36."""
+    T, B, D = 1000, 1, 10
+    gen = torch.Generator().manual_seed(N)
+    draw = lambda *s: torch.randn(*s, generator=gen)
+    ins = dict(x=draw(T, B, D), dt=torch.ones(T, B, D), a=torch.ones(D, N), b=draw(T, B, 1, N), c=draw(T, B, 1, N), d=draw(D), dt_bias=torch.zeros(D),
+               s=torch.zeros(B, D, N))
+    ins["x"][:980] = 0
+    g, gs = draw(T, B, D), torch.zeros(B, D, N)
+    g[20:] = 0
+    want, size = (O.scan(*[t.double() for t in ins.values()], None, False, g.double(), gs.double(), absolute=a) for a in (False, True))
+    on = dict(zip(ins, leaves(*[t.to(dev) for t in ins.values()])))
+    y, s = ss.incremental_selective_scan(**on, dt_softplus=False)
+    names = ("gx", "gdt", "ga", "gb", "gc", "gd", "gbias", "gs")
+    got = dict(zip(names, torch.autograd.grad([y, s], list(on.values()), [g.to(dev), gs.to(dev)])), y=y, s=s)
+    for n, t in got.items():
+        # growth by up to 20 tokens in front of what is compared: their roundings, relative, as in a chain that decays
+        near(t, want[n], size[n], (20 * T + 64 + B + D + 2 * N) * 2.0 ** -24, n)
+    # 1e-36 e^160: two segments, the growth over the first of which (e^89.6) overflows by itself
+    cut = {n: t[:200] if n in ("x", "dt", "b", "c") else t for n, t in ins.items()}
+    cut.update(x=torch.zeros(200, B, D), dt=torch.full((200, B, D), 0.8), s=torch.full((B, D, N), 1e-36), d=torch.zeros(D))
+    want, size = (O.scan(*[t.double() for t in cut.values()], None, False, absolute=a) for a in (False, True))
+    y, s = ss.incremental_selective_scan(**{n: t.to(dev) for n, t in cut.items()}, dt_softplus=False)
+    for n, t in dict(y=y, s=s).items():
+        near(t, want[n], size[n], (20 * 200 + 16 + 2 * N) * 2.0 ** -24, n)
+
+
 @pytest.mark.parametrize("cut", [1, 16, 100, 299])
 def test_scan_in_two_calls(dev, cut):
     """A prompt in two calls is the prompt in one, whichever way either is cut into segments."""
