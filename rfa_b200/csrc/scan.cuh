@@ -74,11 +74,12 @@ __device__ __forceinline__ f32x2 exp2_unit(f32x2 u) {
   return pack2(ex2(v.x), ex2(v.y));
 }
 // v + 2^u s: a state over a whole segment, whose decays may be growth that overflows by itself where the state does not (one that is still zero
-// stays so).  The power goes to the state in two halves; beyond 2^252 every state but a subnormal one is inf.
+// stays so).  What is beyond 2^126 of the power goes to the state by itself; beyond 2^252 every state but a subnormal one is inf.
 __device__ __forceinline__ f32x2 over_segment(f32x2 u, f32x2 s, f32x2 v) {
   const float2 f = split2(u);
-  const f32x2 h = exp2_unit(mul2(pack2(f.x > 252.f ? 252.f : f.x, f.y > 252.f ? 252.f : f.y), both(0.5f)));
-  return fma2(h, mul2(h, s), v);
+  const auto low = [](float u) { return u > 126.f ? 126.f : u; };                        // NaN stays
+  const auto high = [](float u) { return u > 126.f ? fminf(u - 126.f, 126.f) : 0.f; };
+  return fma2(exp2_unit(pack2(low(f.x), low(f.y))), mul2(exp2_unit(pack2(high(f.x), high(f.y))), s), v);
 }
 // The first state's on the FMA units, -126 <= u < 128 (below: 2^-126): u = k + r with k whole (the addition of 1.5 * 2^23 rounds) and
 // |r| <= 1/2, 2^r by a polynomial of degree 5 with 1 + r log 2 in front (least maximum of the relative error, by Lawson's iteration:
