@@ -302,8 +302,8 @@ __device__ __forceinline__ void store4(float* p, int n, bool wide, const float* 
 // 16-byte words) of one channel, LN / 2 lanes a channel, in kRows batch rows, all of whose loads are on the way at once: the step size, a, the
 // group and the addresses, which are most of the instructions, are found once for them.
 template <typename T, int LN, int kRows>
-__global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ rfa_scan_t p, T* y, float* state, bool wide, bool wide_bc) {
-  constexpr int kLanes = LN / 2;
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) scan_step_kernel(const __grid_constant__ rfa_scan_t p, T* y, float* state, bool wide, bool wide_bc) {
+  constexpr int kLanes = LN / 2, kPoly = LN < 8 ? LN / 2 : 4;      // pairs of a thread's states
   const int at_ch = (blockIdx.x * 256 + threadIdx.x) / kLanes, n0 = 8 * (threadIdx.x % kLanes), b0 = blockIdx.y * kRows;
   const bool there = at_ch < p.D;
   const int ch = there ? at_ch : 0, rows = min(kRows, p.B - b0);
@@ -316,34 +316,64 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ 
   float s[kRows][8], a[8];
   Raw<T, 4> rb[kRows][2], rc[kRows][2];
   T x[kRows], dt[kRows];
+  const float bias = p.dt_bias ? p.dt_bias[ch] : 0.f, skip = p.d ? p.d[ch] : 0.f;
+  // What the decays want is asked for in front of the states or behind: 256 x 2048 x 16 in front 14.9 us in bf16
+  // and 15.4 in fp32, behind 13.9 and 16.6
+  constexpr bool kSmallFirst = sizeof(T) == 4;
+  if constexpr (kSmallFirst) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) load4(p.a + (size_t)ch * p.N + n0 + 4 * h, n[h], wide, a + 4 * h);
+  }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int b = b0 + (r < rows ? r : 0);             // a row that is not there: another's loads, nothing stored
+    if constexpr (kSmallFirst) {
+      dt[r] = static_cast<const T*>(p.dt)[(int64_t)b * p.dt_b + ch];
+      x[r] = static_cast<const T*>(p.x)[(int64_t)b * p.x_b + ch];
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       load4(at + (b - b0) * row + 4 * h, n[h], wide, s[r] + 4 * h);
       rb[r][h].load(bp + (int64_t)b * p.b_b + 4 * h, n[h], wide_bc);
       rc[r][h].load(cp + (int64_t)b * p.c_b + 4 * h, n[h], wide_bc);
     }
-    x[r] = static_cast<const T*>(p.x)[(int64_t)b * p.x_b + ch];
-    dt[r] = static_cast<const T*>(p.dt)[(int64_t)b * p.dt_b + ch];
+    if constexpr (!kSmallFirst) {
+      dt[r] = static_cast<const T*>(p.dt)[(int64_t)b * p.dt_b + ch];
+      x[r] = static_cast<const T*>(p.x)[(int64_t)b * p.x_b + ch];
+    }
   }
+  if constexpr (!kSmallFirst) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) load4(p.a + (size_t)ch * p.N + n0 + 4 * h, n[h], wide, a + 4 * h);
-  const float bias = p.dt_bias ? p.dt_bias[ch] : 0.f, skip = p.d ? p.d[ch] : 0.f;
+    for (int h = 0; h < 2; ++h) load4(p.a + (size_t)ch * p.N + n0 + 4 * h, n[h], wide, a + 4 * h);
+  }
+  f32x2 a2[4];                                         // in units of log 2; adjacent states in pairs
 #pragma unroll
-  for (int j = 0; j < 8; ++j) a[j] *= kLog2e;
+  for (int i = 0; i < 4; ++i) a2[i] = mul2(pack2(a[2 * i], a[2 * i + 1]), both(kLog2e));
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const float xv = to_f(x[r]);
-    float delta = to_f(dt[r]) + bias, sig, out = 0.f;
+    float delta = to_f(dt[r]) + bias, sig;
     if (p.softplus) delta = softplus(delta, sig);
-    const float dx = delta * xv;
+    const f32x2 dx = both(delta * xv), step = both(delta);
+    f32x2 e[4], out2 = both(0.f);
+    Poly<kPoly> poly;                                  // the slow states' decays: an error of one sign would add up from call to call
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      s[r][j] = fmaf(ex2(delta * a[j]), s[r][j], dx * rb[r][j / 4].get(j % 4));
-      out = fmaf(s[r][j], rc[r][j / 4].get(j % 4), out);
+    for (int i = 0; i < 4; ++i) {
+      if (i < kPoly) poly.begin(i, mul2(step, a2[i]));
+      else e[i] = exp2_unit(mul2(step, a2[i]));
     }
+    poly.run();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 bt = rb[r][i / 2].get2(i % 2), ct = rc[r][i / 2].get2(i % 2);
+      const f32x2 now = fma2(i < kPoly ? poly.end(i) : e[i], pack2(s[r][2 * i], s[r][2 * i + 1]), mul2(dx, pack2(bt.x, bt.y)));
+      out2 = fma2(now, pack2(ct.x, ct.y), out2);
+      const float2 f = split2(now);
+      s[r][2 * i] = f.x;
+      s[r][2 * i + 1] = f.y;
+    }
+    const float2 halves = split2(out2);
+    float out = halves.x + halves.y;
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) out += __shfl_xor_sync(0xffffffffu, out, o);
     if (r >= rows || !there) continue;

@@ -318,6 +318,39 @@ def test_scan_keeps_fp32_over_long_sequences(dev):
         assert (t.detach().cpu().double() - want[n]).norm() <= 2.0 ** -19 * want[n].norm(), n
 
 
+@pytest.mark.parametrize("steps", ["constant", "varied"])
+@pytest.mark.parametrize("N", [8, 16, 32])
+def test_scan_keeps_fp32_token_by_token(dev, N, steps):
+    """4096 calls of one token each, the state carried through them, for states that remember 1000 tokens.
+
+    Varied steps: each token's roundings are others, so that they add up as in one call over the tokens (2^-19 of the norm, above); so
+    does not what has one sign.  Of the slowest state, the error along the state itself: the polynomial near 1 is off by 2.3e-7 |r|,
+    |r| <= 0.002, 1000 times, the step size by 5e-7 both in the decays and in what is added: 1.5e-6 < 2^-19 (an error of -5e-9 a decay, as
+    the special function unit's there, would be 5e-6).
+    Constant steps: a decay just below 1 is rounded the same way every time, by up to 2^-25, so that what came k tokens ago is off by
+    k 2^-25 of itself.  That is 1000 2^-25 of what the tokens brought, but k = T = 4096 for the initial state, and exp(-4.1) of its 1 is as
+    much as the tokens' sqrt(0.001 / 2): up to T 2^-25 = 2^-13 of the norm."""
+    T, B, D = 4096, 2, 40
+    gen = torch.Generator().manual_seed(N)
+    ins, _, _ = scan_inputs((T, B, D, N, 1), F32, gen)
+    if steps == "constant":
+        ins["dt"].zero_()
+    ins["dt_bias"] = torch.full((D,), -6.9073)                    # softplus of it is 0.001
+    want = O.scan(*[t.double() for t in ins.values()], None, True)
+    on = {n: t.to(dev) for n, t in ins.items()}
+    held, ys = on["s"], []
+    for t in range(T):
+        y, held = ss.incremental_selective_scan(**{**on, **{n: on[n][t:t + 1] for n in ("x", "dt", "b", "c")}, "s": held})
+        ys.append(y)
+    bound = 2.0 ** (-13 if steps == "constant" else -19)
+    for n, got in dict(y=torch.cat(ys), s=held).items():
+        off = float((got.cpu().double() - want[n]).norm() / want[n].norm())
+        assert off <= bound, (n, off)
+    slow, true = held[..., 0].cpu().double(), want["s"][..., 0]
+    along = float(((slow - true) * true).sum() / true.square().sum())
+    assert abs(along) <= bound, along
+
+
 @pytest.mark.parametrize("value", [float("inf"), float("nan")])
 def test_scan_keeps_non_finite_values_where_they_belong(dev, value):
     """One token of one channel's x: its channel from that token on, its group's b and c gradients; nothing else."""
