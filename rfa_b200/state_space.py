@@ -163,9 +163,8 @@ def group_norm(*, x: Tensor, num_groups: int, weight: Optional[Tensor] = None, b
     to the variance), times weight plus bias: n.  Returns ``n * act(gate)``, without a gate ``act(n)``.
 
     x and gate ``[..., channels]``, weight and bias ``[channels]``, all of one dtype, runs of at most 16384 channels;
-    activation "silu" or None.  The
-    statistics are a token's own (``torch.nn.GroupNorm`` on ``[tokens, channels]``), so that a causal layer stays causal
-    and a token's result does not depend on the ones it is called with."""
+    activation "silu" or None.  The statistics are a token's own (``torch.nn.GroupNorm`` on ``[tokens, channels]``), so that
+    a causal layer stays causal and a token's result does not depend on the ones it is called with."""
     silu = _silu(activation)
     if plain_tensors(x, weight, bias, gate):
         return native().group_norm_node(x, num_groups, weight, bias, gate, silu, eps)
@@ -179,7 +178,8 @@ class SelectiveStateSpace(nn.Module):
     the convolution's output, group norm gated by silu(gate), output projection.
 
     a is ``-exp(a_log)``, initialised to -1 ... -state_dim; dt_bias so that the step sizes start log-uniform in
-    [0.001, 0.1].  ``norm_groups`` defaults to groups of 64 channels where they divide, else one group."""
+    [0.001, 0.1].  ``norm_groups`` defaults to groups of 64 channels where they divide, else one group.  What the operators
+    take is asked for here: ``conv_width`` 1 to 8, ``state_dim`` 1 to 64, norm groups of at most 16384 channels."""
 
     def __init__(self, *, embed_dim: int, inner_dim: Optional[int] = None, state_dim: int = 16, conv_width: int = 4,
                  dt_rank: Optional[int] = None, num_groups: int = 1, norm_groups: Optional[int] = None):
@@ -187,8 +187,12 @@ class SelectiveStateSpace(nn.Module):
         inner_dim = 2 * embed_dim if inner_dim is None else inner_dim
         dt_rank = max(1, math.ceil(embed_dim / 16)) if dt_rank is None else dt_rank
         norm_groups = (inner_dim // 64 if inner_dim % 64 == 0 else 1) if norm_groups is None else norm_groups
-        assert inner_dim % num_groups == 0, "inner_dim must be divisible by num_groups"
-        assert inner_dim % norm_groups == 0, "inner_dim must be divisible by norm_groups"
+        assert 1 <= conv_width <= 8, "conv_width must be 1 to 8"
+        assert 1 <= state_dim <= 64, "state_dim must be 1 to 64"
+        assert 1 <= inner_dim <= 1 << 24, "inner_dim must be 1 to 2^24"
+        assert num_groups >= 1 and inner_dim % num_groups == 0, "inner_dim must be divisible by num_groups"
+        assert norm_groups >= 1 and inner_dim % norm_groups == 0, "inner_dim must be divisible by norm_groups"
+        assert inner_dim // norm_groups <= 16384, "norm_groups must leave at most 16384 channels in a group"
         self.embed_dim, self.inner_dim, self.state_dim, self.conv_width = embed_dim, inner_dim, state_dim, conv_width
         self.dt_rank, self.num_groups, self.norm_groups = dt_rank, num_groups, norm_groups
         self.in_proj = nn.Linear(embed_dim, 2 * inner_dim, bias=False)

@@ -223,3 +223,13 @@ def test_c_abi_refuses_outputs_in_place_of_what_other_ctas_read():
     scan = Scan(x=16, dt=16, a=16, b=16, c=16, T=4, B=2, D=8, N=16, G=1, b_t=16)
     assert lib.rfa_selective_scan_bwd(C.addressof(scan), 16, 32, *[16] * 8, 32, 16, 1 << 40, None) == EINVAL
     assert b"gs_in is g_s" in lib.rfa_last_error()
+
+
+@pytest.mark.parametrize("wrong,name", [(dict(conv_width=9), "conv_width"), (dict(conv_width=0), "conv_width"), (dict(state_dim=65), "state_dim"),
+                                        (dict(state_dim=0), "state_dim"), (dict(num_groups=0), "num_groups"), (dict(norm_groups=0), "norm_groups"),
+                                        (dict(norm_groups=-1), "norm_groups"), (dict(inner_dim=0), "inner_dim"),
+                                        (dict(inner_dim=16400, norm_groups=1, state_dim=1, dt_rank=1), "16384")])
+def test_a_layer_that_its_operators_refuse_is_not_built(wrong, name):
+    with pytest.raises(AssertionError, match=name):
+        SelectiveStateSpace(**{**dict(embed_dim=2), **wrong})
+    SelectiveStateSpace(embed_dim=2, conv_width=8, state_dim=64, norm_groups=4)
