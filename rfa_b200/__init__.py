@@ -16,7 +16,7 @@ from .cross_attention import CrossAttention, CrossAttentionProject
 from .state_space import SelectiveStateSpace
 
 __all__ = ["CausalAttention", "CrossAttention", "CrossAttentionState", "CrossAttentionProject",
-           "SelectiveStateSpace",            "install_aliases"]
+           "SelectiveStateSpace", "install_aliases"]
 
 
 def install_aliases() -> None:
