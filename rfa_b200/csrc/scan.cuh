@@ -73,14 +73,6 @@ __device__ __forceinline__ f32x2 exp2_unit(f32x2 u) {
   const float2 v = split2(u);
   return pack2(ex2(v.x), ex2(v.y));
 }
-// v + 2^u s: a state over a whole segment, whose decays may be growth that overflows by itself where the state does not (one that is still zero
-// stays so).  What is beyond 2^126 of the power goes to the state by itself; beyond 2^252 every state but a subnormal one is inf.
-__device__ __forceinline__ f32x2 over_segment(f32x2 u, f32x2 s, f32x2 v) {
-  const float2 f = split2(u);
-  const auto low = [](float u) { return u > 126.f ? 126.f : u; };                        // NaN stays
-  const auto high = [](float u) { return u > 126.f ? fminf(u - 126.f, 126.f) : 0.f; };
-  return fma2(exp2_unit(pack2(low(f.x), low(f.y))), mul2(exp2_unit(pack2(high(f.x), high(f.y))), s), v);
-}
 // The first state's on the FMA units, -126 <= u < 128 (below: 2^-126): u = k + r with k whole (the addition of 1.5 * 2^23 rounds) and
 // |r| <= 1/2, 2^r by a polynomial of degree 5 with 1 + r log 2 in front (least maximum of the relative error, by Lawson's iteration:
 // 1.1e-7, and 2.3e-7 |r| near 0, so that a decay near 1 is as near as its argument is), k added to the exponent.
@@ -280,6 +272,49 @@ template <int K, int LN, int W = LN> __device__ __forceinline__ void lanes_sum(f
     } else {
       v[0] += __shfl_xor_sync(0xffffffffu, v[0], W / 2);
       lanes_sum<1, LN, W / 2>(v, ln);
+    }
+  }
+}
+
+// s -> 2^(sum a) s + v over `count` segments, the first at `at`: a thread's states in front of its own segment (or gradients behind it), from the
+// others' states and sums of deltas.  The decays may be growth that overflows by itself where the state does not (one that is still zero stays
+// so).  A call that meets such a power, beyond 2^126, goes over its segments once more with what is beyond it apart from the rest; beyond
+// 2^252 every state but a subnormal one is inf.
+template <class Thread>
+__device__ __forceinline__ void join_segments(const Thread& th, const ScanShape& sh, const float* states, const float* sums, int at, int count, int step,
+                                              const f32x2* a2, f32x2* s) {
+  const f32x2 start[4] = {s[0], s[1], s[2], s[3]};
+  float most = 0.f;
+  const auto segment = [&](int i, f32x2* u, f32x2* v) {
+    const size_t row = ((size_t)(at + i * step) * sh.B + th.b) * sh.D;
+    th.load_kept(states + row * sh.kn, v);
+    const f32x2 over = th.get1(sums + row);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = mul2(over, a2[j]);
+  };
+  for (int i = 0; i < count; ++i) {
+    f32x2 u[4], v[4];
+    segment(i, u, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = split2(u[j]);
+      most = fmaxf(most, fmaxf(f.x, f.y));
+      s[j] = fma2(exp2_unit(u[j]), s[j], v[j]);
+    }
+  }
+  if (most <= 126.f) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s[j] = start[j];
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    f32x2 u[4], v[4];
+    segment(i, u, v);
+    const auto low = [](float u) { return u > 126.f ? 126.f : u; };                        // NaN stays
+    const auto high = [](float u) { return u > 126.f ? fminf(u - 126.f, 126.f) : 0.f; };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = split2(u[j]);
+      s[j] = fma2(exp2_unit(pack2(low(f.x), low(f.y))), mul2(exp2_unit(pack2(high(f.x), high(f.y))), s[j]), v[j]);
     }
   }
 }

@@ -200,15 +200,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) scan_fwd_kernel(const __grid_c
     a2[j] = mul2(th.get(p.a, j, sh.N), both(kLog2e));
     s[j] = !kSummary && p.s_in ? th.get(p.s_in + (size_t)th.b * sh.D * sh.N, j, sh.N) : both(0.f);
   }
-  if (!kSummary)
-    for (int i = 0; i < seg; ++i) {                    // the segments before this one
-      const size_t at = ((size_t)i * sh.B + th.b) * sh.D;
-      f32x2 v[4];
-      th.load_kept(A.seg_state + at * sh.kn, v);
-      const f32x2 over = th.get1(A.seg_sum + at);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] = over_segment(mul2(over, a2[j]), s[j], v[j]);
-    }
+  if (!kSummary) join_segments(th, sh, A.seg_state, A.seg_sum, 0, seg, 1, a2, s);      // the segments before this one
   for (int tile = tile0; tile < tile1; ++tile) {
     const int buf = (tile - tile0) & 1;
     meet_wait<kFwdThreads>(kFull + buf);

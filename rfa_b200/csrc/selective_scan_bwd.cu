@@ -343,14 +343,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) scan_bwd_kernel(const __grid_c
     da[j] = both(0.f);
   }
   sm.da[0][th.tid] = sm.da[1][th.tid] = make_ulonglong2(0, 0);
-  for (int i = sh.segs - 2; i >= seg; --i) {           // the segments behind this one
-    const size_t at = ((size_t)i * sh.B + th.b) * sh.D;
-    f32x2 v[4];
-    th.load_kept(A.seg_grad + at * sh.kn, v);
-    const f32x2 over = th.get1(A.seg_sum + at);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) G[j] = over_segment(mul2(over, a2[j]), G[j], v[j]);
-  }
+  join_segments(th, sh, A.seg_grad, A.seg_sum, sh.segs - 2, sh.segs - 1 - seg, -1, a2, G);      // the segments behind this one
 
   f32x2 s[4];                                          // the state in front of the tile
   const float* ckpt = A.ckpt + (size_t)th.b * sh.tiles * sh.D * sh.kn;
