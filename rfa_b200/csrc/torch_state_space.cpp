@@ -28,6 +28,12 @@ void need_shape(const char* what, const char* name, const Tensor& t, at::IntArra
 void need_f32(const char* what, const char* name, const Tensor& t) {
   if (t.scalar_type() != at::kFloat) raise(PyExc_TypeError, std::string(what) + ": " + name + " must be fp32, got " + dtype_name(t));
 }
+// A gradient that a caller hands in: of the shape that it is the gradient of, and on its device.
+void need_grad(const char* what, const char* name, const OptTensor& g, at::IntArrayRef shape, const Tensor& x) {
+  if (!g) return;
+  need_shape(what, name, *g, shape);
+  require_device(x, {&*g});
+}
 // Activations are taken with any strides but along the channels.
 Tensor unit_last(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
@@ -127,6 +133,8 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> causal_conv_bwd(const Tensor
                                                                     const OptTensor& mask, bool silu, Tensor g, OptTensor g_state, bool need_weight,
                                                                     bool need_bias, bool need_state) {
   Conv v("causal_conv", x, weight, bias, state, mask, silu);
+  need_grad("causal_conv", "g", g, x.sizes(), x);
+  need_grad("causal_conv", "g_state", g_state, {x.size(1), weight.size(1) - 1, x.size(2)}, x);
   Tensor gx = fresh(x.sizes(), x, x.scalar_type());
   OptTensor gw, gb, gs;
   need_state = need_state && state;
@@ -275,6 +283,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTens
     const Tensor& x, const Tensor& dt, const Tensor& a, const Tensor& b, const Tensor& c, const OptTensor& d, const OptTensor& dt_bias, const OptTensor& s,
     const OptTensor& mask, bool softplus, Tensor g, OptTensor g_s, const OptTensor& kept, bool need_state) {
   Scan v(x, dt, a, b, c, d, dt_bias, s, mask, softplus);
+  need_grad("selective_scan", "g", g, x.sizes(), x);
+  need_grad("selective_scan", "g_s", g_s, {x.size(1), x.size(2), a.size(1)}, x);
   const auto half = x.scalar_type();
   Tensor gx = fresh(x.sizes(), x, half), gdt = fresh(x.sizes(), x, half), ga = fresh(a.sizes(), x, at::kFloat);
   Tensor gb = fresh(b.sizes(), x, half), gc = fresh(b.sizes(), x, half);
@@ -289,7 +299,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTens
     if (gs) g_s ? gs->copy_(*g_s) : gs->zero_();
     return {gx, gdt, ga, gb, gc, gd, gbias, gs};
   }
-  if (!kept) raise(PyExc_ValueError, "selective_scan: a backward pass wants its forward's checkpoints");
+  const size_t kept_bytes = rfa_selective_scan_checkpoint_bytes(v.c.T, v.c.B, v.c.D, v.c.N);
+  if (!kept || !kept->is_contiguous() || kept->nbytes() < kept_bytes) raise(PyExc_ValueError, "selective_scan: a backward pass wants its forward's checkpoints");
+  require_device(x, {&*kept});
   g = g.to(half).contiguous();
   if (g_s) g_s = packed(g_s->to(at::kFloat));
   const Tensor ws = scratch(rfa_selective_scan_workspace_bytes(v.c.T, v.c.B, v.c.D, v.c.N, v.c.G, 1), x);
@@ -404,6 +416,7 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> group_norm_bwd(const Tensor&
                                                                    const OptTensor& gate, bool silu, double eps, Tensor g, bool need_weight, bool need_bias,
                                                                    bool need_gate) {
   Norm v(x, groups, weight, bias, gate, silu, eps);
+  need_grad("group_norm", "g", g, x.sizes(), x);
   Tensor gx = fresh(x.sizes(), x, x.scalar_type());
   OptTensor gw, gb, gg;
   if (need_weight && weight) gw = fresh(weight->sizes(), x, x.scalar_type());

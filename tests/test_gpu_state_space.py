@@ -773,3 +773,36 @@ def test_tensor_level_calls(dev):
     assert kept is None and bool((s == 1).all()) and not torch.equal(out, s)
     with pytest.raises(ValueError, match="checkpoints"):
         ops.selective_scan_bwd(*ts, s, None, True, y, None, None, False)
+
+
+def test_tensor_level_calls_refuse_gradients_of_other_shapes_and_devices(dev):
+    """What autograd hands over fits by itself; a caller of ``ops`` may not: kernels would read beyond it."""
+    _, (x, w, b) = calls(dev)["conv"]
+    s = torch.ones(3, 3, 64, device=dev).half()
+    conv = lambda g, g_state=None: ops.causal_conv_bwd(x, w, b, s, None, True, g, g_state, True, True, True)
+    _, ts = calls(dev)["scan"]
+    y, _, kept = ops.selective_scan_fwd(*ts, save=True)
+    scan = lambda g, g_s=None, k=kept: ops.selective_scan_bwd(*ts, None, None, True, g, g_s, k, False)
+    norm = lambda g: ops.group_norm_bwd(x, 4, b, b, None, True, 1e-5, g, True, True, False)
+    for call in (conv, scan, norm):
+        call(x)
+        for g in (x[1:], x[:, :1], x[..., :32], x[0], x.flatten()):
+            with pytest.raises(AssertionError, match="g is"):
+                call(g)
+        with pytest.raises(RuntimeError, match="expected all tensors on"):
+            call(x.cpu())
+    with pytest.raises(AssertionError, match="g_state is"):
+        conv(x, s[:, 1:])
+    with pytest.raises(RuntimeError, match="expected all tensors on"):
+        conv(x, s.cpu())
+    state = torch.zeros(3, 64, 16, device=dev)
+    scan(x, state)
+    with pytest.raises(AssertionError, match="g_s is"):
+        scan(x, state[..., 1:])
+    with pytest.raises(RuntimeError, match="expected all tensors on"):
+        scan(x, state.cpu())
+    for wrong in (None, kept[:-4], torch.cat([kept, kept])[::2], kept[:0]):
+        with pytest.raises(ValueError, match="checkpoints"):
+            scan(x, None, wrong)
+    with pytest.raises(RuntimeError, match="expected all tensors on"):
+        scan(x, None, kept.cpu())
