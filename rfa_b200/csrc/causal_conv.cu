@@ -2,13 +2,15 @@
 // Padded tokens are left out of the sequence: a window holds the last W tokens that are there.
 //
 // Bound by memory and the sigmoid's two special functions: x once, y once (backward: x, g, gx); 8 x 2048 tokens x 2048 channels of a
-// wider array, W = 4, bf16, forward: 20.5 us of memory, 24 us of that unit, 38 us measured (3.5 TB/s; latency and issue slots, 55 %
+// wider array, W = 4, bf16, forward: 20.5 us of memory, 24 us of that unit, 39 us measured (3.5 TB/s; latency and issue slots, 56 %
 // busy; fp32 51 us, 5.3 TB/s).  A warp takes 32 vectors of four adjacent channels and a run of 32 tokens, and keeps the window in
 // registers, so that x is read once but for the W - 1 tokens in front of a run; four tokens that are there are worked on together
 // while the next four are on the way (token by token, a padded batch took 57 us instead of 39).  Vectors of eight: 43 us, runs of
 // 16: 43.  The backward walks a run and the W - 1 tokens behind it with the gradients of the last W tokens pending in registers: a
 // token's gradient is written when the last window that holds it has passed.  Weight gradients stay in registers over the run,
 // are summed over the CTA's warps in shared memory and over CTAs in sum_parts, in a fixed order.
+// Backward, 64 x 1024 x 1024 in fp16, padded: 184 us, 62 of memory.  Bound by latency: 130 registers leave three CTAs an SM (18 % of the warps), a
+// CTA's four runs are of one row, and issue slots are 46 % busy.
 #include "state_space.cuh"
 
 namespace rfa {

@@ -4,6 +4,7 @@
 //
 // Bound by memory: x and gate once, y once (backward: x, gate, g; gx, ggate); 8 x 2048 tokens x 2048 channels in groups of 64, bf16, forward:
 // 41 us, 4.9 TB/s of 6.5 (issue slots are 73 % busy; a launch of one row per thread, with weight and bias read for each, took 60 us).
+// Backward, 16 x 1531 x 2048: 113 us, 77 of memory for its five passes (issue slots 72 %, two CTAs an SM by registers).
 // A group stays in the registers of 1 to 512 threads, with 16-byte
 // words where the sizes allow; threads keep their channels, and weight and bias, over many rows, the next of which is on the way; mean and variance are two passes over registers (no difference of squares), joined by
 // shuffles, beyond a warp through shared memory.  The backward forms the statistics again rather than reading them; the
@@ -308,6 +309,18 @@ __global__ void __launch_bounds__(norm_threads(TPG)) norm_bwd_kernel(const __gri
 }
 
 // The groups and rows that a CTA takes side by side, and how many CTAs share the rows.
+//
+// Threads of a group: as many as it has vectors up to 32, then 32 for up to 128 vectors (2 or 4 a thread), 128 for up to 512, 512 beyond.
+// us forward / backward of 16 x 1531 x 2048 elements, the rule and (in brackets) other threads, vectors of 8 elements in bf16:
+//   512 channels, 64 vectors     32 threads 68 / 160 (128: 128 / 247)      2048, 256 vectors    128 threads 69 / 144 (32: 103 / 613, 512: 144 / 338)
+//   1024, 128 vectors            32 threads 81 / 220 (128: 68 / 134)       4096, 512 vectors    128 threads 77 / 195 (512: 78 / 193)
+//   256: 65 / 133    64: 63 / 130    8192: 87 / 239    16384: 100 / 763
+// and of 4 elements in fp32:
+//   512, 128 vectors             32 threads 99 / 200 (128: 105 / 213)      1024, 256 vectors    128 threads 118 / 175 (32: 104 / 405)
+//   2048, 512 vectors            128 threads 99 / 189 (512: 127 / 273)     64: 105 / 214    4096: 128 / 201    16384: 220 / 1232
+// What a thread holds decides: up to 16 elements stay in 255 registers; with 32 the backward spills (in 16 bits 168 bytes for 513 to 1024 channels,
+// where 128 threads would be the better rule, 160 for 2049 to 4096).  512 threads have 128 registers: 250 bytes above 4096 channels, 2 KB above
+// 8192; fp32 0.6 and 2.9 KB.
 struct NormGrid {
   int nv, tpg, v, groups_here, rows_here, x, y;
 };

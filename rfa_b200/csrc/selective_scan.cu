@@ -3,13 +3,14 @@
 //
 // Bound by arithmetic: one exponential per token, channel and state, where a token and channel of 16 states moves 6 bytes in 16 bits
 // (8 x 2048 tokens x 2048 channels: 537 M exponentials are 119 us of the special function units, 201 MB are 31 us of memory).  That size
-// takes 226 to 230 us in bf16: of the 105 cycles of a token on an SM's scheduler the special function unit is busy for 56 (with softplus),
+// takes 230 to 232 us in bf16: of the 105 cycles of a token on an SM's scheduler the special function unit is busy for 56 (with softplus),
 // the FMA units for 63, shared memory for 61 of the SM's, and 68 are issue slots; 256 CTAs on 148 SMs leave a seventh of the card idle.
-// Tiles of 32 tokens: 220 us, for twice the shared memory and code.  Layout in scan.cuh.
+// Tiles of 32 tokens: 226 us, for twice the shared memory and code.  Layout in scan.cuh.
 //
 // Few rows (a prompt of one sequence) leave SMs idle: the tokens are then cut into segments.  A first kernel leaves each segment's own state
 // from zero and the sum of its deltas -- over which a whole segment's decay is exp(a sum delta), one exponential -- and the main kernel's
 // CTAs begin with the states of the segments before theirs joined up, which costs the first kernel's pass over dt, x and b once more.
+// 1 x 16384 tokens x 1024 channels, fp16, 37 segments: 87 us the first kernel (special function unit 65 % busy, FMA units 60 %), 118 the main one.
 #include "scan.cuh"
 
 namespace rfa {
@@ -17,11 +18,13 @@ namespace rfa {
 int scan_lanes(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 // Two CTAs run side by side on an SM, 296 in all; one alone takes 0.63 of the time of two (forward, 0.66 backward).  A segment more costs the
-// forward about half of its pass again, the backward an eighth.  us at T = 2048 (N = 16, bf16), one segment / several:
-//   forward   16 CTAs 137 / 37, 64 CTAs 138 / 101 with about 592 in all; 128 CTAs 147 / 183, 160 CTAs 233 / 233, 256 CTAs 233 / 321
-//   backward  the same below 120; above, whatever fills the last round: 160 CTAs 855 / 603 in six, 320 CTAs (T = 1024) 686 / 588 in three,
-//             256 CTAs 877 / 906 in four, so one
-// Segments of less than 96 tokens lose to their own ends (16 CTAs, T = 2048: 19 segments 37 us, 32 segments 42).
+// forward about half of its pass again, the backward an eighth.  us at T = 2048 (N = 16, bf16; a call with its host time of about 10 us), one segment /
+// what the rule takes (other numbers):
+//   forward   16 CTAs 148 / 44 in 19, 64 CTAs 150 / 110 in ten (four 119); above 120 one: 128 CTAs 158 (two 192), 160 CTAs 239 (two 277, four 244),
+//             256 CTAs 241 (two 328)
+//   backward  16 CTAs 527 / 87 in 19, 64 CTAs 579 / 286 in ten; above 120 whatever fills the last round: 128 CTAs 607 / 551 in two (four 548),
+//             160 CTAs 903 / 655 in five (three 716, six 642), 320 CTAs (T = 1024) 726 / 603 in six (three 624), 256 CTAs 937 in one (four 955)
+// Segments of less than 96 tokens lose to their own ends (16 CTAs, T = 2048: 19 segments 42 us, 32 segments 47, 64 segments 66).
 ScanShape scan_shape(int64_t T, int B, int D, int N, int G, bool backward) {
   ScanShape s{};
   const int channels = 256 / scan_lanes(N);
@@ -292,7 +295,8 @@ __device__ __forceinline__ void store4(float* p, int n, bool wide, const float* 
 // ---- one token ---------------------------------------------------------------------------------------------------------------
 // Bound by the state's way from memory and back, 8 bytes per element, where it is large enough.  A thread has eight adjacent states (two
 // 16-byte words) of one channel, LN / 2 lanes a channel, in kRows batch rows, all of whose loads are on the way at once: the step size, a, the
-// group and the addresses, which are most of the instructions, are found once for them.
+// group and the addresses, which are most of the instructions, are found once for them.  256 x 2048 x 16 in bf16: 13.8 us in a graph, 16.4 by itself,
+// 10.8 of memory.  Registers are limited to what leaves an SM four CTAs (three in fp32): 68 of them took 16.9 us.
 template <typename T, int LN, int kRows>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) scan_step_kernel(const __grid_constant__ rfa_scan_t p, T* y, float* state, bool wide, bool wide_bc) {
   constexpr int kLanes = LN / 2, kPoly = LN < 8 ? LN / 2 : 4;      // pairs of a thread's states
@@ -421,7 +425,8 @@ extern "C" int rfa_selective_scan_step(const rfa_scan_t* scan, void* y, float* s
   const int size = scan->dtype == RFA_F32 ? 4 : 2;
   const bool wide = scan->N % 4 == 0 && aligned16(scan->a);
   const bool wide_bc = wide_ok(scan->b, scan->b_b, scan->b_g, size, 4) && wide_ok(scan->c, scan->c_b, scan->c_g, size, 4);
-  // Two rows a thread from eight CTAs of one row per SM on; below, all SMs are wanted.
+  // Two rows a thread from eight CTAs of one row per SM on; below, all SMs are wanted.  us of B x 2048 x 16 in bf16, one row / two: B = 16 2.45 / 2.55,
+  // 32 3.15 / 3.36, 64 (7 a SM) 4.84 / 4.74, 74 (8) 5.23 / 4.91, 128 7.48 / 7.20, 256 14.9 / 14.4
 #define CALL(T, LN)                                                                                                          \
   do {                                                                                                                       \
     const unsigned x = (unsigned)(((int64_t)scan->D * (LN / 2) + 255) / 256);                                                \
