@@ -462,7 +462,8 @@ int rfa_causal_conv_bwd(const rfa_causal_conv_t* conv, const void* g, int64_t g_
  *   s_t = exp(delta_t a) s_(t-1) + delta_t b_t x_t        (N states, 1 <= N <= 64)
  *   y_t = c_t . s_t + d x_t
  * x, dt [T, B, D]; b, c [T, B, G, N], the N adjacent, *_g from group to group; a [D, N]
- * (finite, delta a <= 88), d [D] or NULL, dt_bias [D] or NULL, states [B, D, N], all fp32. */
+ * (finite; delta a <= 88, or results are not defined), d [D] or NULL, dt_bias [D] or NULL,
+ * states [B, D, N], all fp32. */
 typedef struct {
   const void *x, *dt, *b, *c;
   int64_t x_t, x_b, dt_t, dt_b, b_t, b_b, b_g, c_t, c_b, c_g;

@@ -80,9 +80,11 @@ __device__ __forceinline__ f32x2 exp2_unit(f32x2 u) {
 // R of them side by side: few warps share an SM's scheduler, and a chain alone would wait for itself.
 template <int R> struct Poly {
   f32x2 t[R], r[R], p[R];
-  __device__ __forceinline__ void begin(int i, f32x2 u) {
+  // kMost: what overflows is inf, for two instructions (of a prompt's 230 us 6; a single token has them to spare).  Without: not defined.
+  template <bool kMost = false> __device__ __forceinline__ void begin(int i, f32x2 u) {
     const float2 v = split2(u);
-    r[i] = pack2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+    const auto most = [](float f) { return kMost ? fminf(f, 128.f) : f; };
+    r[i] = pack2(most(fmaxf(v.x, -126.f)), most(fmaxf(v.y, -126.f)));
   }
   __device__ __forceinline__ void run() {
 #pragma unroll

@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) scan_step_kernel(
     Poly<kPoly> poly;                                  // the slow states' decays: an error of one sign would add up from call to call
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (i < kPoly) poly.begin(i, mul2(step, a2[i]));
+      if (i < kPoly) poly.template begin<true>(i, mul2(step, a2[i]));
       else e[i] = exp2_unit(mul2(step, a2[i]));
     }
     poly.run();

@@ -119,7 +119,7 @@ def selective_scan(*, x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, d:
     x, dt ``[tgt_len, bsz, channels]``; b, c ``[tgt_len, bsz, num_groups, num_states]`` of x's dtype, shared by the
     ``channels / num_groups`` adjacent channels of a group (their gradients are sums over them); a ``[channels, num_states]``
     (finite, 1 to 64 states), d and dt_bias ``[channels]``, fp32.  ``delta * a`` is to stay below 88, where exp overflows
-    (it is negative in a model, whose states decay)."""
+    (it is negative in a model, whose states decay): beyond that the results are not defined."""
     mask = _mask(key_padding_mask)
     if plain_tensors(x, dt, a, b, c, d, dt_bias, mask):
         return native().selective_scan_node(x, dt, a, b, c, d, dt_bias, mask, dt_softplus)

@@ -283,6 +283,18 @@ def test_scan_of_states_that_grow(dev, N):
         near(t, want[n], size[n], (20 * 200 + 16 + 2 * N) * 2.0 ** -24, n)
 
 
+@pytest.mark.parametrize("N", [3, 16, 40])
+def test_a_token_whose_growth_overflows_leaves_inf(dev, N):
+    """exp(88.5) is the last power that is finite; exp(100), of every state, is inf of the state's sign, and zero stays what is added."""
+    x, bc = torch.ones(1, 2, 6, device=dev), torch.zeros(1, 2, 1, N, device=dev)
+    s = torch.ones(2, 6, N, device=dev)
+    s[1] = -1
+    for power, want in ((88.5, float(torch.tensor(88.5, dtype=torch.float64).exp())), (100.0, float("inf")), (1e30, float("inf"))):
+        _, held = ss.incremental_selective_scan(x=x, dt=x * power, a=torch.ones(6, N, device=dev), b=bc, c=bc, s=s.clone(), dt_softplus=False)
+        # 88.5 log2(e) = 127.7 is rounded by 2^-18 (2.6e-6 of the power), log2(e) by 1.3e-8 (1.2e-6), the power by 2^-22: below 5e-6
+        assert torch.allclose(held, s * want, rtol=5e-6, atol=0)
+
+
 @pytest.mark.parametrize("cut", [1, 16, 100, 299])
 def test_scan_in_two_calls(dev, cut):
     """A prompt in two calls is the prompt in one, whichever way either is cut into segments."""
