@@ -818,3 +818,54 @@ def test_tensor_level_calls_refuse_gradients_of_other_shapes_and_devices(dev):
             scan(x, None, wrong)
     with pytest.raises(RuntimeError, match="expected all tensors on"):
         scan(x, None, kept.cpu())
+
+
+def test_layer_decodes_inside_a_graph(dev):
+    """One token's call with the kept state, captured once and replayed for every token, is the eager loop: the state is updated where it is."""
+    m = layer(dev, F16).requires_grad_(False)
+    x = torch.randn(12, 3, 96, generator=torch.Generator().manual_seed(4)).half().to(dev)
+    eager, kept = {}, {}
+    m(x[:5], saved_state=eager)
+    m(x[:5], saved_state=kept)
+    want = [m(x[t:t + 1], saved_state=eager) for t in range(5, 12)]
+    one = x[5:6].clone()
+    begin = {k: v.clone() for k, v in kept.items()}
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        m(one, saved_state=kept)                                  # warm-up
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = m(one, saved_state=kept)
+    for k, v in begin.items():
+        kept[k].copy_(v)
+    for t, y in zip(range(5, 12), want):
+        one.copy_(x[t:t + 1])
+        graph.replay()
+        # the matrix products may take another algorithm on another stream: a few steps of fp16 through seven roundings
+        assert (out - y).float().norm() <= 1e-2 * y.float().norm()
+    for k in begin:
+        assert (kept[k] - eager[k]).float().norm() <= 1e-2 * eager[k].float().norm()
+
+
+def test_a_state_in_place_of_several_tokens_inside_a_graph(dev):
+    """The incremental forms over a few tokens, captured: each replay goes on from the state that the one before it left, with the eager bits."""
+    _, (x, w, b) = calls(dev)["conv"]
+    _, ts = calls(dev)["scan"]
+    args = dict(zip(("x", "dt", "a", "b", "c", "d", "dt_bias"), ts))
+    for T in (1, 20):
+        xt = x[:T]
+        cut = {k: v[:T] if v.dim() >= 3 else v for k, v in args.items()}
+        held = torch.randn(3, 3, 64, device=dev).half(), torch.randn(3, 64, 16, device=dev)
+        apart = [t.clone() for t in held]
+        call = lambda s: (ss.incremental_causal_conv(x=xt, weight=w, bias=b, state=s[0]), ss.incremental_selective_scan(**cut, s=s[1]))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            (y1, s1), (y2, s2) = call(held)
+        assert s1 is held[0] and s2 is held[1] and all(torch.equal(a, c) for a, c in zip(held, apart))      # capture runs nothing
+        for _ in range(3):
+            graph.replay()
+            (w1, _), (w2, _) = call(apart)
+            assert all(torch.equal(a, c) for a, c in zip((y1, y2, *held), (w1, w2, *apart)))
