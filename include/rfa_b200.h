@@ -511,6 +511,84 @@ int rfa_group_norm_bwd(const rfa_group_norm_t* norm, const void* g, int64_t g_r,
                        void* g_gate, void* g_weight, void* g_bias,
                        void* workspace, size_t workspace_bytes, rfa_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Attention of bounded memory beside causal RFA: linear attention whose state
+ * decays, and softmax attention over a sliding window.  No upstream counterpart.
+ *
+ * Activations are time-major, [T, B, H, width] with a head's numbers adjacent; an
+ * input may have any other strides (in elements: *_t from token to token, *_b from
+ * batch row to batch row, *_h from head to head), outputs and gradients are
+ * contiguous.  dtype (RFA_F16, RFA_F32 or RFA_BF16) is the type of all activations;
+ * states, sums and softmax statistics are fp32.  mask [B, T] bytes or NULL, non-zero
+ * = a padded token: every result of the others is what it would be if padded tokens
+ * were not there, whatever stands in them, and a padded token's outputs and
+ * gradients are zero.  States, caches and workspaces are 16-byte aligned, else no
+ * alignment is asked for.  Heads of at most 256; T < 2^31 - 256, B and H <= 65535,
+ * B H < 2^24; a size of zero is refused.  Outputs overlap neither inputs nor each
+ * other, but for states and caches where that is said.  What a batch row holds reaches
+ * no other row's results; the same call gives the same bits.
+ * ---------------------------------------------------------------------- */
+
+/* Linear attention with a decay for each head:
+ *   S_t = e^(log_decay_t) S_(t-1) + k_t (x) v_t,   out_t = scale q_t S_t
+ * q, k [T, B, H, K], v and out [T, B, H, D], states [B, H, K, D] fp32 (s_in NULL:
+ * zeros), log_decay of decay_dtype with strides g_*, zero where it does not depend on
+ * the token or the batch row. */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_t, q_b, q_h, k_t, k_b, k_h, v_t, v_b, v_h;
+  const void* log_decay;
+  int64_t g_t, g_b, g_h;
+  const float* s_in;
+  const uint8_t* mask;
+  int64_t T;
+  int B, H, K, D, dtype, decay_dtype;
+  int per_head;              /* backward: g_decay is [H], the sum over tokens and batch rows; else [T, B, H] */
+  float scale;
+} rfa_decay_t;
+size_t rfa_decay_workspace_bytes(int64_t T, int B, int H, int K, int D, int dtype, int backward);
+/* s_out: the last state, or NULL; it may be s_in. */
+int rfa_decay_fwd(const rfa_decay_t* decay, void* out, float* s_out,
+                  void* workspace, size_t workspace_bytes, rfa_stream_t stream);
+/* g [T, B, H, D] contiguous, g_s [B, H, K, D] of the last state or NULL -> gq, gk, gv;
+ * g_decay of decay_dtype and gs_in [B, H, K, D], each or NULL. */
+int rfa_decay_bwd(const rfa_decay_t* decay, const void* g, const float* g_s, void* gq,
+                  void* gk, void* gv, void* g_decay, float* gs_in,
+                  void* workspace, size_t workspace_bytes, rfa_stream_t stream);
+/* One token (T = 1): the state s is updated in place (s_in is not read). */
+int rfa_decay_step(const rfa_decay_t* decay, void* out, float* s, rfa_stream_t stream);
+
+/* Softmax attention over a sliding window: token i sees token j <= i where i - j <
+ * window or j < sinks (the first tokens stay visible), padded tokens not counted.
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j
+ * q and out [T, B, H, D], k, v [T, B, G, D]; query heads h G / H ... share a key head.
+ * A query that is padded gets zero. */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_t, q_b, q_h, k_t, k_b, k_h, v_t, v_b, v_h;
+  const uint8_t* mask;
+  int64_t T;
+  int B, H, G, D, dtype, window, sinks;
+  float scale;
+} rfa_window_t;
+/* Scratch of a forward (backward = 0) or backward (1) call. */
+size_t rfa_window_workspace_bytes(int64_t T, int B, int H, int G, int D, int dtype, int window, int sinks, int backward);
+/* lse [B, H, T] fp32, or NULL: what the backward wants of the softmax. */
+int rfa_window_fwd(const rfa_window_t* window, void* out, float* lse,
+                   void* workspace, size_t workspace_bytes, rfa_stream_t stream);
+/* g, out [T, B, H, D] contiguous -> gq [T, B, H, D], gk, gv [T, B, G, D]. */
+int rfa_window_bwd(const rfa_window_t* window, const void* out, const float* lse,
+                   const void* g, void* gq, void* gk, void* gv,
+                   void* workspace, size_t workspace_bytes, rfa_stream_t stream);
+/* Decoding.  The cache: cache_k, cache_v [B, G, sinks + window, D] of dtype, length [B]
+ * int64, the number of tokens so far (below 2^40).  Token number p is kept at p where p <
+ * sinks, else at sinks + (p - sinks) % window.  The call appends its T tokens, attends
+ * and updates cache and length in place; empty != 0: nothing is in the cache yet,
+ * whatever length holds.  Slots that hold no token are neither read nor written. */
+size_t rfa_window_append_workspace_bytes(int64_t T, int B, int H, int G, int D, int dtype, int window, int sinks, int empty);
+int rfa_window_append(const rfa_window_t* window, void* cache_k, void* cache_v, int64_t* length, int empty,
+                      void* out, void* workspace, size_t workspace_bytes, rfa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,9 +14,11 @@ from .utils import CrossAttentionState
 from .causal_attention import CausalAttention
 from .cross_attention import CrossAttention, CrossAttentionProject
 from .state_space import SelectiveStateSpace
+from .decay_attention import DecayAttention
+from .window_attention import WindowAttention
 
 __all__ = ["CausalAttention", "CrossAttention", "CrossAttentionState", "CrossAttentionProject",
-           "SelectiveStateSpace", "install_aliases"]
+           "SelectiveStateSpace", "DecayAttention", "WindowAttention", "install_aliases"]
 
 
 def install_aliases() -> None:

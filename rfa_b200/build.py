@@ -1,5 +1,5 @@
 """Build the C-ABI shared library ``rfa_b200/csrc/librfa_b200.so`` with nvcc for sm_100a, and ``rfa_b200/_native.so``, the
-tensor-level calls over it (``csrc/torch_ops.cpp`` and ``torch_state_space.cpp``, against this interpreter's torch).
+tensor-level calls over it (``csrc/torch_ops.cpp``, ``torch_state_space.cpp`` and ``torch_attention.cpp``, against this interpreter's torch).
 
     python -m rfa_b200.build [--force] [--verbose]
 
@@ -19,7 +19,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "librfa_b200.so")
 NATIVE_SRC, NATIVE = os.path.join(CSRC, "torch_ops.cpp"), os.path.join(HERE, "_native.so")
-NATIVE_SRCS = [NATIVE_SRC, os.path.join(CSRC, "torch_state_space.cpp")]
+NATIVE_SRCS = [NATIVE_SRC, *(os.path.join(CSRC, f) for f in ("torch_state_space.cpp", "torch_attention.cpp"))]
+NATIVE_HEADERS = [*(os.path.join(CSRC, f) for f in ("torch_call.h", "torch_checks.h")), os.path.join(os.path.dirname(HERE), "include", "rfa_b200.h")]
 NATIVE_KEY = os.path.join(HERE, "_native.key")      # what the module was built for (see native_key)
 
 NVCC_FLAGS = [
@@ -77,7 +78,7 @@ def native_key() -> str:
 
 
 def native_stale() -> bool:
-    if stale(NATIVE, [*NATIVE_SRCS, os.path.join(CSRC, "torch_call.h"), os.path.join(os.path.dirname(HERE), "include", "rfa_b200.h")]) or not os.path.exists(NATIVE_KEY):
+    if stale(NATIVE, [*NATIVE_SRCS, *NATIVE_HEADERS]) or not os.path.exists(NATIVE_KEY):
         return True
     with open(NATIVE_KEY) as f:
         return f.read() != native_key()

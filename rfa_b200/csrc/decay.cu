@@ -1,0 +1,136 @@
+// Linear attention with a decay: the C entry points.  Which kernels a call takes is decided here, from its sizes, type and alignment.
+#include <algorithm>
+
+#include "decay.cuh"
+
+namespace rfa {
+
+namespace {
+
+int decay_check(const rfa_decay_t* c, const char* what) {
+  RFA_REQUIRE(c, RFA_EINVAL, "%s: null argument", what);
+  RFA_REQUIRE(c->q && c->k && c->v && c->log_decay, RFA_EINVAL, "%s: null pointer", what);
+  RFA_REQUIRE(c->T > 0 && c->B > 0 && c->H > 0 && c->K > 0 && c->D > 0, RFA_EINVAL, "%s: empty or negative size", what);
+  for (const int t : {c->dtype, c->decay_dtype})
+    RFA_REQUIRE(t == RFA_F16 || t == RFA_F32 || t == RFA_BF16, RFA_EUNSUPPORTED, "%s: dtype %d", what, t);
+  RFA_REQUIRE(c->K <= kDecayMaxWidth && c->D <= kDecayMaxWidth, RFA_EUNSUPPORTED, "%s: heads of %d and %d (at most %d)", what, c->K, c->D, kDecayMaxWidth);
+  RFA_REQUIRE(c->T < ((int64_t)1 << 31) - 256 && c->B <= 65535 && c->H <= 65535 && (int64_t)c->B * c->H < (1 << 24), RFA_EUNSUPPORTED, "%s: T %lld, B %d, H %d", what,
+              (long long)c->T, c->B, c->H);
+  RFA_REQUIRE(aligned16(c->s_in), RFA_EALIGN, "%s: s_in is not 16-byte aligned", what);
+  return 0;
+}
+
+size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Workspace of a backward pass: the arrays of the largest sweep, then what the decays' gradient is made of.
+struct BwdPlan {
+  SweepPlan wide, tall;             // x3 as wide as k (gq, gk), as v (gv)
+  size_t sweep, dots, last, sums;   // bytes; dots: each of two
+  explicit BwdPlan(const rfa_decay_t& c) {
+    const int64_t BH = (int64_t)c.B * c.H;
+    wide = sweep_plan(c.T, BH, c.D, c.K);
+    tall = sweep_plan(c.T, BH, c.K, c.D);
+    sweep = std::max(round256(wide.totals) + round256(wide.seg_decay), round256(tall.totals) + round256(tall.seg_decay));
+    dots = round256(sizeof(float) * sweep_tiles(c.K) * BH * c.T);
+    last = round256(sizeof(float) * BH * c.K * c.D);
+    sums = round256(sizeof(float) * BH);
+  }
+  size_t bytes() const { return sweep + 2 * dots + last + sums; }
+};
+
+SweepArgs sweep_args(const rfa_decay_t& c, int A, int W, bool rev, char* ws, const SweepPlan& plan) {
+  SweepArgs a{};
+  a.decay = {c.log_decay, c.g_t, c.g_b, c.g_h};
+  a.mask = c.mask;
+  a.T = c.T; a.B = c.B; a.H = c.H; a.A = A; a.W = W;
+  a.dtype = c.dtype; a.decay_dtype = c.decay_dtype; a.rev = rev;
+  a.in_scale = rev ? c.scale : 1.f;
+  a.out_scale = rev ? 1.f : c.scale;
+  a.totals = reinterpret_cast<float*>(ws);
+  a.seg_decay = reinterpret_cast<double*>(ws + round256(plan.totals));
+  return a;
+}
+
+}  // namespace
+}  // namespace rfa
+
+extern "C" size_t rfa_decay_workspace_bytes(int64_t T, int B, int H, int K, int D, int dtype, int backward) {
+  using namespace rfa;
+  if (T <= 0 || B <= 0 || H <= 0 || K <= 0 || D <= 0) return 0;
+  rfa_decay_t c{};
+  c.T = T; c.B = B; c.H = H; c.K = K; c.D = D; c.dtype = dtype;
+  if (backward) return BwdPlan(c).bytes();
+  const SweepPlan p = sweep_plan(T, (int64_t)B * H, K, D);
+  return round256(p.totals) + round256(p.seg_decay);
+}
+
+extern "C" int rfa_decay_fwd(const rfa_decay_t* c, void* out, float* s_out, void* workspace, size_t workspace_bytes, rfa_stream_t stream) {
+  using namespace rfa;
+  if (int r = decay_check(c, "decay_fwd")) return r;
+  RFA_REQUIRE(out, RFA_EINVAL, "decay_fwd: null pointer");
+  RFA_REQUIRE(aligned16(s_out) && aligned16(workspace), RFA_EALIGN, "decay_fwd: s_out or workspace is not 16-byte aligned");
+  const size_t need = rfa_decay_workspace_bytes(c->T, c->B, c->H, c->K, c->D, c->dtype, 0);
+  RFA_REQUIRE(!need || (workspace && workspace_bytes >= need), RFA_EWORKSPACE, "decay_fwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
+  const SweepPlan plan = sweep_plan(c->T, (int64_t)c->B * c->H, c->K, c->D);
+  SweepArgs a = sweep_args(*c, c->K, c->D, false, static_cast<char*>(workspace), plan);
+  a.x1 = {c->q, c->q_t, c->q_b, c->q_h};
+  a.x2 = {c->k, c->k_t, c->k_b, c->k_h};
+  a.x3 = {c->v, c->v_t, c->v_b, c->v_h};
+  a.out = out;
+  a.s_in = {const_cast<float*>(c->s_in), c->D, 1};
+  a.s_out = {s_out, c->D, 1};
+  return launch_sweep(a, plan, as_stream(stream));
+}
+
+extern "C" int rfa_decay_bwd(const rfa_decay_t* c, const void* g, const float* g_s, void* gq, void* gk, void* gv, void* g_decay, float* gs_in, void* workspace,
+                             size_t workspace_bytes, rfa_stream_t stream) {
+  using namespace rfa;
+  if (int r = decay_check(c, "decay_bwd")) return r;
+  RFA_REQUIRE(g && gq && gk && gv, RFA_EINVAL, "decay_bwd: null pointer");
+  RFA_REQUIRE(aligned16(g_s) && aligned16(gs_in) && aligned16(workspace), RFA_EALIGN, "decay_bwd: g_s, gs_in or workspace is not 16-byte aligned");
+  const BwdPlan plan(*c);
+  RFA_REQUIRE(workspace && workspace_bytes >= plan.bytes(), RFA_EWORKSPACE, "decay_bwd: workspace %zu bytes, %zu needed", workspace_bytes, plan.bytes());
+  const cudaStream_t st = as_stream(stream);
+  char* ws = static_cast<char*>(workspace);
+  float* q_dots = reinterpret_cast<float*>(ws + plan.sweep);
+  float* k_dots = reinterpret_cast<float*>(ws + plan.sweep + plan.dots);
+  float* last = reinterpret_cast<float*>(ws + plan.sweep + 2 * plan.dots);
+  float* sums = reinterpret_cast<float*>(ws + plan.sweep + 2 * plan.dots + plan.last);
+  const DecayRows q{c->q, c->q_t, c->q_b, c->q_h}, k{c->k, c->k_t, c->k_b, c->k_h}, v{c->v, c->v_t, c->v_b, c->v_h};
+  const DecayRows gr{g, (int64_t)c->B * c->H * c->D, (int64_t)c->H * c->D, c->D};
+  float *s_in = const_cast<float*>(c->s_in), *g_last = const_cast<float*>(g_s);
+
+  SweepArgs a = sweep_args(*c, c->D, c->K, false, ws, plan.wide);
+  a.x1 = gr; a.x2 = v; a.x3 = k; a.out = gq;
+  a.s_in = {s_in, 1, c->D};
+  if (g_decay) {
+    a.x4 = q; a.dots = q_dots;
+    if (g_s) a.s_out = {last, 1, c->D};
+  }
+  if (int r = launch_sweep(a, plan.wide, st)) return r;
+
+  a = sweep_args(*c, c->D, c->K, true, ws, plan.wide);
+  a.x1 = v; a.x2 = gr; a.x3 = q; a.out = gk;
+  a.s_in = {g_last, 1, c->D};
+  if (g_decay) { a.x4 = k; a.dots = k_dots; }
+  if (int r = launch_sweep(a, plan.wide, st)) return r;
+
+  a = sweep_args(*c, c->K, c->D, true, ws, plan.tall);
+  a.x1 = k; a.x2 = q; a.x3 = gr; a.out = gv;
+  a.s_in = {g_last, c->D, 1};
+  a.s_out = {gs_in, c->D, 1};
+  if (int r = launch_sweep(a, plan.tall, st)) return r;
+
+  if (!g_decay) return 0;
+  const int tiles = sweep_tiles(c->K);
+  return launch_decay_grad(q_dots, tiles, k_dots, tiles, g_s, last, c->K * c->D, c->mask, g_decay, c->decay_dtype, c->per_head != 0, sums, c->T, c->B, c->H, st);
+}
+
+extern "C" int rfa_decay_step(const rfa_decay_t* c, void* out, float* s, rfa_stream_t stream) {
+  using namespace rfa;
+  if (int r = decay_check(c, "decay_step")) return r;
+  RFA_REQUIRE(out && s, RFA_EINVAL, "decay_step: null pointer");
+  RFA_REQUIRE(c->T == 1, RFA_EINVAL, "decay_step: %lld tokens", (long long)c->T);
+  RFA_REQUIRE(aligned16(s), RFA_EALIGN, "decay_step: s is not 16-byte aligned");
+  return launch_decay_step(*c, out, s, as_stream(stream));
+}

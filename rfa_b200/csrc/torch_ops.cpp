@@ -564,6 +564,7 @@ Tensor cross_query_node(const Tensor& phi_q, const Tensor& s, const Tensor& z) {
 }  // namespace
 
 void def_state_space(py::module_& m);      // torch_state_space.cpp
+void def_attention(py::module_& m);        // torch_attention.cpp
 
 // Without the interpreter lock, as the foreign calls before them: an allocation, a launch on a full queue or the synchronisation
 // of an error report blocks this thread only.
@@ -592,4 +593,5 @@ PYBIND11_MODULE(_native, m) {
   def("cross_state_node", &cross_state_node);
   def("cross_query_node", &cross_query_node);
   def_state_space(m);
+  def_attention(m);
 }

@@ -1,0 +1,121 @@
+// Sliding-window attention: the C entry points.
+#include "window.cuh"
+
+namespace rfa {
+
+namespace {
+
+int window_check(const rfa_window_t* c, const char* what) {
+  RFA_REQUIRE(c, RFA_EINVAL, "%s: null argument", what);
+  RFA_REQUIRE(c->q && c->k && c->v, RFA_EINVAL, "%s: null pointer", what);
+  RFA_REQUIRE(c->T > 0 && c->B > 0 && c->H > 0 && c->G > 0 && c->D > 0, RFA_EINVAL, "%s: empty or negative size", what);
+  RFA_REQUIRE(c->dtype == RFA_F16 || c->dtype == RFA_F32 || c->dtype == RFA_BF16, RFA_EUNSUPPORTED, "%s: dtype %d", what, c->dtype);
+  RFA_REQUIRE(c->H % c->G == 0, RFA_EUNSUPPORTED, "%s: %d heads share %d key heads", what, c->H, c->G);
+  RFA_REQUIRE(c->D <= kWindowMaxWidth, RFA_EUNSUPPORTED, "%s: heads of %d (at most %d)", what, c->D, kWindowMaxWidth);
+  RFA_REQUIRE(c->window >= 1 && c->sinks >= 0 && (int64_t)c->window + c->sinks < (1 << 30), RFA_EUNSUPPORTED, "%s: window %d, sinks %d", what, c->window, c->sinks);
+  RFA_REQUIRE(c->T < ((int64_t)1 << 30) && c->B <= 65535 && c->H <= 65535 && (int64_t)c->B * c->H < (1 << 24), RFA_EUNSUPPORTED, "%s: T %lld, B %d, H %d", what,
+              (long long)c->T, c->B, c->H);
+  return 0;
+}
+
+size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+size_t order_bytes(int64_t S, int B) { return round256(4 * (size_t)S * B) + round256(4 * (size_t)(S + 1) * B); }
+
+WindowArgs window_args(const rfa_window_t& c) {
+  WindowArgs a{};
+  a.q = {c.q, c.q_t, c.q_b, c.q_h};
+  a.k = {c.k, c.k_t, c.k_b, c.k_h};
+  a.v = {c.v, c.v_t, c.v_b, c.v_h};
+  a.T = a.S = c.T;
+  a.B = c.B; a.H = c.H; a.G = c.G; a.D = c.D; a.window = c.window; a.sinks = c.sinks; a.dtype = c.dtype;
+  a.scale = c.scale;
+  return a;
+}
+// numbers of the places, at the workspace's start
+int number(WindowArgs& a, const rfa_window_t& c, const int64_t* length, int cap, void* workspace, cudaStream_t stream) {
+  int32_t* order = static_cast<int32_t*>(workspace);
+  int32_t* pos = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + round256(4 * (size_t)a.S * c.B));
+  a.order = order;
+  a.pos = pos;
+  return launch_window_order(c.mask, length, cap, order, pos, c.T, c.B, stream);
+}
+
+}  // namespace
+}  // namespace rfa
+
+extern "C" size_t rfa_window_workspace_bytes(int64_t T, int B, int H, int G, int D, int dtype, int window, int sinks, int backward) {
+  using namespace rfa;
+  if (T <= 0 || B <= 0 || H <= 0 || G <= 0 || D <= 0) return 0;
+  return order_bytes(T, B) + (backward ? round256(4 * (size_t)T * B * H) : 0);
+}
+
+extern "C" int rfa_window_fwd(const rfa_window_t* c, void* out, float* lse, void* workspace, size_t workspace_bytes, rfa_stream_t stream) {
+  using namespace rfa;
+  if (int r = window_check(c, "window_fwd")) return r;
+  RFA_REQUIRE(out, RFA_EINVAL, "window_fwd: null pointer");
+  RFA_REQUIRE(aligned16(lse) && aligned16(workspace), RFA_EALIGN, "window_fwd: lse or workspace is not 16-byte aligned");
+  const size_t need = rfa_window_workspace_bytes(c->T, c->B, c->H, c->G, c->D, c->dtype, c->window, c->sinks, 0);
+  RFA_REQUIRE(workspace && workspace_bytes >= need, RFA_EWORKSPACE, "window_fwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
+  WindowArgs a = window_args(*c);
+  a.out = out;
+  a.lse = lse;
+  if (c->mask)
+    if (int r = number(a, *c, nullptr, 0, workspace, as_stream(stream))) return r;
+  return launch_window_fwd_tiles(a, as_stream(stream));
+}
+
+extern "C" int rfa_window_bwd(const rfa_window_t* c, const void* out, const float* lse, const void* g, void* gq, void* gk, void* gv, void* workspace, size_t workspace_bytes,
+                              rfa_stream_t stream) {
+  using namespace rfa;
+  if (int r = window_check(c, "window_bwd")) return r;
+  RFA_REQUIRE(out && lse && g && gq && gk && gv, RFA_EINVAL, "window_bwd: null pointer");
+  RFA_REQUIRE(aligned16(lse) && aligned16(workspace), RFA_EALIGN, "window_bwd: lse or workspace is not 16-byte aligned");
+  const size_t need = rfa_window_workspace_bytes(c->T, c->B, c->H, c->G, c->D, c->dtype, c->window, c->sinks, 1);
+  RFA_REQUIRE(workspace && workspace_bytes >= need, RFA_EWORKSPACE, "window_bwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
+  WindowArgs a = window_args(*c);
+  const int64_t row = (int64_t)c->H * c->D;
+  a.o = {out, c->B * row, row, c->D};
+  a.g = {g, c->B * row, row, c->D};
+  a.lse = const_cast<float*>(lse);
+  a.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + order_bytes(c->T, c->B));
+  a.gq = gq; a.gk = gk; a.gv = gv;
+  if (c->mask)
+    if (int r = number(a, *c, nullptr, 0, workspace, as_stream(stream))) return r;
+  return launch_window_bwd_tiles(a, as_stream(stream));
+}
+
+extern "C" size_t rfa_window_append_workspace_bytes(int64_t T, int B, int H, int G, int D, int dtype, int window, int sinks, int empty) {
+  using namespace rfa;
+  if (T <= 0 || B <= 0 || H <= 0 || G <= 0 || D <= 0 || window < 1 || sinks < 0) return 0;
+  if (T == 1 && !empty) return 0;
+  const int64_t S = T + (empty ? 0 : (int64_t)window + sinks);
+  return order_bytes(S, B) + (empty ? 0 : 2 * round256((size_t)S * B * G * D * (dtype == RFA_F32 ? 4 : 2)));
+}
+
+extern "C" int rfa_window_append(const rfa_window_t* c, void* cache_k, void* cache_v, int64_t* length, int empty, void* out, void* workspace, size_t workspace_bytes,
+                                 rfa_stream_t stream) {
+  using namespace rfa;
+  if (int r = window_check(c, "window_append")) return r;
+  RFA_REQUIRE(cache_k && cache_v && length && out, RFA_EINVAL, "window_append: null pointer");
+  RFA_REQUIRE(aligned16(cache_k) && aligned16(cache_v) && aligned16(workspace), RFA_EALIGN, "window_append: cache or workspace is not 16-byte aligned");
+  const size_t need = rfa_window_append_workspace_bytes(c->T, c->B, c->H, c->G, c->D, c->dtype, c->window, c->sinks, empty);
+  RFA_REQUIRE(!need || (workspace && workspace_bytes >= need), RFA_EWORKSPACE, "window_append: workspace %zu bytes, %zu needed", workspace_bytes, need);
+  const cudaStream_t st = as_stream(stream);
+  if (c->T == 1 && !empty) return launch_window_step(*c, cache_k, cache_v, length, out, st);
+  WindowArgs a = window_args(*c);
+  a.out = out;
+  const int cap = empty ? 0 : c->sinks + c->window;
+  a.S = cap + c->T;
+  if (c->mask || !empty)
+    if (int r = number(a, *c, empty ? nullptr : length, cap, workspace, st)) return r;
+  if (!empty) {
+    char* keys = static_cast<char*>(workspace) + order_bytes(a.S, c->B);
+    char* values = keys + round256((size_t)a.S * c->B * c->G * c->D * (c->dtype == RFA_F32 ? 4 : 2));
+    if (int r = launch_window_gather(*c, cache_k, cache_v, length, keys, values, st)) return r;
+    const int64_t row = (int64_t)c->G * c->D;
+    a.k = {keys, c->B * row, row, c->D};
+    a.v = {values, c->B * row, row, c->D};
+  }
+  if (int r = launch_window_fwd_tiles(a, st)) return r;
+  return launch_window_keep(*c, cache_k, cache_v, length, a.order, empty != 0, st);
+}

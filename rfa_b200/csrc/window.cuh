@@ -1,0 +1,56 @@
+// Shared by the kernels of sliding-window attention (window.cu, window_tiles.cu, window_step.cu).
+//
+// Tokens are numbered within their sequence, padded ones not counted; token number n sees number m <= n where n - m < window or m < sinks.  Without
+// padding and without a cache in front a token's number is its place.  Otherwise `order` holds it, or ~(the number of real tokens before) for a place that holds
+// none, and `pos` the place of each number (S behind the last): both grow along the places, so that a tile's span of keys is two look-ups.
+#pragma once
+
+#include "state_space.cuh"
+
+namespace rfa {
+
+constexpr int kWindowMaxWidth = 256;
+
+struct WindowRows {      // [T][B][heads] of D adjacent elements, strides in elements
+  const void* p;
+  int64_t t, b, h;
+};
+struct WindowArgs {
+  WindowRows q, k, v, g, o;
+  const int32_t *order, *pos;      // [B][S], [B][S + 1]; null: places are numbers
+  void *out, *gq, *gk, *gv;        // contiguous
+  float *lse, *delta;              // [B][H][T], in units of the exponential's base e; the backward's sum of g . out
+  int64_t T, S;                    // queries, keys: query t stands at place S - T + t
+  int B, H, G, D, window, sinks, dtype;
+  float scale;
+};
+
+#ifdef __CUDACC__
+struct WindowNumbers {
+  const int32_t *order, *pos;
+  int64_t S;
+  int window, sinks;
+  __device__ __forceinline__ WindowNumbers(const WindowArgs& a, int b)
+      : order(a.order ? a.order + b * a.S : nullptr), pos(a.pos ? a.pos + b * (a.S + 1) : nullptr), S(a.S), window(a.window), sinks(a.sinks) {}
+  // the number at a place, negative where there is none
+  __device__ __forceinline__ int at(int64_t s) const { return s < 0 || s >= S ? -1 : order ? order[s] : (int)s; }
+  __device__ __forceinline__ int64_t real_before(int64_t s) const { const int n = at(s); return n < 0 ? ~n : n; }      // 0 <= s < S
+  __device__ __forceinline__ int64_t place(int64_t n) const { return n < 0 ? 0 : n >= S ? S : pos ? pos[n] : n; }
+  // queries at places [p0, p1) see keys in front of first_end() and keys from first_key(p0) to p1
+  __device__ __forceinline__ int64_t first_key(int64_t p0) const { return place(real_before(p0) - window + 1); }
+  __device__ __forceinline__ int64_t first_end() const { return sinks > 0 ? min(S, place(sinks - 1) + 1) : 0; }
+  // keys at places [p0, p1) are seen by no query at or behind this place
+  __device__ __forceinline__ int64_t last_query(int64_t p0, int64_t p1) const { return p0 < first_end() ? S : min(S, place(real_before(p1 - 1) + window)); }
+};
+__device__ __forceinline__ bool window_sees(int n, int m, int window, int sinks) { return m >= 0 && m <= n && (n - m < window || m < sinks); }
+#endif
+
+int launch_window_order(const uint8_t* mask, const int64_t* length, int cap, int32_t* order, int32_t* pos, int64_t T, int B, cudaStream_t stream);
+int launch_window_fwd_tiles(const WindowArgs& a, cudaStream_t stream);        // window_tiles.cu: any sizes and types
+int launch_window_bwd_tiles(const WindowArgs& a, cudaStream_t stream);
+int launch_window_step(const rfa_window_t& c, void* cache_k, void* cache_v, int64_t* length, void* out, cudaStream_t stream);      // window_step.cu
+// the cache in front of the new tokens, in the order of their numbers and then themselves: [cap + T][B][G][D]; and back
+int launch_window_gather(const rfa_window_t& c, const void* cache_k, const void* cache_v, const int64_t* length, void* keys, void* values, cudaStream_t stream);
+int launch_window_keep(const rfa_window_t& c, void* cache_k, void* cache_v, int64_t* length, const int32_t* order, bool empty, cudaStream_t stream);
+
+}  // namespace rfa

@@ -1,7 +1,8 @@
 """Tensor-level wrappers over the C ABI: allocate outputs, pass raw pointers and
 the current stream, turn status codes into exceptions.  No arithmetic happens
 here; every function launches kernels from ``librfa_b200.so``.  The calls of the
-forward, backward and decoding paths are in ``csrc/torch_ops.cpp``, those of the state-space operators in ``csrc/torch_state_space.cpp``; the rest go
+forward, backward and decoding paths are in ``csrc/torch_ops.cpp``, those of the state-space operators in ``csrc/torch_state_space.cpp``, those of decaying
+and windowed attention in ``csrc/torch_attention.cpp``; the rest go
 through ctypes.
 """
 from __future__ import annotations
@@ -401,3 +402,34 @@ def group_norm_bwd(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optio
                    need_weight: bool, need_bias: bool, need_gate: bool):
     """(g_x, g_weight, g_bias, g_gate), None for those not needed."""
     return native().group_norm_bwd(x, groups, weight, bias, gate, silu, eps, g, need_weight, need_bias, need_gate)
+
+
+# --------------------------------------------------------------------------- decaying and windowed attention
+def decay_attention_fwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s: Optional[Tensor] = None, mask: Optional[Tensor] = None,
+                        scale: Optional[float] = None, return_state: bool = False, in_place: bool = False):
+    """-> (out, the last state or None: in place of ``s`` with ``in_place``)."""
+    return native().decay_attention_fwd(q, k, v, log_decay, s, mask, scale, return_state, in_place)
+
+
+def decay_attention_bwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s: Optional[Tensor], mask: Optional[Tensor], scale: Optional[float],
+                        g: Tensor, g_s: Optional[Tensor] = None, need_decay: bool = True, need_state: bool = False):
+    """-> (gq, gk, gv, g_log_decay or None, gs or None)."""
+    return native().decay_attention_bwd(q, k, v, log_decay, s, mask, scale, g, g_s, need_decay, need_state)
+
+
+def window_attention_fwd(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, mask: Optional[Tensor] = None, scale: Optional[float] = None,
+                         save: bool = False):
+    """-> (out, with ``save`` what ``window_attention_bwd`` wants of the softmax)."""
+    return native().window_attention_fwd(q, k, v, window, sinks, mask, scale, save)
+
+
+def window_attention_bwd(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, mask: Optional[Tensor], scale: Optional[float], out: Tensor,
+                         lse: Tensor, g: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
+    """-> (gq, gk, gv)."""
+    return native().window_attention_bwd(q, k, v, window, sinks, mask, scale, out, lse, g)
+
+
+def window_attention_append(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, prev_k: Optional[Tensor], prev_v: Optional[Tensor],
+                            prev_len: Optional[Tensor], mask: Optional[Tensor] = None, scale: Optional[float] = None):
+    """-> (out, prev_k, prev_v, prev_len), the cache updated in place."""
+    return native().window_attention_append(q, k, v, window, sinks, prev_k, prev_v, prev_len, mask, scale)
