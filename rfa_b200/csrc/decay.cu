@@ -60,8 +60,9 @@ extern "C" size_t rfa_decay_workspace_bytes(int64_t T, int B, int H, int K, int 
   rfa_decay_t c{};
   c.T = T; c.B = B; c.H = H; c.K = K; c.D = D; c.dtype = dtype;
   if (backward) return BwdPlan(c).bytes();
-  const SweepPlan p = sweep_plan(T, (int64_t)B * H, K, D);
-  return round256(p.totals) + round256(p.seg_decay);
+  size_t most = 0;
+  for (const SweepPlan& p : {sweep_plan(T, (int64_t)B * H, K, D), decay_tc_plan(T, (int64_t)B * H, K, D)}) most = std::max(most, round256(p.totals) + round256(p.seg_decay));
+  return most;
 }
 
 extern "C" int rfa_decay_fwd(const rfa_decay_t* c, void* out, float* s_out, void* workspace, size_t workspace_bytes, rfa_stream_t stream) {
@@ -71,6 +72,7 @@ extern "C" int rfa_decay_fwd(const rfa_decay_t* c, void* out, float* s_out, void
   RFA_REQUIRE(aligned16(s_out) && aligned16(workspace), RFA_EALIGN, "decay_fwd: s_out or workspace is not 16-byte aligned");
   const size_t need = rfa_decay_workspace_bytes(c->T, c->B, c->H, c->K, c->D, c->dtype, 0);
   RFA_REQUIRE(!need || (workspace && workspace_bytes >= need), RFA_EWORKSPACE, "decay_fwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
+  if (decay_tc_ok(*c)) return launch_decay_tc(*c, decay_tc_plan(c->T, (int64_t)c->B * c->H, c->K, c->D), static_cast<char*>(workspace), out, s_out, as_stream(stream));
   const SweepPlan plan = sweep_plan(c->T, (int64_t)c->B * c->H, c->K, c->D);
   SweepArgs a = sweep_args(*c, c->K, c->D, false, static_cast<char*>(workspace), plan);
   a.x1 = {c->q, c->q_t, c->q_b, c->q_h};

@@ -47,18 +47,29 @@ struct SweepPlan {
 SweepPlan sweep_plan(int64_t T, int64_t BH, int A, int W);
 int sweep_tiles(int W);
 int launch_sweep(SweepArgs a, const SweepPlan& plan, cudaStream_t stream);
+// totals: what each segment adds -> the state in front of it; at most 65535 (row, head)s
+int launch_decay_combine(float* totals, const double* seg_decay, DecayState s_in, int nseg, int64_t BH, int A, int W, cudaStream_t stream);
 int launch_decay_grad(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_last, int KD, const uint8_t* mask,
                       void* g_decay, int decay_dtype, bool per_head, float* sums, int64_t T, int B, int H, cudaStream_t stream);
+
+// decay_tc.cu: fp16 and bf16, heads of up to 128 in rows that a tensor map can describe
+bool decay_tc_ok(const rfa_decay_t& c);
+SweepPlan decay_tc_plan(int64_t T, int64_t BH, int K, int D);
+int launch_decay_tc(const rfa_decay_t& c, const SweepPlan& plan, char* workspace, void* out, float* s_out, cudaStream_t stream);
+
 int launch_decay_step(const rfa_decay_t& c, void* out, float* s, cudaStream_t stream);      // decay_step.cu
 
 #ifdef __CUDACC__
 // A log decay as it is taken: below -1e4 it is that (e^-1e4 is nothing beside any state), so that the differences of sums that cross a reset
 // are numbers.
-__device__ __forceinline__ double log_decay_at(const void* p, int dtype, int64_t i) {
-  const float g = dtype == RFA_F32 ? static_cast<const float*>(p)[i]
-                  : dtype == RFA_F16 ? __half2float(static_cast<const __half*>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+__device__ __forceinline__ uint32_t log_decay_bits(const void* p, int dtype, int64_t i) {      // as it stands in memory, to be asked for early
+  return dtype == RFA_F32 ? static_cast<const uint32_t*>(p)[i] : static_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ double log_decay_of(uint32_t bits, int dtype) {
+  const float g = dtype == RFA_F32 ? __uint_as_float(bits) : dtype == RFA_F16 ? __half2float(__ushort_as_half((uint16_t)bits)) : __uint_as_float(bits << 16);
   return (double)(g < -1e4f ? -1e4f : g);
 }
+__device__ __forceinline__ double log_decay_at(const void* p, int dtype, int64_t i) { return log_decay_of(log_decay_bits(p, dtype, i), dtype); }
 // The factor e^x as whole + part, so that e^x times state is fma(state, part, state * whole): a slow decay is taken as one and what it lacks, whose error
 // is 2^-24 of that and not of one.  The factors of a fixed decay are the same for every chunk or token, and an error of theirs adds up along a sequence.
 struct Factor {

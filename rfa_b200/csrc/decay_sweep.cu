@@ -180,17 +180,29 @@ __global__ void __launch_bounds__(kThreads) decay_sweep_kernel(const __grid_cons
   }
 }
 
-// What each segment adds becomes the state in front of it, in the order of the sweep.  Bound by memory; a thread takes one element along all segments.
+// What each segment adds becomes the state in front of it, in the order of the sweep.  Bound by memory; a thread takes one element along all segments, eight of
+// them on the way at a time.
 __global__ void __launch_bounds__(256) decay_combine_kernel(float* totals, const double* seg_decay, DecayState s_in, int nseg, int64_t BH, int A, int W) {
+  constexpr int kFlight = 8;
   const int64_t bh = blockIdx.y;
   const int i = blockIdx.x * 256 + threadIdx.x, n = A * W;
   if (i >= n) return;
   float s = s_in.p ? s_in.p[bh * n + (i / W) * s_in.row + (i % W) * s_in.col] : 0.f;
-  for (int k = 0; k < nseg; ++k) {
-    float* at = totals + ((int64_t)k * BH + bh) * n + i;
-    const float own = *at;
-    *at = s;
-    s = Factor((float)seg_decay[(int64_t)k * BH + bh]).times(s) + own;
+  for (int k0 = 0; k0 < nseg; k0 += kFlight) {
+    float own[kFlight];
+    double log[kFlight];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f)
+      if (k0 + f < nseg) {
+        own[f] = totals[((k0 + f) * BH + bh) * n + i];
+        log[f] = seg_decay[(k0 + f) * BH + bh];
+      }
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f)
+      if (k0 + f < nseg) {
+        totals[((k0 + f) * BH + bh) * n + i] = s;
+        s = Factor((float)log[f]).times(s) + own[f];
+      }
   }
 }
 
@@ -253,6 +265,15 @@ __global__ void __launch_bounds__(kGradThreads) decay_grad_kernel(const float* q
   }
 }
 
+}  // namespace
+
+int launch_decay_combine(float* totals, const double* seg_decay, DecayState s_in, int nseg, int64_t BH, int A, int W, cudaStream_t stream) {
+  decay_combine_kernel<<<dim3((A * W + 255) / 256, (unsigned)BH), 256, 0, stream>>>(totals, seg_decay, s_in, nseg, BH, A, W);
+  return check_launch("rfa_decay (combine)");
+}
+
+namespace {
+
 template <typename T>
 int sweep_launches(const SweepArgs& a, const SweepPlan& plan, cudaStream_t stream) {
   const size_t smem = sweep_smem_bytes(a.A);
@@ -263,8 +284,7 @@ int sweep_launches(const SweepArgs& a, const SweepPlan& plan, cudaStream_t strea
   if (plan.nseg > 1) {
     decay_sweep_kernel<T><<<grid, kThreads, smem, stream>>>(a, true);
     if (int r = check_launch("rfa_decay (segments)")) return r;
-    decay_combine_kernel<<<dim3((a.A * a.W + 255) / 256, (unsigned)BH), 256, 0, stream>>>(a.totals, a.seg_decay, a.s_in, plan.nseg, BH, a.A, a.W);
-    if (int r = check_launch("rfa_decay (combine)")) return r;
+    if (int r = launch_decay_combine(a.totals, a.seg_decay, a.s_in, plan.nseg, BH, a.A, a.W, stream)) return r;
   }
   decay_sweep_kernel<T><<<grid, kThreads, smem, stream>>>(a, false);
   return check_launch("rfa_decay");

@@ -1,0 +1,86 @@
+// Linear attention with a decay on the tensor cores: plans and launches (the kernel: decay_tc.cuh).
+#define RFA_TC_FAMILY 10
+#include "decay_tc.cuh"
+
+namespace rfa {
+
+namespace {
+
+template <typename T, int KB, int DB, bool OUT, bool EXACT>
+int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const DecayTcArgs& a, bool totals_only, cudaStream_t stream) {
+  constexpr uint32_t smem = DecLayout<KB, DB, OUT, EXACT>::bytes;
+  cudaError_t e = cudaFuncSetAttribute(decay_tc_kernel<T, KB, DB, OUT, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return fail((int)e, "decay: cannot reserve %u bytes of shared memory: %s", smem, cudaGetErrorString(e));
+  e = launch_pdl(decay_tc_kernel<T, KB, DB, OUT, EXACT>, dim3((unsigned)((int64_t)a.B * a.H), a.nseg), dim3(kDecThreads), smem, stream, q, k, v, a, totals_only);
+  if (e != cudaSuccess) return fail((int)e, "rfa_decay: launch failed: %s", cudaGetErrorString(e));
+  return check_launch("rfa_decay");
+}
+template <bool OUT, bool EXACT>
+int launch_sizes(bool bf16, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const DecayTcArgs& a, bool totals_only, cudaStream_t stream) {
+  const int at = (bf16 ? 4 : 0) + (a.K > 64 ? 2 : 0) + (a.D > 64 ? 1 : 0);
+  switch (at) {
+    case 0: return launch<__half, 1, 1, OUT, EXACT>(q, k, v, a, totals_only, stream);
+    case 1: return launch<__half, 1, 2, OUT, EXACT>(q, k, v, a, totals_only, stream);
+    case 2: return launch<__half, 2, 1, OUT, EXACT>(q, k, v, a, totals_only, stream);
+    case 3: return launch<__half, 2, 2, OUT, EXACT>(q, k, v, a, totals_only, stream);
+    case 4: return launch<__nv_bfloat16, 1, 1, OUT, EXACT>(q, k, v, a, totals_only, stream);
+    case 5: return launch<__nv_bfloat16, 1, 2, OUT, EXACT>(q, k, v, a, totals_only, stream);
+    case 6: return launch<__nv_bfloat16, 2, 1, OUT, EXACT>(q, k, v, a, totals_only, stream);
+    default: return launch<__nv_bfloat16, 2, 2, OUT, EXACT>(q, k, v, a, totals_only, stream);
+  }
+}
+
+}  // namespace
+
+bool decay_tc_ok(const rfa_decay_t& c) {
+  return c.dtype != RFA_F32 && c.K <= 128 && c.D <= 128 && tmap_rows_ok(c.q, c.T, c.B, c.H, c.K, c.q_t, c.q_b, c.q_h) &&
+         tmap_rows_ok(c.k, c.T, c.B, c.H, c.K, c.k_t, c.k_b, c.k_h) && tmap_rows_ok(c.v, c.T, c.B, c.H, c.D, c.v_t, c.v_b, c.v_h);
+}
+
+SweepPlan decay_tc_plan(int64_t T, int64_t BH, int K, int D) {
+  const int64_t chunks = (T + kTC - 1) / kTC;
+  // Chunks that an SM goes through one after the other, the reading of keys and values for the segments' own states counted as 0.6 of a chunk, and a few chunks'
+  // time for two more launches
+  int64_t best = (BH + 147) / 148 * chunks * 10, best_n = 1;
+  for (int64_t n = 2; n <= 64 && n * 2 <= chunks && BH <= 148; ++n) {
+    const int64_t cost = (BH * n + 147) / 148 * ((chunks + n - 1) / n) * 16 + 60;
+    if (cost < best) { best = cost; best_n = n; }
+  }
+  SweepPlan p{1, T, 0, 0};
+  if (best_n == 1) return p;
+  p.tseg = (chunks + best_n - 1) / best_n * kTC;
+  p.nseg = (int)((T + p.tseg - 1) / p.tseg);
+  p.totals = sizeof(float) * p.nseg * BH * K * D;
+  p.seg_decay = sizeof(double) * p.nseg * BH;
+  return p;
+}
+
+int launch_decay_tc(const rfa_decay_t& c, const SweepPlan& plan, char* workspace, void* out, float* s_out, cudaStream_t stream) {
+  const bool bf16 = c.dtype == RFA_BF16;
+  CUtensorMap q, k, v;
+  if (make_tmap_heads(&q, c.q, bf16, c.T, c.B, c.H, c.K, c.q_t, c.q_b, c.q_h, kTC) || make_tmap_heads(&k, c.k, bf16, c.T, c.B, c.H, c.K, c.k_t, c.k_b, c.k_h, kTC) ||
+      make_tmap_heads(&v, c.v, bf16, c.T, c.B, c.H, c.D, c.v_t, c.v_b, c.v_h, kTC))
+    return fail(RFA_EDEVICE, "decay: cuTensorMapEncodeTiled failed or is unavailable");
+  DecayTcArgs a{};
+  a.decay = {c.log_decay, c.g_t, c.g_b, c.g_h};
+  a.mask = c.mask;
+  a.out = out;
+  a.s_in = {const_cast<float*>(c.s_in), c.D, 1};
+  a.s_out = {s_out, c.D, 1};
+  a.totals = reinterpret_cast<float*>(workspace);
+  a.seg_decay = reinterpret_cast<double*>(workspace + ((plan.totals + 255) & ~(size_t)255));
+  a.T = c.T; a.tseg = plan.tseg;
+  a.B = c.B; a.H = c.H; a.K = c.K; a.D = c.D; a.nseg = plan.nseg; a.decay_dtype = c.decay_dtype;
+  const bool exact = s_out != nullptr;
+  a.in_scale = 1.f;
+  a.out_scale = c.scale;
+  if (plan.nseg > 1) {
+    if (int r = exact ? launch_sizes<false, true>(bf16, q, k, v, a, true, stream) : launch_sizes<false, false>(bf16, q, k, v, a, true, stream)) return r;
+    if (int r = launch_decay_combine(a.totals, a.seg_decay, a.s_in, plan.nseg, (int64_t)c.B * c.H, c.K, c.D, stream)) return r;
+  }
+  return exact ? launch_sizes<true, true>(bf16, q, k, v, a, false, stream) : launch_sizes<true, false>(bf16, q, k, v, a, false, stream);
+}
+
+RFA_TC_UNIT(decay)
+
+}  // namespace rfa

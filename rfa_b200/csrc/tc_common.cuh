@@ -19,7 +19,7 @@ constexpr uint32_t kBox = 128 * 128;           // bytes of one [128 rows][64 hal
 // (100 * RFA_TC_FAMILY + site) is written to a word of mapped host memory when the host has enabled one
 // (rfa_status_mirror_enable), which the host can look at after any later call without synchronising.
 #ifndef RFA_TC_FAMILY
-#error "define RFA_TC_FAMILY (1..9) before including tc_common.cuh"
+#error "define RFA_TC_FAMILY (see api.cu) before including tc_common.cuh"
 #endif
 static __device__ int g_tc_status;
 static __device__ int* g_tc_mirror;
