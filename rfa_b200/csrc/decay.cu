@@ -37,6 +37,10 @@ struct BwdPlan {
   }
   size_t bytes() const { return sweep + 2 * dots + last + sums; }
 };
+size_t bwd_bytes(const rfa_decay_t& c) {
+  const size_t tc = c.dtype != RFA_F32 && c.K <= 128 && c.D <= 128 && c.K % 8 == 0 && c.D % 8 == 0 ? decay_tc_bwd_bytes(c) : 0;
+  return std::max(BwdPlan(c).bytes(), tc);
+}
 
 SweepArgs sweep_args(const rfa_decay_t& c, int A, int W, bool rev, char* ws, const SweepPlan& plan) {
   SweepArgs a{};
@@ -59,7 +63,7 @@ extern "C" size_t rfa_decay_workspace_bytes(int64_t T, int B, int H, int K, int 
   if (T <= 0 || B <= 0 || H <= 0 || K <= 0 || D <= 0) return 0;
   rfa_decay_t c{};
   c.T = T; c.B = B; c.H = H; c.K = K; c.D = D; c.dtype = dtype;
-  if (backward) return BwdPlan(c).bytes();
+  if (backward) return bwd_bytes(c);
   size_t most = 0;
   for (const SweepPlan& p : {sweep_plan(T, (int64_t)B * H, K, D), decay_tc_plan(T, (int64_t)B * H, K, D)}) most = std::max(most, round256(p.totals) + round256(p.seg_decay));
   return most;
@@ -72,7 +76,7 @@ extern "C" int rfa_decay_fwd(const rfa_decay_t* c, void* out, float* s_out, void
   RFA_REQUIRE(aligned16(s_out) && aligned16(workspace), RFA_EALIGN, "decay_fwd: s_out or workspace is not 16-byte aligned");
   const size_t need = rfa_decay_workspace_bytes(c->T, c->B, c->H, c->K, c->D, c->dtype, 0);
   RFA_REQUIRE(!need || (workspace && workspace_bytes >= need), RFA_EWORKSPACE, "decay_fwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
-  if (decay_tc_ok(*c)) return launch_decay_tc(*c, decay_tc_plan(c->T, (int64_t)c->B * c->H, c->K, c->D), static_cast<char*>(workspace), out, s_out, as_stream(stream));
+  if (decay_tc_ok(*c) && aligned16(out)) return launch_decay_tc(*c, decay_tc_plan(c->T, (int64_t)c->B * c->H, c->K, c->D), static_cast<char*>(workspace), out, s_out, as_stream(stream));
   const SweepPlan plan = sweep_plan(c->T, (int64_t)c->B * c->H, c->K, c->D);
   SweepArgs a = sweep_args(*c, c->K, c->D, false, static_cast<char*>(workspace), plan);
   a.x1 = {c->q, c->q_t, c->q_b, c->q_h};
@@ -90,9 +94,12 @@ extern "C" int rfa_decay_bwd(const rfa_decay_t* c, const void* g, const float* g
   if (int r = decay_check(c, "decay_bwd")) return r;
   RFA_REQUIRE(g && gq && gk && gv, RFA_EINVAL, "decay_bwd: null pointer");
   RFA_REQUIRE(aligned16(g_s) && aligned16(gs_in) && aligned16(workspace), RFA_EALIGN, "decay_bwd: g_s, gs_in or workspace is not 16-byte aligned");
-  const BwdPlan plan(*c);
-  RFA_REQUIRE(workspace && workspace_bytes >= plan.bytes(), RFA_EWORKSPACE, "decay_bwd: workspace %zu bytes, %zu needed", workspace_bytes, plan.bytes());
+  const size_t need = bwd_bytes(*c);
+  RFA_REQUIRE(workspace && workspace_bytes >= need, RFA_EWORKSPACE, "decay_bwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
   const cudaStream_t st = as_stream(stream);
+  if (decay_tc_ok(*c) && aligned16(g) && aligned16(gq) && aligned16(gk) && aligned16(gv))
+    return launch_decay_tc_bwd(*c, static_cast<char*>(workspace), g, g_s, gq, gk, gv, g_decay, gs_in, st);
+  const BwdPlan plan(*c);
   char* ws = static_cast<char*>(workspace);
   float* q_dots = reinterpret_cast<float*>(ws + plan.sweep);
   float* k_dots = reinterpret_cast<float*>(ws + plan.sweep + plan.dots);

@@ -1,0 +1,401 @@
+// Linear attention with a decay on the tensor cores: the gradients of a chunk, fp16 and bf16, heads of up to 128.
+//
+// The states in front of each chunk (S) and their gradients behind it (dS, scaled) have been left by two sweeps of decay_tc.cuh as 16-bit tiles.  Then
+// the chunks do not depend on each other, and one CTA takes one chunk of 128 tokens of a (batch row, head).  With w_ij = scale 2^(L_i - L_j), j <= i:
+//     T0 = Q K^T, T1 = G V^T          -> P = T0 o w, D = T1 o w      16 bits, in shared memory
+//     gq_i = (D K)_i + scale 2^(L_i) (G S^T)_i
+//     gk_j = (D^T Q)_j + 2^(L_end - L_j) (V dS^T)_j
+//     gv_j = (P^T G)_j + 2^(L_end - L_j) (K dS)_j
+// The gradient of the log decay at t is the sum over all pairs of a query i >= t and a key j < t: with M = T0 o T1 o w in fp32
+//     g_t = sum_(i >= t) (rows of M + scale 2^(L_i) q_i . (G S^T)_i) - sum_(j >= t) columns of M + sum_(j < t) 2^(L_end - L_j) k_j . (V dS^T)_j + 2^(L_end) S . dS
+// in which only the rows and columns of one and the same M are subtracted from each other.
+//
+// Warp roles (352 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 the decays, warps 3..10 two groups that share the rows' columns 16 by 16: clear padded rows,
+// T0, T1 -> P, D, then the gradients straight from registers.  P takes the place of S.  TMEM: four regions of 128 columns, T0 / T1 / G S^T / V dS^T, the first three
+// of them used again.  All waits are bounded.
+#define RFA_TC_FAMILY 11
+#include "decay_tc.cuh"
+
+namespace rfa {
+
+constexpr int kDgThreads = 352;
+
+struct DecayGradArgs {
+  DecayRows decay;
+  const uint8_t* mask;
+  const void *states, *grads;      // [B H][chunks][copy]
+  void *gq, *gk, *gv;
+  void* g_decay;                   // null; [T][B][H] of decay_dtype, or per_head: fp32 [B][chunks][H]
+  int64_t T;
+  int B, H, K, D, decay_dtype, per_head;
+  float scale;
+};
+
+template <int KB, int DB>
+struct GradLayout {
+  static constexpr uint32_t kCopyBytes = KB * DB * 64 * 128;
+  static constexpr uint32_t q = 0, k = KB * kBox, v = 2 * KB * kBox, g = v + DB * kBox, s = g + DB * kBox;      // s: S, then P [128][128]
+  static constexpr uint32_t d = s + 2 * kBox, ds = d + 2 * kBox, l = ds + (kCopyBytes + 1023) / 1024 * 1024, col = l + 128 * 4, bar = col + 4 * 128 * 4, bytes = bar + 160;
+  static_assert(bytes <= 227 * 1024, "shared memory");
+};
+enum { gQK = 0, gVG, gS, gDS, gL, gClean, gT, gN1, gN2, gX, gP, gO1, gO2, gE1, gO3, gAll, gSum, gNum };
+
+template <typename T, int KB, int DB>
+__global__ void __launch_bounds__(kDgThreads, 1)
+decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                     const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ DecayGradArgs a) {
+  using Lay = GradLayout<KB, DB>;
+  constexpr int KP = KB * 64, DP = DB * 64;
+  extern __shared__ __align__(1024) unsigned char sm[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::bar);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + gNum);
+  float* L = reinterpret_cast<float*>(sm + Lay::l);
+  float* cols = reinterpret_cast<float*>(sm + Lay::col);      // columns of M, summed over the rows of each warp
+  const uint32_t sbase = smem_u32(sm);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t chunks = (a.T + kTC - 1) / kTC, bh = blockIdx.x / chunks, chunk = blockIdx.x % chunks, t0 = chunk * kTC;
+  const int b = (int)(bh / a.H), h = (int)(bh % a.H);
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.T : nullptr;
+  if (tid == 0) {
+    for (int i = 0; i < gNum; ++i) mbar_init(&bars[i], i == gL ? 32 : i == gClean || i == gX || i == gP || i == gE1 || i == gAll ? 256 : i == gSum ? 128 : 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v); tma_prefetch_desc(&tm_g);
+  }
+  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&bars[gQK], 2 * KB * kBox);
+      for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::q + x * kBox, &tm_q, &bars[gQK], x * 64, h, b, (int)t0);
+      for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::k + x * kBox, &tm_k, &bars[gQK], x * 64, h, b, (int)t0);
+      mbar_arrive_expect_tx(&bars[gVG], 2 * DB * kBox);
+      for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::g + x * kBox, &tm_g, &bars[gVG], x * 64, h, b, (int)t0);
+      for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + x * kBox, &tm_v, &bars[gVG], x * 64, h, b, (int)t0);
+      const int64_t at = (bh * chunks + chunk) * Lay::kCopyBytes;
+      mbar_arrive_expect_tx(&bars[gS], Lay::kCopyBytes);
+      bulk_load(sm + Lay::s, static_cast<const unsigned char*>(a.states) + at, Lay::kCopyBytes, &bars[gS]);
+      mbar_arrive_expect_tx(&bars[gDS], Lay::kCopyBytes);
+      bulk_load(sm + Lay::ds, static_cast<const unsigned char*>(a.grads) + at, Lay::kCopyBytes, &bars[gDS]);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t lead = 1u;
+      constexpr uint32_t idT = umma_idesc<T>(128, 128, false, false);                                                    // Q K^T, G V^T
+      constexpr uint32_t idKK = umma_idesc<T>(128, KP, false, false);                                                   // G S^T, V dS^T
+      constexpr uint32_t idD = umma_idesc<T>(128, DP, false, true), idTD = umma_idesc<T>(128, DP, true, true);          // K dS; P^T G
+      constexpr uint32_t idK = umma_idesc<T>(128, KP, false, true), idTK = umma_idesc<T>(128, KP, true, true);          // D K; D^T Q
+      constexpr uint32_t kCopyBlock = (KP * 128) >> 4;
+      const auto rows = [&](uint32_t at) { return umma_smem_desc(sbase + at, 0, 1024, kSwizzle128B); };                 // K-major
+      const auto columns = [&](uint32_t at, uint32_t block) { return umma_smem_desc(sbase + at, block, 1024, kSwizzle128B); };      // MN-major
+      const uint32_t R0 = tmem, R1 = tmem + 128, R2 = tmem + 256, R3 = tmem + 384;
+      do {
+        if (mask && !mbar_wait(&bars[gClean], 0)) { tc_fail(1); break; }
+        if (!mbar_wait(&bars[gQK], 0)) { tc_fail(2); break; }
+        tc_fence_after_sync();
+        umma_chain_ss<4 * KB, kStepK, kBlockK, kStepK, kBlockK>(lead, R0, rows(Lay::q), rows(Lay::k), idT, 0);
+        if (!mbar_wait(&bars[gVG], 0)) { tc_fail(3); break; }
+        umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockK>(lead, R1, rows(Lay::g), rows(Lay::v), idT, 0);
+        umma_commit(&bars[gT]);
+        if (!mbar_wait(&bars[gS], 0)) { tc_fail(4); break; }
+        umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kCopyBlock>(lead, R2, rows(Lay::g), rows(Lay::s), idKK, 0);
+        umma_commit(&bars[gN1]);
+        if (!mbar_wait(&bars[gDS], 0)) { tc_fail(5); break; }
+        umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kCopyBlock>(lead, R3, rows(Lay::v), rows(Lay::ds), idKK, 0);
+        umma_commit(&bars[gN2]);
+        if (!mbar_wait(&bars[gP], 0)) { tc_fail(6); break; }
+        tc_fence_after_sync();
+        umma_chain_ss<8, kStepK, kBlockK, kStepMN, kBlockMN>(lead, R0, rows(Lay::d), columns(Lay::k, kBox), idK, 0);
+        umma_commit(&bars[gO1]);
+        umma_chain_ss<8, kStepMN, kBlockMN, kStepMN, kBlockMN>(lead, R1, columns(Lay::d, kBox), columns(Lay::q, kBox), idTK, 0);
+        umma_commit(&bars[gO2]);
+        if (!mbar_wait(&bars[gE1], 0)) { tc_fail(7); break; }
+        tc_fence_after_sync();
+        umma_chain_ss<8, kStepMN, kBlockMN, kStepMN, kBlockMN>(lead, R0, columns(Lay::s, kBox), columns(Lay::g, kBox), idTD, 0);
+        umma_chain_ss<4 * KB, kStepK, kBlockK, kStepMN, kBlockMN>(lead, R2, rows(Lay::k), columns(Lay::ds, KP * 128), idD, 0);
+        umma_commit(&bars[gO3]);
+      } while (false);
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ decays: a lane takes four adjacent tokens
+    double sum[4], all = 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t t = t0 + lane * 4 + e;
+      if (t < a.T && !(mask && mask[t])) all += fmax(log_decay_at(a.decay.p, a.decay_dtype, b * a.decay.b + h * a.decay.h + t * a.decay.t) * kLog2eD, -64.0);
+      sum[e] = all;
+    }
+    double before = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += up;
+    }
+    before -= all;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) L[lane * 4 + e] = (float)(sum[e] + before);
+    mbar_arrive(&bars[gL]);
+  } else {
+    // ------------------------------------------------------------------ two groups of 128: rows of the chunk, every other 16 columns
+    const int group = (warp - 3) >> 2, quarter = warp & 3, row = quarter * 32 + lane, wtid = tid - 96;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const uint32_t R0 = tmem + lane_addr, R1 = R0 + 128, R2 = R0 + 256, R3 = R0 + 384;
+    const int64_t t = t0 + row;
+    const bool there = t < a.T;
+    const bool want = a.g_decay != nullptr;
+    float x = 0.f, rows_sum = 0.f, keys_sum = 0.f;      // S . dS; rows of M and q . (G S^T); k . (V dS^T)
+    do {
+      if (mask) {      // padded rows may hold anything: zero before a product reads them
+        if (!mbar_wait(&bars[gQK], 0) || !mbar_wait(&bars[gVG], 0)) { tc_fail(8); break; }
+        if (there && mask[t]) {
+          const uint4 zero = make_uint4(0, 0, 0, 0);
+          if (group == 0) {
+#pragma unroll 1
+            for (int ch = 0; ch < 8 * KB; ++ch) {
+              *reinterpret_cast<uint4*>(sm + Lay::q + row_chunk2(row, ch)) = zero;
+              *reinterpret_cast<uint4*>(sm + Lay::k + row_chunk2(row, ch)) = zero;
+            }
+          } else {
+#pragma unroll 1
+            for (int ch = 0; ch < 8 * DB; ++ch) {
+              *reinterpret_cast<uint4*>(sm + Lay::v + row_chunk2(row, ch)) = zero;
+              *reinterpret_cast<uint4*>(sm + Lay::g + row_chunk2(row, ch)) = zero;
+            }
+          }
+        }
+        fence_async_smem();
+        mbar_arrive(&bars[gClean]);
+      }
+      if (!mbar_wait(&bars[gS], 0) || !mbar_wait(&bars[gDS], 0)) { tc_fail(9); break; }
+      if (want) {
+#pragma unroll 1
+        for (uint32_t i = wtid * 16; i < Lay::kCopyBytes; i += 256 * 16) {
+          const uint4 u = *reinterpret_cast<const uint4*>(sm + Lay::s + i), w = *reinterpret_cast<const uint4*>(sm + Lay::ds + i);
+          const uint32_t us[4] = {u.x, u.y, u.z, u.w}, ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack2h<T>(us[e]), g = unpack2h<T>(ws[e]);
+            x = fmaf(f.x, g.x, fmaf(f.y, g.y, x));
+          }
+        }
+      }
+      mbar_release_stage(&bars[gX]);      // S has been read
+      if (!mbar_wait(&bars[gX], 0) || !mbar_wait(&bars[gL], 0)) { tc_fail(10); break; }
+      const float mine = L[row], end = L[127];
+      if (!mbar_wait(&bars[gT], 0) || !mbar_wait(&bars[gN1], 0)) { tc_fail(11); break; }
+      tc_fence_after_sync();
+      const int pieces = 2 * quarter + 2;      // of 16 columns, that reach up to the diagonal
+#pragma unroll 1
+      for (int p = group; p < 8; p += 2) {
+        uint32_t pw[8], dw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pw[i] = dw[i] = 0u;
+        float m[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m[i] = 0.f;
+        if (p < pieces) {
+          uint32_t s0[16], s1[16];
+          tmem_ld16(R0 + p * 16, s0);
+          tmem_ld16(R1 + p * 16, s1);
+          float w[16];
+          const int last = row - p * 16;
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const float4 l = *reinterpret_cast<const float4*>(L + p * 16 + i);
+            w[i] = ex2(mine - l.x); w[i + 1] = ex2(mine - l.y); w[i + 2] = ex2(mine - l.z); w[i + 3] = ex2(mine - l.w);
+          }
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float f0 = i <= last ? a.scale * w[i] : 0.f, f1 = i + 1 <= last ? a.scale * w[i + 1] : 0.f;
+            const float p0 = __uint_as_float(s0[i]) * f0, p1 = __uint_as_float(s0[i + 1]) * f1;
+            pw[i >> 1] = pack2h<T>(p0, p1);
+            dw[i >> 1] = pack2h<T>(__uint_as_float(s1[i]) * f0, __uint_as_float(s1[i + 1]) * f1);
+            m[i] = p0 * __uint_as_float(s1[i]);
+            m[i + 1] = p1 * __uint_as_float(s1[i + 1]);
+          }
+        }
+        *reinterpret_cast<uint4*>(sm + Lay::s + row_chunk2(row, 2 * p)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
+        *reinterpret_cast<uint4*>(sm + Lay::s + row_chunk2(row, 2 * p + 1)) = make_uint4(pw[4], pw[5], pw[6], pw[7]);
+        *reinterpret_cast<uint4*>(sm + Lay::d + row_chunk2(row, 2 * p)) = make_uint4(dw[0], dw[1], dw[2], dw[3]);
+        *reinterpret_cast<uint4*>(sm + Lay::d + row_chunk2(row, 2 * p + 1)) = make_uint4(dw[4], dw[5], dw[6], dw[7]);
+        if (want) {      // sums of the warp's rows: each step halves the columns that a lane has
+#pragma unroll
+          for (int i = 0; i < 16; ++i) rows_sum += m[i];
+#pragma unroll
+          for (int o = 16, n = 8; o >= 2; o >>= 1, n >>= 1) {
+            const bool up = lane & o;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i < n) {
+                const float give = up ? m[i] : m[i + n];
+                m[i] = (up ? m[i + n] : m[i]) + __shfl_xor_sync(0xffffffffu, give, o);
+              }
+          }
+          m[0] += __shfl_xor_sync(0xffffffffu, m[0], 1);
+          if (!(lane & 1)) cols[quarter * 128 + p * 16 + (lane >> 1)] = m[0];
+        }
+      }
+      fence_async_smem();
+      tc_fence_before_sync();
+      mbar_arrive(&bars[gP]);
+
+      const auto sectors = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; };
+      const bool wide_q = a.K % 16 == 0 && sectors(a.gq), wide_k = a.K % 16 == 0 && sectors(a.gk), wide_d = a.D % 16 == 0 && sectors(a.gv);
+      const float fq = a.scale * ex2(mine), fk = ex2(end - mine);
+      const int64_t at = (t * a.B + b) * a.H + h;
+      // ---- gq, gk
+      const auto grad = [&](uint32_t main, uint32_t side, float f, void* out, uint32_t tile, float& sum, bool wide) {
+        T* o = static_cast<T*>(out) + at * a.K;
+#pragma unroll 1
+        for (int c0 = group * 16; c0 < KP; c0 += 32) {
+          uint32_t u[16], n[16];
+          tmem_ld16(main + c0, u);
+          tmem_ld16(side + c0, n);
+          tmem_ld_wait();
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float s = f * __uint_as_float(n[i]);
+            v[i] = __uint_as_float(u[i]) + s;
+            n[i] = __float_as_uint(s);
+          }
+          if (there && c0 < a.K) store_row16(o + c0, v, a.K - c0, wide);
+          if (want) {
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+              const uint4 y = *reinterpret_cast<const uint4*>(sm + tile + row_chunk2(row, (c0 >> 3) + ch));
+              const uint32_t ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 z = unpack2h<T>(ys[e]);
+                sum = fmaf(__uint_as_float(n[8 * ch + 2 * e]), z.x, fmaf(__uint_as_float(n[8 * ch + 2 * e + 1]), z.y, sum));
+              }
+            }
+          }
+        }
+      };
+      if (!mbar_wait(&bars[gO1], 0)) { tc_fail(12); break; }
+      tc_fence_after_sync();
+      grad(R0, R2, fq, a.gq, Lay::q, rows_sum, wide_q);
+      tc_fence_before_sync();
+      mbar_arrive(&bars[gE1]);
+      if (!mbar_wait(&bars[gN2], 0) || !mbar_wait(&bars[gO2], 0)) { tc_fail(13); break; }
+      tc_fence_after_sync();
+      grad(R1, R3, fk, a.gk, Lay::k, keys_sum, wide_k);
+      // ---- gv
+      if (!mbar_wait(&bars[gO3], 0)) { tc_fail(14); break; }
+      tc_fence_after_sync();
+      T* o = static_cast<T*>(a.gv) + at * a.D;
+#pragma unroll 1
+      for (int c0 = group * 16; c0 < DP; c0 += 32) {
+        uint32_t u[16], n[16];
+        tmem_ld16(R0 + c0, u);
+        tmem_ld16(R2 + c0, n);
+        tmem_ld_wait();
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = fmaf(fk, __uint_as_float(n[i]), __uint_as_float(u[i]));
+        if (there && c0 < a.D) store_row16(o + c0, v, a.D - c0, wide_d);
+      }
+      // ---- the decays: everything that was read of the tiles has been (gO3), so that P's place serves the exchange
+      if (want) {
+        float* ex = reinterpret_cast<float*>(sm + Lay::s);      // [2][128] rows and keys of the second group, then a sum of S . dS for each warp
+        x = warp_sum(x);
+        if (lane == 0) ex[512 + (warp - 3)] = x;
+        if (group == 1) { ex[row] = rows_sum; ex[128 + row] = keys_sum; }
+        mbar_arrive(&bars[gAll]);
+        if (!mbar_wait(&bars[gAll], 0)) { tc_fail(15); break; }
+        // suffix sums of rows less columns, prefix sums of keys, by the first group: within a warp, then across
+        if (group == 0) {
+          float down = rows_sum + ex[row] - (cols[row] + cols[128 + row] + cols[256 + row] + cols[384 + row]), up = keys_sum + ex[128 + row];
+          const float own_up = up;
+#pragma unroll
+          for (int o2 = 1; o2 < 32; o2 <<= 1) {
+            const float d = __shfl_down_sync(0xffffffffu, down, o2), u = __shfl_up_sync(0xffffffffu, up, o2);
+            if (lane + o2 < 32) down += d;
+            if (lane >= o2) up += u;
+          }
+          if (lane == 0) ex[528 + quarter] = down;
+          if (lane == 31) ex[532 + quarter] = up;
+          uint32_t phase = 0;
+          if (!epi_sync(&bars[gSum], phase)) { tc_fail(16); break; }
+          float g = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g += ex[512 + i];
+          g = ex2(end) * g + down + up - own_up;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (i > quarter) g += ex[528 + i];
+            if (i < quarter) g += ex[532 + i];
+          }
+          const bool real = there && !(mask && mask[t]);
+          if (!real) g = 0.f;
+          if (!a.per_head) {
+            if (there) {
+              if (a.decay_dtype == RFA_F32) static_cast<float*>(a.g_decay)[at] = g;
+              else if (a.decay_dtype == RFA_F16) static_cast<__half*>(a.g_decay)[at] = __float2half_rn(g);
+              else static_cast<__nv_bfloat16*>(a.g_decay)[at] = __float2bfloat16_rn(g);
+            }
+          } else {
+            g = warp_sum(g);
+            if (lane == 0) ex[536 + quarter] = g;
+            if (!epi_sync(&bars[gSum], phase)) { tc_fail(17); break; }
+            if (row == 0) static_cast<float*>(a.g_decay)[(b * chunks + chunk) * a.H + h] = ex[536] + ex[537] + ex[538] + ex[539];
+          }
+        }
+      }
+    } while (false);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+namespace {
+
+template <typename T, int KB, int DB>
+int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DecayGradArgs& a, cudaStream_t stream) {
+  constexpr uint32_t smem = GradLayout<KB, DB>::bytes;
+  cudaError_t e = cudaFuncSetAttribute(decay_grad_tc_kernel<T, KB, DB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return fail((int)e, "decay_bwd: cannot reserve %u bytes of shared memory: %s", smem, cudaGetErrorString(e));
+  const int64_t ctas = (int64_t)a.B * a.H * ((a.T + kTC - 1) / kTC);
+  RFA_REQUIRE(ctas < (int64_t)1 << 31, RFA_EUNSUPPORTED, "decay_bwd: %lld chunks", (long long)ctas);
+  e = launch_pdl(decay_grad_tc_kernel<T, KB, DB>, dim3((unsigned)ctas), dim3(kDgThreads), smem, stream, q, k, v, g, a);
+  if (e != cudaSuccess) return fail((int)e, "rfa_decay_bwd: launch failed: %s", cudaGetErrorString(e));
+  return check_launch("rfa_decay_bwd");
+}
+
+}  // namespace
+
+int launch_decay_grad_tc(const rfa_decay_t& c, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const void* states, const void* grads,
+                         void* gq, void* gk, void* gv, void* g_decay, cudaStream_t stream) {
+  DecayGradArgs a{};
+  a.decay = {c.log_decay, c.g_t, c.g_b, c.g_h};
+  a.mask = c.mask;
+  a.states = states; a.grads = grads;
+  a.gq = gq; a.gk = gk; a.gv = gv; a.g_decay = g_decay;
+  a.T = c.T; a.B = c.B; a.H = c.H; a.K = c.K; a.D = c.D; a.decay_dtype = c.decay_dtype; a.per_head = c.per_head != 0;
+  a.scale = c.scale;
+  switch ((c.dtype == RFA_BF16 ? 4 : 0) + (c.K > 64 ? 2 : 0) + (c.D > 64 ? 1 : 0)) {
+    case 0: return launch<__half, 1, 1>(q, k, v, g, a, stream);
+    case 1: return launch<__half, 1, 2>(q, k, v, g, a, stream);
+    case 2: return launch<__half, 2, 1>(q, k, v, g, a, stream);
+    case 3: return launch<__half, 2, 2>(q, k, v, g, a, stream);
+    case 4: return launch<__nv_bfloat16, 1, 1>(q, k, v, g, a, stream);
+    case 5: return launch<__nv_bfloat16, 1, 2>(q, k, v, g, a, stream);
+    case 6: return launch<__nv_bfloat16, 2, 1>(q, k, v, g, a, stream);
+    default: return launch<__nv_bfloat16, 2, 2>(q, k, v, g, a, stream);
+  }
+}
+
+RFA_TC_UNIT(decay_bwd)
+
+}  // namespace rfa

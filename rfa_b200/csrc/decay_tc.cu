@@ -55,30 +55,80 @@ SweepPlan decay_tc_plan(int64_t T, int64_t BH, int K, int D) {
   return p;
 }
 
+namespace {
+
+// the sweep over segments where there are several: their own states, the states in front of each, then the sweep itself
+template <bool OUT>
+int sweep(bool bf16, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const DecayTcArgs& a, bool exact, cudaStream_t stream) {
+  if (a.nseg > 1) {
+    DecayTcArgs own = a;
+    own.kept = nullptr;
+    if (int r = exact ? launch_sizes<false, true>(bf16, q, k, v, own, true, stream) : launch_sizes<false, false>(bf16, q, k, v, own, true, stream)) return r;
+    if (int r = launch_decay_combine(a.totals, a.seg_decay, a.s_in, a.nseg, (int64_t)a.B * a.H, a.K, a.D, stream)) return r;
+  }
+  return exact ? launch_sizes<OUT, true>(bf16, q, k, v, a, false, stream) : launch_sizes<OUT, false>(bf16, q, k, v, a, false, stream);
+}
+DecayTcArgs sweep_args(const rfa_decay_t& c, const SweepPlan& plan, char* workspace) {
+  DecayTcArgs a{};
+  a.decay = {c.log_decay, c.g_t, c.g_b, c.g_h};
+  a.mask = c.mask;
+  a.totals = reinterpret_cast<float*>(workspace);
+  a.seg_decay = reinterpret_cast<double*>(workspace + ((plan.totals + 255) & ~(size_t)255));
+  a.T = c.T; a.tseg = plan.tseg;
+  a.B = c.B; a.H = c.H; a.K = c.K; a.D = c.D; a.nseg = plan.nseg; a.decay_dtype = c.decay_dtype;
+  return a;
+}
+size_t kept_bytes(int64_t T, int64_t BH, int K, int D) { return (size_t)((T + kTC - 1) / kTC) * BH * (K > 64 ? 2 : 1) * (D > 64 ? 2 : 1) * 64 * 128; }
+
+}  // namespace
+
+size_t decay_tc_bwd_bytes(const rfa_decay_t& c) {
+  const int64_t BH = (int64_t)c.B * c.H;
+  const SweepPlan plan = decay_tc_plan(c.T, BH, c.K, c.D);
+  return ((plan.totals + 255) & ~(size_t)255) + ((plan.seg_decay + 255) & ~(size_t)255) + 2 * kept_bytes(c.T, BH, c.K, c.D) + sizeof(float) * BH * ((c.T + kTC - 1) / kTC);
+}
+
+int launch_decay_tc_bwd(const rfa_decay_t& c, char* workspace, const void* g, const float* g_s, void* gq, void* gk, void* gv, void* g_decay, float* gs_in, cudaStream_t stream) {
+  const bool bf16 = c.dtype == RFA_BF16;
+  const int64_t BH = (int64_t)c.B * c.H, row = (int64_t)c.H * c.D, chunks = (c.T + kTC - 1) / kTC;
+  CUtensorMap q, k, v, gm;
+  if (make_tmap_heads(&q, c.q, bf16, c.T, c.B, c.H, c.K, c.q_t, c.q_b, c.q_h, kTC) || make_tmap_heads(&k, c.k, bf16, c.T, c.B, c.H, c.K, c.k_t, c.k_b, c.k_h, kTC) ||
+      make_tmap_heads(&v, c.v, bf16, c.T, c.B, c.H, c.D, c.v_t, c.v_b, c.v_h, kTC) || make_tmap_heads(&gm, g, bf16, c.T, c.B, c.H, c.D, c.B * row, row, c.D, kTC))
+    return fail(RFA_EDEVICE, "decay_bwd: cuTensorMapEncodeTiled failed or is unavailable");
+  const SweepPlan plan = decay_tc_plan(c.T, BH, c.K, c.D);
+  char* states = workspace + ((plan.totals + 255) & ~(size_t)255) + ((plan.seg_decay + 255) & ~(size_t)255);
+  char* grads = states + kept_bytes(c.T, BH, c.K, c.D);
+  float* sums = reinterpret_cast<float*>(grads + kept_bytes(c.T, BH, c.K, c.D));
+  DecayTcArgs a = sweep_args(c, plan, workspace);
+  a.in_scale = 1.f;
+  a.s_in = {const_cast<float*>(c.s_in), c.D, 1};
+  a.kept = states;
+  if (int r = sweep<false>(bf16, q, k, v, a, false, stream)) return r;
+  a.in_scale = c.scale;
+  a.rev = 1;
+  a.s_in = {const_cast<float*>(g_s), c.D, 1};
+  a.s_out = {gs_in, c.D, 1};
+  a.kept = grads;
+  if (int r = sweep<false>(bf16, q, q, gm, a, gs_in != nullptr, stream)) return r;
+  if (int r = launch_decay_grad_tc(c, q, k, v, gm, states, grads, gq, gk, gv, g_decay && c.per_head ? sums : g_decay, stream)) return r;
+  if (!g_decay || !c.per_head) return 0;
+  const SumJob job{sums, g_decay, c.H, (int)(c.B * chunks), c.decay_dtype};
+  return sum_parts(&job, 1, stream);
+}
+
 int launch_decay_tc(const rfa_decay_t& c, const SweepPlan& plan, char* workspace, void* out, float* s_out, cudaStream_t stream) {
   const bool bf16 = c.dtype == RFA_BF16;
   CUtensorMap q, k, v;
   if (make_tmap_heads(&q, c.q, bf16, c.T, c.B, c.H, c.K, c.q_t, c.q_b, c.q_h, kTC) || make_tmap_heads(&k, c.k, bf16, c.T, c.B, c.H, c.K, c.k_t, c.k_b, c.k_h, kTC) ||
       make_tmap_heads(&v, c.v, bf16, c.T, c.B, c.H, c.D, c.v_t, c.v_b, c.v_h, kTC))
     return fail(RFA_EDEVICE, "decay: cuTensorMapEncodeTiled failed or is unavailable");
-  DecayTcArgs a{};
-  a.decay = {c.log_decay, c.g_t, c.g_b, c.g_h};
-  a.mask = c.mask;
+  DecayTcArgs a = sweep_args(c, plan, workspace);
   a.out = out;
   a.s_in = {const_cast<float*>(c.s_in), c.D, 1};
   a.s_out = {s_out, c.D, 1};
-  a.totals = reinterpret_cast<float*>(workspace);
-  a.seg_decay = reinterpret_cast<double*>(workspace + ((plan.totals + 255) & ~(size_t)255));
-  a.T = c.T; a.tseg = plan.tseg;
-  a.B = c.B; a.H = c.H; a.K = c.K; a.D = c.D; a.nseg = plan.nseg; a.decay_dtype = c.decay_dtype;
-  const bool exact = s_out != nullptr;
   a.in_scale = 1.f;
   a.out_scale = c.scale;
-  if (plan.nseg > 1) {
-    if (int r = exact ? launch_sizes<false, true>(bf16, q, k, v, a, true, stream) : launch_sizes<false, false>(bf16, q, k, v, a, true, stream)) return r;
-    if (int r = launch_decay_combine(a.totals, a.seg_decay, a.s_in, plan.nseg, (int64_t)c.B * c.H, c.K, c.D, stream)) return r;
-  }
-  return exact ? launch_sizes<true, true>(bf16, q, k, v, a, false, stream) : launch_sizes<true, false>(bf16, q, k, v, a, false, stream);
+  return sweep<true>(bf16, q, k, v, a, s_out != nullptr, stream);
 }
 
 RFA_TC_UNIT(decay)

@@ -490,4 +490,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   if (warp == 1) tmem_dealloc(tmem, Lay::cols);
 }
 
+// decay_bwd_tc.cu
+int launch_decay_grad_tc(const rfa_decay_t& c, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const void* states, const void* grads,
+                         void* gq, void* gk, void* gv, void* g_decay, cudaStream_t stream);
+
 }  // namespace rfa
