@@ -40,6 +40,8 @@ int number(WindowArgs& a, const rfa_window_t& c, const int64_t* length, int cap,
   return launch_window_order(c.mask, length, cap, order, pos, c.T, c.B, stream);
 }
 
+int forward(const WindowArgs& a, cudaStream_t stream) { return window_tc_ok(a) ? launch_window_fwd_tc(a, stream) : launch_window_fwd_tiles(a, stream); }
+
 }  // namespace
 }  // namespace rfa
 
@@ -61,7 +63,7 @@ extern "C" int rfa_window_fwd(const rfa_window_t* c, void* out, float* lse, void
   a.lse = lse;
   if (c->mask)
     if (int r = number(a, *c, nullptr, 0, workspace, as_stream(stream))) return r;
-  return launch_window_fwd_tiles(a, as_stream(stream));
+  return forward(a, as_stream(stream));
 }
 
 extern "C" int rfa_window_bwd(const rfa_window_t* c, const void* out, const float* lse, const void* g, void* gq, void* gk, void* gv, void* workspace, size_t workspace_bytes,
@@ -116,6 +118,6 @@ extern "C" int rfa_window_append(const rfa_window_t* c, void* cache_k, void* cac
     a.k = {keys, c->B * row, row, c->D};
     a.v = {values, c->B * row, row, c->D};
   }
-  if (int r = launch_window_fwd_tiles(a, st)) return r;
+  if (int r = forward(a, st)) return r;
   return launch_window_keep(*c, cache_k, cache_v, length, a.order, empty != 0, st);
 }
