@@ -1,50 +1,75 @@
 // Sliding-window attention on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), fp16 and bf16, heads of up to 128: the forward pass.
 //
-// A CTA takes two units of 128 queries of one batch row that read the same keys -- two heads that share a key head, or else two runs of one head -- and goes
-// through the 128-key tiles that either of them sees: those of the first tokens, then from the window's start on.  Per unit and tile
+// A CTA takes one pair of units after the other, each unit 128 queries of one batch row, that read the same keys -- two heads that share a key head, or else two
+// runs of one head -- and goes through the 128-key tiles that either of them sees: those of the first tokens, then from the window's start on.  Per unit and tile
 //     S = Q K^T (fp32, TMEM)  ->  P = 2^(S scale log2(e) - m), 16 bits, over S  ->  O += P V
-// with a thread to each row: a pass for the row's maximum, one for P and the sum.  m moves only when it is exceeded by more than 8 (P is then at most 256, which both
-// types hold), and only then O is rescaled, by the row's own thread.  Tiles that every query of the unit sees whole need no mask; in the others scores that are not
-// seen are -inf before anything is made of them.  Bound by the exponentials (16 a cycle and SM: 1024 cycles a tile) and the instructions around them.
+// with a thread to each row, whose scores it holds in registers: the row's maximum, then P and the sum.  m moves only when it is exceeded by more than 8 (P is then
+// at most 256, which both types hold), and only then O is rescaled, by the row's own thread.  Tiles that every query of the unit sees whole need no mask; in the
+// others scores that are not seen are -inf before anything is made of them.  Bound by the exponentials (16 a cycle and SM: 1024 cycles a tile) and the instructions
+// around them.
 //
-// With padded tokens or a cache in front (ORDERED) places are not numbers: warps 12..15 fetch the numbers of a tile's keys and clear the values of places that
-// hold no token, whatever stands there.
+// With padded tokens or a cache in front (ORDERED) places are not numbers: warp 3 fetches the numbers of a tile's keys and clears the values of places that hold
+// no token, whatever stands there.
 //
-// Warp roles (384 threads; 512 ORDERED): warp 0 TMA producer, warps 1 and 2 one MMA issuer for each unit, warps 4..7 and 8..11 one softmax group for each unit.  All
-// waits are bounded.
+// Warp roles (384 threads): warp 0 TMA producer, warps 1 and 2 one MMA issuer for each unit, warps 4..7 and 8..11 one softmax group for each unit.  All waits are
+// bounded.
 #define RFA_TC_FAMILY 12
+#include <algorithm>
+
 #include "window_tc.cuh"
 
 namespace rfa {
 
-template <int DB, bool ORDERED>
+constexpr int kWinThreads = 384;
+
+template <int DB>
 struct WinLayout {
-  static constexpr int kStages = DB == 1 ? 4 : 2, kThreads = ORDERED ? 512 : 384;
-  static constexpr uint32_t q = 0, k = 2 * DB * kBox, v = k + kStages * DB * kBox, num = v + kStages * DB * kBox, bar = num + (ORDERED ? kStages * 128 * 4 : 0), bytes = bar + 256;
+  static constexpr int kStages = DB == 1 ? 4 : 2;
+  static constexpr uint32_t q = 0, k = 2 * DB * kBox, v = k + kStages * DB * kBox, num = v + kStages * DB * kBox, bar = num + kStages * 128 * 4, bytes = bar + 256;
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
-enum { wQ = 0, wFullK = 2, wFullV = 6, wEmpty = 10, wNum_ = 14, wS = 18, wP = 20, wO = 22, wCount = 24 };
+enum { wQ = 0, wQEmpty = 2, wFullK = 4, wFullV = 8, wEmpty = 12, wNumbers = 16, wS = 20, wP = 22, wO = 24, wCount = 26 };
+
+// the lowest n bits
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 template <typename T, int DB, bool ORDERED>
-__global__ void __launch_bounds__(WinLayout<DB, ORDERED>::kThreads, 1)
+__global__ void __launch_bounds__(kWinThreads, 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                 const __grid_constant__ WindowArgs a, bool pair_heads) {
-  using Lay = WinLayout<DB, ORDERED>;
+                 const __grid_constant__ WindowArgs a, bool pair_heads, int works) {
+  using Lay = WinLayout<DB>;
   constexpr int DP = DB * 64, kStages = Lay::kStages;
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::bar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + wCount);
   const uint32_t sbase = smem_u32(sm);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // the units: runs of 128 queries from row0 on
-  const int64_t runs = (a.T + 127) / 128, per_head = pair_heads ? runs : (runs + 1) / 2, heads = pair_heads ? a.H / 2 : a.H;
-  const int64_t bh = blockIdx.x / per_head, run = blockIdx.x % per_head;
-  const int b = (int)(bh / heads), h0 = (int)(bh % heads) * (pair_heads ? 2 : 1), kv = h0 / (a.H / a.G);
-  const auto unit_head = [&](int u) { return pair_heads ? h0 + u : h0; };
-  const auto unit_row = [&](int u) { return (pair_heads ? run : 2 * run + u) * 128; };
   const int64_t at = a.S - a.T;
+  const int runs = (int)((a.T + 127) / 128), per_head = pair_heads ? runs : (runs + 1) / 2, heads = pair_heads ? a.H / 2 : a.H;
+  // a work: two units of 128 queries from row[u] on, of heads h0 and h0 + 1 or of one
+  struct Work {
+    int b, h0, kv;
+    int64_t row[2];
+    WindowSpan span[2], both;
+  };
+  const auto work_of = [&](int w, Work& k) {
+    const int bh = w / per_head, run = w % per_head;
+    k.b = bh / heads;
+    k.h0 = bh % heads * (pair_heads ? 2 : 1);
+    k.kv = k.h0 / (a.H / a.G);
+    k.row[0] = (int64_t)(pair_heads ? run : 2 * run) * 128;
+    k.row[1] = pair_heads ? k.row[0] : k.row[0] + 128;
+    const WindowNumbers num(a, k.b);
+    k.span[0] = window_span(num, at, k.row[0], a.T);
+    k.span[1] = pair_heads ? k.span[0] : window_span(num, at, k.row[1], a.T);
+    k.both = k.span[0];
+    if (k.span[1].end > 0) {      // a last run may be without a partner
+      k.both.first = min(k.span[0].first, k.span[1].first);
+      k.both.end = max(k.span[0].end, k.span[1].end);
+    }
+  };
   if (tid == 0) {
-    for (int i = 0; i < wCount; ++i) mbar_init(&bars[i], i >= wP && i < wO ? 128 : i >= wNum_ && i < wS ? 128 : i >= wEmpty && i < wNum_ ? (ORDERED ? 2 + 256 : 2) : 1);
+    for (int i = 0; i < wCount; ++i) mbar_init(&bars[i], i >= wP && i < wO ? 128 : i >= wNumbers && i < wS ? 32 : i >= wEmpty && i < wNumbers ? (ORDERED ? 2 + 256 : 2) : 1);
     mbar_fence_init();
     tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
   }
@@ -56,29 +81,28 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   pdl_wait();
   pdl_launch_dependents();
 
-  const WindowNumbers num(a, b);
-  const WindowSpan span0 = window_span(num, at, unit_row(0), a.T), span1 = window_span(num, at, unit_row(1), a.T);
-  WindowSpan both = span0;
-  if (span1.end > 0) {      // a last run may be without a partner
-    both.first = min(span0.first, span1.first);
-    both.end = max(span0.end, span1.end);
-  }
-
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      for (int u = 0; u < 2; ++u) {
-        mbar_arrive_expect_tx(&bars[wQ + u], DB * kBox);
-        for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::q + (u * DB + x) * kBox, &tm_q, &bars[wQ + u], x * 64, unit_head(u), b, (int)unit_row(u));
-      }
-      int n = 0;
-      for (int64_t kt = both.begin(); kt < both.end; kt = both.next(kt), ++n) {
-        const int st = n % kStages;
-        if (n >= kStages && !mbar_wait(&bars[wEmpty + st], (n / kStages + 1) & 1)) { tc_fail(1); break; }
-        mbar_arrive_expect_tx(&bars[wFullK + st], DB * kBox);
-        for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::k + (st * DB + x) * kBox, &tm_k, &bars[wFullK + st], x * 64, kv, b, (int)(kt * 128));
-        mbar_arrive_expect_tx(&bars[wFullV + st], DB * kBox);
-        for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + (st * DB + x) * kBox, &tm_v, &bars[wFullV + st], x * 64, kv, b, (int)(kt * 128));
+      int n = 0, done = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; ok && w < works; w += gridDim.x, ++done) {
+        Work k;
+        work_of(w, k);
+        for (int u = 0; u < 2; ++u) {
+          if (done > 0 && !mbar_wait(&bars[wQEmpty + u], (done + 1) & 1)) { tc_fail(1); ok = false; break; }
+          mbar_arrive_expect_tx(&bars[wQ + u], DB * kBox);
+          for (int x = 0; x < DB; ++x)
+            tma_load_4d(sm + Lay::q + (u * DB + x) * kBox, &tm_q, &bars[wQ + u], x * 64, k.h0 + (pair_heads ? u : 0), k.b, (int)k.row[u]);
+        }
+        for (int64_t kt = k.both.begin(); ok && kt < k.both.end; kt = k.both.next(kt), ++n) {
+          const int st = n % kStages;
+          if (n >= kStages && !mbar_wait(&bars[wEmpty + st], (n / kStages + 1) & 1)) { tc_fail(2); ok = false; break; }
+          mbar_arrive_expect_tx(&bars[wFullK + st], DB * kBox);
+          for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::k + (st * DB + x) * kBox, &tm_k, &bars[wFullK + st], x * 64, k.kv, k.b, (int)(kt * 128));
+          mbar_arrive_expect_tx(&bars[wFullV + st], DB * kBox);
+          for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + (st * DB + x) * kBox, &tm_v, &bars[wFullV + st], x * 64, k.kv, k.b, (int)(kt * 128));
+        }
       }
     }
   } else if (warp == 1 || warp == 2) {
@@ -86,171 +110,192 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     if (lane == 0) {
       constexpr uint32_t lead = 1u;
       const int u = warp - 1;
-      const WindowSpan own = u ? span1 : span0;
       constexpr uint32_t idS = umma_idesc<T>(128, 128, false, false), idO = umma_idesc<T>(128, DP, false, true);
       const uint64_t dQ = umma_smem_desc(sbase + Lay::q + u * DB * kBox, 0, 1024, kSwizzle128B), dK = umma_smem_desc(sbase + Lay::k, 0, 1024, kSwizzle128B);
       const uint64_t dV = umma_smem_desc(sbase + Lay::v, kBox, 1024, kSwizzle128B);
       constexpr uint64_t kStep = (DB * kBox) >> 4;
       const uint32_t S = tmem + u * 128, O = tmem + 256 + u * DP;
-      if (!mbar_wait(&bars[wQ + u], 0)) tc_fail(2);
-      int n = 0, it = 0;
-      for (int64_t kt = both.begin(); kt < both.end; kt = both.next(kt), ++n) {
-        const int st = n % kStages;
-        const uint32_t filled = (n / kStages) & 1;
-        if (!mbar_wait(&bars[wFullK + st], filled)) { tc_fail(3); break; }
-        if (!own.has(kt)) {
-          if (!mbar_wait(&bars[wFullV + st], filled)) { tc_fail(4); break; }
-          mbar_arrive(&bars[wEmpty + st]);
-          continue;
+      int n = 0, it = 0, done = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; ok && w < works; w += gridDim.x, ++done) {
+        Work k;
+        work_of(w, k);
+        const WindowSpan own = u ? k.span[1] : k.span[0];
+        if (!mbar_wait(&bars[wQ + u], done & 1)) { tc_fail(3); break; }
+        bool first = true;
+        for (int64_t kt = k.both.begin(); kt < k.both.end; kt = k.both.next(kt), ++n) {
+          const int st = n % kStages;
+          const uint32_t filled = (n / kStages) & 1;
+          if (!mbar_wait(&bars[wFullK + st], filled)) { tc_fail(4); ok = false; break; }
+          if (!own.has(kt)) {
+            if (!mbar_wait(&bars[wFullV + st], filled)) { tc_fail(5); ok = false; break; }
+            mbar_arrive(&bars[wEmpty + st]);
+            continue;
+          }
+          tc_fence_after_sync();
+          umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockK>(lead, S, dQ, dK + st * kStep, idS, 0);
+          umma_commit(&bars[wS + u]);
+          if (!mbar_wait(&bars[ORDERED ? wNumbers + st : wFullV + st], filled)) { tc_fail(6); ok = false; break; }
+          if (!mbar_wait(&bars[wP + u], it & 1)) { tc_fail(7); ok = false; break; }
+          tc_fence_after_sync();
+          umma_chain_ts<8, kStepMN, kBlockMN>(lead, O, S, dV + st * kStep, idO, first ? 0u : 1u);
+          umma_commit(&bars[wO + u]);
+          umma_commit(&bars[wEmpty + st]);
+          first = false;
+          ++it;
         }
-        tc_fence_after_sync();
-        umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockK>(lead, S, dQ, dK + st * kStep, idS, 0);
-        umma_commit(&bars[wS + u]);
-        if (!mbar_wait(&bars[ORDERED ? wNum_ + st : wFullV + st], filled)) { tc_fail(5); break; }
-        if (!mbar_wait(&bars[wP + u], it & 1)) { tc_fail(6); break; }
-        tc_fence_after_sync();
-        umma_chain_ts<8, kStepMN, kBlockMN>(lead, O, S, dV + st * kStep, idO, it > 0);
-        umma_commit(&bars[wO + u]);
-        umma_commit(&bars[wEmpty + st]);
-        ++it;
+        if (ok) umma_commit(&bars[wQEmpty + u]);      // everything that reads Q is complete
       }
     }
-  } else if (warp >= 4 && warp < 12) {
+  } else if (warp >= 4) {
     // ------------------------------------------------------------------ softmax groups: a thread to each row
-    const int u = (warp - 4) >> 2;
-    const WindowSpan own = u ? span1 : span0;
-    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const int u = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t S = tmem + u * 128 + ((uint32_t)(quarter * 32) << 16), O = tmem + 256 + u * DP + ((uint32_t)(quarter * 32) << 16);
-    const int64_t i0 = unit_row(u), i = i0 + row, place = at + i;
-    const int mine = i < a.T ? num.at(place) : -1;
     const float scale = a.scale * kLog2e;
-    float top = -1e30f, sum = 0.f;      // the reference that weights are taken against, in units of log 2
+    const bool wide = a.D % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
     int n = 0, it = 0;
     bool ok = true;
-    for (int64_t kt = both.begin(); ok && kt < both.end; kt = both.next(kt), ++n) {
-      if (!own.has(kt)) {
-        if (ORDERED) {
-          if (!mbar_wait(&bars[wNum_ + n % kStages], (n / kStages) & 1)) { tc_fail(12); break; }
-          mbar_arrive(&bars[wEmpty + n % kStages]);
-        }
-        continue;
-      }
-      const int64_t j0 = kt * 128;
-      const int* nums = reinterpret_cast<const int*>(sm + Lay::num) + (n % kStages) * 128;
-      // every query of the unit sees every key of the tile
-      const bool whole = !ORDERED && j0 + 127 <= at + i0 && at + i0 + 127 - j0 < a.window && i0 + 128 <= a.T;
-      const int hi = (int)min((int64_t)128, place - j0), lo = (int)max((int64_t)-1, place - j0 - a.window + 1), first = (int)min((int64_t)128, a.sinks - j0);
-      if (ORDERED && !mbar_wait(&bars[wNum_ + n % kStages], (n / kStages) & 1)) { tc_fail(7); ok = false; break; }
-      if (!mbar_wait(&bars[wS + u], it & 1)) { tc_fail(8); ok = false; break; }
-      tc_fence_after_sync();
-      const auto seen = [&](int c) {
-        if constexpr (ORDERED) return window_sees(mine, nums[c], a.window, a.sinks);
-        else return c <= hi && (c >= lo || c < first);
-      };
-      // the row's maximum
-      float now = -INFINITY;
-      uint32_t next[16], s[16];
-      tmem_ld16(S, next);
+    for (int w = blockIdx.x; ok && w < works; w += gridDim.x) {
+      Work k;
+      work_of(w, k);
+      const WindowSpan own = u ? k.span[1] : k.span[0];
+      const int64_t i0 = u ? k.row[1] : k.row[0], i = i0 + row, place = at + i;
+      const int mine = i < a.T ? WindowNumbers(a, k.b).at(place) : -1;
+      float top = -1e30f, sum = 0.f;      // the reference that weights are taken against, in units of log 2
+      bool first = true;
 #pragma unroll 1
-      for (int p = 0; p < 8; ++p) {
-        tmem_ld_wait();
+      for (int64_t kt = k.both.begin(); kt < k.both.end; kt = k.both.next(kt), ++n) {
+        if (ORDERED && !mbar_wait(&bars[wNumbers + n % kStages], (n / kStages) & 1)) { tc_fail(8); ok = false; break; }
+        if (!own.has(kt)) {
+          if (ORDERED) mbar_arrive(&bars[wEmpty + n % kStages]);
+          continue;
+        }
+        const int64_t j0 = kt * 128;
+        // every query of the unit sees every key of the tile; or else which keys this row sees
+        const bool whole = !ORDERED && j0 + 127 <= at + i0 && at + i0 + 127 - j0 < a.window;
+        uint32_t seen[4];
+        if constexpr (ORDERED) {
+          const int* nums = reinterpret_cast<const int*>(sm + Lay::num) + (n % kStages) * 128;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) s[c] = next[c];
-        tmem_ld16(S + (p < 7 ? p * 16 + 16 : 0), next);      // at the end the first ones again, for the second pass
+          for (int x = 0; x < 4; ++x) {
+            uint32_t bits = 0;
+#pragma unroll 1
+            for (int c = 28; c >= 0; c -= 4) {
+              const int4 m = *reinterpret_cast<const int4*>(nums + x * 32 + c);
+              bits = bits << 4 | (window_sees(mine, m.x, a.window, a.sinks) ? 1u : 0u) | (window_sees(mine, m.y, a.window, a.sinks) ? 2u : 0u) |
+                     (window_sees(mine, m.z, a.window, a.sinks) ? 4u : 0u) | (window_sees(mine, m.w, a.window, a.sinks) ? 8u : 0u);
+            }
+            seen[x] = bits;
+          }
+        } else if (!whole) {
+          const int hi = (int)min((int64_t)128, place - j0 + 1), lo = (int)max((int64_t)0, place - j0 - a.window + 1), front = (int)min((int64_t)128, a.sinks - j0);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) seen[x] = low_bits(hi - 32 * x) & (~low_bits(lo - 32 * x) | low_bits(front - 32 * x));
+        }
+        if (!mbar_wait(&bars[wS + u], it & 1)) { tc_fail(9); ok = false; break; }
+        tc_fence_after_sync();
+        uint32_t s[128];
+        tmem_ld32(S, s);
+        tmem_ld32(S + 32, s + 32);
+        tmem_ld32(S + 64, s + 64);
+        tmem_ld32(S + 96, s + 96);
+        tmem_ld_wait();
         if (!whole) {
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
-            if (!seen(p * 16 + c)) s[c] = 0xff800000u;
+          for (int c = 0; c < 128; ++c)
+            if (!(seen[c >> 5] >> (c & 31) & 1)) s[c] = 0xff800000u;
         }
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 16; c += 2) now = fmaxf(now, fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
-      }
-      now *= scale;
-      const bool move = now > top + 8.f;
-      if (__any_sync(0xffffffffu, move)) {
-        const float ref = move ? now : top, keep = ex2(top - ref);
-        top = ref;
-        sum *= keep;
-        if (it > 0) {      // O of the tiles before has to follow
-          if (!mbar_wait(&bars[wO + u], (it + 1) & 1)) { tc_fail(9); ok = false; break; }
-          tc_fence_after_sync();
-          tmem_ld_wait();
+        for (int c = 0; c < 128; c += 2) most[(c >> 1) & 3] = fmaxf(most[(c >> 1) & 3], fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
+        const float now = scale * fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        const bool move = now > top + 8.f;
+        if (__any_sync(0xffffffffu, move)) {
+          const float ref = move ? now : top, keep = ex2(top - ref);
+          top = ref;
+          sum *= keep;
+          if (!first) {      // O of the tiles before has to follow
+            if (!mbar_wait(&bars[wO + u], (it + 1) & 1)) { tc_fail(10); ok = false; break; }
+            tc_fence_after_sync();
 #pragma unroll 1
-          for (int c0 = 0; c0 < DP; c0 += 16) {
-            uint32_t o[16];
-            tmem_ld16(O + c0, o);
-            tmem_ld_wait();
+            for (int c0 = 0; c0 < DP; c0 += 16) {
+              uint32_t o[16];
+              tmem_ld16(O + c0, o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * keep);
-            tmem_st16(O + c0, o);
+              for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * keep);
+              tmem_st16(O + c0, o);
+            }
           }
         }
-      }
-      // weights
-      float part[2] = {0.f, 0.f};
-#pragma unroll 1
-      for (int p = 0; p < 8; ++p) {
-        tmem_ld_wait();
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < 16; ++c) s[c] = next[c];
-        if (p < 7) tmem_ld16(S + p * 16 + 16, next);
-        if (!whole) {
+        for (int x = 0; x < 4; ++x) {
+          uint32_t p[16];
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
-            if (!seen(p * 16 + c)) s[c] = 0xff800000u;
+          for (int c = 0; c < 32; c += 2) {
+            const float p0 = ex2(fmaf(__uint_as_float(s[x * 32 + c]), scale, -top)), p1 = ex2(fmaf(__uint_as_float(s[x * 32 + c + 1]), scale, -top));
+            part[(c >> 1) & 1] += p0;
+            part[2 + ((c >> 1) & 1)] += p1;
+            p[c >> 1] = pack2h<T>(p0, p1);
+          }
+          tmem_st16(S + x * 16, p);
         }
-        uint32_t w[8];
-#pragma unroll
-        for (int c = 0; c < 16; c += 2) {
-          const float p0 = ex2(fmaf(__uint_as_float(s[c]), scale, -top)), p1 = ex2(fmaf(__uint_as_float(s[c + 1]), scale, -top));
-          part[0] += p0;
-          part[1] += p1;
-          w[c >> 1] = pack2h<T>(p0, p1);
-        }
-        tmem_st8(S + p * 8, w);
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        mbar_arrive(&bars[wP + u]);
+        if (ORDERED) mbar_arrive(&bars[wEmpty + n % kStages]);      // the numbers have been read
+        first = false;
+        ++it;
       }
-      sum += part[0] + part[1];
-      tmem_st_wait();
-      tc_fence_before_sync();
-      mbar_arrive(&bars[wP + u]);
-      if (ORDERED) mbar_arrive(&bars[wEmpty + n % kStages]);      // the numbers have been read
-      ++it;
-    }
-    if (ok && own.end > 0 && it > 0 && !mbar_wait(&bars[wO + u], (it + 1) & 1)) { tc_fail(10); ok = false; }
-    if (ok && own.end > 0) {
+      if (!ok || own.end == 0) continue;
+      if (!first && !mbar_wait(&bars[wO + u], (it + 1) & 1)) { tc_fail(11); break; }
       tc_fence_after_sync();
-      const int h = unit_head(u);
+      const int h = k.h0 + (pair_heads ? u : 0);
       const float inv = sum > 0.f && mine >= 0 ? 1.f / sum : 0.f;      // a query that sees nothing (a padded one) has 0
-      const bool wide = a.D % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
-      T* out = static_cast<T*>(a.out) + ((i * a.B + b) * a.H + h) * a.D;
+      T* out = static_cast<T*>(a.out) + ((i * a.B + k.b) * a.H + h) * a.D;
 #pragma unroll 1
-      for (int c0 = 0; c0 < DP; c0 += 16) {
-        uint32_t o[16];
+      for (int c0 = 0; c0 < DP; c0 += 32) {
+        uint32_t o[32];
         tmem_ld16(O + c0, o);
+        tmem_ld16(O + c0 + 16, o + 16);
         tmem_ld_wait();
-        float v[16];
+        float v[32];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) v[c] = inv > 0.f ? __uint_as_float(o[c]) * inv : 0.f;
+        for (int c = 0; c < 32; ++c) v[c] = inv > 0.f ? __uint_as_float(o[c]) * inv : 0.f;
         if (i < a.T && c0 < a.D) store_row16(out + c0, v, a.D - c0, wide);
+        if (i < a.T && c0 + 16 < a.D) store_row16(out + c0 + 16, v + 16, a.D - c0 - 16, wide);
       }
-      if (a.lse && i < a.T) a.lse[((int64_t)b * a.H + h) * a.T + i] = inv > 0.f ? kLn2 * (top + __log2f(sum)) : 0.f;
+      tc_fence_before_sync();      // the next weights let the issuer write O again
+      if (a.lse && i < a.T) a.lse[((int64_t)k.b * a.H + h) * a.T + i] = inv > 0.f ? kLn2 * (top + __log2f(sum)) : 0.f;
     }
-  } else if (ORDERED && warp >= 12) {
-    // ------------------------------------------------------------------ numbers of a tile's keys; values of places without a token
-    const int j = tid - 384;
+  } else if (ORDERED) {
+    // ------------------------------------------------------------------ warp 3: numbers of a tile's keys; values of places without a token
     int n = 0;
-    for (int64_t kt = both.begin(); kt < both.end; kt = both.next(kt), ++n) {
-      const int st = n % kStages;
-      const int number = num.at(kt * 128 + j);
-      // the stage is empty once it has been filled again: its numbers are no longer read
-      if (!mbar_wait(&bars[wFullV + st], (n / kStages) & 1)) { tc_fail(11); break; }
-      reinterpret_cast<int*>(sm + Lay::num)[st * 128 + j] = number;
-      if (number < 0) {
+    bool ok = true;
+    for (int w = blockIdx.x; ok && w < works; w += gridDim.x) {
+      Work k;
+      work_of(w, k);
+      const WindowNumbers num(a, k.b);
+      for (int64_t kt = k.both.begin(); kt < k.both.end; kt = k.both.next(kt), ++n) {
+        const int st = n % kStages;
+        int number[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) number[e] = num.at(kt * 128 + e * 32 + lane);
+        // the stage has been filled again, so that nobody reads its old numbers
+        if (!mbar_wait(&bars[wFullV + st], (n / kStages) & 1)) { tc_fail(12); ok = false; break; }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          reinterpret_cast<int*>(sm + Lay::num)[st * 128 + e * 32 + lane] = number[e];
+          if (number[e] < 0) {
 #pragma unroll 1
-        for (int ch = 0; ch < 8 * DB; ++ch) *reinterpret_cast<uint4*>(sm + Lay::v + st * DB * kBox + row_chunk2(j, ch)) = make_uint4(0, 0, 0, 0);
+            for (int ch = 0; ch < 8 * DB; ++ch) *reinterpret_cast<uint4*>(sm + Lay::v + st * DB * kBox + row_chunk2(e * 32 + lane, ch)) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_async_smem();
+        mbar_arrive(&bars[wNumbers + st]);
       }
-      fence_async_smem();
-      mbar_arrive(&bars[wNum_ + st]);
     }
   }
   tc_fence_before_sync();
@@ -262,13 +307,13 @@ namespace {
 
 template <typename T, int DB, bool ORDERED>
 int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const WindowArgs& a, cudaStream_t stream) {
-  using Lay = WinLayout<DB, ORDERED>;
+  using Lay = WinLayout<DB>;
   cudaError_t e = cudaFuncSetAttribute(window_tc_kernel<T, DB, ORDERED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Lay::bytes);
   if (e != cudaSuccess) return fail((int)e, "window_fwd: cannot reserve %u bytes of shared memory: %s", Lay::bytes, cudaGetErrorString(e));
   const bool pair_heads = a.H / a.G % 2 == 0;
   const int64_t runs = (a.T + 127) / 128, ctas = pair_heads ? runs * a.B * (a.H / 2) : (runs + 1) / 2 * a.B * a.H;
   RFA_REQUIRE(ctas < (int64_t)1 << 31, RFA_EUNSUPPORTED, "window_fwd: %lld tiles", (long long)ctas);
-  e = launch_pdl(window_tc_kernel<T, DB, ORDERED>, dim3((unsigned)ctas), dim3(Lay::kThreads), Lay::bytes, stream, q, k, v, a, pair_heads);
+  e = launch_pdl(window_tc_kernel<T, DB, ORDERED>, dim3((unsigned)std::min<int64_t>(ctas, 148)), dim3(kWinThreads), Lay::bytes, stream, q, k, v, a, pair_heads, (int)ctas);
   if (e != cudaSuccess) return fail((int)e, "rfa_window_fwd: launch failed: %s", cudaGetErrorString(e));
   return check_launch("rfa_window_fwd");
 }
