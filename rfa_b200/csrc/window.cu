@@ -83,7 +83,9 @@ extern "C" int rfa_window_bwd(const rfa_window_t* c, const void* out, const floa
   a.gq = gq; a.gk = gk; a.gv = gv;
   if (c->mask)
     if (int r = number(a, *c, nullptr, 0, workspace, as_stream(stream))) return r;
-  return launch_window_bwd_tiles(a, as_stream(stream));
+  bool tc = window_tc_ok(a);
+  for (const void* p : {out, g, static_cast<const void*>(gq), static_cast<const void*>(gk), static_cast<const void*>(gv)}) tc = tc && aligned16(p);
+  return tc ? launch_window_bwd_tc(a, c->mask, as_stream(stream)) : launch_window_bwd_tiles(a, as_stream(stream));
 }
 
 extern "C" size_t rfa_window_append_workspace_bytes(int64_t T, int B, int H, int G, int D, int dtype, int window, int sinks, int empty) {

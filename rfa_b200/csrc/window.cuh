@@ -50,6 +50,7 @@ int launch_window_fwd_tiles(const WindowArgs& a, cudaStream_t stream);        //
 int launch_window_bwd_tiles(const WindowArgs& a, cudaStream_t stream);
 bool window_tc_ok(const WindowArgs& a);                                       // window_tc.cu: fp16 and bf16, heads of up to 128 in rows that a tensor map can describe
 int launch_window_fwd_tc(const WindowArgs& a, cudaStream_t stream);
+int launch_window_bwd_tc(const WindowArgs& a, const uint8_t* mask, cudaStream_t stream);      // window_bwd_tc.cu
 int launch_window_step(const rfa_window_t& c, void* cache_k, void* cache_v, int64_t* length, void* out, cudaStream_t stream);      // window_step.cu
 // the cache in front of the new tokens, in the order of their numbers and then themselves: [cap + T][B][G][D]; and back
 int launch_window_gather(const rfa_window_t& c, const void* cache_k, const void* cache_v, const int64_t* length, void* keys, void* values, cudaStream_t stream);

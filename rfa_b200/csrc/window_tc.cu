@@ -32,9 +32,6 @@ enum { wQ = 0, wQEmpty = 2, wFullK = 4, wFullV = 8, wEmpty = 12, wNumbers = 16, 
 // wTurn: a group's exponentials of a tile wait for the other group's before them, so that one group's products, maxima and waits fall in the other's exponentials.
 // Left alone the two run in step, and the special function unit idles for more than half of the time (6000 cycles for a pair of tiles, 64 and 128 wide).
 
-// the lowest n bits
-__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
-
 template <typename T, int DB, bool ORDERED>
 __global__ void __launch_bounds__(kWinThreads, 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,

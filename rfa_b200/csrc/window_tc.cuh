@@ -20,6 +20,8 @@ __device__ __forceinline__ WindowSpan window_span(const WindowNumbers& num, int6
   if (row0 >= T) return {0, 0, 0};
   return {num.first_key(at + row0) / kTile, (num.first_end() + kTile - 1) / kTile, (at + min(T, row0 + 128) + kTile - 1) / kTile};
 }
+// the lowest n bits
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 #endif
 
 }  // namespace rfa
