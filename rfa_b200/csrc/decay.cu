@@ -24,25 +24,25 @@ size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Workspace of a backward pass: the arrays of the largest sweep, then what the decays' gradient is made of.
 struct BwdPlan {
-  SweepPlan wide, tall;             // x3 as wide as k (gq, gk), as v (gv)
-  size_t sweep, dots, last, sums;   // bytes; dots: each of two
+  SweepPlan sweeps;
+  size_t dots, last, sums;   // bytes; dots: each of two
   explicit BwdPlan(const rfa_decay_t& c) {
     const int64_t BH = (int64_t)c.B * c.H;
-    wide = sweep_plan(c.T, BH, c.D, c.K);
-    tall = sweep_plan(c.T, BH, c.K, c.D);
-    sweep = std::max(round256(wide.totals) + round256(wide.seg_decay), round256(tall.totals) + round256(tall.seg_decay));
+    sweeps = sweep_plan(c.T, BH, 2 * sweep_tiles(c.K) + sweep_tiles(c.D), 3, c.K, c.D);
     dots = round256(sizeof(float) * sweep_tiles(c.K) * BH * c.T);
     last = round256(sizeof(float) * BH * c.K * c.D);
     sums = round256(sizeof(float) * BH);
   }
-  size_t bytes() const { return sweep + 2 * dots + last + sums; }
+  size_t sweep() const { return round256(sweeps.totals) + round256(sweeps.seg_decay); }
+  size_t bytes() const { return sweep() + 2 * dots + last + sums; }
 };
 size_t bwd_bytes(const rfa_decay_t& c) {
   const size_t tc = c.dtype != RFA_F32 && c.K <= 128 && c.D <= 128 && c.K % 8 == 0 && c.D % 8 == 0 ? decay_tc_bwd_bytes(c) : 0;
   return std::max(BwdPlan(c).bytes(), tc);
 }
 
-SweepArgs sweep_args(const rfa_decay_t& c, int A, int W, bool rev, char* ws, const SweepPlan& plan) {
+// sweep `i` of `n` in a launch
+SweepArgs sweep_args(const rfa_decay_t& c, int A, int W, bool rev, char* ws, const SweepPlan& plan, int i, int n) {
   SweepArgs a{};
   a.decay = {c.log_decay, c.g_t, c.g_b, c.g_h};
   a.mask = c.mask;
@@ -50,8 +50,8 @@ SweepArgs sweep_args(const rfa_decay_t& c, int A, int W, bool rev, char* ws, con
   a.dtype = c.dtype; a.decay_dtype = c.decay_dtype; a.rev = rev;
   a.in_scale = rev ? c.scale : 1.f;
   a.out_scale = rev ? 1.f : c.scale;
-  a.totals = reinterpret_cast<float*>(ws);
-  a.seg_decay = reinterpret_cast<double*>(ws + round256(plan.totals));
+  a.totals = reinterpret_cast<float*>(ws) + plan.totals / sizeof(float) / n * i;
+  a.seg_decay = reinterpret_cast<double*>(ws + round256(plan.totals)) + plan.seg_decay / sizeof(double) / n * i;
   return a;
 }
 
@@ -65,7 +65,7 @@ extern "C" size_t rfa_decay_workspace_bytes(int64_t T, int B, int H, int K, int 
   c.T = T; c.B = B; c.H = H; c.K = K; c.D = D; c.dtype = dtype;
   if (backward) return bwd_bytes(c);
   size_t most = 0;
-  for (const SweepPlan& p : {sweep_plan(T, (int64_t)B * H, K, D), decay_tc_plan(T, (int64_t)B * H, K, D)}) most = std::max(most, round256(p.totals) + round256(p.seg_decay));
+  for (const SweepPlan& p : {sweep_plan(T, (int64_t)B * H, sweep_tiles(D), 1, K, D), decay_tc_plan(T, (int64_t)B * H, K, D)}) most = std::max(most, round256(p.totals) + round256(p.seg_decay));
   return most;
 }
 
@@ -77,15 +77,18 @@ extern "C" int rfa_decay_fwd(const rfa_decay_t* c, void* out, float* s_out, void
   const size_t need = rfa_decay_workspace_bytes(c->T, c->B, c->H, c->K, c->D, c->dtype, 0);
   RFA_REQUIRE(!need || (workspace && workspace_bytes >= need), RFA_EWORKSPACE, "decay_fwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
   if (decay_tc_ok(*c) && aligned16(out)) return launch_decay_tc(*c, decay_tc_plan(c->T, (int64_t)c->B * c->H, c->K, c->D), static_cast<char*>(workspace), out, s_out, as_stream(stream));
-  const SweepPlan plan = sweep_plan(c->T, (int64_t)c->B * c->H, c->K, c->D);
-  SweepArgs a = sweep_args(*c, c->K, c->D, false, static_cast<char*>(workspace), plan);
+  const SweepPlan plan = sweep_plan(c->T, (int64_t)c->B * c->H, sweep_tiles(c->D), 1, c->K, c->D);
+  SweepBatch batch{};
+  batch.count = 1;
+  SweepArgs& a = batch.sweep[0];
+  a = sweep_args(*c, c->K, c->D, false, static_cast<char*>(workspace), plan, 0, 1);
   a.x1 = {c->q, c->q_t, c->q_b, c->q_h};
   a.x2 = {c->k, c->k_t, c->k_b, c->k_h};
   a.x3 = {c->v, c->v_t, c->v_b, c->v_h};
   a.out = out;
   a.s_in = {const_cast<float*>(c->s_in), c->D, 1};
   a.s_out = {s_out, c->D, 1};
-  return launch_sweep(a, plan, as_stream(stream));
+  return launch_sweeps(batch, plan, as_stream(stream));
 }
 
 extern "C" int rfa_decay_bwd(const rfa_decay_t* c, const void* g, const float* g_s, void* gq, void* gk, void* gv, void* g_decay, float* gs_in, void* workspace,
@@ -100,35 +103,35 @@ extern "C" int rfa_decay_bwd(const rfa_decay_t* c, const void* g, const float* g
   if (decay_tc_ok(*c) && aligned16(g) && aligned16(gq) && aligned16(gk) && aligned16(gv))
     return launch_decay_tc_bwd(*c, static_cast<char*>(workspace), g, g_s, gq, gk, gv, g_decay, gs_in, st);
   const BwdPlan plan(*c);
-  char* ws = static_cast<char*>(workspace);
-  float* q_dots = reinterpret_cast<float*>(ws + plan.sweep);
-  float* k_dots = reinterpret_cast<float*>(ws + plan.sweep + plan.dots);
-  float* last = reinterpret_cast<float*>(ws + plan.sweep + 2 * plan.dots);
-  float* sums = reinterpret_cast<float*>(ws + plan.sweep + 2 * plan.dots + plan.last);
+  char *ws = static_cast<char*>(workspace), *rest = ws + plan.sweep();
+  float* q_dots = reinterpret_cast<float*>(rest);
+  float* k_dots = reinterpret_cast<float*>(rest + plan.dots);
+  float* last = reinterpret_cast<float*>(rest + 2 * plan.dots);
+  float* sums = reinterpret_cast<float*>(rest + 2 * plan.dots + plan.last);
   const DecayRows q{c->q, c->q_t, c->q_b, c->q_h}, k{c->k, c->k_t, c->k_b, c->k_h}, v{c->v, c->v_t, c->v_b, c->v_h};
   const DecayRows gr{g, (int64_t)c->B * c->H * c->D, (int64_t)c->H * c->D, c->D};
   float *s_in = const_cast<float*>(c->s_in), *g_last = const_cast<float*>(g_s);
-
-  SweepArgs a = sweep_args(*c, c->D, c->K, false, ws, plan.wide);
+  SweepBatch batch{};
+  batch.count = 3;
+  SweepArgs& a = batch.sweep[0];
+  a = sweep_args(*c, c->D, c->K, false, ws, plan.sweeps, 0, 3);
   a.x1 = gr; a.x2 = v; a.x3 = k; a.out = gq;
   a.s_in = {s_in, 1, c->D};
+  SweepArgs& ak = batch.sweep[1];
+  ak = sweep_args(*c, c->D, c->K, true, ws, plan.sweeps, 1, 3);
+  ak.x1 = v; ak.x2 = gr; ak.x3 = q; ak.out = gk;
+  ak.s_in = {g_last, 1, c->D};
+  SweepArgs& av = batch.sweep[2];
+  av = sweep_args(*c, c->K, c->D, true, ws, plan.sweeps, 2, 3);
+  av.x1 = k; av.x2 = q; av.x3 = gr; av.out = gv;
+  av.s_in = {g_last, c->D, 1};
+  av.s_out = {gs_in, c->D, 1};
   if (g_decay) {
     a.x4 = q; a.dots = q_dots;
+    ak.x4 = k; ak.dots = k_dots;
     if (g_s) a.s_out = {last, 1, c->D};
   }
-  if (int r = launch_sweep(a, plan.wide, st)) return r;
-
-  a = sweep_args(*c, c->D, c->K, true, ws, plan.wide);
-  a.x1 = v; a.x2 = gr; a.x3 = q; a.out = gk;
-  a.s_in = {g_last, 1, c->D};
-  if (g_decay) { a.x4 = k; a.dots = k_dots; }
-  if (int r = launch_sweep(a, plan.wide, st)) return r;
-
-  a = sweep_args(*c, c->K, c->D, true, ws, plan.tall);
-  a.x1 = k; a.x2 = q; a.x3 = gr; a.out = gv;
-  a.s_in = {g_last, c->D, 1};
-  a.s_out = {gs_in, c->D, 1};
-  if (int r = launch_sweep(a, plan.tall, st)) return r;
+  if (int r = launch_sweeps(batch, plan.sweeps, st)) return r;
 
   if (!g_decay) return 0;
   const int tiles = sweep_tiles(c->K);

@@ -37,16 +37,22 @@ struct SweepArgs {
   float in_scale, out_scale;
 };
 
+// Sweeps that do not depend on each other, in one launch: the same tokens, rows and heads
+struct SweepBatch {
+  SweepArgs sweep[3];
+  int tiles[3], count;
+};
+
 // decay_sweep.cu: any sizes up to kDecayMaxWidth, any types
 constexpr int kDecayMaxWidth = 256;
 struct SweepPlan {
   int nseg;
   int64_t tseg;
-  size_t totals, seg_decay;      // workspace bytes of the two arrays
+  size_t totals, seg_decay;      // workspace bytes of the two arrays, for all of a launch's sweeps
 };
-SweepPlan sweep_plan(int64_t T, int64_t BH, int A, int W);
+SweepPlan sweep_plan(int64_t T, int64_t BH, int tiles, int states, int A, int W);      // tiles: of all sweeps together; `states` of A x W
 int sweep_tiles(int W);
-int launch_sweep(SweepArgs a, const SweepPlan& plan, cudaStream_t stream);
+int launch_sweeps(SweepBatch batch, const SweepPlan& plan, cudaStream_t stream);
 // totals: what each segment adds -> the state in front of it; at most 65535 (row, head)s
 int launch_decay_combine(float* totals, const double* seg_decay, DecayState s_in, int nseg, int64_t BH, int A, int W, cudaStream_t stream);
 int launch_decay_grad(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_last, int KD, const uint8_t* mask,

@@ -10,15 +10,15 @@
 //     g_t = sum_(i >= t) (rows of M + scale 2^(L_i) q_i . (G S^T)_i) - sum_(j >= t) columns of M + sum_(j < t) 2^(L_end - L_j) k_j . (V dS^T)_j + 2^(L_end) S . dS
 // in which only the rows and columns of one and the same M are subtracted from each other.
 //
-// Warp roles (352 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 the decays, warps 3..10 two groups that share the rows' columns 16 by 16: clear padded rows,
-// T0, T1 -> P, D, then the gradients straight from registers.  P takes the place of S.  TMEM: four regions of 128 columns, T0 / T1 / G S^T / V dS^T, the first three
+// Warp roles (608 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 the decays, warps 3..18 four groups that share the rows' columns 16 by 16: clear padded
+// rows, T0, T1 -> P, D, then the gradients straight from registers.  P takes the place of S.  TMEM: four regions of 128 columns, T0 / T1 / G S^T / V dS^T, the first three
 // of them used again.  All waits are bounded.
 #define RFA_TC_FAMILY 11
 #include "decay_tc.cuh"
 
 namespace rfa {
 
-constexpr int kDgThreads = 352;
+constexpr int kDgThreads = 608, kDgGroups = 4, kDgRows = kDgGroups * 128;
 
 struct DecayGradArgs {
   DecayRows decay;
@@ -57,7 +57,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const int b = (int)(bh / a.H), h = (int)(bh % a.H);
   const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.T : nullptr;
   if (tid == 0) {
-    for (int i = 0; i < gNum; ++i) mbar_init(&bars[i], i == gL ? 32 : i == gClean || i == gX || i == gP || i == gE1 || i == gAll ? 256 : i == gSum ? 128 : 1);
+    for (int i = 0; i < gNum; ++i) mbar_init(&bars[i], i == gL ? 32 : i == gClean || i == gX || i == gP || i == gE1 || i == gAll ? kDgRows : i == gSum ? 128 : 1);
     mbar_fence_init();
     tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v); tma_prefetch_desc(&tm_g);
   }
@@ -143,7 +143,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     for (int e = 0; e < 4; ++e) L[lane * 4 + e] = (float)(sum[e] + before);
     mbar_arrive(&bars[gL]);
   } else {
-    // ------------------------------------------------------------------ two groups of 128: rows of the chunk, every other 16 columns
+    // ------------------------------------------------------------------ four groups of 128: rows of the chunk, every fourth 16 columns
     const int group = (warp - 3) >> 2, quarter = warp & 3, row = quarter * 32 + lane, wtid = tid - 96;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const uint32_t R0 = tmem + lane_addr, R1 = R0 + 128, R2 = R0 + 256, R3 = R0 + 384;
@@ -162,7 +162,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
               *reinterpret_cast<uint4*>(sm + Lay::q + row_chunk2(row, ch)) = zero;
               *reinterpret_cast<uint4*>(sm + Lay::k + row_chunk2(row, ch)) = zero;
             }
-          } else {
+          } else if (group == 1) {
 #pragma unroll 1
             for (int ch = 0; ch < 8 * DB; ++ch) {
               *reinterpret_cast<uint4*>(sm + Lay::v + row_chunk2(row, ch)) = zero;
@@ -176,7 +176,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       if (!mbar_wait(&bars[gS], 0) || !mbar_wait(&bars[gDS], 0)) { tc_fail(9); break; }
       if (want) {
 #pragma unroll 1
-        for (uint32_t i = wtid * 16; i < Lay::kCopyBytes; i += 256 * 16) {
+        for (uint32_t i = wtid * 16; i < Lay::kCopyBytes; i += kDgRows * 16) {
           const uint4 u = *reinterpret_cast<const uint4*>(sm + Lay::s + i), w = *reinterpret_cast<const uint4*>(sm + Lay::ds + i);
           const uint32_t us[4] = {u.x, u.y, u.z, u.w}, ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -193,7 +193,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       tc_fence_after_sync();
       const int pieces = 2 * quarter + 2;      // of 16 columns, that reach up to the diagonal
 #pragma unroll 1
-      for (int p = group; p < 8; p += 2) {
+      for (int p = group; p < 8; p += kDgGroups) {
         uint32_t pw[8], dw[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) pw[i] = dw[i] = 0u;
@@ -255,7 +255,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       const auto grad = [&](uint32_t main, uint32_t side, float f, void* out, uint32_t tile, float& sum, bool wide) {
         T* o = static_cast<T*>(out) + at * a.K;
 #pragma unroll 1
-        for (int c0 = group * 16; c0 < KP; c0 += 32) {
+        for (int c0 = group * 16; c0 < KP; c0 += kDgGroups * 16) {
           uint32_t u[16], n[16];
           tmem_ld16(main + c0, u);
           tmem_ld16(side + c0, n);
@@ -295,7 +295,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       tc_fence_after_sync();
       T* o = static_cast<T*>(a.gv) + at * a.D;
 #pragma unroll 1
-      for (int c0 = group * 16; c0 < DP; c0 += 32) {
+      for (int c0 = group * 16; c0 < DP; c0 += kDgGroups * 16) {
         uint32_t u[16], n[16];
         tmem_ld16(R0 + c0, u);
         tmem_ld16(R2 + c0, n);
@@ -307,15 +307,25 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       }
       // ---- the decays: everything that was read of the tiles has been (gO3), so that P's place serves the exchange
       if (want) {
-        float* ex = reinterpret_cast<float*>(sm + Lay::s);      // [2][128] rows and keys of the second group, then a sum of S . dS for each warp
+        // P's place: [group][128] rows, [group][128] keys of the other groups, a sum of S . dS for each warp, the first group's warps' sums
+        float* ex = reinterpret_cast<float*>(sm + Lay::s);
+        float *ex_x = ex + 2 * kDgRows, *ex_down = ex_x + 16, *ex_up = ex_down + 4, *ex_all = ex_up + 4;
         x = warp_sum(x);
-        if (lane == 0) ex[512 + (warp - 3)] = x;
-        if (group == 1) { ex[row] = rows_sum; ex[128 + row] = keys_sum; }
+        if (lane == 0) ex_x[warp - 3] = x;
+        if (group > 0) {
+          ex[group * 128 + row] = rows_sum;
+          ex[kDgRows + group * 128 + row] = keys_sum;
+        }
         mbar_arrive(&bars[gAll]);
         if (!mbar_wait(&bars[gAll], 0)) { tc_fail(15); break; }
         // suffix sums of rows less columns, prefix sums of keys, by the first group: within a warp, then across
         if (group == 0) {
-          float down = rows_sum + ex[row] - (cols[row] + cols[128 + row] + cols[256 + row] + cols[384 + row]), up = keys_sum + ex[128 + row];
+          float down = rows_sum - (cols[row] + cols[128 + row] + cols[256 + row] + cols[384 + row]), up = keys_sum;
+#pragma unroll
+          for (int i = 1; i < kDgGroups; ++i) {
+            down += ex[i * 128 + row];
+            up += ex[kDgRows + i * 128 + row];
+          }
           const float own_up = up;
 #pragma unroll
           for (int o2 = 1; o2 < 32; o2 <<= 1) {
@@ -323,18 +333,18 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             if (lane + o2 < 32) down += d;
             if (lane >= o2) up += u;
           }
-          if (lane == 0) ex[528 + quarter] = down;
-          if (lane == 31) ex[532 + quarter] = up;
+          if (lane == 0) ex_down[quarter] = down;
+          if (lane == 31) ex_up[quarter] = up;
           uint32_t phase = 0;
           if (!epi_sync(&bars[gSum], phase)) { tc_fail(16); break; }
           float g = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g += ex[512 + i];
+          for (int i = 0; i < 4 * kDgGroups; ++i) g += ex_x[i];
           g = ex2(end) * g + down + up - own_up;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (i > quarter) g += ex[528 + i];
-            if (i < quarter) g += ex[532 + i];
+            if (i > quarter) g += ex_down[i];
+            if (i < quarter) g += ex_up[i];
           }
           const bool real = there && !(mask && mask[t]);
           if (!real) g = 0.f;
@@ -346,9 +356,9 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             }
           } else {
             g = warp_sum(g);
-            if (lane == 0) ex[536 + quarter] = g;
+            if (lane == 0) ex_all[quarter] = g;
             if (!epi_sync(&bars[gSum], phase)) { tc_fail(17); break; }
-            if (row == 0) static_cast<float*>(a.g_decay)[(b * chunks + chunk) * a.H + h] = ex[536] + ex[537] + ex[538] + ex[539];
+            if (row == 0) static_cast<float*>(a.g_decay)[(b * chunks + chunk) * a.H + h] = ex_all[0] + ex_all[1] + ex_all[2] + ex_all[3];
           }
         }
       }

@@ -1,9 +1,9 @@
 // Linear attention with a decay, any sizes and types: the sweep of decay.cuh in fp32 multiply-adds, the joining of its segments, and the gradient
 // of the decays.
 //
-// One CTA takes a (batch row, head), a tile of x3's columns and a segment of the tokens, in chunks of 32.  The tile's columns of the state stay in shared
+// One CTA takes a (batch row, head), a tile of 32 or 64 of x3's columns and a segment of the tokens, in chunks of 32.  The tile's columns of the state stay in shared
 // memory.  Sums of log decays are 64 bits: what is subtracted from each other there is the sum over a chunk, and the difference may be that of
-// two neighbours.  Bound by shared memory's reads (a thread's 8 multiply-adds take one 16-byte and two 4-byte reads).  Where there are
+// two neighbours.  Bound by shared memory's reads (a thread's 8 multiply-adds of out take one 16-byte and two 4-byte reads).  Where there are
 // few (row, head, tile)s the tokens are cut into segments: each one's own state first, then the states in front of each (combine), then the sweep proper.
 #include <algorithm>
 
@@ -13,23 +13,39 @@ namespace rfa {
 
 namespace {
 
-constexpr int kC = 32, kThreads = 256, DT = 32;
-constexpr int kCols = DT / 4, kRowGroups = kThreads / kCols, kRows = kC / kRowGroups;     // a thread: kRows rows of 4 columns
-size_t sweep_smem_bytes(int A) {
+constexpr int kC = 32, kThreads = 256;
+constexpr int tile_of(int W) { return W <= 32 ? 32 : 64; }      // columns of x3 that a CTA takes
+size_t sweep_smem_bytes(int A, int DT) {
   return sizeof(float) * ((size_t)2 * kC * (A + 1) + kC * DT + (size_t)A * DT + kC * (kC + 1) + 2 * kC) + sizeof(double) * kC;
 }
 
+// `n` rows of `width` numbers from column c0 on, `cols` of a row in shared memory, ld apart; the others and padded rows are zero, whatever stands there.  Eight numbers
+// (and their rows' mask) on the way at a time.
 template <typename T>
-__device__ __forceinline__ void load_rows(float* dst, int ld, const DecayRows& x, int64_t base, int64_t t0, int n, int c0, int width, const uint8_t* mask, int tid) {
-  for (int i = tid; i < kC * width; i += kThreads) {
-    const int r = i / width, c = i - r * width;
-    const bool there = r < n && !(mask && mask[t0 + r]);
-    dst[r * ld + c] = there ? to_f<T>(static_cast<const T*>(x.p)[base + (t0 + r) * x.t + c0 + c]) : 0.f;
+__device__ __forceinline__ void load_rows(float* dst, int ld, int cols, const T* src, int64_t s_t, int n, int width, const uint8_t* mask, int tid) {
+  constexpr int kFlight = 8;
+  for (int i0 = tid; i0 < kC * cols; i0 += kFlight * kThreads) {
+    T v[kFlight];
+    uint8_t gone[kFlight];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int i = i0 + f * kThreads, r = i / cols, c = i - r * cols;
+      const bool there = r < n && c < width;
+      v[f] = there ? src[r * s_t + c] : from_f<T>(0.f);
+      gone[f] = there && mask ? mask[r] : 0;
+    }
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int i = i0 + f * kThreads, r = i / cols;
+      if (i < kC * cols) dst[r * ld + i - r * cols] = gone[f] ? 0.f : to_f<T>(v[f]);
+    }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) decay_sweep_kernel(const __grid_constant__ SweepArgs a, bool state_only) {
+template <typename T, int DT>
+__device__ __forceinline__ void decay_sweep(const SweepArgs& a, int tile, bool state_only) {
+  constexpr int kCols = DT / 4, kRowGroups = kThreads / kCols, kRows = kC / kRowGroups;     // a thread: kRows rows of 4 columns of out
+  constexpr int kStateRows = DT == 64 ? 4 : 2;
   extern __shared__ double sweep_smem[];
   double* L = sweep_smem;
   float* x1 = reinterpret_cast<float*>(L + kC);
@@ -37,7 +53,7 @@ __global__ void __launch_bounds__(kThreads) decay_sweep_kernel(const __grid_cons
   float *x2 = x1 + kC * ld, *x3 = x2 + kC * ld, *S = x3 + kC * DT, *P = S + (size_t)A * DT, *fa = P + kC * (kC + 1), *fb = fa + kC;
   // x1, x2 rows are A + 1 apart (a bank more each); x3 and S rows are read 16 bytes at a time (kC * (A + 1) floats are a multiple of that)
   const int64_t bh = blockIdx.x;
-  const int b = (int)(bh / a.H), h = (int)(bh % a.H), c0 = blockIdx.y * DT, W = min(DT, a.W - c0), seg = blockIdx.z;
+  const int b = (int)(bh / a.H), h = (int)(bh % a.H), c0 = tile * DT, W = min(DT, a.W - c0), seg = blockIdx.z;
   const int64_t BH = (int64_t)a.B * a.H;
   const int place = a.rev ? a.nseg - 1 - seg : seg;                 // segments are counted in the order of the sweep
   const int64_t t_begin = place * a.tseg, t_end = min(a.T, t_begin + a.tseg);
@@ -46,14 +62,18 @@ __global__ void __launch_bounds__(kThreads) decay_sweep_kernel(const __grid_cons
   const int64_t b1 = b * a.x1.b + h * a.x1.h, b2 = b * a.x2.b + h * a.x2.h, b3 = b * a.x3.b + h * a.x3.h, bd = b * a.decay.b + h * a.decay.h;
   const int64_t slot = ((int64_t)seg * BH + bh) * A * a.W;
 
-  for (int i = tid; i < A * DT; i += kThreads) {
-    const int r = i / DT, c = i % DT;
-    float v = 0.f;
-    if (c < W && !state_only) {
-      if (a.nseg > 1) v = a.totals[slot + (int64_t)r * a.W + c0 + c];
-      else if (a.s_in.p) v = a.s_in.p[bh * A * a.W + r * a.s_in.row + (c0 + c) * a.s_in.col];
+  const float* start = state_only ? nullptr : a.nseg > 1 ? a.totals + slot + c0 : a.s_in.p ? a.s_in.p + bh * A * a.W + c0 * a.s_in.col : nullptr;
+  const int64_t start_r = a.nseg > 1 ? a.W : a.s_in.row, start_c = a.nseg > 1 ? 1 : a.s_in.col;
+  for (int i0 = tid; i0 < A * DT; i0 += 8 * kThreads) {
+    float v[8];
+#pragma unroll
+    for (int f = 0; f < 8; ++f) {
+      const int i = i0 + f * kThreads;
+      v[f] = start && i < A * DT && i % DT < W ? start[(i / DT) * start_r + (i % DT) * start_c] : 0.f;
     }
-    S[i] = v;
+#pragma unroll
+    for (int f = 0; f < 8; ++f)
+      if (i0 + f * kThreads < A * DT) S[i0 + f * kThreads] = v[f];
   }
   const int col = (tid % kCols) * 4, rg = tid / kCols;
   double run = 0.0;
@@ -61,14 +81,12 @@ __global__ void __launch_bounds__(kThreads) decay_sweep_kernel(const __grid_cons
     const int64_t t0 = t_begin + (int64_t)(a.rev ? nchunk - 1 - k : k) * kC;
     const int n = (int)min((int64_t)kC, t_end - t0);
     __syncthreads();
-    if (!state_only) load_rows<T>(x1, ld, a.x1, b1, t0, n, 0, A, mask, tid);
-    load_rows<T>(x2, ld, a.x2, b2, t0, n, 0, A, mask, tid);
-    for (int i = tid; i < kC * DT; i += kThreads) {
-      const int r = i / DT, c = i % DT;
-      x3[i] = c < W && r < n && !(mask && mask[t0 + r]) ? to_f<T>(static_cast<const T*>(a.x3.p)[b3 + (t0 + r) * a.x3.t + c0 + c]) : 0.f;
-    }
+    const uint8_t* gone = mask ? mask + t0 : nullptr;
+    if (!state_only) load_rows<T>(x1, ld, A, static_cast<const T*>(a.x1.p) + b1 + t0 * a.x1.t, a.x1.t, n, A, gone, tid);
+    load_rows<T>(x2, ld, A, static_cast<const T*>(a.x2.p) + b2 + t0 * a.x2.t, a.x2.t, n, A, gone, tid);
+    load_rows<T>(x3, DT, DT, static_cast<const T*>(a.x3.p) + b3 + t0 * a.x3.t + c0, a.x3.t, n, W, gone, tid);
     if (tid < kC) {
-      double g = tid < n && !(mask && mask[t0 + tid]) ? log_decay_at(a.decay.p, a.decay_dtype, bd + (t0 + tid) * a.decay.t) : 0.0;
+      double g = tid < n && !(gone && gone[tid]) ? log_decay_at(a.decay.p, a.decay_dtype, bd + (t0 + tid) * a.decay.t) : 0.0;
 #pragma unroll
       for (int o = 1; o < kC; o <<= 1) {
         const double up = __shfl_up_sync(0xffffffffu, g, o);
@@ -84,14 +102,25 @@ __global__ void __launch_bounds__(kThreads) decay_sweep_kernel(const __grid_cons
     run += L[kC - 1];
     const Factor decay((float)L[kC - 1]);
     if (!state_only) {
-      for (int i = tid; i < kC * kC; i += kThreads) {
-        const int r = i / kC, c = i % kC;
-        float p = 0.f;
-        if (a.rev ? c >= r : c <= r) {
-          for (int d = 0; d < A; ++d) p = fmaf(x1[r * ld + d], x2[c * ld + d], p);
-          p *= a.in_scale * expf((float)(a.rev ? L[c] - L[r] : L[r] - L[c]));
+      {      // 2 x 2 scores a thread, one of them beyond the diagonal
+        const int ty = tid / 16, tx = tid % 16;
+        float p[2][2] = {};
+        const float *y0 = x1 + ty * ld, *y1 = y0 + 16 * ld, *z0 = x2 + tx * ld, *z1 = z0 + 16 * ld;
+#pragma unroll 4
+        for (int d = 0; d < A; ++d) {
+          const float u0 = y0[d], u1 = y1[d], w0 = z0[d], w1 = z1[d];
+          p[0][0] = fmaf(u0, w0, p[0][0]);
+          p[1][1] = fmaf(u1, w1, p[1][1]);
+          p[1][0] = fmaf(a.rev ? u0 : u1, a.rev ? w1 : w0, p[1][0]);
         }
-        P[r * (kC + 1) + c] = p;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = ty + 16 * i, c = tx + 16 * j;
+            const float dot = i == j ? p[i][i] : p[1][0];      // that of rows behind 16 and columns before, or backwards the other one
+            P[r * (kC + 1) + c] = (a.rev ? c >= r : c <= r) ? dot * a.in_scale * expf((float)(a.rev ? L[c] - L[r] : L[r] - L[c])) : 0.f;
+          }
       }
       __syncthreads();
       float acc[kRows][4] = {};
@@ -126,45 +155,47 @@ __global__ void __launch_bounds__(kThreads) decay_sweep_kernel(const __grid_cons
         float dot = 0.f;
         if (r < n) {
           T* o = static_cast<T*>(a.out) + ((t * a.B + b) * a.H + h) * a.W + c0;
-          const bool gone = mask && mask[t];
+          const bool padded = gone && r < n && gone[r];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (col + e < W) {
               const float v = a.out_scale * acc[i][e];
               o[col + e] = from_f<T>(v);
-              if (a.x4.p && !gone) dot = fmaf(v, to_f<T>(static_cast<const T*>(a.x4.p)[b * a.x4.b + h * a.x4.h + t * a.x4.t + c0 + col + e]), dot);
+              if (a.x4.p && !padded) dot = fmaf(v, to_f<T>(static_cast<const T*>(a.x4.p)[b * a.x4.b + h * a.x4.h + t * a.x4.t + c0 + col + e]), dot);
             }
         }
         if (a.x4.p) {
 #pragma unroll
           for (int s = kCols / 2; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-          if (col == 0 && r < n) a.dots[((int64_t)blockIdx.y * BH + bh) * a.T + t] = dot;
+          if (col == 0 && r < n) a.dots[((int64_t)tile * BH + bh) * a.T + t] = dot;
         }
       }
       __syncthreads();      // the state is read by all before it changes
     }
-    for (int d0 = 0; d0 < A; d0 += 4 * kRowGroups) {
-      float u[4][4];
+    for (int d0 = rg; d0 < A; d0 += kStateRows * kRowGroups) {
+      float u[kStateRows][4];
+      const float* row[kStateRows];      // rows beyond the last read the last key's number, and are not written
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int d = d0 + rg + m * kRowGroups;
-        const float4 s = d < A ? *reinterpret_cast<const float4*>(S + (size_t)d * DT + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int m = 0; m < kStateRows; ++m) {
+        const int d = min(d0 + m * kRowGroups, A - 1);
+        row[m] = x2 + d;
+        const float4 s = d0 + m * kRowGroups < A ? *reinterpret_cast<const float4*>(S + (size_t)d * DT + col) : make_float4(0.f, 0.f, 0.f, 0.f);
         u[m][0] = decay.times(s.x); u[m][1] = decay.times(s.y); u[m][2] = decay.times(s.z); u[m][3] = decay.times(s.w);
       }
 #pragma unroll 4
       for (int j = 0; j < kC; ++j) {
-        const float4 s = *reinterpret_cast<const float4*>(x3 + j * DT + col);
+        float4 s = *reinterpret_cast<const float4*>(x3 + j * DT + col);
         const float f = fb[j];
+        s.x *= f; s.y *= f; s.z *= f; s.w *= f;
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const int d = d0 + rg + m * kRowGroups;
-          const float kk = d < A ? f * x2[j * ld + d] : 0.f;
+        for (int m = 0; m < kStateRows; ++m) {
+          const float kk = row[m][j * ld];
           u[m][0] = fmaf(kk, s.x, u[m][0]); u[m][1] = fmaf(kk, s.y, u[m][1]); u[m][2] = fmaf(kk, s.z, u[m][2]); u[m][3] = fmaf(kk, s.w, u[m][3]);
         }
       }
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int d = d0 + rg + m * kRowGroups;
+      for (int m = 0; m < kStateRows; ++m) {
+        const int d = d0 + m * kRowGroups;
         if (d < A) *reinterpret_cast<float4*>(S + (size_t)d * DT + col) = make_float4(u[m][0], u[m][1], u[m][2], u[m][3]);
       }
     }
@@ -173,11 +204,20 @@ __global__ void __launch_bounds__(kThreads) decay_sweep_kernel(const __grid_cons
   if (state_only) {
     for (int i = tid; i < A * DT; i += kThreads)
       if (i % DT < W) a.totals[slot + (int64_t)(i / DT) * a.W + c0 + i % DT] = S[i];
-    if (tid == 0 && blockIdx.y == 0) a.seg_decay[(int64_t)seg * BH + bh] = run;
+    if (tid == 0 && tile == 0) a.seg_decay[(int64_t)seg * BH + bh] = run;
   } else if (a.s_out.p && seg == a.nseg - 1) {
     for (int i = tid; i < A * DT; i += kThreads)
       if (i % DT < W) a.s_out.p[bh * A * a.W + (i / DT) * a.s_out.row + (c0 + i % DT) * a.s_out.col] = S[i];
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) decay_sweep_kernel(const __grid_constant__ SweepBatch batch, bool state_only) {
+  int tile = blockIdx.y, which = 0;
+  while (which + 1 < batch.count && tile >= batch.tiles[which]) tile -= batch.tiles[which++];
+  const SweepArgs& a = batch.sweep[which];
+  if (tile_of(a.W) == 32) decay_sweep<T, 32>(a, tile, state_only);
+  else decay_sweep<T, 64>(a, tile, state_only);
 }
 
 // What each segment adds becomes the state in front of it, in the order of the sweep.  Bound by memory; a thread takes one element along all segments, eight of
@@ -275,47 +315,60 @@ int launch_decay_combine(float* totals, const double* seg_decay, DecayState s_in
 namespace {
 
 template <typename T>
-int sweep_launches(const SweepArgs& a, const SweepPlan& plan, cudaStream_t stream) {
-  const size_t smem = sweep_smem_bytes(a.A);
+int sweep_launches(const SweepBatch& batch, const SweepPlan& plan, cudaStream_t stream) {
+  size_t smem = 0;
+  int tiles = 0;
+  for (int i = 0; i < batch.count; ++i) {
+    smem = std::max(smem, sweep_smem_bytes(batch.sweep[i].A, tile_of(batch.sweep[i].W)));
+    tiles += batch.tiles[i];
+  }
   cudaError_t e = cudaFuncSetAttribute(decay_sweep_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return fail((int)e, "decay: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
-  const int64_t BH = (int64_t)a.B * a.H;
-  const dim3 grid((unsigned)BH, (a.W + DT - 1) / DT, plan.nseg);
+  const int64_t BH = (int64_t)batch.sweep[0].B * batch.sweep[0].H;
+  const dim3 grid((unsigned)BH, tiles, plan.nseg);
   if (plan.nseg > 1) {
-    decay_sweep_kernel<T><<<grid, kThreads, smem, stream>>>(a, true);
+    decay_sweep_kernel<T><<<grid, kThreads, smem, stream>>>(batch, true);
     if (int r = check_launch("rfa_decay (segments)")) return r;
-    if (int r = launch_decay_combine(a.totals, a.seg_decay, a.s_in, plan.nseg, BH, a.A, a.W, stream)) return r;
+    for (int i = 0; i < batch.count; ++i) {
+      const SweepArgs& a = batch.sweep[i];
+      if (int r = launch_decay_combine(a.totals, a.seg_decay, a.s_in, plan.nseg, BH, a.A, a.W, stream)) return r;
+    }
   }
-  decay_sweep_kernel<T><<<grid, kThreads, smem, stream>>>(a, false);
+  decay_sweep_kernel<T><<<grid, kThreads, smem, stream>>>(batch, false);
   return check_launch("rfa_decay");
 }
 
 }  // namespace
 
-int sweep_tiles(int W) { return (W + DT - 1) / DT; }
+int sweep_tiles(int W) { return (W + tile_of(W) - 1) / tile_of(W); }
 
-SweepPlan sweep_plan(int64_t T, int64_t BH, int A, int W) {
+SweepPlan sweep_plan(int64_t T, int64_t BH, int tiles, int states, int A, int W) {
   SweepPlan p{1, T, 0, 0};
-  const int64_t ctas = BH * sweep_tiles(W), chunks = (T + kC - 1) / kC;
-  // Segments cost a second reading of two operands.  Wanted: two CTAs an SM; at least 4 chunks a segment.
-  const int64_t want = std::min<int64_t>({(2 * 148 + ctas - 1) / ctas, chunks / 4, 64});
+  const int64_t ctas = BH * tiles, chunks = (T + kC - 1) / kC;
+  // Segments cost a second pass over the keys' side, which idle SMs take.  Wanted: two CTAs an SM, down to a chunk a segment.
+  const int64_t want = std::min<int64_t>({(2 * 148 + ctas - 1) / ctas, chunks, 64});
   if (ctas < 148 && want > 1) {
     const int64_t per = (chunks + want - 1) / want;
     p.tseg = per * kC;
     p.nseg = (int)((T + p.tseg - 1) / p.tseg);
   }
   if (p.nseg <= 1) return {1, T, 0, 0};
-  p.totals = sizeof(float) * p.nseg * BH * A * W;
-  p.seg_decay = sizeof(double) * p.nseg * BH;
+  p.totals = sizeof(float) * states * p.nseg * BH * A * W;
+  p.seg_decay = sizeof(double) * states * p.nseg * BH;
   return p;
 }
 
-int launch_sweep(SweepArgs a, const SweepPlan& plan, cudaStream_t stream) {
-  a.nseg = plan.nseg;
-  a.tseg = plan.tseg;
-  if (a.dtype == RFA_F32) return sweep_launches<float>(a, plan, stream);
-  if (a.dtype == RFA_F16) return sweep_launches<__half>(a, plan, stream);
-  return sweep_launches<__nv_bfloat16>(a, plan, stream);
+int launch_sweeps(SweepBatch batch, const SweepPlan& plan, cudaStream_t stream) {
+  for (int i = 0; i < batch.count; ++i) {
+    SweepArgs& a = batch.sweep[i];
+    a.nseg = plan.nseg;
+    a.tseg = plan.tseg;
+    batch.tiles[i] = sweep_tiles(a.W);
+  }
+  const int dtype = batch.sweep[0].dtype;
+  if (dtype == RFA_F32) return sweep_launches<float>(batch, plan, stream);
+  if (dtype == RFA_F16) return sweep_launches<__half>(batch, plan, stream);
+  return sweep_launches<__nv_bfloat16>(batch, plan, stream);
 }
 
 int launch_decay_grad(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_last, int KD, const uint8_t* mask,

@@ -15,9 +15,9 @@
 // Backwards (states alone), from the last chunk to the first: S = 2^(L_end) S + scale Q'^T G, Q'_i = 2^(L_i) q_i: the gradient of the state.  `kept`: the
 // 16-bit copy of the state in front of each chunk (behind it, backwards) goes to memory as it stands in shared memory, for decay_grad.
 //
-// Warp roles (640 threads): warp 0 TMA producer; warps 1 and 18 MMA issuers (A: Q K^T, P V; B: Q S, the state: issuing one costs the issuing thread about 70
-// cycles, and a chunk has 20 to 40); warps 2..5 score group (A -> P); warps 6..9 state group (state -> 16-bit copy, state times the next chunk's decay); warps
-// 14..17 output group; warp 19 the decays (64-bit sums, because neighbours' are subtracted); warps 10..13 key group: K' in place of K once A is complete, zeros over
+// Warp roles (768 threads): warp 0 TMA producer; warps 1 and 18 MMA issuers (A: Q K^T, P V; B: Q S, the state: issuing one costs the issuing thread about 70
+// cycles, and a chunk has 20 to 40); warps 2..5 score group (A -> P); warps 6..9 and 20..23 state groups, half of the columns each (state -> 16-bit copy,
+// state times the next chunk's decay); warps 14..17 output group; warp 19 the decays (64-bit sums, because neighbours' are subtracted); warps 10..13 key group: K' in place of K once A is complete, zeros over
 // the rows of padded tokens.  Per chunk the serial chain is  state MMA -> copy and decay -> next state MMA.  All waits are bounded.
 #pragma once
 
@@ -26,7 +26,7 @@
 
 namespace rfa {
 
-constexpr int kDecThreads = 640;
+constexpr int kDecThreads = 768;
 constexpr double kLog2eD = 1.4426950408889634;
 
 struct DecayTcArgs {
@@ -48,11 +48,12 @@ template <int KB, int DB, bool OUT, bool EXACT>
 struct DecLayout {
   static constexpr uint32_t kCopyBytes = KB * DB * 64 * 128;            // S's copy: DB boxes of [KB 64][64]
   static constexpr uint32_t kCopyRoom = KB == 1 ? kBox : kCopyBytes;    // an operand's second 64-block may be read past a single box
-  static constexpr uint32_t kFixed = (EXACT ? KB * kBox : 0) + kCopyRoom, kStage = (KB + DB) * kBox, kTail = 4 * 128 * 4 + 16 + 400;
+  static constexpr int kCopies = OUT ? 1 : 2;                           // one on its way to memory while the next is written
+  static constexpr uint32_t kFixed = (EXACT ? KB * kBox : 0) + kCopies * kCopyRoom, kStage = (KB + DB) * kBox, kTail = 4 * 128 * 4 + 16 + 400;
   static constexpr int fit(int extra) { return (int)((227 * 1024 - kTail - kFixed - extra) / (kStage + (OUT ? KB * kBox : 0))); }
   static constexpr int kStages = fit(0) >= 2 ? (fit(0) < kDecMaxStages ? fit(0) : kDecMaxStages) : 2, kQStages = !OUT ? 0 : fit(0) >= 2 ? kStages : 1;
   static constexpr uint32_t q = 0, k = q + kQStages * KB * kBox, v = k + kStages * KB * kBox, low = v + kStages * DB * kBox, copy = low + (EXACT ? KB * kBox : 0);
-  static constexpr uint32_t l = copy + kCopyRoom;
+  static constexpr uint32_t l = copy + kCopies * kCopyRoom;
   static constexpr uint32_t key_fac = l + 2 * 128 * 4, fac = key_fac + 2 * 128 * 4, bar = fac + 16, bytes = bar + 400;
   static constexpr int kA = OUT && DB == 1 ? 2 : 1;                     // buffers of A
   static constexpr uint32_t colS = 0, colN = DB * 64, colO = 2 * DB * 64, colA = 3 * DB * 64, cols = 512;
@@ -89,10 +90,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   if (tid == 0) {
     for (int i = 0; i < dL; ++i) mbar_init(&bars[i], OUT && (i >= dEmptyV || (i >= dEmptyQ && i < dEmptyK)) ? 2 : 1);      // both issuers read Q and V
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars[dL + i], 32); mbar_init(&bars[dLFree + i], 128);
+      mbar_init(&bars[dL + i], 32); mbar_init(&bars[dLFree + i], OUT ? 128 : 256);
       mbar_init(&bars[dA + i], 1); mbar_init(&bars[dP + i], 128); mbar_init(&bars[dKp + i], 128); mbar_init(&bars[dClean + i], 128);
     }
-    mbar_init(&bars[dS], 1); mbar_init(&bars[dSt], 128); mbar_init(&bars[dN], 2); mbar_init(&bars[dNFree], 128); mbar_init(&bars[dKept], 128);
+    mbar_init(&bars[dS], 1); mbar_init(&bars[dSt], 256); mbar_init(&bars[dN], 2); mbar_init(&bars[dNFree], 128); mbar_init(&bars[dKept], 1);
     mbar_fence_init();
     if (OUT) tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
@@ -243,15 +244,17 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         mbar_arrive(&bars[dP + ab]);
       }
     }
-  } else if (warp < 10) {
-    // ------------------------------------------------------------------ state group
+  } else if (warp < 10 || warp >= 20) {
+    // ------------------------------------------------------------------ state groups
     const int quarter = warp & 3, row = quarter * 32 + lane;      // a row of the state
+    const int col0 = warp >= 20 ? DP / 2 : 0, col1 = col0 + DP / 2;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const int64_t slot = ((int64_t)seg * BH + bh) * a.K * a.D;
-    unsigned char* copy = sm + Lay::copy;
-    // 16 numbers of the state, columns from c0 on -> the copy, and times the chunk's decay back to TMEM
-    const auto put = [&](uint32_t* r, int c0, const Factor& f) {
-      if (KP == 128 || row < KP) {
+    const bool copies = OUT || a.kept;
+    // 16 numbers of the state, columns from c0 on -> the copy of chunk c, and times the chunk's decay back to TMEM
+    const auto put = [&](uint32_t* r, int c0, int c, const Factor& f) {
+      if (copies && (KP == 128 || row < KP)) {
+        unsigned char* copy = sm + Lay::copy + (Lay::kCopies == 2 ? (c & 1) * Lay::kCopyRoom : 0);
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
           uint4 p;
@@ -266,26 +269,18 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(f.times(__uint_as_float(r[i])));
       tmem_st16(tmem + lane_addr + Lay::colS + c0, r);
     };
-    const auto keep = [&](int c) {      // the copy of chunk c to memory
-      if (a.kept && tid == 6 * 32) {
-        const int64_t chunk = chunk_t0(c) / kTC, chunks = (a.T + kTC - 1) / kTC;
-        bulk_store(static_cast<unsigned char*>(a.kept) + (bh * chunks + chunk) * Lay::kCopyBytes, copy, Lay::kCopyBytes);
-        tma_store_commit();
-      }
-    };
     bool ok = nchunk > 0;
-    uint32_t kept_phase = 0;
     if (ok && !mbar_wait(&bars[dL], 0)) { tc_fail(12); ok = false; }
     if (ok) {
       const Factor f = fac[0];
       const float* src = totals_only ? nullptr : a.nseg > 1 ? a.totals + slot : a.s_in.p ? a.s_in.p + bh * a.K * a.D : nullptr;
       const int64_t rs = a.nseg > 1 ? a.D : a.s_in.row, cs = a.nseg > 1 ? 1 : a.s_in.col;
 #pragma unroll 1
-      for (int c0 = 0; c0 < DP; c0 += 16) {
+      for (int c0 = col0; c0 < col1; c0 += 16) {
         uint32_t r[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) r[i] = src && row < a.K && c0 + i < a.D ? __float_as_uint(src[row * rs + (c0 + i) * cs]) : 0u;
-        put(r, c0, f);
+        put(r, c0, 0, f);
       }
       tmem_st_wait();
       fence_async_smem();
@@ -293,30 +288,32 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_arrive(&bars[dSt]);
     }
     for (int c = 0; ok && c < nchunk; ++c) {
-      // dSt of this chunk has all 128 arrivals, so the copy is whole
-      if (a.kept) {
-        if (!mbar_wait(&bars[dSt], c & 1)) { tc_fail(19); ok = false; break; }
-        keep(c);
+      if (!OUT && a.kept) {
+        if (tid == 6 * 32) {      // the copy of chunk c to memory, once it is whole; the one before it has then been read
+          if (!mbar_wait(&bars[dSt], c & 1)) { tc_fail(19); ok = false; break; }
+          const int64_t chunk = chunk_t0(c) / kTC, chunks = (a.T + kTC - 1) / kTC;
+          bulk_store(static_cast<unsigned char*>(a.kept) + (bh * chunks + chunk) * Lay::kCopyBytes, sm + Lay::copy + (c & 1) * Lay::kCopyRoom, Lay::kCopyBytes);
+          tma_store_commit();
+          tma_store_wait_read<1>();
+          mbar_arrive(&bars[dKept]);
+        }
+        if (!mbar_wait(&bars[dKept], c & 1)) { tc_fail(20); ok = false; break; }
       }
       if (!mbar_wait(&bars[dS], c & 1)) { tc_fail(13); ok = false; break; }
       tc_fence_after_sync();
       if (c + 1 < nchunk) {
         if (!mbar_wait(&bars[dL + ((c + 1) & 1)], ((c + 1) >> 1) & 1)) { tc_fail(14); ok = false; break; }
-        if (a.kept) {      // the copy's way to memory has read it
-          if (tid == 6 * 32) tma_store_wait_read<0>();
-          if (!epi_sync(&bars[dKept], kept_phase)) { tc_fail(20); ok = false; break; }
-        }
         const Factor f = fac[(c + 1) & 1];
         uint32_t next[16];
-        tmem_ld16(tmem + lane_addr + Lay::colS, next);
+        tmem_ld16(tmem + lane_addr + Lay::colS + col0, next);
 #pragma unroll 1
-        for (int c0 = 0; c0 < DP; c0 += 16) {
+        for (int c0 = col0; c0 < col1; c0 += 16) {
           uint32_t r[16];
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 16; ++i) r[i] = next[i];
-          if (c0 + 16 < DP) tmem_ld16(tmem + lane_addr + Lay::colS + c0 + 16, next);
-          put(r, c0, f);
+          if (c0 + 16 < col1) tmem_ld16(tmem + lane_addr + Lay::colS + c0 + 16, next);
+          put(r, c0, c + 1, f);
         }
         tmem_st_wait();
         fence_async_smem();
@@ -330,7 +327,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (dst) {
       const int64_t rs = totals_only ? a.D : a.s_out.row, cs = totals_only ? 1 : a.s_out.col;
 #pragma unroll 1
-      for (int c0 = 0; c0 < DP; c0 += 16) {
+      for (int c0 = col0; c0 < col1; c0 += 16) {
         uint32_t r[16];
         tmem_ld16(tmem + lane_addr + Lay::colS + c0, r);
         tmem_ld_wait();
