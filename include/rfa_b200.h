@@ -522,8 +522,8 @@ int rfa_group_norm_bwd(const rfa_group_norm_t* norm, const void* g, int64_t g_r,
  * states, sums and softmax statistics are fp32.  mask [B, T] bytes or NULL, non-zero
  * = a padded token: every result of the others is what it would be if padded tokens
  * were not there, whatever stands in them, and a padded token's outputs and
- * gradients are zero.  States, caches and workspaces are 16-byte aligned, else no
- * alignment is asked for.  Heads of at most 256; T < 2^31 - 256, B and H <= 65535,
+ * gradients are zero.  States, caches, outputs and workspaces are 16-byte aligned, else
+ * no alignment is asked for.  Heads of at most 256; T < 2^31 - 256, B and H <= 65535,
  * B H < 2^24; a size of zero is refused.  Outputs overlap neither inputs nor each
  * other, but for states and caches where that is said.  What a batch row holds reaches
  * no other row's results; the same call gives the same bits.
@@ -547,12 +547,15 @@ typedef struct {
   float scale;
 } rfa_decay_t;
 size_t rfa_decay_workspace_bytes(int64_t T, int B, int H, int K, int D, int dtype, int backward);
-/* s_out: the last state, or NULL; it may be s_in. */
-int rfa_decay_fwd(const rfa_decay_t* decay, void* out, float* s_out,
+/* s_out: the last state, or NULL; it may be s_in.  kept: rfa_decay_kept_bytes(decay) bytes
+ * that a backward with the same `decay` goes on from, or NULL. */
+size_t rfa_decay_kept_bytes(const rfa_decay_t* decay);
+int rfa_decay_fwd(const rfa_decay_t* decay, void* out, float* s_out, void* kept,
                   void* workspace, size_t workspace_bytes, rfa_stream_t stream);
-/* g [T, B, H, D] contiguous, g_s [B, H, K, D] of the last state or NULL -> gq, gk, gv;
- * g_decay of decay_dtype and gs_in [B, H, K, D], each or NULL. */
-int rfa_decay_bwd(const rfa_decay_t* decay, const void* g, const float* g_s, void* gq,
+/* g [T, B, H, D] contiguous, g_s [B, H, K, D] of the last state or NULL, the forward's
+ * kept or NULL (it is then computed again) -> gq, gk, gv; g_decay of decay_dtype and gs_in
+ * [B, H, K, D], each or NULL. */
+int rfa_decay_bwd(const rfa_decay_t* decay, const void* g, const float* g_s, const void* kept, void* gq,
                   void* gk, void* gv, void* g_decay, float* gs_in,
                   void* workspace, size_t workspace_bytes, rfa_stream_t stream);
 /* One token (T = 1): the state s is updated in place (s_in is not read). */

@@ -74,8 +74,9 @@ SIGNATURES = {
     "rfa_group_norm_workspace_bytes": (_sz, [_i64, _int, _int]),
     "rfa_group_norm_bwd": (_int, [_vp, _vp, _i64] + [_vp] * 5 + [_sz, _vp]),
     "rfa_decay_workspace_bytes": (_sz, [_i64] + [_int] * 6),
-    "rfa_decay_fwd": (_int, [_vp] * 4 + [_sz, _vp]),
-    "rfa_decay_bwd": (_int, [_vp] * 9 + [_sz, _vp]),
+    "rfa_decay_kept_bytes": (_sz, [_vp]),
+    "rfa_decay_fwd": (_int, [_vp] * 5 + [_sz, _vp]),
+    "rfa_decay_bwd": (_int, [_vp] * 10 + [_sz, _vp]),
     "rfa_decay_step": (_int, [_vp] * 4),
     "rfa_window_workspace_bytes": (_sz, [_i64] + [_int] * 8),
     "rfa_window_fwd": (_int, [_vp] * 4 + [_sz, _vp]),

@@ -69,14 +69,21 @@ extern "C" size_t rfa_decay_workspace_bytes(int64_t T, int B, int H, int K, int 
   return most;
 }
 
-extern "C" int rfa_decay_fwd(const rfa_decay_t* c, void* out, float* s_out, void* workspace, size_t workspace_bytes, rfa_stream_t stream) {
+extern "C" size_t rfa_decay_kept_bytes(const rfa_decay_t* c) {
+  using namespace rfa;
+  if (!c || c->T <= 0 || c->B <= 0 || c->H <= 0 || c->K <= 0 || c->D <= 0 || !decay_tc_ok(*c)) return 0;
+  return decay_tc_kept_bytes(c->T, (int64_t)c->B * c->H, c->K, c->D);
+}
+
+extern "C" int rfa_decay_fwd(const rfa_decay_t* c, void* out, float* s_out, void* kept, void* workspace, size_t workspace_bytes, rfa_stream_t stream) {
   using namespace rfa;
   if (int r = decay_check(c, "decay_fwd")) return r;
   RFA_REQUIRE(out, RFA_EINVAL, "decay_fwd: null pointer");
-  RFA_REQUIRE(aligned16(s_out) && aligned16(workspace), RFA_EALIGN, "decay_fwd: s_out or workspace is not 16-byte aligned");
+  RFA_REQUIRE(aligned16(s_out) && aligned16(kept) && aligned16(workspace), RFA_EALIGN, "decay_fwd: s_out, kept or workspace is not 16-byte aligned");
   const size_t need = rfa_decay_workspace_bytes(c->T, c->B, c->H, c->K, c->D, c->dtype, 0);
   RFA_REQUIRE(!need || (workspace && workspace_bytes >= need), RFA_EWORKSPACE, "decay_fwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
-  if (decay_tc_ok(*c) && aligned16(out)) return launch_decay_tc(*c, decay_tc_plan(c->T, (int64_t)c->B * c->H, c->K, c->D), static_cast<char*>(workspace), out, s_out, as_stream(stream));
+  RFA_REQUIRE(!decay_tc_ok(*c) || aligned16(out), RFA_EALIGN, "decay_fwd: out is not 16-byte aligned");
+  if (decay_tc_ok(*c)) return launch_decay_tc(*c, decay_tc_plan(c->T, (int64_t)c->B * c->H, c->K, c->D), static_cast<char*>(workspace), out, s_out, kept, as_stream(stream));
   const SweepPlan plan = sweep_plan(c->T, (int64_t)c->B * c->H, sweep_tiles(c->D), 1, c->K, c->D);
   SweepBatch batch{};
   batch.count = 1;
@@ -91,17 +98,18 @@ extern "C" int rfa_decay_fwd(const rfa_decay_t* c, void* out, float* s_out, void
   return launch_sweeps(batch, plan, as_stream(stream));
 }
 
-extern "C" int rfa_decay_bwd(const rfa_decay_t* c, const void* g, const float* g_s, void* gq, void* gk, void* gv, void* g_decay, float* gs_in, void* workspace,
+extern "C" int rfa_decay_bwd(const rfa_decay_t* c, const void* g, const float* g_s, const void* kept, void* gq, void* gk, void* gv, void* g_decay, float* gs_in, void* workspace,
                              size_t workspace_bytes, rfa_stream_t stream) {
   using namespace rfa;
   if (int r = decay_check(c, "decay_bwd")) return r;
   RFA_REQUIRE(g && gq && gk && gv, RFA_EINVAL, "decay_bwd: null pointer");
-  RFA_REQUIRE(aligned16(g_s) && aligned16(gs_in) && aligned16(workspace), RFA_EALIGN, "decay_bwd: g_s, gs_in or workspace is not 16-byte aligned");
+  RFA_REQUIRE(aligned16(g_s) && aligned16(gs_in) && aligned16(kept) && aligned16(workspace), RFA_EALIGN, "decay_bwd: g_s, gs_in, kept or workspace is not 16-byte aligned");
   const size_t need = bwd_bytes(*c);
   RFA_REQUIRE(workspace && workspace_bytes >= need, RFA_EWORKSPACE, "decay_bwd: workspace %zu bytes, %zu needed", workspace_bytes, need);
   const cudaStream_t st = as_stream(stream);
-  if (decay_tc_ok(*c) && aligned16(g) && aligned16(gq) && aligned16(gk) && aligned16(gv))
-    return launch_decay_tc_bwd(*c, static_cast<char*>(workspace), g, g_s, gq, gk, gv, g_decay, gs_in, st);
+  if (decay_tc_ok(*c)) RFA_REQUIRE(aligned16(g) && aligned16(gq) && aligned16(gk) && aligned16(gv), RFA_EALIGN, "decay_bwd: g or a gradient is not 16-byte aligned");
+  if (decay_tc_ok(*c))
+    return launch_decay_tc_bwd(*c, static_cast<char*>(workspace), kept, g, g_s, gq, gk, gv, g_decay, gs_in, st);
   const BwdPlan plan(*c);
   char *ws = static_cast<char*>(workspace), *rest = ws + plan.sweep();
   float* q_dots = reinterpret_cast<float*>(rest);

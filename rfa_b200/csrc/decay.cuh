@@ -61,9 +61,10 @@ int launch_decay_grad(const float* q_dots, int q_tiles, const float* k_dots, int
 // decay_tc.cu: fp16 and bf16, heads of up to 128 in rows that a tensor map can describe
 bool decay_tc_ok(const rfa_decay_t& c);
 SweepPlan decay_tc_plan(int64_t T, int64_t BH, int K, int D);
-int launch_decay_tc(const rfa_decay_t& c, const SweepPlan& plan, char* workspace, void* out, float* s_out, cudaStream_t stream);
+int launch_decay_tc(const rfa_decay_t& c, const SweepPlan& plan, char* workspace, void* out, float* s_out, void* kept, cudaStream_t stream);
+size_t decay_tc_kept_bytes(int64_t T, int64_t BH, int K, int D);      // what a forward pass leaves for the backward
 size_t decay_tc_bwd_bytes(const rfa_decay_t& c);
-int launch_decay_tc_bwd(const rfa_decay_t& c, char* workspace, const void* g, const float* g_s, void* gq, void* gk, void* gv, void* g_decay, float* gs_in, cudaStream_t stream);
+int launch_decay_tc_bwd(const rfa_decay_t& c, char* workspace, const void* kept, const void* g, const float* g_s, void* gq, void* gk, void* gv, void* g_decay, float* gs_in, cudaStream_t stream);
 
 int launch_decay_step(const rfa_decay_t& c, void* out, float* s, cudaStream_t stream);      // decay_step.cu
 

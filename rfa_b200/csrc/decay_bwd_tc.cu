@@ -1,19 +1,22 @@
 // Linear attention with a decay on the tensor cores: the gradients of a chunk, fp16 and bf16, heads of up to 128.
 //
 // The states in front of each chunk (S) and their gradients behind it (dS, scaled) have been left by two sweeps of decay_tc.cuh as 16-bit tiles.  Then
-// the chunks do not depend on each other, and one CTA takes one chunk of 128 tokens of a (batch row, head).  With w_ij = scale 2^(L_i - L_j), j <= i:
+// the chunks do not depend on each other, and a CTA takes one chunk of 128 tokens of a (batch row, head) after the other.  With w_ij = scale 2^(L_i - L_j), j <= i:
 //     T0 = Q K^T, T1 = G V^T          -> P = T0 o w, D = T1 o w      16 bits, in shared memory
 //     gq_i = (D K)_i + scale 2^(L_i) (G S^T)_i
 //     gk_j = (D^T Q)_j + 2^(L_end - L_j) (V dS^T)_j
 //     gv_j = (P^T G)_j + 2^(L_end - L_j) (K dS)_j
-// The gradient of the log decay at t is the sum over all pairs of a query i >= t and a key j < t: with M = T0 o T1 o w in fp32
-//     g_t = sum_(i >= t) (rows of M + scale 2^(L_i) q_i . (G S^T)_i) - sum_(j >= t) columns of M + sum_(j < t) 2^(L_end - L_j) k_j . (V dS^T)_j + 2^(L_end) S . dS
-// in which only the rows and columns of one and the same M are subtracted from each other.
+// The gradient of the log decay at t is the sum over all pairs of a query i >= t and a key j < t.  With D as it is rounded, M_ij = D_ij q_i . k_j: its rows' sums are
+// q_i . (D K)_i and its columns' k_j . (D^T Q)_j, both in fp32 and of one and the same matrix, so that little more than fp32's roundings is left of pairs that
+// do not straddle t when they are subtracted:
+//     g_t = sum_(i >= t) q_i . gq_i - sum_(j >= t) k_j . (D^T Q)_j + sum_(j < t) 2^(L_end - L_j) k_j . (V dS^T)_j + 2^(L_end) S . dS
 //
 // Warp roles (608 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 the decays, warps 3..18 four groups that share the rows' columns 16 by 16: clear padded
 // rows, T0, T1 -> P, D, then the gradients straight from registers.  P takes the place of S.  TMEM: four regions of 128 columns, T0 / T1 / G S^T / V dS^T, the first three
 // of them used again.  All waits are bounded.
 #define RFA_TC_FAMILY 11
+#include <algorithm>
+
 #include "decay_tc.cuh"
 
 namespace rfa {
@@ -35,29 +38,42 @@ template <int KB, int DB>
 struct GradLayout {
   static constexpr uint32_t kCopyBytes = KB * DB * 64 * 128;
   static constexpr uint32_t q = 0, k = KB * kBox, v = 2 * KB * kBox, g = v + DB * kBox, s = g + DB * kBox;      // s: S, then P [128][128]
-  static constexpr uint32_t d = s + 2 * kBox, ds = d + 2 * kBox, l = ds + (kCopyBytes + 1023) / 1024 * 1024, col = l + 128 * 4, bar = col + 4 * 128 * 4, bytes = bar + 160;
+  static constexpr uint32_t d = s + 2 * kBox, ds = d + 2 * kBox, l = ds + (kCopyBytes + 1023) / 1024 * 1024, bar = l + 128 * 4, bytes = bar + 160;
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
-enum { gQK = 0, gVG, gS, gDS, gL, gClean, gT, gN1, gN2, gX, gP, gO1, gO2, gE1, gO3, gAll, gSum, gNum };
+enum { gQK = 0, gVG, gS, gDS, gL, gClean, gT, gN1, gN2, gX, gP, gO1, gO2, gE1, gE2, gO3, gE3, gAll, gSum, gNum };
+// Each but gSum completes once a chunk, so that a chunk's parity is every wait's.  gE1, gE2, gE3: gq, gk and gv have been read, with the rows of Q and K.
 
 template <typename T, int KB, int DB>
 __global__ void __launch_bounds__(kDgThreads, 1)
 decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                     const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ DecayGradArgs a) {
+                     const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ DecayGradArgs a, int64_t works) {
   using Lay = GradLayout<KB, DB>;
   constexpr int KP = KB * 64, DP = DB * 64;
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::bar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + gNum);
   float* L = reinterpret_cast<float*>(sm + Lay::l);
-  float* cols = reinterpret_cast<float*>(sm + Lay::col);      // columns of M, summed over the rows of each warp
   const uint32_t sbase = smem_u32(sm);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t chunks = (a.T + kTC - 1) / kTC, bh = blockIdx.x / chunks, chunk = blockIdx.x % chunks, t0 = chunk * kTC;
-  const int b = (int)(bh / a.H), h = (int)(bh % a.H);
-  const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.T : nullptr;
+  const int64_t chunks = (a.T + kTC - 1) / kTC;
+  struct Work {
+    int64_t bh, chunk, t0;
+    int b, h;
+    const uint8_t* mask;
+  };
+  const auto work_of = [&](int64_t w) {
+    Work k;
+    k.bh = w / chunks;
+    k.chunk = w % chunks;
+    k.t0 = k.chunk * kTC;
+    k.b = (int)(k.bh / a.H);
+    k.h = (int)(k.bh % a.H);
+    k.mask = a.mask ? a.mask + (int64_t)k.b * a.T : nullptr;
+    return k;
+  };
   if (tid == 0) {
-    for (int i = 0; i < gNum; ++i) mbar_init(&bars[i], i == gL ? 32 : i == gClean || i == gX || i == gP || i == gE1 || i == gAll ? kDgRows : i == gSum ? 128 : 1);
+    for (int i = 0; i < gNum; ++i) mbar_init(&bars[i], i == gL ? 32 : i == gClean || i == gX || i == gP || (i >= gE1 && i <= gE3 && i != gO3) || i == gAll ? kDgRows : i == gSum ? 128 : 1);
     mbar_fence_init();
     tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v); tma_prefetch_desc(&tm_g);
   }
@@ -72,17 +88,38 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      mbar_arrive_expect_tx(&bars[gQK], 2 * KB * kBox);
-      for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::q + x * kBox, &tm_q, &bars[gQK], x * 64, h, b, (int)t0);
-      for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::k + x * kBox, &tm_k, &bars[gQK], x * 64, h, b, (int)t0);
-      mbar_arrive_expect_tx(&bars[gVG], 2 * DB * kBox);
-      for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::g + x * kBox, &tm_g, &bars[gVG], x * 64, h, b, (int)t0);
-      for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + x * kBox, &tm_v, &bars[gVG], x * 64, h, b, (int)t0);
-      const int64_t at = (bh * chunks + chunk) * Lay::kCopyBytes;
-      mbar_arrive_expect_tx(&bars[gS], Lay::kCopyBytes);
-      bulk_load(sm + Lay::s, static_cast<const unsigned char*>(a.states) + at, Lay::kCopyBytes, &bars[gS]);
-      mbar_arrive_expect_tx(&bars[gDS], Lay::kCopyBytes);
-      bulk_load(sm + Lay::ds, static_cast<const unsigned char*>(a.grads) + at, Lay::kCopyBytes, &bars[gDS]);
+      uint32_t ph = 0;
+      for (int64_t w = blockIdx.x; w < works; w += gridDim.x, ph ^= 1) {
+        const Work k = work_of(w);
+        const int t0 = (int)k.t0;
+        if (w != blockIdx.x && (!mbar_wait(&bars[gE2], ph ^ 1) || !mbar_wait(&bars[gO3], ph ^ 1))) { tc_fail(1); break; }
+        mbar_arrive_expect_tx(&bars[gQK], 2 * KB * kBox);
+        for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::q + x * kBox, &tm_q, &bars[gQK], x * 64, k.h, k.b, t0);
+        for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::k + x * kBox, &tm_k, &bars[gQK], x * 64, k.h, k.b, t0);
+        mbar_arrive_expect_tx(&bars[gVG], 2 * DB * kBox);
+        for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::g + x * kBox, &tm_g, &bars[gVG], x * 64, k.h, k.b, t0);
+        for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + x * kBox, &tm_v, &bars[gVG], x * 64, k.h, k.b, t0);
+        const int64_t at = (k.bh * chunks + k.chunk) * Lay::kCopyBytes;
+        mbar_arrive_expect_tx(&bars[gS], Lay::kCopyBytes);
+        bulk_load(sm + Lay::s, static_cast<const unsigned char*>(a.states) + at, Lay::kCopyBytes, &bars[gS]);
+        mbar_arrive_expect_tx(&bars[gDS], Lay::kCopyBytes);
+        bulk_load(sm + Lay::ds, static_cast<const unsigned char*>(a.grads) + at, Lay::kCopyBytes, &bars[gDS]);
+        if (!mbar_wait(&bars[gDS], ph)) { tc_fail(20); break; }
+        if (w + gridDim.x < works) {      // the next chunk on its way to L2 while this one, which has come, is worked on: its tiles have no room here yet
+          const Work n = work_of(w + gridDim.x);
+          for (int x = 0; x < KB; ++x) {
+            tma_prefetch_4d(&tm_q, x * 64, n.h, n.b, (int)n.t0);
+            tma_prefetch_4d(&tm_k, x * 64, n.h, n.b, (int)n.t0);
+          }
+          for (int x = 0; x < DB; ++x) {
+            tma_prefetch_4d(&tm_g, x * 64, n.h, n.b, (int)n.t0);
+            tma_prefetch_4d(&tm_v, x * 64, n.h, n.b, (int)n.t0);
+          }
+          const int64_t at = (n.bh * chunks + n.chunk) * Lay::kCopyBytes;
+          bulk_prefetch(static_cast<const unsigned char*>(a.states) + at, Lay::kCopyBytes);
+          bulk_prefetch(static_cast<const unsigned char*>(a.grads) + at, Lay::kCopyBytes);
+        }
+      }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
@@ -96,64 +133,85 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       const auto rows = [&](uint32_t at) { return umma_smem_desc(sbase + at, 0, 1024, kSwizzle128B); };                 // K-major
       const auto columns = [&](uint32_t at, uint32_t block) { return umma_smem_desc(sbase + at, block, 1024, kSwizzle128B); };      // MN-major
       const uint32_t R0 = tmem, R1 = tmem + 128, R2 = tmem + 256, R3 = tmem + 384;
-      do {
-        if (mask && !mbar_wait(&bars[gClean], 0)) { tc_fail(1); break; }
-        if (!mbar_wait(&bars[gQK], 0)) { tc_fail(2); break; }
+      uint32_t ph = 0;
+      for (int64_t w = blockIdx.x; w < works; w += gridDim.x, ph ^= 1) {
+        if (w != blockIdx.x && !mbar_wait(&bars[gE3], ph ^ 1)) { tc_fail(18); break; }
+        if (a.mask && !mbar_wait(&bars[gClean], ph)) { tc_fail(1); break; }
+        if (!mbar_wait(&bars[gQK], ph)) { tc_fail(2); break; }
         tc_fence_after_sync();
         umma_chain_ss<4 * KB, kStepK, kBlockK, kStepK, kBlockK>(lead, R0, rows(Lay::q), rows(Lay::k), idT, 0);
-        if (!mbar_wait(&bars[gVG], 0)) { tc_fail(3); break; }
+        if (!mbar_wait(&bars[gVG], ph)) { tc_fail(3); break; }
         umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockK>(lead, R1, rows(Lay::g), rows(Lay::v), idT, 0);
         umma_commit(&bars[gT]);
-        if (!mbar_wait(&bars[gS], 0)) { tc_fail(4); break; }
+        if (!mbar_wait(&bars[gS], ph)) { tc_fail(4); break; }
         umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kCopyBlock>(lead, R2, rows(Lay::g), rows(Lay::s), idKK, 0);
         umma_commit(&bars[gN1]);
-        if (!mbar_wait(&bars[gDS], 0)) { tc_fail(5); break; }
+        if (!mbar_wait(&bars[gDS], ph)) { tc_fail(5); break; }
         umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kCopyBlock>(lead, R3, rows(Lay::v), rows(Lay::ds), idKK, 0);
         umma_commit(&bars[gN2]);
-        if (!mbar_wait(&bars[gP], 0)) { tc_fail(6); break; }
+        if (!mbar_wait(&bars[gP], ph)) { tc_fail(6); break; }
         tc_fence_after_sync();
         umma_chain_ss<8, kStepK, kBlockK, kStepMN, kBlockMN>(lead, R0, rows(Lay::d), columns(Lay::k, kBox), idK, 0);
         umma_commit(&bars[gO1]);
         umma_chain_ss<8, kStepMN, kBlockMN, kStepMN, kBlockMN>(lead, R1, columns(Lay::d, kBox), columns(Lay::q, kBox), idTK, 0);
         umma_commit(&bars[gO2]);
-        if (!mbar_wait(&bars[gE1], 0)) { tc_fail(7); break; }
+        if (!mbar_wait(&bars[gE1], ph)) { tc_fail(7); break; }
         tc_fence_after_sync();
         umma_chain_ss<8, kStepMN, kBlockMN, kStepMN, kBlockMN>(lead, R0, columns(Lay::s, kBox), columns(Lay::g, kBox), idTD, 0);
         umma_chain_ss<4 * KB, kStepK, kBlockK, kStepMN, kBlockMN>(lead, R2, rows(Lay::k), columns(Lay::ds, KP * 128), idD, 0);
         umma_commit(&bars[gO3]);
-      } while (false);
+      }
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ decays: a lane takes four adjacent tokens
-    double sum[4], all = 0.0;
+    // Sums of 40 bits behind the point: as exact as 64-bit floats' for this and several times as fast
+    uint32_t ph = 0;
+    for (int64_t w = blockIdx.x; w < works; w += gridDim.x, ph ^= 1) {
+      const Work k = work_of(w);
+      uint32_t bits[4];
+      bool real[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t t = t0 + lane * 4 + e;
-      if (t < a.T && !(mask && mask[t])) all += fmax(log_decay_at(a.decay.p, a.decay_dtype, b * a.decay.b + h * a.decay.h + t * a.decay.t) * kLog2eD, -64.0);
-      sum[e] = all;
+      for (int e = 0; e < 4; ++e) {
+        const int64_t t = k.t0 + lane * 4 + e;
+        real[e] = t < a.T;
+        bits[e] = real[e] ? log_decay_bits(a.decay.p, a.decay_dtype, k.b * a.decay.b + k.h * a.decay.h + t * a.decay.t) : 0u;
+        if (real[e] && k.mask) real[e] = !k.mask[t];
+      }
+      long long sum[4], all = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (real[e]) all += __double2ll_rn(fmax(log_decay_of(bits[e], a.decay_dtype) * kLog2eD, -64.0) * 1099511627776.0);
+        sum[e] = all;
+      }
+      long long before = all;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += up;
+      }
+      before -= all;
+      if (w != blockIdx.x && !mbar_wait(&bars[gP], ph ^ 1)) { tc_fail(19); break; }      // the last chunk's have been read
+#pragma unroll
+      for (int e = 0; e < 4; ++e) L[lane * 4 + e] = __ll2float_rn(sum[e] + before) * 0x1p-40f;
+      mbar_arrive(&bars[gL]);
     }
-    double before = all;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += up;
-    }
-    before -= all;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) L[lane * 4 + e] = (float)(sum[e] + before);
-    mbar_arrive(&bars[gL]);
   } else {
     // ------------------------------------------------------------------ four groups of 128: rows of the chunk, every fourth 16 columns
     const int group = (warp - 3) >> 2, quarter = warp & 3, row = quarter * 32 + lane, wtid = tid - 96;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const uint32_t R0 = tmem + lane_addr, R1 = R0 + 128, R2 = R0 + 256, R3 = R0 + 384;
-    const int64_t t = t0 + row;
-    const bool there = t < a.T;
     const bool want = a.g_decay != nullptr;
-    float x = 0.f, rows_sum = 0.f, keys_sum = 0.f;      // S . dS; rows of M and q . (G S^T); k . (V dS^T)
-    do {
+    const auto sectors = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; };
+    const bool wide_q = a.K % 16 == 0 && sectors(a.gq), wide_k = a.K % 16 == 0 && sectors(a.gk), wide_d = a.D % 16 == 0 && sectors(a.gv);
+    uint32_t ph = 0, sum_phase = 0;
+    for (int64_t w = blockIdx.x; w < works; w += gridDim.x, ph ^= 1) {
+      const Work k = work_of(w);
+      const uint8_t* mask = k.mask;
+      const int64_t t = k.t0 + row;
+      const bool there = t < a.T;
+      float x = 0.f, rows_sum = 0.f, cols_sum = 0.f, keys_sum = 0.f;      // S . dS; q . gq; k . (D^T Q); k . (V dS^T)
       if (mask) {      // padded rows may hold anything: zero before a product reads them
-        if (!mbar_wait(&bars[gQK], 0) || !mbar_wait(&bars[gVG], 0)) { tc_fail(8); break; }
+        if (!mbar_wait(&bars[gQK], ph) || !mbar_wait(&bars[gVG], ph)) { tc_fail(8); break; }
         if (there && mask[t]) {
           const uint4 zero = make_uint4(0, 0, 0, 0);
           if (group == 0) {
@@ -173,7 +231,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         fence_async_smem();
         mbar_arrive(&bars[gClean]);
       }
-      if (!mbar_wait(&bars[gS], 0) || !mbar_wait(&bars[gDS], 0)) { tc_fail(9); break; }
+      if (!mbar_wait(&bars[gS], ph) || !mbar_wait(&bars[gDS], ph)) { tc_fail(9); break; }
       if (want) {
 #pragma unroll 1
         for (uint32_t i = wtid * 16; i < Lay::kCopyBytes; i += kDgRows * 16) {
@@ -187,9 +245,9 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
       }
       mbar_release_stage(&bars[gX]);      // S has been read
-      if (!mbar_wait(&bars[gX], 0) || !mbar_wait(&bars[gL], 0)) { tc_fail(10); break; }
+      if (!mbar_wait(&bars[gX], ph) || !mbar_wait(&bars[gL], ph)) { tc_fail(10); break; }
       const float mine = L[row], end = L[127];
-      if (!mbar_wait(&bars[gT], 0) || !mbar_wait(&bars[gN1], 0)) { tc_fail(11); break; }
+      if (!mbar_wait(&bars[gT], ph) || !mbar_wait(&bars[gN1], ph)) { tc_fail(11); break; }
       tc_fence_after_sync();
       const int pieces = 2 * quarter + 2;      // of 16 columns, that reach up to the diagonal
 #pragma unroll 1
@@ -197,62 +255,42 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         uint32_t pw[8], dw[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) pw[i] = dw[i] = 0u;
-        float m[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m[i] = 0.f;
         if (p < pieces) {
           uint32_t s0[16], s1[16];
           tmem_ld16(R0 + p * 16, s0);
           tmem_ld16(R1 + p * 16, s1);
-          float w[16];
-          const int last = row - p * 16;
+          float f[16];
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
             const float4 l = *reinterpret_cast<const float4*>(L + p * 16 + i);
-            w[i] = ex2(mine - l.x); w[i + 1] = ex2(mine - l.y); w[i + 2] = ex2(mine - l.z); w[i + 3] = ex2(mine - l.w);
+            f[i] = a.scale * ex2(mine - l.x); f[i + 1] = a.scale * ex2(mine - l.y); f[i + 2] = a.scale * ex2(mine - l.z); f[i + 3] = a.scale * ex2(mine - l.w);
+          }
+          if (p >= 2 * quarter) {      // the diagonal's
+            const int last = row - p * 16;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (i > last) f[i] = 0.f;
           }
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            float f0 = i <= last ? a.scale * w[i] : 0.f, f1 = i + 1 <= last ? a.scale * w[i + 1] : 0.f;
-            const float p0 = __uint_as_float(s0[i]) * f0, p1 = __uint_as_float(s0[i + 1]) * f1;
-            pw[i >> 1] = pack2h<T>(p0, p1);
-            dw[i >> 1] = pack2h<T>(__uint_as_float(s1[i]) * f0, __uint_as_float(s1[i + 1]) * f1);
-            m[i] = p0 * __uint_as_float(s1[i]);
-            m[i + 1] = p1 * __uint_as_float(s1[i + 1]);
+            pw[i >> 1] = pack2h<T>(__uint_as_float(s0[i]) * f[i], __uint_as_float(s0[i + 1]) * f[i + 1]);
+            dw[i >> 1] = pack2h<T>(__uint_as_float(s1[i]) * f[i], __uint_as_float(s1[i + 1]) * f[i + 1]);
           }
         }
         *reinterpret_cast<uint4*>(sm + Lay::s + row_chunk2(row, 2 * p)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
         *reinterpret_cast<uint4*>(sm + Lay::s + row_chunk2(row, 2 * p + 1)) = make_uint4(pw[4], pw[5], pw[6], pw[7]);
         *reinterpret_cast<uint4*>(sm + Lay::d + row_chunk2(row, 2 * p)) = make_uint4(dw[0], dw[1], dw[2], dw[3]);
         *reinterpret_cast<uint4*>(sm + Lay::d + row_chunk2(row, 2 * p + 1)) = make_uint4(dw[4], dw[5], dw[6], dw[7]);
-        if (want) {      // sums of the warp's rows: each step halves the columns that a lane has
-#pragma unroll
-          for (int i = 0; i < 16; ++i) rows_sum += m[i];
-#pragma unroll
-          for (int o = 16, n = 8; o >= 2; o >>= 1, n >>= 1) {
-            const bool up = lane & o;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (i < n) {
-                const float give = up ? m[i] : m[i + n];
-                m[i] = (up ? m[i + n] : m[i]) + __shfl_xor_sync(0xffffffffu, give, o);
-              }
-          }
-          m[0] += __shfl_xor_sync(0xffffffffu, m[0], 1);
-          if (!(lane & 1)) cols[quarter * 128 + p * 16 + (lane >> 1)] = m[0];
-        }
       }
       fence_async_smem();
       tc_fence_before_sync();
       mbar_arrive(&bars[gP]);
 
-      const auto sectors = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; };
-      const bool wide_q = a.K % 16 == 0 && sectors(a.gq), wide_k = a.K % 16 == 0 && sectors(a.gk), wide_d = a.D % 16 == 0 && sectors(a.gv);
       const float fq = a.scale * ex2(mine), fk = ex2(end - mine);
-      const int64_t at = (t * a.B + b) * a.H + h;
+      const int64_t at = (t * a.B + k.b) * a.H + k.h;
       // ---- gq, gk
-      const auto grad = [&](uint32_t main, uint32_t side, float f, void* out, uint32_t tile, float& sum, bool wide) {
+      const auto grad = [&](uint32_t main, uint32_t side, float f, void* out, uint32_t tile, float& own, float& across, bool wide) {
         T* o = static_cast<T*>(out) + at * a.K;
 #pragma unroll 1
         for (int c0 = group * 16; c0 < KP; c0 += kDgGroups * 16) {
@@ -276,22 +314,24 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float2 z = unpack2h<T>(ys[e]);
-                sum = fmaf(__uint_as_float(n[8 * ch + 2 * e]), z.x, fmaf(__uint_as_float(n[8 * ch + 2 * e + 1]), z.y, sum));
+                own = fmaf(__uint_as_float(u[8 * ch + 2 * e]), z.x, fmaf(__uint_as_float(u[8 * ch + 2 * e + 1]), z.y, own));
+                across = fmaf(__uint_as_float(n[8 * ch + 2 * e]), z.x, fmaf(__uint_as_float(n[8 * ch + 2 * e + 1]), z.y, across));
               }
             }
           }
         }
       };
-      if (!mbar_wait(&bars[gO1], 0)) { tc_fail(12); break; }
+      if (!mbar_wait(&bars[gO1], ph)) { tc_fail(12); break; }
       tc_fence_after_sync();
-      grad(R0, R2, fq, a.gq, Lay::q, rows_sum, wide_q);
+      grad(R0, R2, fq, a.gq, Lay::q, rows_sum, rows_sum, wide_q);
       tc_fence_before_sync();
       mbar_arrive(&bars[gE1]);
-      if (!mbar_wait(&bars[gN2], 0) || !mbar_wait(&bars[gO2], 0)) { tc_fail(13); break; }
+      if (!mbar_wait(&bars[gN2], ph) || !mbar_wait(&bars[gO2], ph)) { tc_fail(13); break; }
       tc_fence_after_sync();
-      grad(R1, R3, fk, a.gk, Lay::k, keys_sum, wide_k);
+      grad(R1, R3, fk, a.gk, Lay::k, cols_sum, keys_sum, wide_k);
+      mbar_release_stage(&bars[gE2]);
       // ---- gv
-      if (!mbar_wait(&bars[gO3], 0)) { tc_fail(14); break; }
+      if (!mbar_wait(&bars[gO3], ph)) { tc_fail(14); break; }
       tc_fence_after_sync();
       T* o = static_cast<T*>(a.gv) + at * a.D;
 #pragma unroll 1
@@ -305,22 +345,24 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         for (int i = 0; i < 16; ++i) v[i] = fmaf(fk, __uint_as_float(n[i]), __uint_as_float(u[i]));
         if (there && c0 < a.D) store_row16(o + c0, v, a.D - c0, wide_d);
       }
-      // ---- the decays: everything that was read of the tiles has been (gO3), so that P's place serves the exchange
+      tc_fence_before_sync();
+      mbar_arrive(&bars[gE3]);
+      // ---- the decays: D has been read by its products (gO1, gO2), so that its place serves the exchange
       if (want) {
-        // P's place: [group][128] rows, [group][128] keys of the other groups, a sum of S . dS for each warp, the first group's warps' sums
-        float* ex = reinterpret_cast<float*>(sm + Lay::s);
+        // [group][128] rows less columns, [group][128] keys of the other groups, a sum of S . dS for each warp, the first group's warps' sums
+        float* ex = reinterpret_cast<float*>(sm + Lay::d);
         float *ex_x = ex + 2 * kDgRows, *ex_down = ex_x + 16, *ex_up = ex_down + 4, *ex_all = ex_up + 4;
         x = warp_sum(x);
         if (lane == 0) ex_x[warp - 3] = x;
         if (group > 0) {
-          ex[group * 128 + row] = rows_sum;
+          ex[group * 128 + row] = rows_sum - cols_sum;
           ex[kDgRows + group * 128 + row] = keys_sum;
         }
         mbar_arrive(&bars[gAll]);
-        if (!mbar_wait(&bars[gAll], 0)) { tc_fail(15); break; }
+        if (!mbar_wait(&bars[gAll], ph)) { tc_fail(15); break; }
         // suffix sums of rows less columns, prefix sums of keys, by the first group: within a warp, then across
         if (group == 0) {
-          float down = rows_sum - (cols[row] + cols[128 + row] + cols[256 + row] + cols[384 + row]), up = keys_sum;
+          float down = rows_sum - cols_sum, up = keys_sum;
 #pragma unroll
           for (int i = 1; i < kDgGroups; ++i) {
             down += ex[i * 128 + row];
@@ -335,8 +377,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           }
           if (lane == 0) ex_down[quarter] = down;
           if (lane == 31) ex_up[quarter] = up;
-          uint32_t phase = 0;
-          if (!epi_sync(&bars[gSum], phase)) { tc_fail(16); break; }
+          if (!epi_sync(&bars[gSum], sum_phase)) { tc_fail(16); break; }
           float g = 0.f;
 #pragma unroll
           for (int i = 0; i < 4 * kDgGroups; ++i) g += ex_x[i];
@@ -357,12 +398,12 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           } else {
             g = warp_sum(g);
             if (lane == 0) ex_all[quarter] = g;
-            if (!epi_sync(&bars[gSum], phase)) { tc_fail(17); break; }
-            if (row == 0) static_cast<float*>(a.g_decay)[(b * chunks + chunk) * a.H + h] = ex_all[0] + ex_all[1] + ex_all[2] + ex_all[3];
+            if (!epi_sync(&bars[gSum], sum_phase)) { tc_fail(17); break; }
+            if (row == 0) static_cast<float*>(a.g_decay)[(k.b * chunks + k.chunk) * a.H + k.h] = ex_all[0] + ex_all[1] + ex_all[2] + ex_all[3];
           }
         }
       }
-    } while (false);
+    }
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -377,8 +418,7 @@ int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, con
   cudaError_t e = cudaFuncSetAttribute(decay_grad_tc_kernel<T, KB, DB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return fail((int)e, "decay_bwd: cannot reserve %u bytes of shared memory: %s", smem, cudaGetErrorString(e));
   const int64_t ctas = (int64_t)a.B * a.H * ((a.T + kTC - 1) / kTC);
-  RFA_REQUIRE(ctas < (int64_t)1 << 31, RFA_EUNSUPPORTED, "decay_bwd: %lld chunks", (long long)ctas);
-  e = launch_pdl(decay_grad_tc_kernel<T, KB, DB>, dim3((unsigned)ctas), dim3(kDgThreads), smem, stream, q, k, v, g, a);
+  e = launch_pdl(decay_grad_tc_kernel<T, KB, DB>, dim3((unsigned)std::min<int64_t>(ctas, 148)), dim3(kDgThreads), smem, stream, q, k, v, g, a, ctas);
   if (e != cudaSuccess) return fail((int)e, "rfa_decay_bwd: launch failed: %s", cudaGetErrorString(e));
   return check_launch("rfa_decay_bwd");
 }

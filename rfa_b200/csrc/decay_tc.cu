@@ -88,7 +88,9 @@ size_t decay_tc_bwd_bytes(const rfa_decay_t& c) {
   return ((plan.totals + 255) & ~(size_t)255) + ((plan.seg_decay + 255) & ~(size_t)255) + 2 * kept_bytes(c.T, BH, c.K, c.D) + sizeof(float) * BH * ((c.T + kTC - 1) / kTC);
 }
 
-int launch_decay_tc_bwd(const rfa_decay_t& c, char* workspace, const void* g, const float* g_s, void* gq, void* gk, void* gv, void* g_decay, float* gs_in, cudaStream_t stream) {
+size_t decay_tc_kept_bytes(int64_t T, int64_t BH, int K, int D) { return kept_bytes(T, BH, K, D); }
+
+int launch_decay_tc_bwd(const rfa_decay_t& c, char* workspace, const void* kept, const void* g, const float* g_s, void* gq, void* gk, void* gv, void* g_decay, float* gs_in, cudaStream_t stream) {
   const bool bf16 = c.dtype == RFA_BF16;
   const int64_t BH = (int64_t)c.B * c.H, row = (int64_t)c.H * c.D, chunks = (c.T + kTC - 1) / kTC;
   CUtensorMap q, k, v, gm;
@@ -100,23 +102,25 @@ int launch_decay_tc_bwd(const rfa_decay_t& c, char* workspace, const void* g, co
   char* grads = states + kept_bytes(c.T, BH, c.K, c.D);
   float* sums = reinterpret_cast<float*>(grads + kept_bytes(c.T, BH, c.K, c.D));
   DecayTcArgs a = sweep_args(c, plan, workspace);
-  a.in_scale = 1.f;
-  a.s_in = {const_cast<float*>(c.s_in), c.D, 1};
-  a.kept = states;
-  if (int r = sweep<false>(bf16, q, k, v, a, false, stream)) return r;
+  if (!kept) {      // the states in front of the chunks once more
+    a.in_scale = 1.f;
+    a.s_in = {const_cast<float*>(c.s_in), c.D, 1};
+    a.kept = states;
+    if (int r = sweep<false>(bf16, q, k, v, a, false, stream)) return r;
+  }
   a.in_scale = c.scale;
   a.rev = 1;
   a.s_in = {const_cast<float*>(g_s), c.D, 1};
   a.s_out = {gs_in, c.D, 1};
   a.kept = grads;
   if (int r = sweep<false>(bf16, q, q, gm, a, gs_in != nullptr, stream)) return r;
-  if (int r = launch_decay_grad_tc(c, q, k, v, gm, states, grads, gq, gk, gv, g_decay && c.per_head ? sums : g_decay, stream)) return r;
+  if (int r = launch_decay_grad_tc(c, q, k, v, gm, kept ? kept : states, grads, gq, gk, gv, g_decay && c.per_head ? sums : g_decay, stream)) return r;
   if (!g_decay || !c.per_head) return 0;
   const SumJob job{sums, g_decay, c.H, (int)(c.B * chunks), c.decay_dtype};
   return sum_parts(&job, 1, stream);
 }
 
-int launch_decay_tc(const rfa_decay_t& c, const SweepPlan& plan, char* workspace, void* out, float* s_out, cudaStream_t stream) {
+int launch_decay_tc(const rfa_decay_t& c, const SweepPlan& plan, char* workspace, void* out, float* s_out, void* kept, cudaStream_t stream) {
   const bool bf16 = c.dtype == RFA_BF16;
   CUtensorMap q, k, v;
   if (make_tmap_heads(&q, c.q, bf16, c.T, c.B, c.H, c.K, c.q_t, c.q_b, c.q_h, kTC) || make_tmap_heads(&k, c.k, bf16, c.T, c.B, c.H, c.K, c.k_t, c.k_b, c.k_h, kTC) ||
@@ -124,6 +128,7 @@ int launch_decay_tc(const rfa_decay_t& c, const SweepPlan& plan, char* workspace
     return fail(RFA_EDEVICE, "decay: cuTensorMapEncodeTiled failed or is unavailable");
   DecayTcArgs a = sweep_args(c, plan, workspace);
   a.out = out;
+  a.kept = kept;
   a.s_in = {const_cast<float*>(c.s_in), c.D, 1};
   a.s_out = {s_out, c.D, 1};
   a.in_scale = 1.f;

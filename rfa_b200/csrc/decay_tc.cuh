@@ -13,7 +13,7 @@
 // good as the 16-bit copies of S and P.  A log decay below -64 (in units of log 2) is taken as that.
 //
 // Backwards (states alone), from the last chunk to the first: S = 2^(L_end) S + scale Q'^T G, Q'_i = 2^(L_i) q_i: the gradient of the state.  `kept`: the
-// 16-bit copy of the state in front of each chunk (behind it, backwards) goes to memory as it stands in shared memory, for decay_grad.
+// 16-bit copy of the state in front of each chunk (behind it, backwards) goes to memory as it stands in shared memory, for decay_bwd_tc.cu.
 //
 // Warp roles (768 threads): warp 0 TMA producer; warps 1 and 18 MMA issuers (A: Q K^T, P V; B: Q S, the state: issuing one costs the issuing thread about 70
 // cycles, and a chunk has 20 to 40); warps 2..5 score group (A -> P); warps 6..9 and 20..23 state groups, half of the columns each (state -> 16-bit copy,
@@ -288,13 +288,13 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_arrive(&bars[dSt]);
     }
     for (int c = 0; ok && c < nchunk; ++c) {
-      if (!OUT && a.kept) {
-        if (tid == 6 * 32) {      // the copy of chunk c to memory, once it is whole; the one before it has then been read
+      if (a.kept) {
+        if (tid == 6 * 32) {      // the copy of chunk c to memory, once it is whole; the place of the next one has been read then
           if (!mbar_wait(&bars[dSt], c & 1)) { tc_fail(19); ok = false; break; }
           const int64_t chunk = chunk_t0(c) / kTC, chunks = (a.T + kTC - 1) / kTC;
-          bulk_store(static_cast<unsigned char*>(a.kept) + (bh * chunks + chunk) * Lay::kCopyBytes, sm + Lay::copy + (c & 1) * Lay::kCopyRoom, Lay::kCopyBytes);
+          bulk_store(static_cast<unsigned char*>(a.kept) + (bh * chunks + chunk) * Lay::kCopyBytes, sm + Lay::copy + (Lay::kCopies == 2 ? (c & 1) * Lay::kCopyRoom : 0), Lay::kCopyBytes);
           tma_store_commit();
-          tma_store_wait_read<1>();
+          tma_store_wait_read<Lay::kCopies - 1>();
           mbar_arrive(&bars[dKept]);
         }
         if (!mbar_wait(&bars[dKept], c & 1)) { tc_fail(20); ok = false; break; }

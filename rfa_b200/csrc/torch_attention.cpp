@@ -49,42 +49,44 @@ struct Decay {
   Tensor workspace(bool backward) const { return scratch(rfa_decay_workspace_bytes(c.T, c.B, c.H, c.K, c.D, c.dtype, backward), q); }
 };
 
-// -> out; the last state where asked, in place of `s` where that is asked too
-std::tuple<Tensor, OptTensor> decay_attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const OptTensor& s, const OptTensor& mask,
-                                                  std::optional<double> scale, bool return_state, bool in_place) {
+// -> out; the last state where asked, in place of `s` where that is asked too; with `save` what the backward goes on from, if anything
+std::tuple<Tensor, OptTensor, OptTensor> decay_attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const OptTensor& s, const OptTensor& mask,
+                                                  std::optional<double> scale, bool return_state, bool in_place, bool save) {
   Decay d(q, k, v, log_decay, s, mask, scale);
   if (in_place && s && !s->is_contiguous()) raise(PyExc_ValueError, "decay_attention: the state must be contiguous (it is updated in place)");
   const std::vector<int64_t> state{q.size(1), q.size(2), q.size(3), v.size(3)};
   if (d.empty()) {
     Tensor out = at::zeros(v.sizes(), v.options().requires_grad(false));
-    if (!return_state) return {out, std::nullopt};
-    if (in_place && s) return {out, *s};
-    return {out, s ? s->clone() : fresh_zeros(state, q)};
+    if (!return_state) return {out, std::nullopt, std::nullopt};
+    if (in_place && s) return {out, *s, std::nullopt};
+    return {out, s ? s->clone() : fresh_zeros(state, q), std::nullopt};
   }
   Tensor out = fresh(v.sizes(), q, q.scalar_type());
-  OptTensor last;
+  OptTensor last, kept;
   const bool here = in_place && s && d.s->is_same(*s);
-  if (d.c.T == 1 && return_state) {                    // the state is read and written once
+  if (d.c.T == 1 && return_state && !save) {           // the state is read and written once
     last = here ? *s : s ? d.s->is_same(*s) || d.s->is_alias_of(*s) ? d.s->clone() : *d.s : fresh_zeros(state, q);
     Call call(q);
     check(rfa_decay_step(&d.c, out.data_ptr(), last->data_ptr<float>(), call.stream), "rfa_decay_step");
   } else {
     if (return_state) last = here ? *s : fresh(state, q, at::kFloat);
+    const size_t bytes = save ? rfa_decay_kept_bytes(&d.c) : 0;
+    if (bytes) kept = scratch(bytes, q);
     const Tensor ws = d.workspace(false);
     Call call(q);
-    check(rfa_decay_fwd(&d.c, out.data_ptr(), last ? last->data_ptr<float>() : nullptr, ws.data_ptr(), ws.numel(), call.stream), "rfa_decay_fwd");
+    check(rfa_decay_fwd(&d.c, out.data_ptr(), last ? last->data_ptr<float>() : nullptr, maybe_out(kept), ws.data_ptr(), ws.numel(), call.stream), "rfa_decay_fwd");
   }
   if (last && here) written(*s);
   if (last && in_place && s && !here) {
     s->copy_(*last);
     last = s;
   }
-  return {out, last};
+  return {out, last, kept};
 }
 
 // -> gq, gk, gv, g_decay, gs
 std::tuple<Tensor, Tensor, Tensor, OptTensor, OptTensor> decay_attention_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const OptTensor& s,
-                                                                             const OptTensor& mask, std::optional<double> scale, Tensor g, OptTensor g_s, bool need_decay,
+                                                                             const OptTensor& mask, std::optional<double> scale, Tensor g, OptTensor g_s, const OptTensor& kept, bool need_decay,
                                                                              bool need_state) {
   Decay d(q, k, v, log_decay, s, mask, scale);
   need_grad("decay_attention", "g", g, v.sizes(), q);
@@ -100,11 +102,13 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor, OptTensor> decay_attention_bwd(con
     if (gs) g_s ? gs->copy_(*g_s) : gs->zero_();
     return {gq, gk, gv, gd, gs};
   }
+  if (kept && (!kept->is_contiguous() || kept->nbytes() < rfa_decay_kept_bytes(&d.c))) raise(PyExc_ValueError, "decay_attention: kept is not what this call's forward left");
+  if (kept) require_device(q, {&*kept});
   g = packed(g.to(half));
   if (g_s) g_s = packed(g_s->to(at::kFloat));
   const Tensor ws = d.workspace(true);
   Call call(q);
-  check(rfa_decay_bwd(&d.c, g.data_ptr(), maybe_f(g_s), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), maybe_out(gd), gs ? gs->data_ptr<float>() : nullptr, ws.data_ptr(),
+  check(rfa_decay_bwd(&d.c, g.data_ptr(), maybe_f(g_s), maybe(kept), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), maybe_out(gd), gs ? gs->data_ptr<float>() : nullptr, ws.data_ptr(),
                       ws.numel(), call.stream),
         "rfa_decay_bwd");
   return {gq, gk, gv, gd, gs};
@@ -114,10 +118,10 @@ struct DecayAttentionBackward : torch::autograd::Function<DecayAttentionBackward
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const OptTensor& s, const OptTensor& mask,
                                std::optional<double> scale, bool return_state) {
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, v, log_decay, plain(s), plain(mask)});
     ctx->saved_data["scale"] = scale_of(scale, q.size(3));
     ctx->saved_data["need"] = static_cast<int64_t>(log_decay.requires_grad() | wants(s) << 1);
-    auto [out, last] = decay_attention_fwd(q, k, v, log_decay, s, mask, scale, return_state, false);
+    auto [out, last, kept] = decay_attention_fwd(q, k, v, log_decay, s, mask, scale, return_state, false, true);
+    ctx->save_for_backward({q, k, v, log_decay, plain(s), plain(mask), plain(kept)});
     if (!return_state) return {out};
     return {out, *last};
   }
@@ -127,19 +131,19 @@ struct DecayAttentionBackward : torch::autograd::Function<DecayAttentionBackward
     const int64_t need = ctx->saved_data["need"].toInt();
     const Tensor go = g[0].defined() ? g[0] : at::zeros_like(t[2]);
     auto [gq, gk, gv, gd, gs] = decay_attention_bwd(t[0], t[1], t[2], t[3], opt(t[4]), opt(t[5]), ctx->saved_data["scale"].toDouble(), go,
-                                                    g.size() > 1 ? opt(g[1]) : OptTensor(), need & 1, need & 2);
+                                                    g.size() > 1 ? opt(g[1]) : OptTensor(), opt(t[6]), need & 1, need & 2);
     return {gq, gk, gv, plain(gd), plain(gs), Tensor(), Tensor(), Tensor()};
   }
 };
 
 Tensor decay_attention_node(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const OptTensor& mask, std::optional<double> scale) {
-  if (!records(q, k, v, log_decay)) return std::get<0>(decay_attention_fwd(q, k, v, log_decay, std::nullopt, mask, scale, false, false));
+  if (!records(q, k, v, log_decay)) return std::get<0>(decay_attention_fwd(q, k, v, log_decay, std::nullopt, mask, scale, false, false, false));
   return DecayAttentionBackward::apply(q, k, v, log_decay, OptTensor(), mask, scale, false)[0];
 }
 std::tuple<Tensor, Tensor> incremental_decay_attention_node(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const OptTensor& s,
                                                             const OptTensor& mask, std::optional<double> scale) {
   if (!records(q, k, v, log_decay, s)) {
-    auto [out, last] = decay_attention_fwd(q, k, v, log_decay, s, mask, scale, true, true);
+    auto [out, last, kept] = decay_attention_fwd(q, k, v, log_decay, s, mask, scale, true, true, false);
     return {out, *last};
   }
   const variable_list r = DecayAttentionBackward::apply(q, k, v, log_decay, s, mask, scale, true);

@@ -33,18 +33,18 @@ class _DecayAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, s, mask, scale, return_state):
-        ctx.save_for_backward(q, k, v, log_decay, s, mask)
+        out, last, kept = ops.decay_attention_fwd(q, k, v, log_decay, s, mask, scale, return_state, False, True)
+        ctx.save_for_backward(q, k, v, log_decay, s, mask, kept)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        out, last = ops.decay_attention_fwd(q, k, v, log_decay, s, mask, scale, return_state)
         return (out, last) if return_state else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, g_s=None):
-        q, k, v, log_decay, s, mask = ctx.saved_tensors
+        q, k, v, log_decay, s, mask, kept = ctx.saved_tensors
         g = torch.zeros_like(v) if g is None else g
-        grads = ops.decay_attention_bwd(q, k, v, log_decay, s, mask, ctx.scale, g, g_s, ctx.needs_input_grad[3], ctx.needs_input_grad[4])
+        grads = ops.decay_attention_bwd(q, k, v, log_decay, s, mask, ctx.scale, g, g_s, kept, ctx.needs_input_grad[3], ctx.needs_input_grad[4])
         return (*grads, None, None, None)
 
 
@@ -69,7 +69,7 @@ def incremental_decay_attention(*, q: Tensor, k: Tensor, v: Tensor, log_decay: T
     if plain_tensors(q, k, v, log_decay, s, mask):
         return native().incremental_decay_attention_node(q, k, v, log_decay, s, mask, scale)
     if _underived(q, k, v, log_decay, s):
-        return ops.decay_attention_fwd(q, k, v, log_decay, s, mask, scale, True, True)
+        return ops.decay_attention_fwd(q, k, v, log_decay, s, mask, scale, True, True)[:2]
     return _DecayAttention.apply(q, k, v, log_decay, s, mask, scale, True)
 
 

@@ -406,15 +406,16 @@ def group_norm_bwd(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optio
 
 # --------------------------------------------------------------------------- decaying and windowed attention
 def decay_attention_fwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s: Optional[Tensor] = None, mask: Optional[Tensor] = None,
-                        scale: Optional[float] = None, return_state: bool = False, in_place: bool = False):
-    """-> (out, the last state or None: in place of ``s`` with ``in_place``)."""
-    return native().decay_attention_fwd(q, k, v, log_decay, s, mask, scale, return_state, in_place)
+                        scale: Optional[float] = None, return_state: bool = False, in_place: bool = False, save: bool = False):
+    """-> (out, the last state or None: in place of ``s`` with ``in_place``, with ``save`` what ``decay_attention_bwd`` goes on from, where it is
+    anything)."""
+    return native().decay_attention_fwd(q, k, v, log_decay, s, mask, scale, return_state, in_place, save)
 
 
 def decay_attention_bwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s: Optional[Tensor], mask: Optional[Tensor], scale: Optional[float],
-                        g: Tensor, g_s: Optional[Tensor] = None, need_decay: bool = True, need_state: bool = False):
-    """-> (gq, gk, gv, g_log_decay or None, gs or None)."""
-    return native().decay_attention_bwd(q, k, v, log_decay, s, mask, scale, g, g_s, need_decay, need_state)
+                        g: Tensor, g_s: Optional[Tensor] = None, kept: Optional[Tensor] = None, need_decay: bool = True, need_state: bool = False):
+    """-> (gq, gk, gv, g_log_decay or None, gs or None).  Without ``kept`` the forward's states are computed again."""
+    return native().decay_attention_bwd(q, k, v, log_decay, s, mask, scale, g, g_s, kept, need_decay, need_state)
 
 
 def window_attention_fwd(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, mask: Optional[Tensor] = None, scale: Optional[float] = None,

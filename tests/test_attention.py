@@ -29,8 +29,8 @@ def window(**kw):
 def test_decay_refusals(kw, code):
     from rfa_b200 import _lib
     lib, c = _lib.load(), decay(**kw)
-    assert lib.rfa_decay_fwd(C.byref(c), 16, None, None, 0, None) == code
-    assert lib.rfa_decay_bwd(C.byref(c), 16, None, 16, 16, 16, None, None, 16, 1 << 40, None) == code
+    assert lib.rfa_decay_fwd(C.byref(c), 16, None, None, None, 0, None) == code
+    assert lib.rfa_decay_bwd(C.byref(c), 16, None, None, 16, 16, 16, None, None, 16, 1 << 40, None) == code
     assert lib.rfa_decay_step(C.byref(c), 16, 16, None) == code
 
 
@@ -38,17 +38,17 @@ def test_decay_refusals_of_buffers():
     from rfa_b200 import _lib
     lib = _lib.load()
     c = decay()
-    assert lib.rfa_decay_fwd(None, 16, None, None, 0, None) == -1
-    assert lib.rfa_decay_fwd(C.byref(c), None, None, None, 0, None) == -1
-    assert lib.rfa_decay_fwd(C.byref(c), 16, 8, None, 0, None) == -2
+    assert lib.rfa_decay_fwd(None, 16, None, None, None, 0, None) == -1
+    assert lib.rfa_decay_fwd(C.byref(c), None, None, None, None, 0, None) == -1
+    assert lib.rfa_decay_fwd(C.byref(c), 16, 8, None, None, 0, None) == -2
     assert lib.rfa_decay_step(C.byref(c), 16, 16, None) == -1                                   # four tokens
     assert lib.rfa_decay_step(C.byref(decay(T=1)), 16, 8, None) == -2
-    assert lib.rfa_decay_bwd(C.byref(c), 16, None, 16, 16, 16, None, None, 16, 0, None) == -4   # no workspace
-    assert lib.rfa_decay_bwd(C.byref(c), None, None, 16, 16, 16, None, None, 16, 1 << 40, None) == -1
+    assert lib.rfa_decay_bwd(C.byref(c), 16, None, None, 16, 16, 16, None, None, 16, 0, None) == -4   # no workspace
+    assert lib.rfa_decay_bwd(C.byref(c), None, None, None, 16, 16, 16, None, None, 16, 1 << 40, None) == -1
     long = decay(T=100000, B=1, H=1)
     need = lib.rfa_decay_workspace_bytes(100000, 1, 1, 16, 16, 0, 0)
     assert need > 0 and need == lib.rfa_decay_workspace_bytes(100000, 1, 1, 16, 16, 0, 0)
-    assert lib.rfa_decay_fwd(C.byref(long), 16, None, 16, need - 1, None) == -4
+    assert lib.rfa_decay_fwd(C.byref(long), 16, None, None, 16, need - 1, None) == -4
     assert lib.rfa_decay_workspace_bytes(0, 1, 1, 16, 16, 0, 0) == 0
 
 
