@@ -55,7 +55,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
     k.b = w % per / rows_heads;
     k.head = w % per % rows_heads;
     const WindowNumbers num(a, k.b);
-    if (KEYS) k.span = {k.row0 / kWbTile, 0, (num.last_query(k.row0, min(a.S, k.row0 + 128)) + kWbTile - 1) / kWbTile};
+    if (KEYS) k.span = {(int)(k.row0 / kWbTile), 0, (int)((num.last_query(k.row0, min(a.S, k.row0 + 128)) + kWbTile - 1) / kWbTile)};
     else k.span = window_span<kWbTile>(num, 0, k.row0, a.T);
   };
   // heads of the other side that a work goes through, and where
@@ -88,19 +88,20 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
         for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::r1 + x * kBox, &tm_r1, &bars[bR], x * 64, k.head, k.b, (int)k.row0);
         for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::r2 + x * kBox, &tm_r2, &bars[bR], x * 64, k.head, k.b, (int)k.row0);
         for (int h = first_head(k); ok && h < first_head(k) + other_heads; ++h)
-          for (int64_t t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
+          for (int t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
             const int st = n % kStages;
             if (n >= kStages && !mbar_wait(&bars[bEmpty + st], (n / kStages + 1) & 1)) { tc_fail(2); ok = false; break; }
             mbar_arrive_expect_tx(&bars[bFull + st], 2 * DB * Lay::kHalf);
-            for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::x1 + (st * DB + x) * Lay::kHalf, &tm_x1, &bars[bFull + st], x * 64, h, k.b, (int)(t * kWbTile));
-            for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::x2 + (st * DB + x) * Lay::kHalf, &tm_x2, &bars[bFull + st], x * 64, h, k.b, (int)(t * kWbTile));
+            for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::x1 + (st * DB + x) * Lay::kHalf, &tm_x1, &bars[bFull + st], x * 64, h, k.b, t * kWbTile);
+            for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::x2 + (st * DB + x) * Lay::kHalf, &tm_x2, &bars[bFull + st], x * 64, h, k.b, t * kWbTile);
           }
       }
     }
   } else if (warp == 1 || warp == 2) {
     // ------------------------------------------------------------------ MMA issuers
-    if (lane == 0) {
-      constexpr uint32_t lead = 1u;
+    // the whole warp goes through the loop and one lane issues (see umma_ss_w)
+    {
+      const uint32_t lead = lane == 0;
       constexpr uint32_t idS = umma_idesc<T>(128, kWbTile, false, false), idG = umma_idesc<T>(128, DP, false, true);
       constexpr uint32_t kBlockX = Lay::kHalf >> 4;
       constexpr uint64_t kStep = (DB * Lay::kHalf) >> 4;
@@ -113,31 +114,31 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
         Work k;
         work_of(w, k);
         if (warp == 1) {
-          if (!mbar_wait(&bars[bR], done & 1)) { tc_fail(3); break; }
-        } else if (done > 0 && !mbar_wait(&bars[bAccFree], (done + 1) & 1)) { tc_fail(4); break; }
+          if (!mbar_wait(&bars[bR], done & 1)) { if (lead) tc_fail(3); break; }
+        } else if (done > 0 && !mbar_wait(&bars[bAccFree], (done + 1) & 1)) { if (lead) tc_fail(4); break; }
         bool first = true;
         for (int h = 0; ok && h < other_heads; ++h)
-          for (int64_t t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
+          for (int t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
             const int st = n % kStages, buf = n & 1;
             if (warp == 1) {
-              if (!mbar_wait(&bars[ORDERED ? bCols + st : bFull + st], (n / kStages) & 1)) { tc_fail(5); ok = false; break; }
-              if (n >= 2 && !mbar_wait(&bars[bFree + buf], ((n >> 1) + 1) & 1)) { tc_fail(6); ok = false; break; }
+              if (!mbar_wait(&bars[ORDERED ? bCols + st : bFull + st], (n / kStages) & 1)) { if (lead) tc_fail(5); ok = false; break; }
+              if (n >= 2 && !mbar_wait(&bars[bFree + buf], ((n >> 1) + 1) & 1)) { if (lead) tc_fail(6); ok = false; break; }
               tc_fence_after_sync();
               umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, tmem + buf * 128, dR1, dX1 + st * kStep, idS, 0);
               umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, tmem + buf * 128 + 64, dR2, dX2 + st * kStep, idS, 0);
-              umma_commit(&bars[bS + buf]);
-              umma_commit(&bars[bEmpty + st]);
+              umma_commit_w(lead, &bars[bS + buf]);
+              umma_commit_w(lead, &bars[bEmpty + st]);
             } else {
-              if (!mbar_wait(&bars[bP + buf], (n >> 1) & 1)) { tc_fail(7); ok = false; break; }
+              if (!mbar_wait(&bars[bP + buf], (n >> 1) & 1)) { if (lead) tc_fail(7); ok = false; break; }
               tc_fence_after_sync();
               if constexpr (KEYS) umma_chain_ts<4, kStepMN, kBlockMN>(lead, tmem + 256 + DP, tmem + buf * 128, dX2t + st * kStep, idG, first ? 0u : 1u);
               umma_chain_ts<4, kStepMN, kBlockMN>(lead, tmem + 256, tmem + buf * 128 + 64, dX1t + st * kStep, idG, first ? 0u : 1u);
-              umma_commit(&bars[bFree + buf]);
-              umma_commit(&bars[bEmpty + st]);
+              umma_commit_w(lead, &bars[bFree + buf]);
+              umma_commit_w(lead, &bars[bEmpty + st]);
               first = false;
             }
           }
-        if (ok) umma_commit(&bars[warp == 1 ? bREmpty : bAcc]);
+        if (ok) umma_commit_w(lead, &bars[warp == 1 ? bREmpty : bAcc]);
       }
     }
   } else if (warp == 3) {
@@ -150,13 +151,13 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
         work_of(w, k);
         const WindowNumbers num(a, k.b);
         for (int h = first_head(k); ok && h < first_head(k) + other_heads; ++h)
-          for (int64_t t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
+          for (int t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
             const int st = n % kStages;
             int number[2] = {0, 0};
             float lse[2] = {0.f, 0.f}, delta[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int64_t i = t * kWbTile + e * 32 + lane;
+              const int64_t i = (int64_t)t * kWbTile + e * 32 + lane;
               if (ORDERED) number[e] = num.at(i);
               if (KEYS && i < a.T) {
                 lse[e] = kLog2e * a.lse[((int64_t)k.b * a.H + h) * a.T + i];
@@ -206,10 +207,10 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
         delta = a.delta[((int64_t)k.b * a.H + k.head) * a.T + i];
       }
       for (int h = 0; ok && h < other_heads; ++h)
-        for (int64_t t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
+        for (int t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
           if ((n & 1) != g) continue;
           const int st = n % kStages;
-          const int64_t c0 = t * kWbTile;
+          const int64_t c0 = (int64_t)t * kWbTile;
           bool whole;
           uint32_t seen[2] = {0u, 0u};
           if constexpr (ORDERED) whole = false;

@@ -1,12 +1,13 @@
 // Sliding-window attention on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), fp16 and bf16, heads of up to 128: the forward pass.
 //
 // A CTA takes one pair of units after the other, each unit 128 queries of one batch row, that read the same keys -- two heads that share a key head, or else two
-// runs of one head -- and goes through the 128-key tiles that either of them sees: those of the first tokens, then from the window's start on.  Per unit and tile
+// runs of one head -- and goes through the 64-key tiles that either of them sees: those of the first tokens, then from the window's start on.  Per unit and tile
 //     S = Q K^T (fp32, TMEM)  ->  P = 2^(S scale log2(e) - m), 16 bits, over S  ->  O += P V
 // with a thread to each row, whose scores it holds in registers: the row's maximum, then P and the sum.  m moves only when it is exceeded by more than 8 (P is then
 // at most 256, which both types hold), and only then O is rescaled, by the row's own thread.  Tiles that every query of the unit sees whole need no mask; in the
-// others scores that are not seen are -inf before anything is made of them.  Bound by the exponentials (16 a cycle and SM: 1024 cycles a tile) and the instructions
-// around them.
+// others scores that are not seen are -inf before anything is made of them.  A unit's scores have two places in TMEM, so that the products of the next tile run under the
+// exponentials of this one: with tiles of 128 keys and one place a unit's chain of products, maxima, exponentials and products again took 4500 cycles, of which the
+// special function unit worked 2048 (16 exponentials a cycle and SM, two units).
 //
 // With padded tokens or a cache in front (ORDERED) places are not numbers: warp 3 fetches the numbers of a tile's keys and clears the values of places that hold
 // no token, whatever stands there.
@@ -22,15 +23,16 @@ namespace rfa {
 
 constexpr int kWinThreads = 384;
 
+constexpr int kWinTile = 64;
 template <int DB>
 struct WinLayout {
-  static constexpr int kStages = DB == 1 ? 4 : 2;
-  static constexpr uint32_t q = 0, k = 2 * DB * kBox, v = k + kStages * DB * kBox, num = v + kStages * DB * kBox, bar = num + kStages * 128 * 4, bytes = bar + 256;
+  static constexpr int kStages = 4;
+  static constexpr uint32_t kHalf = kBox / 2;      // 64 rows of 128 bytes
+  static constexpr uint32_t q = 0, k = 2 * DB * kBox, v = k + kStages * DB * kHalf, num = v + kStages * DB * kHalf, bar = num + kStages * kWinTile * 4, bytes = bar + 256;
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
-enum { wQ = 0, wQEmpty = 2, wFullK = 4, wFullV = 8, wEmpty = 12, wNumbers = 16, wS = 20, wP = 22, wO = 24, wTurn = 26, wCount = 28 };
-// wTurn: a group's exponentials of a tile wait for the other group's before them, so that one group's products, maxima and waits fall in the other's exponentials.
-// Left alone the two run in step, and the special function unit idles for more than half of the time (6000 cycles for a pair of tiles, 64 and 128 wide).
+// wS, wP: [unit][place of the scores]
+enum { wQ = 0, wQEmpty = 2, wFullK = 4, wFullV = 8, wEmpty = 12, wNumbers = 16, wS = 20, wP = 24, wO = 28, wCount = 30 };
 
 template <typename T, int DB, bool ORDERED>
 __global__ void __launch_bounds__(kWinThreads, 1)
@@ -59,8 +61,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     k.row[0] = (int64_t)(pair_heads ? run : 2 * run) * 128;
     k.row[1] = pair_heads ? k.row[0] : k.row[0] + 128;
     const WindowNumbers num(a, k.b);
-    k.span[0] = window_span(num, at, k.row[0], a.T);
-    k.span[1] = pair_heads ? k.span[0] : window_span(num, at, k.row[1], a.T);
+    k.span[0] = window_span<kWinTile>(num, at, k.row[0], a.T);
+    k.span[1] = pair_heads ? k.span[0] : window_span<kWinTile>(num, at, k.row[1], a.T);
     k.both = k.span[0];
     if (k.span[1].end > 0) {      // a last run may be without a partner
       k.both.first = min(k.span[0].first, k.span[1].first);
@@ -68,7 +70,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     }
   };
   if (tid == 0) {
-    for (int i = 0; i < wCount; ++i) mbar_init(&bars[i], (i >= wP && i < wO) || i >= wTurn ? 128 : i >= wNumbers && i < wS ? 32 : i >= wEmpty && i < wNumbers ? (ORDERED ? 2 + 256 : 2) : 1);
+    for (int i = 0; i < wCount; ++i) mbar_init(&bars[i], i >= wP && i < wO ? 128 : i >= wNumbers && i < wS ? 32 : i >= wEmpty && i < wNumbers ? (ORDERED ? 2 + 256 : 2) : 1);
     mbar_fence_init();
     tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
   }
@@ -94,56 +96,75 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           for (int x = 0; x < DB; ++x)
             tma_load_4d(sm + Lay::q + (u * DB + x) * kBox, &tm_q, &bars[wQ + u], x * 64, k.h0 + (pair_heads ? u : 0), k.b, (int)k.row[u]);
         }
-        for (int64_t kt = k.both.begin(); ok && kt < k.both.end; kt = k.both.next(kt), ++n) {
+        for (int kt = k.both.begin(); ok && kt < k.both.end; kt = k.both.next(kt), ++n) {
           const int st = n % kStages;
           if (n >= kStages && !mbar_wait(&bars[wEmpty + st], (n / kStages + 1) & 1)) { tc_fail(2); ok = false; break; }
-          mbar_arrive_expect_tx(&bars[wFullK + st], DB * kBox);
-          for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::k + (st * DB + x) * kBox, &tm_k, &bars[wFullK + st], x * 64, k.kv, k.b, (int)(kt * 128));
-          mbar_arrive_expect_tx(&bars[wFullV + st], DB * kBox);
-          for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + (st * DB + x) * kBox, &tm_v, &bars[wFullV + st], x * 64, k.kv, k.b, (int)(kt * 128));
+          mbar_arrive_expect_tx(&bars[wFullK + st], DB * Lay::kHalf);
+          for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::k + (st * DB + x) * Lay::kHalf, &tm_k, &bars[wFullK + st], x * 64, k.kv, k.b, kt * kWinTile);
+          mbar_arrive_expect_tx(&bars[wFullV + st], DB * Lay::kHalf);
+          for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + (st * DB + x) * Lay::kHalf, &tm_v, &bars[wFullV + st], x * 64, k.kv, k.b, kt * kWinTile);
         }
       }
     }
   } else if (warp == 1 || warp == 2) {
     // ------------------------------------------------------------------ MMA issuers
-    if (lane == 0) {
-      constexpr uint32_t lead = 1u;
+    // The whole warp goes through the loop and one lane issues: descriptors stay in uniform registers (see umma_ss_w).
+    {
+      const uint32_t lead = lane == 0;
       const int u = warp - 1;
-      constexpr uint32_t idS = umma_idesc<T>(128, 128, false, false), idO = umma_idesc<T>(128, DP, false, true);
+      constexpr uint32_t idS = umma_idesc<T>(128, kWinTile, false, false), idO = umma_idesc<T>(128, DP, false, true);
+      constexpr uint32_t kBlockX = Lay::kHalf >> 4;
       const uint64_t dQ = umma_smem_desc(sbase + Lay::q + u * DB * kBox, 0, 1024, kSwizzle128B), dK = umma_smem_desc(sbase + Lay::k, 0, 1024, kSwizzle128B);
-      const uint64_t dV = umma_smem_desc(sbase + Lay::v, kBox, 1024, kSwizzle128B);
-      constexpr uint64_t kStep = (DB * kBox) >> 4;
+      const uint64_t dV = umma_smem_desc(sbase + Lay::v, Lay::kHalf, 1024, kSwizzle128B);
+      constexpr uint64_t kStep = (DB * Lay::kHalf) >> 4;
       const uint32_t S = tmem + u * 128, O = tmem + 256 + u * DP;
-      int n = 0, it = 0, done = 0;
+      int n = 0, is = 0, it = 0, done = 0;      // tiles; of this unit: scores, sums
       bool ok = true;
       for (int w = blockIdx.x; ok && w < works; w += gridDim.x, ++done) {
         Work k;
         work_of(w, k);
         const WindowSpan own = u ? k.span[1] : k.span[0];
-        if (!mbar_wait(&bars[wQ + u], done & 1)) { tc_fail(3); break; }
+        if (!mbar_wait(&bars[wQ + u], done & 1)) { if (lead) tc_fail(3); break; }
+        // Scores run up to two of the unit's tiles ahead of the sums.  No tile is waited for whose stage the unit's own sums have yet to give back.
+        int kt = k.both.begin();
+        int ahead[2] = {0, 0}, pending = 0;      // tiles whose scores have been issued and whose sums have not, the older first
         bool first = true;
-        for (int64_t kt = k.both.begin(); kt < k.both.end; kt = k.both.next(kt), ++n) {
-          const int st = n % kStages;
-          const uint32_t filled = (n / kStages) & 1;
-          if (!mbar_wait(&bars[wFullK + st], filled)) { tc_fail(4); ok = false; break; }
-          if (!own.has(kt)) {
-            if (!mbar_wait(&bars[wFullV + st], filled)) { tc_fail(5); ok = false; break; }
-            mbar_arrive(&bars[wEmpty + st]);
-            continue;
+        while (ok && (pending > 0 || kt < k.both.end)) {
+          while (pending < 2 && kt < k.both.end && (pending == 0 || n - ahead[0] < kStages)) {
+            const int st = n % kStages;
+            const uint32_t filled = (n / kStages) & 1;
+            if (!mbar_wait(&bars[wFullK + st], filled)) { if (lead) tc_fail(4); ok = false; break; }
+            if (own.has(kt)) {
+              tc_fence_after_sync();
+              umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, S + (is & 1) * 64, dQ, dK + st * kStep, idS, 0);
+              umma_commit_w(lead, &bars[wS + 2 * u + (is & 1)]);
+              ++is;
+              if (pending == 0) ahead[0] = n;
+              else ahead[1] = n;
+              ++pending;
+            } else {
+              if (!mbar_wait(&bars[wFullV + st], filled)) { if (lead) tc_fail(5); ok = false; break; }
+              if (lead) mbar_arrive(&bars[wEmpty + st]);
+            }
+            kt = k.both.next(kt);
+            ++n;
           }
+          if (!ok || pending == 0) continue;
+          const int st = ahead[0] % kStages;
+          const uint32_t filled = (ahead[0] / kStages) & 1;
+          if (!mbar_wait(&bars[ORDERED ? wNumbers + st : wFullV + st], filled)) { if (lead) tc_fail(6); ok = false; break; }
+          if (!mbar_wait(&bars[wP + 2 * u + (it & 1)], (it >> 1) & 1)) { if (lead) tc_fail(7); ok = false; break; }
           tc_fence_after_sync();
-          umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockK>(lead, S, dQ, dK + st * kStep, idS, 0);
-          umma_commit(&bars[wS + u]);
-          if (!mbar_wait(&bars[ORDERED ? wNumbers + st : wFullV + st], filled)) { tc_fail(6); ok = false; break; }
-          if (!mbar_wait(&bars[wP + u], it & 1)) { tc_fail(7); ok = false; break; }
-          tc_fence_after_sync();
-          umma_chain_ts<8, kStepMN, kBlockMN>(lead, O, S, dV + st * kStep, idO, first ? 0u : 1u);
-          umma_commit(&bars[wO + u]);
-          umma_commit(&bars[wEmpty + st]);
+          umma_chain_ts<4, kStepMN, kBlockMN>(lead, O, S + (it & 1) * 64, dV + st * kStep, idO, first ? 0u : 1u);
+          umma_commit_w(lead, &bars[wO + u]);
+          umma_commit_w(lead, &bars[wEmpty + st]);
           first = false;
           ++it;
+          ahead[0] = ahead[1];
+          --pending;
         }
-        if (ok) umma_commit(&bars[wQEmpty + u]);      // everything that reads Q is complete
+        if (!ok) break;
+        umma_commit_w(lead, &bars[wQEmpty + u]);      // everything that reads Q is complete
       }
     }
   } else if (warp >= 4) {
@@ -163,24 +184,21 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       float top = -1e30f, sum = 0.f;      // the reference that weights are taken against, in units of log 2
       bool first = true;
 #pragma unroll 1
-      for (int64_t kt = k.both.begin(); kt < k.both.end; kt = k.both.next(kt), ++n) {
+      for (int kt = k.both.begin(); kt < k.both.end; kt = k.both.next(kt), ++n) {
         if (ORDERED && !mbar_wait(&bars[wNumbers + n % kStages], (n / kStages) & 1)) { tc_fail(8); ok = false; break; }
-        // the other group's exponentials of the tile before (first unit) or of this tile (second) are done
-        const auto turn = [&]() { return (u == 0 && n == 0) || mbar_wait(&bars[wTurn + u], u == 0 ? (n + 1) & 1 : n & 1); };
         if (!own.has(kt)) {
           if (ORDERED) mbar_arrive(&bars[wEmpty + n % kStages]);
-          if (!turn()) { tc_fail(13); ok = false; break; }
-          mbar_arrive(&bars[wTurn + 1 - u]);
           continue;
         }
-        const int64_t j0 = kt * 128;
+        const int64_t j0 = (int64_t)kt * kWinTile;
+        const uint32_t Sp = S + (it & 1) * 64;
         // every query of the unit sees every key of the tile; or else which keys this row sees
-        const bool whole = !ORDERED && j0 + 127 <= at + i0 && at + i0 + 127 - j0 < a.window;
-        uint32_t seen[4];
+        const bool whole = !ORDERED && j0 + kWinTile - 1 <= at + i0 && at + i0 + 127 - j0 < a.window;
+        uint32_t seen[2];
         if constexpr (ORDERED) {
-          const int* nums = reinterpret_cast<const int*>(sm + Lay::num) + (n % kStages) * 128;
+          const int* nums = reinterpret_cast<const int*>(sm + Lay::num) + (n % kStages) * kWinTile;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < 2; ++x) {
             uint32_t bits = 0;
 #pragma unroll 1
             for (int c = 28; c >= 0; c -= 4) {
@@ -191,26 +209,24 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             seen[x] = bits;
           }
         } else if (!whole) {
-          const int hi = (int)min((int64_t)128, place - j0 + 1), lo = (int)max((int64_t)0, place - j0 - a.window + 1), front = (int)min((int64_t)128, a.sinks - j0);
+          const int hi = (int)min((int64_t)64, place - j0 + 1), lo = (int)min((int64_t)64, max((int64_t)0, place - j0 - a.window + 1)), front = (int)min((int64_t)64, a.sinks - j0);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) seen[x] = low_bits(hi - 32 * x) & (~low_bits(lo - 32 * x) | low_bits(front - 32 * x));
+          for (int x = 0; x < 2; ++x) seen[x] = low_bits(hi - 32 * x) & (~low_bits(lo - 32 * x) | low_bits(front - 32 * x));
         }
-        if (!mbar_wait(&bars[wS + u], it & 1)) { tc_fail(9); ok = false; break; }
+        if (!mbar_wait(&bars[wS + 2 * u + (it & 1)], (it >> 1) & 1)) { tc_fail(9); ok = false; break; }
         tc_fence_after_sync();
-        uint32_t s[128];
-        tmem_ld32(S, s);
-        tmem_ld32(S + 32, s + 32);
-        tmem_ld32(S + 64, s + 64);
-        tmem_ld32(S + 96, s + 96);
+        uint32_t s[64];
+        tmem_ld32(Sp, s);
+        tmem_ld32(Sp + 32, s + 32);
         tmem_ld_wait();
         if (!whole) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
+          for (int c = 0; c < 64; ++c)
             if (!(seen[c >> 5] >> (c & 31) & 1)) s[c] = 0xff800000u;
         }
         float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 128; c += 2) most[(c >> 1) & 3] = fmaxf(most[(c >> 1) & 3], fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
+        for (int c = 0; c < 64; c += 2) most[(c >> 1) & 3] = fmaxf(most[(c >> 1) & 3], fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
         const float now = scale * fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
         const bool move = now > top + 8.f;
         if (__any_sync(0xffffffffu, move)) {
@@ -231,10 +247,9 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             }
           }
         }
-        if (!turn()) { tc_fail(14); ok = false; break; }
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < 2; ++x) {
           uint32_t p[16];
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
@@ -243,13 +258,12 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             part[2 + ((c >> 1) & 1)] += p1;
             p[c >> 1] = pack2h<T>(p0, p1);
           }
-          tmem_st16(S + x * 16, p);
+          tmem_st16(Sp + x * 16, p);
         }
-        mbar_arrive(&bars[wTurn + 1 - u]);
         sum += (part[0] + part[1]) + (part[2] + part[3]);
         tmem_st_wait();
         tc_fence_before_sync();
-        mbar_arrive(&bars[wP + u]);
+        mbar_arrive(&bars[wP + 2 * u + (it & 1)]);
         if (ORDERED) mbar_arrive(&bars[wEmpty + n % kStages]);      // the numbers have been read
         first = false;
         ++it;
@@ -283,19 +297,21 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       Work k;
       work_of(w, k);
       const WindowNumbers num(a, k.b);
-      for (int64_t kt = k.both.begin(); kt < k.both.end; kt = k.both.next(kt), ++n) {
+      for (int kt = k.both.begin(); kt < k.both.end; kt = k.both.next(kt), ++n) {
         const int st = n % kStages;
-        int number[4];
+        int number[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) number[e] = num.at(kt * 128 + e * 32 + lane);
+        for (int e = 0; e < 2; ++e) number[e] = num.at((int64_t)kt * kWinTile + e * 32 + lane);
         // the stage has been filled again, so that nobody reads its old numbers
         if (!mbar_wait(&bars[wFullV + st], (n / kStages) & 1)) { tc_fail(12); ok = false; break; }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          reinterpret_cast<int*>(sm + Lay::num)[st * 128 + e * 32 + lane] = number[e];
+        for (int e = 0; e < 2; ++e) {
+          const int j = e * 32 + lane;
+          reinterpret_cast<int*>(sm + Lay::num)[st * kWinTile + j] = number[e];
           if (number[e] < 0) {
 #pragma unroll 1
-            for (int ch = 0; ch < 8 * DB; ++ch) *reinterpret_cast<uint4*>(sm + Lay::v + st * DB * kBox + row_chunk2(e * 32 + lane, ch)) = make_uint4(0, 0, 0, 0);
+            for (int ch = 0; ch < 8 * DB; ++ch)
+              *reinterpret_cast<uint4*>(sm + Lay::v + (st * DB + (ch >> 3)) * Lay::kHalf + row_chunk1(j, ch & 7)) = make_uint4(0, 0, 0, 0);
           }
         }
         fence_async_smem();
@@ -338,8 +354,8 @@ bool window_tc_ok(const WindowArgs& a) {
 int launch_window_fwd_tc(const WindowArgs& a, cudaStream_t stream) {
   const bool bf16 = a.dtype == RFA_BF16;
   CUtensorMap q, k, v;
-  if (make_tmap_heads(&q, a.q.p, bf16, a.T, a.B, a.H, a.D, a.q.t, a.q.b, a.q.h, 128) || make_tmap_heads(&k, a.k.p, bf16, a.S, a.B, a.G, a.D, a.k.t, a.k.b, a.k.h, 128) ||
-      make_tmap_heads(&v, a.v.p, bf16, a.S, a.B, a.G, a.D, a.v.t, a.v.b, a.v.h, 128))
+  if (make_tmap_heads(&q, a.q.p, bf16, a.T, a.B, a.H, a.D, a.q.t, a.q.b, a.q.h, 128) || make_tmap_heads(&k, a.k.p, bf16, a.S, a.B, a.G, a.D, a.k.t, a.k.b, a.k.h, kWinTile) ||
+      make_tmap_heads(&v, a.v.p, bf16, a.S, a.B, a.G, a.D, a.v.t, a.v.b, a.v.h, kWinTile))
     return fail(RFA_EDEVICE, "window_fwd: cuTensorMapEncodeTiled failed or is unavailable");
   if (bf16) return a.D <= 64 ? launch_order<__nv_bfloat16, 1>(q, k, v, a, stream) : launch_order<__nv_bfloat16, 2>(q, k, v, a, stream);
   return a.D <= 64 ? launch_order<__half, 1>(q, k, v, a, stream) : launch_order<__half, 2>(q, k, v, a, stream);
