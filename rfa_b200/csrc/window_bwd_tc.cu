@@ -5,12 +5,13 @@
 // streams tiles of 64 of the other side past them:
 //     S = R1 X1^T, D = R2 X2^T (fp32, TMEM)  ->  P = 2^(S scale log2(e) - lse), dS = P o (D - delta), 16 bits, over S and D
 //     gq += dS X1 (X1 = k);   KEYS: gv += P X2 (X2 = g), gk += dS X1 (X1 = q), over all query heads that share the key head
-// Scores and their gradients have two buffers and two groups of warps, which take the tiles in turn, a thread to each row.  delta = sum of g o out comes from a
+// Scores and their gradients have three places (two where the sums leave no room for a third) and as many groups of warps, which take the tiles in turn, a thread to
+// each row.  delta = sum of g o out comes from a
 // kernel of its own.  Tiles that are seen whole need no mask.  Padded places: as in window_tc.cu, warp 3 fetches numbers (and, KEYS, lse and delta of the queries)
 // and clears the rows that are summed over.
 //
-// Warp roles (384 threads): warp 0 TMA producer, warp 1 issues S and D, warp 2 the sums, warp 3 columns' data, warps 4..7 and 8..11 the two groups.  All waits are
-// bounded.
+// Warp roles (512 or 384 threads): warp 0 TMA producer, warp 1 issues S and D, warp 2 the sums, warp 3 columns' data, warps 4..7, 8..11, 12..15 the groups.  All
+// waits are bounded.
 #define RFA_TC_FAMILY 13
 #include <algorithm>
 
@@ -18,25 +19,29 @@
 
 namespace rfa {
 
-constexpr int kWbThreads = 384, kWbTile = 64;
+constexpr int kWbTile = 64;
 
-template <int DB>
+template <int DB, bool KEYS>
 struct WbLayout {
+  // groups of warps, each with a place for its scores and their gradients: as many as TMEM holds beside the sums
+  static constexpr int kGroups = KEYS && DB == 2 ? 2 : 3, kThreads = 128 + kGroups * 128;
+  static constexpr uint32_t colAcc = kGroups * 128;
+  static_assert(colAcc + DB * 64 * (KEYS ? 2 : 1) <= 512, "TMEM");
   static constexpr int kStages = 4;
   static constexpr uint32_t kHalf = kBox / 2;      // 64 rows of 128 bytes
   static constexpr uint32_t r1 = 0, r2 = DB * kBox, x1 = 2 * DB * kBox, x2 = x1 + kStages * DB * kHalf, num = x2 + kStages * DB * kHalf, lse = num + kStages * kWbTile * 4,
                             delta = lse + kStages * kWbTile * 4, bar = delta + kStages * kWbTile * 4, bytes = bar + 256;
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
-enum { bR = 0, bREmpty, bFull, bEmpty = bFull + 4, bCols = bEmpty + 4, bS = bCols + 4, bP = bS + 2, bFree = bP + 2, bAcc = bFree + 2, bAccFree, bCount };
+enum { bR = 0, bREmpty, bFull, bEmpty = bFull + 4, bCols = bEmpty + 4, bS = bCols + 4, bP = bS + 3, bFree = bP + 3, bAcc = bFree + 3, bAccFree, bCount };
 static_assert(bCount * 8 + 4 <= 256, "barriers");
 
 template <typename T, int DB, bool KEYS, bool ORDERED>
-__global__ void __launch_bounds__(kWbThreads, 1)
+__global__ void __launch_bounds__(WbLayout<DB, KEYS>::kThreads, 1)
 window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_constant__ CUtensorMap tm_r2, const __grid_constant__ CUtensorMap tm_x1,
                      const __grid_constant__ CUtensorMap tm_x2, const __grid_constant__ WindowArgs a, int works) {
-  using Lay = WbLayout<DB>;
-  constexpr int DP = DB * 64, kStages = Lay::kStages;
+  using Lay = WbLayout<DB, KEYS>;
+  constexpr int DP = DB * 64, kStages = Lay::kStages, kGroups = Lay::kGroups;
   constexpr bool kColumns = KEYS || ORDERED;
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::bar);
@@ -63,7 +68,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
   const int other_heads = KEYS ? group : 1;
   if (tid == 0) {
     for (int i = 0; i < bCount; ++i)
-      mbar_init(&bars[i], i >= bEmpty && i < bCols ? (kColumns ? 130 : 2) : i >= bCols && i < bS ? 32 : i >= bP && i < bFree ? 128 : i == bAccFree ? 256 : 1);
+      mbar_init(&bars[i], i >= bEmpty && i < bCols ? (kColumns ? 130 : 2) : i >= bCols && i < bS ? 32 : i >= bP && i < bFree ? 128 : i == bAccFree ? kGroups * 128 : 1);
     mbar_fence_init();
     tma_prefetch_desc(&tm_r1); tma_prefetch_desc(&tm_r2); tma_prefetch_desc(&tm_x1); tma_prefetch_desc(&tm_x2);
   }
@@ -108,7 +113,8 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
       const uint64_t dR1 = umma_smem_desc(sbase + Lay::r1, 0, 1024, kSwizzle128B), dR2 = umma_smem_desc(sbase + Lay::r2, 0, 1024, kSwizzle128B);
       const uint64_t dX1 = umma_smem_desc(sbase + Lay::x1, 0, 1024, kSwizzle128B), dX2 = umma_smem_desc(sbase + Lay::x2, 0, 1024, kSwizzle128B);
       const uint64_t dX1t = umma_smem_desc(sbase + Lay::x1, Lay::kHalf, 1024, kSwizzle128B), dX2t = umma_smem_desc(sbase + Lay::x2, Lay::kHalf, 1024, kSwizzle128B);
-      int n = 0, done = 0;
+      int n = 0, done = 0, buf = 0;      // buf: the tile's place and group; turn: parity of the places' uses
+      uint32_t turn = 0;
       bool ok = true;
       for (int w = blockIdx.x; ok && w < works; w += gridDim.x, ++done) {
         Work k;
@@ -119,24 +125,25 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
         bool first = true;
         for (int h = 0; ok && h < other_heads; ++h)
           for (int t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
-            const int st = n % kStages, buf = n & 1;
+            const int st = n % kStages;
             if (warp == 1) {
               if (!mbar_wait(&bars[ORDERED ? bCols + st : bFull + st], (n / kStages) & 1)) { if (lead) tc_fail(5); ok = false; break; }
-              if (n >= 2 && !mbar_wait(&bars[bFree + buf], ((n >> 1) + 1) & 1)) { if (lead) tc_fail(6); ok = false; break; }
+              if (n >= kGroups && !mbar_wait(&bars[bFree + buf], turn ^ 1)) { if (lead) tc_fail(6); ok = false; break; }
               tc_fence_after_sync();
               umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, tmem + buf * 128, dR1, dX1 + st * kStep, idS, 0);
               umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, tmem + buf * 128 + 64, dR2, dX2 + st * kStep, idS, 0);
               umma_commit_w(lead, &bars[bS + buf]);
               umma_commit_w(lead, &bars[bEmpty + st]);
             } else {
-              if (!mbar_wait(&bars[bP + buf], (n >> 1) & 1)) { if (lead) tc_fail(7); ok = false; break; }
+              if (!mbar_wait(&bars[bP + buf], turn)) { if (lead) tc_fail(7); ok = false; break; }
               tc_fence_after_sync();
-              if constexpr (KEYS) umma_chain_ts<4, kStepMN, kBlockMN>(lead, tmem + 256 + DP, tmem + buf * 128, dX2t + st * kStep, idG, first ? 0u : 1u);
-              umma_chain_ts<4, kStepMN, kBlockMN>(lead, tmem + 256, tmem + buf * 128 + 64, dX1t + st * kStep, idG, first ? 0u : 1u);
+              if constexpr (KEYS) umma_chain_ts<4, kStepMN, kBlockMN>(lead, tmem + Lay::colAcc + DP, tmem + buf * 128, dX2t + st * kStep, idG, first ? 0u : 1u);
+              umma_chain_ts<4, kStepMN, kBlockMN>(lead, tmem + Lay::colAcc, tmem + buf * 128 + 64, dX1t + st * kStep, idG, first ? 0u : 1u);
               umma_commit_w(lead, &bars[bFree + buf]);
               umma_commit_w(lead, &bars[bEmpty + st]);
               first = false;
             }
+            if (++buf == kGroups) { buf = 0; turn ^= 1; }
           }
         if (ok) umma_commit_w(lead, &bars[warp == 1 ? bREmpty : bAcc]);
       }
@@ -188,12 +195,13 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
       }
     }
   } else {
-    // ------------------------------------------------------------------ groups: a thread to each row, every other tile
+    // ------------------------------------------------------------------ groups: a thread to each row, one tile of kGroups
     const int g = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, S = tmem + lanes + g * 128, D = S + 64, acc = tmem + lanes + 256;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, S = tmem + lanes + g * 128, D = S + 64, acc = tmem + lanes + Lay::colAcc;
     const float scale = a.scale * kLog2e;
     const auto sectors = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; };
-    int n = 0, done = 0;
+    int n = 0, done = 0, buf = 0;
+    uint32_t turn = 0;
     bool ok = true;
     for (int w = blockIdx.x; ok && w < works; w += gridDim.x, ++done) {
       Work k;
@@ -208,7 +216,10 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
       }
       for (int h = 0; ok && h < other_heads; ++h)
         for (int t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
-          if ((n & 1) != g) continue;
+          const bool ours = buf == g;
+          const uint32_t use = turn;
+          if (++buf == kGroups) { buf = 0; turn ^= 1; }
+          if (!ours) continue;
           const int st = n % kStages;
           const int64_t c0 = (int64_t)t * kWbTile;
           bool whole;
@@ -242,18 +253,17 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
 #pragma unroll
             for (int x = 0; x < 2; ++x) seen[x] = low_bits(hi - 32 * x) & (~low_bits(lo - 32 * x) | low_bits(front - 32 * x));
           }
-          if (!mbar_wait(&bars[bS + g], (n >> 1) & 1)) { tc_fail(10); ok = false; break; }
+          if (!mbar_wait(&bars[bS + g], use)) { tc_fail(10); ok = false; break; }
           tc_fence_after_sync();
           const float* cl = reinterpret_cast<const float*>(sm + Lay::lse) + st * kWbTile;
           const float* cd = reinterpret_cast<const float*>(sm + Lay::delta) + st * kWbTile;
-          uint32_t s[64], d[64];
-          tmem_ld32(S, s);
-          tmem_ld32(D, d);
-          tmem_ld32(S + 32, s + 32);
-          tmem_ld32(D + 32, d + 32);
-          tmem_ld_wait();
+          // 32 columns at a time: P takes the first half of the place of the scores that it is made of
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
+            uint32_t s[32], d[32];
+            tmem_ld32(S + x * 32, s);
+            tmem_ld32(D + x * 32, d);
+            tmem_ld_wait();
             uint32_t pw[16], dw[16];
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
@@ -265,9 +275,8 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
               }
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
-                const int at = x * 32 + c + y;
-                p[y] = ex2(fmaf(__uint_as_float(s[at]), scale, -l[y]));
-                ds[y] = p[y] * (__uint_as_float(d[at]) - e[y]);
+                p[y] = ex2(fmaf(__uint_as_float(s[c + y]), scale, -l[y]));
+                ds[y] = p[y] * (__uint_as_float(d[c + y]) - e[y]);
                 if (!whole && !(seen[x] >> (c + y) & 1)) p[y] = ds[y] = 0.f;
               }
               pw[c >> 1] = pack2h<T>(p[0], p[1]);
@@ -284,7 +293,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
           if (kColumns) mbar_arrive(&bars[bEmpty + st]);
         }
       if (!ok) break;
-      // ---- the gradients: the groups take every other 16 columns
+      // ---- the gradients: the groups take 16 columns in turn
       if (!mbar_wait(&bars[bAcc], done & 1)) { tc_fail(11); break; }
       tc_fence_after_sync();
       const int heads = KEYS ? a.G : a.H;
@@ -294,7 +303,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
         T* out = static_cast<T*>(to) + at;
         const bool wide = a.D % 16 == 0 && sectors(to);
 #pragma unroll 1
-        for (int c0 = g * 16; c0 < DP; c0 += 32) {
+        for (int c0 = g * 16; c0 < DP; c0 += kGroups * 16) {
           uint32_t u[16];
           tmem_ld16(from + c0, u);
           tmem_ld_wait();
@@ -343,12 +352,13 @@ namespace {
 
 template <typename T, int DB, bool KEYS, bool ORDERED>
 int launch(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& x1, const CUtensorMap& x2, const WindowArgs& a, cudaStream_t stream) {
-  constexpr uint32_t smem = WbLayout<DB>::bytes;
+  using Lay = WbLayout<DB, KEYS>;
+  constexpr uint32_t smem = Lay::bytes;
   cudaError_t e = cudaFuncSetAttribute(window_bwd_tc_kernel<T, DB, KEYS, ORDERED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return fail((int)e, "window_bwd: cannot reserve %u bytes of shared memory: %s", smem, cudaGetErrorString(e));
   const int64_t works = (a.T + 127) / 128 * a.B * (KEYS ? a.G : a.H);
   RFA_REQUIRE(works < (int64_t)1 << 31, RFA_EUNSUPPORTED, "window_bwd: %lld tiles", (long long)works);
-  e = launch_pdl(window_bwd_tc_kernel<T, DB, KEYS, ORDERED>, dim3((unsigned)std::min<int64_t>(works, 148)), dim3(kWbThreads), smem, stream, r1, r2, x1, x2, a, (int)works);
+  e = launch_pdl(window_bwd_tc_kernel<T, DB, KEYS, ORDERED>, dim3((unsigned)std::min<int64_t>(works, 148)), dim3(Lay::kThreads), smem, stream, r1, r2, x1, x2, a, (int)works);
   if (e != cudaSuccess) return fail((int)e, "rfa_window_bwd: launch failed: %s", cudaGetErrorString(e));
   return check_launch("rfa_window_bwd");
 }
