@@ -49,22 +49,24 @@ struct DecLayout {
   static constexpr uint32_t kCopyBytes = KB * DB * 64 * 128;            // S's copy: DB boxes of [KB 64][64]
   static constexpr uint32_t kCopyRoom = KB == 1 ? kBox : kCopyBytes;    // an operand's second 64-block may be read past a single box
   static constexpr int kCopies = OUT ? 1 : 2;                           // one on its way to memory while the next is written
-  static constexpr uint32_t kFixed = (EXACT ? KB * kBox : 0) + kCopies * kCopyRoom, kStage = (KB + DB) * kBox, kTail = 4 * 128 * 4 + 16 + 400;
-  static constexpr int fit(int extra) { return (int)((227 * 1024 - kTail - kFixed - extra) / (kStage + (OUT ? KB * kBox : 0))); }
-  static constexpr int kStages = fit(0) >= 2 ? (fit(0) < kDecMaxStages ? fit(0) : kDecMaxStages) : 2, kQStages = !OUT ? 0 : fit(0) >= 2 ? kStages : 1;
+  static constexpr uint32_t kFixed = (EXACT ? KB * kBox : 0) + kCopies * kCopyRoom, kStage = (KB + DB) * kBox, kTail = 8 * 128 * 4 + 32 + 400;
+  static constexpr int kFit = (int)((227 * 1024 - kTail - kFixed) / (kStage + (OUT ? KB * kBox : 0)));
+  static constexpr int kStages = kFit >= 2 ? (kFit < kDecMaxStages ? kFit : kDecMaxStages) : 2, kQStages = !OUT ? 0 : kFit >= 2 ? kStages : 1;
+  static constexpr int kL = kFit >= 2 ? 4 : 2;                          // chunks' decays at a time: they run ahead of what waits for the state
   static constexpr uint32_t q = 0, k = q + kQStages * KB * kBox, v = k + kStages * KB * kBox, low = v + kStages * DB * kBox, copy = low + (EXACT ? KB * kBox : 0);
   static constexpr uint32_t l = copy + kCopies * kCopyRoom;
-  static constexpr uint32_t key_fac = l + 2 * 128 * 4, fac = key_fac + 2 * 128 * 4, bar = fac + 16, bytes = bar + 400;
+  static constexpr uint32_t key_fac = l + kL * 128 * 4, fac = key_fac + kL * 128 * 4, bar = fac + 8 * kL, bytes = bar + 400;
   static constexpr int kA = OUT && DB == 1 ? 2 : 1;                     // buffers of A
   static constexpr uint32_t colS = 0, colN = DB * 64, colO = 2 * DB * 64, colA = 3 * DB * 64, cols = 512;
   static_assert(colA + kA * 128 <= 512, "TMEM");
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
-enum { dFullQ = 0, dFullK = 5, dFullV = 10, dEmptyQ = 15, dEmptyK = 20, dEmptyV = 25, dL = 30, dLFree = 32, dA = 34, dP = 36, dKp = 38, dClean = 40, dS = 42, dSt, dN, dNFree, dKept, dNum };
+enum { dFull = 0, dFree = 5, dFullQ = 10, dFreeQ, dL = 12, dLFree = 16, dA = 20, dP = 22, dKp = 24, dClean = 28, dS = 32, dSt, dNFree, dKept, dNum };
 static_assert(dNum * 8 + 4 <= 400, "barriers");
+// dFull, dFree: a stage's tiles have come, all products of its chunk are complete (out may be read); dFullQ, dFreeQ: the same of Q where it has one stage only.
 // dL / dLFree: a chunk's L and factors are there, have been used.  dClean: the rows of padded tokens are zero (waited for where there is a mask).  dKp: K' stands in
 // place of K.  dS: the state's MMAs of a chunk are complete.  dSt: the copy of the state and the decayed state are there.  Barriers in pairs alternate with the
-// chunk where their waiter could otherwise be two phases behind (nobody is more than two chunks ahead, by dLFree).
+// chunk where their waiter could otherwise be two phases behind (the decays, and so the key group, are at most kL chunks ahead, by dLFree).
 
 template <typename T, int KB, int DB, bool OUT, bool EXACT>
 __global__ void __launch_bounds__(kDecThreads, 1)
@@ -72,6 +74,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 const __grid_constant__ DecayTcArgs a, bool totals_only) {
   using Lay = DecLayout<KB, DB, OUT, EXACT>;
   constexpr int KP = KB * 64, DP = DB * 64;
+  constexpr bool kOneQ = Lay::kQStages == 1;
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::bar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + dNum);
@@ -88,12 +91,15 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const auto chunk_t0 = [&](int c) { return t_begin + (int64_t)(a.rev ? nchunk - 1 - c : c) * kTC; };
 
   if (tid == 0) {
-    for (int i = 0; i < dL; ++i) mbar_init(&bars[i], OUT && (i >= dEmptyV || (i >= dEmptyQ && i < dEmptyK)) ? 2 : 1);      // both issuers read Q and V
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < dL; ++i) mbar_init(&bars[i], OUT && (i >= dFree && i != dFullQ) ? 2 : 1);      // both issuers
+    for (int i = 0; i < Lay::kL; ++i) {
       mbar_init(&bars[dL + i], 32); mbar_init(&bars[dLFree + i], OUT ? 128 : 256);
-      mbar_init(&bars[dA + i], 1); mbar_init(&bars[dP + i], 128); mbar_init(&bars[dKp + i], 128); mbar_init(&bars[dClean + i], 128);
+      mbar_init(&bars[dKp + i], 128); mbar_init(&bars[dClean + i], 128);
     }
-    mbar_init(&bars[dS], 1); mbar_init(&bars[dSt], 256); mbar_init(&bars[dN], 2); mbar_init(&bars[dNFree], 128); mbar_init(&bars[dKept], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars[dA + i], 1); mbar_init(&bars[dP + i], 128);
+    }
+    mbar_init(&bars[dS], 1); mbar_init(&bars[dSt], 256); mbar_init(&bars[dNFree], 128); mbar_init(&bars[dKept], 1);
     mbar_fence_init();
     if (OUT) tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
@@ -111,18 +117,18 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (lane == 0) {
       for (int c = 0; c < nchunk; ++c) {
         const int st = c % Lay::kStages, n = c / Lay::kStages, t0 = (int)chunk_t0(c);
-        if (n >= 1 && !mbar_wait(&bars[dEmptyK + st], (n + 1) & 1)) { tc_fail(1); break; }
-        mbar_arrive_expect_tx(&bars[dFullK + st], KB * kBox);
-        for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::k + (st * KB + x) * kBox, &tm_k, &bars[dFullK + st], x * 64, h, b, t0);
+        if (n >= 1 && !mbar_wait(&bars[dFree + st], (n + 1) & 1)) { tc_fail(1); break; }
+        mbar_arrive_expect_tx(&bars[dFull + st], (KB + DB + (OUT && !kOneQ ? KB : 0)) * kBox);
+        for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::k + (st * KB + x) * kBox, &tm_k, &bars[dFull + st], x * 64, h, b, t0);
+        for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + (st * DB + x) * kBox, &tm_v, &bars[dFull + st], x * 64, h, b, t0);
         if constexpr (OUT) {
-          const int qs = c % Lay::kQStages, qn = c / Lay::kQStages;
-          if (qn >= 1 && !mbar_wait(&bars[dEmptyQ + qs], (qn + 1) & 1)) { tc_fail(2); break; }
-          mbar_arrive_expect_tx(&bars[dFullQ + qs], KB * kBox);
-          for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::q + (qs * KB + x) * kBox, &tm_q, &bars[dFullQ + qs], x * 64, h, b, t0);
+          uint64_t* full = &bars[kOneQ ? dFullQ : dFull + st];
+          if (kOneQ) {
+            if (c >= 1 && !mbar_wait(&bars[dFreeQ], (c + 1) & 1)) { tc_fail(2); break; }
+            mbar_arrive_expect_tx(full, KB * kBox);
+          }
+          for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::q + ((kOneQ ? 0 : st) * KB + x) * kBox, &tm_q, full, x * 64, h, b, t0);
         }
-        if (n >= 1 && !mbar_wait(&bars[dEmptyV + st], (n + 1) & 1)) { tc_fail(3); break; }
-        mbar_arrive_expect_tx(&bars[dFullV + st], DB * kBox);
-        for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + (st * DB + x) * kBox, &tm_v, &bars[dFullV + st], x * 64, h, b, t0);
       }
     }
   } else if (warp == 1 || warp == 18) {
@@ -136,20 +142,19 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const uint64_t dKt = umma_smem_desc(sbase + Lay::k, kBox, 1024, kSwizzle128B), dLow = umma_smem_desc(sbase + Lay::low, kBox, 1024, kSwizzle128B);
       const uint64_t dV = umma_smem_desc(sbase + Lay::v, kBox, 1024, kSwizzle128B), dC = umma_smem_desc(sbase + Lay::copy, KP * 128, 1024, kSwizzle128B);
       constexpr uint64_t kK = (KB * kBox) >> 4, kV = (DB * kBox) >> 4;
-      constexpr int kQS = OUT ? Lay::kQStages : 1;
       if (warp == 1) {
         // ---- issuer A: the scores of the next chunk as early as they can be, O = P V
         if constexpr (OUT) {
           const auto issue_A = [&](int c) {
             const int before = c - Lay::kA;      // the key group has seen this buffer's last completion
-            if (before >= 0 && !mbar_wait(&bars[dKp + (before & 1)], (before >> 1) & 1)) { tc_fail(27); return false; }
-            const int qs = c % kQS, ab = Lay::kA == 2 ? c & 1 : 0, ks = c % Lay::kStages;
-            if (!mbar_wait(&bars[dFullQ + qs], (c / kQS) & 1) || !mbar_wait(&bars[dFullK + ks], (c / Lay::kStages) & 1)) { tc_fail(4); return false; }
-            if (mask && !mbar_wait(&bars[dClean + (c & 1)], (c >> 1) & 1)) { tc_fail(5); return false; }
+            if (before >= 0 && !mbar_wait(&bars[dKp + before % Lay::kL], (before / Lay::kL) & 1)) { tc_fail(27); return false; }
+            const int ab = Lay::kA == 2 ? c & 1 : 0, st = c % Lay::kStages;
+            if (!mbar_wait(&bars[dFull + st], (c / Lay::kStages) & 1) || (kOneQ && !mbar_wait(&bars[dFullQ], c & 1))) { tc_fail(4); return false; }
+            if (mask && !mbar_wait(&bars[dClean + c % Lay::kL], (c / Lay::kL) & 1)) { tc_fail(5); return false; }
             tc_fence_after_sync();
-            umma_chain_ss<4 * KB, kStepK, kBlockK, kStepK, kBlockK>(lead, tmem + Lay::colA + ab * 128, dQ + qs * kK, dK + ks * kK, idA, 0);
+            umma_chain_ss<4 * KB, kStepK, kBlockK, kStepK, kBlockK>(lead, tmem + Lay::colA + ab * 128, dQ + (kOneQ ? 0 : st) * kK, dK + st * kK, idA, 0);
             umma_commit(&bars[dA + ab]);
-            umma_commit(&bars[dEmptyQ + qs]);
+            if (kOneQ) umma_commit(&bars[dFreeQ]);
             return true;
           };
           bool ok = nchunk > 0 && issue_A(0);
@@ -157,38 +162,33 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           for (int c = 0; ok && c < nchunk; ++c) {
             const int st = c % Lay::kStages, ab = Lay::kA == 2 ? c & 1 : 0, an = Lay::kA == 2 ? c >> 1 : c;
             if (Lay::kA == 2 && c + 1 < nchunk && !issue_A(c + 1)) break;
-            if (!mbar_wait(&bars[dFullV + st], (c / Lay::kStages) & 1)) { tc_fail(24); break; }
             if (c >= 1 && !mbar_wait(&bars[dNFree], (c + 1) & 1)) { tc_fail(25); break; }
             if (!mbar_wait(&bars[dP + ab], an & 1)) { tc_fail(9); break; }
             tc_fence_after_sync();
             umma_chain_ts<8, kStepMN, kBlockMN>(lead, tmem + Lay::colO, tmem + Lay::colA + ab * 128, dV + st * kV, idN, 0);
-            umma_commit(&bars[dN]);
-            umma_commit(&bars[dEmptyV + st]);
+            umma_commit(&bars[dFree + st]);
             if (Lay::kA == 1 && c + 1 < nchunk && !issue_A(c + 1)) break;
           }
         }
       } else {
-        // ---- issuer B: N = Q S, S += K'^T V
+        // ---- issuer B: S += K'^T V, N = Q S
 #pragma unroll 1
         for (int c = 0; c < nchunk; ++c) {
           const int st = c % Lay::kStages;
-          if (!mbar_wait(&bars[dKp + (c & 1)], (c >> 1) & 1) || !mbar_wait(&bars[dFullV + st], (c / Lay::kStages) & 1)) { tc_fail(8); break; }
+          if (!mbar_wait(&bars[dFull + st], (c / Lay::kStages) & 1) || !mbar_wait(&bars[dKp + c % Lay::kL], (c / Lay::kL) & 1)) { tc_fail(8); break; }
           if (!mbar_wait(&bars[dSt], c & 1)) { tc_fail(6); break; }
           tc_fence_after_sync();
           umma_chain_ss<8, kStepMN, kBlockMN, kStepMN, kBlockMN>(lead, tmem + Lay::colS, dKt + st * kK, dV + st * kV, idS, 1);
           if (EXACT) umma_chain_ss<8, kStepMN, kBlockMN, kStepMN, kBlockMN>(lead, tmem + Lay::colS, dLow, dV + st * kV, idS, 1);
-          umma_commit(&bars[dEmptyK + st]);
-          umma_commit(&bars[dEmptyV + st]);
           if constexpr (OUT) {
-            const int qs = c % kQS;
-            if (!mbar_wait(&bars[dFullQ + qs], (c / kQS) & 1)) { tc_fail(26); break; }
+            if (kOneQ && !mbar_wait(&bars[dFullQ], c & 1)) { tc_fail(26); break; }
             if (c >= 1 && !mbar_wait(&bars[dNFree], (c + 1) & 1)) { tc_fail(7); break; }
             tc_fence_after_sync();
-            umma_chain_ss<4 * KB, kStepK, kBlockK, kStepMN, kBlockMN>(lead, tmem + Lay::colN, dQ + qs * kK, dC, idN, 0);
-            umma_commit(&bars[dN]);
-            umma_commit(&bars[dEmptyQ + qs]);
+            umma_chain_ss<4 * KB, kStepK, kBlockK, kStepMN, kBlockMN>(lead, tmem + Lay::colN, dQ + (kOneQ ? 0 : st) * kK, dC, idN, 0);
+            if (kOneQ) umma_commit(&bars[dFreeQ]);
           }
           umma_commit(&bars[dS]);                // the copy has been read, too
+          umma_commit(&bars[dFree + st]);
         }
       }
     }
@@ -200,8 +200,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       for (int c = 0; c < nchunk; ++c) {
         const int ab = Lay::kA == 2 ? c & 1 : 0, an = Lay::kA == 2 ? c >> 1 : c;
         const uint32_t col = tmem + lane_addr + Lay::colA + ab * 128;
-        if (!mbar_wait(&bars[dL + (c & 1)], (c >> 1) & 1)) { tc_fail(10); break; }
-        const float* L = Ls + (c & 1) * 128;
+        if (!mbar_wait(&bars[dL + c % Lay::kL], (c / Lay::kL) & 1)) { tc_fail(10); break; }
+        const float* L = Ls + c % Lay::kL * 128;
         const float mine = L[row];
         if (!mbar_wait(&bars[dA + ab], an & 1)) { tc_fail(11); break; }
         tc_fence_after_sync();
@@ -302,8 +302,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (!mbar_wait(&bars[dS], c & 1)) { tc_fail(13); ok = false; break; }
       tc_fence_after_sync();
       if (c + 1 < nchunk) {
-        if (!mbar_wait(&bars[dL + ((c + 1) & 1)], ((c + 1) >> 1) & 1)) { tc_fail(14); ok = false; break; }
-        const Factor f = fac[(c + 1) & 1];
+        if (!mbar_wait(&bars[dL + (c + 1) % Lay::kL], ((c + 1) / Lay::kL) & 1)) { tc_fail(14); ok = false; break; }
+        const Factor f = fac[(c + 1) % Lay::kL];
         uint32_t next[16];
         tmem_ld16(tmem + lane_addr + Lay::colS + col0, next);
 #pragma unroll 1
@@ -320,7 +320,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         tc_fence_before_sync();
         mbar_arrive(&bars[dSt]);
       }
-      if (!OUT) mbar_arrive(&bars[dLFree + (c & 1)]);
+      if (!OUT) mbar_arrive(&bars[dLFree + c % Lay::kL]);
     }
     // the state behind the last chunk; the last wait on dS ordered it
     float* dst = !ok ? nullptr : totals_only ? a.totals + slot : a.s_out.p && seg == a.nseg - 1 ? a.s_out.p + bh * a.K * a.D : nullptr;
@@ -353,11 +353,11 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
       const bool wide = a.D % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
       for (int c = 0; c < nchunk; ++c) {
-        if (!mbar_wait(&bars[dL + (c & 1)], (c >> 1) & 1) || !mbar_wait(&bars[dN], c & 1)) { tc_fail(15); break; }
+        if (!mbar_wait(&bars[dL + c % Lay::kL], (c / Lay::kL) & 1) || !mbar_wait(&bars[dFree + c % Lay::kStages], (c / Lay::kStages) & 1)) { tc_fail(15); break; }
         tc_fence_after_sync();
         const int64_t t = chunk_t0(c) + row;
         const bool there = t < t_end, gone = there && mask && mask[t];
-        const float f = a.out_scale * ex2(Ls[(c & 1) * 128 + row]);
+        const float f = a.out_scale * ex2(Ls[c % Lay::kL * 128 + row]);
         T* o = static_cast<T*>(a.out) + ((t * a.B + b) * a.H + h) * a.D;
 #pragma unroll 1
         for (int c0 = 0; c0 < DP; c0 += 16) {
@@ -374,7 +374,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           for (int i = 0; i < 16; ++i) v[i] = gone ? 0.f : fmaf(f, __uint_as_float(n[i]), a.out_scale * __uint_as_float(p[i]));
           if (there && c0 < a.D) store_row16(o + c0, v, a.D - c0, wide);
         }
-        mbar_arrive(&bars[dLFree + (c & 1)]);
+        mbar_arrive(&bars[dLFree + c % Lay::kL]);
       }
     }
   } else if (warp == 19) {
@@ -396,7 +396,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     };
     if (nchunk > 0) ask(0);
     for (int c = 0; c < nchunk; ++c) {
-      const int lb = c & 1;
+      const int lb = c % Lay::kL;
       double L[4], all = 0.0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -421,7 +421,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         f[e] = a.in_scale * exp2f((float)(a.rev ? L[e] : end - L[e]));
       }
       const Factor whole((float)(end / kLog2eD));
-      if (c >= 2 && !mbar_wait(&bars[dLFree + lb], ((c >> 1) + 1) & 1)) { tc_fail(17); break; }
+      if (c >= Lay::kL && !mbar_wait(&bars[dLFree + lb], (c / Lay::kL + 1) & 1)) { tc_fail(17); break; }
       *reinterpret_cast<float4*>(Ls + lb * 128 + lane * 4) = make_float4(l[0], l[1], l[2], l[3]);
       *reinterpret_cast<float4*>(key_fac + lb * 128 + lane * 4) = make_float4(f[0], f[1], f[2], f[3]);
       if (lane == 0) fac[lb] = whole;
@@ -433,13 +433,13 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const int j = tid - 320;
     uint8_t ahead = mask && nchunk > 0 && chunk_t0(0) + j < t_end ? mask[chunk_t0(0) + j] : 0;
     for (int c = 0; c < nchunk; ++c) {
-      const int st = c % Lay::kStages, lb = c & 1;
+      const int st = c % Lay::kStages, lb = c % Lay::kL;
       const uint32_t filled = (c / Lay::kStages) & 1;
       unsigned char* krow = sm + Lay::k + st * KB * kBox;
       if (mask) {      // padded rows of K and V may hold anything: zero before a product reads them
         const bool gone = ahead;
         if (c + 1 < nchunk) ahead = chunk_t0(c + 1) + j < t_end ? mask[chunk_t0(c + 1) + j] : 0;
-        if (!mbar_wait(&bars[dFullK + st], filled) || !mbar_wait(&bars[dFullV + st], filled)) { tc_fail(18); break; }
+        if (!mbar_wait(&bars[dFull + st], filled)) { tc_fail(18); break; }
         if (gone) {
 #pragma unroll
           for (int ch = 0; ch < 8 * KB; ++ch) *reinterpret_cast<uint4*>(krow + row_chunk2(j, ch)) = make_uint4(0, 0, 0, 0);
@@ -449,12 +449,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         fence_async_smem();
         mbar_arrive(&bars[dClean + lb]);
       }
-      if (!mbar_wait(&bars[dL + lb], (c >> 1) & 1)) { tc_fail(16); break; }
-      const float f = key_fac[lb * 128 + j];
+      if (!mbar_wait(&bars[dL + c % Lay::kL], (c / Lay::kL) & 1)) { tc_fail(16); break; }
+      const float f = key_fac[c % Lay::kL * 128 + j];
       if (OUT) {
-        const int ab = Lay::kA == 2 ? lb : 0, an = Lay::kA == 2 ? c >> 1 : c;
+        const int ab = Lay::kA == 2 ? c & 1 : 0, an = Lay::kA == 2 ? c >> 1 : c;
         if (!mbar_wait(&bars[dA + ab], an & 1)) { tc_fail(21); break; }
-      } else if (!mbar_wait(&bars[dFullK + st], filled)) { tc_fail(22); break; }
+      } else if (!mbar_wait(&bars[dFull + st], filled)) { tc_fail(22); break; }
       if (EXACT && c >= 1 && !mbar_wait(&bars[dS], (c + 1) & 1)) { tc_fail(23); break; }      // the second part of the chunk before has been read
 #pragma unroll 1
       for (int c8 = 0; c8 < 8 * KB; c8 += 2) {

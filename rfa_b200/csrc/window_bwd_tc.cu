@@ -68,7 +68,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
   const int other_heads = KEYS ? group : 1;
   if (tid == 0) {
     for (int i = 0; i < bCount; ++i)
-      mbar_init(&bars[i], i >= bEmpty && i < bCols ? (kColumns ? 130 : 2) : i >= bCols && i < bS ? 32 : i >= bP && i < bFree ? 128 : i == bAccFree ? kGroups * 128 : 1);
+      mbar_init(&bars[i], i >= bEmpty && i < bCols ? (kColumns ? 129 : 1) : i >= bCols && i < bS ? 32 : i >= bP && i < bFree ? 128 : i == bAccFree ? kGroups * 128 : 1);
     mbar_fence_init();
     tma_prefetch_desc(&tm_r1); tma_prefetch_desc(&tm_r2); tma_prefetch_desc(&tm_x1); tma_prefetch_desc(&tm_x2);
   }
@@ -132,8 +132,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
               tc_fence_after_sync();
               umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, tmem + buf * 128, dR1, dX1 + st * kStep, idS, 0);
               umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, tmem + buf * 128 + 64, dR2, dX2 + st * kStep, idS, 0);
-              umma_commit_w(lead, &bars[bS + buf]);
-              umma_commit_w(lead, &bars[bEmpty + st]);
+              umma_commit_w(lead, &bars[bS + buf]);      // the stage is given back by the sums, which come after
             } else {
               if (!mbar_wait(&bars[bP + buf], turn)) { if (lead) tc_fail(7); ok = false; break; }
               tc_fence_after_sync();
