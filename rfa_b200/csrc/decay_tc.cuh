@@ -51,9 +51,11 @@ struct DecLayout {
   static constexpr int kCopies = OUT ? 1 : 2;                           // one on its way to memory while the next is written
   static constexpr uint32_t kFixed = (EXACT ? KB * kBox : 0) + kCopies * kCopyRoom, kStage = (KB + DB) * kBox, kTail = 8 * 128 * 4 + 32 + 400;
   static constexpr int kFit = (int)((227 * 1024 - kTail - kFixed) / (kStage + (OUT ? KB * kBox : 0)));
-  static constexpr int kStages = kFit >= 2 ? (kFit < kDecMaxStages ? kFit : kDecMaxStages) : 2, kQStages = !OUT ? 0 : kFit >= 2 ? kStages : 1;
+  static constexpr int kStages = kFit >= 2 ? (kFit < kDecMaxStages ? kFit : kDecMaxStages) : 2, kQStages = OUT ? kStages : 0;
+  // Where two whole stages have no room it is V that has one place: its load runs beside the key group's work, Q's would run in front of it.
+  static constexpr int kVStages = OUT && kFit < 2 ? 1 : kStages;
   static constexpr int kL = kFit >= 2 ? 4 : 2;                          // chunks' decays at a time: they run ahead of what waits for the state
-  static constexpr uint32_t q = 0, k = q + kQStages * KB * kBox, v = k + kStages * KB * kBox, low = v + kStages * DB * kBox, copy = low + (EXACT ? KB * kBox : 0);
+  static constexpr uint32_t q = 0, k = q + kQStages * KB * kBox, v = k + kStages * KB * kBox, low = v + kVStages * DB * kBox, copy = low + (EXACT ? KB * kBox : 0);
   static constexpr uint32_t l = copy + kCopies * kCopyRoom;
   static constexpr uint32_t key_fac = l + kL * 128 * 4, fac = key_fac + kL * 128 * 4, bar = fac + 8 * kL, bytes = bar + 400;
   static constexpr int kA = OUT && DB == 1 ? 2 : 1;                     // buffers of A
@@ -61,9 +63,9 @@ struct DecLayout {
   static_assert(colA + kA * 128 <= 512, "TMEM");
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
-enum { dFull = 0, dFree = 5, dFullQ = 10, dFreeQ, dL = 12, dLFree = 16, dA = 20, dP = 22, dKp = 24, dClean = 28, dS = 32, dSt, dNFree, dKept, dNum };
+enum { dFull = 0, dFree = 5, dFullV = 10, dFreeV, dL = 12, dLFree = 16, dA = 20, dP = 22, dKp = 24, dClean = 28, dS = 32, dSt, dNFree, dKept, dNum };
 static_assert(dNum * 8 + 4 <= 400, "barriers");
-// dFull, dFree: a stage's tiles have come, all products of its chunk are complete (out may be read); dFullQ, dFreeQ: the same of Q where it has one stage only.
+// dFull, dFree: a stage's tiles have come, all products of its chunk are complete (out may be read); dFullV, dFreeV: the same of V where it has one place only.
 // dL / dLFree: a chunk's L and factors are there, have been used.  dClean: the rows of padded tokens are zero (waited for where there is a mask).  dKp: K' stands in
 // place of K.  dS: the state's MMAs of a chunk are complete.  dSt: the copy of the state and the decayed state are there.  Barriers in pairs alternate with the
 // chunk where their waiter could otherwise be two phases behind (the decays, and so the key group, are at most kL chunks ahead, by dLFree).
@@ -74,7 +76,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 const __grid_constant__ DecayTcArgs a, bool totals_only) {
   using Lay = DecLayout<KB, DB, OUT, EXACT>;
   constexpr int KP = KB * 64, DP = DB * 64;
-  constexpr bool kOneQ = Lay::kQStages == 1;
+  constexpr bool kOneV = Lay::kVStages == 1;
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::bar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + dNum);
@@ -91,7 +93,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const auto chunk_t0 = [&](int c) { return t_begin + (int64_t)(a.rev ? nchunk - 1 - c : c) * kTC; };
 
   if (tid == 0) {
-    for (int i = 0; i < dL; ++i) mbar_init(&bars[i], OUT && (i >= dFree && i != dFullQ) ? 2 : 1);      // both issuers
+    for (int i = 0; i < dL; ++i) mbar_init(&bars[i], OUT && (i >= dFree && i != dFullV) ? 2 : 1);      // both issuers
     for (int i = 0; i < Lay::kL; ++i) {
       mbar_init(&bars[dL + i], 32); mbar_init(&bars[dLFree + i], OUT ? 128 : 256);
       mbar_init(&bars[dKp + i], 128); mbar_init(&bars[dClean + i], 128);
@@ -118,17 +120,16 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       for (int c = 0; c < nchunk; ++c) {
         const int st = c % Lay::kStages, n = c / Lay::kStages, t0 = (int)chunk_t0(c);
         if (n >= 1 && !mbar_wait(&bars[dFree + st], (n + 1) & 1)) { tc_fail(1); break; }
-        mbar_arrive_expect_tx(&bars[dFull + st], (KB + DB + (OUT && !kOneQ ? KB : 0)) * kBox);
+        mbar_arrive_expect_tx(&bars[dFull + st], (KB + (OUT ? KB : 0) + (kOneV ? 0 : DB)) * kBox);
         for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::k + (st * KB + x) * kBox, &tm_k, &bars[dFull + st], x * 64, h, b, t0);
-        for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + (st * DB + x) * kBox, &tm_v, &bars[dFull + st], x * 64, h, b, t0);
-        if constexpr (OUT) {
-          uint64_t* full = &bars[kOneQ ? dFullQ : dFull + st];
-          if (kOneQ) {
-            if (c >= 1 && !mbar_wait(&bars[dFreeQ], (c + 1) & 1)) { tc_fail(2); break; }
-            mbar_arrive_expect_tx(full, KB * kBox);
-          }
-          for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::q + ((kOneQ ? 0 : st) * KB + x) * kBox, &tm_q, full, x * 64, h, b, t0);
+        if constexpr (OUT)
+          for (int x = 0; x < KB; ++x) tma_load_4d(sm + Lay::q + (st * KB + x) * kBox, &tm_q, &bars[dFull + st], x * 64, h, b, t0);
+        uint64_t* full = &bars[kOneV ? dFullV : dFull + st];
+        if (kOneV) {
+          if (c >= 1 && !mbar_wait(&bars[dFreeV], (c + 1) & 1)) { tc_fail(2); break; }
+          mbar_arrive_expect_tx(full, DB * kBox);
         }
+        for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + ((kOneV ? 0 : st) * DB + x) * kBox, &tm_v, full, x * 64, h, b, t0);
       }
     }
   } else if (warp == 1 || warp == 18) {
@@ -149,12 +150,11 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             const int before = c - Lay::kA;      // the key group has seen this buffer's last completion
             if (before >= 0 && !mbar_wait(&bars[dKp + before % Lay::kL], (before / Lay::kL) & 1)) { tc_fail(27); return false; }
             const int ab = Lay::kA == 2 ? c & 1 : 0, st = c % Lay::kStages;
-            if (!mbar_wait(&bars[dFull + st], (c / Lay::kStages) & 1) || (kOneQ && !mbar_wait(&bars[dFullQ], c & 1))) { tc_fail(4); return false; }
+            if (!mbar_wait(&bars[dFull + st], (c / Lay::kStages) & 1)) { tc_fail(4); return false; }
             if (mask && !mbar_wait(&bars[dClean + c % Lay::kL], (c / Lay::kL) & 1)) { tc_fail(5); return false; }
             tc_fence_after_sync();
-            umma_chain_ss<4 * KB, kStepK, kBlockK, kStepK, kBlockK>(lead, tmem + Lay::colA + ab * 128, dQ + (kOneQ ? 0 : st) * kK, dK + st * kK, idA, 0);
+            umma_chain_ss<4 * KB, kStepK, kBlockK, kStepK, kBlockK>(lead, tmem + Lay::colA + ab * 128, dQ + st * kK, dK + st * kK, idA, 0);
             umma_commit(&bars[dA + ab]);
-            if (kOneQ) umma_commit(&bars[dFreeQ]);
             return true;
           };
           bool ok = nchunk > 0 && issue_A(0);
@@ -163,10 +163,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             const int st = c % Lay::kStages, ab = Lay::kA == 2 ? c & 1 : 0, an = Lay::kA == 2 ? c >> 1 : c;
             if (Lay::kA == 2 && c + 1 < nchunk && !issue_A(c + 1)) break;
             if (c >= 1 && !mbar_wait(&bars[dNFree], (c + 1) & 1)) { tc_fail(25); break; }
+            if (kOneV && !mbar_wait(&bars[dFullV], c & 1)) { tc_fail(24); break; }
             if (!mbar_wait(&bars[dP + ab], an & 1)) { tc_fail(9); break; }
             tc_fence_after_sync();
-            umma_chain_ts<8, kStepMN, kBlockMN>(lead, tmem + Lay::colO, tmem + Lay::colA + ab * 128, dV + st * kV, idN, 0);
+            umma_chain_ts<8, kStepMN, kBlockMN>(lead, tmem + Lay::colO, tmem + Lay::colA + ab * 128, dV + (kOneV ? 0 : st) * kV, idN, 0);
             umma_commit(&bars[dFree + st]);
+            if (kOneV) umma_commit(&bars[dFreeV]);
             if (Lay::kA == 1 && c + 1 < nchunk && !issue_A(c + 1)) break;
           }
         }
@@ -176,16 +178,16 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         for (int c = 0; c < nchunk; ++c) {
           const int st = c % Lay::kStages;
           if (!mbar_wait(&bars[dFull + st], (c / Lay::kStages) & 1) || !mbar_wait(&bars[dKp + c % Lay::kL], (c / Lay::kL) & 1)) { tc_fail(8); break; }
+          if (kOneV && !mbar_wait(&bars[dFullV], c & 1)) { tc_fail(26); break; }
           if (!mbar_wait(&bars[dSt], c & 1)) { tc_fail(6); break; }
           tc_fence_after_sync();
-          umma_chain_ss<8, kStepMN, kBlockMN, kStepMN, kBlockMN>(lead, tmem + Lay::colS, dKt + st * kK, dV + st * kV, idS, 1);
-          if (EXACT) umma_chain_ss<8, kStepMN, kBlockMN, kStepMN, kBlockMN>(lead, tmem + Lay::colS, dLow, dV + st * kV, idS, 1);
+          umma_chain_ss<8, kStepMN, kBlockMN, kStepMN, kBlockMN>(lead, tmem + Lay::colS, dKt + st * kK, dV + (kOneV ? 0 : st) * kV, idS, 1);
+          if (EXACT) umma_chain_ss<8, kStepMN, kBlockMN, kStepMN, kBlockMN>(lead, tmem + Lay::colS, dLow, dV + (kOneV ? 0 : st) * kV, idS, 1);
+          if (kOneV) umma_commit(&bars[dFreeV]);
           if constexpr (OUT) {
-            if (kOneQ && !mbar_wait(&bars[dFullQ], c & 1)) { tc_fail(26); break; }
             if (c >= 1 && !mbar_wait(&bars[dNFree], (c + 1) & 1)) { tc_fail(7); break; }
             tc_fence_after_sync();
-            umma_chain_ss<4 * KB, kStepK, kBlockK, kStepMN, kBlockMN>(lead, tmem + Lay::colN, dQ + (kOneQ ? 0 : st) * kK, dC, idN, 0);
-            if (kOneQ) umma_commit(&bars[dFreeQ]);
+            umma_chain_ss<4 * KB, kStepK, kBlockK, kStepMN, kBlockMN>(lead, tmem + Lay::colN, dQ + st * kK, dC, idN, 0);
           }
           umma_commit(&bars[dS]);                // the copy has been read, too
           umma_commit(&bars[dFree + st]);
@@ -439,12 +441,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (mask) {      // padded rows of K and V may hold anything: zero before a product reads them
         const bool gone = ahead;
         if (c + 1 < nchunk) ahead = chunk_t0(c + 1) + j < t_end ? mask[chunk_t0(c + 1) + j] : 0;
-        if (!mbar_wait(&bars[dFull + st], filled)) { tc_fail(18); break; }
+        if (!mbar_wait(&bars[dFull + st], filled) || (kOneV && !mbar_wait(&bars[dFullV], c & 1))) { tc_fail(18); break; }
         if (gone) {
 #pragma unroll
           for (int ch = 0; ch < 8 * KB; ++ch) *reinterpret_cast<uint4*>(krow + row_chunk2(j, ch)) = make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (int ch = 0; ch < 8 * DB; ++ch) *reinterpret_cast<uint4*>(sm + Lay::v + st * DB * kBox + row_chunk2(j, ch)) = make_uint4(0, 0, 0, 0);
+          for (int ch = 0; ch < 8 * DB; ++ch) *reinterpret_cast<uint4*>(sm + Lay::v + (kOneV ? 0 : st) * DB * kBox + row_chunk2(j, ch)) = make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
         mbar_arrive(&bars[dClean + lb]);
