@@ -28,11 +28,13 @@ template <int DB>
 struct WinLayout {
   static constexpr int kStages = 4;
   static constexpr uint32_t kHalf = kBox / 2;      // 64 rows of 128 bytes
-  static constexpr uint32_t q = 0, k = 2 * DB * kBox, v = k + kStages * DB * kHalf, num = v + kStages * DB * kHalf, bar = num + kStages * kWinTile * 4, bytes = bar + 256;
+  static constexpr uint32_t q = 0, k = 2 * DB * kBox, v = k + kStages * DB * kHalf, num = v + kStages * DB * kHalf, bar = num + kStages * kWinTile * 4, bytes = bar + 288;
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
-// wS, wP: [unit][place of the scores]
-enum { wQ = 0, wQEmpty = 2, wFullK = 4, wFullV = 8, wEmpty = 12, wNumbers = 16, wS = 20, wP = 24, wO = 28, wCount = 30 };
+// wS, wP, wO: [unit][place of the scores].  wO (a tile's sums are complete) is not waited for at every tile, and the tile before the last may be pending when it is:
+// one barrier for both would take the completion before that for the one that is wanted.
+enum { wQ = 0, wQEmpty = 2, wFullK = 4, wFullV = 8, wEmpty = 12, wNumbers = 16, wS = 20, wP = 24, wO = 28, wCount = 32 };
+static_assert(wCount * 8 + 4 <= 288, "barriers");
 
 template <typename T, int DB, bool ORDERED>
 __global__ void __launch_bounds__(kWinThreads, 1)
@@ -156,7 +158,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           if (!mbar_wait(&bars[wP + 2 * u + (it & 1)], (it >> 1) & 1)) { if (lead) tc_fail(7); ok = false; break; }
           tc_fence_after_sync();
           umma_chain_ts<4, kStepMN, kBlockMN>(lead, O, S + (it & 1) * 64, dV + st * kStep, idO, first ? 0u : 1u);
-          umma_commit_w(lead, &bars[wO + u]);
+          umma_commit_w(lead, &bars[wO + 2 * u + (it & 1)]);
           umma_commit_w(lead, &bars[wEmpty + st]);
           first = false;
           ++it;
@@ -234,7 +236,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           top = ref;
           sum *= keep;
           if (!first) {      // O of the tiles before has to follow
-            if (!mbar_wait(&bars[wO + u], (it + 1) & 1)) { tc_fail(10); ok = false; break; }
+            if (!mbar_wait(&bars[wO + 2 * u + ((it - 1) & 1)], ((it - 1) >> 1) & 1)) { tc_fail(10); ok = false; break; }
             tc_fence_after_sync();
 #pragma unroll 1
             for (int c0 = 0; c0 < DP; c0 += 16) {
@@ -269,7 +271,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         ++it;
       }
       if (!ok || own.end == 0) continue;
-      if (!first && !mbar_wait(&bars[wO + u], (it + 1) & 1)) { tc_fail(11); break; }
+      if (!first && !mbar_wait(&bars[wO + 2 * u + ((it - 1) & 1)], ((it - 1) >> 1) & 1)) { tc_fail(11); break; }
       tc_fence_after_sync();
       const int h = k.h0 + (pair_heads ? u : 0);
       const float inv = sum > 0.f && mine >= 0 ? 1.f / sum : 0.f;      // a query that sees nothing (a padded one) has 0

@@ -89,6 +89,10 @@ def some_mask(kind, B, T):
     m = torch.rand(B, T, device="cuda") < 0.3 if kind == "any" else torch.arange(T, device="cuda")[None] >= torch.randint((T + 1) // 2, T + 1, (B, 1), device="cuda")
     if kind == "left":
         m = m.flip(1)
+    if kind == "gap":           # stretches without a token, longer than a tile
+        m = torch.zeros(B, T, dtype=torch.bool, device="cuda")
+        m[:, T // 5:T // 5 + T // 2] = True
+        m[-1, :T // 8] = m[-1, -3:] = True
     if kind == "any" and B > 1:
         m[0] = True             # a row with nothing in it
     return m
@@ -124,6 +128,10 @@ DECAY = [
     (140, 1, 2, 37, 90, "token", "any", "fp16"),
     (130, 1, 2, 256, 256, "token", None, "bf16"),
     (640, 40, 4, 64, 64, "token", "right", "bf16"),
+    (1, 3, 2, 64, 64, "token", "any", "fp16"),
+    (3, 200, 2, 128, 64, "head", "any", "fp16"),
+    (2100, 2, 1, 128, 128, "token", "any", "fp16"),
+    (5000, 1, 1, 64, 128, "token", None, "bf16"),
 ]
 
 
@@ -241,6 +249,8 @@ def test_decay_strides_streams_and_sizes_of_zero():
         near(decay_attention(q=q, k=k, v=v, log_decay=g), want, torch.float16)
     near(decay_attention(q=q, k=k, v=v, log_decay=g[:1].expand(140, 2, 3), scale=0.5), decay_dense(*(x.double() for x in (q, k, v, g[:1].expand(140, 2, 3))), scale=0.5)[0],
          torch.float16)
+    shared = k[:, :, :1].expand(-1, -1, 3, -1)                         # one head's keys for all: a stride of zero
+    near(decay_attention(q=q, k=shared, v=v, log_decay=g), decay_dense(*(x.double() for x in (q, shared, v, g)))[0], torch.float16)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -277,6 +287,10 @@ WINDOW = [
     (260, 1, 2, 1, 33, 50, 9, "any", "bf16"),
     (140, 1, 2, 1, 200, 60, 2, "any", "fp16"),
     (300, 12, 16, 4, 64, 100, 4, "right", "bf16"),
+    (1, 3, 2, 2, 64, 5, 1, "any", "fp16"),
+    (700, 2, 2, 1, 64, 30, 70, "gap", "fp16"),
+    (1100, 1, 3, 3, 128, 1, 0, "gap", "fp16"),
+    (1500, 1, 2, 2, 64, 2000, 3, None, "fp16"),
 ]
 
 
@@ -573,3 +587,51 @@ def test_refusals_on_the_gpu():
     for y in (decay_attention(q=x, k=q, v=q, log_decay=g), window_attention(q=x, k=q, v=q, window=3)):
         with pytest.raises(RuntimeError):
             torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_decay_backward_without_what_the_forward_kept():
+    """The tensor-level backward computes the states again where it is not handed them, with the same bits."""
+    from rfa_b200 import ops
+    torch.manual_seed(23)
+    for K, D in ((64, 64), (128, 128)):
+        q, k, v = make(400, 2, (2, 2, 2), (K, K, D), torch.float16, False)
+        g, s = (-0.1 * torch.rand(400, 2, 2, device="cuda")).half(), torch.randn(2, 2, K, D, device="cuda")
+        go = torch.randn_like(v)
+        out, last, kept = ops.decay_attention_fwd(q, k, v, g, s, save=True, return_state=True)
+        assert kept is not None and ops.decay_attention_fwd(q, k, v, g, s)[2] is None
+        with_it = ops.decay_attention_bwd(q, k, v, g, s, None, None, go, kept=kept, need_state=True)
+        without = ops.decay_attention_bwd(q, k, v, g, s, None, None, go, need_state=True)
+        _, want = grads(lambda *a: decay_dense(*a), (q, k, v, g, s), [go])
+        for a, b, w in zip(with_it, without, want):
+            near(a, w, torch.float16, 12.0, terms=q.double().square().sum(-1) * 0 + 1 if w.dim() == 3 else None)
+            near(b, w, torch.float16, 12.0, terms=q.double().square().sum(-1) * 0 + 1 if w.dim() == 3 else None)
+        with pytest.raises(ValueError):
+            ops.decay_attention_bwd(q, k, v, g, s, None, None, go, kept=kept[:100])
+
+
+def test_calls_on_two_streams_at_once_and_the_same_bits_again():
+    from rfa_b200.decay_attention import decay_attention, incremental_decay_attention
+    from rfa_b200.window_attention import window_attention
+    torch.manual_seed(29)
+    jobs = []
+    for i in range(2):
+        q, k, v = make(900, 2, (4, 4, 4), (64, 64, 64), torch.float16)
+        jobs.append((q, k, v, -0.1 * torch.rand(900, 2, 4, device="cuda")))
+
+    def work(q, k, v, g):
+        a, b, c = (x.detach().requires_grad_() for x in (q, k, v))
+        o = decay_attention(q=a, k=b, v=c, log_decay=g) + window_attention(q=a, k=b, v=c, window=200, sinks=3)
+        return (o, *torch.autograd.grad(o, (a, b, c), q), *incremental_decay_attention(q=q, k=k, v=v, log_decay=g))
+
+    want = [work(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(3):
+        got = []
+        for s, j in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(work(*j))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y)
