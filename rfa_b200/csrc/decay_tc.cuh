@@ -17,8 +17,8 @@
 //
 // Warp roles (768 threads): warp 0 TMA producer; warps 1 and 18 MMA issuers (A: Q K^T, P V; B: Q S, the state: issuing one costs the issuing thread about 70
 // cycles, and a chunk has 20 to 40); warps 2..5 score group (A -> P); warps 6..9 and 20..23 state groups, half of the columns each (state -> 16-bit copy,
-// state times the next chunk's decay); warps 14..17 output group; warp 19 the decays (64-bit sums, because neighbours' are subtracted); warps 10..13 key group: K' in place of K once A is complete, zeros over
-// the rows of padded tokens.  Per chunk the serial chain is  state MMA -> copy and decay -> next state MMA.  All waits are bounded.
+// state times the next chunk's decay); warps 14..17 output group; warp 19 the decays (64-bit sums, because neighbours' are subtracted); warps 10..13 key group (states alone: with 2..5): K' in place of K once A is complete,
+// zeros over the rows of padded tokens.  Per chunk the serial chain is  state MMA -> copy and decay -> next state MMA.  All waits are bounded.
 #pragma once
 
 #include "decay.cuh"
@@ -96,7 +96,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     for (int i = 0; i < dL; ++i) mbar_init(&bars[i], OUT && (i >= dFree && i != dFullV) ? 2 : 1);      // both issuers
     for (int i = 0; i < Lay::kL; ++i) {
       mbar_init(&bars[dL + i], 32); mbar_init(&bars[dLFree + i], OUT ? 128 : 256);
-      mbar_init(&bars[dKp + i], 128); mbar_init(&bars[dClean + i], 128);
+      mbar_init(&bars[dKp + i], OUT ? 128 : 256); mbar_init(&bars[dClean + i], 128);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[dA + i], 1); mbar_init(&bars[dP + i], 128);
@@ -194,7 +194,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
     }
-  } else if (warp < 6) {
+  } else if (OUT && warp < 6) {
     // ------------------------------------------------------------------ score group: P = A o w
     if constexpr (OUT) {
       const int quarter = warp & 3, row = quarter * 32 + lane;
@@ -246,7 +246,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         mbar_arrive(&bars[dP + ab]);
       }
     }
-  } else if (warp < 10 || warp >= 20) {
+  } else if ((warp >= 6 && warp < 10) || warp >= 20) {
     // ------------------------------------------------------------------ state groups
     const int quarter = warp & 3, row = quarter * 32 + lane;      // a row of the state
     const int col0 = warp >= 20 ? DP / 2 : 0, col1 = col0 + DP / 2;
@@ -431,14 +431,17 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     }
     if (totals_only && lane == 0) a.seg_decay[(int64_t)seg * BH + bh] = run / kLog2eD;
   } else {
-    // ------------------------------------------------------------------ key group: the token's row of K
-    const int j = tid - 320;
+    // ------------------------------------------------------------------ key group: the token's row of K; with states alone warps 2..5 take half of it
+    const bool second = !OUT && warp < 6;
+    const int j = second ? tid - 64 : tid - 320;
     uint8_t ahead = mask && nchunk > 0 && chunk_t0(0) + j < t_end ? mask[chunk_t0(0) + j] : 0;
     for (int c = 0; c < nchunk; ++c) {
       const int st = c % Lay::kStages, lb = c % Lay::kL;
       const uint32_t filled = (c / Lay::kStages) & 1;
       unsigned char* krow = sm + Lay::k + st * KB * kBox;
-      if (mask) {      // padded rows of K and V may hold anything: zero before a product reads them
+      if (mask && second) {
+        if (!mbar_wait(&bars[dClean + lb], (c / Lay::kL) & 1)) { tc_fail(29); break; }
+      } else if (mask) {      // padded rows of K and V may hold anything: zero before a product reads them
         const bool gone = ahead;
         if (c + 1 < nchunk) ahead = chunk_t0(c + 1) + j < t_end ? mask[chunk_t0(c + 1) + j] : 0;
         if (!mbar_wait(&bars[dFull + st], filled) || (kOneV && !mbar_wait(&bars[dFullV], c & 1))) { tc_fail(18); break; }
@@ -459,7 +462,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       } else if (!mbar_wait(&bars[dFull + st], filled)) { tc_fail(22); break; }
       if (EXACT && c >= 1 && !mbar_wait(&bars[dS], (c + 1) & 1)) { tc_fail(23); break; }      // the second part of the chunk before has been read
 #pragma unroll 1
-      for (int c8 = 0; c8 < 8 * KB; c8 += 2) {
+      for (int c8 = second ? 4 * KB : 0; c8 < (OUT || second ? 8 : 4) * KB; c8 += 2) {
         uint4 k8[2];
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) k8[ch] = *reinterpret_cast<const uint4*>(krow + row_chunk2(j, c8 + ch));

@@ -10,7 +10,7 @@
 // kernel of its own.  Tiles that are seen whole need no mask.  Padded places: as in window_tc.cu, warp 3 fetches numbers (and, KEYS, lse and delta of the queries)
 // and clears the rows that are summed over.
 //
-// Warp roles (512 or 384 threads): warp 0 TMA producer, warp 1 issues S and D, warp 2 the sums, warp 3 columns' data, warps 4..7, 8..11, 12..15 the groups.  All
+// Warp roles (512 or 384 threads): warp 0 TMA producer, warp 1 issues S and D, warp 2 the sums, warp 3 columns' data or, where there are none, D, warps 4..7, 8..11, 12..15 the groups.  All
 // waits are bounded.
 #define RFA_TC_FAMILY 13
 #include <algorithm>
@@ -43,6 +43,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
   using Lay = WbLayout<DB, KEYS>;
   constexpr int DP = DB * 64, kStages = Lay::kStages, kGroups = Lay::kGroups;
   constexpr bool kColumns = KEYS || ORDERED;
+  constexpr bool kApart = !kColumns;      // warp 3 has no columns to fetch: it issues D beside warp 1's S
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::bar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + bCount);
@@ -68,7 +69,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
   const int other_heads = KEYS ? group : 1;
   if (tid == 0) {
     for (int i = 0; i < bCount; ++i)
-      mbar_init(&bars[i], i >= bEmpty && i < bCols ? (kColumns ? 129 : 1) : i >= bCols && i < bS ? 32 : i >= bP && i < bFree ? 128 : i == bAccFree ? kGroups * 128 : 1);
+      mbar_init(&bars[i], i >= bEmpty && i < bCols ? (kColumns ? 129 : 1) : i >= bCols && i < bS ? 32 : i >= bP && i < bFree ? 128 : i == bAccFree ? kGroups * 128 : kApart && (i == bREmpty || (i >= bS && i < bP)) ? 2 : 1);
     mbar_fence_init();
     tma_prefetch_desc(&tm_r1); tma_prefetch_desc(&tm_r2); tma_prefetch_desc(&tm_x1); tma_prefetch_desc(&tm_x2);
   }
@@ -102,7 +103,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
           }
       }
     }
-  } else if (warp == 1 || warp == 2) {
+  } else if (warp == 1 || warp == 2 || (kApart && warp == 3)) {
     // ------------------------------------------------------------------ MMA issuers
     // the whole warp goes through the loop and one lane issues (see umma_ss_w)
     {
@@ -119,19 +120,19 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
       for (int w = blockIdx.x; ok && w < works; w += gridDim.x, ++done) {
         Work k;
         work_of(w, k);
-        if (warp == 1) {
+        if (warp != 2) {
           if (!mbar_wait(&bars[bR], done & 1)) { if (lead) tc_fail(3); break; }
         } else if (done > 0 && !mbar_wait(&bars[bAccFree], (done + 1) & 1)) { if (lead) tc_fail(4); break; }
         bool first = true;
         for (int h = 0; ok && h < other_heads; ++h)
           for (int t = k.span.begin(); t < k.span.end; t = k.span.next(t), ++n) {
             const int st = n % kStages;
-            if (warp == 1) {
+            if (warp != 2) {
               if (!mbar_wait(&bars[ORDERED ? bCols + st : bFull + st], (n / kStages) & 1)) { if (lead) tc_fail(5); ok = false; break; }
               if (n >= kGroups && !mbar_wait(&bars[bFree + buf], turn ^ 1)) { if (lead) tc_fail(6); ok = false; break; }
               tc_fence_after_sync();
-              umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, tmem + buf * 128, dR1, dX1 + st * kStep, idS, 0);
-              umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, tmem + buf * 128 + 64, dR2, dX2 + st * kStep, idS, 0);
+              if (!kApart || warp == 1) umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, tmem + buf * 128, dR1, dX1 + st * kStep, idS, 0);
+              if (!kApart || warp == 3) umma_chain_ss<4 * DB, kStepK, kBlockK, kStepK, kBlockX>(lead, tmem + buf * 128 + 64, dR2, dX2 + st * kStep, idS, 0);
               umma_commit_w(lead, &bars[bS + buf]);      // the stage is given back by the sums, which come after
             } else {
               if (!mbar_wait(&bars[bP + buf], turn)) { if (lead) tc_fail(7); ok = false; break; }
@@ -144,7 +145,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
             }
             if (++buf == kGroups) { buf = 0; turn ^= 1; }
           }
-        if (ok) umma_commit_w(lead, &bars[warp == 1 ? bREmpty : bAcc]);
+        if (ok) umma_commit_w(lead, &bars[warp != 2 ? bREmpty : bAcc]);
       }
     }
   } else if (warp == 3) {
