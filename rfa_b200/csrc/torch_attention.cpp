@@ -6,6 +6,30 @@ namespace {
 
 double scale_of(const std::optional<double>& scale, int64_t width) { return scale ? *scale : width > 0 ? 1.0 / std::sqrt(static_cast<double>(width)) : 1.0; }
 
+// The tensor-core kernels take 16-bit heads of up to 128 whose rows start on 16 bytes.  Other rows of those types are copied for them, widths that are no multiple
+// of 8 filled with zeros, which add nothing to a product: a copy reads and writes a row once where the kernels for any rows take several times as long for it.  Below 64
+// tokens the copies' launches cost more (8 x 16 heads of 64, forward, tensor cores / any rows, us: 2 tokens 6 / 11, 64 6 / 35, 256 9 / 113; a copy 2 to 3).
+bool copies_pay(const Tensor& q, int64_t width) { return (q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16) && width >= 1 && width <= 128 && q.size(0) >= 64; }
+bool rows_fit(const Tensor& t) {
+  if (!aligned(t) || (t.size(-1) > 1 && t.stride(-1) != 1)) return false;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (t.size(d) > 1 && (t.stride(d) <= 0 || t.stride(d) % 8)) return false;
+  return true;
+}
+Tensor filled(const Tensor& t) {
+  const int64_t rest = (8 - t.size(-1) % 8) % 8;
+  if (rest) return at::constant_pad_nd(t, {0, rest});
+  return rows_fit(t) ? t : packed(t);
+}
+Tensor cut(const Tensor& t, int64_t width) { return t.size(-1) == width ? t : t.narrow(-1, 0, width).contiguous(); }
+Tensor filled_state(const Tensor& s) {
+  const int64_t rows = (8 - s.size(-2) % 8) % 8, cols = (8 - s.size(-1) % 8) % 8;
+  return rows || cols ? at::constant_pad_nd(s, {0, cols, 0, rows}) : s;
+}
+Tensor cut_state(const Tensor& s, int64_t rows, int64_t cols) {
+  return s.size(-2) == rows && s.size(-1) == cols ? s : s.narrow(-2, 0, rows).narrow(-1, 0, cols).contiguous();
+}
+
 // ---- linear attention with a decay ------------------------------------------------------------------------------------------
 struct Decay {
   rfa_decay_t c{};
@@ -46,6 +70,9 @@ struct Decay {
     c.mask = static_cast<const uint8_t*>(maybe(mask));
   }
   bool empty() const { return c.T == 0 || c.B == 0 || c.H == 0 || c.K == 0 || c.D == 0; }
+  bool wants_copies() const {
+    return !empty() && copies_pay(q, c.K) && c.D <= 128 && (c.K % 8 || c.D % 8 || !rows_fit(q) || !rows_fit(k) || !rows_fit(v));
+  }
   Tensor workspace(bool backward) const { return scratch(rfa_decay_workspace_bytes(c.T, c.B, c.H, c.K, c.D, c.dtype, backward), q); }
 };
 
@@ -60,6 +87,18 @@ std::tuple<Tensor, OptTensor, OptTensor> decay_attention_fwd(const Tensor& q, co
     if (!return_state) return {out, std::nullopt, std::nullopt};
     if (in_place && s) return {out, *s, std::nullopt};
     return {out, s ? s->clone() : fresh_zeros(state, q), std::nullopt};
+  }
+  if (d.wants_copies()) {
+    const int64_t K = q.size(3), D = v.size(3);
+    auto [out, last, kept] = decay_attention_fwd(filled(q), filled(k), filled(v), log_decay, s ? OptTensor(filled_state(*s)) : s, mask, scale_of(scale, K), return_state, false, save);
+    if (last) {
+      last = cut_state(*last, K, D);
+      if (in_place && s) {
+        s->copy_(*last);
+        last = s;
+      }
+    }
+    return {cut(out, D), last, kept};
   }
   Tensor out = fresh(v.sizes(), q, q.scalar_type());
   OptTensor last, kept;
@@ -101,6 +140,12 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor, OptTensor> decay_attention_bwd(con
     if (gd) gd->zero_();
     if (gs) g_s ? gs->copy_(*g_s) : gs->zero_();
     return {gq, gk, gv, gd, gs};
+  }
+  if (d.wants_copies()) {
+    const int64_t K = q.size(3), D = v.size(3);
+    auto [pq, pk, pv, pd, ps] = decay_attention_bwd(filled(q), filled(k), filled(v), log_decay, s ? OptTensor(filled_state(*s)) : s, mask, scale_of(scale, K), filled(g.to(half)),
+                                                    g_s ? OptTensor(filled_state(g_s->to(at::kFloat))) : g_s, kept, need_decay, need_state);
+    return {cut(pq, K), cut(pk, K), cut(pv, D), pd, ps ? OptTensor(cut_state(*ps, K, D)) : ps};
   }
   if (kept && (!kept->is_contiguous() || kept->nbytes() < rfa_decay_kept_bytes(&d.c))) raise(PyExc_ValueError, "decay_attention: kept is not what this call's forward left");
   if (kept) require_device(q, {&*kept});
@@ -183,6 +228,7 @@ struct Window {
     c.mask = static_cast<const uint8_t*>(maybe(mask));
   }
   bool empty() const { return c.T == 0 || c.B == 0 || c.H == 0 || c.D == 0; }
+  bool wants_copies() const { return !empty() && copies_pay(q, c.D) && c.scale > 0.f && (c.D % 8 || !rows_fit(q) || !rows_fit(k) || !rows_fit(v)); }
   Tensor workspace(bool backward) const {
     return scratch(rfa_window_workspace_bytes(c.T, c.B, c.H, c.G, c.D, c.dtype, c.window, c.sinks, backward), q);
   }
@@ -192,6 +238,10 @@ struct Window {
 std::tuple<Tensor, OptTensor> window_attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, const OptTensor& mask,
                                                    std::optional<double> scale, bool save) {
   Window w(q, k, v, window, sinks, mask, scale);
+  if (w.wants_copies()) {
+    auto [out, lse] = window_attention_fwd(filled(q), filled(k), filled(v), window, sinks, mask, scale_of(scale, q.size(3)), save);
+    return {cut(out, q.size(3)), lse};
+  }
   Tensor out = fresh(q.sizes(), q, q.scalar_type());
   OptTensor lse;
   if (save) lse = fresh({q.size(1), q.size(2), q.size(0)}, q, at::kFloat);
@@ -212,6 +262,11 @@ std::tuple<Tensor, Tensor, Tensor> window_attention_bwd(const Tensor& q, const T
   same_dtype("window_attention", q, {&out});
   need_f32("window_attention", "lse", lse);
   const auto half = q.scalar_type();
+  if (w.wants_copies()) {
+    const int64_t D = q.size(3);
+    auto [pq, pk, pv] = window_attention_bwd(filled(q), filled(k), filled(v), window, sinks, mask, scale_of(scale, D), filled(out), lse, filled(g.to(half)));
+    return {cut(pq, D), cut(pk, D), cut(pv, D)};
+  }
   Tensor gq = fresh(q.sizes(), q, half), gk = fresh(k.sizes(), q, half), gv = fresh(v.sizes(), q, half);
   if (w.empty()) {
     gk.zero_();

@@ -132,6 +132,10 @@ DECAY = [
     (3, 200, 2, 128, 64, "head", "any", "fp16"),
     (2100, 2, 1, 128, 128, "token", "any", "fp16"),
     (5000, 1, 1, 64, 128, "token", None, "bf16"),
+    (64, 2, 2, 33, 127, "token", "any", "fp16"),
+    (63, 2, 2, 33, 127, "token", "any", "fp16"),
+    (500, 1, 2, 100, 5, "head", None, "bf16"),
+    (300, 2, 3, 1, 64, "token", "right", "fp16"),
 ]
 
 
@@ -291,6 +295,9 @@ WINDOW = [
     (700, 2, 2, 1, 64, 30, 70, "gap", "fp16"),
     (1100, 1, 3, 3, 128, 1, 0, "gap", "fp16"),
     (1500, 1, 2, 2, 64, 2000, 3, None, "fp16"),
+    (64, 2, 2, 1, 35, 20, 2, "any", "fp16"),
+    (63, 2, 2, 1, 35, 20, 2, "any", "fp16"),
+    (400, 1, 4, 2, 127, 90, 0, None, "bf16"),
 ]
 
 
