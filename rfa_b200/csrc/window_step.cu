@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(kThreads) window_step_kernel(const __grid_cons
 // columns of the scores, then the depth of the sums.  Both operands come straight from memory in 16-byte pieces: the order of a product's depth is free, so that a
 // lane's 8 adjacent numbers of a key are its operands of two depth steps, and so is the order of the columns, so that its 8 adjacent numbers of four values
 // are, halves of two put together, its operands of 8 column tiles.  32 products stand for 16 slots of 128, where the lanes' own multiply-adds take about 1000
-// instructions for 4 heads: 256 x 8 key heads x 1028 slots x 128 took 418 us, and 8 x 16 x 516 x 64 with one head 11.9 us.
+// instructions for 4 heads: 256 x 8 key heads x 1028 slots x 128 (4 heads each) take 194 us, 5.6 TB/s, where the lanes took 418; 8 x 16 x 516 x 64 with one head 8.4 where
+// they took 11.9.  Weights are rounded to the type for the second product, each off by half a step of itself.
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1, __half) {      // rows 8..15 of A are zero
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1));
