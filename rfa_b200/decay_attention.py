@@ -10,7 +10,11 @@ adjacent (views of a projection's output are taken as they are); sums and states
 passes are not differentiable themselves.  No upstream counterpart.
 
 ``key_padding_mask`` ``[bsz, tgt_len]`` (1 = padding): padded tokens are skipped, wherever they stand -- every result is what it
-would be without them, whatever values they hold, and their own outputs and gradients are zero."""
+would be without them, whatever values they hold, and their own outputs and gradients are zero.  A real token that is not finite may
+reach the outputs of any token less than 128 places from it, as it reaches all behind it.
+
+In fp16 and bf16 the outputs of several tokens come from 16-bit copies of the state (its own value is fp32): in fp16 a state beyond
+65504 gives outputs that are not finite."""
 from typing import Dict, Optional, Tuple
 
 import math

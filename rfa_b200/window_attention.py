@@ -10,7 +10,8 @@ have fewer heads than q: ``num_heads / num_kv_heads`` adjacent query heads share
 backward pass is not differentiable itself.  No upstream counterpart.
 
 ``key_padding_mask`` ``[bsz, tgt_len]`` (1 = padding): padded tokens are skipped, wherever they stand, and not counted in distances --
-every result is what it would be without them, whatever values they hold, and their own outputs and gradients are zero."""
+every result is what it would be without them, whatever values they hold, and their own outputs and gradients are zero.  A real
+token that is not finite may reach the outputs of any token less than 128 places from it."""
 from typing import Dict, Optional, Tuple
 
 import math

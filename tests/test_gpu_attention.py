@@ -642,3 +642,31 @@ def test_calls_on_two_streams_at_once_and_the_same_bits_again():
         for a, b in zip(got, want):
             for x, y in zip(a, b):
                 assert torch.equal(x, y)
+
+
+def test_offsets_beyond_32_bits():
+    """A cache of 2^31 numbers a row and key head, and a batch whose activations pass 2^31 numbers: the last rows are what they are by themselves."""
+    from rfa_b200.decay_attention import decay_attention
+    from rfa_b200.window_attention import incremental_window_attention, window_attention
+    torch.manual_seed(31)
+    D, window = 128, 2 ** 24
+    pk, pv = (torch.zeros(2, 1, window, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    at = window - 3                                       # only the last few slots of the second row weigh anything
+    pk[1, 0, at:], pv[1, 0, at:] = torch.randn(3, D, device="cuda").bfloat16(), torch.randn(3, D, device="cuda").bfloat16()
+    q = torch.randn(1, 2, 4, D, device="cuda").bfloat16() * 40
+    k, v = (torch.randn(1, 2, 1, D, device="cuda").bfloat16() for _ in range(2))
+    length = torch.tensor([5, 3 * window + at + 2], device="cuda")
+    out, nk, nv, nl = incremental_window_attention(q=q, k=k, v=v, window=window, prev_k=pk, prev_v=pv, prev_len=length)
+    assert nl.tolist() == [6, 3 * window + at + 3] and torch.equal(nk[1, 0, -1], k[0, 1, 0]) and torch.equal(nv[1, 0, -1], v[0, 1, 0])
+    s = torch.einsum("hd,sd->hs", q[0, 1].double(), pk[1, 0, at:].double()) * D ** -0.5
+    rest = (window - 3) * torch.exp(-s.amax(1, keepdim=True))
+    p = torch.exp(s - s.amax(1, keepdim=True))
+    near(out[0, 1], (p / (p.sum(1, keepdim=True) + rest)) @ pv[1, 0, at:].double(), torch.bfloat16)
+    del pk, pv, nk, nv
+    T, B, H = 4200, 64, 64                                # 2.2e9 numbers an array
+    q, k, v = (torch.empty(T, B, H, D, device="cuda", dtype=torch.bfloat16).normal_() for _ in range(3))
+    g = torch.full((H,), -0.5, device="cuda")             # e^-64 after 128 tokens
+    w = [x[-300:, -1:, -2:].clone() for x in (q, k, v)]
+    with torch.no_grad():
+        near(decay_attention(q=q, k=k, v=v, log_decay=g)[-100:, -1:, -2:], decay_dense(*(x.double() for x in w), g[-2:].double())[0][-100:], torch.bfloat16)
+        near(window_attention(q=q, k=k, v=v, window=100)[-100:, -1:, -2:], window_dense(*(x.double() for x in w), 100, 0)[-100:], torch.bfloat16)
