@@ -292,7 +292,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
           tmem_st_wait();
           tc_fence_before_sync();
           mbar_arrive(&bars[bP + g]);
-          if (kColumns) mbar_arrive(&bars[bEmpty + st]);
+          if (kColumns) mbar_release_stage(&bars[bEmpty + st]);
         }
       if (!ok) break;
       // ---- the gradients: the groups take 16 columns in turn

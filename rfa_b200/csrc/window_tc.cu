@@ -146,7 +146,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
               ++pending;
             } else {
               if (!mbar_wait(&bars[wFullV + st], filled)) { if (lead) tc_fail(5); ok = false; break; }
-              if (lead) mbar_arrive(&bars[wEmpty + st]);
+              if (lead) mbar_release_stage(&bars[wEmpty + st]);
             }
             kt = k.both.next(kt);
             ++n;
@@ -189,7 +189,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       for (int kt = k.both.begin(); kt < k.both.end; kt = k.both.next(kt), ++n) {
         if (ORDERED && !mbar_wait(&bars[wNumbers + n % kStages], (n / kStages) & 1)) { tc_fail(8); ok = false; break; }
         if (!own.has(kt)) {
-          if (ORDERED) mbar_arrive(&bars[wEmpty + n % kStages]);
+          if (ORDERED) mbar_release_stage(&bars[wEmpty + n % kStages]);
           continue;
         }
         const int64_t j0 = (int64_t)kt * kWinTile;
@@ -266,7 +266,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tmem_st_wait();
         tc_fence_before_sync();
         mbar_arrive(&bars[wP + 2 * u + (it & 1)]);
-        if (ORDERED) mbar_arrive(&bars[wEmpty + n % kStages]);      // the numbers have been read
+        if (ORDERED) mbar_release_stage(&bars[wEmpty + n % kStages]);      // the numbers have been read
         first = false;
         ++it;
       }
