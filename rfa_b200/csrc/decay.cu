@@ -143,7 +143,7 @@ extern "C" int rfa_decay_bwd(const rfa_decay_t* c, const void* g, const float* g
 
   if (!g_decay) return 0;
   const int tiles = sweep_tiles(c->K);
-  return launch_decay_grad(q_dots, tiles, k_dots, tiles, g_s, last, c->K * c->D, c->mask, g_decay, c->decay_dtype, c->per_head != 0, sums, c->T, c->B, c->H, st);
+  return launch_decay_grad(q_dots, tiles, k_dots, tiles, g_s, last, c->K * c->D, c->mask, g_decay, c->decay_dtype, c->per_head != 0, !c->s_in, sums, c->T, c->B, c->H, st);
 }
 
 extern "C" int rfa_decay_step(const rfa_decay_t* c, void* out, float* s, rfa_stream_t stream) {

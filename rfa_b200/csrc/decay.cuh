@@ -56,7 +56,7 @@ int launch_sweeps(SweepBatch batch, const SweepPlan& plan, cudaStream_t stream);
 // totals: what each segment adds -> the state in front of it; at most 65535 (row, head)s
 int launch_decay_combine(float* totals, const double* seg_decay, DecayState s_in, int nseg, int64_t BH, int A, int W, cudaStream_t stream);
 int launch_decay_grad(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_last, int KD, const uint8_t* mask,
-                      void* g_decay, int decay_dtype, bool per_head, float* sums, int64_t T, int B, int H, cudaStream_t stream);
+                      void* g_decay, int decay_dtype, bool per_head, bool from_zero, float* sums, int64_t T, int B, int H, cudaStream_t stream);
 
 // decay_tc.cu: fp16 and bf16, heads of up to 128 in rows that a tensor map can describe
 bool decay_tc_ok(const rfa_decay_t& c);

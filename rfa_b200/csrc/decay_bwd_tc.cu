@@ -33,6 +33,7 @@ struct DecayGradArgs {
   void* g_decay;                   // null; [T][B][H] of decay_dtype, or per_head: fp32 [B][chunks][H]
   int64_t T;
   int B, H, K, D, decay_dtype, per_head;
+  bool from_zero;                  // no state in front of the first token
   float scale;
 };
 
@@ -390,7 +391,11 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             if (i < quarter) g += ex_up[i];
           }
           const bool real = there && !(mask && mask[t]);
-          if (!real) g = 0.f;
+          // the first token with nothing in front decays nothing: 0, not the rounding of sums that cancel.  Looked for in the first chunk only; behind 128
+          // padded places the rounding stays
+          bool first = a.from_zero && k.chunk == 0 && real;
+          for (int64_t before = t - 1; first && before >= 0; --before) first = mask && mask[before];
+          if (!real || first) g = 0.f;
           if (!a.per_head) {
             if (there) {
               if (a.decay_dtype == RFA_F32) static_cast<float*>(a.g_decay)[at] = g;
@@ -435,6 +440,7 @@ int launch_decay_grad_tc(const rfa_decay_t& c, const CUtensorMap& q, const CUten
   a.states = states; a.grads = grads;
   a.gq = gq; a.gk = gk; a.gv = gv; a.g_decay = g_decay;
   a.T = c.T; a.B = c.B; a.H = c.H; a.K = c.K; a.D = c.D; a.decay_dtype = c.decay_dtype; a.per_head = c.per_head != 0;
+  a.from_zero = !c.s_in;
   a.scale = c.scale;
   switch ((c.dtype == RFA_BF16 ? 4 : 0) + (c.K > 64 ? 2 : 0) + (c.D > 64 ? 1 : 0)) {
     case 0: return launch<__half, 1, 1>(q, k, v, g, a, stream);

@@ -253,7 +253,8 @@ __global__ void __launch_bounds__(256) decay_combine_kernel(float* totals, const
 }
 
 // g_decay_t = sum over i >= t of (q_i . gq_i - k_i . gk_i) + g_s . s_last.  One CTA per (batch row, head), from the last token to the first; sums in 64 bits,
-// because near numbers are subtracted.
+// because near numbers are subtracted.  The sequence's first token decays nothing where no state is in front (`from_zero`): exactly 0, not the rounding that
+// the sum over all tokens leaves.
 constexpr int kGradThreads = 512;
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
@@ -266,11 +267,21 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   return s;
 }
 __global__ void __launch_bounds__(kGradThreads) decay_grad_kernel(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_last,
-                                                                  int KD, const uint8_t* mask, void* g_decay, int dtype, bool per_head, float* sums, int64_t T, int B, int H) {
+                                                                  int KD, const uint8_t* mask, void* g_decay, int dtype, bool per_head, bool from_zero, float* sums, int64_t T, int B,
+                                                                  int H) {
+  __shared__ int head;
   __shared__ double red[kGradThreads / 32];
   const int64_t bh = blockIdx.x, BH = (int64_t)B * H;
   const int b = (int)(bh / H), h = (int)(bh % H), tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   double carry = 0.0, all = 0.0;
+  int64_t first = from_zero ? 0 : -1;
+  if (from_zero && mask) {
+    if (tid == 0) head = kGradThreads;
+    while (first < T && !__syncthreads_or(first + tid < T && !mask[(int64_t)b * T + first + tid])) first += kGradThreads;
+    if (first + tid < T && !mask[(int64_t)b * T + first + tid]) atomicMin(&head, tid);
+    __syncthreads();
+    first += head;
+  }
   if (g_s) {
     double v = 0.0;
     for (int i = tid; i < KD; i += kGradThreads) v += (double)g_s[bh * KD + i] * (double)s_last[bh * KD + i];
@@ -295,7 +306,7 @@ __global__ void __launch_bounds__(kGradThreads) decay_grad_kernel(const float* q
     for (int w = 0; w < kGradThreads / 32; ++w) carry += red[w];
     __syncthreads();
     if (t >= 0) {
-      const double r = mask && mask[(int64_t)b * T + t] ? 0.0 : before + v;
+      const double r = t == first || (mask && mask[(int64_t)b * T + t]) ? 0.0 : before + v;
       all += r;
       if (!per_head) {
         const int64_t i = (t * B + b) * H + h;
@@ -378,9 +389,9 @@ int launch_sweeps(SweepBatch batch, const SweepPlan& plan, cudaStream_t stream) 
 }
 
 int launch_decay_grad(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_last, int KD, const uint8_t* mask,
-                      void* g_decay, int decay_dtype, bool per_head, float* sums, int64_t T, int B, int H, cudaStream_t stream) {
+                      void* g_decay, int decay_dtype, bool per_head, bool from_zero, float* sums, int64_t T, int B, int H, cudaStream_t stream) {
   decay_grad_kernel<<<(unsigned)((int64_t)B * H), kGradThreads, 0, stream>>>(q_dots, q_tiles, k_dots, k_tiles, g_s, s_last, KD, mask, g_decay, decay_dtype, per_head,
-                                                                            sums, T, B, H);
+                                                                            from_zero, sums, T, B, H);
   if (int r = check_launch("rfa_decay_bwd (decays)")) return r;
   if (!per_head) return 0;
   const SumJob job{sums, g_decay, H, B, decay_dtype};

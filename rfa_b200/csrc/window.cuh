@@ -39,6 +39,11 @@ struct WindowNumbers {
   // queries at places [p0, p1) see keys in front of first_end() and keys from first_key(p0) to p1
   __device__ __forceinline__ int64_t first_key(int64_t p0) const { return place(real_before(p0) - window + 1); }
   __device__ __forceinline__ int64_t first_end() const { return sinks > 0 ? min(S, place(sinks - 1) + 1) : 0; }
+  // A query that sees one key gives it the weight 1 whatever both are: its gradient is exactly 0, not the rounding of g . v - g . out; so is the gradient of a
+  // key that only such queries see.  Factors for query number n and for any key of the sequence.
+  __device__ __forceinline__ bool single() const { return window == 1 && sinks <= 0; }
+  __device__ __forceinline__ float query_factor(int n) const { return n == 0 || single() ? 0.f : 1.f; }
+  __device__ __forceinline__ float key_factor() const { return place(1) >= S || single() ? 0.f : 1.f; }
   // keys at places [p0, p1) are seen by no query at or behind this place
   __device__ __forceinline__ int64_t last_query(int64_t p0, int64_t p1) const { return p0 < first_end() ? S : min(S, place(real_before(p1 - 1) + window)); }
 };

@@ -315,7 +315,8 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
           if (there && c0 < a.D) store_row16(out + c0, v, a.D - c0, wide);
         }
       };
-      store(acc, KEYS ? a.gk : a.gq, a.scale);
+      const WindowNumbers num(a, k.b);
+      store(acc, KEYS ? a.gk : a.gq, a.scale * (KEYS ? num.key_factor() : num.query_factor(mine)));
       if (KEYS) store(acc + DP, a.gv, 1.f);
       tc_fence_before_sync();
       mbar_arrive(&bars[bAccFree]);

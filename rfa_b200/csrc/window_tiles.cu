@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, NC <= 2 ? 2 : 1) window_gq_kernel(co
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = 4 * ty + i;
-    if (r < rows) store_part<T, NC>(static_cast<T*>(a.gq) + (((i0 + r) * a.B + b) * a.H + h) * D, acc[i], D, tx, 1.f);
+    if (r < rows) store_part<T, NC>(static_cast<T*>(a.gq) + (((i0 + r) * a.B + b) * a.H + h) * D, acc[i], D, tx, num.query_factor(nq[r]));
   }
 }
 
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 2 : 1) window_gkv_kernel(c
     const int r = 4 * ty + i;
     if (r >= rows) continue;
     const int64_t at = (((j0 + r) * a.B + b) * a.G + kv) * D;
-    store_part<T, NC>(static_cast<T*>(a.gk) + at, gk[i], D, tx, 1.f);
+    store_part<T, NC>(static_cast<T*>(a.gk) + at, gk[i], D, tx, num.key_factor());
     store_part<T, NC>(static_cast<T*>(a.gv) + at, gv[i], D, tx, 1.f);
   }
 }

@@ -432,6 +432,49 @@ def test_window_masked_rubbish_strides_and_streams():
             assert incremental_window_attention(q=q, k=q, v=q, window=3)[0].shape == q.shape
 
 
+# ------------------------------------------------------------------------------------------------ gradients that are zero
+@pytest.mark.parametrize("dtype,D", [("fp32", 16), ("fp16", 64), ("bf16", 128), ("fp16", 33), ("bf16", 200)])
+def test_gradients_that_are_zero(dtype, D):
+    """A query that sees one key weighs it by 1, and a sequence's first token decays nothing, whatever the inputs are: zeros, and not the roundings of sums that cancel."""
+    from rfa_b200.decay_attention import decay_attention, incremental_decay_attention
+    from rfa_b200.window_attention import window_attention
+    torch.manual_seed(D)
+    T, B, H = 150, 3, 2
+    one = torch.ones(B, T, dtype=torch.bool, device="cuda")              # a single token in each sequence, at another place
+    one[0, 0] = one[1, 140] = one[2, 149] = False
+    left = torch.arange(T, device="cuda")[None] < torch.tensor([[0], [7], [100]], device="cuda")
+
+    def leaves(heads, t=T):
+        return [torch.randn(t, B, h, D, device="cuda").to(TYPES[dtype]).requires_grad_() for h in heads]
+
+    for t, window, sinks, mask in ((T, 1, 0, None), (T, 1, 0, left), (1, 5, 0, None), (1, 5, 2, None), (T, 5, 0, one), (T, 5, 2, one)):
+        q, k, v = leaves((H, 1, 1), t)
+        out = window_attention(q=q, k=k, v=v, window=window, sinks=sinks, key_padding_mask=mask)
+        gq, gk, gv = torch.autograd.grad(out, (q, k, v), torch.randn_like(out))
+        assert not gq.any() and not gk.any() and gv.any(), (t, window, sinks)
+    q, k, v = leaves((H, 1, 1))
+    out = window_attention(q=q, k=k, v=v, window=5, sinks=2, key_padding_mask=left)
+    gq, gk, _ = torch.autograd.grad(out, (q, k, v), torch.randn_like(out))
+    for b, n in enumerate((0, 7, 100)):
+        assert not gq[:n + 1, b].any() and gq[n + 1:, b].any(-1).all() and not gk[:n, b].any() and gk[n:, b].any(-1).all()
+
+    for t, mask, first in ((T, None, (0, 0, 0)), (T, left, (0, 7, 100)), (1, None, (0, 0, 0)), (2, torch.tensor([[0, 1]] * 3, device="cuda").bool(), (0, 0, 0))):
+        q, k, v = leaves((H, H, H), t)
+        g = (-0.1 * torch.rand(t, B, H, device="cuda")).to(TYPES[dtype]).requires_grad_()
+        out = decay_attention(q=q, k=k, v=v, log_decay=g, key_padding_mask=mask)
+        gg, = torch.autograd.grad(out, g, torch.randn_like(out))
+        real = torch.ones(t, B, dtype=torch.bool, device="cuda") if mask is None else ~mask.t()
+        for b, n in enumerate(first):
+            assert not gg[:n + 1, b].any() and gg[n + 1:, b][real[n + 1:, b]].any(-1).all(), (t, b)
+        per_head = torch.full((H,), -0.1, device="cuda", requires_grad=True)
+        out = decay_attention(q=q, k=k, v=v, log_decay=per_head, key_padding_mask=mask)
+        assert bool(torch.autograd.grad(out, per_head, torch.randn_like(out))[0].any()) == (t == T)
+    q, k, v = leaves((H, H, H), 1)                                       # a state in front of the first token is decayed by it
+    g, s = torch.full((1, B, H), -0.1, device="cuda", requires_grad=True), torch.randn(B, H, D, D, device="cuda")
+    out, _ = incremental_decay_attention(q=q, k=k, v=v, log_decay=g, s=s)
+    assert torch.autograd.grad(out, g, torch.randn_like(out))[0].all()
+
+
 # ------------------------------------------------------------------------------------------------ gradients against differences
 def test_gradients_against_differences():
     from rfa_b200.decay_attention import decay_attention
