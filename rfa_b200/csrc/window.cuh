@@ -36,16 +36,28 @@ struct WindowNumbers {
   __device__ __forceinline__ int at(int64_t s) const { return s < 0 || s >= S ? -1 : order ? order[s] : (int)s; }
   __device__ __forceinline__ int64_t real_before(int64_t s) const { const int n = at(s); return n < 0 ? ~n : n; }      // 0 <= s < S
   __device__ __forceinline__ int64_t place(int64_t n) const { return n < 0 ? 0 : n >= S ? S : pos ? pos[n] : n; }
-  // queries at places [p0, p1) see keys in front of first_end() and keys from first_key(p0) to p1
-  __device__ __forceinline__ int64_t first_key(int64_t p0) const { return place(real_before(p0) - window + 1); }
+  __device__ __forceinline__ int64_t real_to(int64_t s) const { const int n = at(s); return n < 0 ? ~n : n + 1; }           // up to s, 0 <= s < S
+  // queries at places [p0, p1) see keys from front() to first_end() and keys from first_key(p0) to last_key(p0, p1), 0 where no query is real
+  __device__ __forceinline__ int64_t front() const { return place(0); }
+  __device__ __forceinline__ int64_t first_key(int64_t p0) const { return place(max((int64_t)0, real_before(p0) - window + 1)); }
   __device__ __forceinline__ int64_t first_end() const { return sinks > 0 ? min(S, place(sinks - 1) + 1) : 0; }
+  __device__ __forceinline__ int64_t last_key(int64_t p0, int64_t p1) const {
+    if (!order) return p1;
+    const int64_t n = real_to(p1 - 1);
+    return n > real_before(p0) ? place(n - 1) + 1 : 0;
+  }
   // A query that sees one key gives it the weight 1 whatever both are: its gradient is exactly 0, not the rounding of g . v - g . out; so is the gradient of a
   // key that only such queries see.  Factors for query number n and for any key of the sequence.
   __device__ __forceinline__ bool single() const { return window == 1 && sinks <= 0; }
   __device__ __forceinline__ float query_factor(int n) const { return n == 0 || single() ? 0.f : 1.f; }
   __device__ __forceinline__ float key_factor() const { return place(1) >= S || single() ? 0.f : 1.f; }
-  // keys at places [p0, p1) are seen by no query at or behind this place
-  __device__ __forceinline__ int64_t last_query(int64_t p0, int64_t p1) const { return p0 < first_end() ? S : min(S, place(real_before(p1 - 1) + window)); }
+  // keys at places [p0, p1) are seen by no query at or behind this place, p0 where no key is real
+  __device__ __forceinline__ int64_t last_query(int64_t p0, int64_t p1) const {
+    if (!order) return p0 < first_end() ? S : min(S, p1 - 1 + window);
+    if (real_to(p1 - 1) == real_before(p0)) return p0;
+    const int64_t end = place(real_to(S - 1) - 1) + 1;
+    return p0 < first_end() ? end : min(end, place(real_before(p1 - 1) + window));
+  }
 };
 __device__ __forceinline__ bool window_sees(int n, int m, int window, int sinks) { return m >= 0 && m <= n && (n - m < window || m < sinks); }
 #endif

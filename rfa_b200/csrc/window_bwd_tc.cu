@@ -63,7 +63,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
     k.b = w % per / rows_heads;
     k.head = w % per % rows_heads;
     const WindowNumbers num(a, k.b);
-    if (KEYS) k.span = {(int)(k.row0 / kWbTile), 0, (int)((num.last_query(k.row0, min(a.S, k.row0 + 128)) + kWbTile - 1) / kWbTile)};
+    if (KEYS) k.span = {0, 0, (int)(k.row0 / kWbTile), (int)((max(k.row0 + 1, num.last_query(k.row0, min(a.S, k.row0 + 128))) + kWbTile - 1) / kWbTile)};
     else k.span = window_span<kWbTile>(num, 0, k.row0, a.T);
   };
   // heads of the other side that a work goes through, and where

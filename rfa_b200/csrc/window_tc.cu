@@ -68,6 +68,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     k.both = k.span[0];
     if (k.span[1].end > 0) {      // a last run may be without a partner
       k.both.first = min(k.span[0].first, k.span[1].first);
+      k.both.front = min(k.span[0].front, k.span[1].front);
+      k.both.firsts = max(k.span[0].firsts, k.span[1].firsts);
       k.both.end = max(k.span[0].end, k.span[1].end);
     }
   };

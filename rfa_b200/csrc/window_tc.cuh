@@ -9,16 +9,21 @@ namespace rfa {
 #ifdef __CUDACC__
 // The tiles of kTile keys that queries see: those of the first tokens, then from `first` on.
 struct WindowSpan {
-  int first, firsts, end;      // firsts: tiles that hold first tokens
-  __device__ __forceinline__ int begin() const { return firsts > 0 ? 0 : first; }
+  int front, firsts, first, end;      // tiles [front, firsts) hold first tokens
+  __device__ __forceinline__ int begin() const { return firsts > 0 ? front : first; }
   __device__ __forceinline__ int next(int kt) const { return kt + 1 < firsts ? kt + 1 : max(kt + 1, first); }
-  __device__ __forceinline__ bool has(int kt) const { return kt < end && (kt < firsts || kt >= first); }
+  __device__ __forceinline__ bool has(int kt) const { return kt < end && ((kt >= front && kt < firsts) || kt >= first); }
 };
 // of the 128 queries from row0 on, which stand at places at + row
 template <int kTile = 128>
 __device__ __forceinline__ WindowSpan window_span(const WindowNumbers& num, int64_t at, int64_t row0, int64_t T) {
-  if (row0 >= T) return {0, 0, 0};
-  return {(int)(num.first_key(at + row0) / kTile), (int)((num.first_end() + kTile - 1) / kTile), (int)((at + min(T, row0 + 128) + kTile - 1) / kTile)};
+  if (row0 >= T) return {0, 0, 0, 0};
+  const int64_t end = num.last_key(at + row0, at + min(T, row0 + 128));
+  if (end == 0) {      // no query is real: one tile, of which they see nothing
+    const int own = (int)((at + row0) / kTile);
+    return {own, 0, own, own + 1};
+  }
+  return {(int)(num.front() / kTile), (int)((num.first_end() + kTile - 1) / kTile), (int)(num.first_key(at + row0) / kTile), (int)((end + kTile - 1) / kTile)};
 }
 // the lowest n bits
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }

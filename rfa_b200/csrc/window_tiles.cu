@@ -114,11 +114,11 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1) window_fwd_kernel(c
   if (tid < kRows) nq[tid] = tid < rows ? num.at(at + i0 + tid) : -1;
   __syncthreads();
   load_tile<T, kRows>(Q, ld, a.q, b, h, i0, a.T, D, nq);
-  const int64_t first = num.first_key(at + i0) / kOther, sink_tiles = (num.first_end() + kOther - 1) / kOther, end = (at + i0 + rows + kOther - 1) / kOther;
+  const int64_t first = num.first_key(at + i0) / kOther, sink_tiles = (num.first_end() + kOther - 1) / kOther, end = (num.last_key(at + i0, at + i0 + rows) + kOther - 1) / kOther;
   float acc[4][NC][4] = {}, top[4], sum[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) { top[i] = -INFINITY; sum[i] = 0.f; }
-  for (int64_t kt = sink_tiles > 0 ? 0 : first; kt < end; kt = kt + 1 < sink_tiles ? kt + 1 : max(kt + 1, first)) {
+  for (int64_t kt = sink_tiles > 0 ? num.front() / kOther : first; kt < end; kt = kt + 1 < sink_tiles ? kt + 1 : max(kt + 1, first)) {
     __syncthreads();
     if (tid < kOther) nk[tid] = num.at(kt * kOther + tid);
     __syncthreads();
@@ -197,9 +197,9 @@ __global__ void __launch_bounds__(kThreads, NC <= 2 ? 2 : 1) window_gq_kernel(co
       if (r < rows) a.delta[bh * a.T + i0 + r] = d;
     }
   }
-  const int64_t first = num.first_key(i0) / kOther, sink_tiles = (num.first_end() + kOther - 1) / kOther, end = (i0 + rows + kOther - 1) / kOther;
+  const int64_t first = num.first_key(i0) / kOther, sink_tiles = (num.first_end() + kOther - 1) / kOther, end = (num.last_key(i0, i0 + rows) + kOther - 1) / kOther;
   float acc[4][NC][4] = {};
-  for (int64_t kt = sink_tiles > 0 ? 0 : first; kt < end; kt = kt + 1 < sink_tiles ? kt + 1 : max(kt + 1, first)) {
+  for (int64_t kt = sink_tiles > 0 ? num.front() / kOther : first; kt < end; kt = kt + 1 < sink_tiles ? kt + 1 : max(kt + 1, first)) {
     __syncthreads();
     if (tid < kOther) nk[tid] = num.at(kt * kOther + tid);
     __syncthreads();
