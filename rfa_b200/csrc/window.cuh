@@ -23,6 +23,8 @@ struct WindowArgs {
   int64_t T, S;                    // queries, keys: query t stands at place S - T + t
   int B, H, G, D, window, sinks, dtype;
   float scale;
+  float* parts;                    // [B][G][splits][min(sinks, T)][2][D]: what each part of the queries adds to gk and gv of the first tokens
+  int splits;                      // 1: no parts
 };
 
 #ifdef __CUDACC__
@@ -51,6 +53,19 @@ struct WindowNumbers {
   __device__ __forceinline__ bool single() const { return window == 1 && sinks <= 0; }
   __device__ __forceinline__ float query_factor(int n) const { return n == 0 || single() ? 0.f : 1.f; }
   __device__ __forceinline__ float key_factor() const { return place(1) >= S || single() ? 0.f : 1.f; }
+  // The first tokens' keys are seen by all queries behind, many times a window's.  Where `splits` > 1, what a tile of `rows` keys that holds some of them takes is
+  // split: the queries up to near_query(), which is all for its other keys, and the rest of them in splits - 1 parts.  Of tiles from front() on this many are
+  // split: all that hold first tokens, unless padding is among these; the ones behind then go through all their queries.
+  __device__ __forceinline__ int first_tiles(int rows) const { return (int)((min((int64_t)sinks, S) + rows - 1) / rows) + (order ? 1 : 0); }
+  __device__ __forceinline__ bool is_split(int64_t p0, int rows, int splits) const {
+    const int64_t tile = p0 / rows - front() / rows;
+    return splits > 1 && p0 < first_end() && tile >= 0 && tile < first_tiles(rows);
+  }
+  __device__ __forceinline__ int64_t near_query(int64_t p0, int64_t p1) const {
+    if (!order) return min(S, p1 - 1 + window);
+    if (real_to(p1 - 1) == real_before(p0)) return p0;
+    return min(place(real_to(S - 1) - 1) + 1, place(real_before(p1 - 1) + window));
+  }
   // keys at places [p0, p1) are seen by no query at or behind this place, p0 where no key is real
   __device__ __forceinline__ int64_t last_query(int64_t p0, int64_t p1) const {
     if (!order) return p0 < first_end() ? S : min(S, p1 - 1 + window);
@@ -65,6 +80,7 @@ __device__ __forceinline__ bool window_sees(int n, int m, int window, int sinks)
 int launch_window_order(const uint8_t* mask, const int64_t* length, int cap, int32_t* order, int32_t* pos, int64_t T, int B, cudaStream_t stream);
 int launch_window_fwd_tiles(const WindowArgs& a, cudaStream_t stream);        // window_tiles.cu: any sizes and types
 int launch_window_bwd_tiles(const WindowArgs& a, cudaStream_t stream);
+int launch_window_parts(const WindowArgs& a, int rows, float scale, cudaStream_t stream);      // the parts' sums, those of gk times scale, for tiles of `rows` keys
 bool window_tc_ok(const WindowArgs& a);                                       // window_tc.cu: fp16 and bf16, heads of up to 128 in rows that a tensor map can describe
 int launch_window_fwd_tc(const WindowArgs& a, cudaStream_t stream);
 int launch_window_bwd_tc(const WindowArgs& a, const uint8_t* mask, cudaStream_t stream);      // window_bwd_tc.cu

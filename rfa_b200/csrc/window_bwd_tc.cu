@@ -35,10 +35,11 @@ struct WbLayout {
                             delta = lse + kStages * kWbTile * 4, bar = delta + kStages * kWbTile * 4, bytes = bar + 256;
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
-enum { bR = 0, bREmpty, bFull, bEmpty = bFull + 4, bCols = bEmpty + 4, bS = bCols + 4, bP = bS + 3, bFree = bP + 3, bAcc = bFree + 3, bAccFree, bCount };
+enum { bR = 0, bREmpty, bFull, bEmpty = bFull + 4, bCols = bEmpty + 4, bColsFree = bCols + 4, bS = bColsFree + 4, bP = bS + 3, bFree = bP + 3, bAcc = bFree + 3, bAccFree, bCount };
 static_assert(bCount * 8 + 4 <= 256, "barriers");
 
-template <typename T, int DB, bool KEYS, bool ORDERED>
+// SPLIT: first tokens' queries are split (window.cuh); 4 % slower where they are not, 424 us against 407 with 8 x 16 heads x 2048 x 64, window 512 + 4
+template <typename T, int DB, bool KEYS, bool ORDERED, bool SPLIT>
 __global__ void __launch_bounds__(WbLayout<DB, KEYS>::kThreads, 1)
 window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_constant__ CUtensorMap tm_r2, const __grid_constant__ CUtensorMap tm_x1,
                      const __grid_constant__ CUtensorMap tm_x2, const __grid_constant__ WindowArgs a, int works) {
@@ -56,22 +57,46 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
     int b, head;
     int64_t row0;
     WindowSpan span;      // of 64-wide tiles of the other side
+    int split : 16, part : 8, none : 8;      // KEYS: the part of the queries, where first tokens' are split (part); none: no query
   };
   const auto work_of = [&](int w, Work& k) {      // the first rows first: keys there may be seen by all queries
     const int per = a.B * rows_heads;
     k.row0 = (int64_t)(w / per) * 128;
     k.b = w % per / rows_heads;
     k.head = w % per % rows_heads;
-    const WindowNumbers num(a, k.b);
-    if (KEYS) k.span = {0, 0, (int)(k.row0 / kWbTile), (int)((max(k.row0 + 1, num.last_query(k.row0, min(a.S, k.row0 + 128))) + kWbTile - 1) / kWbTile)};
-    else k.span = window_span<kWbTile>(num, 0, k.row0, a.T);
+    k.split = 0;
+    k.part = k.none = 0;
+    if (!KEYS) {
+      k.span = window_span<kWbTile>(WindowNumbers(a, k.b), 0, k.row0, a.T);
+      return;
+    }
+    const auto tile_end = [&](int64_t q) { return (max(k.row0 + 1, q) + kWbTile - 1) / kWbTile; };
+    if (!SPLIT || k.row0 < a.S) {
+      const WindowNumbers num(a, k.b);
+      const int64_t p1 = min(a.S, k.row0 + 128);
+      k.part = SPLIT && num.is_split(k.row0, 128, a.splits);
+      k.span = {0, 0, (int)(k.row0 / kWbTile), (int)tile_end(k.part ? num.near_query(k.row0, p1) : num.last_query(k.row0, p1))};
+    } else {      // behind the tiles: the parts
+      const int x = w - (int)((a.S + 127) / 128) * per, far = a.splits - 1, y = x / far, tiles = WindowNumbers(a, 0).first_tiles(128);
+      k.split = 1 + x % far;
+      k.b = y / tiles / a.G;
+      k.head = y / tiles % a.G;
+      const WindowNumbers num(a, k.b);
+      k.row0 = (num.front() / 128 + y % tiles) * 128;
+      k.part = k.row0 < num.first_end();
+      if (!k.part) k.row0 = 0;
+      const int64_t p1 = min(a.S, k.row0 + 128), from = tile_end(num.near_query(k.row0, p1)), all = tile_end(num.last_query(k.row0, p1)) - from;
+      const int64_t lo = from + all * (k.split - 1) / far, hi = from + all * k.split / far;
+      k.none = !k.part || lo >= hi;
+      k.span = k.none ? WindowSpan{0, 0, (int)(k.row0 / kWbTile), (int)(k.row0 / kWbTile) + 1} : WindowSpan{0, 0, (int)lo, (int)hi};
+    }
   };
   // heads of the other side that a work goes through, and where
   const auto first_head = [&](const Work& k) { return KEYS ? k.head * group : k.head / group; };
   const int other_heads = KEYS ? group : 1;
   if (tid == 0) {
     for (int i = 0; i < bCount; ++i)
-      mbar_init(&bars[i], i >= bEmpty && i < bCols ? (kColumns ? 129 : 1) : i >= bCols && i < bS ? 32 : i >= bP && i < bFree ? 128 : i == bAccFree ? kGroups * 128 : kApart && (i == bREmpty || (i >= bS && i < bP)) ? 2 : 1);
+      mbar_init(&bars[i], i >= bCols && i < bColsFree ? 32 : i >= bColsFree && i < bS ? 128 : i >= bP && i < bFree ? 128 : i == bAccFree ? kGroups * 128 : kApart && (i == bREmpty || (i >= bS && i < bP)) ? 2 : 1);
     mbar_fence_init();
     tma_prefetch_desc(&tm_r1); tma_prefetch_desc(&tm_r2); tma_prefetch_desc(&tm_x1); tma_prefetch_desc(&tm_x2);
   }
@@ -173,7 +198,8 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
                 delta[e] = a.delta[((int64_t)k.b * a.H + h) * a.T + i];
               }
             }
-            if (!mbar_wait(&bars[bFull + st], (n / kStages) & 1)) { tc_fail(8); ok = false; break; }      // and so nobody reads the stage's old ones
+            if (n >= kStages && !mbar_wait(&bars[bColsFree + st], (n / kStages + 1) & 1)) { tc_fail(12); ok = false; break; }
+            if (ORDERED && !mbar_wait(&bars[bFull + st], (n / kStages) & 1)) { tc_fail(8); ok = false; break; }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int j = st * kWbTile + e * 32 + lane;
@@ -210,7 +236,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
       work_of(w, k);
       const int64_t i = k.row0 + row;
       const bool there = i < (KEYS ? a.S : a.T);
-      const int mine = there ? WindowNumbers(a, k.b).at(i) : -1;
+      const int mine = there && !k.none ? WindowNumbers(a, k.b).at(i) : -1;
       float lse = 0.f, delta = 0.f;
       if (!KEYS && there) {
         lse = kLog2e * a.lse[((int64_t)k.b * a.H + k.head) * a.T + i];
@@ -227,7 +253,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
           bool whole;
           uint32_t seen[2] = {0u, 0u};
           if constexpr (ORDERED) whole = false;
-          else if constexpr (KEYS) whole = c0 >= k.row0 + 127 && c0 + kWbTile - 1 - k.row0 < a.window && c0 + kWbTile <= a.T;
+          else if constexpr (KEYS) whole = c0 >= k.row0 + 127 && c0 + kWbTile - 1 - k.row0 < a.window && c0 + kWbTile <= a.T;      // never where no query is (none): c0 = row0
           else whole = c0 + kWbTile - 1 <= k.row0 && k.row0 + 127 - c0 < a.window;
           if (kColumns && !mbar_wait(&bars[bCols + st], (n / kStages) & 1)) { tc_fail(9); ok = false; break; }
           if constexpr (ORDERED) {
@@ -245,7 +271,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
             if (KEYS) {
               lo = (int)min((int64_t)64, max((int64_t)0, i - c0));
               hi = (int)min((int64_t)64, (i < a.sinks ? a.T : min(a.T, i + a.window)) - c0);
-              if (!there) hi = 0;
+              if (mine < 0) hi = 0;
             } else {
               hi = (int)min((int64_t)64, i - c0 + 1);
               lo = (int)min((int64_t)64, max((int64_t)0, i - c0 - a.window + 1));
@@ -292,7 +318,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
           tmem_st_wait();
           tc_fence_before_sync();
           mbar_arrive(&bars[bP + g]);
-          if (kColumns) mbar_release_stage(&bars[bEmpty + st]);
+          if (kColumns) mbar_arrive(&bars[bColsFree + st]);      // warp 3's plain stores come next; the stage itself is given back by the products
         }
       if (!ok) break;
       // ---- the gradients: the groups take 16 columns in turn
@@ -300,7 +326,15 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
       tc_fence_after_sync();
       const int heads = KEYS ? a.G : a.H;
       const int64_t at = ((i * a.B + k.b) * heads + k.head) * a.D;
+      const WindowNumbers num(a, k.b);
       const bool real = there && mine >= 0;
+      bool whole_row = there;
+      float* parts = nullptr;      // where this row's part goes
+      if (SPLIT) {
+        const int number = there && k.part ? num.at(i) : -1;
+        if (number >= 0 && number < a.sinks) parts = a.parts + ((((int64_t)k.b * a.G + k.head) * a.splits + k.split) * min((int64_t)a.sinks, a.T) + number) * 2 * a.D;
+        whole_row = there && !parts && k.split == 0;
+      }
       const auto store = [&](uint32_t from, void* to, float f) {
         T* out = static_cast<T*>(to) + at;
         const bool wide = a.D % 16 == 0 && sectors(to);
@@ -312,10 +346,15 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
           float v[16];
 #pragma unroll
           for (int c = 0; c < 16; ++c) v[c] = real ? f * __uint_as_float(u[c]) : 0.f;
-          if (there && c0 < a.D) store_row16(out + c0, v, a.D - c0, wide);
+          if (whole_row && c0 < a.D) store_row16(out + c0, v, a.D - c0, wide);
+          if (SPLIT && parts) {
+            float* to_parts = parts + (to == a.gv ? a.D : 0) + c0;
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              if (c0 + c < a.D) to_parts[c] = real ? __uint_as_float(u[c]) : 0.f;
+          }
         }
       };
-      const WindowNumbers num(a, k.b);
       store(acc, KEYS ? a.gk : a.gq, a.scale * (KEYS ? num.key_factor() : num.query_factor(mine)));
       if (KEYS) store(acc + DP, a.gv, 1.f);
       tc_fence_before_sync();
@@ -353,20 +392,22 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const T* __restrict__
 
 namespace {
 
-template <typename T, int DB, bool KEYS, bool ORDERED>
+template <typename T, int DB, bool KEYS, bool ORDERED, bool SPLIT = false>
 int launch(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& x1, const CUtensorMap& x2, const WindowArgs& a, cudaStream_t stream) {
   using Lay = WbLayout<DB, KEYS>;
   constexpr uint32_t smem = Lay::bytes;
-  cudaError_t e = cudaFuncSetAttribute(window_bwd_tc_kernel<T, DB, KEYS, ORDERED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(window_bwd_tc_kernel<T, DB, KEYS, ORDERED, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return fail((int)e, "window_bwd: cannot reserve %u bytes of shared memory: %s", smem, cudaGetErrorString(e));
-  const int64_t works = (a.T + 127) / 128 * a.B * (KEYS ? a.G : a.H);
+  int64_t works = (a.T + 127) / 128 * a.B * (KEYS ? a.G : a.H);
+  if (SPLIT) works += ((std::min<int64_t>(a.sinks, a.T) + 127) / 128 + (a.order ? 1 : 0)) * (a.splits - 1) * a.B * a.G;
   RFA_REQUIRE(works < (int64_t)1 << 31, RFA_EUNSUPPORTED, "window_bwd: %lld tiles", (long long)works);
-  e = launch_pdl(window_bwd_tc_kernel<T, DB, KEYS, ORDERED>, dim3((unsigned)std::min<int64_t>(works, 148)), dim3(Lay::kThreads), smem, stream, r1, r2, x1, x2, a, (int)works);
+  e = launch_pdl(window_bwd_tc_kernel<T, DB, KEYS, ORDERED, SPLIT>, dim3((unsigned)std::min<int64_t>(works, 148)), dim3(Lay::kThreads), smem, stream, r1, r2, x1, x2, a, (int)works);
   if (e != cudaSuccess) return fail((int)e, "rfa_window_bwd: launch failed: %s", cudaGetErrorString(e));
   return check_launch("rfa_window_bwd");
 }
 template <typename T, int DB, bool KEYS>
 int launch_order(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& x1, const CUtensorMap& x2, const WindowArgs& a, cudaStream_t stream) {
+  if (KEYS && a.splits > 1) return a.order ? launch<T, DB, KEYS, true, KEYS>(r1, r2, x1, x2, a, stream) : launch<T, DB, KEYS, false, KEYS>(r1, r2, x1, x2, a, stream);
   return a.order ? launch<T, DB, KEYS, true>(r1, r2, x1, x2, a, stream) : launch<T, DB, KEYS, false>(r1, r2, x1, x2, a, stream);
 }
 template <typename T>
@@ -382,10 +423,12 @@ int launch_type(const CUtensorMap (&m)[8], const WindowArgs& a, const uint8_t* m
   if (int r = launch_delta<T>(a, mask, stream)) return r;
   if (a.D <= 64) {
     if (int r = launch_order<T, 1, false>(m[0], m[1], m[6], m[7], a, stream)) return r;
-    return launch_order<T, 1, true>(m[2], m[3], m[4], m[5], a, stream);
+    if (int r = launch_order<T, 1, true>(m[2], m[3], m[4], m[5], a, stream)) return r;
+  } else {
+    if (int r = launch_order<T, 2, false>(m[0], m[1], m[6], m[7], a, stream)) return r;
+    if (int r = launch_order<T, 2, true>(m[2], m[3], m[4], m[5], a, stream)) return r;
   }
-  if (int r = launch_order<T, 2, false>(m[0], m[1], m[6], m[7], a, stream)) return r;
-  return launch_order<T, 2, true>(m[2], m[3], m[4], m[5], a, stream);
+  return a.splits > 1 ? launch_window_parts(a, 128, a.scale, stream) : 0;
 }
 
 }  // namespace

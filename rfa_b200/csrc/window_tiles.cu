@@ -238,15 +238,32 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 2 : 1) window_gkv_kernel(c
   __shared__ float lse[kOther], delta[kOther];
   const int D = a.D, ld = row_floats(D), tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
   float *K = tiles_smem, *V = K + kRows * ld, *Q = V + kRows * ld, *Gr = Q + kOther * ld, *P = Gr + kOther * ld, *dS = P + kOther * kLdP;
-  const int64_t tiles = (a.S + kRows - 1) / kRows, bg = blockIdx.x / tiles, j0 = blockIdx.x % tiles * kRows;
+  const int64_t tiles = (a.S + kRows - 1) / kRows, normal = tiles * a.B * a.G;
+  int64_t bg = blockIdx.x / tiles, j0 = blockIdx.x % tiles * kRows;
+  int split = 0, far = a.splits - 1;
+  if (blockIdx.x >= normal) {      // a part of the queries that see a tile of first tokens
+    const int64_t x = blockIdx.x - normal, y = x / far;
+    const int count = WindowNumbers(a, 0).first_tiles(kRows);
+    split = 1 + (int)(x % far);
+    bg = y / count;
+    const WindowNumbers num(a, (int)(bg / a.G));
+    j0 = (num.front() / kRows + y % count) * kRows;
+    if (j0 >= num.first_end()) return;
+  }
   const int b = (int)(bg / a.G), kv = (int)(bg % a.G), group = a.H / a.G;
   const WindowNumbers num(a, b);
+  const bool part = num.is_split(j0, kRows, a.splits);
   const int rows = (int)min((int64_t)kRows, a.S - j0);
   if (tid < kRows) nk[tid] = tid < rows ? num.at(j0 + tid) : -1;
   __syncthreads();
   load_tile<T, kRows>(K, ld, a.k, b, kv, j0, a.S, D, nk);
   load_tile<T, kRows>(V, ld, a.v, b, kv, j0, a.S, D, nk);
-  const int64_t first = j0 / kOther, end = (num.last_query(j0, j0 + rows) + kOther - 1) / kOther;
+  int64_t first = j0 / kOther, end = (num.last_query(j0, j0 + rows) + kOther - 1) / kOther;
+  if (part) {
+    const int64_t near = (num.near_query(j0, j0 + rows) + kOther - 1) / kOther, all = end - near;
+    if (split == 0) end = near;
+    else { first = near + all * (split - 1) / far; end = near + all * split / far; }
+  }
   float gk[4][NC][4] = {}, gv[4][NC][4] = {};
   for (int h = kv * group; h < (kv + 1) * group; ++h)
     for (int64_t qt = first; qt < end; ++qt) {
@@ -285,19 +302,45 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 2 : 1) window_gkv_kernel(c
   for (int i = 0; i < 4; ++i) {
     const int r = 4 * ty + i;
     if (r >= rows) continue;
+    if (part && nk[r] >= 0 && nk[r] < a.sinks) {
+      float* parts = a.parts + ((bg * a.splits + split) * min((int64_t)a.sinks, a.T) + nk[r]) * 2 * D;
+      store_part<float, NC>(parts, gk[i], D, tx, 1.f);
+      store_part<float, NC>(parts + D, gv[i], D, tx, 1.f);
+      continue;
+    }
+    if (split > 0) continue;
     const int64_t at = (((j0 + r) * a.B + b) * a.G + kv) * D;
     store_part<T, NC>(static_cast<T*>(a.gk) + at, gk[i], D, tx, num.key_factor());
     store_part<T, NC>(static_cast<T*>(a.gv) + at, gv[i], D, tx, 1.f);
   }
 }
 
+// gk and gv of the first tokens from their parts, in the parts' order: one CTA per (row, head, token)
+template <typename T>
+__global__ void __launch_bounds__(128) window_parts_kernel(const __grid_constant__ WindowArgs a, int rows, float scale) {
+  const int64_t firsts = min((int64_t)a.sinks, a.T), bg = blockIdx.x / firsts, m = blockIdx.x % firsts;
+  const int b = (int)(bg / a.G), kv = (int)(bg % a.G);
+  const WindowNumbers num(a, b);
+  const int64_t j = num.place(m);
+  if (j >= a.S || !num.is_split(j / rows * rows, rows, a.splits)) return;
+  const int64_t at = ((j * a.B + b) * a.G + kv) * a.D;
+  const float* parts = a.parts + (bg * a.splits * firsts + m) * 2 * a.D;
+  for (int c = threadIdx.x; c < 2 * a.D; c += 128) {
+    float sum = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) sum += parts[s * firsts * 2 * a.D + c];
+    if (c < a.D) static_cast<T*>(a.gk)[at + c] = from_f<T>(scale * num.key_factor() * sum);
+    else static_cast<T*>(a.gv)[at + c - a.D] = from_f<T>(sum);
+  }
+}
+
 size_t tile_bytes(int rows, int others, int scores, int D) {
   return sizeof(float) * ((size_t)rows * kRows * row_floats(D) + (size_t)others * kOther * row_floats(D) + (size_t)scores * kOther * kLdP);
 }
-int run(void (*kernel)(const WindowArgs), const WindowArgs& a, int64_t places, int heads, size_t smem, cudaStream_t stream, const char* what) {
+int run(void (*kernel)(const WindowArgs), const WindowArgs& a, int64_t places, int heads, size_t smem, cudaStream_t stream, const char* what, int64_t more = 0) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return fail((int)e, "%s: cannot reserve %zu bytes of shared memory: %s", what, smem, cudaGetErrorString(e));
-  const int64_t ctas = (places + kRows - 1) / kRows * a.B * heads;
+  const int64_t ctas = (places + kRows - 1) / kRows * a.B * heads + more;
   RFA_REQUIRE(ctas < (int64_t)1 << 31, RFA_EUNSUPPORTED, "%s: %lld tiles", what, (long long)ctas);
   kernel<<<(unsigned)ctas, kThreads, smem, stream>>>(a);
   return check_launch(what);
@@ -309,7 +352,9 @@ int fwd(const WindowArgs& a, cudaStream_t stream) {
 template <typename T, int NC>
 int bwd(const WindowArgs& a, cudaStream_t stream) {
   if (int r = run(window_gq_kernel<T, NC>, a, a.T, a.H, tile_bytes(2, 2, 1, a.D), stream, "rfa_window_bwd (q)")) return r;
-  return run(window_gkv_kernel<T, NC>, a, a.S, a.G, tile_bytes(2, 2, 2, a.D), stream, "rfa_window_bwd (k, v)");
+  const int64_t parts = a.splits > 1 ? ((std::min<int64_t>(a.sinks, a.T) + kRows - 1) / kRows + (a.order ? 1 : 0)) * (a.splits - 1) * a.B * a.G : 0;
+  if (int r = run(window_gkv_kernel<T, NC>, a, a.S, a.G, tile_bytes(2, 2, 2, a.D), stream, "rfa_window_bwd (k, v)", parts)) return r;
+  return a.splits > 1 ? launch_window_parts(a, kRows, 1.f, stream) : 0;
 }
 #define RFA_WINDOW_TILES(CALL)                                                                                       \
   do {                                                                                                               \
@@ -320,6 +365,14 @@ int bwd(const WindowArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
+int launch_window_parts(const WindowArgs& a, int rows, float scale, cudaStream_t stream) {
+  const int64_t ctas = std::min<int64_t>(a.sinks, a.T) * a.B * a.G;
+  RFA_REQUIRE(ctas < (int64_t)1 << 31, RFA_EUNSUPPORTED, "window_bwd: %lld first tokens", (long long)ctas);
+  if (a.dtype == RFA_F32) window_parts_kernel<float><<<(unsigned)ctas, 128, 0, stream>>>(a, rows, scale);
+  else if (a.dtype == RFA_F16) window_parts_kernel<__half><<<(unsigned)ctas, 128, 0, stream>>>(a, rows, scale);
+  else window_parts_kernel<__nv_bfloat16><<<(unsigned)ctas, 128, 0, stream>>>(a, rows, scale);
+  return check_launch("rfa_window_bwd (first tokens)");
+}
 int launch_window_fwd_tiles(const WindowArgs& a, cudaStream_t stream) { RFA_WINDOW_TILES(fwd); }
 int launch_window_bwd_tiles(const WindowArgs& a, cudaStream_t stream) { RFA_WINDOW_TILES(bwd); }
 

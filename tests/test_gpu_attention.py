@@ -298,6 +298,15 @@ WINDOW = [
     (64, 2, 2, 1, 35, 20, 2, "any", "fp16"),
     (63, 2, 2, 1, 35, 20, 2, "any", "fp16"),
     (400, 1, 4, 2, 127, 90, 0, None, "bf16"),
+    # first tokens whose many queries are split
+    (1500, 1, 2, 1, 64, 30, 4, None, "bf16"),
+    (1501, 1, 2, 1, 64, 30, 4, "left", "fp16"),
+    (1100, 2, 2, 1, 33, 16, 70, "any", "fp32"),
+    (2100, 1, 3, 3, 128, 100, 130, "right", "bf16"),
+    (1300, 2, 2, 2, 24, 40, 3, "gap", "fp32"),
+    (1300, 1, 2, 1, 128, 1, 200, "gap", "fp16"),
+    (1000, 1, 4, 1, 64, 3, 1, "any", "fp16"),
+    (1030, 2, 2, 1, 100, 8, 5, "right", "bf16"),
 ]
 
 
