@@ -8,7 +8,8 @@
 // Scores and their gradients have three places (two where the sums leave no room for a third) and as many groups of warps, which take the tiles in turn, a thread to
 // each row.  delta = sum of g o out comes from a
 // kernel of its own.  Tiles that are seen whole need no mask.  Padded places: as in window_tc.cu, warp 3 fetches numbers (and, KEYS, lse and delta of the queries)
-// and clears the rows that are summed over.
+// and clears the rows that are summed over.  First tokens' keys: works behind the tiles' take parts of their queries (SPLIT; window.cuh), whose sums stay in 32 bits for
+// window_parts_kernel.
 //
 // Warp roles (512 or 384 threads): warp 0 TMA producer, warp 1 issues S and D, warp 2 the sums, warp 3 columns' data or, where there are none, D, warps 4..7, 8..11, 12..15 the groups.  All
 // waits are bounded.
