@@ -276,7 +276,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       if (!first && !mbar_wait(&bars[wO + 2 * u + ((it - 1) & 1)], ((it - 1) >> 1) & 1)) { tc_fail(11); break; }
       tc_fence_after_sync();
       const int h = k.h0 + (pair_heads ? u : 0);
-      const float inv = sum > 0.f && mine >= 0 ? 1.f / sum : 0.f;      // a query that sees nothing (a padded one) has 0
+      const bool real = mine >= 0;                       // sees itself at least; a padded query has 0
+      const float inv = real ? 1.f / sum : 0.f;          // whatever the sum is: a NaN score makes the row NaN
       T* out = static_cast<T*>(a.out) + ((i * a.B + k.b) * a.H + h) * a.D;
 #pragma unroll 1
       for (int c0 = 0; c0 < DP; c0 += 32) {
@@ -286,12 +287,12 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tmem_ld_wait();
         float v[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = inv > 0.f ? __uint_as_float(o[c]) * inv : 0.f;
+        for (int c = 0; c < 32; ++c) v[c] = real ? __uint_as_float(o[c]) * inv : 0.f;
         if (i < a.T && c0 < a.D) store_row16(out + c0, v, a.D - c0, wide);
         if (i < a.T && c0 + 16 < a.D) store_row16(out + c0 + 16, v + 16, a.D - c0 - 16, wide);
       }
       tc_fence_before_sync();      // the next weights let the issuer write O again
-      if (a.lse && i < a.T) a.lse[((int64_t)k.b * a.H + h) * a.T + i] = inv > 0.f ? kLn2 * (top + __log2f(sum)) : 0.f;
+      if (a.lse && i < a.T) a.lse[((int64_t)k.b * a.H + h) * a.T + i] = real ? kLn2 * (top + __log2f(sum)) : 0.f;
     }
   } else if (ORDERED) {
     // ------------------------------------------------------------------ warp 3: numbers of a tile's keys; values of places without a token

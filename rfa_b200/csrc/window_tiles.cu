@@ -152,14 +152,15 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1) window_fwd_kernel(c
   for (int i = 0; i < 4; ++i) {
     const int r = 4 * ty + i;
     if (r >= rows) continue;
-    const float inv = sum[i] > 0.f && nq[r] >= 0 ? 1.f / sum[i] : 0.f;       // a query that sees nothing (a padded one) has 0
-    if (inv == 0.f)
+    const bool real = nq[r] >= 0;                       // sees itself at least; a padded query has 0
+    const float inv = real ? 1.f / sum[i] : 0.f;        // whatever the sum is: a NaN score makes the row NaN
+    if (!real)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][c][e] = 0.f;
     store_part<T, NC>(static_cast<T*>(a.out) + (((i0 + r) * a.B + b) * a.H + h) * D, acc[i], D, tx, inv);
-    if (a.lse && tx == 0) a.lse[bh * a.T + i0 + r] = sum[i] > 0.f ? top[i] + logf(sum[i]) : 0.f;
+    if (a.lse && tx == 0) a.lse[bh * a.T + i0 + r] = real ? top[i] + logf(sum[i]) : 0.f;
   }
 }
 
