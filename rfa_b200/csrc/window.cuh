@@ -28,6 +28,8 @@ struct WindowArgs {
 };
 
 #ifdef __CUDACC__
+// The reference of weights before a key has been seen: the lowest number, so that any finite score moves it, and not -inf, which taken from itself is no number.
+constexpr float kLowest = -3.402823466e38f;
 struct WindowNumbers {
   const int32_t *order, *pos;
   int64_t S;

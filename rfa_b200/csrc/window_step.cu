@@ -36,7 +36,7 @@ __device__ __forceinline__ void join_parts(const StepArgs& a, float (&red)[kWarp
   __syncthreads();
   for (int i = tid; i < kHeads * kWidth; i += kThreads) {
     const int h = i / kWidth, c = i % kWidth;
-    float t = -1e30f, n = 0.f, o = 0.f;
+    float t = kLowest, n = 0.f, o = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) t = fmaxf(t, red[w][h][kWidth]);
 #pragma unroll
@@ -60,7 +60,7 @@ __device__ __forceinline__ void join_parts(const StepArgs& a, float (&red)[kWarp
     cluster.sync();
     for (int i = part * kThreads + tid; i < kHeads * kWidth; i += a.parts * kThreads) {
       const int h = i / kWidth, c = i % kWidth;
-      float t = -1e30f, n = 0.f, o = 0.f;
+      float t = kLowest, n = 0.f, o = 0.f;
       for (int r = 0; r < a.parts; ++r) t = fmaxf(t, cluster.map_shared_rank(&whole[h][0], r)[kWidth]);
       for (int r = 0; r < a.parts; ++r) {
         const float* w = cluster.map_shared_rank(&whole[h][0], r);
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) window_step_kernel(const __grid_cons
     if (h < heads) load(static_cast<const T*>(a.q.p) + b * a.q.b + (h0 + h) * a.q.h, r);
 #pragma unroll
     for (int e = 0; e < 8; ++e) q[h][e] = r.get(e) * (a.scale * kLog2e);
-    top[h] = -1e30f;
+    top[h] = kLowest;
   }
   const int step = kWarps * kSlots;
   for (int j0 = lo + warp * kSlots; j0 < hi; j0 += kFlight * step) {      // the same number of times for a warp's lanes
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kMmaThreads, DB == 1 ? 5 : 3) window_step_mma_
   T* ck = static_cast<T*>(a.cache_k) + bg * cap * a.D;
   T* cv = static_cast<T*>(a.cache_v) + bg * cap * a.D;
   const float scale = a.scale * kLog2e;
-  float o[8 * DB][4] = {}, top = -1e30f, sum = 0.f;      // column tile 8 y + j, columns 2 t and 2 t + 1: numbers 64 y + 16 t + j and + 8 of head g
+  float o[8 * DB][4] = {}, top = kLowest, sum = 0.f;      // column tile 8 y + j, columns 2 t and 2 t + 1: numbers 64 y + 16 t + j and + 8 of head g
   const auto piece = [&](const T* row, int at) { return at < a.D ? *reinterpret_cast<const uint4*>(row + at) : zero; };
   for (int j0 = lo + warp * 16; j0 < hi; j0 += kMmaWarps * 16) {
     uint4 k[2][2 * DB], v[4][DB];

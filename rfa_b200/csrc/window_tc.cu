@@ -2,7 +2,7 @@
 //
 // A CTA takes one pair of units after the other, each unit 128 queries of one batch row, that read the same keys -- two heads that share a key head, or else two
 // runs of one head -- and goes through the 64-key tiles that either of them sees: those of the first tokens, then from the window's start on.  Per unit and tile
-//     S = Q K^T (fp32, TMEM)  ->  P = 2^(S scale log2(e) - m), 16 bits, over S  ->  O += P V
+//     S = Q K^T (fp32, TMEM)  ->  P = 2^(scale log2(e) (S - m)), 16 bits, over S  ->  O += P V
 // with a thread to each row, whose scores it holds in registers: the row's maximum, then P and the sum.  m moves only when it is exceeded by more than 8 (P is then
 // at most 256, which both types hold), and only then O is rescaled, by the row's own thread.  Tiles that every query of the unit sees whole need no mask; in the
 // others scores that are not seen are -inf before anything is made of them.  A unit's scores have two places in TMEM, so that the products of the next tile run under the
@@ -185,7 +185,9 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const WindowSpan own = u ? k.span[1] : k.span[0];
       const int64_t i0 = u ? k.row[1] : k.row[0], i = i0 + row, place = at + i;
       const int mine = i < a.T ? WindowNumbers(a, k.b).at(place) : -1;
-      float top = -1e30f, sum = 0.f;      // the reference that weights are taken against, in units of log 2
+      // The score that weights are taken against.  It is subtracted before the scale, two scores at a time: scaled and subtracted in one, the rest of the product's
+      // rounding stays, and from scores of 2^28 on 2 to that is beyond fp16.
+      float top = kLowest, sum = 0.f;
       bool first = true;
 #pragma unroll 1
       for (int kt = k.both.begin(); kt < k.both.end; kt = k.both.next(kt), ++n) {
@@ -231,10 +233,10 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < 64; c += 2) most[(c >> 1) & 3] = fmaxf(most[(c >> 1) & 3], fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
-        const float now = scale * fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-        const bool move = now > top + 8.f;
+        const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        const bool move = scale * (now - top) > 8.f;
         if (__any_sync(0xffffffffu, move)) {
-          const float ref = move ? now : top, keep = ex2(top - ref);
+          const float ref = move ? now : top, keep = ex2(scale * (top - ref));
           top = ref;
           sum *= keep;
           if (!first) {      // O of the tiles before has to follow
@@ -257,7 +259,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           uint32_t p[16];
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            const float p0 = ex2(fmaf(__uint_as_float(s[x * 32 + c]), scale, -top)), p1 = ex2(fmaf(__uint_as_float(s[x * 32 + c + 1]), scale, -top));
+            const float2 e = scaled_rest(__uint_as_float(s[x * 32 + c]), __uint_as_float(s[x * 32 + c + 1]), top, scale);
+            const float p0 = ex2(e.x), p1 = ex2(e.y);
             part[(c >> 1) & 1] += p0;
             part[2 + ((c >> 1) & 1)] += p1;
             p[c >> 1] = pack2h<T>(p0, p1);
@@ -292,7 +295,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (i < a.T && c0 + 16 < a.D) store_row16(out + c0 + 16, v + 16, a.D - c0 - 16, wide);
       }
       tc_fence_before_sync();      // the next weights let the issuer write O again
-      if (a.lse && i < a.T) a.lse[((int64_t)k.b * a.H + h) * a.T + i] = real ? kLn2 * (top + __log2f(sum)) : 0.f;
+      if (a.lse && i < a.T) a.lse[((int64_t)k.b * a.H + h) * a.T + i] = real ? kLn2 * fmaf(top, scale, __log2f(sum)) : 0.f;
     }
   } else if (ORDERED) {
     // ------------------------------------------------------------------ warp 3: numbers of a tile's keys; values of places without a token

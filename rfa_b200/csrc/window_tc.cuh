@@ -25,6 +25,15 @@ __device__ __forceinline__ WindowSpan window_span(const WindowNumbers& num, int6
   }
   return {(int)(num.front() / kTile), (int)((num.first_end() + kTile - 1) / kTile), (int)(num.first_key(at + row0) / kTile), (int)((end + kTile - 1) / kTile)};
 }
+// scale (a - top), scale (b - top)
+__device__ __forceinline__ float2 scaled_rest(float a, float b, float top, float scale) {
+  float2 r;
+  asm("{\n\t.reg .b64 v, f, t;\n\t"
+      "mov.b64 v, {%2, %3};\n\tmov.b64 t, {%4, %4};\n\tmov.b64 f, {%5, %5};\n\t"
+      "add.rn.f32x2 v, v, t;\n\tmul.rn.f32x2 v, v, f;\n\t"
+      "mov.b64 {%0, %1}, v;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a), "f"(b), "f"(-top), "f"(scale));
+  return r;
+}
 // the lowest n bits
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 #endif

@@ -73,3 +73,23 @@ def test_window_passes_on_what_is_not_finite(dtype, D, scale, pad, what, value):
     gq, = torch.autograd.grad(out, leaves[0], torch.randn_like(out))
     bad = ~torch.isfinite(want).all(-1)
     assert not torch.isfinite(gq[bad]).all(-1).any() and torch.isfinite(gq[:, 0]).all()
+
+
+@pytest.mark.parametrize("dtype,D,pad", [("fp32", 24, None), ("bf16", 64, None), ("bf16", 128, "any"), ("bf16", 200, None)])
+def test_window_scores_far_below_zero(dtype, D, pad):
+    """Scores of -1e32 and less have a largest one too."""
+    from rfa_b200.window_attention import incremental_window_attention, window_attention
+    torch.manual_seed(D)
+    T, B, H, window, dt = 150, 2, 2, 7, TYPES[dtype]
+    v = torch.randn(T, B, H, D, device="cuda").to(dt)
+    q = torch.full_like(v, 1e16)
+    k = (torch.full_like(v, -1e16).float() * (1 + torch.arange(T, device="cuda") % 10 / 16)[:, None, None, None]).to(dt)      # steps of 6 %, so that one key has all the weight
+    mask = some_mask(pad, B, T)
+    want = window_by_rows(q, k, v, sees(mask, T, B, window, 1), D ** -0.5)
+    near(window_attention(q=q, k=k, v=v, window=window, sinks=1, key_padding_mask=mask), want, dt)
+    state, outs = {}, []
+    for a, b in [(0, 30)] + [(t, t + 1) for t in range(30, T)]:
+        o, *new = incremental_window_attention(q=q[a:b], k=k[a:b], v=v[a:b], window=window, sinks=1, key_padding_mask=None if mask is None else mask[:, a:b], **state)
+        state = dict(zip(("prev_k", "prev_v", "prev_len"), new))
+        outs.append(o)
+    near(torch.cat(outs), want, dt)
