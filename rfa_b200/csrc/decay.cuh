@@ -74,8 +74,11 @@ int launch_decay_step(const rfa_decay_t& c, void* out, float* s, cudaStream_t st
 __device__ __forceinline__ uint32_t log_decay_bits(const void* p, int dtype, int64_t i) {      // as it stands in memory, to be asked for early
   return dtype == RFA_F32 ? static_cast<const uint32_t*>(p)[i] : static_cast<const uint16_t*>(p)[i];
 }
+__device__ __forceinline__ float log_decay_number(uint32_t bits, int dtype) {
+  return dtype == RFA_F32 ? __uint_as_float(bits) : dtype == RFA_F16 ? __half2float(__ushort_as_half((uint16_t)bits)) : __uint_as_float(bits << 16);
+}
 __device__ __forceinline__ double log_decay_of(uint32_t bits, int dtype) {
-  const float g = dtype == RFA_F32 ? __uint_as_float(bits) : dtype == RFA_F16 ? __half2float(__ushort_as_half((uint16_t)bits)) : __uint_as_float(bits << 16);
+  const float g = log_decay_number(bits, dtype);
   return (double)(g < -1e4f ? -1e4f : g);
 }
 __device__ __forceinline__ double log_decay_at(const void* p, int dtype, int64_t i) { return log_decay_of(log_decay_bits(p, dtype, i), dtype); }

@@ -180,12 +180,20 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         bits[e] = real[e] ? log_decay_bits(a.decay.p, a.decay_dtype, k.b * a.decay.b + k.h * a.decay.h + t * a.decay.t) : 0u;
         if (real[e] && k.mask) real[e] = !k.mask[t];
       }
+      // Growth beyond 2^32768 (e^22713) is taken as that: an infinite weight still, and 128 of them fit 64 bits.  What is no number makes L none from its token on.
       long long sum[4], all = 0;
+      bool none[4], any = false;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (real[e]) all += __double2ll_rn(fmax(log_decay_of(bits[e], a.decay_dtype) * kLog2eD, -64.0) * 1099511627776.0);
+        if (real[e]) {
+          const float g = log_decay_number(bits[e], a.decay_dtype);
+          any |= g != g;
+          all += __double2ll_rn((double)fminf(fmaxf(g, kDecayFloor), 22713.f) * (kLog2eD * 1099511627776.0));
+        }
         sum[e] = all;
+        none[e] = any;
       }
+      const bool behind = (__ballot_sync(0xffffffffu, any) & ((1u << lane) - 1)) != 0;
       long long before = all;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -195,7 +203,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       before -= all;
       if (w != blockIdx.x && !mbar_wait(&bars[gP], ph ^ 1)) { tc_fail(19); break; }      // the last chunk's have been read
 #pragma unroll
-      for (int e = 0; e < 4; ++e) L[lane * 4 + e] = __ll2float_rn(sum[e] + before) * 0x1p-40f;
+      for (int e = 0; e < 4; ++e) L[lane * 4 + e] = none[e] || behind ? __int_as_float(0x7fffffff) : __ll2float_rn(sum[e] + before) * 0x1p-40f;
       mbar_arrive(&bars[gL]);
     }
   } else {

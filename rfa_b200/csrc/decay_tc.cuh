@@ -31,6 +31,7 @@ namespace rfa {
 
 constexpr int kDecThreads = 768;
 constexpr double kLog2eD = 1.4426950408889634;
+constexpr float kDecayFloor = -44.3614196f;      // -64 in units of log 2
 
 struct DecayTcArgs {
   DecayRows decay;
@@ -405,7 +406,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       double L[4], all = 0.0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (real[e]) all += fmax(log_decay_of(bits[e], a.decay_dtype) * kLog2eD, -64.0);      // in units of log 2
+        if (real[e]) {      // in units of log 2; NaN stays NaN
+          const float g = log_decay_number(bits[e], a.decay_dtype);
+          all += (double)(g < kDecayFloor ? kDecayFloor : g) * kLog2eD;
+        }
         L[e] = all;
       }
       if (c + 1 < nchunk) ask(c + 1);
@@ -416,7 +420,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (lane >= o) before += up;
       }
       const double end = __shfl_sync(0xffffffffu, before, 31);
-      before -= all;
+      before = __shfl_up_sync(0xffffffffu, before, 1);      // and not less its own sum: a lane's first tokens know nothing of its last
+      if (lane == 0) before = 0.0;
       run += end;
       float l[4], f[4];
 #pragma unroll

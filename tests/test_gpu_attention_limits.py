@@ -93,3 +93,59 @@ def test_window_scores_far_below_zero(dtype, D, pad):
         state = dict(zip(("prev_k", "prev_v", "prev_len"), new))
         outs.append(o)
     near(torch.cat(outs), want, dt)
+
+
+# ------------------------------------------------------------------------------------------------ decay
+@pytest.mark.parametrize("value", [math.nan, math.inf, 1e30])
+@pytest.mark.parametrize("at", [0, 150])
+@pytest.mark.parametrize("dtype,K,D,decay", [("fp32", 24, 40, "token"), ("fp16", 64, 64, "token"), ("bf16", 128, 128, "token"), ("bf16", 64, 128, "fp32"), ("bf16", 200, 64, "token"),
+                                             ("fp16", 33, 90, "token")])
+def test_decay_that_is_not_finite(dtype, K, D, decay, at, value):
+    """A decay that is no number, or growth beyond all numbers, shows in every result that it is part of, in prompts, states, gradients and single tokens alike."""
+    from rfa_b200.decay_attention import decay_attention, incremental_decay_attention
+    torch.manual_seed(K)
+    T, dt = 400, TYPES[dtype]
+    if value == 1e30 and dt == torch.float16:
+        value = 60000.0
+    q, k, v = make(T, 2, (2, 2, 2), (K, K, D), dt, False)
+    g = (-0.1 * torch.rand(T, 2, 2, device="cuda")).to(torch.float32 if decay == "fp32" else dt)
+    s = torch.randn(2, 2, K, D, device="cuda")
+    go = torch.randn_like(v)
+    bad = g.clone()
+    bad[at, 1, 1] = value
+
+    def results(g):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, g)]
+        out = decay_attention(q=leaves[0], k=leaves[1], v=leaves[2], log_decay=leaves[3])
+        with_state, last = incremental_decay_attention(q=q, k=k, v=v, log_decay=g, s=s.clone())
+        tokens, one = [], s.clone()
+        for t in range(max(at - 2, 0), at + 3):
+            tokens.append(incremental_decay_attention(q=q[t:t + 1], k=k[t:t + 1], v=v[t:t + 1], log_decay=g[t:t + 1], s=one)[0])
+        return [out, with_state, *torch.autograd.grad(out, leaves, go)], [last, one], torch.cat(tokens)
+
+    clean, dirty = results(g), results(bad)
+    for x, y in zip(clean[0], dirty[0]):                    # other rows and heads, and what came before, as they were
+        assert torch.isfinite(x).all()
+        assert torch.equal(x[:, 0], y[:, 0]) and torch.equal(x[:, 1, 0], y[:, 1, 0])
+    out, with_state, gq, gk, gv, gg = (x[:, 1, 1] for x in dirty[0])
+    assert not torch.isfinite(with_state[at:]).all(-1).any()
+    if at:
+        assert not torch.isfinite(out[at:]).all(-1).any() and not torch.isfinite(gq[at:]).all(-1).any()
+        assert torch.equal(out[:at], clean[0][0][:at, 1, 1]) and torch.equal(with_state[:at], clean[0][1][:at, 1, 1])
+        assert not torch.isfinite(gk[:at]).all(-1).any() and not torch.isfinite(gv[:at]).all(-1).any() and not torch.isfinite(gg[1:at]).any()
+    for x, y in zip(clean[1], dirty[1]):
+        assert torch.isfinite(x).all() and not torch.isfinite(y[1, 1]).any() and torch.equal(x[0], y[0]) and torch.equal(x[1, 0], y[1, 0])
+    first = min(at, 2)
+    assert not torch.isfinite(dirty[2][first:, 1, 1]).all(-1).any() and torch.equal(dirty[2][:first], clean[2][:first])
+
+
+def test_decay_of_a_head_that_is_not_finite():
+    from rfa_b200.decay_attention import decay_attention
+    torch.manual_seed(2)
+    for dt, K in ((torch.float32, 24), (torch.float16, 64), (torch.bfloat16, 128)):
+        q, k, v = make(300, 2, (3, 3, 3), (K, K, K), dt, False)
+        g = torch.tensor([-0.1, math.nan, -0.2], device="cuda", requires_grad=True)
+        out = decay_attention(q=q, k=k, v=v, log_decay=g)
+        gg, = torch.autograd.grad(out, g, torch.randn_like(out))
+        assert torch.isfinite(out[:, :, ::2]).all() and torch.isnan(out[:, :, 1]).all()
+        assert torch.isfinite(gg).tolist() == [True, False, True]
