@@ -1,5 +1,7 @@
 // Linear attention with a decay on the tensor cores: plans and launches (the kernel: decay_tc.cuh).
 #define RFA_TC_FAMILY 10
+#include <cmath>
+
 #include "decay_tc.cuh"
 
 namespace rfa {
@@ -133,6 +135,8 @@ int launch_decay_tc(const rfa_decay_t& c, const SweepPlan& plan, char* workspace
   a.s_out = {s_out, c.D, 1};
   a.in_scale = 1.f;
   a.out_scale = c.scale;
+  a.p_scale = std::fabs(c.scale) <= 1.f ? c.scale : 1.f;
+  a.o_scale = std::fabs(c.scale) <= 1.f ? 1.f : c.scale;
   return sweep<true>(bf16, q, k, v, a, s_out != nullptr, stream);
 }
 

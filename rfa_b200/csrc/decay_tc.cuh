@@ -8,6 +8,7 @@
 //     O  = P V
 //     S  = 2^(L_end) S + K'^T V
 //     out_i = scale (2^(L_i) N_i + O_i)
+// A scale of at most one goes into P, a larger one to what comes of it: fp16 then holds scores that fit with the scale or without it.
 // L_i - L_j is at most 0 in a model, so that nothing overflows whatever the decays are.  S is exact where it leaves the call (EXACT): K' goes in as two 16-bit
 // parts then (bf16's hold 16 bits: the products are off by 2^-17, the state by 3e-6 of its norm).  Where only outputs are wanted its first part is as
 // good as the 16-bit copies of S and P.  A log decay below -64 (in units of log 2) is taken as that.
@@ -42,7 +43,8 @@ struct DecayTcArgs {
   double* seg_decay;
   int64_t T, tseg;
   int B, H, K, D, nseg, decay_dtype, rev;
-  float in_scale, out_scale;
+  float in_scale, out_scale;     // of the scores; out_scale = p_scale o_scale: in P, of its products
+  float p_scale, o_scale;
 };
 
 // Offsets in shared memory, from a 1024-aligned base, and TMEM columns.  KB, DB: 64-wide boxes of a key, of a value.  As many stages as there is room for: a load
@@ -223,8 +225,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
             const float4 l = *reinterpret_cast<const float4*>(L + piece * 16 + i);
-            float x[4] = {__uint_as_float(s[i]) * ex2(mine - l.x), __uint_as_float(s[i + 1]) * ex2(mine - l.y), __uint_as_float(s[i + 2]) * ex2(mine - l.z),
-                          __uint_as_float(s[i + 3]) * ex2(mine - l.w)};
+            float x[4] = {__uint_as_float(s[i]) * a.p_scale * ex2(mine - l.x), __uint_as_float(s[i + 1]) * a.p_scale * ex2(mine - l.y),
+                          __uint_as_float(s[i + 2]) * a.p_scale * ex2(mine - l.z), __uint_as_float(s[i + 3]) * a.p_scale * ex2(mine - l.w)};
             if constexpr (decltype(DIAG)::value) {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
@@ -377,7 +379,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
           float v[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = gone ? 0.f : fmaf(f, __uint_as_float(n[i]), a.out_scale * __uint_as_float(p[i]));
+          for (int i = 0; i < 16; ++i) v[i] = gone ? 0.f : fmaf(f, __uint_as_float(n[i]), a.o_scale * __uint_as_float(p[i]));
           if (there && c0 < a.D) store_row16(o + c0, v, a.D - c0, wide);
         }
         mbar_arrive(&bars[dLFree + c % Lay::kL]);

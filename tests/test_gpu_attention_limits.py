@@ -5,7 +5,7 @@ import math
 
 import pytest
 import torch
-from test_gpu_attention import TYPES, make, near, places, some_mask
+from test_gpu_attention import TYPES, decay_dense, make, near, places, some_mask
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +149,29 @@ def test_decay_of_a_head_that_is_not_finite():
         gg, = torch.autograd.grad(out, g, torch.randn_like(out))
         assert torch.isfinite(out[:, :, ::2]).all() and torch.isnan(out[:, :, 1]).all()
         assert torch.isfinite(gg).tolist() == [True, False, True]
+
+
+@pytest.mark.parametrize("T", [20, 300])
+def test_decay_scores_beyond_half(T):
+    """fp16, raw scores of 131072: what counts is the scaled score."""
+    from rfa_b200.decay_attention import decay_attention, incremental_decay_attention
+    torch.manual_seed(3)
+    q, k = (torch.full((T, 2, 2, 128), 32.0, device="cuda").half() for _ in range(2))
+    v = (0.1 * torch.randn(T, 2, 2, 128, device="cuda")).half()
+    g = torch.full((T, 2, 2), -0.1, device="cuda")
+    want, last = decay_dense(*(x.double() for x in (q, k, v, g)))
+    near(decay_attention(q=q, k=k, v=v, log_decay=g), want, torch.float16)
+    out, s = incremental_decay_attention(q=q, k=k, v=v, log_decay=g)
+    near(out, want, torch.float16)
+    near(s, last, torch.float32, 8.0)
+
+
+def test_decay_scores_that_fit_without_their_scale():
+    """fp16, scores of 100 and a scale of 1e4: what counts is the product with the values."""
+    from rfa_b200.decay_attention import decay_attention
+    torch.manual_seed(4)
+    q, k = (torch.randn(150, 2, 2, 64, device="cuda").half() for _ in range(2))
+    v = (1e-3 * torch.randn(150, 2, 2, 64, device="cuda")).half()
+    g = torch.full((150, 2, 2), -0.1, device="cuda")
+    for scale in (1e4, -1e4, 0.0, -0.25):
+        near(decay_attention(q=q, k=k, v=v, log_decay=g, scale=scale), decay_dense(*(x.double() for x in (q, k, v, g)), scale=scale)[0], torch.float16)
