@@ -38,6 +38,12 @@ struct WindowNumbers {
       : order(a.order ? a.order + b * a.S : nullptr), pos(a.pos ? a.pos + b * (a.S + 1) : nullptr), S(a.S), window(a.window), sinks(a.sinks) {}
   // the number at a place, negative where there is none
   __device__ __forceinline__ int at(int64_t s) const { return s < 0 || s >= S ? -1 : order ? order[s] : (int)s; }
+  // of a key in a tile in front of all windows (`front`): there only first tokens count, and the rows beside them are cleared like those of padding -- a weight of nothing
+  // times what is not finite is not nothing
+  __device__ __forceinline__ int key_of_tile(int64_t s, bool front) const {
+    const int n = at(s);
+    return front && n >= sinks ? -1 : n;
+  }
   __device__ __forceinline__ int64_t real_before(int64_t s) const { const int n = at(s); return n < 0 ? ~n : n; }      // 0 <= s < S
   __device__ __forceinline__ int64_t place(int64_t n) const { return n < 0 ? 0 : n >= S ? S : pos ? pos[n] : n; }
   __device__ __forceinline__ int64_t real_to(int64_t s) const { const int n = at(s); return n < 0 ? ~n : n + 1; }           // up to s, 0 <= s < S

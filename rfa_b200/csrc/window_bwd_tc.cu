@@ -7,7 +7,7 @@
 //     gq += dS X1 (X1 = k);   KEYS: gv += P X2 (X2 = g), gk += dS X1 (X1 = q), over all query heads that share the key head
 // Scores and their gradients have three places (two where the sums leave no room for a third) and as many groups of warps, which take the tiles in turn, a thread to
 // each row.  delta = sum of g o out comes from a
-// kernel of its own.  Tiles that are seen whole need no mask.  Padded places: as in window_tc.cu, warp 3 fetches numbers (and, KEYS, lse and delta of the queries)
+// kernel of its own.  Tiles that are seen whole need no mask.  Padded places and, beside the queries, keys beside first tokens: as in window_tc.cu, warp 3 fetches numbers (and, KEYS, lse and delta of the queries)
 // and clears the rows that are summed over.  First tokens' keys: works behind the tiles' take parts of their queries (SPLIT; window.cuh), whose sums stay in 32 bits for
 // window_parts_kernel.
 //
@@ -43,7 +43,7 @@ static_assert(bCount * 8 + 4 <= 256, "barriers");
 template <typename T, int DB, bool KEYS, bool ORDERED, bool SPLIT>
 __global__ void __launch_bounds__(WbLayout<DB, KEYS>::kThreads, 1)
 window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_constant__ CUtensorMap tm_r2, const __grid_constant__ CUtensorMap tm_x1,
-                     const __grid_constant__ CUtensorMap tm_x2, const __grid_constant__ WindowArgs a, int works) {
+                     const __grid_constant__ CUtensorMap tm_x2, const __grid_constant__ CUtensorMap tm_first, const __grid_constant__ WindowArgs a, int works) {
   using Lay = WbLayout<DB, KEYS>;
   constexpr int DP = DB * 64, kStages = Lay::kStages, kGroups = Lay::kGroups;
   constexpr bool kColumns = KEYS || ORDERED;
@@ -126,7 +126,8 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
             const int st = n % kStages;
             if (n >= kStages && !mbar_wait(&bars[bEmpty + st], (n / kStages + 1) & 1)) { tc_fail(2); ok = false; break; }
             mbar_arrive_expect_tx(&bars[bFull + st], 2 * DB * Lay::kHalf);
-            for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::x1 + (st * DB + x) * Lay::kHalf, &tm_x1, &bars[bFull + st], x * 64, h, k.b, t * kWbTile);
+            const CUtensorMap* summed = !KEYS && !ORDERED && t < k.span.first ? &tm_first : &tm_x1;
+            for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::x1 + (st * DB + x) * Lay::kHalf, summed, &bars[bFull + st], x * 64, h, k.b, t * kWbTile);
             for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::x2 + (st * DB + x) * Lay::kHalf, &tm_x2, &bars[bFull + st], x * 64, h, k.b, t * kWbTile);
           }
       }
@@ -193,7 +194,7 @@ window_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_r1, const __grid_con
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int64_t i = (int64_t)t * kWbTile + e * 32 + lane;
-              if (ORDERED) number[e] = num.at(i);
+              if (ORDERED) number[e] = num.key_of_tile(i, !KEYS && t < k.span.first);
               if (KEYS && i < a.T) {
                 lse[e] = kLog2e * a.lse[((int64_t)k.b * a.H + h) * a.T + i];
                 delta[e] = a.delta[((int64_t)k.b * a.H + h) * a.T + i];
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const T* __restrict__
 namespace {
 
 template <typename T, int DB, bool KEYS, bool ORDERED, bool SPLIT = false>
-int launch(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& x1, const CUtensorMap& x2, const WindowArgs& a, cudaStream_t stream) {
+int launch(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& x1, const CUtensorMap& x2, const CUtensorMap& first, const WindowArgs& a, cudaStream_t stream) {
   using Lay = WbLayout<DB, KEYS>;
   constexpr uint32_t smem = Lay::bytes;
   cudaError_t e = cudaFuncSetAttribute(window_bwd_tc_kernel<T, DB, KEYS, ORDERED, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -402,14 +403,14 @@ int launch(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& x1, 
   int64_t works = (a.T + 127) / 128 * a.B * (KEYS ? a.G : a.H);
   if (SPLIT) works += ((std::min<int64_t>(a.sinks, a.T) + 127) / 128 + (a.order ? 1 : 0)) * (a.splits - 1) * a.B * a.G;
   RFA_REQUIRE(works < (int64_t)1 << 31, RFA_EUNSUPPORTED, "window_bwd: %lld tiles", (long long)works);
-  e = launch_pdl(window_bwd_tc_kernel<T, DB, KEYS, ORDERED, SPLIT>, dim3((unsigned)std::min<int64_t>(works, 148)), dim3(Lay::kThreads), smem, stream, r1, r2, x1, x2, a, (int)works);
+  e = launch_pdl(window_bwd_tc_kernel<T, DB, KEYS, ORDERED, SPLIT>, dim3((unsigned)std::min<int64_t>(works, 148)), dim3(Lay::kThreads), smem, stream, r1, r2, x1, x2, first, a, (int)works);
   if (e != cudaSuccess) return fail((int)e, "rfa_window_bwd: launch failed: %s", cudaGetErrorString(e));
   return check_launch("rfa_window_bwd");
 }
 template <typename T, int DB, bool KEYS>
-int launch_order(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& x1, const CUtensorMap& x2, const WindowArgs& a, cudaStream_t stream) {
-  if (KEYS && a.splits > 1) return a.order ? launch<T, DB, KEYS, true, KEYS>(r1, r2, x1, x2, a, stream) : launch<T, DB, KEYS, false, KEYS>(r1, r2, x1, x2, a, stream);
-  return a.order ? launch<T, DB, KEYS, true>(r1, r2, x1, x2, a, stream) : launch<T, DB, KEYS, false>(r1, r2, x1, x2, a, stream);
+int launch_order(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& x1, const CUtensorMap& x2, const CUtensorMap& first, const WindowArgs& a, cudaStream_t stream) {
+  if (KEYS && a.splits > 1) return a.order ? launch<T, DB, KEYS, true, KEYS>(r1, r2, x1, x2, first, a, stream) : launch<T, DB, KEYS, false, KEYS>(r1, r2, x1, x2, first, a, stream);
+  return a.order ? launch<T, DB, KEYS, true>(r1, r2, x1, x2, first, a, stream) : launch<T, DB, KEYS, false>(r1, r2, x1, x2, first, a, stream);
 }
 template <typename T>
 int launch_delta(const WindowArgs& a, const uint8_t* mask, cudaStream_t stream) {
@@ -420,14 +421,14 @@ int launch_delta(const WindowArgs& a, const uint8_t* mask, cudaStream_t stream) 
   return check_launch("rfa_window_bwd (delta)");
 }
 template <typename T>
-int launch_type(const CUtensorMap (&m)[8], const WindowArgs& a, const uint8_t* mask, cudaStream_t stream) {
+int launch_type(const CUtensorMap (&m)[9], const WindowArgs& a, const uint8_t* mask, cudaStream_t stream) {
   if (int r = launch_delta<T>(a, mask, stream)) return r;
   if (a.D <= 64) {
-    if (int r = launch_order<T, 1, false>(m[0], m[1], m[6], m[7], a, stream)) return r;
-    if (int r = launch_order<T, 1, true>(m[2], m[3], m[4], m[5], a, stream)) return r;
+    if (int r = launch_order<T, 1, false>(m[0], m[1], m[6], m[7], m[8], a, stream)) return r;
+    if (int r = launch_order<T, 1, true>(m[2], m[3], m[4], m[5], m[4], a, stream)) return r;
   } else {
-    if (int r = launch_order<T, 2, false>(m[0], m[1], m[6], m[7], a, stream)) return r;
-    if (int r = launch_order<T, 2, true>(m[2], m[3], m[4], m[5], a, stream)) return r;
+    if (int r = launch_order<T, 2, false>(m[0], m[1], m[6], m[7], m[8], a, stream)) return r;
+    if (int r = launch_order<T, 2, true>(m[2], m[3], m[4], m[5], m[4], a, stream)) return r;
   }
   return a.splits > 1 ? launch_window_parts(a, 128, a.scale, stream) : 0;
 }
@@ -437,13 +438,14 @@ int launch_type(const CUtensorMap (&m)[8], const WindowArgs& a, const uint8_t* m
 int launch_window_bwd_tc(const WindowArgs& a, const uint8_t* mask, cudaStream_t stream) {
   const bool bf16 = a.dtype == RFA_BF16;
   // as resident rows: q, g, k, v; streamed: q, g, k, v
-  CUtensorMap m[8];
+  CUtensorMap m[9];      // and the keys' first tokens, streamed
   const WindowRows* x[4] = {&a.q, &a.g, &a.k, &a.v};
   for (int i = 0; i < 8; ++i) {
     const WindowRows& r = *x[i & 3];
     if (make_tmap_heads(&m[i], r.p, bf16, a.T, a.B, (i & 3) < 2 ? a.H : a.G, a.D, r.t, r.b, r.h, i < 4 ? 128 : kWbTile))
       return fail(RFA_EDEVICE, "window_bwd: cuTensorMapEncodeTiled failed or is unavailable");
   }
+  if (make_tmap_first(&m[8], m[6], a, a.k)) return fail(RFA_EDEVICE, "window_bwd: cuTensorMapEncodeTiled failed or is unavailable");
   return bf16 ? launch_type<__nv_bfloat16>(m, a, mask, stream) : launch_type<__half>(m, a, mask, stream);
 }
 

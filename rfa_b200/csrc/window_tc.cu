@@ -9,8 +9,11 @@
 // exponentials of this one: with tiles of 128 keys and one place a unit's chain of products, maxima, exponentials and products again took 4500 cycles, of which the
 // special function unit worked 2048 (16 exponentials a cycle and SM, two units).
 //
+// Tiles in front of all windows are seen for their first tokens only.  Their values come by a tensor map that ends behind these, so that the rows beside them are
+// zero: a weight of nothing times what is not finite is not nothing, and such a tile is seen by every query.
+//
 // With padded tokens or a cache in front (ORDERED) places are not numbers: warp 3 fetches the numbers of a tile's keys and clears the values of places that hold
-// no token, whatever stands there.
+// no token, whatever stands there, and those beside first tokens.
 //
 // Warp roles (384 threads): warp 0 TMA producer, warps 1 and 2 one MMA issuer for each unit, warps 4..7 and 8..11 one softmax group for each unit.  All waits are
 // bounded.  Window 256 + 4 of 8 x 16 (4) heads x 2048 x 64, bf16: 77 us; 1024 + 4 of 16 (4) x 32768 x 128: 365 to 400 us (690 TFLOP/s of what is seen).
@@ -39,7 +42,7 @@ static_assert(wCount * 8 + 4 <= 288, "barriers");
 template <typename T, int DB, bool ORDERED>
 __global__ void __launch_bounds__(kWinThreads, 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                 const __grid_constant__ WindowArgs a, bool pair_heads, int works) {
+                 const __grid_constant__ CUtensorMap tm_first, const __grid_constant__ WindowArgs a, bool pair_heads, int works) {
   using Lay = WinLayout<DB>;
   constexpr int DP = DB * 64, kStages = Lay::kStages;
   extern __shared__ __align__(1024) unsigned char sm[];
@@ -106,7 +109,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           mbar_arrive_expect_tx(&bars[wFullK + st], DB * Lay::kHalf);
           for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::k + (st * DB + x) * Lay::kHalf, &tm_k, &bars[wFullK + st], x * 64, k.kv, k.b, kt * kWinTile);
           mbar_arrive_expect_tx(&bars[wFullV + st], DB * Lay::kHalf);
-          for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + (st * DB + x) * Lay::kHalf, &tm_v, &bars[wFullV + st], x * 64, k.kv, k.b, kt * kWinTile);
+          const CUtensorMap* values = !ORDERED && kt < k.both.first ? &tm_first : &tm_v;
+          for (int x = 0; x < DB; ++x) tma_load_4d(sm + Lay::v + (st * DB + x) * Lay::kHalf, values, &bars[wFullV + st], x * 64, k.kv, k.b, kt * kWinTile);
         }
       }
     }
@@ -309,7 +313,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         const int st = n % kStages;
         int number[2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) number[e] = num.at((int64_t)kt * kWinTile + e * 32 + lane);
+        for (int e = 0; e < 2; ++e) number[e] = num.key_of_tile((int64_t)kt * kWinTile + e * 32 + lane, kt < k.both.first);
         // the stage has been filled again, so that nobody reads its old numbers
         if (!mbar_wait(&bars[wFullV + st], (n / kStages) & 1)) { tc_fail(12); ok = false; break; }
 #pragma unroll
@@ -335,20 +339,20 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 namespace {
 
 template <typename T, int DB, bool ORDERED>
-int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const WindowArgs& a, cudaStream_t stream) {
+int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& first, const WindowArgs& a, cudaStream_t stream) {
   using Lay = WinLayout<DB>;
   cudaError_t e = cudaFuncSetAttribute(window_tc_kernel<T, DB, ORDERED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Lay::bytes);
   if (e != cudaSuccess) return fail((int)e, "window_fwd: cannot reserve %u bytes of shared memory: %s", Lay::bytes, cudaGetErrorString(e));
   const bool pair_heads = a.H / a.G % 2 == 0;
   const int64_t runs = (a.T + 127) / 128, ctas = pair_heads ? runs * a.B * (a.H / 2) : (runs + 1) / 2 * a.B * a.H;
   RFA_REQUIRE(ctas < (int64_t)1 << 31, RFA_EUNSUPPORTED, "window_fwd: %lld tiles", (long long)ctas);
-  e = launch_pdl(window_tc_kernel<T, DB, ORDERED>, dim3((unsigned)std::min<int64_t>(ctas, 148)), dim3(kWinThreads), Lay::bytes, stream, q, k, v, a, pair_heads, (int)ctas);
+  e = launch_pdl(window_tc_kernel<T, DB, ORDERED>, dim3((unsigned)std::min<int64_t>(ctas, 148)), dim3(kWinThreads), Lay::bytes, stream, q, k, v, first, a, pair_heads, (int)ctas);
   if (e != cudaSuccess) return fail((int)e, "rfa_window_fwd: launch failed: %s", cudaGetErrorString(e));
   return check_launch("rfa_window_fwd");
 }
 template <typename T, int DB>
-int launch_order(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const WindowArgs& a, cudaStream_t stream) {
-  return a.order ? launch<T, DB, true>(q, k, v, a, stream) : launch<T, DB, false>(q, k, v, a, stream);
+int launch_order(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& first, const WindowArgs& a, cudaStream_t stream) {
+  return a.order ? launch<T, DB, true>(q, k, v, first, a, stream) : launch<T, DB, false>(q, k, v, first, a, stream);
 }
 
 }  // namespace
@@ -361,12 +365,13 @@ bool window_tc_ok(const WindowArgs& a) {
 
 int launch_window_fwd_tc(const WindowArgs& a, cudaStream_t stream) {
   const bool bf16 = a.dtype == RFA_BF16;
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, first;
   if (make_tmap_heads(&q, a.q.p, bf16, a.T, a.B, a.H, a.D, a.q.t, a.q.b, a.q.h, 128) || make_tmap_heads(&k, a.k.p, bf16, a.S, a.B, a.G, a.D, a.k.t, a.k.b, a.k.h, kWinTile) ||
       make_tmap_heads(&v, a.v.p, bf16, a.S, a.B, a.G, a.D, a.v.t, a.v.b, a.v.h, kWinTile))
     return fail(RFA_EDEVICE, "window_fwd: cuTensorMapEncodeTiled failed or is unavailable");
-  if (bf16) return a.D <= 64 ? launch_order<__nv_bfloat16, 1>(q, k, v, a, stream) : launch_order<__nv_bfloat16, 2>(q, k, v, a, stream);
-  return a.D <= 64 ? launch_order<__half, 1>(q, k, v, a, stream) : launch_order<__half, 2>(q, k, v, a, stream);
+  if (make_tmap_first(&first, v, a, a.v)) return fail(RFA_EDEVICE, "window_fwd: cuTensorMapEncodeTiled failed or is unavailable");
+  if (bf16) return a.D <= 64 ? launch_order<__nv_bfloat16, 1>(q, k, v, first, a, stream) : launch_order<__nv_bfloat16, 2>(q, k, v, first, a, stream);
+  return a.D <= 64 ? launch_order<__half, 1>(q, k, v, first, a, stream) : launch_order<__half, 2>(q, k, v, first, a, stream);
 }
 
 RFA_TC_UNIT(window)

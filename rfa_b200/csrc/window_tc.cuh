@@ -6,6 +6,13 @@
 
 namespace rfa {
 
+// Of keys or values as tiles of 64: the map that ends behind the first tokens, where tiles may lie in front of all windows and places are numbers; else the map of all.
+inline int make_tmap_first(CUtensorMap* m, const CUtensorMap& all, const WindowArgs& a, const WindowRows& x) {
+  *m = all;
+  if (a.order || a.sinks <= 0 || a.sinks >= a.S || a.S <= a.window) return 0;
+  return make_tmap_heads(m, x.p, a.dtype == RFA_BF16, a.sinks, a.B, a.G, a.D, x.t, x.b, x.h, 64);
+}
+
 #ifdef __CUDACC__
 // The tiles of kTile keys that queries see: those of the first tokens, then from `first` on.
 struct WindowSpan {

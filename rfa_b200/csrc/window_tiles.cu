@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1) window_fwd_kernel(c
   for (int i = 0; i < 4; ++i) { top[i] = -INFINITY; sum[i] = 0.f; }
   for (int64_t kt = sink_tiles > 0 ? num.front() / kOther : first; kt < end; kt = kt + 1 < sink_tiles ? kt + 1 : max(kt + 1, first)) {
     __syncthreads();
-    if (tid < kOther) nk[tid] = num.at(kt * kOther + tid);
+    if (tid < kOther) nk[tid] = num.key_of_tile(kt * kOther + tid, kt < first);
     __syncthreads();
     load_tile<T, kOther>(K, ld, a.k, b, kv, kt * kOther, a.S, D, nk);
     load_tile<T, kOther>(V, ld, a.v, b, kv, kt * kOther, a.S, D, nk);
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, NC <= 2 ? 2 : 1) window_gq_kernel(co
   float acc[4][NC][4] = {};
   for (int64_t kt = sink_tiles > 0 ? num.front() / kOther : first; kt < end; kt = kt + 1 < sink_tiles ? kt + 1 : max(kt + 1, first)) {
     __syncthreads();
-    if (tid < kOther) nk[tid] = num.at(kt * kOther + tid);
+    if (tid < kOther) nk[tid] = num.key_of_tile(kt * kOther + tid, kt < first);
     __syncthreads();
     load_tile<T, kOther>(K, ld, a.k, b, kv, kt * kOther, a.S, D, nk);
     load_tile<T, kOther>(V, ld, a.v, b, kv, kt * kOther, a.S, D, nk);

@@ -11,7 +11,8 @@ backward pass is not differentiable itself.  No upstream counterpart.
 
 ``key_padding_mask`` ``[bsz, tgt_len]`` (1 = padding): padded tokens are skipped, wherever they stand, and not counted in distances --
 every result is what it would be without them, whatever values they hold, and their own outputs and gradients are zero.  A real
-token that is not finite may reach the outputs of any token less than 128 places from it."""
+token that is not finite reaches the tokens that see it, and may reach the outputs and the gradients of q of tokens less than 320 from one of these.  The
+gradients of k and v gather from the tokens that see a key, and may from ones as near to these; of keys less than 128 places from a first token, from any."""
 from typing import Dict, Optional, Tuple
 
 import math

@@ -5,7 +5,7 @@ import math
 
 import pytest
 import torch
-from test_gpu_attention import TYPES, decay_dense, make, near, places, some_mask
+from test_gpu_attention import TYPES, decay_dense, grads, make, near, places, some_mask, window_dense
 
 pytestmark = pytest.mark.gpu
 
@@ -93,6 +93,72 @@ def test_window_scores_far_below_zero(dtype, D, pad):
         state = dict(zip(("prev_k", "prev_v", "prev_len"), new))
         outs.append(o)
     near(torch.cat(outs), want, dt)
+
+
+@pytest.mark.parametrize("dtype,D,pad,window,sinks,at", [("fp32", 24, None, 64, 4, 40), ("fp16", 64, None, 64, 4, 40), ("bf16", 128, None, 64, 4, 40), ("fp16", 64, "left", 64, 4, 90),
+                                                         ("bf16", 128, "gap", 50, 70, 100), ("bf16", 200, None, 64, 4, 20), ("fp16", 64, None, 2, 0, 832), ("fp16", 64, None, 300, 130, 140),
+                                                         ("fp32", 24, "right", 2, 1, 9), ("bf16", 100, None, 30, 1, 2)])
+def test_window_reach_of_what_is_not_finite(dtype, D, pad, window, sinks, at):
+    """Outputs and queries' gradients 320 tokens and more from the last that sees a token, and the same in front of it, are what they are without it -- behind first tokens
+    that lie beside it, too."""
+    from rfa_b200.window_attention import incremental_window_attention, window_attention
+    torch.manual_seed(D)
+    T, B, H, G, dt = 1500, 2, 4, 2, TYPES[dtype]
+    q, k, v = make(T, B, (H, G, G), (D, D, D), dt, False)
+    mask = some_mask(pad, B, T)
+    n, real = places(mask, T, B)
+    place = ((n[1] == at) & real[1]).nonzero()[0, 0]
+    assert at >= sinks
+    k[place, 1] = v[place, 1] = 0.0
+    go = torch.randn_like(q)
+    (want,), gw = grads(lambda *a: window_dense(*a, window, sinks, mask), (q, k, v), [go])
+    beyond = real[1] & ((n[1] >= at + window - 1 + 320) | (n[1] <= at - 320))
+    spared = ~sees(mask, T, B, window, sinks)[1, :, place] & beyond
+    assert spared.any()
+    k[place, 1], v[place, 1] = math.nan, math.inf
+    kw = dict(window=window, sinks=sinks, key_padding_mask=mask)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = window_attention(q=leaves[0], k=leaves[1], v=leaves[2], **kw)
+    gq, = torch.autograd.grad(out, leaves[0], go)
+    with torch.no_grad():
+        later = incremental_window_attention(q=q, k=k, v=v, **kw)[0]
+        first = incremental_window_attention(q=q[:600], k=k[:600], v=v[:600], **{**kw, "key_padding_mask": None if mask is None else mask[:, :600]})
+        then = incremental_window_attention(q=q[600:], k=k[600:], v=v[600:], prev_k=first[1], prev_v=first[2], prev_len=first[3],
+                                            **{**kw, "key_padding_mask": None if mask is None else mask[:, 600:]})[0]
+    delta = D ** -0.5 * (go.double() * want).sum(-1)
+    for x in (out, later, torch.cat([first[0], then])):
+        near(x[spared, 1], want[spared, 1], dt)
+        near(x[:, 0], want[:, 0], dt)
+    near(gq[spared, 1], gw[0][spared, 1], dt, 4.0, terms=delta[spared, 1])
+    near(gq[:, 0], gw[0][:, 0], dt, 4.0, terms=delta[:, 0])
+
+
+@pytest.mark.parametrize("dtype,D,G,pad,window,sinks", [("fp32", 24, 2, None, 64, 4), ("fp16", 64, 2, None, 64, 4), ("bf16", 128, 2, "right", 50, 4), ("bf16", 64, 1, None, 30, 70), ("fp16", 64, 2, None, 40, 0)])
+def test_window_reach_of_gradients_that_are_not_finite(dtype, D, G, pad, window, sinks):
+    from rfa_b200.window_attention import window_attention
+    torch.manual_seed(D)
+    T, B, H, dt = 1500, 2, 4, TYPES[dtype]
+    q, k, v = make(T, B, (H, G, G), (D, D, D), dt, False)
+    mask, at = some_mask(pad, B, T), 700
+    n, real = places(mask, T, B)
+    go = torch.randn_like(q)
+    go[at, 1] = 0.0
+    (want,), gw = grads(lambda *a: window_dense(*a, window, sinks, mask), (q, k, v), [go])
+    go[at, 1] = math.nan
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    gq, gk, gv = torch.autograd.grad(window_attention(q=leaves[0], k=leaves[1], v=leaves[2], window=window, sinks=sinks, key_padding_mask=mask), leaves, go)
+    delta = D ** -0.5 * (go.nan_to_num().double() * want).sum(-1)
+    others = torch.arange(T, device="cuda") != at
+    near(gq[others, 1], gw[0][others, 1], dt, 4.0, terms=delta[others, 1])
+    assert not torch.isfinite(gq[at, 1]).any()
+    seen = sees(mask, T, B, window, sinks)[1, at]
+    assert not torch.isfinite(gk[seen, 1]).any() and not torch.isfinite(gv[seen, 1]).any()
+    spared = real[1] & ((n[1] >= at + 320) | (n[1] <= at - (window - 1) - 320)) & (n[1] >= (sinks + 128 if sinks else 0))
+    assert spared.sum() > 300
+    near(gk[spared, 1], gw[1][spared, 1], dt, 4.0, terms=delta[spared, 1])
+    near(gv[spared, 1], gw[2][spared, 1], dt, 4.0)
+    for x, w in ((gk, gw[1]), (gv, gw[2])):
+        near(x[:, 0], w[:, 0], dt, 4.0, terms=delta[:, 0] if w is gw[1] else None)
 
 
 # ------------------------------------------------------------------------------------------------ decay
