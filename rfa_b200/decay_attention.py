@@ -81,7 +81,7 @@ class DecayAttention(nn.Module):
     """A causal layer of the same call as ``CausalAttention``'s, without random matrices: projections to q, k, v and a gate, attention
     with a decay, group norm of each head gated by silu(gate), output projection.
 
-    ``decay`` "head": a factor of ``1 - 2 ** (-5 - 8 h / num_heads)`` for head h, a buffer.  "token": one for each token and head,
+    ``decay`` "head": a factor of ``1 - 2 ** (-5 - 8 h / num_heads)`` for head h, a buffer that stays fp32 whatever type the layer gets.  "token": one for each token and head,
     ``sigmoid(x W + b) ** (1 / 16)``, learned."""
 
     def __init__(self, *, embed_dim: int, num_heads: int, key_dim: Optional[int] = None, head_dim: Optional[int] = None, decay: str = "token"):
@@ -101,6 +101,15 @@ class DecayAttention(nn.Module):
         else:
             self.register_buffer("log_decay", torch.log1p(-torch.exp2(-5.0 - 8.0 * torch.arange(num_heads, dtype=torch.float32) / num_heads)))
         self.reset_parameters()
+
+    def _apply(self, fn, *args, **kwargs):
+        # The fixed decays stay in fp32 when the parameters become 16 bits: 0.4 % of a rate (bf16) would add up along a sequence.
+        fixed = self._buffers.get("log_decay")
+        super()._apply(fn, *args, **kwargs)
+        moved = self._buffers.get("log_decay")
+        if moved is not None and moved.dtype != fixed.dtype:
+            self._buffers["log_decay"] = fixed.to(moved.device)
+        return self
 
     def reset_parameters(self):
         for lin in (self.in_proj, self.out_proj):

@@ -102,3 +102,26 @@ def test_layers_refuse_what_the_operators_would():
     state = dict(prev_k=torch.arange(3.).view(3, 1, 1, 1), prev_len=torch.tensor([4, 5, 6]))
     layer.reorder_incremental_state(state, torch.tensor([2, 0, 0]))
     assert state["prev_len"].tolist() == [6, 4, 4] and state["prev_k"].flatten().tolist() == [2.0, 0.0, 0.0]
+
+
+def test_fixed_decays_stay_fp32():
+    """Of a layer that becomes 16 bits, is copied, moved, or loaded."""
+    import copy
+    from rfa_b200 import DecayAttention
+    layer = DecayAttention(embed_dim=64, num_heads=4, decay="head")
+    want = torch.log1p(-torch.exp2(-5.0 - 8.0 * torch.arange(4) / 4))
+    for f in (lambda m: m.half(), lambda m: m.bfloat16(), lambda m: copy.deepcopy(m).half(), lambda m: m.to(torch.device("cpu"), torch.float16), lambda m: m.double(),
+              lambda m: torch.nn.Sequential(m).bfloat16()[0], lambda m: m.float()):
+        other = f(layer)
+        assert other.log_decay.dtype == torch.float32 and torch.equal(other.log_decay, want)
+        assert "log_decay" in dict(other.named_buffers()) and torch.equal(other.state_dict()["log_decay"], want)
+    layer.half()
+    layer.log_decay.fill_(-0.3)                  # a value of the user's own
+    layer.bfloat16()
+    assert layer.in_proj.weight.dtype == torch.bfloat16 and torch.equal(layer.log_decay, torch.full((4,), -0.3))
+    fresh = DecayAttention(embed_dim=64, num_heads=4, decay="head").half()
+    fresh.load_state_dict(layer.state_dict())
+    assert torch.equal(fresh.log_decay, torch.full((4,), -0.3))
+    meta = DecayAttention(embed_dim=64, num_heads=4, decay="head").to("meta").half().to_empty(device="cpu")
+    assert meta.log_decay.dtype == torch.float32 and meta.in_proj.weight.dtype == torch.float16
+    DecayAttention(embed_dim=64, num_heads=4).half()
