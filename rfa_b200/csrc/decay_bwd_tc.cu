@@ -399,10 +399,24 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             if (i < quarter) g += ex_up[i];
           }
           const bool real = there && !(mask && mask[t]);
-          // the first token with nothing in front decays nothing: 0, not the rounding of sums that cancel.  Looked for in the first chunk only; behind 128
-          // padded places the rounding stays
-          bool first = a.from_zero && k.chunk == 0 && real;
-          for (int64_t before = t - 1; first && before >= 0; --before) first = mask && mask[before];
+          // The first token with nothing in front decays nothing: 0, not the rounding of sums that cancel.  It is a warp's first one, if padding or nothing is right in
+          // front of that and in all places before, which the warp looks at 128 at a time.
+          const bool edge = lane > 0 || t == 0 || (there && mask && mask[t - 1]);
+          const unsigned reals = __ballot_sync(0xffffffffu, real), edges = __ballot_sync(0xffffffffu, edge);
+          const int lead = __ffs(reals) - 1;
+          bool first = a.from_zero && reals && (lead > 0 || (edges & 1u));
+          if (first)
+            for (int64_t p = k.t0 + quarter * 32 + lead - 1 - lane; __any_sync(0xffffffffu, p >= 0); p -= 128) {
+              bool found = false;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (p - 32 * i >= 0) found |= !mask[p - 32 * i];
+              if (__any_sync(0xffffffffu, found)) {
+                first = false;
+                break;
+              }
+            }
+          first = first && lane == lead;
           if (!real || first) g = 0.f;
           if (!a.per_head) {
             if (there) {

@@ -241,3 +241,20 @@ def test_decay_scores_that_fit_without_their_scale():
     g = torch.full((150, 2, 2), -0.1, device="cuda")
     for scale in (1e4, -1e4, 0.0, -0.25):
         near(decay_attention(q=q, k=k, v=v, log_decay=g, scale=scale), decay_dense(*(x.double() for x in (q, k, v, g)), scale=scale)[0], torch.float16)
+
+
+@pytest.mark.parametrize("dtype,K", [("fp32", 16), ("fp16", 64), ("bf16", 128), ("bf16", 200)])
+def test_zero_gradient_of_a_first_token_behind_long_padding(dtype, K):
+    from rfa_b200.decay_attention import decay_attention
+    torch.manual_seed(K)
+    T, H, first = 900, 2, (0, 127, 128, 129, 300, 512, 898, 899)
+    B = len(first)
+    mask = torch.arange(T, device="cuda")[None] < torch.tensor(first, device="cuda")[:, None]
+    mask[4, 400:700] = True                                 # a gap behind the first token
+    mask[2, 200] = mask[2, 256] = True
+    q, k, v = make(T, B, (H, H, H), (K, K, K), TYPES[dtype], False)
+    g = (-0.1 * torch.rand(T, B, H, device="cuda")).to(TYPES[dtype]).requires_grad_()
+    out = decay_attention(q=q, k=k, v=v, log_decay=g, key_padding_mask=mask)
+    gg, = torch.autograd.grad(out, g, torch.randn_like(out))
+    for b, n in enumerate(first):
+        assert not gg[:n + 1, b].any() and gg[n + 1:, b][~mask[b, n + 1:]].any(-1).all(), b
