@@ -326,7 +326,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> window_attention_append(const Tensor&
     if (len.scalar_type() != at::kLong) raise(PyExc_TypeError, "window_attention: prev_len must be int64, got " + dtype_name(len));
     if (!ck.is_contiguous() || !cv.is_contiguous() || !len.is_contiguous())
       raise(PyExc_ValueError, "window_attention: prev_k, prev_v and prev_len must be contiguous (they are updated in place)");
-    if (ck.numel() && ck.data_ptr() == cv.data_ptr()) raise(PyExc_ValueError, "window_attention: prev_k and prev_v are the same memory");
+    const auto *k0 = static_cast<const char*>(ck.data_ptr()), *v0 = static_cast<const char*>(cv.data_ptr());
+    if (ck.numel() && k0 < v0 + cv.nbytes() && v0 < k0 + ck.nbytes()) raise(PyExc_ValueError, "window_attention: prev_k and prev_v share memory");
   } else {                                             // slots that no token reaches are zero, so that a copy of the cache is a number
     ck = at::zeros(shape, q.options().requires_grad(false));
     cv = at::zeros(shape, q.options().requires_grad(false));

@@ -161,6 +161,21 @@ def test_window_reach_of_gradients_that_are_not_finite(dtype, D, G, pad, window,
         near(x[:, 0], w[:, 0], dt, 4.0, terms=delta[:, 0] if w is gw[1] else None)
 
 
+def test_window_caches_that_overlap_are_refused():
+    from rfa_b200.window_attention import incremental_window_attention
+    room = torch.zeros(2 * 2 * 4 * 16 + 64, device="cuda").half()
+    q, n = torch.zeros(1, 2, 2, 16, device="cuda").half(), 2 * 2 * 4 * 16
+    length = torch.zeros(2, device="cuda", dtype=torch.long)
+    pk = room[:n].view(2, 2, 4, 16)
+    for off in (64, 16, 8):
+        for a, b in ((pk, room[off:off + n].view_as(pk)), (room[off:off + n].view_as(pk), pk)):
+            with pytest.raises(ValueError):
+                incremental_window_attention(q=q, k=q, v=q, window=4, prev_k=a, prev_v=b, prev_len=length)
+    both = torch.zeros(2 * n, device="cuda").half()      # side by side is fine
+    incremental_window_attention(q=q, k=q, v=q, window=4, prev_k=both[:n].view_as(pk), prev_v=both[n:].view_as(pk), prev_len=length)
+    assert length.tolist() == [1, 1]
+
+
 # ------------------------------------------------------------------------------------------------ decay
 @pytest.mark.parametrize("value", [math.nan, math.inf, 1e30])
 @pytest.mark.parametrize("at", [0, 150])
