@@ -273,3 +273,38 @@ def test_zero_gradient_of_a_first_token_behind_long_padding(dtype, K):
     gg, = torch.autograd.grad(out, g, torch.randn_like(out))
     for b, n in enumerate(first):
         assert not gg[:n + 1, b].any() and gg[n + 1:, b][~mask[b, n + 1:]].any(-1).all(), b
+
+
+def test_decay_backward_on_states_of_its_own_has_the_same_bits():
+    """Behind a forward that returned no state, what it kept and what the backward computes for itself are the same."""
+    from rfa_b200 import ops
+    torch.manual_seed(23)
+    for dt, K, D, T in ((torch.float16, 64, 64, 400), (torch.bfloat16, 128, 128, 400), (torch.bfloat16, 64, 128, 5000)):
+        q, k, v = make(T, 2, (2, 2, 2), (K, K, D), dt, False)
+        g, go = (-0.1 * torch.rand(T, 2, 2, device="cuda")).to(dt), torch.randn_like(v)
+        kept = ops.decay_attention_fwd(q, k, v, g, save=True)[2]
+        assert kept is not None
+        for a, b in zip(ops.decay_attention_bwd(q, k, v, g, None, None, None, go, kept=kept)[:4], ops.decay_attention_bwd(q, k, v, g, None, None, None, go)[:4]):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype,K", [("fp32", 24), ("fp16", 64), ("bf16", 128), ("fp16", 33), ("bf16", 200)])
+def test_decay_reach_of_what_is_not_finite(dtype, K):
+    """A token that is not finite reaches all outputs behind it, in its row and head, and none 128 places and more in front."""
+    from rfa_b200.decay_attention import decay_attention, incremental_decay_attention
+    torch.manual_seed(K)
+    T, dt, at = 500, TYPES[dtype], 300
+    q, k, v = make(T, 2, (2, 2, 2), (K, K, K), dt, False)
+    g = -0.01 * torch.rand(T, 2, 2, device="cuda")
+    clean = decay_attention(q=q, k=k, v=v, log_decay=g)
+    for i, value in ((0, math.nan), (1, math.nan), (1, math.inf), (2, -math.inf)):
+        x = [y.clone() for y in (q, k, v)]
+        x[i][at, 1, 1, 2] = value
+        for out in (decay_attention(q=x[0], k=x[1], v=x[2], log_decay=g), incremental_decay_attention(q=x[0], k=x[1], v=x[2], log_decay=g)[0]):
+            near(out[:, 0], clean[:, 0].double(), dt)
+            near(out[:, 1, 0], clean[:, 1, 0].double(), dt)
+            near(out[:at - 127, 1, 1], clean[:at - 127, 1, 1].double(), dt)
+            behind = out[at:at + 1, 1, 1] if i == 0 else out[at:, 1, 1]
+            assert not torch.isfinite(behind).all(-1).any()
+            if i == 0:
+                near(out[at + 1:, 1, 1], clean[at + 1:, 1, 1].double(), dt)
