@@ -12,17 +12,21 @@
 // L_i - L_j is at most 0 in a model, so that nothing overflows whatever the decays are.  S is exact where it leaves the call (EXACT): K' goes in as two 16-bit
 // parts then (bf16's hold 16 bits: the products are off by 2^-17, the state by 3e-6 of its norm).  Where only outputs are wanted its first part is as
 // good as the 16-bit copies of S and P.  A log decay below -64 (in units of log 2) is taken as that.
+// L is summed in 64 bits and stored in 32: its rounding, 2^-24 |L|, is a weight's error.  That is 1e-6 for gates whose chunk fades by e^-10, and with resets, each worth
+// 64, 3e-6 apiece: up to what fp16 rounds a weight by (2^-11) where a chunk is nothing but resets, and between these no weight is left.  A pair of floats would
+// take one more instruction and read a score.
 //
 // Backwards (states alone), from the last chunk to the first: S = 2^(L_end) S + scale Q'^T G, Q'_i = 2^(L_i) q_i: the gradient of the state.  `kept`: the
 // 16-bit copy of the state in front of each chunk (behind it, backwards) goes to memory as it stands in shared memory, for decay_bwd_tc.cu.
 //
 // Warp roles (768 threads): warp 0 TMA producer; warps 1 and 18 MMA issuers (A: Q K^T, P V; B: Q S, the state: issuing one costs the issuing thread about 70
 // cycles, and a chunk has 20 to 40); warps 2..5 score group (A -> P); warps 6..9 and 20..23 state groups, half of the columns each (state -> 16-bit copy,
-// state times the next chunk's decay); warps 14..17 output group; warp 19 the decays (64-bit sums, because neighbours' are subtracted); warps 10..13 key group (states alone: with 2..5): K' in place of K once A is complete,
+// state times the next chunk's decay); warps 14..17 output group; warp 19 the decays (64-bit sums); warps 10..13 key group (states alone: with 2..5): K' in place of K once A is complete,
 // zeros over the rows of padded tokens.  Per chunk the serial chain is  state MMA -> copy and decay -> next state MMA.  All waits are bounded.
 //
-// 8 x 16 heads x 2048, bf16: 64 wide with an exact state 45 us (3.0 TB/s of what it cannot do without), 128 wide with states kept 62 us, states alone 36 us (5.6 TB/s).  From two tokens on it
-// is faster than the sweep for any sizes (decay_sweep.cu): 8 x 16 heads of 64, us, 2 tokens 6 / 11, 64 6 / 35, 1024 22 / 385.
+// 8 x 16 heads x 2048, bf16: 64 wide with an exact state 45 us (3.0 TB/s of what it cannot do without), 128 wide with states kept 62 us, states alone 36 us (5.6 TB/s).  It takes
+// every length: 8 x 16 heads of 64, here / the sweep for any sizes (decay_sweep.cu), us, 2 tokens 6 / 11, 64 6 / 35, 1024 22 / 385.  Many narrow heads of a few tokens would be faster
+// there (168 x 16 x 2 tokens x 8 x 32: 111 / 52), because a chunk takes its 6 us however little is in it.
 #pragma once
 
 #include "decay.cuh"

@@ -16,7 +16,7 @@
 // no token, whatever stands there, and those beside first tokens.
 //
 // Warp roles (384 threads): warp 0 TMA producer, warps 1 and 2 one MMA issuer for each unit, warps 4..7 and 8..11 one softmax group for each unit.  All waits are
-// bounded.  Window 256 + 4 of 8 x 16 (4) heads x 2048 x 64, bf16: 77 us; 1024 + 4 of 16 (4) x 32768 x 128: 365 to 400 us (690 TFLOP/s of what is seen).
+// bounded.  Window 256 + 4 of 8 x 16 (4) heads x 2048 x 64, bf16: 77 us; 1024 + 4 of 16 (4) x 32768 x 128: 386 to 395 us (690 TFLOP/s of what is seen).
 #define RFA_TC_FAMILY 12
 #include <algorithm>
 

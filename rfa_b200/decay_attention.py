@@ -6,15 +6,17 @@ of ``causal_attention.py`` and ``state_space.py``:
 * ``incremental_decay_attention`` -> the same from a state and with the last one returned, over any number of tokens
 
 Activations are time-major, ``[tgt_len, bsz, num_heads, width]``, fp16, bf16 or fp32, with any strides as long as a head's numbers are
-adjacent (views of a projection's output are taken as they are); sums and states are fp32.  Heads of at most 256.  The backward
+adjacent (views of a projection's output are taken as they are); sums and states are fp32 (a state that several bf16 tokens leave is made of keys in two
+parts of 8 bits and off by up to 3e-6 of its norm).  Heads of at most 256.  The backward
 passes are not differentiable themselves.  No upstream counterpart.
 
 ``key_padding_mask`` ``[bsz, tgt_len]`` (1 = padding): padded tokens are skipped, wherever they stand -- every result is what it
 would be without them, whatever values they hold, and their own outputs and gradients are zero.  A real token that is not finite may
-reach the outputs of any token less than 128 places from it, as it reaches all behind it.
+reach the outputs of any token less than 128 places from it, as it reaches all behind it; gradients likewise, those of the decays anywhere in its sequence.
 
-In fp16 and bf16 the outputs of several tokens come from 16-bit copies of the state (its own value is fp32): in fp16 a state beyond
-65504 gives outputs that are not finite."""
+In fp16 and bf16 the outputs of several tokens come from 16-bit copies of the state (its own value is fp32) and of the weights, scale times q . k times the decay
+between two tokens: in fp16 a state or a weight beyond 65504 gives outputs that are not finite.  A log decay below -44.36 (a factor of 2 ** -64) is taken as that
+there.  Gradients pass through 16-bit products: fp16 ones below about 1e-4 lose digits, 0.3 % at 1e-5, so that a small loss wants scaling."""
 from typing import Dict, Optional, Tuple
 
 import math

@@ -5,7 +5,8 @@ one size whatever the sequence's length.  Functional forms and the ``WindowAtten
 * ``incremental_window_attention`` -> the same behind the tokens that a cache holds, which it updates, over any number of tokens
 
 Activations are time-major, ``[tgt_len, bsz, num_heads, head_dim]``, fp16, bf16 or fp32, with any strides as long as a head's numbers are
-adjacent (views of a projection's output are taken as they are); scores, softmax and sums are fp32.  Heads of at most 256.  k and v may
+adjacent (views of a projection's output are taken as they are); scores, softmax and sums are fp32, in 16 bits the weights and their gradients are
+rounded for the products with values, keys and queries.  The backward makes the weights again from fp32 log-sums: scores of size m cost them m 2 ** -23.  Heads of at most 256.  k and v may
 have fewer heads than q: ``num_heads / num_kv_heads`` adjacent query heads share one, whose gradients are sums over them.  The
 backward pass is not differentiable itself.  No upstream counterpart.
 
