@@ -25,16 +25,16 @@ size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 // Workspace of a backward pass: the arrays of the largest sweep, then what the decays' gradient is made of.
 struct BwdPlan {
   SweepPlan sweeps;
-  size_t dots, last, sums;   // bytes; dots: each of two
+  size_t dots, front, sums;   // bytes; dots: each of two
   explicit BwdPlan(const rfa_decay_t& c) {
     const int64_t BH = (int64_t)c.B * c.H;
     sweeps = sweep_plan(c.T, BH, 2 * sweep_tiles(c.K) + sweep_tiles(c.D), 3, c.K, c.D);
-    dots = round256(sizeof(float) * sweep_tiles(c.K) * BH * c.T);
-    last = round256(sizeof(float) * BH * c.K * c.D);
+    dots = round256(2 * sizeof(float) * sweep_tiles(c.K) * BH * c.T);
+    front = round256(sizeof(float) * BH * c.K * c.D);
     sums = round256(sizeof(float) * BH);
   }
   size_t sweep() const { return round256(sweeps.totals) + round256(sweeps.seg_decay); }
-  size_t bytes() const { return sweep() + 2 * dots + last + sums; }
+  size_t bytes() const { return sweep() + 2 * dots + front + sums; }
 };
 size_t bwd_bytes(const rfa_decay_t& c) {
   const size_t tc = c.dtype != RFA_F32 && c.K <= 128 && c.D <= 128 && c.K % 8 == 0 && c.D % 8 == 0 ? decay_tc_bwd_bytes(c) : 0;
@@ -114,8 +114,8 @@ extern "C" int rfa_decay_bwd(const rfa_decay_t* c, const void* g, const float* g
   char *ws = static_cast<char*>(workspace), *rest = ws + plan.sweep();
   float* q_dots = reinterpret_cast<float*>(rest);
   float* k_dots = reinterpret_cast<float*>(rest + plan.dots);
-  float* last = reinterpret_cast<float*>(rest + 2 * plan.dots);
-  float* sums = reinterpret_cast<float*>(rest + 2 * plan.dots + plan.last);
+  float* front = reinterpret_cast<float*>(rest + 2 * plan.dots);
+  float* sums = reinterpret_cast<float*>(rest + 2 * plan.dots + plan.front);
   const DecayRows q{c->q, c->q_t, c->q_b, c->q_h}, k{c->k, c->k_t, c->k_b, c->k_h}, v{c->v, c->v_t, c->v_b, c->v_h};
   const DecayRows gr{g, (int64_t)c->B * c->H * c->D, (int64_t)c->H * c->D, c->D};
   float *s_in = const_cast<float*>(c->s_in), *g_last = const_cast<float*>(g_s);
@@ -137,13 +137,16 @@ extern "C" int rfa_decay_bwd(const rfa_decay_t* c, const void* g, const float* g
   if (g_decay) {
     a.x4 = q; a.dots = q_dots;
     ak.x4 = k; ak.dots = k_dots;
-    if (g_s) a.s_out = {last, 1, c->D};
+    if (g_s) {
+      a.s_out = {front, 1, c->D};
+      a.front_out = true;
+    }
   }
   if (int r = launch_sweeps(batch, plan.sweeps, st)) return r;
 
   if (!g_decay) return 0;
   const int tiles = sweep_tiles(c->K);
-  return launch_decay_grad(q_dots, tiles, k_dots, tiles, g_s, last, c->K * c->D, c->mask, g_decay, c->decay_dtype, c->per_head != 0, !c->s_in, sums, c->T, c->B, c->H, st);
+  return launch_decay_grad(q_dots, tiles, k_dots, tiles, g_s, front, c->K * c->D, c->mask, a.decay, g_decay, c->decay_dtype, c->per_head != 0, !c->s_in, sums, c->T, c->B, c->H, st);
 }
 
 extern "C" int rfa_decay_step(const rfa_decay_t* c, void* out, float* s, rfa_stream_t stream) {

@@ -24,12 +24,13 @@ struct DecayState {      // fp32 [B * H] of [x2's width][x3's width], strides in
 };
 struct SweepArgs {
   DecayRows x1, x2, x3;       // x1.p null: the state alone
-  DecayRows x4;               // null, or: dots[tile][b * H + h][t] = out_t . x4_t over a tile's columns
+  DecayRows x4;               // null, or: dots[tile][b * H + h][t] = (far, near), out_t . x4_t over a tile's columns, of the state and of the chunk's other tokens
   DecayRows decay;            // of decay_dtype, strides of 0 where it does not depend on the token or the batch row
   const uint8_t* mask;        // [B][T]
   void* out;                  // [T][B][H][width3], x1's type
   float* dots;
   DecayState s_in, s_out;     // p null: zeros, nowhere
+  bool front_out;             // s_out is the state without the last chunk's tokens, times that chunk's decay
   float* totals;              // segments: what each adds [segment][b * H + h][width2][width3], then the state in front of each
   double* seg_decay;          // [segment][b * H + h]
   int64_t T, tseg;
@@ -55,7 +56,7 @@ int sweep_tiles(int W);
 int launch_sweeps(SweepBatch batch, const SweepPlan& plan, cudaStream_t stream);
 // totals: what each segment adds -> the state in front of it; at most 65535 (row, head)s
 int launch_decay_combine(float* totals, const double* seg_decay, DecayState s_in, int nseg, int64_t BH, int A, int W, cudaStream_t stream);
-int launch_decay_grad(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_last, int KD, const uint8_t* mask,
+int launch_decay_grad(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_front, int KD, const uint8_t* mask, const DecayRows& decay,
                       void* g_decay, int decay_dtype, bool per_head, bool from_zero, float* sums, int64_t T, int B, int H, cudaStream_t stream);
 
 // decay_tc.cu: fp16 and bf16, heads of up to 128 in rows that a tensor map can describe

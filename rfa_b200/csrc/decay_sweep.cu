@@ -17,7 +17,7 @@ namespace {
 constexpr int kC = 32, kThreads = 256;
 constexpr int tile_of(int W) { return W <= 32 ? 32 : 64; }      // columns of x3 that a CTA takes
 size_t sweep_smem_bytes(int A, int DT) {
-  return sizeof(float) * ((size_t)2 * kC * (A + 1) + kC * DT + (size_t)A * DT + kC * (kC + 1) + 2 * kC) + sizeof(double) * kC;
+  return sizeof(float) * ((size_t)2 * kC * (A + 1) + kC * DT + (size_t)A * DT + kC * (kC + 1) + 3 * kC) + sizeof(double) * kC;
 }
 
 // kC rows of `width` numbers, `cols` of a row in shared memory, ld apart; rows from n on and padded ones are zero, whatever stands there.  A thread takes runs of 4 numbers of
@@ -56,7 +56,7 @@ __device__ __forceinline__ void decay_sweep(const SweepArgs& a, int tile, bool s
   double* L = sweep_smem;
   float* x1 = reinterpret_cast<float*>(L + kC);
   const int A = a.A, ld = A + 1, tid = threadIdx.x;
-  float *x2 = x1 + kC * ld, *x3 = x2 + kC * ld, *S = x3 + kC * DT, *P = S + (size_t)A * DT, *fa = P + kC * (kC + 1), *fb = fa + kC;
+  float *x2 = x1 + kC * ld, *x3 = x2 + kC * ld, *S = x3 + kC * DT, *P = S + (size_t)A * DT, *fa = P + kC * (kC + 1), *fb = fa + kC, *own = fb + kC;
   // x1, x2 rows are A + 1 apart (a bank more each); x3 and S rows are read 16 bytes at a time (kC * (A + 1) floats are a multiple of that)
   const int64_t bh = blockIdx.x;
   const int b = (int)(bh / a.H), h = (int)(bh % a.H), c0 = tile * DT, W = min(DT, a.W - c0), seg = blockIdx.z;
@@ -82,6 +82,7 @@ __device__ __forceinline__ void decay_sweep(const SweepArgs& a, int tile, bool s
       if (i0 + f * kThreads < A * DT) S[i0 + f * kThreads] = v[f];
   }
   const int col = (tid % kCols) * 4, rg = tid / kCols;
+  const bool dots = a.x4.p != nullptr;
   double run = 0.0;
   for (int k = 0; k < nchunk; ++k) {
     const int64_t t0 = t_begin + (int64_t)(a.rev ? nchunk - 1 - k : k) * kC;
@@ -102,7 +103,7 @@ __device__ __forceinline__ void decay_sweep(const SweepArgs& a, int tile, bool s
       L[tid] = g;
       const float in = expf((float)g), rest = expf((float)(end - g));
       fa[tid] = a.rev ? rest : in;
-      fb[tid] = a.in_scale * (a.rev ? in : rest);
+      fb[tid] = a.front_out && seg == a.nseg - 1 && k == nchunk - 1 ? 0.f : a.in_scale * (a.rev ? in : rest);
     }
     __syncthreads();
     run += L[kC - 1];
@@ -125,7 +126,12 @@ __device__ __forceinline__ void decay_sweep(const SweepArgs& a, int tile, bool s
           for (int j = 0; j < 2; ++j) {
             const int r = ty + 16 * i, c = tx + 16 * j;
             const float dot = i == j ? p[i][i] : p[1][0];      // that of rows behind 16 and columns before, or backwards the other one
-            P[r * (kC + 1) + c] = (a.rev ? c >= r : c <= r) ? dot * a.in_scale * expf((float)(a.rev ? L[c] - L[r] : L[r] - L[c])) : 0.f;
+            float w = (a.rev ? c >= r : c <= r) ? dot * a.in_scale * expf((float)(a.rev ? L[c] - L[r] : L[r] - L[c])) : 0.f;
+            if (dots && r == c) {      // a token with itself is in no sum of the dots
+              own[r] = w;
+              w = 0.f;
+            }
+            P[r * (kC + 1) + c] = w;
           }
       }
       __syncthreads();
@@ -144,36 +150,47 @@ __device__ __forceinline__ void decay_sweep(const SweepArgs& a, int tile, bool s
       for (int i = 0; i < kRows; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][e] *= fa[rg + i * kRowGroups];
+      float near[kRows][4];      // of the chunk's own tokens, apart from the state's where dots are wanted
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) near[i][e] = dots ? 0.f : acc[i][e];
 #pragma unroll 4
       for (int j = 0; j < kC; ++j) {
         const float4 s = *reinterpret_cast<const float4*>(x3 + j * DT + col);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
           const float p = P[(rg + i * kRowGroups) * (kC + 1) + j];
-          acc[i][0] = fmaf(p, s.x, acc[i][0]); acc[i][1] = fmaf(p, s.y, acc[i][1]);
-          acc[i][2] = fmaf(p, s.z, acc[i][2]); acc[i][3] = fmaf(p, s.w, acc[i][3]);
+          near[i][0] = fmaf(p, s.x, near[i][0]); near[i][1] = fmaf(p, s.y, near[i][1]);
+          near[i][2] = fmaf(p, s.z, near[i][2]); near[i][3] = fmaf(p, s.w, near[i][3]);
         }
       }
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         const int r = rg + i * kRowGroups;
         const int64_t t = t0 + r;
-        float dot = 0.f;
+        float far_dot = 0.f, near_dot = 0.f;
         if (r < n) {
           T* o = static_cast<T*>(a.out) + ((t * a.B + b) * a.H + h) * a.W + c0;
           const bool padded = gone && r < n && gone[r];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (col + e < W) {
-              const float v = a.out_scale * acc[i][e];
-              o[col + e] = from_f<T>(v);
-              if (a.x4.p && !padded) dot = fmaf(v, to_f<T>(static_cast<const T*>(a.x4.p)[b * a.x4.b + h * a.x4.h + t * a.x4.t + c0 + col + e]), dot);
+              o[col + e] = from_f<T>(a.out_scale * (dots ? acc[i][e] + fmaf(own[r], x3[r * DT + col + e], near[i][e]) : near[i][e]));
+              if (dots && !padded) {
+                const float y = a.out_scale * to_f<T>(static_cast<const T*>(a.x4.p)[b * a.x4.b + h * a.x4.h + t * a.x4.t + c0 + col + e]);
+                far_dot = fmaf(acc[i][e], y, far_dot);
+                near_dot = fmaf(near[i][e], y, near_dot);
+              }
             }
         }
-        if (a.x4.p) {
+        if (dots) {
 #pragma unroll
-          for (int s = kCols / 2; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-          if (col == 0 && r < n) a.dots[((int64_t)tile * BH + bh) * a.T + t] = dot;
+          for (int s = kCols / 2; s > 0; s >>= 1) {
+            far_dot += __shfl_xor_sync(0xffffffffu, far_dot, s);
+            near_dot += __shfl_xor_sync(0xffffffffu, near_dot, s);
+          }
+          if (col == 0 && r < n) reinterpret_cast<float2*>(a.dots)[((int64_t)tile * BH + bh) * a.T + t] = make_float2(far_dot, near_dot);
         }
       }
       __syncthreads();      // the state is read by all before it changes
@@ -252,9 +269,17 @@ __global__ void __launch_bounds__(256) decay_combine_kernel(float* totals, const
   }
 }
 
-// g_decay_t = sum over i >= t of (q_i . gq_i - k_i . gk_i) + g_s . s_last.  One CTA per (batch row, head), from the last token to the first; sums in 64 bits,
-// because near numbers are subtracted.  The sequence's first token decays nothing where no state is in front (`from_zero`): exactly 0, not the rounding that
-// the sum over all tokens leaves.
+// The gradient of the log decay at t is the sum over all pairs of a query i >= t and a key j < t (the end's gradient counts as a query behind all, a first state as a key in
+// front of all).  Of a query's and of a key's pairs the sweeps give two sums each, `far` over those outside its chunk and `near` over those with other tokens of
+// it: q_i . gq_i and k_j . gk_j without the token itself.  With across_c the pairs with a query behind the chunk c of t and a key in front of it,
+//     g_t = across_c + sum over i >= t in c of (far_q + near_q - near_k) + sum over j < t in c of far_k
+//     across_(c - 1) = across_c + sum over c of far_q - sum over c - 1 of far_k
+// from the last chunk to the first, where across is g_s . s_front (the state in front of the last chunk, times its decay).  What does not straddle t is left out wherever
+// it can be, rather than added and subtracted: a token with itself, pairs within other chunks, and where a chunk fades by e^-16 and more all that would cross it.
+// These are of the size of a gradient without decay, and what their roundings leave grows with the sequence while the rest shrinks with the decay: as one
+// difference of q_i . gq_i and k_j . gk_j over all tokens, 1000 tokens that fade by e^-3 each had 3e-3 of their gradient wrong.
+// One CTA per (batch row, head), a warp to a chunk; sums in 64 bits, because near numbers are subtracted.  The sequence's first token decays nothing where no state
+// is in front (`from_zero`): exactly 0, not the rounding that the sum over all tokens leaves.
 constexpr int kGradThreads = 512;
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
@@ -266,11 +291,12 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   __syncthreads();
   return s;
 }
-__global__ void __launch_bounds__(kGradThreads) decay_grad_kernel(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_last,
-                                                                  int KD, const uint8_t* mask, void* g_decay, int dtype, bool per_head, bool from_zero, float* sums, int64_t T, int B,
+__global__ void __launch_bounds__(kGradThreads) decay_grad_kernel(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_front,
+                                                                  int KD, const uint8_t* mask, DecayRows decay, void* g_decay, int dtype, bool per_head, bool from_zero, float* sums, int64_t T, int B,
                                                                   int H) {
   __shared__ int head;
-  __shared__ double red[kGradThreads / 32];
+  __shared__ double red[kGradThreads / 32], from_keys[kGradThreads / 32];
+  __shared__ bool faded[kGradThreads / 32];
   const int64_t bh = blockIdx.x, BH = (int64_t)B * H;
   const int b = (int)(bh / H), h = (int)(bh % H), tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   double carry = 0.0, all = 0.0;
@@ -284,29 +310,57 @@ __global__ void __launch_bounds__(kGradThreads) decay_grad_kernel(const float* q
   }
   if (g_s) {
     double v = 0.0;
-    for (int i = tid; i < KD; i += kGradThreads) v += (double)g_s[bh * KD + i] * (double)s_last[bh * KD + i];
+    for (int i = tid; i < KD; i += kGradThreads) v += (double)g_s[bh * KD + i] * (double)s_front[bh * KD + i];
     carry = block_sum(v, red);
   }
-  for (int64_t p0 = 0; p0 < T; p0 += kGradThreads) {
-    const int64_t t = T - 1 - p0 - tid;
-    double v = 0.0;
-    if (t >= 0) {
-      for (int i = 0; i < q_tiles; ++i) v += (double)q_dots[((int64_t)i * BH + bh) * T + t];
-      for (int i = 0; i < k_tiles; ++i) v -= (double)k_dots[((int64_t)i * BH + bh) * T + t];
+  static_assert(kC == 32, "a warp to a chunk");
+  constexpr float kFaded = -16.f;
+  const int64_t places = (T + kC - 1) / kC * kC;
+  const float2 *qd = reinterpret_cast<const float2*>(q_dots), *kd = reinterpret_cast<const float2*>(k_dots);
+  for (int64_t p0 = 0; p0 < places; p0 += kGradThreads) {
+    const int64_t t = places - 1 - p0 - tid;
+    const bool there = t >= 0 && t < T, gone = there && mask && mask[(int64_t)b * T + t];
+    double far_q = 0.0, far_k = 0.0, v = 0.0;
+    float fade = there && !gone ? (float)log_decay_at(decay.p, dtype, b * decay.b + h * decay.h + t * decay.t) : 0.f;
+    if (there) {
+      for (int i = 0; i < q_tiles; ++i) {
+        const float2 d = qd[((int64_t)i * BH + bh) * T + t];
+        far_q += (double)d.x;
+        v += (double)d.y;
+      }
+      for (int i = 0; i < k_tiles; ++i) {
+        const float2 d = kd[((int64_t)i * BH + bh) * T + t];
+        far_k += (double)d.x;
+        v -= (double)d.y;
+      }
     }
+    v += far_q;
+    double keys = far_k;      // of this token and the ones before
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffffu, v, o);
+      const double up = __shfl_up_sync(0xffffffffu, v, o), down = __shfl_down_sync(0xffffffffu, keys, o);
       if (lane >= o) v += up;
+      if (lane + o < 32) keys += down;
+      far_q += __shfl_xor_sync(0xffffffffu, far_q, o);
+      fade += __shfl_xor_sync(0xffffffffu, fade, o);
     }
-    if (lane == 31) red[warp] = v;
+    const double before = __shfl_down_sync(0xffffffffu, keys, 1);
+    if (lane < 31) v += before;
+    if (lane == 0) {
+      red[warp] = far_q;
+      from_keys[warp] = keys;
+      faded[warp] = fade < kFaded;
+    }
     __syncthreads();
-    double before = carry;
-    for (int w = 0; w < warp; ++w) before += red[w];
-    for (int w = 0; w < kGradThreads / 32; ++w) carry += red[w];
+    double across = 0.0;
+    for (int w = 0; w < kGradThreads / 32; ++w) {
+      if (p0 > 0 || w > 0) carry = faded[w] ? 0.0 : carry - from_keys[w];
+      if (w == warp) across = carry;
+      carry += red[w];
+    }
     __syncthreads();
-    if (t >= 0) {
-      const double r = t == first || (mask && mask[(int64_t)b * T + t]) ? 0.0 : before + v;
+    if (there) {
+      const double r = t == first || gone ? 0.0 : across + v;
       all += r;
       if (!per_head) {
         const int64_t i = (t * B + b) * H + h;
@@ -388,9 +442,9 @@ int launch_sweeps(SweepBatch batch, const SweepPlan& plan, cudaStream_t stream) 
   return sweep_launches<__nv_bfloat16>(batch, plan, stream);
 }
 
-int launch_decay_grad(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_last, int KD, const uint8_t* mask,
+int launch_decay_grad(const float* q_dots, int q_tiles, const float* k_dots, int k_tiles, const float* g_s, const float* s_front, int KD, const uint8_t* mask, const DecayRows& decay,
                       void* g_decay, int decay_dtype, bool per_head, bool from_zero, float* sums, int64_t T, int B, int H, cudaStream_t stream) {
-  decay_grad_kernel<<<(unsigned)((int64_t)B * H), kGradThreads, 0, stream>>>(q_dots, q_tiles, k_dots, k_tiles, g_s, s_last, KD, mask, g_decay, decay_dtype, per_head,
+  decay_grad_kernel<<<(unsigned)((int64_t)B * H), kGradThreads, 0, stream>>>(q_dots, q_tiles, k_dots, k_tiles, g_s, s_front, KD, mask, decay, g_decay, decay_dtype, per_head,
                                                                             from_zero, sums, T, B, H);
   if (int r = check_launch("rfa_decay_bwd (decays)")) return r;
   if (!per_head) return 0;

@@ -308,3 +308,24 @@ def test_decay_reach_of_what_is_not_finite(dtype, K):
             assert not torch.isfinite(behind).all(-1).any()
             if i == 0:
                 near(out[at + 1:, 1, 1], clean[at + 1:, 1, 1].double(), dt)
+
+
+@pytest.mark.parametrize("dtype,K,D", [("fp32", 64, 64), ("fp32", 24, 40), ("fp32", 130, 72), ("bf16", 200, 64)])
+@pytest.mark.parametrize("rate", [0.01, 1.0, 3.0, 10.0])
+def test_gradient_of_decays_of_any_strength(dtype, K, D, rate):
+    """Of the gradient itself and not of what cancels in it: pairs of tokens that a decay is not between leave nothing.  Sums over 700 tokens of terms of any sign, each with the rounding
+    of its weight and of two products: 12 roundings of the norm over the heads."""
+    from rfa_b200.decay_attention import decay_attention, incremental_decay_attention
+    torch.manual_seed(K)
+    T, H, dt = 700, 8, TYPES[dtype]
+    q, k, v = make(T, 2, (H, H, H), (K, K, D), dt, False)
+    s, go = torch.randn(2, H, K, D, device="cuda"), torch.randn_like(v)
+    gs = torch.randn_like(s)
+    mask = some_mask("any", 2, T)
+    mask[0] = False
+    for g in (torch.full((H,), -rate, device="cuda"), -rate * (0.5 + 0.5 * torch.rand(T, 2, H, device="cuda"))):
+        x = g.clone().requires_grad_()
+        got, = torch.autograd.grad(decay_attention(q=q, k=k, v=v, log_decay=x, key_padding_mask=mask), x, go)
+        near(got, grads(lambda g: decay_dense(q.double(), k.double(), v.double(), g, mask=mask)[0], (g,), [go])[1][0], dt, 12.0)
+        got, = torch.autograd.grad(incremental_decay_attention(q=q, k=k, v=v, log_decay=x, s=s, key_padding_mask=mask), x, (go, gs))
+        near(got, grads(lambda g: decay_dense(q.double(), k.double(), v.double(), g, s.double(), mask), (g,), [go, gs])[1][0], dt, 12.0)
