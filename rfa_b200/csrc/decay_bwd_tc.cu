@@ -8,14 +8,15 @@
 //     gv_j = (P^T G)_j + 2^(L_end - L_j) (K dS)_j
 // The gradient of the log decay at t is the sum over all pairs of a query i >= t and a key j < t.  With D as it is rounded, M_ij = D_ij q_i . k_j: its rows' sums are
 // q_i . (D K)_i and its columns' k_j . (D^T Q)_j, both in fp32 and of one and the same matrix, so that little more than fp32's roundings is left of pairs that
-// do not straddle t when they are subtracted:
+// do not straddle t when they are subtracted.  A token's pair with itself straddles none and does not shrink with the decays: D's diagonal is kept out of the products and
+// sums and its part added to gq and gk by itself (where decays of -10 are a head's, it left 10 to 40 % of their gradient wrong; 3 % of the time, where that gradient is wanted).
 //     g_t = sum_(i >= t) q_i . gq_i - sum_(j >= t) k_j . (D^T Q)_j + sum_(j < t) 2^(L_end - L_j) k_j . (V dS^T)_j + 2^(L_end) S . dS
 //
 // Warp roles (608 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 the decays, warps 3..18 four groups that share the rows' columns 16 by 16: clear padded
 // rows, T0, T1 -> P, D, then the gradients straight from registers.  P takes the place of S.  TMEM: four regions of 128 columns, T0 / T1 / G S^T / V dS^T, the first three
 // of them used again.  All waits are bounded.
 //
-// 8 x 16 heads x 2048 x 128, bf16: 136 us (the whole forward and backward 259 to 284, by the machine), 580 MB of memory traffic (4.3 TB/s); a chunk's chain of loads and products is what the rest waits for.
+// 8 x 16 heads x 2048 x 128, bf16: 144 us (the whole forward and backward 267 to 289, by the machine), 580 MB of memory traffic (4.0 TB/s); a chunk's chain of loads and products is what the rest waits for.
 #define RFA_TC_FAMILY 11
 #include <algorithm>
 
@@ -41,7 +42,7 @@ template <int KB, int DB>
 struct GradLayout {
   static constexpr uint32_t kCopyBytes = KB * DB * 64 * 128;
   static constexpr uint32_t q = 0, k = KB * kBox, v = 2 * KB * kBox, g = v + DB * kBox, s = g + DB * kBox;      // s: S, then P [128][128]
-  static constexpr uint32_t d = s + 2 * kBox, ds = d + 2 * kBox, l = ds + (kCopyBytes + 1023) / 1024 * 1024, bar = l + 128 * 4, bytes = bar + 160;
+  static constexpr uint32_t d = s + 2 * kBox, ds = d + 2 * kBox, l = ds + (kCopyBytes + 1023) / 1024 * 1024, own = l + 128 * 4, bar = own + 128 * 4, bytes = bar + 160;
   static_assert(bytes <= 227 * 1024, "shared memory");
 };
 enum { gQK = 0, gVG, gS, gDS, gL, gClean, gT, gN1, gN2, gX, gP, gO1, gO2, gE1, gE2, gO3, gE3, gAll, gSum, gNum };
@@ -56,7 +57,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Lay::bar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + gNum);
-  float* L = reinterpret_cast<float*>(sm + Lay::l);
+  float *L = reinterpret_cast<float*>(sm + Lay::l), *own = reinterpret_cast<float*>(sm + Lay::own);      // own: D's diagonal
   const uint32_t sbase = smem_u32(sm);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t chunks = (a.T + kTC - 1) / kTC;
@@ -220,7 +221,7 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       const uint8_t* mask = k.mask;
       const int64_t t = k.t0 + row;
       const bool there = t < a.T;
-      float x = 0.f, rows_sum = 0.f, cols_sum = 0.f, keys_sum = 0.f;      // S . dS; q . gq; k . (D^T Q); k . (V dS^T)
+      float x = 0.f, rows_sum = 0.f, cols_sum = 0.f, keys_sum = 0.f;      // S . dS; q . gq; k . (D^T Q), both without the token itself; k . (V dS^T)
       if (mask) {      // padded rows may hold anything: zero before a product reads them
         if (!mbar_wait(&bars[gQK], ph) || !mbar_wait(&bars[gVG], ph)) { tc_fail(8); break; }
         if (there && mask[t]) {
@@ -283,11 +284,18 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
               if (i > last) f[i] = 0.f;
           }
           tmem_ld_wait();
+          const int self = want ? row - p * 16 : -1;      // the token with itself: apart, see the decays below
+          float with_itself = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
+            float d0 = __uint_as_float(s1[i]) * f[i], d1 = __uint_as_float(s1[i + 1]) * f[i + 1];
+            with_itself = i == self ? d0 : i + 1 == self ? d1 : with_itself;
+            d0 = i == self ? 0.f : d0;
+            d1 = i + 1 == self ? 0.f : d1;
             pw[i >> 1] = pack2h<T>(__uint_as_float(s0[i]) * f[i], __uint_as_float(s0[i + 1]) * f[i + 1]);
-            dw[i >> 1] = pack2h<T>(__uint_as_float(s1[i]) * f[i], __uint_as_float(s1[i + 1]) * f[i + 1]);
+            dw[i >> 1] = pack2h<T>(d0, d1);
           }
+          if (self >= 0 && self < 16) own[row] = with_itself;
         }
         *reinterpret_cast<uint4*>(sm + Lay::s + row_chunk2(row, 2 * p)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
         *reinterpret_cast<uint4*>(sm + Lay::s + row_chunk2(row, 2 * p + 1)) = make_uint4(pw[4], pw[5], pw[6], pw[7]);
@@ -301,8 +309,9 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       const float fq = a.scale * ex2(mine), fk = ex2(end - mine);
       const int64_t at = (t * a.B + k.b) * a.H + k.h;
       // ---- gq, gk
-      const auto grad = [&](uint32_t main, uint32_t side, float f, void* out, uint32_t tile, float& own, float& across, bool wide) {
+      const auto grad = [&](uint32_t main, uint32_t side, float f, void* out, uint32_t tile, uint32_t other, float& inside, float& across, bool wide) {
         T* o = static_cast<T*>(out) + at * a.K;
+        const float self = want ? own[row] : 0.f;
 #pragma unroll 1
         for (int c0 = group * 16; c0 < KP; c0 += kDgGroups * 16) {
           uint32_t u[16], n[16];
@@ -316,7 +325,6 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             v[i] = __uint_as_float(u[i]) + s;
             n[i] = __float_as_uint(s);
           }
-          if (there && c0 < a.K) store_row16(o + c0, v, a.K - c0, wide);
           if (want) {
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch) {
@@ -325,21 +333,30 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float2 z = unpack2h<T>(ys[e]);
-                own = fmaf(__uint_as_float(u[8 * ch + 2 * e]), z.x, fmaf(__uint_as_float(u[8 * ch + 2 * e + 1]), z.y, own));
+                inside = fmaf(__uint_as_float(u[8 * ch + 2 * e]), z.x, fmaf(__uint_as_float(u[8 * ch + 2 * e + 1]), z.y, inside));
                 across = fmaf(__uint_as_float(n[8 * ch + 2 * e]), z.x, fmaf(__uint_as_float(n[8 * ch + 2 * e + 1]), z.y, across));
+              }
+              const uint4 y2 = *reinterpret_cast<const uint4*>(sm + other + row_chunk2(row, (c0 >> 3) + ch));
+              const uint32_t y2s[4] = {y2.x, y2.y, y2.z, y2.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 z = unpack2h<T>(y2s[e]);
+                v[8 * ch + 2 * e] = fmaf(self, z.x, v[8 * ch + 2 * e]);
+                v[8 * ch + 2 * e + 1] = fmaf(self, z.y, v[8 * ch + 2 * e + 1]);
               }
             }
           }
+          if (there && c0 < a.K) store_row16(o + c0, v, a.K - c0, wide);
         }
       };
-      if (!mbar_wait(&bars[gO1], ph)) { tc_fail(12); break; }
+      if ((want && !mbar_wait(&bars[gP], ph)) || !mbar_wait(&bars[gO1], ph)) { tc_fail(12); break; }      // gP: `own` is there
       tc_fence_after_sync();
-      grad(R0, R2, fq, a.gq, Lay::q, rows_sum, rows_sum, wide_q);
+      grad(R0, R2, fq, a.gq, Lay::q, Lay::k, rows_sum, rows_sum, wide_q);
       tc_fence_before_sync();
       mbar_arrive(&bars[gE1]);
       if (!mbar_wait(&bars[gN2], ph) || !mbar_wait(&bars[gO2], ph)) { tc_fail(13); break; }
       tc_fence_after_sync();
-      grad(R1, R3, fk, a.gk, Lay::k, cols_sum, keys_sum, wide_k);
+      grad(R1, R3, fk, a.gk, Lay::k, Lay::q, cols_sum, keys_sum, wide_k);
       mbar_release_stage(&bars[gE2]);
       // ---- gv
       if (!mbar_wait(&bars[gO3], ph)) { tc_fail(14); break; }

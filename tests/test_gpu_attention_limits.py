@@ -310,7 +310,7 @@ def test_decay_reach_of_what_is_not_finite(dtype, K):
                 near(out[at + 1:, 1, 1], clean[at + 1:, 1, 1].double(), dt)
 
 
-@pytest.mark.parametrize("dtype,K,D", [("fp32", 64, 64), ("fp32", 24, 40), ("fp32", 130, 72), ("bf16", 200, 64)])
+@pytest.mark.parametrize("dtype,K,D", [("fp32", 64, 64), ("fp32", 24, 40), ("fp32", 130, 72), ("bf16", 200, 64), ("fp16", 64, 64), ("bf16", 128, 128), ("bf16", 64, 128), ("fp16", 33, 90)])
 @pytest.mark.parametrize("rate", [0.01, 1.0, 3.0, 10.0])
 def test_gradient_of_decays_of_any_strength(dtype, K, D, rate):
     """Of the gradient itself and not of what cancels in it: pairs of tokens that a decay is not between leave nothing.  Sums over 700 tokens of terms of any sign, each with the rounding
