@@ -9,14 +9,14 @@
 // The gradient of the log decay at t is the sum over all pairs of a query i >= t and a key j < t.  With D as it is rounded, M_ij = D_ij q_i . k_j: its rows' sums are
 // q_i . (D K)_i and its columns' k_j . (D^T Q)_j, both in fp32 and of one and the same matrix, so that little more than fp32's roundings is left of pairs that
 // do not straddle t when they are subtracted.  A token's pair with itself straddles none and does not shrink with the decays: D's diagonal is kept out of the products and
-// sums and its part added to gq and gk by itself (where decays of -10 are a head's, it left 10 to 40 % of their gradient wrong; 3 % of the time, where that gradient is wanted).
+// sums and its part added to gq and gk by itself (where decays of -10 are a head's, it left 10 to 40 % of their gradient wrong; 2 % of a training step).
 //     g_t = sum_(i >= t) q_i . gq_i - sum_(j >= t) k_j . (D^T Q)_j + sum_(j < t) 2^(L_end - L_j) k_j . (V dS^T)_j + 2^(L_end) S . dS
 //
 // Warp roles (608 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 the decays, warps 3..18 four groups that share the rows' columns 16 by 16: clear padded
 // rows, T0, T1 -> P, D, then the gradients straight from registers.  P takes the place of S.  TMEM: four regions of 128 columns, T0 / T1 / G S^T / V dS^T, the first three
 // of them used again.  All waits are bounded.
 //
-// 8 x 16 heads x 2048 x 128, bf16: 144 us (the whole forward and backward 267 to 289, by the machine), 580 MB of memory traffic (4.0 TB/s); a chunk's chain of loads and products is what the rest waits for.
+// 8 x 16 heads x 2048 x 128, bf16: 141 us, 149 under the profiler (the whole forward and backward 264 to 287, by the machine), 580 MB of memory traffic (4.1 TB/s); a chunk's chain of loads and products is what the rest waits for.
 #define RFA_TC_FAMILY 11
 #include <algorithm>
 
@@ -277,25 +277,23 @@ decay_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             const float4 l = *reinterpret_cast<const float4*>(L + p * 16 + i);
             f[i] = a.scale * ex2(mine - l.x); f[i + 1] = a.scale * ex2(mine - l.y); f[i + 2] = a.scale * ex2(mine - l.z); f[i + 3] = a.scale * ex2(mine - l.w);
           }
-          if (p >= 2 * quarter) {      // the diagonal's
-            const int last = row - p * 16;
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (i > last) f[i] = 0.f;
-          }
           tmem_ld_wait();
-          const int self = want ? row - p * 16 : -1;      // the token with itself: apart, see the decays below
-          float with_itself = 0.f;
+          if (p >= 2 * quarter) {      // the diagonal's
+            const int last = row - p * 16, self = want ? last : -1;
+            float with_itself = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              f[i] = i > last ? 0.f : f[i];
+              with_itself = i == self ? __uint_as_float(s1[i]) * f[i] : with_itself;
+              s1[i] = i == self ? 0u : s1[i];      // the token with itself: apart, see the decays below
+            }
+            if (self >= 0 && self < 16) own[row] = with_itself;
+          }
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            float d0 = __uint_as_float(s1[i]) * f[i], d1 = __uint_as_float(s1[i + 1]) * f[i + 1];
-            with_itself = i == self ? d0 : i + 1 == self ? d1 : with_itself;
-            d0 = i == self ? 0.f : d0;
-            d1 = i + 1 == self ? 0.f : d1;
             pw[i >> 1] = pack2h<T>(__uint_as_float(s0[i]) * f[i], __uint_as_float(s0[i + 1]) * f[i + 1]);
-            dw[i >> 1] = pack2h<T>(d0, d1);
+            dw[i >> 1] = pack2h<T>(__uint_as_float(s1[i]) * f[i], __uint_as_float(s1[i + 1]) * f[i + 1]);
           }
-          if (self >= 0 && self < 16) own[row] = with_itself;
         }
         *reinterpret_cast<uint4*>(sm + Lay::s + row_chunk2(row, 2 * p)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
         *reinterpret_cast<uint4*>(sm + Lay::s + row_chunk2(row, 2 * p + 1)) = make_uint4(pw[4], pw[5], pw[6], pw[7]);
