@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kGradThreads) decay_grad_kernel(const float* q
     __syncthreads();
     double across = 0.0;
     for (int w = 0; w < kGradThreads / 32; ++w) {
-      if (p0 > 0 || w > 0) carry = faded[w] ? 0.0 : carry - from_keys[w];
+      if (p0 > 0 || w > 0) carry = (carry - from_keys[w]) * (faded[w] ? 0.0 : 1.0);      // times zero, so that what is no number stays none
       if (w == warp) across = carry;
       carry += red[w];
     }
